@@ -25,6 +25,9 @@ enum DeviceError : int32_t {
     kDevBadSelection = 0x201,
     kDevF16Range = 0x301,      // an f32 input is outside the f16 range of the tensor-core mode
     kDevBadBlockTable = 0x401, // a paged-KV block table entry lies outside the pool
+    kDevBadLength = 0x501,     // a sequence length of a batch lies outside [0, max_kv_len]
+    kDevWaitDecode = 0x601,    // a decode KV unit did not arrive (or leave) in time
+    kDevWaitWeights = 0x602,   // a prompt-weight tile did not arrive (or leave) in time
 };
 
 // The device error word is err[0] of a 4-word record: the kernel whose
@@ -222,6 +225,110 @@ cudaError_t launch_copy_rows(const void* src, void* dst, size_t bytes, cudaStrea
 // paged pool (16-byte vectors on the SMs).
 cudaError_t launch_copy_rows_paged(const void* src, void* dst_pool, int32_t row_begin, int32_t n_rows, size_t row_bytes,
                                    const KvPaging& pg, int32_t* err, cudaStream_t s);
+
+// ---------------------------------------------------------------------------
+// Serving: a batch of sequences in the KV cache of one layer.
+
+// Rows of sequence s: through tables[s][r / block_rows] when block_rows > 0,
+// else at s * seq_rows + r.  rows = rows of the whole k / v tensors.
+struct BatchKv {
+    const int32_t* lens = nullptr;    // device [n_seq]
+    const int32_t* tables = nullptr;  // device [n_seq][table_stride]
+    int32_t n_seq = 0, max_kv_len = 0;
+    int32_t table_stride = 0, block_rows = 0, seq_rows = 0;
+    int32_t rows = 0;
+};
+
+#if defined(__CUDACC__)
+// Length of sequence s; one outside [0, max_kv_len] is recorded and read as 0.
+__device__ __forceinline__ int32_t batch_len(const BatchKv& b, int32_t s, int32_t* err) {
+    const int32_t n = __ldg(b.lens + s);
+    if (n < 0 || n > b.max_kv_len) {
+        report_error(err, kDevBadLength, 0x90, s);
+        return 0;
+    }
+    return n;
+}
+
+// Cache row of row r of sequence s, -1 (recorded) when its table entry lies
+// outside the pool.
+__device__ __forceinline__ int32_t batch_row(const BatchKv& b, int32_t s, int32_t r, int32_t* err) {
+    if (b.block_rows <= 0) return s * b.seq_rows + r;
+    const int32_t i = r / b.block_rows;
+    const int64_t blk = __ldg(b.tables + (int64_t)s * b.table_stride + i);
+    const int64_t row = blk * b.block_rows + (r - i * b.block_rows);
+    if (blk < 0 || row >= b.rows) {
+        report_error(err, kDevBadBlockTable, 0x91, s);
+        return -1;
+    }
+    return (int32_t)row;
+}
+#endif
+
+// Attention of one token per sequence over its lens[s] cache rows.
+struct DecodeArgs {
+    BatchKv kv;
+    const void* q;      // [n_seq][n_head][d]
+    void* k;            // cache rows [rows][Hkv][d]
+    void* v;
+    const void* k_new;  // [n_seq][Hkv][d]: written to row lens[s] - 1 first (null: already there)
+    const void* v_new;
+    void* out;          // [n_seq][n_head][d] in out_dtype
+    int32_t dtype, out_dtype;
+    int32_t n_head, n_head_kv, head_dim;
+    float kq_scale;
+    float* acc;         // [n_seq][Hkv][acc_stride] += softmax weights (null: not kept)
+    int32_t acc_stride;
+    void* ws;
+    int32_t* err;
+    uint64_t timeout_ns;
+};
+size_t decode_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                       bool weights);
+cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t s);
+
+// Softmax weights of the query rows [row_begin, n_tok) of a call (causal, every
+// cache row up to the query's own), summed over rows and the query heads of
+// each KV head.
+struct WeightArgs {
+    const void* q;  // [n_tok][n_head][d]
+    const void* k;  // [kv_len][Hkv][d], or a pool under paging
+    KvPaging paging;
+    int32_t dtype, n_head, n_head_kv, head_dim, page_size;
+    int32_t kv_len, n_tok, row_begin;
+    float kq_scale;
+    int32_t accumulate;  // 1: add to acc, 0: overwrite [0, kv_len)
+    float* acc;          // [Hkv][acc_stride]
+    int32_t acc_stride;
+    void* ws;
+    int32_t* err;
+    uint64_t timeout_ns;
+};
+size_t weights_ws_bytes(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv);
+cudaError_t launch_prompt_weights(const WeightArgs& a, cudaStream_t s);
+
+// Eviction: per sequence and KV head the sink rows, the recent rows and the
+// rows of largest weight, gathered in order into the destination cache.
+struct EvictArgs {
+    BatchKv src, dst;  // dst.lens unused
+    const void* k;
+    const void* v;
+    const float* acc;  // [n_seq][Hkv][acc_stride]
+    int32_t acc_stride;
+    int32_t n_keep, sink_rows, recent_rows;
+    void* k_dst;
+    void* v_dst;
+    float* acc_dst;    // [n_seq][Hkv][acc_dst_stride] or null
+    int32_t acc_dst_stride;
+    int32_t* new_lens;   // [n_seq] or null
+    int32_t* kept_rows;  // [n_seq][Hkv][n_keep] or null
+    int32_t n_head_kv, head_dim, elem_bytes;
+    int32_t in_place;  // k_dst / v_dst are k / v and the tables are the same
+    void* ws;
+    int32_t* err;
+};
+size_t evict_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t n_head_kv);
+cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s);
 
 // Reads and clears the device error word of the no-allocation selection path
 // on the current device (0 when that device never ran it).

@@ -215,6 +215,41 @@ int32_t launch_attn(ep_sp_ctx* ctx, const epsp::AttnArgs& aa, cudaStream_t s) {
     return kOk;
 }
 
+}  // namespace
+
+namespace edge_prefill_b200 {
+
+int32_t ctx_fail(ep_sp_ctx* ctx, int32_t rc, const std::string& msg) { return fail(ctx, rc, msg); }
+
+int32_t ctx_ensure_device(ep_sp_ctx* ctx) { return ensure_device(ctx); }
+
+void* ctx_profile_begin(ep_sp_ctx* ctx, int kind, void* stream) {
+    ++ctx->launches[kind];
+    if (!ctx->profiling) return nullptr;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &cap) != cudaSuccess ||
+        cap != cudaStreamCaptureStatusNone)
+        return nullptr;
+    void* a = take_event(ctx);
+    if (a) cudaEventRecord(static_cast<cudaEvent_t>(a), static_cast<cudaStream_t>(stream));
+    return a;
+}
+
+void ctx_profile_end(ep_sp_ctx* ctx, int kind, void* start, void* stream) {
+    if (!start) return;
+    void* b = take_event(ctx);
+    if (!b) {
+        ctx->event_pool.push_back(start);
+        return;
+    }
+    cudaEventRecord(static_cast<cudaEvent_t>(b), static_cast<cudaStream_t>(stream));
+    ctx->events.push_back({kind, start, b});
+}
+
+}  // namespace edge_prefill_b200
+
+namespace {
+
 constexpr size_t kXchgHeader = 4096;  // per-slot uint64 counters, then the slots
 constexpr int32_t kXchgMaxSlots = 64;
 
@@ -395,7 +430,7 @@ int32_t ep_sp_sync_status(ep_sp_ctx* ctx, void* stream) {
                         "attends it in f32)");
         char buf[160];
         std::snprintf(buf, sizeof buf,
-                      "device error word 0x%x (bounded wait expired, bad selection or block table); where 0x%x, "
+                      "device error word 0x%x (bounded wait expired, bad selection, block table or length); where 0x%x, "
                       "block %d, tile %d",
                       err, rec[1], rec[2], rec[3]);
         return fail(ctx, kPrefill, buf);
@@ -797,18 +832,19 @@ int32_t ep_sp_profile_enable(ep_sp_ctx* ctx, int32_t on) {
         ctx->event_pool.push_back(ev.stop);
     }
     ctx->events.clear();
-    for (int i = 0; i < EP_SP_NUM_KERNELS; ++i) ctx->launches[i] = 0;
+    for (int i = 0; i < EP_SP_NUM_FAMILIES; ++i) ctx->launches[i] = 0;
     ctx->profiling = on != 0;
     return kOk;
 }
 
-int32_t ep_sp_profile_read(ep_sp_ctx* ctx, double* ms, int64_t* launches) {
-    if (!ctx || !ms || !launches) return kInvalid;
-    for (int i = 0; i < EP_SP_NUM_KERNELS; ++i) {
+int32_t ep_sp_profile_read_families(ep_sp_ctx* ctx, int32_t n, double* ms, int64_t* launches) {
+    if (!ctx || !ms || !launches || n < 1 || n > EP_SP_NUM_FAMILIES) return kInvalid;
+    for (int i = 0; i < n; ++i) {
         ms[i] = 0.0;
         launches[i] = ctx->launches[i];
     }
     for (auto& ev : ctx->events) {
+        if (ev.kind >= n) continue;
         cudaError_t e = cudaEventSynchronize(static_cast<cudaEvent_t>(ev.stop));
         if (e != cudaSuccess) return cuda_fail(ctx, e, "profile event");
         float t = 0.f;
@@ -817,6 +853,10 @@ int32_t ep_sp_profile_read(ep_sp_ctx* ctx, double* ms, int64_t* launches) {
         ms[ev.kind] += t;
     }
     return kOk;
+}
+
+int32_t ep_sp_profile_read(ep_sp_ctx* ctx, double* ms, int64_t* launches) {
+    return ep_sp_profile_read_families(ctx, EP_SP_NUM_KERNELS, ms, launches);
 }
 
 int32_t ep_sp_layer_work(const ep_sp_ctx* ctx, int32_t layer, int32_t kv_len, int32_t n_tok, double* out) {

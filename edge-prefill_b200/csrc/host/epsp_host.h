@@ -157,7 +157,7 @@ struct ep_sp_ctx {
     };
     std::vector<Ev> events;       // recorded since the last enable
     std::vector<void*> event_pool;
-    int64_t launches[EP_SP_NUM_KERNELS] = {0, 0, 0, 0, 0, 0};
+    int64_t launches[EP_SP_NUM_FAMILIES] = {};
 
     // head-parallel output exchange (ep_sp_xchg_*)
     void* xchg_base = nullptr;            // this rank's buffer: [header][slots]
@@ -170,3 +170,16 @@ struct ep_sp_ctx {
     void* xchg_mc = nullptr;              // multicast mapping of every rank's buffer (or null)
     bool xchg_external = false;           // buffers owned by the caller (ep_sp_xchg_attach_buffers)
 };
+
+namespace edge_prefill_b200 {
+
+// Shared by the files behind the ABI: records the message and returns rc.
+int32_t ctx_fail(ep_sp_ctx* ctx, int32_t rc, const std::string& msg);
+// The device state of a compute call (reserved on first use).
+int32_t ctx_ensure_device(ep_sp_ctx* ctx);
+// Brackets a launch of family `kind` with events while profiling (take before
+// the launch, give after it; nothing is recorded on a capturing stream).
+void* ctx_profile_begin(ep_sp_ctx* ctx, int kind, void* stream);
+void ctx_profile_end(ep_sp_ctx* ctx, int kind, void* start, void* stream);
+
+}  // namespace edge_prefill_b200

@@ -33,10 +33,14 @@ EXPORTS = [
     "ep_sp_cta_work", "ep_sp_set_attn_tiles", "ep_sp_get_attn_tiles", "ep_sp_append_kv",
     "ep_sp_set_f32_attention", "ep_sp_get_f32_attention", "ep_sp_get_pooled_pages", "ep_sp_set_head_routing",
     "ep_sp_get_head_routing", "ep_sp_set_paged_kv", "ep_sp_xchg_attach_buffers", "ep_sp_xchg_bytes",
+    "ep_sp_decode_bytes", "ep_sp_decode_layer", "ep_sp_prompt_weights_bytes", "ep_sp_prompt_weights",
+    "ep_sp_evict_bytes", "ep_sp_evict_layer", "ep_sp_profile_read_families",
 ]
 NUM_KERNELS = 6  # EP_SP_NUM_KERNELS
 KERNEL_NAMES = ["k1_pool_pages", "k2_select_pages", "k3_sparse_attention", "k4_compact", "k4_scatter",
                 "k5_exchange_wait"]
+NUM_FAMILIES = 9  # EP_SP_NUM_FAMILIES
+FAMILY_NAMES = KERNEL_NAMES + ["k6_decode", "k7_prompt_weights", "k8_evict"]
 XCHG_HANDLE_BYTES = 64
 
 
@@ -59,6 +63,15 @@ class PrefillStats(ctypes.Structure):
     _fields_ = [
         ("chunks", c_uint32), ("query_gating", c_int32), ("attn_fallback", c_int32), ("qg_groups", c_uint32),
         ("chunk_attn_rows", c_uint32),
+    ]
+
+
+class KvBatchDesc(ctypes.Structure):
+    """ep_sp_kv_batch."""
+
+    _fields_ = [
+        ("n_seq", c_int32), ("max_kv_len", c_int32), ("kv_lens", c_void_p), ("block_tables", c_void_p),
+        ("table_stride", c_int32), ("block_rows", c_int32), ("pool_rows", c_int32), ("seq_rows", c_int32),
     ]
 
 
@@ -126,6 +139,16 @@ def _load() -> ctypes.CDLL:
         "ep_sp_set_paged_kv": (c_int32, [P, c_int32, P, c_int32, c_int32]),
         "ep_sp_xchg_attach_buffers": (c_int32, [P, c_int32, c_int32, c_int32, c_int32, POINTER(P), P]),
         "ep_sp_xchg_bytes": (c_int32, [P, c_int32, c_int32, POINTER(c_size_t)]),
+        "ep_sp_decode_bytes": (c_int32, [P, c_int32, c_int32, c_int32, POINTER(c_size_t)]),
+        "ep_sp_decode_layer": (c_int32, [P, c_int32, POINTER(KvBatchDesc), P, P, P, P, P, P, P, c_int32, P, c_size_t,
+                                         P]),
+        "ep_sp_prompt_weights_bytes": (c_int32, [P, c_int32, c_int32, c_int32, POINTER(c_size_t)]),
+        "ep_sp_prompt_weights": (c_int32, [P, c_int32, P, P, c_int32, c_int32, c_int32, c_int32, P, c_int32, P,
+                                           c_size_t, P]),
+        "ep_sp_evict_bytes": (c_int32, [P, c_int32, c_int32, c_int32, POINTER(c_size_t)]),
+        "ep_sp_evict_layer": (c_int32, [P, c_int32, POINTER(KvBatchDesc), P, P, P, c_int32, c_int32, c_int32, c_int32,
+                                        POINTER(KvBatchDesc), P, P, P, c_int32, P, P, P, c_size_t, P]),
+        "ep_sp_profile_read_families": (c_int32, [P, c_int32, POINTER(c_double), POINTER(ctypes.c_int64)]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -177,6 +200,48 @@ def device_view(ptr: int, shape, dtype: int):
     return t.view(torch.bfloat16) if dtype == BF16 else t
 
 
+_DTYPE_NAMES = {F32: "torch.float32", F16: "torch.float16", BF16: "torch.bfloat16"}
+
+
+def _check(name, t, dtype, shape, device):
+    """The library sees plain pointers: what a tensor is must be checked here.  A shape entry None is any size."""
+    if str(t.dtype) != dtype:
+        raise ValueError(f"{name} is {t.dtype}, not {dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} is not contiguous (strides {tuple(t.stride())})")
+    if t.device.type != "cuda" or t.device.index != device:
+        raise ValueError(f"{name} is on {t.device}, not cuda:{device}")
+    if len(t.shape) != len(shape) or any(w is not None and h != w for h, w in zip(t.shape, shape)):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
+
+
+class KvBatch:
+    """A batch of sequences in one layer's cache (ep_sp_kv_batch).  kv_lens: int32 [n_seq] on the device (None for an
+    eviction's destination, with n_seq given).  Paged: block_tables int32 [n_seq][entries] on the device, block_rows
+    and pool_rows; contiguous: block_rows 0 and seq_rows rows from one sequence to the next.  Keeps its tensors
+    alive; kv_lens and the tables may be rewritten in place between calls."""
+
+    def __init__(self, kv_lens, max_kv_len, block_tables=None, block_rows=0, pool_rows=0, seq_rows=0, n_seq=None):
+        ref = kv_lens if kv_lens is not None else block_tables
+        if kv_lens is None and n_seq is None:
+            raise ValueError("a batch without kv_lens needs n_seq")
+        self.n_seq = int(n_seq) if n_seq is not None else kv_lens.shape[0]
+        self.kv_lens, self.block_tables = kv_lens, block_tables
+        self.device = None if ref is None else ref.device.index
+        if kv_lens is not None:
+            _check("kv_lens", kv_lens, "torch.int32", (self.n_seq,), self.device)
+        entries = 0
+        if block_rows:
+            if block_tables is None:
+                raise ValueError("block_rows without block_tables")
+            _check("block_tables", block_tables, "torch.int32", (self.n_seq, None), self.device)
+            entries = block_tables.shape[1]
+        self.rows = pool_rows if block_rows else self.n_seq * seq_rows
+        self.desc = KvBatchDesc(self.n_seq, max_kv_len, _ptr(kv_lens), _ptr(block_tables) if block_rows else None,
+                                entries, block_rows, pool_rows, seq_rows)
+        self.ref = ctypes.byref(self.desc)
+
+
 class Context:
     """One ep_sp_ctx.  Methods return the C status code; `check()` raises."""
 
@@ -184,6 +249,7 @@ class Context:
                  page_size=32, device=0, kv_head_offset=0, n_head_kv_total=0, kq_scale=0.0):
         self.cfg = Config(n_layer, n_head, n_head_kv, head_dim, dtype, dtype if out_dtype is None else out_dtype,
                           max_ctx, page_size, device, kv_head_offset, n_head_kv_total, kq_scale)
+        self._pool_rows = 0  # rows of the pools of set_paged_kv
         self.h = c_void_p()
         rc = lib.ep_sp_create(ctypes.byref(self.cfg), ctypes.byref(self.h))
         if rc != OK:
@@ -329,7 +395,110 @@ class Context:
         return lib.ep_sp_get_attn_tiles(self.h)
 
     def set_paged_kv(self, block_rows, block_table=None, n_entries=0, pool_rows=0):
-        return lib.ep_sp_set_paged_kv(self.h, block_rows, _ptr(block_table), n_entries, pool_rows)
+        rc = lib.ep_sp_set_paged_kv(self.h, block_rows, _ptr(block_table), n_entries, pool_rows)
+        if rc == OK:
+            self._pool_rows = pool_rows if block_rows else 0
+        return rc
+
+    # ------------------------------- answering from and shrinking the cache
+    def _cache_tensors(self, kv, k, v, what=("k", "v")):
+        c = self.cfg
+        if kv.device is not None and kv.device != c.device:
+            raise ValueError(f"the batch is on cuda:{kv.device}, not cuda:{c.device}")
+        shape, dt = (None, c.n_head_kv, c.head_dim), _DTYPE_NAMES[c.dtype]
+        for name, t in zip(what, (k, v)):
+            _check(name, t.flatten(0, -3) if t.dim() > 3 and t.is_contiguous() else t, dt, shape, c.device)
+            if t.numel() < kv.rows * c.n_head_kv * c.head_dim:
+                raise ValueError(f"{name} holds fewer than the batch's {kv.rows} rows")
+
+    def _workspace(self, t):
+        if t is None:
+            return None, 0
+        if not t.is_contiguous() or t.device.index != self.cfg.device:
+            raise ValueError(f"the workspace must be a contiguous tensor on cuda:{self.cfg.device}")
+        return t.data_ptr(), t.numel() * t.element_size()
+
+    def decode_bytes(self, n_seq, max_kv_len, with_acc=False):
+        n = c_size_t()
+        self.check(lib.ep_sp_decode_bytes(self.h, n_seq, max_kv_len, 1 if with_acc else 0, ctypes.byref(n)))
+        return n.value
+
+    def decode_layer(self, layer, kv, q, k, v, out, workspace, k_new=None, v_new=None, acc=None, stream=None):
+        """kv: KvBatch; q, out [n_seq][n_head][head_dim]; k, v the cache's rows; k_new, v_new [n_seq][n_head_kv]
+        [head_dim]; acc f32 [n_seq][n_head_kv][stride].  Raises ValueError for a tensor of another type, shape,
+        layout or device; returns the status code."""
+        c = self.cfg
+        dt = _DTYPE_NAMES[c.dtype]
+        self._cache_tensors(kv, k, v)
+        _check("q", q, dt, (kv.n_seq, c.n_head, c.head_dim), c.device)
+        _check("out", out, _DTYPE_NAMES[c.out_dtype], (kv.n_seq, c.n_head, c.head_dim), c.device)
+        for name, t in (("k_new", k_new), ("v_new", v_new)):
+            if t is not None:
+                _check(name, t, dt, (kv.n_seq, c.n_head_kv, c.head_dim), c.device)
+        if acc is not None:
+            _check("acc", acc, "torch.float32", (kv.n_seq, c.n_head_kv, None), c.device)
+        ws, n = self._workspace(workspace)
+        return lib.ep_sp_decode_layer(self.h, layer, kv.ref, q.data_ptr(), _ptr(k_new), _ptr(v_new), k.data_ptr(),
+                                      v.data_ptr(), out.data_ptr(), _ptr(acc), 0 if acc is None else acc.shape[-1],
+                                      ws, n, self._stream(stream))
+
+    def prompt_weights_bytes(self, kv_len, n_tok, row_begin):
+        n = c_size_t()
+        self.check(lib.ep_sp_prompt_weights_bytes(self.h, kv_len, n_tok, row_begin, ctypes.byref(n)))
+        return n.value
+
+    def prompt_weights(self, layer, q, k, kv_len, n_tok, row_begin, acc, workspace, accumulate=False, stream=None):
+        """q [n_tok][n_head][head_dim]; k the cache (paged under set_paged_kv); acc f32 [n_head_kv][stride]."""
+        c = self.cfg
+        dt = _DTYPE_NAMES[c.dtype]
+        _check("q", q, dt, (n_tok, c.n_head, c.head_dim), c.device)
+        _check("k", k, dt, (None, c.n_head_kv, c.head_dim), c.device)
+        if k.shape[0] < (self._pool_rows or kv_len):
+            raise ValueError(f"k holds {k.shape[0]} rows, the call reads {self._pool_rows or kv_len}")
+        _check("acc", acc, "torch.float32", (c.n_head_kv, None), c.device)
+        ws, n = self._workspace(workspace)
+        return lib.ep_sp_prompt_weights(self.h, layer, q.data_ptr(), k.data_ptr(), kv_len, n_tok, row_begin,
+                                        1 if accumulate else 0, acc.data_ptr(), acc.shape[-1], ws, n,
+                                        self._stream(stream))
+
+    def evict_bytes(self, n_seq, max_kv_len, n_keep):
+        n = c_size_t()
+        self.check(lib.ep_sp_evict_bytes(self.h, n_seq, max_kv_len, n_keep, ctypes.byref(n)))
+        return n.value
+
+    def evict_layer(self, layer, src, k, v, acc, n_keep, sink_rows, recent_rows, dst, k_dst, v_dst, workspace,
+                    acc_dst=None, new_lens=None, kept_rows=None, stream=None):
+        """src, dst: KvBatch (the same object and tensors compact in place); acc f32 [n_seq][n_head_kv][stride];
+        acc_dst likewise; new_lens int32 [n_seq]; kept_rows int32 [n_seq][n_head_kv][n_keep]."""
+        c = self.cfg
+        self._cache_tensors(src, k, v)
+        self._cache_tensors(dst, k_dst, v_dst, ("k_dst", "v_dst"))
+        _check("acc", acc, "torch.float32", (src.n_seq, c.n_head_kv, None), c.device)
+        if acc_dst is not None:
+            _check("acc_dst", acc_dst, "torch.float32", (src.n_seq, c.n_head_kv, None), c.device)
+        if new_lens is not None:
+            _check("new_lens", new_lens, "torch.int32", (src.n_seq,), c.device)
+        if kept_rows is not None:
+            _check("kept_rows", kept_rows, "torch.int32", (src.n_seq, c.n_head_kv, n_keep), c.device)
+        ws, n = self._workspace(workspace)
+        return lib.ep_sp_evict_layer(self.h, layer, src.ref, k.data_ptr(), v.data_ptr(), acc.data_ptr(),
+                                     acc.shape[-1], n_keep, sink_rows, recent_rows, dst.ref, k_dst.data_ptr(),
+                                     v_dst.data_ptr(), _ptr(acc_dst), 0 if acc_dst is None else acc_dst.shape[-1],
+                                     _ptr(new_lens), _ptr(kept_rows), ws, n, self._stream(stream))
+
+    def profile_families(self):
+        """{family name: (milliseconds, launches)} since the last ep_sp_profile_enable."""
+        ms, n = (c_double * NUM_FAMILIES)(), (ctypes.c_int64 * NUM_FAMILIES)()
+        self.check(lib.ep_sp_profile_read_families(self.h, NUM_FAMILIES, ms, n))
+        return {name: (ms[i], n[i]) for i, name in enumerate(FAMILY_NAMES)}
+
+    def _stream(self, stream):
+        """The given stream, or the current one of the context's device."""
+        if stream is None:
+            import torch
+
+            return torch.cuda.current_stream(self.cfg.device).cuda_stream
+        return stream if isinstance(stream, int) else stream.cuda_stream
 
     def set_head_routing(self, mode, threshold):
         return lib.ep_sp_set_head_routing(self.h, mode, threshold)

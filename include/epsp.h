@@ -422,10 +422,118 @@ int32_t ep_sp_ffn_scatter(ep_sp_ctx* ctx, int32_t layer, const void* ffn_out, vo
                           const int32_t* row_ids, const int32_t* n_keep, int32_t n_rows,
                           int32_t hidden, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Answering from the cache a prefill leaves: one new token per sequence, and
+ * shrinking the cache by the attention its rows receive.  No reference
+ * counterpart (the reference ends at the prefill; decoding there is
+ * llama.cpp's).  These calls are dense over the cache's rows: the page gating
+ * and prefill mode do not affect them.  They allocate nothing and work in the
+ * caller's workspace (device memory, 16-byte aligned, at least the _bytes
+ * call's size, contents undefined before and after): calls that may overlap
+ * on the GPU (two streams, two replayed graphs) need a workspace each.  All of
+ * them can be captured into a CUDA graph once ep_sp_reserve has run (rc 2
+ * before); kernel timing is not recorded under capture.  They run on the
+ * context's device whatever device is current.
+ *
+ * A batch of sequences in one layer's cache.  With block_rows > 0 the k / v
+ * tensors are POOLS of pool_rows rows ([pool_rows][n_head_kv][head_dim]) and
+ * row r of sequence s is pool row
+ *   block_tables[s * table_stride + r / block_rows] * block_rows + r % block_rows
+ * (block_rows a multiple of the page size, pool_rows a multiple of
+ * block_rows, table_stride * block_rows >= max_kv_len).  With block_rows == 0
+ * the tensors are [n_seq][seq_rows][n_head_kv][head_dim] and row r of
+ * sequence s is row s * seq_rows + r (seq_rows >= max_kv_len; block_tables,
+ * table_stride and pool_rows are not read).  kv_lens are the sequences'
+ * lengths on the DEVICE, each in [0, max_kv_len], so a captured step can be
+ * replayed as they grow; max_kv_len is the host's bound on them.  A length
+ * outside that range is read as 0 and a table entry outside the pool is not
+ * followed; both are reported by ep_sp_sync_status (rc 6).  Table entries past
+ * a sequence's length are not read, and cache rows past it may hold anything
+ * (NaN too).  Two sequences may share blocks that no call writes. */
+typedef struct ep_sp_kv_batch {
+    int32_t n_seq;
+    int32_t max_kv_len;          /* 1..max_ctx */
+    const int32_t* kv_lens;      /* DEVICE [n_seq] */
+    const int32_t* block_tables; /* DEVICE [n_seq][table_stride] block ids */
+    int32_t table_stride;
+    int32_t block_rows;          /* 0: contiguous */
+    int32_t pool_rows;
+    int32_t seq_rows;
+} ep_sp_kv_batch;
+
+/* Attention of one token per sequence over its kv_lens[s] rows (the token's
+ * own row included): out[s] = softmax(q[s] . K^T * kq_scale) V per query head;
+ * a sequence of length 0 gets a zero row.
+ *   q, out        [n_seq][n_head][head_dim] (dtype / out_dtype)
+ *   k_new, v_new  NULL, or [n_seq][n_head_kv][head_dim]: written to row
+ *                 kv_lens[s] - 1 of the caches by this call and attended as
+ *                 that row (a sequence of length 0 writes nothing);
+ *   acc           NULL, or [n_seq][n_head_kv][acc_stride] f32 (acc_stride >=
+ *                 max_kv_len): acc[s][h][r] += the row's softmax weights
+ *                 summed over the query heads of KV head h, r < kv_lens[s].
+ * q, k, v, k_new, v_new, out and the workspace are 16-byte aligned.  Scores,
+ * softmax statistics and sums are f32; an f32 context multiplies in f32
+ * whatever ep_sp_set_f32_attention says.  A sequence's result does not depend
+ * on timing, only on the batch (the cache is split over the SMs by the lengths
+ * of the whole batch).  rc 2 on bad arguments, 12 on a CUDA launch error; a
+ * bounded wait that expired is rc 6 from ep_sp_sync_status.
+ * ep_sp_decode_bytes gives the workspace size of a call with n_seq sequences
+ * of up to max_kv_len rows, with_acc 1 when acc is given. */
+int32_t ep_sp_decode_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_len, int32_t with_acc, size_t* bytes);
+int32_t ep_sp_decode_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* kv, const void* q, const void* k_new,
+                           const void* v_new, void* k, void* v, void* out, float* acc, int32_t acc_stride,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Softmax weights that the query rows [row_begin, n_tok) of one ubatch give
+ * the cache rows, causal and dense over [0, kv_len), summed over those rows
+ * and the query heads of each KV head:
+ *   acc[h][r] (+)= sum_{t, g} softmax_r(q[t][h * G + g] . K^T * kq_scale)
+ * for r < kv_len; accumulate 0 overwrites acc[h][0, kv_len), 1 adds to it.
+ * Arguments as in ep_sp_attend_layer (q is the call's [n_tok][n_head]
+ * [head_dim], k the cache, paged under ep_sp_set_paged_kv); acc is
+ * [n_head_kv][acc_stride] f32 with acc_stride >= kv_len.  q, k and the
+ * workspace are 16-byte aligned.  Each row's weights are added in a fixed
+ * order.  rc 2 on bad arguments. */
+int32_t ep_sp_prompt_weights_bytes(const ep_sp_ctx* ctx, int32_t kv_len, int32_t n_tok, int32_t row_begin,
+                                   size_t* bytes);
+int32_t ep_sp_prompt_weights(ep_sp_ctx* ctx, int32_t layer, const void* q, const void* k, int32_t kv_len,
+                             int32_t n_tok, int32_t row_begin, int32_t accumulate, float* acc, int32_t acc_stride,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated weight.  Of each sequence s and KV head h, with n =
+ * kv_lens[s] rows, m = min(n, n_keep) rows are kept: all of them when n <=
+ * n_keep, else rows [0, sink_rows), rows [n - recent_rows, n) and of the rows
+ * between those of largest acc[s][h][r] (ties: the lower row; NaN ranks as
+ * -inf; sink_rows + recent_rows <= n_keep).  The kept rows of K and V go, in
+ * ascending order, to rows [0, m) of the destination cache (each head its own
+ * selection; later rows of the destination stay as they are).
+ *   dst        the destination's layout (n_seq as in src, max_kv_len and room >=
+ *              min(n_keep, src's max_kv_len); its kv_lens is not read).  Either the same cache (k_dst
+ *              == k, v_dst == v and the same layout and table pointer), which
+ *              is compacted in place, or blocks / rows that are none of the
+ *              source's (the same pool under another table is fine);
+ *   acc_dst    NULL, or [n_seq][n_head_kv][acc_dst_stride]: the kept rows'
+ *              weights, zero from m to acc_dst_stride (acc_dst_stride >=
+ *              min(n_keep, src's max_kv_len); may be acc itself, with the
+ *              same stride);
+ *   new_lens   NULL, or device [n_seq] receiving m (may be src's kv_lens);
+ *   kept_rows  NULL, or device [n_seq][n_head_kv][n_keep]: the kept rows'
+ *              indices in the source, -1 from m on.
+ * After it the layer's page sums and f16 shadows in the context are
+ * forgotten, so a later gated prefill call on the shrunk cache pools it again
+ * (after replaying a captured eviction call ep_sp_reset does that).  rc 2 on
+ * bad arguments. */
+int32_t ep_sp_evict_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_len, int32_t n_keep, size_t* bytes);
+int32_t ep_sp_evict_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* src, const void* k, const void* v,
+                          const float* acc, int32_t acc_stride, int32_t n_keep, int32_t sink_rows,
+                          int32_t recent_rows, const ep_sp_kv_batch* dst, void* k_dst, void* v_dst, float* acc_dst,
+                          int32_t acc_dst_stride, int32_t* new_lens, int32_t* kept_rows, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 /* Synchronises the stream and reads the context's device error word: rc 6
  * (Prefill) when a kernel's bounded wait expired or a selection was out of
- * range or a paged-KV block table entry lay outside the pool since the last
- * check, rc 9 (Unsupported) when an f32 input left the
+ * range or a paged-KV block table entry lay outside the pool or a batch's
+ * sequence length outside its range since the last check, rc 9 (Unsupported) when an f32 input left the
  * f16 range of the tensor-core mode (the word is then cleared), 12 on a CUDA
  * error.
  * It also reads and clears the error word of ep_sp_select_pages_noalloc on
@@ -441,6 +549,10 @@ int32_t ep_sp_sync_status(ep_sp_ctx* ctx, void* stream);
 #define EP_SP_NUM_KERNELS 6
 int32_t ep_sp_profile_enable(ep_sp_ctx* ctx, int32_t on);
 int32_t ep_sp_profile_read(ep_sp_ctx* ctx, double* ms, int64_t* launches);
+/* The first n of all families: those of ep_sp_profile_read, then 6 decode, 7
+ * prompt weights, 8 eviction (n <= EP_SP_NUM_FAMILIES; rc 2 otherwise). */
+#define EP_SP_NUM_FAMILIES 9
+int32_t ep_sp_profile_read_families(ep_sp_ctx* ctx, int32_t n, double* ms, int64_t* launches);
 
 /* Algorithmic work of one ep_sp_attend_layer(layer, kv_len, n_tok) call with
  * the context's current settings, from the same block plan the kernels use:

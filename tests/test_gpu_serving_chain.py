@@ -1,0 +1,119 @@
+"""The operators as they are used together: a gated prefill through the paged cache, the prompt's weights, an eviction,
+decode steps that keep the weights up to date, a second eviction in place, and a further prefill chunk on the shrunk
+cache -- each step against the same steps in 64 bits on a plain cache."""
+import math
+
+import pytest
+import torch
+
+import epsp
+import workloads as W
+from serving_util import context, decode64, kept64, prompt64, rounding, workspace
+
+pytestmark = pytest.mark.gpu
+
+
+class Plain:
+    """One sequence's rows per head, as plain tensors (what a Cache offers to decode64)."""
+
+    def __init__(self, k, v):
+        self.k, self.v, self.lens, self.cap = k, v, [k.shape[0]], k.shape[0]
+
+    def seq(self, i):
+        return self.k, self.v
+
+
+@pytest.mark.parametrize("dtype,heads,page", [(epsp.BF16, (32, 8, 128), 128), (epsp.F16, (14, 2, 64), 64),
+                                              (epsp.F32, (8, 2, 64), 32)], ids=str)
+def test_prefill_evict_decode_evict_prefill(dtype, heads, page):
+    H, K, d = heads
+    n, window, keep, steps, keep2 = 1500, 40, 400, 30, 300
+    w = W.Workload("chain", n + 200, 1, H, K, d, dtype, 512, page, 2, 2 * page)
+    q, k, v = (t.cuda() for t in W.gen_layer(w, 0))
+    B = page
+    ctx = context(H, K, d, dtype, epsp.F32, w.n_tokens, page)
+    ctx.check(ctx.set_ext(1, 0, 0))
+    ctx.check(ctx.set_qg_bound(1, 2, 2, 0))
+    blocks = -(-w.n_tokens // B)
+    g = torch.Generator().manual_seed(3)
+    table = torch.randperm(2 * blocks, generator=g)[:blocks].to(torch.int32).cuda()
+    rows = 2 * blocks * B
+    kp = torch.full((rows, K, d), float("nan"), dtype=k.dtype, device="cuda")
+    vp = kp.clone()
+    ctx.check(ctx.set_paged_kv(B, table, blocks, rows))
+    at = lambda m: table.long()[torch.arange(m, device="cuda") // B] * B + torch.arange(m, device="cuda") % B  # noqa: E731
+    # prefill in chunks, gated
+    ctx.set_prefill_mode(True)
+    out = torch.zeros(n, H, d, device="cuda")
+    for a in range(0, n, 512):
+        b = min(n, a + 512)
+        ctx.check(ctx.append_kv(0, k[a:b].contiguous(), v[a:b].contiguous(), b - a, kp, vp, a))
+        ctx.check(ctx.attend_layer(0, q[a:b].contiguous(), kp, vp, b, b - a, out[a:b]))
+    ctx.set_prefill_mode(False)
+    last = n - (n - 1) // 512 * 512  # the last chunk's rows
+    acc = torch.zeros(K, w.n_tokens, device="cuda")
+    qq = q[n - last:n].contiguous()
+    begin = last - window
+    ctx.check(ctx.prompt_weights(0, qq, kp, n, last, begin, acc, workspace(ctx.prompt_weights_bytes(n, last, begin))))
+    ref, tol = prompt64(qq, k, n, last, begin)
+    assert ((acc[:, :n].double() - ref).abs() <= tol).all()
+    # shrink in place
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    kv = epsp.KvBatch(lens, w.n_tokens, table[None], B, rows)
+    acc3 = acc[None]
+    kept = torch.zeros(1, K, keep, dtype=torch.int32, device="cuda")
+    ws = workspace(max(ctx.evict_bytes(1, w.n_tokens, keep), ctx.decode_bytes(1, w.n_tokens, True)))
+    a_host = acc.cpu().tolist()
+    want = [kept64(a_host[h][:n], n, keep, 4, 64) for h in range(K)]
+    ctx.check(ctx.evict_layer(0, kv, kp, vp, acc3, keep, 4, 64, kv, kp, vp, ws, acc_dst=acc3, new_lens=lens,
+                              kept_rows=kept))
+    assert kept[0].tolist() == want and int(lens) == keep
+    idx = torch.tensor(want, device="cuda")
+    pk = torch.stack([k[idx[h], h] for h in range(K)], 1)
+    pv = torch.stack([v[idx[h], h] for h in range(K)], 1)
+    assert torch.equal(kp[at(keep)], pk) and torch.equal(vp[at(keep)], pv)
+    # decode steps; each writes its row and adds its weights
+    run = acc3.double().clone()
+    lim = torch.zeros_like(run)
+    for i in range(steps):
+        lens.add_(1)
+        m = keep + i + 1
+        kn, vn, qn = (t[n + i][None].contiguous() for t in (k, v, q))
+        pk, pv = torch.cat([pk, kn]), torch.cat([pv, vn])
+        o = torch.zeros(1, H, d, device="cuda")
+        ctx.check(ctx.decode_layer(0, kv, qn, kp, vp, o, ws, k_new=kn, v_new=vn, acc=acc3))
+        r, t, add, add_tol = decode64(Plain(pk, pv), qn)
+        assert ((o.double() - r).abs() <= t + rounding(r, epsp.F32)).all(), i
+        run[:, :, :m] += add
+        lim[:, :, :m] += add_tol
+        lim += run * 2.0 ** -24
+        assert ((acc3.double() - run).abs() <= lim).all(), i
+    # a second eviction, then a gated prefill chunk over the shrunk cache: the same as on a fresh context
+    a_host = acc3[0].cpu().tolist()
+    m = keep + steps
+    want = torch.tensor([kept64(a_host[h][:m], m, keep2, 4, 64) for h in range(K)], device="cuda")
+    ctx.check(ctx.evict_layer(0, kv, kp, vp, acc3, keep2, 4, 64, kv, kp, vp, ws, acc_dst=acc3, new_lens=lens))
+    pk = torch.stack([pk[want[h], h] for h in range(K)], 1)
+    pv = torch.stack([pv[want[h], h] for h in range(K)], 1)
+    assert torch.equal(kp[at(keep2)], pk) and torch.equal(vp[at(keep2)], pv)
+    t = 90
+    more = slice(n + steps, n + steps + t)
+    qn, kn, vn = (x[more].contiguous() for x in (q, k, v))
+    fresh = context(H, K, d, dtype, epsp.F32, w.n_tokens, page)
+    fresh.check(fresh.set_ext(1, 0, 0))
+    outs = []
+    for c, kk, vv in ((ctx, kp, vp), (fresh, torch.cat([pk, kn]).contiguous(), torch.cat([pv, vn]).contiguous())):
+        c.check(c.set_qg_bound(1, 1, 1, 0))
+        c.set_prefill_mode(True)
+        if c is ctx:
+            c.check(c.append_kv(0, kn, vn, t, kk, vv, keep2))
+        o = torch.zeros(t, H, d, device="cuda")
+        sel = torch.full((1, K, 64), -1, dtype=torch.int32, device="cuda")
+        cnt = torch.zeros((1, K), dtype=torch.int32, device="cuda")
+        c.check(c.attend_layer(0, qn, kk, vv, keep2 + t, t, o, sel, cnt, 64))
+        torch.cuda.synchronize()
+        c.check(c.sync_status())
+        outs.append((o, sel, cnt))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert math.isfinite(float(outs[0][0].sum()))
