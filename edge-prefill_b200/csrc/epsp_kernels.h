@@ -284,7 +284,7 @@ struct DecodeArgs {
     uint64_t timeout_ns;
 };
 size_t decode_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
-                       bool weights);
+                       int32_t dtype, bool weights);
 cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t s);
 
 // Softmax weights of the query rows [row_begin, n_tok) of a call (causal, every

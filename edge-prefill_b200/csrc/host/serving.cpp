@@ -121,7 +121,7 @@ int32_t ep_sp_decode_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_l
         (with_acc != 0 && with_acc != 1))
         return kInvalid;
     const ep_sp_config& c = ctx->cfg;
-    *bytes = epsp::decode_ws_bytes(n_seq, max_kv_len, c.n_head, c.n_head_kv, c.head_dim, with_acc != 0);
+    *bytes = epsp::decode_ws_bytes(n_seq, max_kv_len, c.n_head, c.n_head_kv, c.head_dim, c.dtype, with_acc != 0);
     return kOk;
 }
 
@@ -143,7 +143,7 @@ int32_t ep_sp_decode_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* 
         return ctx_fail(ctx, kInvalid, "acc_stride smaller than max_kv_len");
     rc = check_workspace(ctx, workspace, workspace_bytes,
                          epsp::decode_ws_bytes(kv->n_seq, kv->max_kv_len, c.n_head, c.n_head_kv, c.head_dim,
-                                               acc != nullptr));
+                                               c.dtype, acc != nullptr));
     if (rc) return rc;
     DeviceGuard guard;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

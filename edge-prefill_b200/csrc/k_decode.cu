@@ -1,146 +1,911 @@
 // k_decode.cu -- K6: attention of one new token per sequence over its cache.
 //
-// out = softmax(q . K^T * scale) V for each query head over the sequence's
-// rows, in one pass over the cache with a running maximum and sum; the
-// weights variant keeps the scores and adds exp(score - lse) to the rows'
-// accumulated weights afterwards.
+//   x_j = q . k_j * scale,  out = sum_j exp(x_j - m) v_j / sum_j exp(x_j - m)
+//
+// over the rows j < lens[s] of each (sequence, KV head), for the G query heads
+// of the group at once.  Every cache byte is used G times only, so the bytes
+// bound it: what matters is that all SMs stream all the time.
+//
+// Split.  A run is one (sequence, KV head, pass over its query heads, 8 per warp); its
+// rows are cut into units of 32.  All runs' units, laid end to end, are dealt
+// to the CTAs in equal contiguous ranges (computed on the device from the
+// lengths), so ragged batches and one long sequence load the SMs alike.  A run
+// inside one CTA is finished there; one that several CTAs share leaves its
+// running (maximum, sum, output) in the workspace, two slots per CTA, and
+// k6b_join puts them together in a fixed order.
+//
+// CTA: one warp streams K and V units into a ring by TMA (128-byte swizzled
+// rows); units go round robin to the streams of the 8 other warps (4 for f32 rows of 512 bytes), each warp with its
+// own online softmax over 8 query heads (groups of more than 8 heads give a
+// unit to 2, 4 or 8 warps).  No barrier is shared until a run's end, where the
+// warps' states are merged in shared memory.
+//
+// 16-bit: S = Q K^T and O = P V on mma.sync m16n8k16 with 8 heads in rows 0-7.
+// The tensor work is 1/8 of what the pipe could do in the time a unit's bytes
+// take, and the fragments come straight from the ring by ldmatrix; tcgen05
+// would want 128 rows where there are 8.  Rows 8-15 of the P operand carry
+// P - round16(P), so P keeps 16 bits of mantissa (bf16; 22 in f16) at no extra
+// MMA; f32 outputs of bf16 caches add a third part.
+// f32: FMA on the CUDA cores, one key per lane for S, 4 (or 2) columns per
+// lane for O.
+//
+// Weights: the scores are kept in the workspace (4 bytes per query head and
+// row against the 4 d / G of K and V) and k6b_join adds exp(x - lse).
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "epsp_kernels.h"
+#include "tc100.cuh"
 
 namespace epsp {
 namespace {
 
-constexpr int kTile = 128;
+constexpr int kUnit = 32;      // cache rows per unit
+constexpr int kCtas = 148;     // one per SM
+constexpr int kHeads = 8;      // query heads per warp
+constexpr int kChunk = kUnit * 128;  // one 128-byte column block of a unit
+constexpr float kLog2e = 1.4426950408889634f;
+// A call of at most this many units per run and one CTA per run skips the
+// split (and the join).
+constexpr int kDirectUnits = 16;
 
-template <class T>
-__device__ __forceinline__ float to_f(T x) {
-    return static_cast<float>(x);
+struct DecodeSplit {
+    int32_t ctas;      // grid
+    int32_t direct;    // one CTA per run
+    int32_t pass_heads;  // query heads of a pass: 8 per consumer warp
+    int32_t passes;    // passes per KV head
+    int32_t groups;    // warps that share a unit (1, 2, 4, 8), 8 query heads each
+    int32_t score_stride;
+    // workspace
+    int64_t* per;        // units per CTA
+    int64_t* run_start;  // [n_seq][Hkv][passes] first unit of each run
+    float* part_o;       // [2 ctas][groups * 8][D]
+    float2* part_ml;     // [2 ctas][groups * 8] (maximum, sum), log2 units
+    float* lse;          // [n_seq][n_head] log2 units, runs finished by one CTA
+    float* scores;       // [n_seq][n_head][score_stride] log2 units
+};
+
+__host__ __device__ __forceinline__ int units_of(int n) { return (n + kUnit - 1) / kUnit; }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-__device__ __forceinline__ void store_out(void* out, int32_t dtype, int64_t i, float x) {
-    if (dtype == 0) static_cast<float*>(out)[i] = x;
-    else if (dtype == 1) static_cast<__half*>(out)[i] = __float2half_rn(x);
-    else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(x);
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two floats to 16 bits, and what the rounding left over.
+template <bool BF16>
+__device__ __forceinline__ uint32_t split2(float& x, float& y) {
+    uint32_t u;
+    if constexpr (BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        u = *reinterpret_cast<const uint32_t*>(&v);
+        x -= __uint_as_float(u << 16);
+        y -= __uint_as_float(u & 0xffff0000u);
+    } else {
+        const __half2 v = __floats2half2_rn(x, y);
+        u = *reinterpret_cast<const uint32_t*>(&v);
+        const float2 f = __half22float2(v);
+        x -= f.x;
+        y -= f.y;
+    }
+    return u;
 }
 
-// One CTA per (query head, sequence).
-template <class T, int D>
-__global__ void __launch_bounds__(kTile) k6_decode_plain(const DecodeArgs a, float* scores, float* lse, int stride) {
-    __shared__ float qs[D], ps[kTile], red[kTile];
-    __shared__ int rows[kTile];
-    const int hq = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
-    const int G = a.n_head / a.n_head_kv, h = hq / G;
-    const int n = batch_len(a.kv, s, a.err);
-    const T* q = static_cast<const T*>(a.q) + ((int64_t)s * a.n_head + hq) * D;
-    for (int i = t; i < D; i += kTile) qs[i] = to_f(q[i]) * a.kq_scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int j0 = 0; j0 < n; j0 += kTile) {
-        const int j = j0 + t;
-        float x = -INFINITY;
-        if (j < n) {
-            const int row = batch_row(a.kv, s, j, a.err);
-            rows[t] = row;
-            const bool fresh = a.k_new != nullptr && j == n - 1;
-            x = 0.f;
-            if (row >= 0) {
-                const T* kr = fresh ? static_cast<const T*>(a.k_new) + ((int64_t)s * a.n_head_kv + h) * D
-                                    : static_cast<const T*>(a.k) + ((int64_t)row * a.n_head_kv + h) * D;
-                for (int i = 0; i < D; ++i) x += qs[i] * to_f(kr[i]);
-                if (fresh && hq % G == 0) {
-                    const T* vr = static_cast<const T*>(a.v_new) + ((int64_t)s * a.n_head_kv + h) * D;
-                    for (int i = 0; i < D; ++i) {
-                        static_cast<T*>(a.k)[((int64_t)row * a.n_head_kv + h) * D + i] = kr[i];
-                        static_cast<T*>(a.v)[((int64_t)row * a.n_head_kv + h) * D + i] = vr[i];
+__device__ __forceinline__ void store4(void* out, int32_t dtype, int64_t i, float4 x) {
+    if (dtype == 0) {
+        *reinterpret_cast<float4*>(static_cast<float*>(out) + i) = x;
+    } else if (dtype == 1) {
+        const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+        *reinterpret_cast<uint2*>(static_cast<__half*>(out) + i) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + i) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+}
+
+// ET 0 f32, 1 f16, 2 bf16.
+template <int ET, int D>
+struct Layout {
+    static constexpr int kEs = ET == 0 ? 4 : 2;
+    static constexpr int kCols = D * kEs / 128;          // 128-byte column blocks of a row
+    static constexpr int kHalf = kCols * kChunk;         // K (or V) of a unit
+    static constexpr int kStage = 2 * kHalf;
+    // Consumer warps (and a producer).  A stage always falls to the same
+    // stream of warps (kStages is a multiple of kWarps): a warp that found
+    // its stage full knows that the stage's earlier fill had landed, which
+    // the barrier's one phase bit cannot tell it.
+    static constexpr int kWarps = ET == 0 && D == 128 ? 4 : 8;
+    static constexpr int kThreads = (kWarps + 1) * 32;
+    static constexpr int kStages = kStage == 32768 ? 4 : kStage == 16384 ? 8 : 16;
+    static constexpr int kPass = kWarps * kHeads;        // query heads of a pass
+    static constexpr int kOffO = kStages * kStage;       // [8 warps][8 heads][D] merge buffer (f32: q before it)
+    static constexpr int kOffP = kOffO + kWarps * kHeads * D * 4;  // f32: [8 warps][32 keys][8 heads]
+    static constexpr int kOffMl = kOffP + (ET == 0 ? kWarps * kUnit * kHeads * 4 : 0);
+    static constexpr int kOffBar = kOffMl + kWarps * kHeads * 8;
+    static constexpr int kOffPos = kOffBar + 2 * kStages * 8;
+    static constexpr int kBytes = kOffPos + 64 + (kWarps + 1) * 8;
+    static_assert(kStages % kWarps == 0 && kBytes + 1024 <= 232448, "shared memory");
+};
+
+static_assert(kUnit == 32, "a lane per row, a page holds whole units");
+
+// Walks the segments (a run's part inside this CTA) of a CTA's units.
+struct Walk {
+    int32_t s, run, u, n, units;  // sequence, run within it (h * passes + pass), next unit, length, units of the run
+    int64_t left;                 // units of the CTA not walked yet
+    int64_t first;                // the CTA's first unit in the order of all
+};
+
+template <int ET, int D>
+__device__ __forceinline__ void next_run(const DecodeArgs& a, int runs, Walk& w) {
+    w.u = 0;
+    if (++w.run < runs) return;
+    w.run = 0;
+    w.units = 0;
+    while (w.units == 0 && ++w.s < a.kv.n_seq) {
+        w.n = batch_len(a.kv, w.s, a.err);
+        w.units = units_of(w.n);
+    }
+    if (w.units == 0) w.left = 0;
+}
+
+// Overwrites what TMA brought of a sequence's last rows [from, 32) of a unit:
+// row `fresh` (>= 0) from the new token's K and V, V rows from `lim` on with
+// zeros (their P is 0, and 0 * NaN is not 0).
+template <int ET, int D>
+__device__ __forceinline__ void patch_unit(unsigned char* stage, int lane, int lim, int fresh, const char* kn,
+                                           const char* vn) {
+    using LY = Layout<ET, D>;
+    constexpr int nc = LY::kCols * 8;  // 16-byte chunks per row
+    auto at = [&](unsigned char* base, int r, int c) {
+        return reinterpret_cast<uint4*>(base + (c >> 3) * kChunk + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+    };
+    if (fresh >= 0)
+        for (int i = lane; i < 2 * nc; i += 32) {
+            const int c = i % nc;
+            *at(stage + (i < nc ? 0 : LY::kHalf), fresh, c) = *reinterpret_cast<const uint4*>((i < nc ? kn : vn) + c * 16);
+        }
+    for (int i = lane; i < (kUnit - lim) * nc; i += 32)
+        *at(stage + LY::kHalf, lim + i / nc, i % nc) = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes the stage next
+    __syncwarp();
+}
+
+template <int ET, int D, bool P3, int GH>
+__global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
+    k6a_decode(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
+               const DecodeSplit sp) {
+    using LY = Layout<ET, D>;
+    constexpr bool BF16 = ET == 2;
+    constexpr int kWarps = LY::kWarps, kThreads = LY::kThreads, kPass = LY::kPass;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
+    uint64_t* empty = full + LY::kStages;
+    int64_t* pos = reinterpret_cast<int64_t*>(smem + LY::kOffPos);  // [0] total, [1] seq, [2] units before it
+    int64_t* wsum = pos + 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int Hkv = a.n_head_kv, G = a.n_head / Hkv;
+    const int runs = Hkv * sp.passes;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < LY::kStages; ++i) {
+            tc::mbar_init(&full[i], 1);
+            tc::mbar_init(&empty[i], sp.groups);
+        }
+        tc::fence_mbar_init();
+        tc::tma_prefetch_desc(&tmK);
+        tc::tma_prefetch_desc(&tmV);
+    }
+
+    // ----------------------------------------- this CTA's range of the units
+    Walk w0;
+    if (sp.direct) {
+        w0.s = blockIdx.x / runs;
+        w0.run = blockIdx.x % runs;
+        w0.u = 0;
+        w0.n = batch_len(a.kv, w0.s, a.err);
+        w0.units = units_of(w0.n);
+        w0.left = w0.units;
+        w0.first = 0;
+        __syncthreads();
+    } else {
+        int64_t total = 0, per = 0, first = 0;
+        // twice over the sequences: their sum, then the one the range begins in
+        for (int round = 0; round < 2; ++round) {
+            int64_t base = 0;
+            for (int s0 = 0; s0 < a.kv.n_seq; s0 += kThreads) {
+                const int s = s0 + (int)threadIdx.x;
+                const int64_t mine = s < a.kv.n_seq ? (int64_t)units_of(batch_len(a.kv, s, a.err)) * runs : 0;
+                int64_t incl = mine;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
+                    if (lane >= d) incl += v;
+                }
+                __syncthreads();
+                if (lane == 31) wsum[warp] = incl;
+                __syncthreads();
+                int64_t before = base, all = 0;
+                for (int i = 0; i <= kWarps; ++i) {
+                    if (i < warp) before += wsum[i];
+                    all += wsum[i];
+                }
+                incl += before;
+                if (round == 1 && mine > 0 && first >= incl - mine && first < incl) {
+                    pos[1] = s;
+                    pos[2] = incl - mine;
+                }
+                base += all;
+            }
+            if (round == 0) {
+                total = base;
+                // at least one unit per warp of a CTA
+                per = (total + sp.ctas - 1) / sp.ctas;
+                if (per < kWarps) per = kWarps;
+                first = per * blockIdx.x;
+            }
+        }
+        __syncthreads();
+        if (blockIdx.x == 0 && threadIdx.x == 0) *sp.per = per;
+        w0.first = first;
+        w0.left = first >= total ? 0 : (total - first < per ? total - first : per);
+        if (w0.left > 0) {
+            w0.s = (int32_t)pos[1];
+            w0.n = batch_len(a.kv, w0.s, a.err);
+            w0.units = units_of(w0.n);
+            const int64_t off = first - pos[2];
+            w0.run = (int32_t)(off / w0.units);
+            w0.u = (int32_t)(off % w0.units);
+        }
+    }
+    if (w0.left == 0) {
+        if (sp.direct) {  // a sequence without rows
+            const int g0 = (w0.run % sp.passes) * kPass, n = min(kPass, G - g0) * (D / 4);
+            const int64_t at = ((int64_t)w0.s * a.n_head + (w0.run / sp.passes) * G + g0) * D;
+            for (int i = threadIdx.x; i < n; i += kThreads)
+                store4(a.out, a.out_dtype, at + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+        }
+        return;
+    }
+    const uint64_t tmo = a.timeout_ns;
+
+    if (warp == kWarps) {
+        // ------------------------------------------------------- producer --
+        // 32 units' rows at a time (one table entry per lane), lane 0 issues.
+        Walk w = w0;
+        int64_t it = 0;
+        bool ok = true;
+        while (w.left > 0 && ok) {
+            const int n_seg = (int)min((int64_t)(w.units - w.u), w.left);
+            const int h = w.run / sp.passes;
+            for (int i0 = 0; i0 < n_seg && ok; i0 += 32) {
+                int row = a.kv.rows;  // past the end: zeros
+                if (i0 + lane < n_seg) {
+                    const int r = batch_row(a.kv, w.s, (w.u + i0 + lane) * kUnit, a.err);
+                    if (r >= 0) row = r;
+                }
+                const int cnt = min(32, n_seg - i0);
+                for (int i = 0; i < cnt; ++i, ++it) {
+                    const int st = (int)(it % LY::kStages);
+                    const int r = __shfl_sync(0xffffffffu, row, i);
+                    if (lane == 0) {
+                        ok = tc::mbar_wait(&empty[st], ((it / LY::kStages) & 1) ^ 1, tmo);
+                        if (ok) {
+                            tc::mbar_arrive_expect_tx(&full[st], LY::kStage);
+                            unsigned char* base = smem + st * LY::kStage;
+#pragma unroll
+                            for (int c = 0; c < LY::kCols; ++c)
+                                tc::tma_load_3d(base + c * kChunk, &tmK, &full[st], c * (128 / LY::kEs), h, r);
+#pragma unroll
+                            for (int c = 0; c < LY::kCols; ++c)
+                                tc::tma_load_3d(base + LY::kHalf + c * kChunk, &tmV, &full[st], c * (128 / LY::kEs), h,
+                                                r);
+                        }
                     }
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) break;
                 }
             }
-            if (scores) scores[((int64_t)s * a.n_head + hq) * stride + j] = x;
+            w.u += n_seg;
+            w.left -= n_seg;
+            if (w.left > 0) next_run<ET, D>(a, runs, w);
         }
-        red[t] = x;
-        __syncthreads();
-        for (int w = kTile / 2; w > 0; w >>= 1) {
-            if (t < w) red[t] = fmaxf(red[t], red[t + w]);
-            __syncthreads();
+        if (!ok) {
+            if (lane == 0) report_error(a.err, kDevWaitDecode, 0xa1, (int32_t)it);
+            // copies still in flight land before the CTA ends
+            for (int64_t j = it > LY::kStages ? it - LY::kStages : 0; j < it; ++j)
+                tc::mbar_wait(&full[j % LY::kStages], (j / LY::kStages) & 1, tmo);
         }
-        const float m2 = fmaxf(m, red[0]);
-        const float ms = m2 == -INFINITY ? 0.f : m2;
-        const float p = j < n ? expf(x - ms) : 0.f;
-        const float alpha = expf(m - ms);
-        __syncthreads();
-        ps[t] = p;
-        red[t] = p;
-        __syncthreads();
-        for (int w = kTile / 2; w > 0; w >>= 1) {
-            if (t < w) red[t] += red[t + w];
-            __syncthreads();
+        return;
+    }
+
+    // ---------------------------------------------------------- consumers --
+    const int groups = sp.groups, streams = kWarps / groups;
+    const int grp = warp & (groups - 1), stream = warp / groups;
+    const float sl2 = a.kq_scale * kLog2e;
+    float* om = reinterpret_cast<float*>(smem + LY::kOffO);
+    float* om_w = om + warp * kHeads * D;
+    float* ps = reinterpret_cast<float*>(smem + LY::kOffP) + warp * kUnit * kHeads;
+    float2* ml = reinterpret_cast<float2*>(smem + LY::kOffMl);
+    Walk w = w0;
+    int64_t it = 0;
+    bool ok = true;
+    for (int seg = 0; w.left > 0; ++seg) {
+        const int n_seg = (int)min((int64_t)(w.units - w.u), w.left);
+        const int h = w.run / sp.passes, pass = w.run % sp.passes;
+        const int g0 = pass * kPass + grp * kHeads;  // this warp's first query head of the group
+        const int64_t q_row = (int64_t)w.s * a.n_head + (int64_t)h * G;
+        // state: 16-bit o[2 columns x 8 heads in MMA fragments], f32 o[head][columns]
+        constexpr int NO = ET == 0 ? GH * (D / 32) : D / 2;
+        float o[NO];
+#pragma unroll
+        for (int i = 0; i < NO; ++i) o[i] = 0.f;
+        constexpr int NM = ET == 0 ? GH : 1;
+        float m[NM], l[NM];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
         }
-        l = l * alpha + red[0];
-        o *= alpha;
-        if (t < D) {
-            for (int i = 0; i < kTile && j0 + i < n; ++i) {
-                if (rows[i] < 0) continue;
-                const T* vr = a.v_new != nullptr && j0 + i == n - 1
-                                  ? static_cast<const T*>(a.v_new) + ((int64_t)s * a.n_head_kv + h) * D
-                                  : static_cast<const T*>(a.v) + ((int64_t)rows[i] * a.n_head_kv + h) * D;
-                o += ps[i] * to_f(vr[t]);
+        uint32_t qf[ET == 0 ? 1 : D / 8];
+        const int hd = lane >> 2, qc = (lane & 3) * 2;  // 16-bit: head and columns of this lane's fragments
+        if constexpr (ET == 0) {
+            __syncwarp();
+            for (int i = lane; i < GH * (D / 4); i += 32) {
+                const int g = i / (D / 4);
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (g0 + g < G)
+                    x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (q_row + g0 + g) * D +
+                                                         (i % (D / 4)) * 4);
+                reinterpret_cast<float4*>(om_w)[i] = x;
+            }
+            __syncwarp();
+        } else {
+            const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (q_row + g0 + hd) * D + qc;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+                qf[i] = g0 + hd < G ? *reinterpret_cast<const uint32_t*>(qp + i * 8) : 0u;
+        }
+        // first unit of the segment that falls to this stream
+        int i = (int)(((int64_t)stream - it % streams + streams) % streams);
+        for (; i < n_seg; i += streams) {
+            const int64_t at = it + i;
+            const int st = (int)(at % LY::kStages);
+            if (ok) {
+                ok = tc::mbar_wait(&full[st], (at / LY::kStages) & 1, tmo);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xa2, (int32_t)at);
+            }
+            if (!ok) break;
+            unsigned char* stage = smem + st * LY::kStage;
+            const int u = w.u + i, lim = min(kUnit, w.n - u * kUnit);
+            if (u == w.units - 1) {
+                const bool fresh = a.k_new != nullptr;
+                const int64_t nr = ((int64_t)w.s * Hkv + h) * D * LY::kEs;
+                const char* kn = static_cast<const char*>(a.k_new) + nr;
+                const char* vn = static_cast<const char*>(a.v_new) + nr;
+                if (fresh || lim < kUnit) patch_unit<ET, D>(stage, lane, lim, fresh ? lim - 1 : -1, kn, vn);
+                if (fresh && grp == 0 && pass == 0) {
+                    const int row = batch_row(a.kv, w.s, w.n - 1, a.err);
+                    constexpr int nc = D * LY::kEs / 16;
+                    if (row >= 0)
+                        for (int c = lane; c < 2 * nc; c += 32) {
+                            const int64_t to = ((int64_t)row * Hkv + h) * D * LY::kEs + (c % nc) * 16;
+                            *reinterpret_cast<uint4*>(static_cast<char*>(c < nc ? a.k : a.v) + to) =
+                                *reinterpret_cast<const uint4*>((c < nc ? kn : vn) + (c % nc) * 16);
+                        }
+                }
+            }
+            if constexpr (ET != 0) {
+                const uint32_t kb = tc::smem_u32(stage), vb = kb + LY::kHalf;
+                float s4[4][4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    s4[t][0] = s4[t][1] = s4[t][2] = s4[t][3] = 0.f;
+                    const int r = t * 8 + (lane & 7);
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {  // 32 columns (4 chunks) a time
+                        const int ch = (c & 1) * 4 + (lane >> 3);
+                        uint32_t b[4];
+                        ldsm4(b, kb + (c >> 1) * kChunk + r * 128 + ((ch ^ (r & 7)) << 4));
+                        mma16816<BF16>(s4[t], qf[4 * c], 0, qf[4 * c + 1], 0, b[0], b[1]);
+                        mma16816<BF16>(s4[t], qf[4 * c + 2], 0, qf[4 * c + 3], 0, b[2], b[3]);
+                    }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        s4[t][e] = t * 8 + qc + e < lim ? s4[t][e] * sl2 : -INFINITY;
+                        mx = fmaxf(mx, s4[t][e]);
+                    }
+                if (a.acc != nullptr && g0 + hd < G) {
+                    float* sc = sp.scores + (q_row + g0 + hd) * sp.score_stride + u * kUnit + qc;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        *reinterpret_cast<float2*>(sc + t * 8) = make_float2(s4[t][0], s4[t][1]);
+                }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                // the running maximum follows when it is 2^8 behind: p stays below 2^8
+                const bool need = mx > m[0] + 8.f;
+                if (__any_sync(0xffffffffu, need)) {
+                    const float alpha = need ? ex2(m[0] - mx) : 1.f;
+                    if (need) m[0] = mx;
+                    l[0] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < NO; ++j) o[j] *= alpha;
+                }
+                const float ms = m[0] == -INFINITY ? 0.f : m[0];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        s4[t][e] = ex2(s4[t][e] - ms);
+                        l[0] += s4[t][e];
+                    }
+#pragma unroll
+                for (int kb16 = 0; kb16 < 2; ++kb16) {
+                    float* p0 = s4[2 * kb16];
+                    float* p1 = s4[2 * kb16 + 1];
+                    const uint32_t a0 = split2<BF16>(p0[0], p0[1]), a2 = split2<BF16>(p1[0], p1[1]);
+                    const uint32_t a1 = split2<BF16>(p0[0], p0[1]), a3 = split2<BF16>(p1[0], p1[1]);
+                    uint32_t t0 = 0, t2 = 0;
+                    if constexpr (P3) {
+                        t0 = split2<BF16>(p0[0], p0[1]);
+                        t2 = split2<BF16>(p1[0], p1[1]);
+                    }
+                    const int r = kb16 * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) {  // 16 columns (2 chunks) a time
+                        const int ch = (c & 3) * 2 + (lane >> 4);
+                        uint32_t b[4];
+                        ldsm4_t(b, vb + (c >> 2) * kChunk + r * 128 + ((ch ^ (r & 7)) << 4));
+                        float(&o0)[4] = *reinterpret_cast<float(*)[4]>(&o[8 * c]);
+                        float(&o1)[4] = *reinterpret_cast<float(*)[4]>(&o[8 * c + 4]);
+                        mma16816<BF16>(o0, a0, a1, a2, a3, b[0], b[1]);
+                        mma16816<BF16>(o1, a0, a1, a2, a3, b[2], b[3]);
+                        if constexpr (P3) {
+                            mma16816<BF16>(o0, t0, 0, t2, 0, b[0], b[1]);
+                            mma16816<BF16>(o1, t0, 0, t2, 0, b[2], b[3]);
+                        }
+                    }
+                }
+            } else {
+                // S: one key per lane
+                float x[GH];
+#pragma unroll
+                for (int g = 0; g < GH; ++g) x[g] = 0.f;
+                const float4* q4 = reinterpret_cast<const float4*>(om_w);
+#pragma unroll 4
+                for (int c = 0; c < D / 4; ++c) {
+                    const float4 kk = *reinterpret_cast<const float4*>(stage + (c >> 3) * kChunk + lane * 128 +
+                                                                       (((c & 7) ^ (lane & 7)) << 4));
+#pragma unroll
+                    for (int g = 0; g < GH; ++g) {
+                        const float4 qq = q4[g * (D / 4) + c];
+                        x[g] = fmaf(qq.x, kk.x, x[g]);
+                        x[g] = fmaf(qq.y, kk.y, x[g]);
+                        x[g] = fmaf(qq.z, kk.z, x[g]);
+                        x[g] = fmaf(qq.w, kk.w, x[g]);
+                    }
+                }
+                bool need = false;
+                float mx[GH];
+#pragma unroll
+                for (int g = 0; g < GH; ++g) {
+                    x[g] = lane < lim ? x[g] * sl2 : -INFINITY;
+                    if (a.acc != nullptr && g0 + g < G)
+                        sp.scores[(q_row + g0 + g) * sp.score_stride + u * kUnit + lane] = x[g];
+                    mx[g] = x[g];
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) mx[g] = fmaxf(mx[g], __shfl_xor_sync(0xffffffffu, mx[g], d));
+                    need |= mx[g] > m[g] + 8.f;
+                }
+                if (need) {
+#pragma unroll
+                    for (int g = 0; g < GH; ++g)
+                        if (mx[g] > m[g]) {
+                            const float alpha = ex2(m[g] - mx[g]);
+                            m[g] = mx[g];
+                            l[g] *= alpha;
+#pragma unroll
+                            for (int j = 0; j < D / 32; ++j) o[g * (D / 32) + j] *= alpha;
+                        }
+                }
+#pragma unroll
+                for (int g = 0; g < GH; ++g) {
+                    x[g] = ex2(x[g] - (m[g] == -INFINITY ? 0.f : m[g]));
+                    l[g] += x[g];
+                    ps[lane * kHeads + g] = x[g];
+                }
+                __syncwarp();
+                // O: D / 32 columns per lane, over the unit's keys
+                constexpr int NC = D / 32;
+                const int cb = lane * NC * 4;  // byte of the first column
+                const unsigned char* vbase = stage + LY::kHalf + (cb >> 7) * kChunk;
+                const int ch = (cb >> 4) & 7, in = cb & 15;
+#pragma unroll 4
+                for (int j = 0; j < lim; ++j) {
+                    const unsigned char* vp = vbase + j * 128 + ((ch ^ (j & 7)) << 4) + in;
+                    float vv[NC];
+                    if constexpr (NC == 4) {
+                        const float4 t = *reinterpret_cast<const float4*>(vp);
+                        vv[0] = t.x, vv[1] = t.y, vv[2] = t.z, vv[3] = t.w;
+                    } else {
+                        const float2 t = *reinterpret_cast<const float2*>(vp);
+                        vv[0] = t.x, vv[1] = t.y;
+                    }
+#pragma unroll
+                    for (int g = 0; g < GH; ++g) {
+                        const float p = ps[j * kHeads + g];
+#pragma unroll
+                        for (int e = 0; e < NC; ++e) o[g * NC + e] = fmaf(p, vv[e], o[g * NC + e]);
+                    }
+                }
+                __syncwarp();
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&empty[st]);
+        }
+
+        // ------------------------------------------- merge the warps' states
+        if constexpr (ET != 0) {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], 1);
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], 2);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c)  // rows 8-15 hold the P remainders' part
+                *reinterpret_cast<float2*>(om_w + hd * D + c * 8 + qc) =
+                    make_float2(o[4 * c] + o[4 * c + 2], o[4 * c + 1] + o[4 * c + 3]);
+            if ((lane & 3) == 0) ml[warp * kHeads + hd] = make_float2(m[0], l[0]);
+        } else {
+            constexpr int NC = D / 32;
+            __syncwarp();
+#pragma unroll
+            for (int g = 0; g < GH; ++g) {
+                float t = l[g];
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+#pragma unroll
+                for (int e = 0; e < NC; ++e) om_w[g * D + lane * NC + e] = o[g * NC + e];
+                if (lane == 0) ml[warp * kHeads + g] = make_float2(m[g], t);
             }
         }
-        m = m2;
-        __syncthreads();
+        tc::named_bar_sync(1, kWarps * 32);
+        const bool whole = w.u == 0 && n_seg == w.units;
+        const int n_heads = min(groups * kHeads, G - pass * kPass);
+        const int slot = blockIdx.x * 2 + (seg == 0 ? 0 : 1);
+        for (int j = threadIdx.x; j < n_heads * (D / 4); j += kWarps * 32) {
+            const int g = j / (D / 4), c = j % (D / 4);
+            float mt = -INFINITY;
+            for (int r = 0; r < streams; ++r) {
+                const float2 v = ml[(r * groups + g / kHeads) * kHeads + g % kHeads];
+                if (v.y != 0.f) mt = fmaxf(mt, v.x);
+            }
+            const float ms = mt == -INFINITY ? 0.f : mt;
+            float lt = 0.f;
+            float4 ot = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int r = 0; r < streams; ++r) {
+                const int wr = r * groups + g / kHeads;
+                const float2 v = ml[wr * kHeads + g % kHeads];
+                if (v.y == 0.f) continue;  // no unit, or nothing but -inf
+                const float f = ex2(v.x - ms);
+                const float4 t = *reinterpret_cast<const float4*>(om + (wr * kHeads + g % kHeads) * D + c * 4);
+                lt += f * v.y;
+                ot.x += f * t.x, ot.y += f * t.y, ot.z += f * t.z, ot.w += f * t.w;
+            }
+            if (whole) {
+                const float inv = 1.f / lt;
+                store4(a.out, a.out_dtype, (q_row + pass * kPass + g) * D + c * 4,
+                       make_float4(ot.x * inv, ot.y * inv, ot.z * inv, ot.w * inv));
+                if (c == 0 && a.acc != nullptr) sp.lse[q_row + pass * kPass + g] = ms + log2f(lt);
+            } else {
+                const int64_t p = (int64_t)slot * groups * kHeads + g;
+                *reinterpret_cast<float4*>(sp.part_o + p * D + c * 4) = ot;
+                if (c == 0) sp.part_ml[p] = make_float2(mt, lt);
+            }
+        }
+        if (w.u == 0 && !sp.direct && threadIdx.x == 0) sp.run_start[(int64_t)w.s * runs + w.run] = w0.first + it;
+        tc::named_bar_sync(1, kWarps * 32);
+        it += n_seg;
+        w.u += n_seg;
+        w.left -= n_seg;
+        if (w.left > 0) next_run<ET, D>(a, runs, w);
     }
-    if (t < D) store_out(a.out, a.out_dtype, ((int64_t)s * a.n_head + hq) * D + t, n > 0 ? o / l : 0.f);
-    if (lse && t == 0) lse[(int64_t)s * a.n_head + hq] = m + logf(l);
 }
 
-__global__ void k6_add_weights(const DecodeArgs a, const float* scores, const float* lse, int stride) {
-    const int h = blockIdx.y, s = blockIdx.z, j = blockIdx.x * blockDim.x + threadIdx.x;
-    const int G = a.n_head / a.n_head_kv;
-    if (j >= batch_len(a.kv, s, a.err)) return;
-    float w = 0.f;
-    for (int g = 0; g < G; ++g) {
-        const int64_t i = (int64_t)s * a.n_head + h * G + g;
-        w += expf(scores[i * stride + j] - lse[i]);
+// CTAs that share run `at` of sequence s, and each one's slot.
+struct Shares {
+    int64_t per, start;
+    int32_t c0, count;
+    __device__ __forceinline__ int slot(int i) const {
+        const int c = c0 + i;
+        return 2 * c + (i == 0 && start > c * per ? 1 : 0);
     }
-    a.acc[((int64_t)s * a.n_head_kv + h) * a.acc_stride + j] += w;
+};
+__device__ __forceinline__ Shares shares_of(const DecodeSplit& sp, int64_t run, int units) {
+    Shares r{1, 0, 0, 1};
+    if (sp.direct) return r;
+    r.per = *sp.per;
+    r.start = sp.run_start[run];
+    r.c0 = (int32_t)(r.start / r.per);
+    r.count = (int32_t)((r.start + units - 1) / r.per) - r.c0 + 1;
+    return r;
+}
+
+// Maximum and sum of one head over its shares (a warp; the same in every lane).
+__device__ __forceinline__ float2 join_ml(const DecodeSplit& sp, const Shares& sh, int stride, int g, int lane) {
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < sh.count; i += 32) {
+        const float2 v = sp.part_ml[(int64_t)sh.slot(i) * stride + g];
+        if (v.y != 0.f) m = fmaxf(m, v.x);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float ms = m == -INFINITY ? 0.f : m;
+    for (int i = lane; i < sh.count; i += 32) {
+        const float2 v = sp.part_ml[(int64_t)sh.slot(i) * stride + g];
+        if (v.y != 0.f) l += v.y * ex2(v.x - ms);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    return make_float2(ms, l);
+}
+
+constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 1024;  // cache rows per weights CTA
+
+// Grid (n_head + [weights] Hkv * chunks, n_seq): the first n_head CTAs of a
+// sequence put together the outputs of runs that several CTAs shared, the
+// others add the weights of kJoinRows rows of one KV head.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, const DecodeSplit sp) {
+    __shared__ float wgt[kCtas];
+    __shared__ float part[kJoinThreads * 4];
+    __shared__ float lse[128];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int G = a.n_head / a.n_head_kv, runs = a.n_head_kv * sp.passes, stride = sp.groups * kHeads;
+    const int n = batch_len(a.kv, s, a.err), units = units_of(n);
+    if ((int)blockIdx.x < a.n_head) {
+        const int hq = blockIdx.x, h = hq / G, g = hq % G, pass = g / sp.pass_heads;
+        const int64_t out = ((int64_t)s * a.n_head + hq) * D;
+        if (sp.direct) return;
+        if (n == 0) {
+            for (int i = threadIdx.x; i < D / 4; i += kJoinThreads)
+                store4(a.out, a.out_dtype, out + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+            return;
+        }
+        const Shares sh = shares_of(sp, (int64_t)s * runs + h * sp.passes + pass, units);
+        if (sh.count == 1) return;
+        const int gi = g % sp.pass_heads;
+        if (warp == 0) {
+            const float2 v = join_ml(sp, sh, stride, gi, lane);
+            for (int i = lane; i < sh.count; i += 32) {
+                const float2 p = sp.part_ml[(int64_t)sh.slot(i) * stride + gi];
+                wgt[i] = p.y != 0.f ? ex2(p.x - v.x) / v.y : 0.f;
+            }
+        }
+        __syncthreads();
+        constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes;
+        const int c = threadIdx.x % kLanes, r = threadIdx.x / kLanes;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = r; i < sh.count; i += kRows) {
+            const float f = wgt[i];
+            if (f == 0.f) continue;
+            const float4 t =
+                *reinterpret_cast<const float4*>(sp.part_o + ((int64_t)sh.slot(i) * stride + gi) * D + c * 4);
+            o.x += f * t.x, o.y += f * t.y, o.z += f * t.z, o.w += f * t.w;
+        }
+        reinterpret_cast<float4*>(part)[threadIdx.x] = o;
+        __syncthreads();
+        if (r == 0) {
+            for (int i = 1; i < kRows; ++i) {
+                const float4 t = reinterpret_cast<float4*>(part)[i * kLanes + c];
+                o.x += t.x, o.y += t.y, o.z += t.z, o.w += t.w;
+            }
+            store4(a.out, a.out_dtype, out + c * 4, o);
+        }
+        return;
+    }
+    const int id = blockIdx.x - a.n_head, chunks = (gridDim.x - a.n_head) / a.n_head_kv;
+    const int h = id / chunks, j0 = (id % chunks) * kJoinRows;
+    if (j0 >= n) return;
+    for (int g = warp; g < G; g += kJoinThreads / 32) {
+        const int pass = g / sp.pass_heads;
+        const Shares sh = shares_of(sp, (int64_t)s * runs + h * sp.passes + pass, units);
+        float x;
+        if (sh.count == 1) {
+            x = sp.lse[(int64_t)s * a.n_head + h * G + g];
+        } else {
+            const float2 v = join_ml(sp, sh, stride, g % sp.pass_heads, lane);
+            x = v.x + log2f(v.y);
+        }
+        if (lane == 0) lse[g] = x;
+    }
+    __syncthreads();
+    const float* sc = sp.scores + ((int64_t)s * a.n_head + (int64_t)h * G) * sp.score_stride;
+    float* acc = a.acc + ((int64_t)s * a.n_head_kv + h) * a.acc_stride;
+    for (int j = j0 + threadIdx.x; j < min(n, j0 + kJoinRows); j += kJoinThreads) {
+        float w = 0.f;
+        for (int g = 0; g < G; ++g) w += ex2(sc[(int64_t)g * sp.score_stride + j] - lse[g]);
+        acc[j] += w;
+    }
+}
+
+// ---------------------------------------------------------------- host side --
+PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> fn{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 f = fn.load(std::memory_order_acquire);
+    if (!f) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+        fn.store(f, std::memory_order_release);
+    }
+    return f;
+}
+
+// Cache rows [rows][Hkv][d] in boxes of 32 rows x 128 bytes of one head.
+bool cache_map(CUtensorMap* m, const void* base, int32_t dtype, int32_t d, int32_t n_head_kv, int32_t rows) {
+    auto enc = get_encode();
+    if (!enc) return false;
+    const uint64_t es = dtype == 0 ? 4 : 2;
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)n_head_kv, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {d * es, d * es * n_head_kv};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / es), 1, kUnit};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUtensorMapDataType t = dtype == 0   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return enc(m, t, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+// Split of a call and its workspace layout; returns the bytes.
+size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_head_kv, int32_t d, int32_t dtype,
+                bool weights, char* ws, DecodeSplit* sp) {
+    const int G = n_head / n_head_kv;
+    const int warps = dtype == 0 && d == 128 ? Layout<0, 128>::kWarps : Layout<2, 128>::kWarps;
+    sp->pass_heads = warps * kHeads;
+    const int in_pass = G < sp->pass_heads ? G : sp->pass_heads;
+    int groups = 1;
+    while (groups * kHeads < in_pass) groups *= 2;
+    sp->passes = (G + sp->pass_heads - 1) / sp->pass_heads;
+    sp->groups = groups;
+    const int64_t all_runs = (int64_t)n_seq * n_head_kv * sp->passes;
+    const int64_t units = units_of(max_kv_len), total = all_runs * units;
+    sp->direct = all_runs <= kCtas && units <= kDirectUnits;
+    const int64_t ctas = sp->direct ? all_runs : (total + warps - 1) / warps;
+    sp->ctas = (int32_t)(ctas < kCtas ? ctas : kCtas);
+    sp->score_stride = (int32_t)(units * kUnit);
+    size_t at = 16;
+    auto take = [&](size_t bytes) {
+        const size_t was = at;
+        at += up16(bytes);
+        return ws + was;
+    };
+    sp->per = reinterpret_cast<int64_t*>(ws);
+    const int stride = groups * kHeads;
+    if (!sp->direct) {
+        sp->run_start = reinterpret_cast<int64_t*>(take(all_runs * sizeof(int64_t)));
+        sp->part_ml = reinterpret_cast<float2*>(take((size_t)2 * sp->ctas * stride * sizeof(float2)));
+        sp->part_o = reinterpret_cast<float*>(take((size_t)2 * sp->ctas * stride * d * sizeof(float)));
+    }
+    if (weights) {
+        sp->lse = reinterpret_cast<float*>(take((size_t)n_seq * n_head * sizeof(float)));
+        sp->scores = reinterpret_cast<float*>(take((size_t)n_seq * n_head * sp->score_stride * sizeof(float)));
+    }
+    return at;
+}
+
+template <int ET, int D, bool P3, int GH>
+cudaError_t launch_t(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s) {
+    constexpr int kThreads = Layout<ET, D>::kThreads;
+    CUtensorMap mk, mv;
+    if (!cache_map(&mk, a.k, a.dtype, D, a.n_head_kv, a.kv.rows) ||
+        !cache_map(&mv, a.v, a.dtype, D, a.n_head_kv, a.kv.rows))
+        return cudaErrorInvalidValue;
+    const int smem = Layout<ET, D>::kBytes + 1024;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    // one bit per device ordinal < 32 whose attribute is set
+    static std::atomic<unsigned> set_mask{0};
+    if (dev >= 32 || !(set_mask.load(std::memory_order_acquire) & (1u << dev))) {
+        const cudaError_t e = cudaFuncSetAttribute(k6a_decode<ET, D, P3, GH>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        if (dev < 32) set_mask.fetch_or(1u << dev, std::memory_order_release);
+    }
+    k6a_decode<ET, D, P3, GH><<<sp.ctas, kThreads, smem, s>>>(mk, mv, a, sp);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || (sp.direct && !a.acc)) return e;
+    const int chunks = a.acc ? (a.kv.max_kv_len + kJoinRows - 1) / kJoinRows : 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.n_head + a.n_head_kv * chunks, a.kv.n_seq);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k6b_join<D>, a, sp);
+}
+
+template <int ET, int D>
+cudaError_t launch_d(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s) {
+    if constexpr (ET == 0) {
+        const int G = a.n_head / a.n_head_kv;
+        if (G == 1) return launch_t<0, D, false, 1>(a, sp, s);
+        if (G == 2) return launch_t<0, D, false, 2>(a, sp, s);
+        if (G <= 4) return launch_t<0, D, false, 4>(a, sp, s);
+        return launch_t<0, D, false, 8>(a, sp, s);
+    } else if constexpr (ET == 1) {
+        return launch_t<1, D, false, 8>(a, sp, s);
+    } else {
+        return a.out_dtype == 0 ? launch_t<2, D, true, 8>(a, sp, s) : launch_t<2, D, false, 8>(a, sp, s);
+    }
 }
 
 }  // namespace
 
-size_t decode_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t, int32_t, bool weights) {
-    if (!weights) return 16;
-    const size_t stride = (size_t)(max_kv_len + 31) / 32 * 32;
-    return ((size_t)n_seq * n_head * (stride + 1) + 16) * sizeof(float);
+size_t decode_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                       int32_t dtype, bool weights) {
+    DecodeSplit sp{};
+    return split_of(n_seq, max_kv_len, n_head, n_head_kv, head_dim, dtype, weights, nullptr, &sp);
 }
 
 cudaError_t launch_decode(const DecodeArgs& a, cudaStream_t s) {
-    float *scores = nullptr, *lse = nullptr;
-    const int stride = (a.kv.max_kv_len + 31) / 32 * 32;
-    if (a.acc) {
-        scores = static_cast<float*>(a.ws);
-        lse = scores + (size_t)a.kv.n_seq * a.n_head * stride;
+    DecodeSplit sp{};
+    split_of(a.kv.n_seq, a.kv.max_kv_len, a.n_head, a.n_head_kv, a.head_dim, a.dtype, a.acc != nullptr,
+             static_cast<char*>(a.ws), &sp);
+    const bool wide = a.head_dim == 128;
+    switch (a.dtype) {
+        case 0: return wide ? launch_d<0, 128>(a, sp, s) : launch_d<0, 64>(a, sp, s);
+        case 1: return wide ? launch_d<1, 128>(a, sp, s) : launch_d<1, 64>(a, sp, s);
+        default: return wide ? launch_d<2, 128>(a, sp, s) : launch_d<2, 64>(a, sp, s);
     }
-    const dim3 grid(a.n_head, a.kv.n_seq);
-#define GO(T, D) k6_decode_plain<T, D><<<grid, kTile, 0, s>>>(a, scores, lse, stride)
-    if (a.head_dim == 128) {
-        if (a.dtype == 0) GO(float, 128);
-        else if (a.dtype == 1) GO(__half, 128);
-        else GO(__nv_bfloat16, 128);
-    } else {
-        if (a.dtype == 0) GO(float, 64);
-        else if (a.dtype == 1) GO(__half, 64);
-        else GO(__nv_bfloat16, 64);
-    }
-#undef GO
-    cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess && a.acc) {
-        k6_add_weights<<<dim3((a.kv.max_kv_len + 255) / 256, a.n_head_kv, a.kv.n_seq), 256, 0, s>>>(a, scores, lse,
-                                                                                                  stride);
-        e = cudaGetLastError();
-    }
-    return e;
 }
 
 }  // namespace epsp
