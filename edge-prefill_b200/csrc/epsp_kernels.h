@@ -304,7 +304,8 @@ struct WeightArgs {
     int32_t* err;
     uint64_t timeout_ns;
 };
-size_t weights_ws_bytes(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv);
+size_t weights_ws_bytes(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                        int32_t dtype);
 cudaError_t launch_prompt_weights(const WeightArgs& a, cudaStream_t s);
 
 // Eviction: per sequence and KV head the sink rows, the recent rows and the

@@ -173,7 +173,8 @@ int32_t ep_sp_prompt_weights_bytes(const ep_sp_ctx* ctx, int32_t kv_len, int32_t
     if (!ctx || !bytes || n_tok < 1 || kv_len < n_tok || kv_len > ctx->cfg.max_ctx || row_begin < 0 ||
         row_begin >= n_tok)
         return kInvalid;
-    *bytes = epsp::weights_ws_bytes(kv_len, n_tok - row_begin, ctx->cfg.n_head, ctx->cfg.n_head_kv);
+    *bytes = epsp::weights_ws_bytes(kv_len, n_tok - row_begin, ctx->cfg.n_head, ctx->cfg.n_head_kv, ctx->cfg.head_dim,
+                                    ctx->cfg.dtype);
     return kOk;
 }
 
@@ -193,7 +194,8 @@ int32_t ep_sp_prompt_weights(ep_sp_ctx* ctx, int32_t layer, const void* q, const
     if (ctx->paging.block_rows > 0 && (int64_t)ctx->paging.n_entries * ctx->paging.block_rows < kv_len)
         return ctx_fail(ctx, kInvalid, "the block table does not cover kv_len rows");
     int32_t rc = check_workspace(ctx, workspace, workspace_bytes,
-                                 epsp::weights_ws_bytes(kv_len, n_tok - row_begin, c.n_head, c.n_head_kv));
+                                 epsp::weights_ws_bytes(kv_len, n_tok - row_begin, c.n_head, c.n_head_kv, c.head_dim,
+                                                        c.dtype));
     if (rc) return rc;
     DeviceGuard guard;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

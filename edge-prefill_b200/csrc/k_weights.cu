@@ -1,109 +1,829 @@
 // k_weights.cu -- K7: softmax weights of a prompt's last rows over its cache.
 //
-// acc[h][j] = sum over the rows t and heads g of exp(x_tgj - lse_tg) with
-// x = q . k * scale: first each row's lse over the keys it sees, then each
-// key's sum over the rows that see it (one writer per key, fixed order).
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+//   acc[h][j] = sum over rows t and heads g of exp(x_tgj - lse_tg),  x = q . k * scale
+//
+// in two passes over the scores: the statistics pass leaves each query row's
+// (maximum, sum) per key split, k7_join its lse, the sums pass each key's sum.
+// Storing the scores instead would cost 8 bytes a pair; recomputing them costs
+// 2 d flops, which the tensor cores do in a quarter of the time the pair's two
+// exponentials take.  The exponentials bound both passes (16 MUFU results per
+// clock and SM).  Every key has one writer and a fixed order of additions.
+//
+// 16-bit (tcgen05): a query tile packs T = 128 / G tokens x G heads into 128
+// rows.  The two passes are one kernel with the MMA operands exchanged: with
+// queries as the M side a thread (TMEM lane) owns a query row and reduces over
+// keys; with keys as the M side it owns a key and reduces over queries.  Both
+// reductions stay in the thread's registers, no shuffles.  One warp loads
+// tiles by TMA, one issues MMAs into 4 S buffers in TMEM, and 8 warps take
+// the exponentials, each warpgroup 64 of a tile's 128 columns.
+// f32: the same passes on the CUDA cores, 64 x 64 tiles, 4 x 4 per thread.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
 
 #include "epsp_kernels.h"
+#include "tc100.cuh"
 
 namespace epsp {
 namespace {
 
-template <class T>
-__device__ __forceinline__ float to_f(T x) {
-    return static_cast<float>(x);
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-template <class T, int D>
-__device__ __forceinline__ float dot_row(const WeightArgs& a, const float* qs, int j, int h) {
-    bool bad = false;
-    const int row = phys_row(a.paging, j, bad);
-    if (bad) {
-        report_error(a.err, kDevBadBlockTable, 0x92, j);
-        return 0.f;
+// ---------------------------------------------------------- 16-bit: tcgen05 --
+constexpr int BM = 128;                 // rows of a query tile, keys of a key tile
+constexpr int kTcThreads = 384;         // producer, MMA, 2 idle warps, 2 x 4 softmax warps
+constexpr int kHalfTile = BM * 128;     // [128][64 x 16-bit], 128-byte swizzled
+constexpr int kMaxGroup = 4;            // query tiles a statistics CTA keeps on chip
+constexpr int kSBufs = 4;               // S tiles in TMEM (128 columns each)
+constexpr int kSms = 148;
+
+template <int D>
+struct TcLayout {
+    static constexpr int kTile = D / 64 * kHalfTile;
+    static constexpr int kSlots = D == 128 ? 6 : 12;  // query + key tiles on chip
+    static constexpr int kOffStat = kSlots * kTile;   // float2 [2][kMaxGroup * BM] (A) / float [2][2][BM] (B)
+    static constexpr int kOffBar = kOffStat + 2 * kMaxGroup * BM * 8;
+    static constexpr int kBars = 2 * 12 + 2 * 12 + 2 * kSBufs + 1;
+    static constexpr int kBytes = kOffBar + kBars * 8 + 32;
+    static_assert(kBytes + 1024 <= 232448, "shared memory");
+};
+
+struct WeightPlan {
+    int32_t T;         // tokens of a query tile (128 / G)
+    int32_t n_rt;      // query tiles of the window, per KV head
+    int32_t n_kt;      // key tiles
+    int32_t group;     // query tiles of a statistics CTA
+    int32_t n_groups;
+    int32_t splits;    // key splits of the statistics pass
+    int32_t resident;  // sums pass: every query tile stays on chip
+    int32_t q_slots, k_slots;  // sums pass
+    int32_t kg;        // sums pass: key tiles a CTA works on at a time (1, 2)
+    int32_t b_splits;  // sums pass: CTAs per KV head
+    float2* ml;        // [2 splits][Hkv][n_rt * 128]
+    float* lse;        // [Hkv][n_rt * 128], log2 units, +inf for rows that are none
+};
+
+// Barriers of a CTA.
+struct TcBars {
+    uint64_t *qf, *qe, *kf, *ke, *sf, *se, *done;
+    __device__ __forceinline__ explicit TcBars(unsigned char* p) {
+        uint64_t* b = reinterpret_cast<uint64_t*>(p);
+        qf = b, qe = b + 12, kf = b + 24, ke = b + 36, sf = b + 48, se = sf + kSBufs, done = se + kSBufs;
     }
-    const T* kr = static_cast<const T*>(a.k) + ((int64_t)row * a.n_head_kv + h) * D;
-    float x = 0.f;
-    for (int i = 0; i < D; ++i) x += qs[i] * to_f(kr[i]);
-    return x;
+};
+
+// Key tile kt of KV head h into `dst`, one page-sized segment at a time.
+template <int D, int SEG>
+__device__ __forceinline__ void load_keys(const WeightArgs& a, const CUtensorMap* tm, unsigned char* dst, uint64_t* bar,
+                                          int kt, int h) {
+    int rows[BM / SEG];
+#pragma unroll
+    for (int i = 0; i < BM / SEG; ++i) {
+        const int r = kt * BM + i * SEG;
+        rows[i] = r;
+        if (a.paging.block_rows > 0) {
+            rows[i] = a.paging.pool_rows;  // past the pool: zeros
+            if (r < a.kv_len) {
+                bool bad = false;
+                const int pr = phys_row(a.paging, r, bad);
+                if (bad) report_error(a.err, kDevBadBlockTable, 0x92, r);
+                else rows[i] = pr;
+            }
+        }
+    }
+    tc::mbar_arrive_expect_tx(bar, TcLayout<D>::kTile);
+#pragma unroll
+    for (int i = 0; i < BM / SEG; ++i)
+#pragma unroll
+        for (int hf = 0; hf < D / 64; ++hf)
+            tc::tma_load_3d(dst + hf * kHalfTile + i * SEG * 128, tm, bar, hf * 64, h, rows[i]);
 }
 
-// One CTA per (query head, row).
-template <class T, int D>
-__global__ void __launch_bounds__(128) k7_stats_plain(const WeightArgs a, float* lse) {
-    __shared__ float qs[D], rm[128], rl[128];
-    const int hq = blockIdx.x, w = blockIdx.y, t = threadIdx.x;
-    const int h = hq / (a.n_head / a.n_head_kv);
-    const T* q = static_cast<const T*>(a.q) + ((int64_t)(a.row_begin + w) * a.n_head + hq) * D;
-    for (int i = t; i < D; i += 128) qs[i] = to_f(q[i]) * a.kq_scale;
+template <int D>
+__device__ __forceinline__ void load_queries(const WeightArgs& a, const WeightPlan& p, const CUtensorMap* tm,
+                                             unsigned char* dst, uint64_t* bar, int rt, int h) {
+    const int G = a.n_head / a.n_head_kv;
+#pragma unroll
+    for (int hf = 0; hf < D / 64; ++hf)
+        tc::tma_load_3d(dst + hf * kHalfTile, tm, bar, hf * 64, h * G, a.row_begin + rt * p.T);
+}
+
+// S (columns of one TMEM buffer) = A B^T over D.
+template <bool BF16, int D>
+__device__ __forceinline__ void issue_s(uint32_t tmem, int buf, const unsigned char* a_tile, const unsigned char* b_tile) {
+    constexpr uint32_t idesc = tc::make_idesc_f16(BF16, BM, BM, false);
+    const uint64_t da = tc::make_sdesc_sw128(tc::smem_u32(a_tile), 16, 1024);
+    const uint64_t db = tc::make_sdesc_sw128(tc::smem_u32(b_tile), 16, 1024);
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+        const uint64_t off = (uint64_t)(((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4);
+        tc::mma_ss(tmem + buf * BM, da + off, db + off, idesc, kk > 0 ? 1u : 0u);
+    }
+}
+
+// 64 columns of S of this thread's lane; the buffer is handed back at once.
+__device__ __forceinline__ void take_s(uint32_t tmem, int buf, int wg, uint32_t lane_addr, uint64_t* se, int lane,
+                                       float (&s)[64]) {
+    uint32_t u[2][32];
+    tc::tmem_ld32(tmem + lane_addr + buf * BM + wg * 64, u[0]);
+    tc::tmem_ld32(tmem + lane_addr + buf * BM + wg * 64 + 32, u[1]);
+    tc::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(u[i >> 5][i & 31]);
+    tc::fence_before_sync();
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&se[buf]);
+}
+
+// PASS 0: statistics.  CTA (key split, group of query tiles, KV head): the
+// group's query tiles stay, key tiles stream; TMEM lane = query row, so each
+// thread keeps one row's maximum and sum over its half of a key tile's columns.
+// PASS 1: sums.  CTA (slice of key tiles, KV head): TMEM lane = key, columns =
+// query rows, so each thread sums one key's weights in registers; key tiles
+// (kg at a time) against all query tiles, which stay when they fit and
+// stream otherwise.
+template <bool BF16, int D, int SEG, int PASS>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k7_pass(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+            const __grid_constant__ WeightArgs a, const __grid_constant__ WeightPlan p) {
+    using LY = TcLayout<D>;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+    TcBars b(smem + LY::kOffBar);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + LY::kOffBar + LY::kBars * 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int Hkv = a.n_head_kv, G = a.n_head / Hkv;
+    const int t_first = a.kv_len - a.n_tok + a.row_begin;  // cache row of the window's first token
+    const uint64_t tmo = a.timeout_ns;
+
+    // the CTA's part
+    int h, rt0 = 0, n_q, k0, k1, q_slots, k_slots;
+    bool stream_q = false;
+    if constexpr (PASS == 0) {
+        const int sp = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
+        h = rest / p.n_groups;
+        // late groups first: they see the most keys
+        rt0 = (p.n_groups - 1 - rest % p.n_groups) * p.group;
+        n_q = min(p.group, p.n_rt - rt0);
+        const int last = min(t_first + (rt0 + n_q) * p.T, a.kv_len) - 1;
+        const int n_kt = last / BM + 1;
+        k0 = (int)((int64_t)n_kt * sp / p.splits);
+        k1 = (int)((int64_t)n_kt * (sp + 1) / p.splits);
+        q_slots = p.group;
+        k_slots = LY::kSlots - p.group;
+    } else {
+        h = blockIdx.x / p.b_splits;
+        n_q = p.n_rt;
+        k0 = blockIdx.x % p.b_splits;  // groups of kg key tiles: k0, k0 + b_splits, ...
+        k1 = (p.n_kt + p.kg - 1) / p.kg;
+        q_slots = p.q_slots;
+        k_slots = p.k_slots;
+        stream_q = !p.resident;
+    }
+    unsigned char* kbase = smem + q_slots * LY::kTile;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < q_slots; ++i) {
+            tc::mbar_init(&b.qf[i], 1);
+            tc::mbar_init(&b.qe[i], 1);
+        }
+        for (int i = 0; i < k_slots; ++i) {
+            tc::mbar_init(&b.kf[i], 1);
+            tc::mbar_init(&b.ke[i], 1);
+        }
+        for (int i = 0; i < kSBufs; ++i) {
+            tc::mbar_init(&b.sf[i], 1);
+            tc::mbar_init(&b.se[i], 8);
+        }
+        tc::mbar_init(b.done, 1);
+        tc::fence_mbar_init();
+        tc::tma_prefetch_desc(&tmQ);
+        tc::tma_prefetch_desc(&tmK);
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(tmem_slot, kSBufs * BM);
+        tc::tmem_relinquish();
+    }
+    // Query rows past T * G are never written by TMA: zeros, so that no stale
+    // shared memory reaches the tensor cores.
+    if (const int used = p.T * G; used < BM) {
+        const int n16 = (BM - used) * 8;
+        for (int i = threadIdx.x; i < n16 * q_slots * (D / 64); i += kTcThreads)
+            *(reinterpret_cast<uint4*>(smem + (i / n16) * kHalfTile + used * 128) + i % n16) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    tc::fence_before_sync();
     __syncthreads();
-    const int n = a.kv_len - a.n_tok + a.row_begin + w + 1;
+    tc::fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const int q_bytes = D / 64 * 64 * 2 * p.T * G;
+
+    // first query tile that sees any key of group kgi (sums pass)
+    auto rt_from = [&](int kgi) { return max(0, (kgi * p.kg * BM - t_first) / p.T); };
+
+    if (warp == 0) {
+        // ------------------------------------------------------ producer --
+        if (lane == 0) {
+            bool ok = true;
+            int kt_n = 0, qt_n = 0;  // tiles issued into each ring
+            auto keys = [&](int kt) {
+                const int s = kt_n % k_slots;
+                ok = tc::mbar_wait(&b.ke[s], ((kt_n / k_slots) & 1) ^ 1, tmo);
+                if (!ok) return;
+                load_keys<D, SEG>(a, &tmK, kbase + s * LY::kTile, &b.kf[s], kt, h);
+                ++kt_n;
+            };
+            if (!stream_q) {
+                tc::mbar_arrive_expect_tx(&b.qf[0], q_bytes * n_q);
+                for (int i = 0; i < n_q; ++i)
+                    load_queries<D>(a, p, &tmQ, smem + i * LY::kTile, &b.qf[0], rt0 + i, h);
+            }
+            if constexpr (PASS == 0) {
+                for (int kt = k0; kt < k1 && ok; ++kt) keys(kt);
+            } else {
+                for (int g = k0; g < k1 && ok; g += p.b_splits) {
+                    const int r0 = rt_from(g);
+                    if (r0 >= n_q) continue;
+                    for (int k = 0; k < p.kg && g * p.kg + k < p.n_kt && ok; ++k) keys(g * p.kg + k);
+                    for (int rt = r0; rt < n_q && ok && stream_q; ++rt) {
+                        const int s = qt_n % q_slots;
+                        ok = tc::mbar_wait(&b.qe[s], ((qt_n / q_slots) & 1) ^ 1, tmo);
+                        if (!ok) break;
+                        tc::mbar_arrive_expect_tx(&b.qf[s], q_bytes);
+                        load_queries<D>(a, p, &tmQ, smem + s * LY::kTile, &b.qf[s], rt, h);
+                        ++qt_n;
+                    }
+                }
+            }
+            if (!ok) report_error(a.err, kDevWaitWeights, 0xb0 + PASS, kt_n);
+            // copies still in flight land before the CTA ends
+            for (int j = max(0, kt_n - k_slots); j < kt_n; ++j)
+                tc::mbar_wait(&b.kf[j % k_slots], (j / k_slots) & 1, tmo);
+            if (!stream_q) tc::mbar_wait(&b.qf[0], 0, tmo);
+            for (int j = max(0, qt_n - q_slots); j < qt_n; ++j)
+                tc::mbar_wait(&b.qf[j % q_slots], (j / q_slots) & 1, tmo);
+        }
+    } else if (warp == 1) {
+        // ----------------------------------------------------------- MMA --
+        const bool leader = tc::elect_one();
+        bool ok = true;
+        int step = 0, kt_n = 0, qt_n = 0;
+        auto wait = [&](uint64_t* bar, uint32_t par) {
+            if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(bar, par, tmo));
+            return ok;
+        };
+        auto commit = [&](uint64_t* bar) {
+            if (leader) tc::mma_commit(bar);
+            __syncwarp();
+        };
+        auto one = [&](const unsigned char* q, const unsigned char* k) {
+            const int buf = step % kSBufs;
+            if (!wait(&b.se[buf], ((step / kSBufs) & 1) ^ 1)) return;
+            tc::fence_after_sync();
+            if (leader) issue_s<BF16, D>(tmem, buf, PASS == 0 ? q : k, PASS == 0 ? k : q);
+            __syncwarp();
+            commit(&b.sf[buf]);
+            ++step;
+        };
+        if (!stream_q) wait(&b.qf[0], 0);
+        if constexpr (PASS == 0) {
+            for (int kt = k0; kt < k1 && ok; ++kt, ++kt_n) {
+                const int s = kt_n % k_slots;
+                wait(&b.kf[s], (kt_n / k_slots) & 1);
+                for (int r = 0; r < n_q && ok; ++r) one(smem + r * LY::kTile, kbase + s * LY::kTile);
+                if (ok) commit(&b.ke[s]);
+            }
+        } else {
+            for (int g = k0; g < k1 && ok; g += p.b_splits) {
+                const int r0 = rt_from(g);
+                if (r0 >= n_q) continue;
+                const int nk = min(p.kg, p.n_kt - g * p.kg);
+                for (int rt = r0; rt < n_q && ok; ++rt) {
+                    const int qs = stream_q ? qt_n % q_slots : rt;
+                    if (stream_q) wait(&b.qf[qs], (qt_n / q_slots) & 1);
+                    for (int k = 0; k < nk && ok; ++k) {
+                        const int s = (kt_n + k) % k_slots;
+                        if (rt == r0) wait(&b.kf[s], ((kt_n + k) / k_slots) & 1);
+                        if (ok) one(smem + qs * LY::kTile, kbase + s * LY::kTile);
+                    }
+                    if (stream_q && ok) commit(&b.qe[qs]);
+                    ++qt_n;
+                }
+                for (int k = 0; k < nk && ok; ++k) commit(&b.ke[(kt_n + k) % k_slots]);
+                kt_n += nk;
+            }
+        }
+        if (!ok && lane == 0) report_error(a.err, kDevWaitWeights, 0xb2 + PASS, step);
+        // every MMA retires before TMEM is freed
+        commit(b.done);
+        tc::mbar_wait(b.done, 0, tmo);
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ------------------------------------------------------- softmax --
+        const int wg = (warp - 4) >> 2, wq = warp & 3, row = wq * 32 + lane;
+        const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
+        const float sl2 = a.kq_scale * 1.4426950408889634f;
+        const float2 sl2_2 = make_float2(sl2, sl2);
+        bool ok = true;
+        int step = 0;
+        auto next = [&]() {  // the buffer of the next step, once it is full
+            const int buf = step % kSBufs;
+            if (ok) {
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(&b.sf[buf], (step / kSBufs) & 1, tmo));
+                if (!ok && lane == 0) report_error(a.err, kDevWaitWeights, 0xb4 + PASS, step);
+                tc::fence_after_sync();
+            }
+            ++step;
+            return buf;
+        };
+        if constexpr (PASS == 0) {
+            float2* stat = reinterpret_cast<float2*>(smem + LY::kOffStat) + wg * kMaxGroup * BM + row;
+            for (int r = 0; r < n_q; ++r) stat[r * BM] = make_float2(-INFINITY, 0.f);
+            for (int kt = k0; kt < k1 && ok; ++kt) {
+                for (int r = 0; r < n_q && ok; ++r) {
+                    const int buf = next();
+                    if (!ok) break;
+                    float s[64];
+                    take_s(tmem, buf, wg, lane_addr, b.se, lane, s);
+                    const int tt = t_first + (rt0 + r) * p.T, key = kt * BM + wg * 64;
+                    if (key + 63 > tt) {
+                        const int lim = tt + row / G - key;
+#pragma unroll
+                        for (int c = 0; c < 64; ++c)
+                            if (c > lim) s[c] = -INFINITY;
+                    }
+                    float mx[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mx[i] = fmaxf(s[i], s[i + 4]);
+#pragma unroll
+                        for (int c = 8 + i; c < 64; c += 4) mx[i] = fmaxf(mx[i], s[c]);
+                    }
+                    const float2 st = stat[r * BM];
+                    const float m = fmaxf(st.x, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
+                    const float ms = m == -INFINITY ? 0.f : m;
+                    const float2 nm = make_float2(-ms, -ms);
+                    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        const float2 x = __ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2_2, nm);
+                        acc[c & 1] = __fadd2_rn(acc[c & 1], make_float2(ex2(x.x), ex2(x.y)));
+                    }
+                    const float2 t = __fadd2_rn(acc[0], acc[1]);
+                    stat[r * BM] = make_float2(m, st.y * ex2(st.x - ms) + (t.x + t.y));
+                }
+            }
+            const int sp = blockIdx.x % p.splits;
+            float2* out = p.ml + ((int64_t)(sp * 2 + wg) * Hkv + h) * p.n_rt * BM + rt0 * BM + row;
+            for (int r = 0; r < n_q; ++r) out[r * BM] = stat[r * BM];
+        } else {
+            float* red = reinterpret_cast<float*>(smem + LY::kOffStat);  // [2][2][BM]
+            const float* lse = p.lse + (int64_t)h * p.n_rt * BM;
+            int turn = 0;
+            for (int g = k0; g < k1; g += p.b_splits) {
+                const int r0 = rt_from(g), nk = min(p.kg, p.n_kt - g * p.kg);
+                float sum[2] = {0.f, 0.f};
+                for (int rt = r0; rt < n_q && ok; ++rt) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        if (k >= nk) break;
+                        const int buf = next();
+                        if (!ok) break;
+                        float s[64];
+                        take_s(tmem, buf, wg, lane_addr, b.se, lane, s);
+                        const float4* l4 = reinterpret_cast<const float4*>(lse + rt * BM + wg * 64);
+                        const int key0 = (g * p.kg + k) * BM, tt = t_first + rt * p.T;
+                        if (key0 + BM - 1 > tt) {
+                            // some of these rows come before some of these keys
+                            int tok = tt + wg * 64 / G, rem = wg * 64 % G;
+#pragma unroll
+                            for (int c = 0; c < 64; ++c) {
+                                if (key0 + row > tok) s[c] = -INFINITY;
+                                if (++rem == G) rem = 0, ++tok;
+                            }
+                        }
+                        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            const float4 l = l4[c];
+                            const float2 x = __ffma2_rn(make_float2(s[4 * c], s[4 * c + 1]), sl2_2, make_float2(-l.x, -l.y));
+                            const float2 y =
+                                __ffma2_rn(make_float2(s[4 * c + 2], s[4 * c + 3]), sl2_2, make_float2(-l.z, -l.w));
+                            acc[0] = __fadd2_rn(acc[0], make_float2(ex2(x.x), ex2(x.y)));
+                            acc[1] = __fadd2_rn(acc[1], make_float2(ex2(y.x), ex2(y.y)));
+                        }
+                        const float2 t = __fadd2_rn(acc[0], acc[1]);
+                        sum[k] += t.x + t.y;
+                    }
+                }
+                // the two warpgroups' halves of the query rows
+                if (wg == 1) {
+                    red[(turn * 2 + 0) * BM + row] = sum[0];
+                    red[(turn * 2 + 1) * BM + row] = sum[1];
+                }
+                tc::named_bar_sync(1, 256);
+                if (wg == 0 && ok) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int key = (g * p.kg + k) * BM + row;
+                        if (k >= nk || key >= a.kv_len) continue;
+                        const float v = sum[k] + red[(turn * 2 + k) * BM + row];
+                        float* out = a.acc + (int64_t)h * a.acc_stride + key;
+                        *out = a.accumulate ? *out + v : v;
+                    }
+                }
+                turn ^= 1;
+            }
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, kSBufs * BM);
+    }
+}
+
+// The rows' log-sum-exp from the splits' statistics.
+__global__ void k7_join(const WeightArgs a, const WeightPlan p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int n = p.n_rt * BM, G = a.n_head / a.n_head_kv;
+    const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, stride = (int64_t)n * a.n_head_kv;
+    if (at >= stride) return;
+    const int i = (int)(at % n), r = i % BM;
+    const bool there = r < p.T * G && i / BM * p.T + r / G < a.n_tok - a.row_begin;
     float m = -INFINITY, l = 0.f;
-    for (int j = t; j < n; j += 128) {
-        const float x = dot_row<T, D>(a, qs, j, h), m2 = fmaxf(m, x);
-        const float ms = m2 == -INFINITY ? 0.f : m2;
-        l = l * expf(m - ms) + expf(x - ms);
-        m = m2;
+    for (int s = 0; there && s < 2 * p.splits; ++s) m = fmaxf(m, p.ml[s * stride + at].x);
+    const float ms = m == -INFINITY ? 0.f : m;
+    for (int s = 0; there && s < 2 * p.splits; ++s) {
+        const float2 v = p.ml[s * stride + at];
+        l += v.y * ex2(v.x - ms);
     }
-    rm[t] = m;
-    rl[t] = l;
-    __syncthreads();
-    for (int k = 64; k > 0; k >>= 1) {
-        if (t < k) {
-            const float m2 = fmaxf(rm[t], rm[t + k]), ms = m2 == -INFINITY ? 0.f : m2;
-            rl[t] = rl[t] * expf(rm[t] - ms) + rl[t + k] * expf(rm[t + k] - ms);
-            rm[t] = m2;
+    p.lse[at] = there ? ms + log2f(l) : INFINITY;
+}
+
+// ------------------------------------------------------------ f32: CUDA cores --
+constexpr int FT = 64;          // query rows, and keys, of a tile
+constexpr int kF32Threads = 256;  // 16 x 16 threads, 4 rows x 4 keys each
+
+struct F32Plan {
+    int64_t n_rows;  // (token, head) rows of the window per KV head
+    int32_t n_rt, n_kt, splits;
+    float2* ml;      // [splits][Hkv][n_rt * 64]
+    float* lse;      // [Hkv][n_rt * 64], +inf for rows that are none
+};
+
+// 64 rows of `D` floats into shared memory, rows padded by 16 bytes (the 4 x 4
+// product reads 8 rows at once without a bank conflict).  src(r): the row's
+// address, null for zeros.
+template <int D, class F>
+__device__ __forceinline__ void load_rows_f32(float* dst, F&& src) {
+    for (int i = threadIdx.x; i < FT * (D / 4); i += kF32Threads) {
+        const int r = i / (D / 4), c = i % (D / 4);
+        const float* p = src(r);
+        *reinterpret_cast<float4*>(dst + r * (D + 4) + c * 4) =
+            p != nullptr ? *reinterpret_cast<const float4*>(p + c * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void load_queries_f32(const WeightArgs& a, const F32Plan& p, float* dst, int rt, int h) {
+    const int G = a.n_head / a.n_head_kv;
+    load_rows_f32<D>(dst, [&](int r) -> const float* {
+        const int64_t i = (int64_t)rt * FT + r;
+        if (i >= p.n_rows) return nullptr;
+        return static_cast<const float*>(a.q) + ((a.row_begin + i / G) * a.n_head + (int64_t)h * G + i % G) * D;
+    });
+}
+
+template <int D>
+__device__ __forceinline__ void load_keys_f32(const WeightArgs& a, float* dst, int kt, int h) {
+    load_rows_f32<D>(dst, [&](int r) -> const float* {
+        const int j = kt * FT + r;
+        if (j >= a.kv_len) return nullptr;
+        bool bad = false;
+        const int row = phys_row(a.paging, j, bad);
+        if (bad) {
+            report_error(a.err, kDevBadBlockTable, 0x92, j);
+            return nullptr;
         }
+        return static_cast<const float*>(a.k) + ((int64_t)row * a.n_head_kv + h) * D;
+    });
+}
+
+// x[i][j] = q row (ty + 16 i) . k row (tx + 16 j)
+template <int D>
+__device__ __forceinline__ void scores_f32(const float* q, const float* k, int ty, int tx, float (&x)[4][4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][j] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < D; c += 4) {
+        float4 qq[4], kk[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            qq[i] = *reinterpret_cast<const float4*>(q + (ty + 16 * i) * (D + 4) + c);
+            kk[i] = *reinterpret_cast<const float4*>(k + (tx + 16 * i) * (D + 4) + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[i][j] = fmaf(qq[i].x, kk[j].x, x[i][j]);
+                x[i][j] = fmaf(qq[i].y, kk[j].y, x[i][j]);
+                x[i][j] = fmaf(qq[i].z, kk[j].z, x[i][j]);
+                x[i][j] = fmaf(qq[i].w, kk[j].w, x[i][j]);
+            }
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, const F32Plan p) {
+    extern __shared__ __align__(16) float sm[];
+    float *q = sm, *k = sm + FT * (D + 4);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int sp = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
+    const int rt = p.n_rt - 1 - rest % p.n_rt, h = rest / p.n_rt;  // late rows first: they see the most keys
+    const int G = a.n_head / a.n_head_kv, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int t_first = a.kv_len - a.n_tok + a.row_begin;
+    const float sl2 = a.kq_scale * 1.4426950408889634f;
+    const int64_t last_row = min((int64_t)rt * FT + FT, p.n_rows) - 1;
+    const int n_kt = (int)((t_first + last_row / G) / FT) + 1;
+    const int k0 = (int)((int64_t)n_kt * sp / p.splits), k1 = (int)((int64_t)n_kt * (sp + 1) / p.splits);
+    int tok[4];
+    float m[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        tok[i] = t_first + (int)(((int64_t)rt * FT + ty + 16 * i) / G);
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+    }
+    load_queries_f32<D>(a, p, q, rt, h);
+    for (int kt = k0; kt < k1; ++kt) {
         __syncthreads();
-    }
-    if (t == 0) lse[(int64_t)w * a.n_head + hq] = rm[0] + logf(rl[0]);
-}
-
-// One thread per key of one KV head.
-template <class T, int D>
-__global__ void __launch_bounds__(128) k7_sums_plain(const WeightArgs a, const float* lse) {
-    __shared__ float qs[D];
-    const int h = blockIdx.y, j = blockIdx.x * 128 + threadIdx.x, G = a.n_head / a.n_head_kv;
-    const int first = max(0, (int)(blockIdx.x * 128) - (a.kv_len - a.n_tok + a.row_begin));  // first row that sees the tile
-    float sum = 0.f;
-    for (int w = first; w < a.n_tok - a.row_begin; ++w)
-        for (int g = 0; g < G; ++g) {
-            const int hq = h * G + g;
-            __syncthreads();
-            for (int i = threadIdx.x; i < D; i += 128)
-                qs[i] = to_f(static_cast<const T*>(a.q)[((int64_t)(a.row_begin + w) * a.n_head + hq) * D + i]) * a.kq_scale;
-            __syncthreads();
-            if (j <= a.kv_len - a.n_tok + a.row_begin + w)
-                sum += expf(dot_row<T, D>(a, qs, j, h) - lse[(int64_t)w * a.n_head + hq]);
+        load_keys_f32<D>(a, k, kt, h);
+        __syncthreads();
+        float x[4][4];
+        scores_f32<D>(q, k, ty, tx, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float mx = m[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[i][j] = kt * FT + tx + 16 * j <= tok[i] ? x[i][j] * sl2 : -INFINITY;
+                mx = fmaxf(mx, x[i][j]);
+            }
+            const float ms = mx == -INFINITY ? 0.f : mx;
+            l[i] *= ex2(m[i] - ms);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l[i] += ex2(x[i][j] - ms);
+            m[i] = mx;
         }
-    if (j < a.kv_len) {
-        float* p = a.acc + (int64_t)h * a.acc_stride + j;
-        *p = a.accumulate ? *p + sum : sum;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m[i], d), l2 = __shfl_xor_sync(0xffffffffu, l[i], d);
+            const float mx = fmaxf(m[i], m2), ms = mx == -INFINITY ? 0.f : mx;
+            l[i] = l[i] * ex2(m[i] - ms) + l2 * ex2(m2 - ms);
+            m[i] = mx;
+        }
+        if (tx == 0)
+            p.ml[((int64_t)sp * a.n_head_kv + h) * p.n_rt * FT + (int64_t)rt * FT + ty + 16 * i] =
+                make_float2(m[i], l[i]);
     }
 }
 
-template <class T, int D>
-cudaError_t go(const WeightArgs& a, cudaStream_t s) {
-    float* lse = static_cast<float*>(a.ws);
-    const int rows = a.n_tok - a.row_begin;
-    if (rows > 65535) return cudaErrorNotSupported;
-    k7_stats_plain<T, D><<<dim3(a.n_head, rows), 128, 0, s>>>(a, lse);
-    k7_sums_plain<T, D><<<dim3((a.kv_len + 127) / 128, a.n_head_kv), 128, 0, s>>>(a, lse);
-    return cudaGetLastError();
+__global__ void k7_join_f32(const WeightArgs a, const F32Plan p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int64_t n = (int64_t)p.n_rt * FT, at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (at >= n * a.n_head_kv) return;
+    const int64_t stride = n * a.n_head_kv;
+    const bool there = at % n < p.n_rows;
+    float m = -INFINITY, l = 0.f;
+    for (int s = 0; there && s < p.splits; ++s) m = fmaxf(m, p.ml[s * stride + at].x);
+    const float ms = m == -INFINITY ? 0.f : m;
+    for (int s = 0; there && s < p.splits; ++s) l += p.ml[s * stride + at].y * ex2(p.ml[s * stride + at].x - ms);
+    p.lse[at] = there ? ms + log2f(l) : INFINITY;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, const F32Plan p) {
+    extern __shared__ __align__(16) float sm[];
+    float *q = sm, *k = sm + FT * (D + 4);
+    const int kt = blockIdx.x % p.n_kt, h = blockIdx.x / p.n_kt;
+    const int G = a.n_head / a.n_head_kv, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int t_first = a.kv_len - a.n_tok + a.row_begin;
+    const float sl2 = a.kq_scale * 1.4426950408889634f;
+    load_keys_f32<D>(a, k, kt, h);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const float* lse = p.lse + (int64_t)h * p.n_rt * FT;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const int r0 = max(0, (int)((int64_t)(kt * FT - t_first) * G / FT));  // first tile with a row that sees the keys
+    for (int rt = r0; rt < p.n_rt; ++rt) {
+        __syncthreads();
+        load_queries_f32<D>(a, p, q, rt, h);
+        __syncthreads();
+        float x[4][4];
+        scores_f32<D>(q, k, ty, tx, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = (int64_t)rt * FT + ty + 16 * i;
+            const int tok = t_first + (int)(r / G);
+            const float ls = lse[r];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (kt * FT + tx + 16 * j <= tok) sum[j] += ex2(fmaf(x[i][j], sl2, -ls));
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[ty * FT + tx + 16 * j] = sum[j];
+    __syncthreads();
+    if (threadIdx.x < FT && kt * FT + (int)threadIdx.x < a.kv_len) {
+        float v = 0.f;
+        for (int i = 0; i < 16; ++i) v += q[i * FT + threadIdx.x];
+        float* out = a.acc + (int64_t)h * a.acc_stride + kt * FT + threadIdx.x;
+        *out = a.accumulate ? *out + v : v;
+    }
+}
+
+// ---------------------------------------------------------------- host side --
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+size_t plan_f32(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, char* ws, F32Plan* p) {
+    p->n_rows = (int64_t)rows * (n_head / n_head_kv);
+    p->n_rt = (int32_t)((p->n_rows + FT - 1) / FT);
+    p->n_kt = (kv_len + FT - 1) / FT;
+    // three CTAs fit an SM: split the keys until the device is full
+    const int64_t ctas = (int64_t)n_head_kv * p->n_rt;
+    p->splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_kt, 3 * kSms / ctas));
+    const size_t n = (size_t)n_head_kv * p->n_rt * FT, ml = up16(n * p->splits * sizeof(float2));
+    p->ml = reinterpret_cast<float2*>(ws);
+    p->lse = reinterpret_cast<float*>(ws + ml);
+    return ml + up16(n * sizeof(float));
+}
+
+size_t plan_tc(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, int32_t d, char* ws, WeightPlan* p) {
+    const int slots = d == 128 ? TcLayout<128>::kSlots : TcLayout<64>::kSlots;
+    p->T = BM / (n_head / n_head_kv);
+    p->n_rt = (rows + p->T - 1) / p->T;
+    p->n_kt = (kv_len + BM - 1) / BM;
+    p->n_groups = (p->n_rt + kMaxGroup - 1) / kMaxGroup;
+    p->group = (p->n_rt + p->n_groups - 1) / p->n_groups;
+    p->n_groups = (p->n_rt + p->group - 1) / p->group;
+    p->splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_kt, kSms / ((int64_t)n_head_kv * p->n_groups)));
+    // sums pass: query tiles that leave two slots for keys stay on chip, more
+    // of them stream; then two key tiles share each query tile's load once
+    // there are enough key tiles to fill the device that way
+    p->resident = p->n_rt <= slots - 2;
+    p->q_slots = p->resident ? p->n_rt : slots / 2;
+    p->k_slots = slots - p->q_slots;
+    p->kg = !p->resident && (int64_t)n_head_kv * p->n_kt >= 2 * kSms ? 2 : 1;
+    const int n_kg = (p->n_kt + p->kg - 1) / p->kg;
+    p->b_splits = std::max(1, std::min(n_kg, kSms / n_head_kv));
+    const size_t n = (size_t)n_head_kv * p->n_rt * BM, ml = up16(n * 2 * p->splits * sizeof(float2));
+    p->ml = reinterpret_cast<float2*>(ws);
+    p->lse = reinterpret_cast<float*>(ws + ml);
+    return ml + up16(n * sizeof(float));
+}
+
+template <class... P, class... A>
+cudaError_t launch_after(void (*k)(P...), int64_t grid, int threads, int smem, cudaStream_t s, const A&... args) {
+    if (grid < 1 || grid > INT_MAX) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
+// Dynamic shared memory of a kernel, set once per device (`mask`: a bit per
+// device ordinal < 32).
+cudaError_t allow_smem(const void* f, int bytes, std::atomic<unsigned>& mask) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 32 && (mask.load(std::memory_order_acquire) & (1u << dev))) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 32) mask.fetch_or(1u << dev, std::memory_order_release);
+    return e;
+}
+
+template <int D>
+cudaError_t launch_f32(const WeightArgs& a, cudaStream_t s) {
+    F32Plan p{};
+    plan_f32(a.kv_len, a.n_tok - a.row_begin, a.n_head, a.n_head_kv, static_cast<char*>(a.ws), &p);
+    const int smem = 2 * FT * (D + 4) * (int)sizeof(float);
+    static std::atomic<unsigned> m0{0}, m1{0};
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(&k7_stats_f32<D>), smem, m0);
+    if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_sums_f32<D>), smem, m1);
+    if (e != cudaSuccess) return e;
+    const int64_t ctas = (int64_t)a.n_head_kv * p.n_rt * p.splits, rows = (int64_t)a.n_head_kv * p.n_rt * FT;
+    if (ctas > INT_MAX) return cudaErrorInvalidValue;
+    k7_stats_f32<D><<<(unsigned)ctas, kF32Threads, smem, s>>>(a, p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    e = launch_after(k7_join_f32, (rows + 255) / 256, 256, 0, s, a, p);
+    if (e != cudaSuccess) return e;
+    return launch_after(k7_sums_f32<D>, (int64_t)a.n_head_kv * p.n_kt, kF32Threads, smem, s, a, p);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> fn{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 f = fn.load(std::memory_order_acquire);
+    if (!f) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+        fn.store(f, std::memory_order_release);
+    }
+    return f;
+}
+
+// [rows][heads][d] 16-bit elements in boxes of box_rows x box_heads x 64.
+bool make_map(CUtensorMap* m, const void* base, bool bf16, int d, int heads, int rows, int box_heads, int box_rows) {
+    auto enc = get_encode();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)d * 2 * heads};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+               dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF16, int D, int SEG>
+cudaError_t launch_tc(const WeightArgs& a, cudaStream_t s) {
+    WeightPlan p{};
+    plan_tc(a.kv_len, a.n_tok - a.row_begin, a.n_head, a.n_head_kv, D, static_cast<char*>(a.ws), &p);
+    CUtensorMap mq, mk;
+    const int rows = a.paging.block_rows > 0 ? a.paging.pool_rows : a.kv_len;
+    if (!make_map(&mq, a.q, BF16, D, a.n_head, a.n_tok, a.n_head / a.n_head_kv, p.T) ||
+        !make_map(&mk, a.k, BF16, D, a.n_head_kv, rows, 1, SEG))
+        return cudaErrorInvalidValue;
+    const int smem = TcLayout<D>::kBytes + 1024;
+    static std::atomic<unsigned> m0{0}, m1{0};
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 0>), smem, m0);
+    if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 1>), smem, m1);
+    if (e != cudaSuccess) return e;
+    const int64_t ctas = (int64_t)a.n_head_kv * p.n_groups * p.splits, n = (int64_t)p.n_rt * BM;
+    if (ctas > INT_MAX || n > INT_MAX) return cudaErrorInvalidValue;
+    k7_pass<BF16, D, SEG, 0><<<(unsigned)ctas, kTcThreads, smem, s>>>(mq, mk, a, p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    e = launch_after(k7_join, (n * a.n_head_kv + 255) / 256, 256, 0, s, a, p);
+    if (e != cudaSuccess) return e;
+    return launch_after(k7_pass<BF16, D, SEG, 1>, (int64_t)a.n_head_kv * p.b_splits, kTcThreads, smem, s, mq, mk, a, p);
+}
+
+template <bool BF16, int D>
+cudaError_t launch_seg(const WeightArgs& a, cudaStream_t s) {
+    switch (a.page_size) {
+        case 32: return launch_tc<BF16, D, 32>(a, s);
+        case 64: return launch_tc<BF16, D, 64>(a, s);
+        default: return launch_tc<BF16, D, 128>(a, s);
+    }
 }
 
 }  // namespace
 
-size_t weights_ws_bytes(int32_t, int32_t rows, int32_t n_head, int32_t) { return (size_t)rows * n_head * sizeof(float); }
+size_t weights_ws_bytes(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                        int32_t dtype) {
+    if (dtype == 0) {
+        F32Plan p{};
+        return plan_f32(kv_len, rows, n_head, n_head_kv, nullptr, &p);
+    }
+    WeightPlan p{};
+    return plan_tc(kv_len, rows, n_head, n_head_kv, head_dim, nullptr, &p);
+}
 
 cudaError_t launch_prompt_weights(const WeightArgs& a, cudaStream_t s) {
     const bool wide = a.head_dim == 128;
     switch (a.dtype) {
-        case 0: return wide ? go<float, 128>(a, s) : go<float, 64>(a, s);
-        case 1: return wide ? go<__half, 128>(a, s) : go<__half, 64>(a, s);
-        default: return wide ? go<__nv_bfloat16, 128>(a, s) : go<__nv_bfloat16, 64>(a, s);
+        case 0: return wide ? launch_f32<128>(a, s) : launch_f32<64>(a, s);
+        case 1: return wide ? launch_seg<false, 128>(a, s) : launch_seg<false, 64>(a, s);
+        default: return wide ? launch_seg<true, 128>(a, s) : launch_seg<true, 64>(a, s);
     }
 }
 
