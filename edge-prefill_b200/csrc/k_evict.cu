@@ -1,15 +1,37 @@
 // k_evict.cu -- K8: eviction by accumulated weight.
 //
-// K8a picks, per sequence and KV head, the rows to keep: a radix selection
-// finds the weight of the last row that stays (32-bit order-preserving keys,
-// most significant digit first), then one pass in row order lists the rows
-// above it and the first of those equal to it.  K8b moves the listed rows.
+// K8a picks, per sequence and KV head, the rows to keep.  A radix selection
+// over 32-bit order-preserving keys (digits of 11, 11 and 10 bits, most
+// significant first) finds the weight of the last row that stays; then every
+// row above it, and the first of those equal to it, get their place by a
+// prefix sum in row order.  The rows of one head are split over a cluster of
+// up to 8 CTAs, which keep their slice of the weights in shared memory (one
+// read of the weights) and add their histograms through distributed shared
+// memory; only counts are exchanged, so the result is exact and has no order.
+// Latency bounds it: three histogram rounds, each with one cluster barrier.
+//
+// K8b moves the listed rows, which the bytes bound: a warp takes 32 rows, K in
+// its lower half's lanes and V in the upper's.  In place there is an order to
+// keep (a row may only be written once every row read from it has been), and
+// K8c gives each CTA a 32-byte column of one head, which it compacts from the
+// first row to the last: a kept row never moves up, so a step's loads need
+// only be done before its own stores.
+#include <cooperative_groups.h>
+
+#include <atomic>
+
 #include "epsp_kernels.h"
 
 namespace epsp {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 1024;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kMaxCluster = 8;
+constexpr int kCacheRows = 32768;  // weights a CTA keeps in shared memory (128 KB)
 
 // Order-preserving key of a weight: larger weight, larger key; NaN as -inf;
 // +0 and -0 alike.
@@ -20,64 +42,95 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-struct Plan {  // per sequence, in the workspace
-    int32_t n, m;
+struct EvictPlan {
+    int32_t* kept;  // [n_seq] rows kept
+    int32_t* list;  // [n_seq][Hkv][cap] kept rows, ascending
+    int32_t cap;
+    int32_t cluster;
+    int32_t cached;  // the slices fit in shared memory
 };
 
-// Inclusive sum over the CTA's threads.
-__device__ int scan_cta(int x, int* warp_sums, int& total) {
+// Inclusive sum over the CTA's threads (two 32-bit counts in one word).
+__device__ __forceinline__ uint64_t scan_cta(uint64_t x, uint64_t* warp_sums, uint64_t& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int v = x;
+#pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= d) v += u;
+        const uint64_t u = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += u;
     }
-    if (lane == 31) warp_sums[warp] = v;
+    if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
     if (warp == 0) {
-        int w = warp_sums[lane];
+        uint64_t w = warp_sums[lane];
+#pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, w, d);
+            const uint64_t u = __shfl_up_sync(0xffffffffu, w, d);
             if (lane >= d) w += u;
         }
         warp_sums[lane] = w;
     }
     __syncthreads();
-    if (warp > 0) v += warp_sums[warp - 1];
+    if (warp > 0) x += warp_sums[warp - 1];
     total = warp_sums[31];
     __syncthreads();
-    return v;
+    return x;
 }
 
-__global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, int32_t* list, Plan* plan, int cap) {
-    __shared__ int hist[256], warp_sums[32];
+__global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, const EvictPlan p) {
+    extern __shared__ float cache[];  // this CTA's weights
+    __shared__ int hist[3][kBins];
+    __shared__ uint64_t warp_sums[32], counts[kThreads], mine;
     __shared__ int s_digit, s_above;
-    const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
+    cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int C = p.cluster, rank = blockIdx.x % C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int h = blockIdx.x / C % a.n_head_kv, s = blockIdx.x / C / a.n_head_kv;
     const int n = batch_len(a.src, s, a.err), m = min(n, a.n_keep);
     const int64_t sh = (int64_t)s * a.n_head_kv + h;
     const float* acc = a.acc + sh * a.acc_stride;
-    int32_t* out = list + sh * cap;
-    if (h == 0 && t == 0) plan[s] = {n, m};
-    // the candidates are rows [lo, hi); `want` of them stay
+    if (h == 0 && rank == 0 && t == 0) p.kept[s] = m;
+    // rows [r0, r1) are this CTA's; [lo, hi) the candidates, of which `want` stay
+    const int per = ((n + C - 1) / C + 31) & ~31;
+    const int r0 = min(n, rank * per), r1 = min(n, r0 + per);
     const int lo = n > m ? a.sink_rows : n, hi = n > m ? n - a.recent_rows : n;
     const int want = n > m ? m - a.sink_rows - a.recent_rows : 0;
+    const bool ranked = want > 0;  // else no candidate stays (or there is none)
+
+    for (int i = t; i < 3 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
+    if (p.cached)
+        for (int r = r0 + t; r < r1; r += kThreads) cache[r - r0] = acc[r];
+    auto weight = [&](int r) { return p.cached ? cache[r - r0] : acc[r]; };
+    __syncthreads();
     uint32_t key = 0;
     int ties = 0;
-    if (want > 0 && want < hi - lo) {
+    if (ranked) {  // the same in the whole cluster
         int left = want;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = t; i < 256; i += kThreads) hist[i] = 0;
-            __syncthreads();
-            for (int r = lo + t; r < hi; r += kThreads) {
-                const uint32_t k = weight_key(acc[r]);
-                if (shift == 24 || (k >> (shift + 8)) == (key >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+        const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+            const int shift = shifts[d], bins = 1 << bits[d];
+            for (int r = max(r0, lo) + t; r < min(r1, hi); r += kThreads) {
+                const uint32_t k = weight_key(weight(r));
+                if (d == 0 || (k >> (shift + bits[d])) == (key >> (shift + bits[d])))
+                    atomicAdd(&hist[d][(k >> shift) & (bins - 1)], 1);
             }
-            __syncthreads();
-            if (t == 0) {
-                int above = 0, d = 255;
-                while (above + hist[d] < left) above += hist[d--];
-                s_digit = d;
-                s_above = above;
+            cluster.sync();
+            // thread t has bins b and b - 1, counted from the top
+            const int b = bins - 1 - 2 * t;
+            int c0 = 0, c1 = 0;
+            if (b > 0)
+                for (int c = 0; c < C; ++c) {
+                    const int* other = cluster.map_shared_rank(&hist[d][0], c);
+                    c0 += other[b];
+                    c1 += other[b - 1];
+                }
+            uint64_t total;
+            const int upto = (int)scan_cta((uint64_t)(c0 + c1), warp_sums, total);
+            const int above = upto - c0 - c1;
+            if (above < left && left <= upto) {
+                const bool first = left <= above + c0;
+                s_digit = first ? b : b - 1;
+                s_above = first ? above : above + c0;
             }
             __syncthreads();
             key |= (uint32_t)s_digit << shift;
@@ -86,85 +139,241 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, i
         }
         ties = left;  // rows equal to `key` that stay, the first ones
     }
-    const bool all = want >= hi - lo;
-    int base = 0, seen = 0;  // rows listed, rows equal to key met
-    for (int r0 = 0; r0 < n; r0 += kThreads) {
-        const int r = r0 + t;
-        const bool cand = r >= lo && r < hi;
-        const uint32_t k = cand && !all && want > 0 ? weight_key(acc[r]) : 0;
-        const bool equal = cand && !all && want > 0 && k == key;
-        int n_eq = 0, n_keep = 0;
-        const int rank = seen + scan_cta(equal, warp_sums, n_eq);
-        const bool keep = r < n && (!cand || all || (want > 0 && (k > key || (equal && rank <= ties))));
-        const int at = base + scan_cta(keep, warp_sums, n_keep) - 1;
-        if (keep) out[at] = r;
-        base += n_keep;
-        seen += n_eq;
-    }
-    if (a.kept_rows) {
+    // 1 << 32: the row stays whatever comes before it; 1: it equals `key`
+    auto mark = [&](int r) -> uint64_t {
+        if (r >= r1) return 0;
+        if (r < lo || r >= hi) return 1ull << 32;
+        if (!ranked) return 0;
+        const uint32_t k = weight_key(weight(r));
+        return k > key ? 1ull << 32 : k == key ? 1ull : 0ull;
+    };
+    // this CTA's counts, then those of the CTAs before it
+    uint64_t sum = 0;
+    for (int r = r0 + t; r < r1; r += kThreads) sum += mark(r);
+    uint64_t total;
+    scan_cta(sum, warp_sums, total);
+    if (t == 0) mine = total;
+    cluster.sync();
+    uint64_t base = 0;
+    for (int c = 0; c < rank; ++c) base += *cluster.map_shared_rank(&mine, c);
+    // places, up to 1024 runs of 32 rows at a time
+    int32_t* list = p.list + sh * p.cap;
+    int32_t* kept_rows = a.kept_rows ? a.kept_rows + sh * a.n_keep : nullptr;
+    float* acc_dst = a.acc_dst && (p.cached || a.acc_dst != a.acc) ? a.acc_dst + sh * a.acc_dst_stride : nullptr;
+    for (int c0 = r0; c0 < r1; c0 += kThreads * 32) {
+        const int runs = min(kThreads, (r1 - c0 + 31) / 32);
+        for (int g = warp; g < runs; g += kWarps) {
+            const uint64_t f = mark(c0 + g * 32 + lane);
+            const uint32_t hard = __ballot_sync(0xffffffffu, f >> 32 != 0), eq = __ballot_sync(0xffffffffu, f & 1);
+            if (lane == 0) counts[g] = ((uint64_t)__popc(hard) << 32) | (uint32_t)__popc(eq);
+        }
         __syncthreads();
-        for (int i = t; i < a.n_keep; i += kThreads) a.kept_rows[sh * a.n_keep + i] = i < m ? out[i] : -1;
+        const uint64_t own = t < runs ? counts[t] : 0;
+        const uint64_t incl = scan_cta(own, warp_sums, total);
+        counts[t] = base + incl - own;
+        __syncthreads();
+        for (int g = warp; g < runs; g += kWarps) {
+            const int r = c0 + g * 32 + lane;
+            const uint64_t f = mark(r);
+            const uint32_t hard = __ballot_sync(0xffffffffu, f >> 32 != 0), eq = __ballot_sync(0xffffffffu, f & 1);
+            const uint32_t below = (1u << lane) - 1;
+            const uint64_t before = counts[g];
+            const int n_hard = (int)(before >> 32) + __popc(hard & below);
+            const int n_eq = (int)(uint32_t)before + __popc(eq & below);
+            if (f >> 32 != 0 || ((f & 1) && n_eq < ties)) {
+                const int at = n_hard + min(n_eq, ties);
+                list[at] = r;
+                if (kept_rows) kept_rows[at] = r;
+                if (acc_dst) acc_dst[at] = weight(r);
+            }
+        }
+        base += total;
+        __syncthreads();
+    }
+    if (kept_rows)
+        for (int i = m + rank * kThreads + t; i < a.n_keep; i += C * kThreads) kept_rows[i] = -1;
+    if (acc_dst)
+        for (int i = m + rank * kThreads + t; i < a.acc_dst_stride; i += C * kThreads) acc_dst[i] = 0.f;
+    cluster.sync();  // no CTA leaves while another reads its counts
+}
+
+constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = kMoveThreads / 32 * 32;  // kept rows per CTA
+
+// Grid (KV head, rows / kMoveRows, sequence): gathers into other rows than the
+// source's.
+template <int NV>  // 16-byte vectors of a row
+__global__ void __launch_bounds__(kMoveThreads) k8b_move(const EvictArgs a, const EvictPlan p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int h = blockIdx.x, s = blockIdx.z, lane = threadIdx.x & 31;
+    const int i0 = (blockIdx.y * (kMoveThreads / 32) + (threadIdx.x >> 5)) * 32;
+    const int m = p.kept[s];
+    if (a.new_lens && h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_lens[s] = m;
+    if (i0 >= m) return;
+    int from = -1, to = -1;
+    if (i0 + lane < m) {
+        from = batch_row(a.src, s, p.list[((int64_t)s * a.n_head_kv + h) * p.cap + i0 + lane], a.err);
+        to = batch_row(a.dst, s, i0 + lane, a.err);
+    }
+    // a row of K and V is 2 NV vectors: 32 / (2 NV) rows at a time (or 2 NV / 32 turns for one)
+    constexpr int kTurns = 2 * NV > 32 ? 2 * NV / 32 : 1;
+    constexpr int kAtOnce = 2 * NV > 32 ? 1 : 32 / (2 * NV);
+    const int cnt = min(32, m - i0);
+    constexpr int kUnroll = 8;
+    for (int j0 = 0; j0 < cnt; j0 += kAtOnce * kUnroll) {
+        uint4 x[kUnroll][kTurns];
+        int dst[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int j = j0 + u * kAtOnce + (kAtOnce > 1 ? lane / (2 * NV) : 0);
+            const int f = __shfl_sync(0xffffffffu, from, j & 31), d = __shfl_sync(0xffffffffu, to, j & 31);
+            dst[u] = j < cnt && f >= 0 ? d : -1;
+#pragma unroll
+            for (int v = 0; v < kTurns; ++v) {
+                const int c = (lane + v * 32) % (2 * NV);
+                const void* base = c < NV ? a.k : a.v;
+                if (dst[u] >= 0)
+                    x[u][v] = *(static_cast<const uint4*>(base) + ((int64_t)f * a.n_head_kv + h) * NV + c % NV);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int v = 0; v < kTurns; ++v) {
+                const int c = (lane + v * 32) % (2 * NV);
+                void* base = c < NV ? a.k_dst : a.v_dst;
+                if (dst[u] >= 0) *(static_cast<uint4*>(base) + ((int64_t)dst[u] * a.n_head_kv + h) * NV + c % NV) = x[u][v];
+            }
     }
 }
 
-// One CTA per (KV head, sequence) moves in row order, so that it can also
-// compact in place: a kept row never moves up.
-__global__ void __launch_bounds__(kThreads) k8b_move(const EvictArgs a, const int32_t* list, const Plan* plan, int cap) {
-    const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
-    const int m = plan[s].m;
-    const int64_t sh = (int64_t)s * a.n_head_kv + h;
-    const int32_t* rows = list + sh * cap;
-    const int row_bytes = a.head_dim * a.elem_bytes, nv = row_bytes / 16;
-    const int per = kThreads / nv;
-    for (int i0 = 0; i0 < m; i0 += per) {
-        const int i = i0 + t / nv, c = t % nv;
-        uint4 kk, vv;
-        int to = -1;
-        if (i < m && t < per * nv) {
-            const int from = batch_row(a.src, s, rows[i], a.err);
-            to = batch_row(a.dst, s, i, a.err);
-            if (from < 0) to = -1;
-            if (to >= 0) {
-                const int64_t f = ((int64_t)from * a.n_head_kv + h) * row_bytes + c * 16;
-                kk = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.k) + f);
-                vv = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.v) + f);
-            }
+constexpr int kPlaceThreads = 512;
+
+// Grid (2 * row bytes / 32, KV head, sequence): compacts one 32-byte column of
+// K or V where it is.
+__global__ void __launch_bounds__(kPlaceThreads) k8c_compact(const EvictArgs a, const EvictPlan p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int nv = a.head_dim * a.elem_bytes / 16, cols = nv / 2;  // 16-byte vectors, 32-byte columns of a row
+    const int h = blockIdx.y, s = blockIdx.z, t = threadIdx.x;
+    const int m = p.kept[s];
+    if (a.new_lens && h == 0 && blockIdx.x == 0 && t == 0) a.new_lens[s] = m;
+    uint4* base = static_cast<uint4*>((int)blockIdx.x < cols ? a.k_dst : a.v_dst);
+    const int vec = (blockIdx.x % cols) * 2 + (t & 1);
+    const int32_t* list = p.list + ((int64_t)s * a.n_head_kv + h) * p.cap;
+    constexpr int kUnroll = 4, kRows = kPlaceThreads / 2;
+    for (int i0 = 0; i0 < m; i0 += kRows * kUnroll) {
+        uint4 x[kUnroll];
+        int64_t to[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int i = i0 + u * kRows + (t >> 1);
+            to[u] = -1;
+            if (i >= m || list[i] == i) continue;
+            const int from = batch_row(a.src, s, list[i], a.err), d = batch_row(a.src, s, i, a.err);
+            if (from < 0 || d < 0) continue;
+            to[u] = ((int64_t)d * a.n_head_kv + h) * nv + vec;
+            x[u] = base[((int64_t)from * a.n_head_kv + h) * nv + vec];
         }
         __syncthreads();
-        if (to >= 0) {
-            const int64_t f = ((int64_t)to * a.n_head_kv + h) * row_bytes + c * 16;
-            *reinterpret_cast<uint4*>(static_cast<char*>(a.k_dst) + f) = kk;
-            *reinterpret_cast<uint4*>(static_cast<char*>(a.v_dst) + f) = vv;
-        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (to[u] >= 0) base[to[u]] = x[u];
+    }
+}
+
+// Grid (KV head, sequence): the weights of a slice too long for shared memory,
+// where they are.
+__global__ void __launch_bounds__(kThreads) k8d_compact_weights(const EvictArgs a, const EvictPlan p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t sh = (int64_t)blockIdx.y * a.n_head_kv + blockIdx.x;
+    const int m = p.kept[blockIdx.y];
+    float* acc = a.acc_dst + sh * a.acc_dst_stride;
+    for (int i0 = 0; i0 < a.acc_dst_stride; i0 += kThreads) {
+        const int i = i0 + threadIdx.x;
+        const float x = i < m ? acc[p.list[sh * p.cap + i]] : 0.f;
         __syncthreads();
+        if (i < a.acc_dst_stride) acc[i] = x;
     }
-    if (a.acc_dst) {
-        for (int i0 = 0; i0 < a.acc_dst_stride; i0 += kThreads) {
-            const int i = i0 + t;
-            const float x = i < m ? a.acc[sh * a.acc_stride + rows[i]] : 0.f;
-            __syncthreads();
-            if (i < a.acc_dst_stride) a.acc_dst[sh * a.acc_dst_stride + i] = x;
-            __syncthreads();
-        }
-    }
-    if (a.new_lens && h == 0 && t == 0) a.new_lens[s] = m;
+}
+
+// ---------------------------------------------------------------- host side --
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+size_t plan_of(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t n_head_kv, char* ws, EvictPlan* p) {
+    p->cap = n_keep < max_kv_len ? n_keep : max_kv_len;
+    // a CTA per 2048 rows, up to 8 per head
+    p->cluster = 1;
+    while (p->cluster < kMaxCluster && p->cluster * 2048 < max_kv_len) p->cluster *= 2;
+    p->cached = (max_kv_len + p->cluster - 1) / p->cluster + 31 <= kCacheRows;
+    p->kept = reinterpret_cast<int32_t*>(ws);
+    const size_t head = up16((size_t)n_seq * sizeof(int32_t));
+    p->list = reinterpret_cast<int32_t*>(ws + head);
+    return head + up16((size_t)n_seq * n_head_kv * p->cap * sizeof(int32_t));
+}
+
+template <class... P, class... A>
+cudaError_t launch_after(void (*k)(P...), dim3 grid, int threads, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
 }  // namespace
 
 size_t evict_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t n_head_kv) {
-    const size_t cap = n_keep < max_kv_len ? n_keep : max_kv_len;
-    return (size_t)n_seq * (sizeof(Plan) + n_head_kv * cap * sizeof(int32_t));
+    EvictPlan p{};
+    return plan_of(n_seq, max_kv_len, n_keep, n_head_kv, nullptr, &p);
 }
 
 cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s) {
-    const int cap = a.n_keep < a.src.max_kv_len ? a.n_keep : a.src.max_kv_len;
-    Plan* plan = static_cast<Plan*>(a.ws);
-    int32_t* list = reinterpret_cast<int32_t*>(plan + a.src.n_seq);
-    const dim3 grid(a.n_head_kv, a.src.n_seq);
-    k8a_select_rows<<<grid, kThreads, 0, s>>>(a, list, plan, cap);
-    k8b_move<<<grid, kThreads, 0, s>>>(a, list, plan, cap);
-    return cudaGetLastError();
+    EvictPlan p{};
+    plan_of(a.src.n_seq, a.src.max_kv_len, a.n_keep, a.n_head_kv, static_cast<char*>(a.ws), &p);
+    const int smem = p.cached ? (((a.src.max_kv_len + p.cluster - 1) / p.cluster + 31) & ~31) * (int)sizeof(float) : 0;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    static std::atomic<unsigned> set_mask{0};
+    if (dev >= 32 || !(set_mask.load(std::memory_order_acquire) & (1u << dev))) {
+        const cudaError_t e = cudaFuncSetAttribute(k8a_select_rows, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   kCacheRows * (int)sizeof(float));
+        if (e != cudaSuccess) return e;
+        if (dev < 32) set_mask.fetch_or(1u << dev, std::memory_order_release);
+    }
+    const int64_t ctas = (int64_t)a.src.n_seq * a.n_head_kv * p.cluster;
+    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = p.cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, k8a_select_rows, a, p);
+    if (e != cudaSuccess) return e;
+    const int nv = a.head_dim * a.elem_bytes / 16;
+    if (a.in_place) {
+        e = launch_after(k8c_compact, dim3(nv, a.n_head_kv, a.src.n_seq), kPlaceThreads, s, a, p);
+    } else {
+        const dim3 grid(a.n_head_kv, (p.cap + kMoveRows - 1) / kMoveRows, a.src.n_seq);
+        if (nv == 8) e = launch_after(k8b_move<8>, grid, kMoveThreads, s, a, p);
+        else if (nv == 16) e = launch_after(k8b_move<16>, grid, kMoveThreads, s, a, p);
+        else e = launch_after(k8b_move<32>, grid, kMoveThreads, s, a, p);
+    }
+    if (e == cudaSuccess && a.acc_dst == a.acc && !p.cached) {
+        k8d_compact_weights<<<dim3(a.n_head_kv, a.src.n_seq), kThreads, 0, s>>>(a, p);
+        e = cudaGetLastError();
+    }
+    return e;
 }
 
 }  // namespace epsp

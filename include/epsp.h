@@ -510,7 +510,8 @@ int32_t ep_sp_prompt_weights(ep_sp_ctx* ctx, int32_t layer, const void* q, const
  *   dst        the destination's layout (n_seq as in src, max_kv_len and room >=
  *              min(n_keep, src's max_kv_len); its kv_lens is not read).  Either the same cache (k_dst
  *              == k, v_dst == v and the same layout and table pointer), which
- *              is compacted in place, or blocks / rows that are none of the
+ *              is compacted in place (no two sequences may then share a
+ *              block), or blocks / rows that are none of the
  *              source's (the same pool under another table is fine);
  *   acc_dst    NULL, or [n_seq][n_head_kv][acc_dst_stride]: the kept rows'
  *              weights, zero from m to acc_dst_stride (acc_dst_stride >=

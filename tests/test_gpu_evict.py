@@ -113,6 +113,11 @@ def test_long_sequences(n, n_keep, mode):
     run_case([n], n_keep, 0, 0, (4, 2, 64), BF16, 64, 64, "ties", mode, seed=n)
 
 
+@pytest.mark.parametrize("mode", ["gather", "place"])
+def test_weights_longer_than_a_cluster_keeps_on_chip(mode):
+    run_case([300001, 5], 70000, 4, 1000, (1, 1, 64), F16, 32, 32, "ties", mode, seed=8)
+
+
 def test_many_short_sequences():
     run_case([1 + 13 * i % 200 for i in range(200)], 40, 2, 10, (14, 2, 64), F16, 64, 64)
 
