@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstdint>
 #include <string>
 
 #include "../epsp_kernels.h"
@@ -103,6 +104,7 @@ int32_t check_batch(ep_sp_ctx* c, const ep_sp_kv_batch* b, int32_t min_rows, boo
 
 int32_t check_workspace(ep_sp_ctx* c, const void* ws, size_t have, size_t need) {
     if (need == 0) return kOk;
+    if (need == SIZE_MAX) return ctx_fail(c, kInvalid, "more cache rows than one call takes");
     if (!ws || have < need)
         return ctx_fail(c, kInvalid, "the workspace holds " + std::to_string(ws ? have : 0) + " bytes, the call needs " +
                                          std::to_string(need));
@@ -122,6 +124,7 @@ int32_t ep_sp_decode_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_l
         return kInvalid;
     const ep_sp_config& c = ctx->cfg;
     *bytes = epsp::decode_ws_bytes(n_seq, max_kv_len, c.n_head, c.n_head_kv, c.head_dim, c.dtype, with_acc != 0);
+    if (*bytes == SIZE_MAX) return kInvalid;
     return kOk;
 }
 

@@ -37,6 +37,8 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <climits>
+#include <cstdint>
 
 #include "epsp_kernels.h"
 #include "tc100.cuh"
@@ -48,6 +50,12 @@ constexpr int kUnit = 32;      // cache rows per unit
 constexpr int kCtas = 148;     // one per SM
 constexpr int kHeads = 8;      // query heads per warp
 constexpr int kChunk = kUnit * 128;  // one 128-byte column block of a unit
+// Fewest units dealt to a CTA.
+#ifndef K6_MIN_UNITS
+#define K6_MIN_UNITS 4
+#endif
+constexpr int kMinUnits = K6_MIN_UNITS;
+constexpr int kLensOnChip = 1024;  // lengths a CTA keeps in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 // A call of at most this many units per run and one CTA per run skips the
 // split (and the join).
@@ -61,8 +69,8 @@ struct DecodeSplit {
     int32_t groups;    // warps that share a unit (1, 2, 4, 8), 8 query heads each
     int32_t score_stride;
     // workspace
-    int64_t* per;        // units per CTA
-    int64_t* run_start;  // [n_seq][Hkv][passes] first unit of each run
+    int32_t* per;        // units per CTA
+    int32_t* run_start;  // [n_seq][Hkv][passes] first unit of each run
     float* part_o;       // [2 ctas][groups * 8][D]
     float2* part_ml;     // [2 ctas][groups * 8] (maximum, sum), log2 units
     float* lse;          // [n_seq][n_head] log2 units, runs finished by one CTA
@@ -136,59 +144,118 @@ __device__ __forceinline__ void store4(void* out, int32_t dtype, int64_t i, floa
     }
 }
 
-// ET 0 f32, 1 f16, 2 bf16.
-template <int ET, int D>
+// ET 0 f32, 1 f16, 2 bf16; W consumer warps (and a producer).
+template <int ET, int D, int W>
 struct Layout {
     static constexpr int kEs = ET == 0 ? 4 : 2;
     static constexpr int kCols = D * kEs / 128;          // 128-byte column blocks of a row
     static constexpr int kHalf = kCols * kChunk;         // K (or V) of a unit
     static constexpr int kStage = 2 * kHalf;
-    // Consumer warps (and a producer).  A stage always falls to the same
-    // stream of warps (kStages is a multiple of kWarps): a warp that found
-    // its stage full knows that the stage's earlier fill had landed, which
-    // the barrier's one phase bit cannot tell it.
-    static constexpr int kWarps = ET == 0 && D == 128 ? 4 : 8;
-    static constexpr int kThreads = (kWarps + 1) * 32;
-    static constexpr int kStages = kStage == 32768 ? 4 : kStage == 16384 ? 8 : 16;
-    static constexpr int kPass = kWarps * kHeads;        // query heads of a pass
-    static constexpr int kOffO = kStages * kStage;       // [8 warps][8 heads][D] merge buffer (f32: q before it)
-    static constexpr int kOffP = kOffO + kWarps * kHeads * D * 4;  // f32: [8 warps][32 keys][8 heads]
+    // A stage always falls to the same stream of warps (kStages is a multiple
+    // of W): a warp that found its stage full knows that the stage's earlier
+    // fill had landed, which the barrier's one phase bit cannot tell it.
+    static constexpr int kWarps = W;
+    static constexpr int kThreads = (W + 1) * 32;
+    static constexpr int kStages = (W == 4 && ET != 0 ? 196608 : 131072) / kStage;
+    static constexpr int kPass = W == 4 && ET != 0 ? 16 : W * kHeads;  // query heads of a pass
+    static constexpr int kOffQ = kStages * kStage;       // [2][kPass][D] queries of a segment
+    static constexpr int kQBytes = kPass * D * kEs;
+    static constexpr int kOffO = kOffQ + 2 * kQBytes;    // [kWarps][8 heads][D] merge buffer
+    static constexpr int kOffP = kOffO + kWarps * kHeads * D * 4;  // f32: [kWarps][32 keys][8 heads]
     static constexpr int kOffMl = kOffP + (ET == 0 ? kWarps * kUnit * kHeads * 4 : 0);
-    static constexpr int kOffBar = kOffMl + kWarps * kHeads * 8;
-    static constexpr int kOffPos = kOffBar + 2 * kStages * 8;
-    static constexpr int kBytes = kOffPos + 64 + (kWarps + 1) * 8;
+    static constexpr int kOffBar = kOffMl + 2 * kWarps * kHeads * 8;
+    static constexpr int kOffLens = kOffBar + (2 * kStages + 4) * 8;
+    static constexpr int kBytes = kOffLens + kLensOnChip * 4;
     static_assert(kStages % kWarps == 0 && kBytes + 1024 <= 232448, "shared memory");
 };
 
 static_assert(kUnit == 32, "a lane per row, a page holds whole units");
 
+// The sequences' lengths: on chip when there are few.
+struct Lens {
+    const int32_t* chip;
+    __device__ __forceinline__ int32_t at(const DecodeArgs& a, int s) const {
+        return chip != nullptr ? chip[s] : batch_len(a.kv, s, a.err);
+    }
+};
+
 // Walks the segments (a run's part inside this CTA) of a CTA's units.
 struct Walk {
     int32_t s, run, u, n, units;  // sequence, run within it (h * passes + pass), next unit, length, units of the run
-    int64_t left;                 // units of the CTA not walked yet
-    int64_t first;                // the CTA's first unit in the order of all
+    int32_t left;                 // units of the CTA not walked yet
+    int32_t first;                // the CTA's first unit in the order of all
+
+    __device__ __forceinline__ void advance(const DecodeArgs& a, const Lens& lens, int runs, int n_seg) {
+        u += n_seg;
+        left -= n_seg;
+        if (left == 0) return;
+        u = 0;
+        if (++run < runs) return;
+        run = 0;
+        units = 0;
+        while (units == 0 && ++s < a.kv.n_seq) {
+            n = lens.at(a, s);
+            units = units_of(n);
+        }
+        if (units == 0) left = 0;
+    }
 };
 
-template <int ET, int D>
-__device__ __forceinline__ void next_run(const DecodeArgs& a, int runs, Walk& w) {
-    w.u = 0;
-    if (++w.run < runs) return;
-    w.run = 0;
-    w.units = 0;
-    while (w.units == 0 && ++w.s < a.kv.n_seq) {
-        w.n = batch_len(a.kv, w.s, a.err);
-        w.units = units_of(w.n);
+// This CTA's share of all runs' units (every warp on its own): lane i adds up
+// a 32nd of the sequences, the lane whose part holds the CTA's first unit
+// looks for its sequence.
+__device__ __forceinline__ Walk share_of(const DecodeArgs& a, const DecodeSplit& sp, const Lens& lens, int runs,
+                                         int lane) {
+    Walk w{};
+    const int n_seq = a.kv.n_seq, part = (n_seq + 31) / 32;
+    const int s0 = min(n_seq, lane * part), s1 = min(n_seq, s0 + part);
+    int32_t mine = 0;
+    for (int s = s0; s < s1; ++s) mine += units_of(lens.at(a, s));
+    mine *= runs;
+    int32_t incl = mine;
+    if (n_seq > 1) {
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int32_t v = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += v;
+        }
     }
-    if (w.units == 0) w.left = 0;
+    const int32_t total = __shfl_sync(0xffffffffu, incl, n_seq > 1 ? 31 : 0);
+    const int32_t per = max((int32_t)(((uint32_t)total + sp.ctas - 1) / (uint32_t)sp.ctas), kMinUnits);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *sp.per = per;
+    if (total / per < (int)blockIdx.x) return w;  // (the product below stays under total)
+    w.first = per * blockIdx.x;
+    if (w.first >= total) return w;
+    w.left = min(per, total - w.first);
+    const bool here = mine > 0 && w.first >= incl - mine && w.first < incl;
+    if (here) {
+        int32_t off = w.first - (incl - mine);
+        w.s = s0;
+        for (;; ++w.s) {
+            w.n = lens.at(a, w.s);
+            w.units = units_of(w.n);
+            if (off < w.units * runs) break;
+            off -= w.units * runs;
+        }
+        w.run = (int32_t)((uint32_t)off / (uint32_t)w.units);
+        w.u = off - w.run * w.units;
+    }
+    const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    w.s = __shfl_sync(0xffffffffu, w.s, from);
+    w.n = __shfl_sync(0xffffffffu, w.n, from);
+    w.units = __shfl_sync(0xffffffffu, w.units, from);
+    w.run = __shfl_sync(0xffffffffu, w.run, from);
+    w.u = __shfl_sync(0xffffffffu, w.u, from);
+    return w;
 }
 
 // Overwrites what TMA brought of a sequence's last rows [from, 32) of a unit:
 // row `fresh` (>= 0) from the new token's K and V, V rows from `lim` on with
 // zeros (their P is 0, and 0 * NaN is not 0).
-template <int ET, int D>
+template <int ET, int D, int W>
 __device__ __forceinline__ void patch_unit(unsigned char* stage, int lane, int lim, int fresh, const char* kn,
                                            const char* vn) {
-    using LY = Layout<ET, D>;
+    using LY = Layout<ET, D, W>;
     constexpr int nc = LY::kCols * 8;  // 16-byte chunks per row
     auto at = [&](unsigned char* base, int r, int c) {
         return reinterpret_cast<uint4*>(base + (c >> 3) * kChunk + r * 128 + (((c & 7) ^ (r & 7)) << 4));
@@ -204,36 +271,43 @@ __device__ __forceinline__ void patch_unit(unsigned char* stage, int lane, int l
     __syncwarp();
 }
 
-template <int ET, int D, bool P3, int GH>
-__global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
+template <int ET, int D, int W, bool P3, int GH>
+__global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
     k6a_decode(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
                const DecodeSplit sp) {
-    using LY = Layout<ET, D>;
+    using LY = Layout<ET, D, W>;
     constexpr bool BF16 = ET == 2;
     constexpr int kWarps = LY::kWarps, kThreads = LY::kThreads, kPass = LY::kPass;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
     uint64_t* empty = full + LY::kStages;
-    int64_t* pos = reinterpret_cast<int64_t*>(smem + LY::kOffPos);  // [0] total, [1] seq, [2] units before it
-    int64_t* wsum = pos + 8;
+    uint64_t* q_full = empty + LY::kStages;
+    uint64_t* q_empty = q_full + 2;
+    int32_t* lens_s = reinterpret_cast<int32_t*>(smem + LY::kOffLens);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int Hkv = a.n_head_kv, G = a.n_head / Hkv;
     const int runs = Hkv * sp.passes;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int i = 0; i < LY::kStages; ++i) {
             tc::mbar_init(&full[i], 1);
             tc::mbar_init(&empty[i], sp.groups);
         }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&q_full[i], 1);
+            tc::mbar_init(&q_empty[i], kWarps);
+        }
         tc::fence_mbar_init();
         tc::tma_prefetch_desc(&tmK);
         tc::tma_prefetch_desc(&tmV);
     }
+    tc::pdl_wait();
+    tc::pdl_launch();
 
     // ----------------------------------------- this CTA's range of the units
     Walk w0;
+    Lens lens{nullptr};
     if (sp.direct) {
         w0.s = blockIdx.x / runs;
         w0.run = blockIdx.x % runs;
@@ -244,53 +318,12 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
         w0.first = 0;
         __syncthreads();
     } else {
-        int64_t total = 0, per = 0, first = 0;
-        // twice over the sequences: their sum, then the one the range begins in
-        for (int round = 0; round < 2; ++round) {
-            int64_t base = 0;
-            for (int s0 = 0; s0 < a.kv.n_seq; s0 += kThreads) {
-                const int s = s0 + (int)threadIdx.x;
-                const int64_t mine = s < a.kv.n_seq ? (int64_t)units_of(batch_len(a.kv, s, a.err)) * runs : 0;
-                int64_t incl = mine;
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
-                    if (lane >= d) incl += v;
-                }
-                __syncthreads();
-                if (lane == 31) wsum[warp] = incl;
-                __syncthreads();
-                int64_t before = base, all = 0;
-                for (int i = 0; i <= kWarps; ++i) {
-                    if (i < warp) before += wsum[i];
-                    all += wsum[i];
-                }
-                incl += before;
-                if (round == 1 && mine > 0 && first >= incl - mine && first < incl) {
-                    pos[1] = s;
-                    pos[2] = incl - mine;
-                }
-                base += all;
-            }
-            if (round == 0) {
-                total = base;
-                // at least one unit per warp of a CTA
-                per = (total + sp.ctas - 1) / sp.ctas;
-                if (per < kWarps) per = kWarps;
-                first = per * blockIdx.x;
-            }
+        if (a.kv.n_seq <= kLensOnChip) {
+            for (int s = threadIdx.x; s < a.kv.n_seq; s += kThreads) lens_s[s] = batch_len(a.kv, s, a.err);
+            lens.chip = lens_s;
         }
         __syncthreads();
-        if (blockIdx.x == 0 && threadIdx.x == 0) *sp.per = per;
-        w0.first = first;
-        w0.left = first >= total ? 0 : (total - first < per ? total - first : per);
-        if (w0.left > 0) {
-            w0.s = (int32_t)pos[1];
-            w0.n = batch_len(a.kv, w0.s, a.err);
-            w0.units = units_of(w0.n);
-            const int64_t off = first - pos[2];
-            w0.run = (int32_t)(off / w0.units);
-            w0.u = (int32_t)(off % w0.units);
-        }
+        w0 = share_of(a, sp, lens, runs, lane);
     }
     if (w0.left == 0) {
         if (sp.direct) {  // a sequence without rows
@@ -307,11 +340,27 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
         // ------------------------------------------------------- producer --
         // 32 units' rows at a time (one table entry per lane), lane 0 issues.
         Walk w = w0;
-        int64_t it = 0;
+        int it = 0;
         bool ok = true;
-        while (w.left > 0 && ok) {
-            const int n_seg = (int)min((int64_t)(w.units - w.u), w.left);
-            const int h = w.run / sp.passes;
+        int seg = 0;
+        const uint64_t policy = tc::policy_evict_first();  // the cache is read once
+        for (; w.left > 0 && ok; ++seg) {
+            const int n_seg = min(w.units - w.u, w.left);
+            const int h = w.run / sp.passes, pass = w.run % sp.passes;
+            if (lane == 0) {
+                const int b = seg & 1;
+                ok = tc::mbar_wait(&q_empty[b], ((seg >> 1) & 1) ^ 1, tmo);
+                if (ok) {
+                    const uint32_t bytes = min(kPass, G - pass * kPass) * D * LY::kEs;
+                    tc::mbar_arrive_expect_tx(&q_full[b], bytes);
+                    tc::bulk_load(smem + LY::kOffQ + b * LY::kQBytes,
+                                  static_cast<const char*>(a.q) +
+                                      ((int64_t)w.s * a.n_head + (int64_t)h * G + pass * kPass) * D * LY::kEs,
+                                  bytes, &q_full[b]);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) break;
             for (int i0 = 0; i0 < n_seg && ok; i0 += 32) {
                 int row = a.kv.rows;  // past the end: zeros
                 if (i0 + lane < n_seg) {
@@ -320,7 +369,7 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
                 }
                 const int cnt = min(32, n_seg - i0);
                 for (int i = 0; i < cnt; ++i, ++it) {
-                    const int st = (int)(it % LY::kStages);
+                    const int st = it % LY::kStages;
                     const int r = __shfl_sync(0xffffffffu, row, i);
                     if (lane == 0) {
                         ok = tc::mbar_wait(&empty[st], ((it / LY::kStages) & 1) ^ 1, tmo);
@@ -329,26 +378,25 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
                             unsigned char* base = smem + st * LY::kStage;
 #pragma unroll
                             for (int c = 0; c < LY::kCols; ++c)
-                                tc::tma_load_3d(base + c * kChunk, &tmK, &full[st], c * (128 / LY::kEs), h, r);
+                                tc::tma_load_3d(base + c * kChunk, &tmK, &full[st], c * (128 / LY::kEs), h, r, policy);
 #pragma unroll
                             for (int c = 0; c < LY::kCols; ++c)
                                 tc::tma_load_3d(base + LY::kHalf + c * kChunk, &tmV, &full[st], c * (128 / LY::kEs), h,
-                                                r);
+                                                r, policy);
                         }
                     }
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     if (!ok) break;
                 }
             }
-            w.u += n_seg;
-            w.left -= n_seg;
-            if (w.left > 0) next_run<ET, D>(a, runs, w);
+            w.advance(a, lens, runs, n_seg);
         }
         if (!ok) {
-            if (lane == 0) report_error(a.err, kDevWaitDecode, 0xa1, (int32_t)it);
+            if (lane == 0) report_error(a.err, kDevWaitDecode, 0xa1, it);
             // copies still in flight land before the CTA ends
-            for (int64_t j = it > LY::kStages ? it - LY::kStages : 0; j < it; ++j)
+            for (int j = max(0, it - LY::kStages); j < it; ++j)
                 tc::mbar_wait(&full[j % LY::kStages], (j / LY::kStages) & 1, tmo);
+            for (int j = max(0, seg - 1); j <= seg; ++j) tc::mbar_wait(&q_full[j & 1], (j >> 1) & 1, tmo);
         }
         return;
     }
@@ -360,12 +408,11 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
     float* om = reinterpret_cast<float*>(smem + LY::kOffO);
     float* om_w = om + warp * kHeads * D;
     float* ps = reinterpret_cast<float*>(smem + LY::kOffP) + warp * kUnit * kHeads;
-    float2* ml = reinterpret_cast<float2*>(smem + LY::kOffMl);
     Walk w = w0;
-    int64_t it = 0;
+    int it = 0;
     bool ok = true;
     for (int seg = 0; w.left > 0; ++seg) {
-        const int n_seg = (int)min((int64_t)(w.units - w.u), w.left);
+        const int n_seg = min(w.units - w.u, w.left);
         const int h = w.run / sp.passes, pass = w.run % sp.passes;
         const int g0 = pass * kPass + grp * kHeads;  // this warp's first query head of the group
         const int64_t q_row = (int64_t)w.s * a.n_head + (int64_t)h * G;
@@ -383,32 +430,24 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
         }
         uint32_t qf[ET == 0 ? 1 : D / 8];
         const int hd = lane >> 2, qc = (lane & 3) * 2;  // 16-bit: head and columns of this lane's fragments
-        if constexpr (ET == 0) {
-            __syncwarp();
-            for (int i = lane; i < GH * (D / 4); i += 32) {
-                const int g = i / (D / 4);
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (g0 + g < G)
-                    x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (q_row + g0 + g) * D +
-                                                         (i % (D / 4)) * 4);
-                reinterpret_cast<float4*>(om_w)[i] = x;
-            }
-            __syncwarp();
-        } else {
-            const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (q_row + g0 + hd) * D + qc;
+        const unsigned char* qs = smem + LY::kOffQ + (seg & 1) * LY::kQBytes + grp * kHeads * D * LY::kEs;
+        if (ok) {
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(&q_full[seg & 1], (seg >> 1) & 1, tmo));
+            if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xa3, seg);
+        }
+        if constexpr (ET != 0) {
 #pragma unroll
             for (int i = 0; i < D / 8; ++i)
-                qf[i] = g0 + hd < G ? *reinterpret_cast<const uint32_t*>(qp + i * 8) : 0u;
+                qf[i] = g0 + hd < G ? *reinterpret_cast<const uint32_t*>(qs + (hd * D + qc + i * 8) * 2) : 0u;
         }
         // first unit of the segment that falls to this stream
-        int i = (int)(((int64_t)stream - it % streams + streams) % streams);
+        int i = (stream - it) & (streams - 1);
         for (; i < n_seg; i += streams) {
-            const int64_t at = it + i;
-            const int st = (int)(at % LY::kStages);
+            const int at = it + i, st = at % LY::kStages;
             if (ok) {
                 ok = tc::mbar_wait(&full[st], (at / LY::kStages) & 1, tmo);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xa2, (int32_t)at);
+                if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xa2, at);
             }
             if (!ok) break;
             unsigned char* stage = smem + st * LY::kStage;
@@ -418,7 +457,7 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
                 const int64_t nr = ((int64_t)w.s * Hkv + h) * D * LY::kEs;
                 const char* kn = static_cast<const char*>(a.k_new) + nr;
                 const char* vn = static_cast<const char*>(a.v_new) + nr;
-                if (fresh || lim < kUnit) patch_unit<ET, D>(stage, lane, lim, fresh ? lim - 1 : -1, kn, vn);
+                if (fresh || lim < kUnit) patch_unit<ET, D, W>(stage, lane, lim, fresh ? lim - 1 : -1, kn, vn);
                 if (fresh && grp == 0 && pass == 0) {
                     const int row = batch_row(a.kv, w.s, w.n - 1, a.err);
                     constexpr int nc = D * LY::kEs / 16;
@@ -511,7 +550,7 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
                 float x[GH];
 #pragma unroll
                 for (int g = 0; g < GH; ++g) x[g] = 0.f;
-                const float4* q4 = reinterpret_cast<const float4*>(om_w);
+                const float4* q4 = reinterpret_cast<const float4*>(qs);  // (heads past the group: any values, not used)
 #pragma unroll 4
                 for (int c = 0; c < D / 4; ++c) {
                     const float4 kk = *reinterpret_cast<const float4*>(stage + (c >> 3) * kChunk + lane * 128 +
@@ -585,25 +624,45 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
         }
 
         // ------------------------------------------- merge the warps' states
+        // (ml alternates between two buffers: a warp may write the next
+        // segment's before another has read this one's sums)
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&q_empty[seg & 1]);
+        float2* ml = reinterpret_cast<float2*>(smem + LY::kOffMl) + (seg & 1) * kWarps * kHeads;
         if constexpr (ET != 0) {
             l[0] += __shfl_xor_sync(0xffffffffu, l[0], 1);
             l[0] += __shfl_xor_sync(0xffffffffu, l[0], 2);
+            if ((lane & 3) == 0) ml[warp * kHeads + hd] = make_float2(m[0], l[0]);
+        } else {
+#pragma unroll
+            for (int g = 0; g < GH; ++g) {
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], d);
+                if (lane == 0) ml[warp * kHeads + g] = make_float2(m[g], l[g]);
+            }
+        }
+        tc::named_bar_sync(1, kWarps * 32);
+        // the streams' common maximum of a head of this warp's group
+        auto top = [&](int g) {
+            float mt = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < kWarps; ++r)
+                if (r < streams) mt = fmaxf(mt, ml[(r * groups + grp) * kHeads + g].x);
+            return mt == -INFINITY ? 0.f : mt;
+        };
+        if constexpr (ET != 0) {
+            const float f = ex2(m[0] - top(hd));
 #pragma unroll
             for (int c = 0; c < D / 8; ++c)  // rows 8-15 hold the P remainders' part
                 *reinterpret_cast<float2*>(om_w + hd * D + c * 8 + qc) =
-                    make_float2(o[4 * c] + o[4 * c + 2], o[4 * c + 1] + o[4 * c + 3]);
-            if ((lane & 3) == 0) ml[warp * kHeads + hd] = make_float2(m[0], l[0]);
+                    make_float2((o[4 * c] + o[4 * c + 2]) * f, (o[4 * c + 1] + o[4 * c + 3]) * f);
         } else {
             constexpr int NC = D / 32;
-            __syncwarp();
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
-                float t = l[g];
+                const float f = ex2(m[g] - top(g));
 #pragma unroll
-                for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
-#pragma unroll
-                for (int e = 0; e < NC; ++e) om_w[g * D + lane * NC + e] = o[g * NC + e];
-                if (lane == 0) ml[warp * kHeads + g] = make_float2(m[g], t);
+                for (int e = 0; e < NC; ++e) om_w[g * D + lane * NC + e] = o[g * NC + e] * f;
             }
         }
         tc::named_bar_sync(1, kWarps * 32);
@@ -611,24 +670,27 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
         const int n_heads = min(groups * kHeads, G - pass * kPass);
         const int slot = blockIdx.x * 2 + (seg == 0 ? 0 : 1);
         for (int j = threadIdx.x; j < n_heads * (D / 4); j += kWarps * 32) {
-            const int g = j / (D / 4), c = j % (D / 4);
+            const int g = j / (D / 4), c = j % (D / 4), gw = g / kHeads, gh = g % kHeads;
+            float2 v[kWarps];
+            float4 t[kWarps];
             float mt = -INFINITY;
-            for (int r = 0; r < streams; ++r) {
-                const float2 v = ml[(r * groups + g / kHeads) * kHeads + g % kHeads];
-                if (v.y != 0.f) mt = fmaxf(mt, v.x);
-            }
+#pragma unroll
+            for (int r = 0; r < kWarps; ++r)
+                if (r < streams) {
+                    const int wr = (r * groups + gw) * kHeads + gh;
+                    v[r] = ml[wr];
+                    t[r] = *reinterpret_cast<const float4*>(om + wr * D + c * 4);
+                    mt = fmaxf(mt, v[r].x);
+                }
             const float ms = mt == -INFINITY ? 0.f : mt;
             float lt = 0.f;
             float4 ot = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int r = 0; r < streams; ++r) {
-                const int wr = r * groups + g / kHeads;
-                const float2 v = ml[wr * kHeads + g % kHeads];
-                if (v.y == 0.f) continue;  // no unit, or nothing but -inf
-                const float f = ex2(v.x - ms);
-                const float4 t = *reinterpret_cast<const float4*>(om + (wr * kHeads + g % kHeads) * D + c * 4);
-                lt += f * v.y;
-                ot.x += f * t.x, ot.y += f * t.y, ot.z += f * t.z, ot.w += f * t.w;
-            }
+#pragma unroll
+            for (int r = 0; r < kWarps; ++r)
+                if (r < streams) {
+                    lt += v[r].y * ex2(v[r].x - ms);
+                    ot.x += t[r].x, ot.y += t[r].y, ot.z += t[r].z, ot.w += t[r].w;
+                }
             if (whole) {
                 const float inv = 1.f / lt;
                 store4(a.out, a.out_dtype, (q_row + pass * kPass + g) * D + c * 4,
@@ -637,22 +699,18 @@ __global__ void __launch_bounds__(Layout<ET, D>::kThreads, 1)
             } else {
                 const int64_t p = (int64_t)slot * groups * kHeads + g;
                 *reinterpret_cast<float4*>(sp.part_o + p * D + c * 4) = ot;
-                if (c == 0) sp.part_ml[p] = make_float2(mt, lt);
+                if (c == 0) sp.part_ml[p] = make_float2(ms, lt);
             }
         }
         if (w.u == 0 && !sp.direct && threadIdx.x == 0) sp.run_start[(int64_t)w.s * runs + w.run] = w0.first + it;
-        tc::named_bar_sync(1, kWarps * 32);
         it += n_seg;
-        w.u += n_seg;
-        w.left -= n_seg;
-        if (w.left > 0) next_run<ET, D>(a, runs, w);
+        w.advance(a, lens, runs, n_seg);
     }
 }
 
 // CTAs that share run `at` of sequence s, and each one's slot.
 struct Shares {
-    int64_t per, start;
-    int32_t c0, count;
+    int32_t per, start, c0, count;
     __device__ __forceinline__ int slot(int i) const {
         const int c = c0 + i;
         return 2 * c + (i == 0 && start > c * per ? 1 : 0);
@@ -663,8 +721,8 @@ __device__ __forceinline__ Shares shares_of(const DecodeSplit& sp, int64_t run, 
     if (sp.direct) return r;
     r.per = *sp.per;
     r.start = sp.run_start[run];
-    r.c0 = (int32_t)(r.start / r.per);
-    r.count = (int32_t)((r.start + units - 1) / r.per) - r.c0 + 1;
+    r.c0 = r.start / r.per;
+    r.count = (r.start + units - 1) / r.per - r.c0 + 1;
     return r;
 }
 
@@ -698,9 +756,10 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
     __shared__ float wgt[kCtas];
     __shared__ float part[kJoinThreads * 4];
     __shared__ float lse[128];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = a.n_head / a.n_head_kv, runs = a.n_head_kv * sp.passes, stride = sp.groups * kHeads;
+    tc::pdl_wait();
+    tc::pdl_launch();
     const int n = batch_len(a.kv, s, a.err), units = units_of(n);
     if ((int)blockIdx.x < a.n_head) {
         const int hq = blockIdx.x, h = hq / G, g = hq % G, pass = g / sp.pass_heads;
@@ -714,6 +773,16 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
         const Shares sh = shares_of(sp, (int64_t)s * runs + h * sp.passes + pass, units);
         if (sh.count == 1) return;
         const int gi = g % sp.pass_heads;
+        constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes, kHeld = 4;
+        const int c = threadIdx.x % kLanes, r = threadIdx.x / kLanes;
+        auto part_of = [&](int i) {
+            return *reinterpret_cast<const float4*>(sp.part_o + ((int64_t)sh.slot(i) * stride + gi) * D + c * 4);
+        };
+        // the first few shares' outputs are on their way while the weights are made
+        float4 held[kHeld];
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+            if (r + k * kRows < sh.count) held[k] = part_of(r + k * kRows);
         if (warp == 0) {
             const float2 v = join_ml(sp, sh, stride, gi, lane);
             for (int i = lane; i < sh.count; i += 32) {
@@ -722,16 +791,16 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
             }
         }
         __syncthreads();
-        constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes;
-        const int c = threadIdx.x % kLanes, r = threadIdx.x / kLanes;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = r; i < sh.count; i += kRows) {
+        auto add = [&](int i, const float4& t) {
             const float f = wgt[i];
-            if (f == 0.f) continue;
-            const float4 t =
-                *reinterpret_cast<const float4*>(sp.part_o + ((int64_t)sh.slot(i) * stride + gi) * D + c * 4);
+            if (f == 0.f) return;  // nothing but -inf there: its sums may be anything
             o.x += f * t.x, o.y += f * t.y, o.z += f * t.z, o.w += f * t.w;
-        }
+        };
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+            if (r + k * kRows < sh.count) add(r + k * kRows, held[k]);
+        for (int i = r + kHeld * kRows; i < sh.count; i += kRows) add(i, part_of(i));
         reinterpret_cast<float4*>(part)[threadIdx.x] = o;
         __syncthreads();
         if (r == 0) {
@@ -802,12 +871,16 @@ bool cache_map(CUtensorMap* m, const void* base, int32_t dtype, int32_t d, int32
 
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
-// Split of a call and its workspace layout; returns the bytes.
+constexpr int kSmallGroup = 16;  // query heads per KV head up to which 4 warps do (16-bit)
+
+// Split of a call and its workspace layout; returns the bytes (SIZE_MAX: more
+// units than the 32-bit counts hold).
 size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_head_kv, int32_t d, int32_t dtype,
                 bool weights, char* ws, DecodeSplit* sp) {
     const int G = n_head / n_head_kv;
-    const int warps = dtype == 0 && d == 128 ? Layout<0, 128>::kWarps : Layout<2, 128>::kWarps;
-    sp->pass_heads = warps * kHeads;
+    sp->pass_heads = dtype == 0 ? (d == 128 ? Layout<0, 128, 4>::kPass : Layout<0, 64, 8>::kPass)
+                     : G <= kSmallGroup ? Layout<2, 128, 4>::kPass
+                                        : Layout<2, 128, 8>::kPass;
     const int in_pass = G < sp->pass_heads ? G : sp->pass_heads;
     int groups = 1;
     while (groups * kHeads < in_pass) groups *= 2;
@@ -815,8 +888,9 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
     sp->groups = groups;
     const int64_t all_runs = (int64_t)n_seq * n_head_kv * sp->passes;
     const int64_t units = units_of(max_kv_len), total = all_runs * units;
+    if (total > INT_MAX) return SIZE_MAX;
     sp->direct = all_runs <= kCtas && units <= kDirectUnits;
-    const int64_t ctas = sp->direct ? all_runs : (total + warps - 1) / warps;
+    const int64_t ctas = sp->direct ? all_runs : (total + kMinUnits - 1) / kMinUnits;
     sp->ctas = (int32_t)(ctas < kCtas ? ctas : kCtas);
     sp->score_stride = (int32_t)(units * kUnit);
     size_t at = 16;
@@ -825,10 +899,10 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
         at += up16(bytes);
         return ws + was;
     };
-    sp->per = reinterpret_cast<int64_t*>(ws);
+    sp->per = reinterpret_cast<int32_t*>(ws);
     const int stride = groups * kHeads;
     if (!sp->direct) {
-        sp->run_start = reinterpret_cast<int64_t*>(take(all_runs * sizeof(int64_t)));
+        sp->run_start = reinterpret_cast<int32_t*>(take(all_runs * sizeof(int32_t)));
         sp->part_ml = reinterpret_cast<float2*>(take((size_t)2 * sp->ctas * stride * sizeof(float2)));
         sp->part_o = reinterpret_cast<float*>(take((size_t)2 * sp->ctas * stride * d * sizeof(float)));
     }
@@ -839,52 +913,64 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
     return at;
 }
 
-template <int ET, int D, bool P3, int GH>
+template <int ET, int D, int W, bool P3, int GH>
 cudaError_t launch_t(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s) {
-    constexpr int kThreads = Layout<ET, D>::kThreads;
+    constexpr int kThreads = Layout<ET, D, W>::kThreads;
     CUtensorMap mk, mv;
     if (!cache_map(&mk, a.k, a.dtype, D, a.n_head_kv, a.kv.rows) ||
         !cache_map(&mv, a.v, a.dtype, D, a.n_head_kv, a.kv.rows))
         return cudaErrorInvalidValue;
-    const int smem = Layout<ET, D>::kBytes + 1024;
+    const int smem = Layout<ET, D, W>::kBytes + 1024;
     int dev = 0;
     cudaGetDevice(&dev);
     // one bit per device ordinal < 32 whose attribute is set
     static std::atomic<unsigned> set_mask{0};
     if (dev >= 32 || !(set_mask.load(std::memory_order_acquire) & (1u << dev))) {
-        const cudaError_t e = cudaFuncSetAttribute(k6a_decode<ET, D, P3, GH>,
+        const cudaError_t e = cudaFuncSetAttribute(k6a_decode<ET, D, W, P3, GH>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         if (dev < 32) set_mask.fetch_or(1u << dev, std::memory_order_release);
     }
-    k6a_decode<ET, D, P3, GH><<<sp.ctas, kThreads, smem, s>>>(mk, mv, a, sp);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || (sp.direct && !a.acc)) return e;
-    const int chunks = a.acc ? (a.kv.max_kv_len + kJoinRows - 1) / kJoinRows : 0;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.n_head + a.n_head_kv * chunks, a.kv.n_seq);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = s;
+    // both kernels may start before what precedes them on the stream has
+    // ended: they wait for it on the device
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
     cfg.attrs = &at;
     cfg.numAttrs = 1;
+    cfg.stream = s;
+    cfg.gridDim = dim3(sp.ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k6a_decode<ET, D, W, P3, GH>, mk, mv, a, sp);
+    if (e != cudaSuccess || (sp.direct && !a.acc)) return e;
+    const int chunks = a.acc ? (a.kv.max_kv_len + kJoinRows - 1) / kJoinRows : 0;
+    cfg.gridDim = dim3(a.n_head + a.n_head_kv * chunks, a.kv.n_seq);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, k6b_join<D>, a, sp);
+}
+
+template <int ET, int D, int W>
+cudaError_t launch_w(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s) {
+    if constexpr (ET == 2) {
+        if (a.out_dtype == 0) return launch_t<2, D, W, true, 8>(a, sp, s);
+    }
+    return launch_t<ET, D, W, false, 8>(a, sp, s);
 }
 
 template <int ET, int D>
 cudaError_t launch_d(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s) {
+    const int G = a.n_head / a.n_head_kv;
     if constexpr (ET == 0) {
-        const int G = a.n_head / a.n_head_kv;
-        if (G == 1) return launch_t<0, D, false, 1>(a, sp, s);
-        if (G == 2) return launch_t<0, D, false, 2>(a, sp, s);
-        if (G <= 4) return launch_t<0, D, false, 4>(a, sp, s);
-        return launch_t<0, D, false, 8>(a, sp, s);
-    } else if constexpr (ET == 1) {
-        return launch_t<1, D, false, 8>(a, sp, s);
+        constexpr int W = D == 128 ? 4 : 8;
+        if (G == 1) return launch_t<0, D, W, false, 1>(a, sp, s);
+        if (G == 2) return launch_t<0, D, W, false, 2>(a, sp, s);
+        if (G <= 4) return launch_t<0, D, W, false, 4>(a, sp, s);
+        return launch_t<0, D, W, false, 8>(a, sp, s);
     } else {
-        return a.out_dtype == 0 ? launch_t<2, D, true, 8>(a, sp, s) : launch_t<2, D, false, 8>(a, sp, s);
+        return G <= kSmallGroup ? launch_w<ET, D, 4>(a, sp, s) : launch_w<ET, D, 8>(a, sp, s);
     }
 }
 
