@@ -48,13 +48,18 @@ namespace {
 
 constexpr int kUnit = 32;      // cache rows per unit
 constexpr int kCtas = 148;     // one per SM
-constexpr int kHeads = 8;      // query heads per warp
 constexpr int kChunk = kUnit * 128;  // one 128-byte column block of a unit
 // Fewest units dealt to a CTA.
 #ifndef K6_MIN_UNITS
 #define K6_MIN_UNITS 4
 #endif
 constexpr int kMinUnits = K6_MIN_UNITS;
+// What a run costs a CTA besides its units (the merge of the warps' states),
+// in units: the ranges are equal in this measure.
+#ifndef K6_RUN_COST
+#define K6_RUN_COST 4
+#endif
+constexpr int kRunCost = K6_RUN_COST;
 constexpr int kLensOnChip = 1024;  // lengths a CTA keeps in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 // A call of at most this many units per run and one CTA per run skips the
@@ -64,13 +69,14 @@ constexpr int kDirectUnits = 16;
 struct DecodeSplit {
     int32_t ctas;      // grid
     int32_t direct;    // one CTA per run
-    int32_t pass_heads;  // query heads of a pass: 8 per consumer warp
+    int32_t pass_heads;  // query heads of a pass, at most
     int32_t passes;    // passes per KV head
-    int32_t groups;    // warps that share a unit (1, 2, 4, 8), 8 query heads each
+    int32_t groups;    // warps that share a unit (1, 2, 4, 8)
+    int32_t heads;     // query heads per warp
     int32_t score_stride;
     // workspace
-    int32_t* per;        // units per CTA
-    int32_t* run_start;  // [n_seq][Hkv][passes] first unit of each run
+    int32_t* per;        // cost per CTA
+    int32_t* run_start;  // [n_seq][Hkv][passes] where each run starts in the cost of all
     float* part_o;       // [2 ctas][groups * 8][D]
     float2* part_ml;     // [2 ctas][groups * 8] (maximum, sum), log2 units
     float* lse;          // [n_seq][n_head] log2 units, runs finished by one CTA
@@ -145,28 +151,29 @@ __device__ __forceinline__ void store4(void* out, int32_t dtype, int64_t i, floa
 }
 
 // ET 0 f32, 1 f16, 2 bf16; W consumer warps (and a producer).
-template <int ET, int D, int W>
+// HW query heads per warp.
+template <int ET, int D, int W, int HW>
 struct Layout {
     static constexpr int kEs = ET == 0 ? 4 : 2;
     static constexpr int kCols = D * kEs / 128;          // 128-byte column blocks of a row
     static constexpr int kHalf = kCols * kChunk;         // K (or V) of a unit
     static constexpr int kStage = 2 * kHalf;
     // A stage always falls to the same stream of warps (kStages is a multiple
-    // of W): a warp that found its stage full knows that the stage's earlier
+    // of the streams; f32 rows of 512 bytes have 4 stages and at most 4
+    // streams, of two warps or more): a warp that found its stage full knows that the stage's earlier
     // fill had landed, which the barrier's one phase bit cannot tell it.
     static constexpr int kWarps = W;
-    static constexpr int kThreads = (W + 1) * 32;
     static constexpr int kStages = (W == 4 && ET != 0 ? 196608 : 131072) / kStage;
-    static constexpr int kPass = W == 4 && ET != 0 ? 16 : W * kHeads;  // query heads of a pass
+    static constexpr int kPass = W == 4 ? 16 : W * (ET == 0 ? 4 : 8);  // query heads of a pass, at most
     static constexpr int kOffQ = kStages * kStage;       // [2][kPass][D] queries of a segment
     static constexpr int kQBytes = kPass * D * kEs;
-    static constexpr int kOffO = kOffQ + 2 * kQBytes;    // [kWarps][8 heads][D] merge buffer
-    static constexpr int kOffP = kOffO + kWarps * kHeads * D * 4;  // f32: [kWarps][32 keys][8 heads]
-    static constexpr int kOffMl = kOffP + (ET == 0 ? kWarps * kUnit * kHeads * 4 : 0);
-    static constexpr int kOffBar = kOffMl + 2 * kWarps * kHeads * 8;
+    static constexpr int kOffO = kOffQ + 2 * kQBytes;    // [kWarps][HW][D] merge buffer
+    static constexpr int kOffP = kOffO + kWarps * HW * D * 4;  // f32: [kWarps][32 keys][HW]
+    static constexpr int kOffMl = kOffP + (ET == 0 ? kWarps * kUnit * HW * 4 : 0);
+    static constexpr int kOffBar = kOffMl + 2 * kWarps * HW * 8;
     static constexpr int kOffLens = kOffBar + (2 * kStages + 4) * 8;
     static constexpr int kBytes = kOffLens + kLensOnChip * 4;
-    static_assert(kStages % kWarps == 0 && kBytes + 1024 <= 232448, "shared memory");
+    static_assert((kStages % kWarps == 0 || (ET == 0 && D == 128 && kStages == 4)) && kBytes + 1024 <= 232448, "shared memory");
 };
 
 static_assert(kUnit == 32, "a lane per row, a page holds whole units");
@@ -182,13 +189,14 @@ struct Lens {
 // Walks the segments (a run's part inside this CTA) of a CTA's units.
 struct Walk {
     int32_t s, run, u, n, units;  // sequence, run within it (h * passes + pass), next unit, length, units of the run
-    int32_t left;                 // units of the CTA not walked yet
-    int32_t first;                // the CTA's first unit in the order of all
+    int32_t left;                 // cost of the CTA's range from here on
+    int32_t at;                   // where the run starts in the cost of all
 
+    __device__ __forceinline__ int segment() const { return min(units - u, left); }
     __device__ __forceinline__ void advance(const DecodeArgs& a, const Lens& lens, int runs, int n_seg) {
-        u += n_seg;
-        left -= n_seg;
-        if (left == 0) return;
+        left -= n_seg + kRunCost;
+        if (left <= 0) return;
+        at += units + kRunCost;
         u = 0;
         if (++run < runs) return;
         run = 0;
@@ -200,17 +208,18 @@ struct Walk {
         if (units == 0) left = 0;
     }
 };
+__device__ __forceinline__ int cost_of(int units) { return units > 0 ? units + kRunCost : 0; }
 
 // This CTA's share of all runs' units (every warp on its own): lane i adds up
-// a 32nd of the sequences, the lane whose part holds the CTA's first unit
-// looks for its sequence.
+// a 32nd of the sequences, the lane whose part holds the start of the CTA's
+// range looks for its sequence.
 __device__ __forceinline__ Walk share_of(const DecodeArgs& a, const DecodeSplit& sp, const Lens& lens, int runs,
                                          int lane) {
     Walk w{};
     const int n_seq = a.kv.n_seq, part = (n_seq + 31) / 32;
     const int s0 = min(n_seq, lane * part), s1 = min(n_seq, s0 + part);
     int32_t mine = 0;
-    for (int s = s0; s < s1; ++s) mine += units_of(lens.at(a, s));
+    for (int s = s0; s < s1; ++s) mine += cost_of(units_of(lens.at(a, s)));
     mine *= runs;
     int32_t incl = mine;
     if (n_seq > 1) {
@@ -224,21 +233,25 @@ __device__ __forceinline__ Walk share_of(const DecodeArgs& a, const DecodeSplit&
     const int32_t per = max((int32_t)(((uint32_t)total + sp.ctas - 1) / (uint32_t)sp.ctas), kMinUnits);
     if (blockIdx.x == 0 && threadIdx.x == 0) *sp.per = per;
     if (total / per < (int)blockIdx.x) return w;  // (the product below stays under total)
-    w.first = per * blockIdx.x;
-    if (w.first >= total) return w;
-    w.left = min(per, total - w.first);
-    const bool here = mine > 0 && w.first >= incl - mine && w.first < incl;
+    const int32_t first = per * blockIdx.x;
+    if (first >= total) return w;
+    w.left = min(per, total - first);
+    const bool here = mine > 0 && first >= incl - mine && first < incl;
     if (here) {
-        int32_t off = w.first - (incl - mine);
+        int32_t off = first - (incl - mine);
         w.s = s0;
         for (;; ++w.s) {
             w.n = lens.at(a, w.s);
             w.units = units_of(w.n);
-            if (off < w.units * runs) break;
-            off -= w.units * runs;
+            if (off < cost_of(w.units) * runs) break;
+            off -= cost_of(w.units) * runs;
         }
-        w.run = (int32_t)((uint32_t)off / (uint32_t)w.units);
-        w.u = off - w.run * w.units;
+        w.run = (int32_t)((uint32_t)off / (uint32_t)cost_of(w.units));
+        off -= w.run * cost_of(w.units);
+        // a run's cost comes before its units
+        w.at = first - off;
+        w.u = max(0, off - kRunCost);
+        w.left -= max(0, kRunCost - off);
     }
     const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
     w.s = __shfl_sync(0xffffffffu, w.s, from);
@@ -246,16 +259,32 @@ __device__ __forceinline__ Walk share_of(const DecodeArgs& a, const DecodeSplit&
     w.units = __shfl_sync(0xffffffffu, w.units, from);
     w.run = __shfl_sync(0xffffffffu, w.run, from);
     w.u = __shfl_sync(0xffffffffu, w.u, from);
+    w.at = __shfl_sync(0xffffffffu, w.at, from);
+    w.left = __shfl_sync(0xffffffffu, w.left, from);
     return w;
 }
+
+// The weights of one key for a warp's heads (f32).
+template <int GH>
+struct PVec {
+    using type = float4;
+};
+template <>
+struct PVec<2> {
+    using type = float2;
+};
+template <>
+struct PVec<1> {
+    using type = float;
+};
 
 // Overwrites what TMA brought of a sequence's last rows [from, 32) of a unit:
 // row `fresh` (>= 0) from the new token's K and V, V rows from `lim` on with
 // zeros (their P is 0, and 0 * NaN is not 0).
-template <int ET, int D, int W>
+template <int ET, int D>
 __device__ __forceinline__ void patch_unit(unsigned char* stage, int lane, int lim, int fresh, const char* kn,
                                            const char* vn) {
-    using LY = Layout<ET, D, W>;
+    using LY = Layout<ET, D, 8, 1>;
     constexpr int nc = LY::kCols * 8;  // 16-byte chunks per row
     auto at = [&](unsigned char* base, int r, int c) {
         return reinterpret_cast<uint4*>(base + (c >> 3) * kChunk + r * 128 + (((c & 7) ^ (r & 7)) << 4));
@@ -272,12 +301,13 @@ __device__ __forceinline__ void patch_unit(unsigned char* stage, int lane, int l
 }
 
 template <int ET, int D, int W, bool P3, int GH>
-__global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
+__global__ void __launch_bounds__((W + 1) * 32, 1)
     k6a_decode(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
                const DecodeSplit sp) {
-    using LY = Layout<ET, D, W>;
+    constexpr int kHeads = ET == 0 ? GH : 8;  // query heads per warp
+    using LY = Layout<ET, D, W, kHeads>;
     constexpr bool BF16 = ET == 2;
-    constexpr int kWarps = LY::kWarps, kThreads = LY::kThreads, kPass = LY::kPass;
+    constexpr int kWarps = LY::kWarps, kThreads = (W + 1) * 32, kPass = LY::kPass;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
@@ -315,7 +345,6 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
         w0.n = batch_len(a.kv, w0.s, a.err);
         w0.units = units_of(w0.n);
         w0.left = w0.units;
-        w0.first = 0;
         __syncthreads();
     } else {
         if (a.kv.n_seq <= kLensOnChip) {
@@ -325,7 +354,7 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
         __syncthreads();
         w0 = share_of(a, sp, lens, runs, lane);
     }
-    if (w0.left == 0) {
+    if (w0.left <= 0) {
         if (sp.direct) {  // a sequence without rows
             const int g0 = (w0.run % sp.passes) * kPass, n = min(kPass, G - g0) * (D / 4);
             const int64_t at = ((int64_t)w0.s * a.n_head + (w0.run / sp.passes) * G + g0) * D;
@@ -345,7 +374,7 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
         int seg = 0;
         const uint64_t policy = tc::policy_evict_first();  // the cache is read once
         for (; w.left > 0 && ok; ++seg) {
-            const int n_seg = min(w.units - w.u, w.left);
+            const int n_seg = w.segment();
             const int h = w.run / sp.passes, pass = w.run % sp.passes;
             if (lane == 0) {
                 const int b = seg & 1;
@@ -412,7 +441,7 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
     int it = 0;
     bool ok = true;
     for (int seg = 0; w.left > 0; ++seg) {
-        const int n_seg = min(w.units - w.u, w.left);
+        const int n_seg = w.segment();
         const int h = w.run / sp.passes, pass = w.run % sp.passes;
         const int g0 = pass * kPass + grp * kHeads;  // this warp's first query head of the group
         const int64_t q_row = (int64_t)w.s * a.n_head + (int64_t)h * G;
@@ -457,7 +486,7 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
                 const int64_t nr = ((int64_t)w.s * Hkv + h) * D * LY::kEs;
                 const char* kn = static_cast<const char*>(a.k_new) + nr;
                 const char* vn = static_cast<const char*>(a.v_new) + nr;
-                if (fresh || lim < kUnit) patch_unit<ET, D, W>(stage, lane, lim, fresh ? lim - 1 : -1, kn, vn);
+                if (fresh || lim < kUnit) patch_unit<ET, D>(stage, lane, lim, fresh ? lim - 1 : -1, kn, vn);
                 if (fresh && grp == 0 && pass == 0) {
                     const int row = batch_row(a.kv, w.s, w.n - 1, a.err);
                     constexpr int nc = D * LY::kEs / 16;
@@ -547,7 +576,7 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
                 }
             } else {
                 // S: one key per lane
-                float x[GH];
+                alignas(16) float x[GH];
 #pragma unroll
                 for (int g = 0; g < GH; ++g) x[g] = 0.f;
                 const float4* q4 = reinterpret_cast<const float4*>(qs);  // (heads past the group: any values, not used)
@@ -591,8 +620,9 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
                 for (int g = 0; g < GH; ++g) {
                     x[g] = ex2(x[g] - (m[g] == -INFINITY ? 0.f : m[g]));
                     l[g] += x[g];
-                    ps[lane * kHeads + g] = x[g];
                 }
+                using Vec = typename PVec<GH>::type;
+                reinterpret_cast<Vec*>(ps)[lane] = *reinterpret_cast<const Vec*>(x);
                 __syncwarp();
                 // O: D / 32 columns per lane, over the unit's keys
                 constexpr int NC = D / 32;
@@ -610,12 +640,12 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
                         const float2 t = *reinterpret_cast<const float2*>(vp);
                         vv[0] = t.x, vv[1] = t.y;
                     }
+                    alignas(16) float p[GH];
+                    *reinterpret_cast<Vec*>(p) = reinterpret_cast<const Vec*>(ps)[j];
 #pragma unroll
-                    for (int g = 0; g < GH; ++g) {
-                        const float p = ps[j * kHeads + g];
+                    for (int g = 0; g < GH; ++g)
 #pragma unroll
-                        for (int e = 0; e < NC; ++e) o[g * NC + e] = fmaf(p, vv[e], o[g * NC + e]);
-                    }
+                        for (int e = 0; e < NC; ++e) o[g * NC + e] = fmaf(p[g], vv[e], o[g * NC + e]);
                 }
                 __syncwarp();
             }
@@ -667,7 +697,7 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
         }
         tc::named_bar_sync(1, kWarps * 32);
         const bool whole = w.u == 0 && n_seg == w.units;
-        const int n_heads = min(groups * kHeads, G - pass * kPass);
+        const int n_heads = min(min(groups * kHeads, kPass), G - pass * kPass);
         const int slot = blockIdx.x * 2 + (seg == 0 ? 0 : 1);
         for (int j = threadIdx.x; j < n_heads * (D / 4); j += kWarps * 32) {
             const int g = j / (D / 4), c = j % (D / 4), gw = g / kHeads, gh = g % kHeads;
@@ -702,7 +732,7 @@ __global__ void __launch_bounds__(Layout<ET, D, W>::kThreads, 1)
                 if (c == 0) sp.part_ml[p] = make_float2(ms, lt);
             }
         }
-        if (w.u == 0 && !sp.direct && threadIdx.x == 0) sp.run_start[(int64_t)w.s * runs + w.run] = w0.first + it;
+        if (w.u == 0 && !sp.direct && threadIdx.x == 0) sp.run_start[(int64_t)w.s * runs + w.run] = w.at;
         it += n_seg;
         w.advance(a, lens, runs, n_seg);
     }
@@ -716,14 +746,9 @@ struct Shares {
         return 2 * c + (i == 0 && start > c * per ? 1 : 0);
     }
 };
-__device__ __forceinline__ Shares shares_of(const DecodeSplit& sp, int64_t run, int units) {
-    Shares r{1, 0, 0, 1};
-    if (sp.direct) return r;
-    r.per = *sp.per;
-    r.start = sp.run_start[run];
-    r.c0 = r.start / r.per;
-    r.count = (r.start + units - 1) / r.per - r.c0 + 1;
-    return r;
+__device__ __forceinline__ Shares shares_of(int32_t per, int32_t start, int units) {
+    const int u0 = start + kRunCost, c0 = u0 / per;  // the first unit comes after the run's cost
+    return {per, start, c0, (u0 + units - 1) / per - c0 + 1};
 }
 
 // Maximum and sum of one head over its shares (a warp; the same in every lane).
@@ -757,20 +782,22 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
     __shared__ float part[kJoinThreads * 4];
     __shared__ float lse[128];
     const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int G = a.n_head / a.n_head_kv, runs = a.n_head_kv * sp.passes, stride = sp.groups * kHeads;
+    const int G = a.n_head / a.n_head_kv, runs = a.n_head_kv * sp.passes, stride = sp.groups * sp.heads;
     tc::pdl_wait();
     tc::pdl_launch();
-    const int n = batch_len(a.kv, s, a.err), units = units_of(n);
     if ((int)blockIdx.x < a.n_head) {
+        if (sp.direct) return;
         const int hq = blockIdx.x, h = hq / G, g = hq % G, pass = g / sp.pass_heads;
         const int64_t out = ((int64_t)s * a.n_head + hq) * D;
-        if (sp.direct) return;
+        // (a run that was not walked has no start: read, but not used, when n is 0)
+        const int32_t per = *sp.per, start = sp.run_start[(int64_t)s * runs + h * sp.passes + pass];
+        const int n = batch_len(a.kv, s, a.err), units = units_of(n);
         if (n == 0) {
             for (int i = threadIdx.x; i < D / 4; i += kJoinThreads)
                 store4(a.out, a.out_dtype, out + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
             return;
         }
-        const Shares sh = shares_of(sp, (int64_t)s * runs + h * sp.passes + pass, units);
+        const Shares sh = shares_of(per, start, units);
         if (sh.count == 1) return;
         const int gi = g % sp.pass_heads;
         constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes, kHeld = 4;
@@ -814,10 +841,13 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
     }
     const int id = blockIdx.x - a.n_head, chunks = (gridDim.x - a.n_head) / a.n_head_kv;
     const int h = id / chunks, j0 = (id % chunks) * kJoinRows;
+    const int n = batch_len(a.kv, s, a.err), units = units_of(n);
     if (j0 >= n) return;
+    const int32_t per = sp.direct ? 1 : *sp.per;
     for (int g = warp; g < G; g += kJoinThreads / 32) {
         const int pass = g / sp.pass_heads;
-        const Shares sh = shares_of(sp, (int64_t)s * runs + h * sp.passes + pass, units);
+        const Shares sh = sp.direct ? Shares{1, 0, 0, 1}
+                                    : shares_of(per, sp.run_start[(int64_t)s * runs + h * sp.passes + pass], units);
         float x;
         if (sh.count == 1) {
             x = sp.lse[(int64_t)s * a.n_head + h * G + g];
@@ -830,10 +860,25 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
     __syncthreads();
     const float* sc = sp.scores + ((int64_t)s * a.n_head + (int64_t)h * G) * sp.score_stride;
     float* acc = a.acc + ((int64_t)s * a.n_head_kv + h) * a.acc_stride;
-    for (int j = j0 + threadIdx.x; j < min(n, j0 + kJoinRows); j += kJoinThreads) {
-        float w = 0.f;
-        for (int g = 0; g < G; ++g) w += ex2(sc[(int64_t)g * sp.score_stride + j] - lse[g]);
-        acc[j] += w;
+    // four rows a thread, two heads at a time: eight loads under way
+    constexpr int kR = kJoinRows / kJoinThreads;
+    const int end = min(n, j0 + kJoinRows);
+    float w[kR] = {};
+    int j[kR];
+#pragma unroll
+    for (int k = 0; k < kR; ++k) j[k] = min(j0 + (int)threadIdx.x + k * kJoinThreads, end - 1);
+#pragma unroll 2
+    for (int g = 0; g < G; ++g) {
+        float x[kR];
+#pragma unroll
+        for (int k = 0; k < kR; ++k) x[k] = sc[(int64_t)g * sp.score_stride + j[k]];
+#pragma unroll
+        for (int k = 0; k < kR; ++k) w[k] += ex2(x[k] - lse[g]);
+    }
+#pragma unroll
+    for (int k = 0; k < kR; ++k) {
+        const int r = j0 + threadIdx.x + k * kJoinThreads;
+        if (r < end) acc[r] += w[k];
     }
 }
 
@@ -878,16 +923,23 @@ constexpr int kSmallGroup = 16;  // query heads per KV head up to which 4 warps 
 size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_head_kv, int32_t d, int32_t dtype,
                 bool weights, char* ws, DecodeSplit* sp) {
     const int G = n_head / n_head_kv;
-    sp->pass_heads = dtype == 0 ? (d == 128 ? Layout<0, 128, 4>::kPass : Layout<0, 64, 8>::kPass)
-                     : G <= kSmallGroup ? Layout<2, 128, 4>::kPass
-                                        : Layout<2, 128, 8>::kPass;
+    if (dtype == 0) {
+        // 4 heads per warp keep a unit's latency low; rows of 512 bytes want
+        // two warps per unit at least (4 stages)
+        sp->pass_heads = 32;
+        const int least = d == 128 ? 2 : 1;
+        sp->heads = G <= least ? 1 : G <= 2 * least ? 2 : 4;
+        sp->groups = least;
+    } else {
+        sp->pass_heads = G <= kSmallGroup ? 16 : 64;
+        sp->heads = 8;
+        sp->groups = 1;
+    }
     const int in_pass = G < sp->pass_heads ? G : sp->pass_heads;
-    int groups = 1;
-    while (groups * kHeads < in_pass) groups *= 2;
+    while (sp->groups * sp->heads < in_pass) sp->groups *= 2;
     sp->passes = (G + sp->pass_heads - 1) / sp->pass_heads;
-    sp->groups = groups;
     const int64_t all_runs = (int64_t)n_seq * n_head_kv * sp->passes;
-    const int64_t units = units_of(max_kv_len), total = all_runs * units;
+    const int64_t units = units_of(max_kv_len), total = all_runs * (units + kRunCost);
     if (total > INT_MAX) return SIZE_MAX;
     sp->direct = all_runs <= kCtas && units <= kDirectUnits;
     const int64_t ctas = sp->direct ? all_runs : (total + kMinUnits - 1) / kMinUnits;
@@ -900,7 +952,7 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
         return ws + was;
     };
     sp->per = reinterpret_cast<int32_t*>(ws);
-    const int stride = groups * kHeads;
+    const int stride = sp->groups * sp->heads;
     if (!sp->direct) {
         sp->run_start = reinterpret_cast<int32_t*>(take(all_runs * sizeof(int32_t)));
         sp->part_ml = reinterpret_cast<float2*>(take((size_t)2 * sp->ctas * stride * sizeof(float2)));
@@ -915,12 +967,12 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
 
 template <int ET, int D, int W, bool P3, int GH>
 cudaError_t launch_t(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s) {
-    constexpr int kThreads = Layout<ET, D, W>::kThreads;
+    constexpr int kThreads = (W + 1) * 32;
     CUtensorMap mk, mv;
     if (!cache_map(&mk, a.k, a.dtype, D, a.n_head_kv, a.kv.rows) ||
         !cache_map(&mv, a.v, a.dtype, D, a.n_head_kv, a.kv.rows))
         return cudaErrorInvalidValue;
-    const int smem = Layout<ET, D, W>::kBytes + 1024;
+    const int smem = Layout<ET, D, W, ET == 0 ? GH : 8>::kBytes + 1024;
     int dev = 0;
     cudaGetDevice(&dev);
     // one bit per device ordinal < 32 whose attribute is set
@@ -964,11 +1016,9 @@ template <int ET, int D>
 cudaError_t launch_d(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s) {
     const int G = a.n_head / a.n_head_kv;
     if constexpr (ET == 0) {
-        constexpr int W = D == 128 ? 4 : 8;
-        if (G == 1) return launch_t<0, D, W, false, 1>(a, sp, s);
-        if (G == 2) return launch_t<0, D, W, false, 2>(a, sp, s);
-        if (G <= 4) return launch_t<0, D, W, false, 4>(a, sp, s);
-        return launch_t<0, D, W, false, 8>(a, sp, s);
+        if (sp.heads == 1) return launch_t<0, D, 8, false, 1>(a, sp, s);
+        if (sp.heads == 2) return launch_t<0, D, 8, false, 2>(a, sp, s);
+        return launch_t<0, D, 8, false, 4>(a, sp, s);
     } else {
         return G <= kSmallGroup ? launch_w<ET, D, 4>(a, sp, s) : launch_w<ET, D, 8>(a, sp, s);
     }

@@ -200,18 +200,32 @@ def device_view(ptr: int, shape, dtype: int):
     return t.view(torch.bfloat16) if dtype == BF16 else t
 
 
-_DTYPE_NAMES = {F32: "torch.float32", F16: "torch.float16", BF16: "torch.bfloat16"}
+def _torch_dtypes():
+    import torch
+
+    return {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16, "i32": torch.int32}
+
+
+_DTYPES: dict = {}  # the torch types of F32, F16, BF16 and "i32", filled by the first batch or context call
+
+
+def _dtype(code):
+    if not _DTYPES:
+        _DTYPES.update(_torch_dtypes())
+    return _DTYPES[code]
 
 
 def _check(name, t, dtype, shape, device):
-    """The library sees plain pointers: what a tensor is must be checked here.  A shape entry None is any size."""
-    if str(t.dtype) != dtype:
+    """The library sees plain pointers: what a tensor is must be checked here.  The trailing dimensions are `shape`
+    (an entry None is any size)."""
+    if t.dtype is not dtype:
         raise ValueError(f"{name} is {t.dtype}, not {dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name} is not contiguous (strides {tuple(t.stride())})")
-    if t.device.type != "cuda" or t.device.index != device:
+    if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, not cuda:{device}")
-    if len(t.shape) != len(shape) or any(w is not None and h != w for h, w in zip(t.shape, shape)):
+    if t.shape != shape and (len(t.shape) != len(shape)
+                             or any(w is not None and h != w for h, w in zip(t.shape, shape))):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
 
 
@@ -227,14 +241,14 @@ class KvBatch:
             raise ValueError("a batch without kv_lens needs n_seq")
         self.n_seq = int(n_seq) if n_seq is not None else kv_lens.shape[0]
         self.kv_lens, self.block_tables = kv_lens, block_tables
-        self.device = None if ref is None else ref.device.index
+        self.device = None if ref is None else ref.get_device()
         if kv_lens is not None:
-            _check("kv_lens", kv_lens, "torch.int32", (self.n_seq,), self.device)
+            _check("kv_lens", kv_lens, _dtype("i32"), (self.n_seq,), self.device)
         entries = 0
         if block_rows:
             if block_tables is None:
                 raise ValueError("block_rows without block_tables")
-            _check("block_tables", block_tables, "torch.int32", (self.n_seq, None), self.device)
+            _check("block_tables", block_tables, _dtype("i32"), (self.n_seq, None), self.device)
             entries = block_tables.shape[1]
         self.rows = pool_rows if block_rows else self.n_seq * seq_rows
         self.desc = KvBatchDesc(self.n_seq, max_kv_len, _ptr(kv_lens), _ptr(block_tables) if block_rows else None,
@@ -405,16 +419,19 @@ class Context:
         c = self.cfg
         if kv.device is not None and kv.device != c.device:
             raise ValueError(f"the batch is on cuda:{kv.device}, not cuda:{c.device}")
-        shape, dt = (None, c.n_head_kv, c.head_dim), _DTYPE_NAMES[c.dtype]
+        dt, heads, d, need = _dtype(c.dtype), c.n_head_kv, c.head_dim, kv.rows * c.n_head_kv * c.head_dim
         for name, t in zip(what, (k, v)):
-            _check(name, t.flatten(0, -3) if t.dim() > 3 and t.is_contiguous() else t, dt, shape, c.device)
-            if t.numel() < kv.rows * c.n_head_kv * c.head_dim:
+            # rows in any number of leading dimensions
+            if (t.dtype is not dt or t.get_device() != c.device or not t.is_contiguous()
+                    or t.shape[-2:] != (heads, d)):
+                _check(name, t, dt, t.shape[:-2] + (heads, d), c.device)
+            if t.numel() < need:
                 raise ValueError(f"{name} holds fewer than the batch's {kv.rows} rows")
 
     def _workspace(self, t):
         if t is None:
             return None, 0
-        if not t.is_contiguous() or t.device.index != self.cfg.device:
+        if not t.is_contiguous() or t.get_device() != self.cfg.device:
             raise ValueError(f"the workspace must be a contiguous tensor on cuda:{self.cfg.device}")
         return t.data_ptr(), t.numel() * t.element_size()
 
@@ -428,15 +445,15 @@ class Context:
         [head_dim]; acc f32 [n_seq][n_head_kv][stride].  Raises ValueError for a tensor of another type, shape,
         layout or device; returns the status code."""
         c = self.cfg
-        dt = _DTYPE_NAMES[c.dtype]
+        dt = _dtype(c.dtype)
         self._cache_tensors(kv, k, v)
         _check("q", q, dt, (kv.n_seq, c.n_head, c.head_dim), c.device)
-        _check("out", out, _DTYPE_NAMES[c.out_dtype], (kv.n_seq, c.n_head, c.head_dim), c.device)
+        _check("out", out, _dtype(c.out_dtype), (kv.n_seq, c.n_head, c.head_dim), c.device)
         for name, t in (("k_new", k_new), ("v_new", v_new)):
             if t is not None:
                 _check(name, t, dt, (kv.n_seq, c.n_head_kv, c.head_dim), c.device)
         if acc is not None:
-            _check("acc", acc, "torch.float32", (kv.n_seq, c.n_head_kv, None), c.device)
+            _check("acc", acc, _dtype(F32), (kv.n_seq, c.n_head_kv, None), c.device)
         ws, n = self._workspace(workspace)
         return lib.ep_sp_decode_layer(self.h, layer, kv.ref, q.data_ptr(), _ptr(k_new), _ptr(v_new), k.data_ptr(),
                                       v.data_ptr(), out.data_ptr(), _ptr(acc), 0 if acc is None else acc.shape[-1],
@@ -450,12 +467,12 @@ class Context:
     def prompt_weights(self, layer, q, k, kv_len, n_tok, row_begin, acc, workspace, accumulate=False, stream=None):
         """q [n_tok][n_head][head_dim]; k the cache (paged under set_paged_kv); acc f32 [n_head_kv][stride]."""
         c = self.cfg
-        dt = _DTYPE_NAMES[c.dtype]
+        dt = _dtype(c.dtype)
         _check("q", q, dt, (n_tok, c.n_head, c.head_dim), c.device)
         _check("k", k, dt, (None, c.n_head_kv, c.head_dim), c.device)
         if k.shape[0] < (self._pool_rows or kv_len):
             raise ValueError(f"k holds {k.shape[0]} rows, the call reads {self._pool_rows or kv_len}")
-        _check("acc", acc, "torch.float32", (c.n_head_kv, None), c.device)
+        _check("acc", acc, _dtype(F32), (c.n_head_kv, None), c.device)
         ws, n = self._workspace(workspace)
         return lib.ep_sp_prompt_weights(self.h, layer, q.data_ptr(), k.data_ptr(), kv_len, n_tok, row_begin,
                                         1 if accumulate else 0, acc.data_ptr(), acc.shape[-1], ws, n,
@@ -473,13 +490,13 @@ class Context:
         c = self.cfg
         self._cache_tensors(src, k, v)
         self._cache_tensors(dst, k_dst, v_dst, ("k_dst", "v_dst"))
-        _check("acc", acc, "torch.float32", (src.n_seq, c.n_head_kv, None), c.device)
+        _check("acc", acc, _dtype(F32), (src.n_seq, c.n_head_kv, None), c.device)
         if acc_dst is not None:
-            _check("acc_dst", acc_dst, "torch.float32", (src.n_seq, c.n_head_kv, None), c.device)
+            _check("acc_dst", acc_dst, _dtype(F32), (src.n_seq, c.n_head_kv, None), c.device)
         if new_lens is not None:
-            _check("new_lens", new_lens, "torch.int32", (src.n_seq,), c.device)
+            _check("new_lens", new_lens, _dtype("i32"), (src.n_seq,), c.device)
         if kept_rows is not None:
-            _check("kept_rows", kept_rows, "torch.int32", (src.n_seq, c.n_head_kv, n_keep), c.device)
+            _check("kept_rows", kept_rows, _dtype("i32"), (src.n_seq, c.n_head_kv, n_keep), c.device)
         ws, n = self._workspace(workspace)
         return lib.ep_sp_evict_layer(self.h, layer, src.ref, k.data_ptr(), v.data_ptr(), acc.data_ptr(),
                                      acc.shape[-1], n_keep, sink_rows, recent_rows, dst.ref, k_dst.data_ptr(),
