@@ -36,6 +36,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cstdint>
@@ -77,6 +78,7 @@ struct DecodeSplit {
     // workspace
     int32_t* per;        // cost per CTA
     int32_t* run_start;  // [n_seq][Hkv][passes] where each run starts in the cost of all
+    int4* cut;           // [ctas] (sequence, run, start, units) of a run that goes on past the CTA it began in; -1: none
     float* part_o;       // [2 ctas][groups * 8][D]
     float2* part_ml;     // [2 ctas][groups * 8] (maximum, sum), log2 units
     float* lse;          // [n_seq][n_head] log2 units, runs finished by one CTA
@@ -353,6 +355,12 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
         }
         __syncthreads();
         w0 = share_of(a, sp, lens, runs, lane);
+        // sequences without rows, dealt out to the CTAs
+        for (int s = blockIdx.x; s < a.kv.n_seq; s += gridDim.x)
+            if (lens.at(a, s) == 0)
+                for (int i = threadIdx.x; i < a.n_head * (D / 4); i += kThreads)
+                    store4(a.out, a.out_dtype, (int64_t)s * a.n_head * D + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+        if (w0.left <= 0 && threadIdx.x == 0) sp.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
     if (w0.left <= 0) {
         if (sp.direct) {  // a sequence without rows
@@ -732,7 +740,11 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                 if (c == 0) sp.part_ml[p] = make_float2(ms, lt);
             }
         }
-        if (w.u == 0 && !sp.direct && threadIdx.x == 0) sp.run_start[(int64_t)w.s * runs + w.run] = w.at;
+        if (!sp.direct && threadIdx.x == 0) {
+            if (w.u == 0) sp.run_start[(int64_t)w.s * runs + w.run] = w.at;
+            // the CTA's last segment has the last word
+            sp.cut[blockIdx.x] = w.u == 0 && n_seg < w.units ? make_int4(w.s, w.run, w.at, w.units) : make_int4(-1, 0, 0, 0);
+        }
         it += n_seg;
         w.advance(a, lens, runs, n_seg);
     }
@@ -773,33 +785,29 @@ __device__ __forceinline__ float2 join_ml(const DecodeSplit& sp, const Shares& s
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 1024;  // cache rows per weights CTA
 
-// Grid (n_head + [weights] Hkv * chunks, n_seq): the first n_head CTAs of a
-// sequence put together the outputs of runs that several CTAs shared, the
-// others add the weights of kJoinRows rows of one KV head.
+// The first ctas * heads CTAs put together the outputs of the runs that several
+// CTAs shared (one CTA per query head of a run; at most one such run begins in
+// a CTA of k6a); the others, [n_seq][Hkv][chunks], add the weights of kJoinRows
+// rows of one KV head.
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, const DecodeSplit sp) {
+__global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, const DecodeSplit sp, int heads,
+                                                         int chunks) {
     __shared__ float wgt[kCtas];
     __shared__ float part[kJoinThreads * 4];
     __shared__ float lse[128];
-    const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = a.n_head / a.n_head_kv, runs = a.n_head_kv * sp.passes, stride = sp.groups * sp.heads;
+    const int joins = sp.direct ? 0 : sp.ctas * heads;
     tc::pdl_wait();
     tc::pdl_launch();
-    if ((int)blockIdx.x < a.n_head) {
-        if (sp.direct) return;
-        const int hq = blockIdx.x, h = hq / G, g = hq % G, pass = g / sp.pass_heads;
-        const int64_t out = ((int64_t)s * a.n_head + hq) * D;
-        // (a run that was not walked has no start: read, but not used, when n is 0)
-        const int32_t per = *sp.per, start = sp.run_start[(int64_t)s * runs + h * sp.passes + pass];
-        const int n = batch_len(a.kv, s, a.err), units = units_of(n);
-        if (n == 0) {
-            for (int i = threadIdx.x; i < D / 4; i += kJoinThreads)
-                store4(a.out, a.out_dtype, out + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-            return;
-        }
-        const Shares sh = shares_of(per, start, units);
-        if (sh.count == 1) return;
-        const int gi = g % sp.pass_heads;
+    if ((int)blockIdx.x < joins) {
+        const int4 cut = sp.cut[blockIdx.x / heads];
+        const int32_t per = *sp.per;
+        if (cut.x < 0) return;
+        const int gi = blockIdx.x % heads, h = cut.y / sp.passes, g = cut.y % sp.passes * sp.pass_heads + gi;
+        if (g >= G) return;
+        const int64_t out = ((int64_t)cut.x * a.n_head + h * G + g) * D;
+        const Shares sh = shares_of(per, cut.z, cut.w);
         constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes, kHeld = 4;
         const int c = threadIdx.x % kLanes, r = threadIdx.x / kLanes;
         auto part_of = [&](int i) {
@@ -839,8 +847,8 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
         }
         return;
     }
-    const int id = blockIdx.x - a.n_head, chunks = (gridDim.x - a.n_head) / a.n_head_kv;
-    const int h = id / chunks, j0 = (id % chunks) * kJoinRows;
+    const int id = blockIdx.x - joins, s = id / chunks / a.n_head_kv;
+    const int h = id / chunks % a.n_head_kv, j0 = (id % chunks) * kJoinRows;
     const int n = batch_len(a.kv, s, a.err), units = units_of(n);
     if (j0 >= n) return;
     const int32_t per = sp.direct ? 1 : *sp.per;
@@ -955,6 +963,7 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
     const int stride = sp->groups * sp->heads;
     if (!sp->direct) {
         sp->run_start = reinterpret_cast<int32_t*>(take(all_runs * sizeof(int32_t)));
+        sp->cut = reinterpret_cast<int4*>(take(sp->ctas * sizeof(int4)));
         sp->part_ml = reinterpret_cast<float2*>(take((size_t)2 * sp->ctas * stride * sizeof(float2)));
         sp->part_o = reinterpret_cast<float*>(take((size_t)2 * sp->ctas * stride * d * sizeof(float)));
     }
@@ -998,10 +1007,13 @@ cudaError_t launch_t(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s)
     const cudaError_t e = cudaLaunchKernelEx(&cfg, k6a_decode<ET, D, W, P3, GH>, mk, mv, a, sp);
     if (e != cudaSuccess || (sp.direct && !a.acc)) return e;
     const int chunks = a.acc ? (a.kv.max_kv_len + kJoinRows - 1) / kJoinRows : 0;
-    cfg.gridDim = dim3(a.n_head + a.n_head_kv * chunks, a.kv.n_seq);
+    const int heads = std::min(a.n_head / a.n_head_kv, sp.pass_heads);
+    const int64_t grid = (sp.direct ? 0 : sp.ctas * heads) + (int64_t)a.kv.n_seq * a.n_head_kv * chunks;
+    if (grid > INT_MAX) return cudaErrorInvalidValue;
+    cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, k6b_join<D>, a, sp);
+    return cudaLaunchKernelEx(&cfg, k6b_join<D>, a, sp, heads, chunks);
 }
 
 template <int ET, int D, int W>

@@ -209,6 +209,14 @@ def _torch_dtypes():
 _DTYPES: dict = {}  # the torch types of F32, F16, BF16 and "i32", filled by the first batch or context call
 
 
+def _current_stream(device):
+    """The raw current stream of a device (the direct query where torch has it: a tenth of the time)."""
+    import torch
+
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def _dtype(code):
     if not _DTYPES:
         _DTYPES.update(_torch_dtypes())
@@ -512,9 +520,7 @@ class Context:
     def _stream(self, stream):
         """The given stream, or the current one of the context's device."""
         if stream is None:
-            import torch
-
-            return torch.cuda.current_stream(self.cfg.device).cuda_stream
+            return _current_stream(self.cfg.device)
         return stream if isinstance(stream, int) else stream.cuda_stream
 
     def set_head_routing(self, mode, threshold):
