@@ -178,6 +178,7 @@ int32_t ep_sp_prompt_weights_bytes(const ep_sp_ctx* ctx, int32_t kv_len, int32_t
         return kInvalid;
     *bytes = epsp::weights_ws_bytes(kv_len, n_tok - row_begin, ctx->cfg.n_head, ctx->cfg.n_head_kv, ctx->cfg.head_dim,
                                     ctx->cfg.dtype);
+    if (*bytes == SIZE_MAX) return kInvalid;
     return kOk;
 }
 

@@ -7,15 +7,15 @@
 // Storing the scores instead would cost 8 bytes a pair; recomputing them costs
 // 2 d flops, which the tensor cores do in a quarter of the time the pair's two
 // exponentials take.  The exponentials bound both passes (16 MUFU results per
-// clock and SM).  Every key has one writer and a fixed order of additions.
+// clock and SM, a third of the pairs on the FMA pipe instead).  Every key has one writer and a fixed order of additions.
 //
 // 16-bit (tcgen05): a query tile packs T = 128 / G tokens x G heads into 128
 // rows.  The two passes are one kernel with the MMA operands exchanged: with
 // queries as the M side a thread (TMEM lane) owns a query row and reduces over
 // keys; with keys as the M side it owns a key and reduces over queries.  Both
 // reductions stay in the thread's registers, no shuffles.  One warp loads
-// tiles by TMA, one issues MMAs into 4 S buffers in TMEM, and 8 warps take
-// the exponentials, each warpgroup 64 of a tile's 128 columns.
+// tiles by TMA, one issues MMAs into 4 S buffers in TMEM, and 16 warps take
+// the exponentials.
 // f32: the same passes on the CUDA cores, 64 x 64 tiles, 4 x 4 per thread.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cstdint>
 
 #include "epsp_kernels.h"
 #include "tc100.cuh"
@@ -35,10 +36,45 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3f(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
+// 2^x of a pair on the FMA pipe.  x >= -126 (below: 2^-126; NaN stays) is split
+// into n + r, n = round(x), r in [-0.5, 0.5]: adding 1.5 * 2^23 + 127 leaves
+// n + 127 in the low mantissa bits, which shifted up are 2^n's bits.  2^r is a
+// polynomial of degree 5, fitted here for the least relative error on that
+// interval (7.5e-8, 2.4e-7 with f32 coefficients and steps: ex2's own error).
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+    const float2 t = __fadd2_rn(x, make_float2(12583039.f, 12583039.f));
+    const float2 n = __fadd2_rn(t, make_float2(-12583039.f, -12583039.f));
+    const float2 r = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 p = __ffma2_rn(make_float2(1.3276472454890609e-3f, 1.3276472454890609e-3f), r,
+                          make_float2(9.675540961325169e-3f, 9.675540961325169e-3f));
+    p = __ffma2_rn(p, r, make_float2(5.550713092088699e-2f, 5.550713092088699e-2f));
+    p = __ffma2_rn(p, r, make_float2(0.24022120237350464f, 0.24022120237350464f));
+    p = __ffma2_rn(p, r, make_float2(0.6931469440460205f, 0.6931469440460205f));
+    p = __ffma2_rn(p, r, make_float2(1.0000001192092896f, 1.0000001192092896f));
+    return __fmul2_rn(p, make_float2(__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23)));
+}
+
+// Exponentials of pair i of a run of pairs: one pair in kPolyEvery on the FMA
+// pipe, the rest on MUFU.
+#ifndef K7_POLY_EVERY
+#define K7_POLY_EVERY 3
+#endif
+constexpr int kPolyEvery = K7_POLY_EVERY;
+__device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
+    return i % kPolyEvery == kPolyEvery - 1 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+}
 
 // ---------------------------------------------------------- 16-bit: tcgen05 --
 constexpr int BM = 128;                 // rows of a query tile, keys of a key tile
-constexpr int kTcThreads = 384;         // producer, MMA, 2 idle warps, 2 x 4 softmax warps
+constexpr int kTcThreads = 640;         // producer, MMA, 2 idle warps, 4 x 4 softmax warps
 constexpr int kHalfTile = BM * 128;     // [128][64 x 16-bit], 128-byte swizzled
 constexpr int kMaxGroup = 4;            // query tiles a statistics CTA keeps on chip
 constexpr int kSBufs = 4;               // S tiles in TMEM (128 columns each)
@@ -48,8 +84,12 @@ template <int D>
 struct TcLayout {
     static constexpr int kTile = D / 64 * kHalfTile;
     static constexpr int kSlots = D == 128 ? 6 : 12;  // query + key tiles on chip
-    static constexpr int kOffStat = kSlots * kTile;   // float2 [2][kMaxGroup * BM] (A) / float [2][2][BM] (B)
-    static constexpr int kOffBar = kOffStat + 2 * kMaxGroup * BM * 8;
+    // statistics pass: float2 [4][kMaxGroup * BM]; sums pass: float
+    // [kSlots][BM] lse of the query tiles on chip, then [2][3][2][BM] sums
+    static constexpr int kOffStat = kSlots * kTile;
+    static constexpr int kOffRed = kOffStat + kSlots * BM * 4;
+    static constexpr int kOffBar = kOffStat + 4 * kMaxGroup * BM * 8;
+    static_assert(kOffRed + 2 * 3 * 2 * BM * 4 <= kOffBar, "sums pass");
     static constexpr int kBars = 2 * 12 + 2 * 12 + 2 * kSBufs + 1;
     static constexpr int kBytes = kOffBar + kBars * 8 + 32;
     static_assert(kBytes + 1024 <= 232448, "shared memory");
@@ -66,8 +106,8 @@ struct WeightPlan {
     int32_t q_slots, k_slots;  // sums pass
     int32_t kg;        // sums pass: key tiles a CTA works on at a time (1, 2)
     int32_t b_splits;  // sums pass: CTAs per KV head
-    float2* ml;        // [2 splits][Hkv][n_rt * 128]
-    float* lse;        // [Hkv][n_rt * 128], log2 units, +inf for rows that are none
+    float2* ml;        // [splits][Hkv][n_rt * 128]
+    float* nlse;       // [Hkv][n_rt * 128]: minus the lse, log2 units, -inf for rows that are none
 };
 
 // Barriers of a CTA.
@@ -129,11 +169,11 @@ __device__ __forceinline__ void issue_s(uint32_t tmem, int buf, const unsigned c
 }
 
 // 64 columns of S of this thread's lane; the buffer is handed back at once.
-__device__ __forceinline__ void take_s(uint32_t tmem, int buf, int wg, uint32_t lane_addr, uint64_t* se, int lane,
+__device__ __forceinline__ void take_s(uint32_t tmem, int buf, int half, uint32_t lane_addr, uint64_t* se, int lane,
                                        float (&s)[64]) {
     uint32_t u[2][32];
-    tc::tmem_ld32(tmem + lane_addr + buf * BM + wg * 64, u[0]);
-    tc::tmem_ld32(tmem + lane_addr + buf * BM + wg * 64 + 32, u[1]);
+    tc::tmem_ld32(tmem + lane_addr + buf * BM + half * 64, u[0]);
+    tc::tmem_ld32(tmem + lane_addr + buf * BM + half * 64 + 32, u[1]);
     tc::tmem_wait_ld();
 #pragma unroll
     for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(u[i >> 5][i & 31]);
@@ -144,11 +184,14 @@ __device__ __forceinline__ void take_s(uint32_t tmem, int buf, int wg, uint32_t 
 
 // PASS 0: statistics.  CTA (key split, group of query tiles, KV head): the
 // group's query tiles stay, key tiles stream; TMEM lane = query row, so each
-// thread keeps one row's maximum and sum over its half of a key tile's columns.
+// thread keeps the maximum and sum of one row over its columns.
 // PASS 1: sums.  CTA (slice of key tiles, KV head): TMEM lane = key, columns =
 // query rows, so each thread sums one key's weights in registers; key tiles
 // (kg at a time) against all query tiles, which stay when they fit and
 // stream otherwise.
+// A step is one (query tile, key tile); two warpgroups take the even steps,
+// two the odd ones, each 64 of the 128 columns: with four warps to a scheduler
+// one's loads and waits hide behind the others' exponentials.
 template <bool BF16, int D, int SEG, int PASS>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k7_pass(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -188,11 +231,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         stream_q = !p.resident;
     }
     unsigned char* kbase = smem + q_slots * LY::kTile;
+    float* lse_s = reinterpret_cast<float*>(smem + LY::kOffStat);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < q_slots; ++i) {
             tc::mbar_init(&b.qf[i], 1);
-            tc::mbar_init(&b.qe[i], 1);
+            tc::mbar_init(&b.qe[i], 17);  // the MMAs' commit and the 16 softmax warps
         }
         for (int i = 0; i < k_slots; ++i) {
             tc::mbar_init(&b.kf[i], 1);
@@ -219,8 +263,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             *(reinterpret_cast<uint4*>(smem + (i / n16) * kHalfTile + used * 128) + i % n16) = make_uint4(0, 0, 0, 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    tc::pdl_wait();
+    tc::pdl_launch();
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -243,9 +287,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 ++kt_n;
             };
             if (!stream_q) {
-                tc::mbar_arrive_expect_tx(&b.qf[0], q_bytes * n_q);
+                tc::mbar_arrive_expect_tx(&b.qf[0], (q_bytes + (PASS == 1 ? BM * 4 : 0)) * n_q);
                 for (int i = 0; i < n_q; ++i)
                     load_queries<D>(a, p, &tmQ, smem + i * LY::kTile, &b.qf[0], rt0 + i, h);
+                if constexpr (PASS == 1)
+                    tc::bulk_load(lse_s, p.nlse + (int64_t)h * p.n_rt * BM, BM * 4 * n_q, &b.qf[0]);
             }
             if constexpr (PASS == 0) {
                 for (int kt = k0; kt < k1 && ok; ++kt) keys(kt);
@@ -258,8 +304,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const int s = qt_n % q_slots;
                         ok = tc::mbar_wait(&b.qe[s], ((qt_n / q_slots) & 1) ^ 1, tmo);
                         if (!ok) break;
-                        tc::mbar_arrive_expect_tx(&b.qf[s], q_bytes);
+                        tc::mbar_arrive_expect_tx(&b.qf[s], q_bytes + BM * 4);
                         load_queries<D>(a, p, &tmQ, smem + s * LY::kTile, &b.qf[s], rt, h);
+                        tc::bulk_load(lse_s + s * BM, p.nlse + ((int64_t)h * p.n_rt + rt) * BM, BM * 4, &b.qf[s]);
                         ++qt_n;
                     }
                 }
@@ -329,85 +376,101 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
     } else if (warp >= 4) {
         // ------------------------------------------------------- softmax --
-        const int wg = (warp - 4) >> 2, wq = warp & 3, row = wq * 32 + lane;
+        const int wg = (warp - 4) >> 2, odd = wg >> 1, half = wg & 1, wq = warp & 3, row = wq * 32 + lane;
         const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
         const float sl2 = a.kq_scale * 1.4426950408889634f;
         const float2 sl2_2 = make_float2(sl2, sl2);
         bool ok = true;
-        int step = 0;
-        auto next = [&]() {  // the buffer of the next step, once it is full
-            const int buf = step % kSBufs;
+        auto wait = [&](uint64_t* bar, uint32_t par, int step) {
             if (ok) {
-                ok = __all_sync(0xffffffffu, tc::mbar_wait(&b.sf[buf], (step / kSBufs) & 1, tmo));
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(bar, par, tmo));
                 if (!ok && lane == 0) report_error(a.err, kDevWaitWeights, 0xb4 + PASS, step);
-                tc::fence_after_sync();
             }
-            ++step;
-            return buf;
+            return ok;
         };
         if constexpr (PASS == 0) {
-            float2* stat = reinterpret_cast<float2*>(smem + LY::kOffStat) + wg * kMaxGroup * BM + row;
+            float2* stats = reinterpret_cast<float2*>(smem + LY::kOffStat);
+            float2* stat = stats + wg * kMaxGroup * BM + row;
             for (int r = 0; r < n_q; ++r) stat[r * BM] = make_float2(-INFINITY, 0.f);
-            for (int kt = k0; kt < k1 && ok; ++kt) {
-                for (int r = 0; r < n_q && ok; ++r) {
-                    const int buf = next();
-                    if (!ok) break;
-                    float s[64];
-                    take_s(tmem, buf, wg, lane_addr, b.se, lane, s);
-                    const int tt = t_first + (rt0 + r) * p.T, key = kt * BM + wg * 64;
-                    if (key + 63 > tt) {
-                        const int lim = tt + row / G - key;
+            const int steps = (k1 - k0) * n_q;
+            int kt = k0, r = odd;
+            if (r >= n_q) r -= n_q, ++kt;
+            for (int step = odd; step < steps; step += 2) {
+                const int buf = step % kSBufs;
+                if (!wait(&b.sf[buf], (step / kSBufs) & 1, step)) break;
+                tc::fence_after_sync();
+                float s[64];
+                take_s(tmem, buf, half, lane_addr, b.se, lane, s);
+                const int tt = t_first + (rt0 + r) * p.T, key = kt * BM + half * 64;
+                if (key + 63 > tt) {
+                    const int lim = tt + row / G - key;
 #pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c > lim) s[c] = -INFINITY;
-                    }
-                    float mx[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        mx[i] = fmaxf(s[i], s[i + 4]);
-#pragma unroll
-                        for (int c = 8 + i; c < 64; c += 4) mx[i] = fmaxf(mx[i], s[c]);
-                    }
-                    const float2 st = stat[r * BM];
-                    const float m = fmaxf(st.x, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
-                    const float ms = m == -INFINITY ? 0.f : m;
-                    const float2 nm = make_float2(-ms, -ms);
-                    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const float2 x = __ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2_2, nm);
-                        acc[c & 1] = __fadd2_rn(acc[c & 1], make_float2(ex2(x.x), ex2(x.y)));
-                    }
-                    const float2 t = __fadd2_rn(acc[0], acc[1]);
-                    stat[r * BM] = make_float2(m, st.y * ex2(st.x - ms) + (t.x + t.y));
+                    for (int c = 0; c < 64; ++c)
+                        if (c > lim) s[c] = -INFINITY;
                 }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int c = 4; c < 60; c += 8)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], s[c + i], s[c + 4 + i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], s[60 + i]);
+                const float2 st = stat[r * BM];
+                const float m = fmaxf(st.x, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
+                const float ms = m == -INFINITY ? 0.f : m;
+                const float2 nm = make_float2(-ms, -ms);
+                float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    acc[c & 1] = __fadd2_rn(
+                        acc[c & 1], exp2_pair(__ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2_2, nm), c));
+                const float2 t = __fadd2_rn(acc[0], acc[1]);
+                stat[r * BM] = make_float2(m, st.y * ex2(st.x - ms) + (t.x + t.y));
+                r += 2;
+                while (r >= n_q) r -= n_q, ++kt;
             }
+            // the four warpgroups' statistics of each row
+            tc::named_bar_sync(1, 512);
             const int sp = blockIdx.x % p.splits;
-            float2* out = p.ml + ((int64_t)(sp * 2 + wg) * Hkv + h) * p.n_rt * BM + rt0 * BM + row;
-            for (int r = 0; r < n_q; ++r) out[r * BM] = stat[r * BM];
+            float2* out = p.ml + ((int64_t)sp * Hkv + h) * p.n_rt * BM + rt0 * BM;
+            for (int i = wg * BM + row; i < n_q * BM; i += 4 * BM) {
+                float2 v[4];
+                float m = -INFINITY, l = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    v[w] = stats[w * kMaxGroup * BM + i];
+                    m = fmaxf(m, v[w].x);
+                }
+                const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) l += v[w].y * ex2(v[w].x - ms);
+                out[i] = make_float2(m, l);
+            }
         } else {
-            float* red = reinterpret_cast<float*>(smem + LY::kOffStat);  // [2][2][BM]
-            const float* lse = p.lse + (int64_t)h * p.n_rt * BM;
-            int turn = 0;
+            float* red = reinterpret_cast<float*>(smem + LY::kOffRed);  // [2 turns][3 warpgroups][2][BM]
+            int turn = 0, step = 0, qt_n = 0;
+            if (!stream_q) wait(&b.qf[0], 0, 0);
             for (int g = k0; g < k1; g += p.b_splits) {
                 const int r0 = rt_from(g), nk = min(p.kg, p.n_kt - g * p.kg);
-                float sum[2] = {0.f, 0.f};
+                float sum0 = 0.f, sum1 = 0.f;
                 for (int rt = r0; rt < n_q && ok; ++rt) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        if (k >= nk) break;
-                        const int buf = next();
-                        if (!ok) break;
+                    const int qs = stream_q ? qt_n % q_slots : rt;
+                    if (stream_q) wait(&b.qf[qs], (qt_n / q_slots) & 1, step);
+                    for (int k = 0; k < nk; ++k, ++step) {
+                        if ((step & 1) != odd) continue;
+                        const int buf = step % kSBufs;
+                        if (!wait(&b.sf[buf], (step / kSBufs) & 1, step)) break;
+                        tc::fence_after_sync();
                         float s[64];
-                        take_s(tmem, buf, wg, lane_addr, b.se, lane, s);
-                        const float4* l4 = reinterpret_cast<const float4*>(lse + rt * BM + wg * 64);
-                        const int key0 = (g * p.kg + k) * BM, tt = t_first + rt * p.T;
-                        if (key0 + BM - 1 > tt) {
+                        take_s(tmem, buf, half, lane_addr, b.se, lane, s);
+                        const float4* l4 = reinterpret_cast<const float4*>(lse_s + qs * BM + half * 64);
+                        const int key = (g * p.kg + k) * BM + row, tt = t_first + rt * p.T;
+                        if (key - row + BM - 1 > tt) {
                             // some of these rows come before some of these keys
-                            int tok = tt + wg * 64 / G, rem = wg * 64 % G;
+                            int tok = tt + half * 64 / G, rem = half * 64 % G;
 #pragma unroll
                             for (int c = 0; c < 64; ++c) {
-                                if (key0 + row > tok) s[c] = -INFINITY;
+                                if (key > tok) s[c] = -INFINITY;
                                 if (++rem == G) rem = 0, ++tok;
                             }
                         }
@@ -415,28 +478,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                         for (int c = 0; c < 16; ++c) {
                             const float4 l = l4[c];
-                            const float2 x = __ffma2_rn(make_float2(s[4 * c], s[4 * c + 1]), sl2_2, make_float2(-l.x, -l.y));
-                            const float2 y =
-                                __ffma2_rn(make_float2(s[4 * c + 2], s[4 * c + 3]), sl2_2, make_float2(-l.z, -l.w));
-                            acc[0] = __fadd2_rn(acc[0], make_float2(ex2(x.x), ex2(x.y)));
-                            acc[1] = __fadd2_rn(acc[1], make_float2(ex2(y.x), ex2(y.y)));
+                            acc[0] = __fadd2_rn(acc[0], exp2_pair(__ffma2_rn(make_float2(s[4 * c], s[4 * c + 1]), sl2_2,
+                                                                             make_float2(l.x, l.y)),
+                                                                  2 * c));
+                            acc[1] = __fadd2_rn(acc[1], exp2_pair(__ffma2_rn(make_float2(s[4 * c + 2], s[4 * c + 3]),
+                                                                             sl2_2, make_float2(l.z, l.w)),
+                                                                  2 * c + 1));
                         }
                         const float2 t = __fadd2_rn(acc[0], acc[1]);
-                        sum[k] += t.x + t.y;
+                        if (k == 0) sum0 += t.x + t.y;
+                        else sum1 += t.x + t.y;
                     }
+                    if (stream_q) {
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&b.qe[qs]);
+                    }
+                    ++qt_n;
                 }
-                // the two warpgroups' halves of the query rows
-                if (wg == 1) {
-                    red[(turn * 2 + 0) * BM + row] = sum[0];
-                    red[(turn * 2 + 1) * BM + row] = sum[1];
-                }
-                tc::named_bar_sync(1, 256);
+                // the warpgroups' sums of each key
+                float* mine = red + (turn * 3 + wg - 1) * 2 * BM + row;
+                if (wg > 0) mine[0] = sum0, mine[BM] = sum1;
+                tc::named_bar_sync(1, 512);
                 if (wg == 0 && ok) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
+                    for (int k = 0; k < nk; ++k) {
                         const int key = (g * p.kg + k) * BM + row;
-                        if (k >= nk || key >= a.kv_len) continue;
-                        const float v = sum[k] + red[(turn * 2 + k) * BM + row];
+                        if (key >= a.kv_len) break;
+                        float v = k == 0 ? sum0 : sum1;
+#pragma unroll
+                        for (int w = 0; w < 3; ++w) v += red[((turn * 3 + w) * 2 + k) * BM + row];
                         float* out = a.acc + (int64_t)h * a.acc_stride + key;
                         *out = a.accumulate ? *out + v : v;
                     }
@@ -454,23 +523,37 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 }
 
-// The rows' log-sum-exp from the splits' statistics.
-__global__ void k7_join(const WeightArgs a, const WeightPlan p) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int n = p.n_rt * BM, G = a.n_head / a.n_head_kv;
-    const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, stride = (int64_t)n * a.n_head_kv;
-    if (at >= stride) return;
-    const int i = (int)(at % n), r = i % BM;
-    const bool there = r < p.T * G && i / BM * p.T + r / G < a.n_tok - a.row_begin;
+// The rows' (minus) log-sum-exp from the splits' statistics: 16 lanes to a row.
+// `there`: whether row i of a head's n is one.
+constexpr int kJoinThreads = 256;
+template <class F>
+__device__ __forceinline__ void join_rows(const float2* ml, float* nlse, int64_t n, int heads, int splits, F&& there) {
+    const int64_t at = (int64_t)blockIdx.x * (kJoinThreads / 16) + threadIdx.x / 16, stride = n * heads;
+    const int part = threadIdx.x % 16;
+    if (at >= stride) return;  // (whole groups of 16 lanes)
+    const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
     float m = -INFINITY, l = 0.f;
-    for (int s = 0; there && s < 2 * p.splits; ++s) m = fmaxf(m, p.ml[s * stride + at].x);
+    for (int s = part; s < splits; s += 16) m = fmaxf(m, ml[s * stride + at].x);
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(lanes, m, d));
     const float ms = m == -INFINITY ? 0.f : m;
-    for (int s = 0; there && s < 2 * p.splits; ++s) {
-        const float2 v = p.ml[s * stride + at];
+    for (int s = part; s < splits; s += 16) {
+        const float2 v = ml[s * stride + at];
         l += v.y * ex2(v.x - ms);
     }
-    p.lse[at] = there ? ms + log2f(l) : INFINITY;
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) l += __shfl_xor_sync(lanes, l, d);
+    if (part == 0) nlse[at] = there(at % n) ? -(ms + log2f(l)) : -INFINITY;
+}
+
+__global__ void __launch_bounds__(kJoinThreads) k7_join(const WeightArgs a, const WeightPlan p) {
+    tc::pdl_wait();
+    tc::pdl_launch();
+    const int G = a.n_head / a.n_head_kv;
+    join_rows(p.ml, p.nlse, (int64_t)p.n_rt * BM, a.n_head_kv, p.splits, [&](int64_t i) {
+        const int r = (int)(i % BM);
+        return r < p.T * G && (int)(i / BM) * p.T + r / G < a.n_tok - a.row_begin;
+    });
 }
 
 // ------------------------------------------------------------ f32: CUDA cores --
@@ -478,10 +561,10 @@ constexpr int FT = 64;          // query rows, and keys, of a tile
 constexpr int kF32Threads = 256;  // 16 x 16 threads, 4 rows x 4 keys each
 
 struct F32Plan {
-    int64_t n_rows;  // (token, head) rows of the window per KV head
+    int32_t n_rows;  // (token, head) rows of the window per KV head
     int32_t n_rt, n_kt, splits;
     float2* ml;      // [splits][Hkv][n_rt * 64]
-    float* lse;      // [Hkv][n_rt * 64], +inf for rows that are none
+    float* nlse;     // [Hkv][n_rt * 64]: minus the lse, -inf for rows that are none
 };
 
 // 64 rows of `D` floats into shared memory, rows padded by 16 bytes (the 4 x 4
@@ -501,9 +584,11 @@ template <int D>
 __device__ __forceinline__ void load_queries_f32(const WeightArgs& a, const F32Plan& p, float* dst, int rt, int h) {
     const int G = a.n_head / a.n_head_kv;
     load_rows_f32<D>(dst, [&](int r) -> const float* {
-        const int64_t i = (int64_t)rt * FT + r;
+        const int i = rt * FT + r;
         if (i >= p.n_rows) return nullptr;
-        return static_cast<const float*>(a.q) + ((a.row_begin + i / G) * a.n_head + (int64_t)h * G + i % G) * D;
+        const int tok = i / G;
+        return static_cast<const float*>(a.q) +
+               ((int64_t)(a.row_begin + tok) * a.n_head + h * G + (i - tok * G)) * D;
     });
 }
 
@@ -553,20 +638,21 @@ template <int D>
 __global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, const F32Plan p) {
     extern __shared__ __align__(16) float sm[];
     float *q = sm, *k = sm + FT * (D + 4);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    tc::pdl_wait();
+    tc::pdl_launch();
     const int sp = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
     const int rt = p.n_rt - 1 - rest % p.n_rt, h = rest / p.n_rt;  // late rows first: they see the most keys
     const int G = a.n_head / a.n_head_kv, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     const int t_first = a.kv_len - a.n_tok + a.row_begin;
     const float sl2 = a.kq_scale * 1.4426950408889634f;
-    const int64_t last_row = min((int64_t)rt * FT + FT, p.n_rows) - 1;
-    const int n_kt = (int)((t_first + last_row / G) / FT) + 1;
+    const int last_row = min(rt * FT + FT, p.n_rows) - 1;
+    const int n_kt = (t_first + last_row / G) / FT + 1;
     const int k0 = (int)((int64_t)n_kt * sp / p.splits), k1 = (int)((int64_t)n_kt * (sp + 1) / p.splits);
     int tok[4];
     float m[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        tok[i] = t_first + (int)(((int64_t)rt * FT + ty + 16 * i) / G);
+        tok[i] = t_first + (rt * FT + ty + 16 * i) / G;
         m[i] = -INFINITY;
         l[i] = 0.f;
     }
@@ -607,18 +693,10 @@ __global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, 
     }
 }
 
-__global__ void k7_join_f32(const WeightArgs a, const F32Plan p) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int64_t n = (int64_t)p.n_rt * FT, at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (at >= n * a.n_head_kv) return;
-    const int64_t stride = n * a.n_head_kv;
-    const bool there = at % n < p.n_rows;
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; there && s < p.splits; ++s) m = fmaxf(m, p.ml[s * stride + at].x);
-    const float ms = m == -INFINITY ? 0.f : m;
-    for (int s = 0; there && s < p.splits; ++s) l += p.ml[s * stride + at].y * ex2(p.ml[s * stride + at].x - ms);
-    p.lse[at] = there ? ms + log2f(l) : INFINITY;
+__global__ void __launch_bounds__(kJoinThreads) k7_join_f32(const WeightArgs a, const F32Plan p) {
+    tc::pdl_wait();
+    tc::pdl_launch();
+    join_rows(p.ml, p.nlse, (int64_t)p.n_rt * FT, a.n_head_kv, p.splits, [&](int64_t i) { return i < p.n_rows; });
 }
 
 template <int D>
@@ -629,9 +707,10 @@ __global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, c
     const int G = a.n_head / a.n_head_kv, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     const int t_first = a.kv_len - a.n_tok + a.row_begin;
     const float sl2 = a.kq_scale * 1.4426950408889634f;
+    tc::pdl_wait();
+    tc::pdl_launch();
     load_keys_f32<D>(a, k, kt, h);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const float* lse = p.lse + (int64_t)h * p.n_rt * FT;
+    const float* nlse = p.nlse + (int64_t)h * p.n_rt * FT;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     const int r0 = max(0, (int)((int64_t)(kt * FT - t_first) * G / FT));  // first tile with a row that sees the keys
     for (int rt = r0; rt < p.n_rt; ++rt) {
@@ -642,12 +721,11 @@ __global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, c
         scores_f32<D>(q, k, ty, tx, x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int64_t r = (int64_t)rt * FT + ty + 16 * i;
-            const int tok = t_first + (int)(r / G);
-            const float ls = lse[r];
+            const int r = rt * FT + ty + 16 * i, tok = t_first + r / G;
+            const float ls = nlse[r];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (kt * FT + tx + 16 * j <= tok) sum[j] += ex2(fmaf(x[i][j], sl2, -ls));
+                if (kt * FT + tx + 16 * j <= tok) sum[j] += ex2(fmaf(x[i][j], sl2, ls));
         }
     }
     __syncthreads();
@@ -665,16 +743,20 @@ __global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, c
 // ---------------------------------------------------------------- host side --
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
+// Workspace layouts; they return the bytes (SIZE_MAX: more rows than 32 bits
+// count).
 size_t plan_f32(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, char* ws, F32Plan* p) {
-    p->n_rows = (int64_t)rows * (n_head / n_head_kv);
-    p->n_rt = (int32_t)((p->n_rows + FT - 1) / FT);
+    const int64_t n_rows = (int64_t)rows * (n_head / n_head_kv);
+    if (n_rows > INT_MAX - FT) return SIZE_MAX;
+    p->n_rows = (int32_t)n_rows;
+    p->n_rt = (p->n_rows + FT - 1) / FT;
     p->n_kt = (kv_len + FT - 1) / FT;
     // three CTAs fit an SM: split the keys until the device is full
     const int64_t ctas = (int64_t)n_head_kv * p->n_rt;
     p->splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_kt, 3 * kSms / ctas));
     const size_t n = (size_t)n_head_kv * p->n_rt * FT, ml = up16(n * p->splits * sizeof(float2));
     p->ml = reinterpret_cast<float2*>(ws);
-    p->lse = reinterpret_cast<float*>(ws + ml);
+    p->nlse = reinterpret_cast<float*>(ws + ml);
     return ml + up16(n * sizeof(float));
 }
 
@@ -682,6 +764,7 @@ size_t plan_tc(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, 
     const int slots = d == 128 ? TcLayout<128>::kSlots : TcLayout<64>::kSlots;
     p->T = BM / (n_head / n_head_kv);
     p->n_rt = (rows + p->T - 1) / p->T;
+    if ((int64_t)p->n_rt * BM > INT_MAX) return SIZE_MAX;
     p->n_kt = (kv_len + BM - 1) / BM;
     p->n_groups = (p->n_rt + kMaxGroup - 1) / kMaxGroup;
     p->group = (p->n_rt + p->n_groups - 1) / p->n_groups;
@@ -696,9 +779,9 @@ size_t plan_tc(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, 
     p->kg = !p->resident && (int64_t)n_head_kv * p->n_kt >= 2 * kSms ? 2 : 1;
     const int n_kg = (p->n_kt + p->kg - 1) / p->kg;
     p->b_splits = std::max(1, std::min(n_kg, kSms / n_head_kv));
-    const size_t n = (size_t)n_head_kv * p->n_rt * BM, ml = up16(n * 2 * p->splits * sizeof(float2));
+    const size_t n = (size_t)n_head_kv * p->n_rt * BM, ml = up16(n * p->splits * sizeof(float2));
     p->ml = reinterpret_cast<float2*>(ws);
-    p->lse = reinterpret_cast<float*>(ws + ml);
+    p->nlse = reinterpret_cast<float*>(ws + ml);
     return ml + up16(n * sizeof(float));
 }
 
@@ -739,10 +822,9 @@ cudaError_t launch_f32(const WeightArgs& a, cudaStream_t s) {
     if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_sums_f32<D>), smem, m1);
     if (e != cudaSuccess) return e;
     const int64_t ctas = (int64_t)a.n_head_kv * p.n_rt * p.splits, rows = (int64_t)a.n_head_kv * p.n_rt * FT;
-    if (ctas > INT_MAX) return cudaErrorInvalidValue;
-    k7_stats_f32<D><<<(unsigned)ctas, kF32Threads, smem, s>>>(a, p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    e = launch_after(k7_join_f32, (rows + 255) / 256, 256, 0, s, a, p);
+    e = launch_after(k7_stats_f32<D>, ctas, kF32Threads, smem, s, a, p);
+    if (e == cudaSuccess)
+        e = launch_after(k7_join_f32, (rows + kJoinThreads / 16 - 1) / (kJoinThreads / 16), kJoinThreads, 0, s, a, p);
     if (e != cudaSuccess) return e;
     return launch_after(k7_sums_f32<D>, (int64_t)a.n_head_kv * p.n_kt, kF32Threads, smem, s, a, p);
 }
@@ -789,10 +871,9 @@ cudaError_t launch_tc(const WeightArgs& a, cudaStream_t s) {
     if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 1>), smem, m1);
     if (e != cudaSuccess) return e;
     const int64_t ctas = (int64_t)a.n_head_kv * p.n_groups * p.splits, n = (int64_t)p.n_rt * BM;
-    if (ctas > INT_MAX || n > INT_MAX) return cudaErrorInvalidValue;
-    k7_pass<BF16, D, SEG, 0><<<(unsigned)ctas, kTcThreads, smem, s>>>(mq, mk, a, p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    e = launch_after(k7_join, (n * a.n_head_kv + 255) / 256, 256, 0, s, a, p);
+    e = launch_after(k7_pass<BF16, D, SEG, 0>, ctas, kTcThreads, smem, s, mq, mk, a, p);
+    if (e == cudaSuccess)
+        e = launch_after(k7_join, n * a.n_head_kv / (kJoinThreads / 16), kJoinThreads, 0, s, a, p);
     if (e != cudaSuccess) return e;
     return launch_after(k7_pass<BF16, D, SEG, 1>, (int64_t)a.n_head_kv * p.b_splits, kTcThreads, smem, s, mq, mk, a, p);
 }
