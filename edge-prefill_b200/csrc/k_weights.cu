@@ -79,17 +79,18 @@ constexpr int kHalfTile = BM * 128;     // [128][64 x 16-bit], 128-byte swizzled
 constexpr int kMaxGroup = 4;            // query tiles a statistics CTA keeps on chip
 constexpr int kSBufs = 4;               // S tiles in TMEM (128 columns each)
 constexpr int kSms = 148;
+constexpr int kBatch = 4;               // key tiles whose sums are put together at a time
 
 template <int D>
 struct TcLayout {
     static constexpr int kTile = D / 64 * kHalfTile;
     static constexpr int kSlots = D == 128 ? 6 : 12;  // query + key tiles on chip
     // statistics pass: float2 [4][kMaxGroup * BM]; sums pass: float
-    // [kSlots][BM] lse of the query tiles on chip, then [2][3][2][BM] sums
+    // [kSlots][BM] lse of the query tiles on chip, then [2][kBatch][4][BM] sums
     static constexpr int kOffStat = kSlots * kTile;
     static constexpr int kOffRed = kOffStat + kSlots * BM * 4;
-    static constexpr int kOffBar = kOffStat + 4 * kMaxGroup * BM * 8;
-    static_assert(kOffRed + 2 * 3 * 2 * BM * 4 <= kOffBar, "sums pass");
+    static constexpr int kOffBar = kOffRed + 2 * kBatch * 4 * BM * 4;
+    static_assert(kOffStat + 4 * kMaxGroup * BM * 8 <= kOffBar, "statistics pass");
     static constexpr int kBars = 2 * 12 + 2 * 12 + 2 * kSBufs + 1;
     static constexpr int kBytes = kOffBar + kBars * 8 + 32;
     static_assert(kBytes + 1024 <= 232448, "shared memory");
@@ -155,12 +156,23 @@ __device__ __forceinline__ void load_queries(const WeightArgs& a, const WeightPl
         tc::tma_load_3d(dst + hf * kHalfTile, tm, bar, hf * 64, h * G, a.row_begin + rt * p.T);
 }
 
-// S (columns of one TMEM buffer) = A B^T over D.
+// A position in a ring of tiles: its slot and the parity of that slot's fill.
+struct Ring {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next(int slots) {
+        if (++slot == slots) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// S (columns of one TMEM buffer) = A B^T over D; operand descriptors of a tile
+// in slot i are the base plus i tiles.
 template <bool BF16, int D>
-__device__ __forceinline__ void issue_s(uint32_t tmem, int buf, const unsigned char* a_tile, const unsigned char* b_tile) {
+__device__ __forceinline__ void issue_s(uint32_t tmem, int buf, uint64_t da, uint64_t db) {
     constexpr uint32_t idesc = tc::make_idesc_f16(BF16, BM, BM, false);
-    const uint64_t da = tc::make_sdesc_sw128(tc::smem_u32(a_tile), 16, 1024);
-    const uint64_t db = tc::make_sdesc_sw128(tc::smem_u32(b_tile), 16, 1024);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
         const uint64_t off = (uint64_t)(((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4);
@@ -169,17 +181,16 @@ __device__ __forceinline__ void issue_s(uint32_t tmem, int buf, const unsigned c
 }
 
 // 64 columns of S of this thread's lane; the buffer is handed back at once.
-__device__ __forceinline__ void take_s(uint32_t tmem, int buf, int half, uint32_t lane_addr, uint64_t* se, int lane,
-                                       float (&s)[64]) {
+__device__ __forceinline__ void take_s(uint32_t addr, uint64_t* se, int lane, float (&s)[64]) {
     uint32_t u[2][32];
-    tc::tmem_ld32(tmem + lane_addr + buf * BM + half * 64, u[0]);
-    tc::tmem_ld32(tmem + lane_addr + buf * BM + half * 64 + 32, u[1]);
+    tc::tmem_ld32(addr, u[0]);
+    tc::tmem_ld32(addr + 32, u[1]);
     tc::tmem_wait_ld();
 #pragma unroll
     for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(u[i >> 5][i & 31]);
     tc::fence_before_sync();
     __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&se[buf]);
+    if (lane == 0) tc::mbar_arrive(se);
 }
 
 // PASS 0: statistics.  CTA (key split, group of query tiles, KV head): the
@@ -189,9 +200,8 @@ __device__ __forceinline__ void take_s(uint32_t tmem, int buf, int half, uint32_
 // query rows, so each thread sums one key's weights in registers; key tiles
 // (kg at a time) against all query tiles, which stay when they fit and
 // stream otherwise.
-// A step is one (query tile, key tile); two warpgroups take the even steps,
-// two the odd ones, each 64 of the 128 columns: with four warps to a scheduler
-// one's loads and waits hide behind the others' exponentials.
+// A step is one (query tile, key tile), its S in buffer step % 4; two
+// warpgroups take the even steps, two the odd ones, each 64 of the 128 columns.
 template <bool BF16, int D, int SEG, int PASS>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k7_pass(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -244,7 +254,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         for (int i = 0; i < kSBufs; ++i) {
             tc::mbar_init(&b.sf[i], 1);
-            tc::mbar_init(&b.se[i], 8);
+            tc::mbar_init(&b.se[i], 8);  // the warps of two warpgroups
         }
         tc::mbar_init(b.done, 1);
         tc::fence_mbar_init();
@@ -272,18 +282,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int q_bytes = D / 64 * 64 * 2 * p.T * G;
 
     // first query tile that sees any key of group kgi (sums pass)
-    auto rt_from = [&](int kgi) { return max(0, (kgi * p.kg * BM - t_first) / p.T); };
+    auto rt_from = [&](int kgi) {
+        const int late = kgi * p.kg * BM - t_first;
+        return late < p.T ? 0 : late / p.T;
+    };
 
     if (warp == 0) {
         // ------------------------------------------------------ producer --
         if (lane == 0) {
             bool ok = true;
             int kt_n = 0, qt_n = 0;  // tiles issued into each ring
+            Ring kr, qr;
             auto keys = [&](int kt) {
-                const int s = kt_n % k_slots;
-                ok = tc::mbar_wait(&b.ke[s], ((kt_n / k_slots) & 1) ^ 1, tmo);
+                ok = tc::mbar_wait(&b.ke[kr.slot], kr.phase ^ 1, tmo);
                 if (!ok) return;
-                load_keys<D, SEG>(a, &tmK, kbase + s * LY::kTile, &b.kf[s], kt, h);
+                load_keys<D, SEG>(a, &tmK, kbase + kr.slot * LY::kTile, &b.kf[kr.slot], kt, h);
+                kr.next(k_slots);
                 ++kt_n;
             };
             if (!stream_q) {
@@ -297,16 +311,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int kt = k0; kt < k1 && ok; ++kt) keys(kt);
             } else {
                 for (int g = k0; g < k1 && ok; g += p.b_splits) {
-                    const int r0 = rt_from(g);
-                    if (r0 >= n_q) continue;
                     for (int k = 0; k < p.kg && g * p.kg + k < p.n_kt && ok; ++k) keys(g * p.kg + k);
-                    for (int rt = r0; rt < n_q && ok && stream_q; ++rt) {
-                        const int s = qt_n % q_slots;
-                        ok = tc::mbar_wait(&b.qe[s], ((qt_n / q_slots) & 1) ^ 1, tmo);
+                    if (!stream_q) continue;
+                    for (int rt = rt_from(g); rt < n_q && ok; ++rt) {
+                        const int s = qr.slot;
+                        ok = tc::mbar_wait(&b.qe[s], qr.phase ^ 1, tmo);
                         if (!ok) break;
                         tc::mbar_arrive_expect_tx(&b.qf[s], q_bytes + BM * 4);
                         load_queries<D>(a, p, &tmQ, smem + s * LY::kTile, &b.qf[s], rt, h);
                         tc::bulk_load(lse_s + s * BM, p.nlse + ((int64_t)h * p.n_rt + rt) * BM, BM * 4, &b.qf[s]);
+                        qr.next(q_slots);
                         ++qt_n;
                     }
                 }
@@ -323,7 +337,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // ----------------------------------------------------------- MMA --
         const bool leader = tc::elect_one();
         bool ok = true;
-        int step = 0, kt_n = 0, qt_n = 0;
+        int step = 0;
+        Ring kr, qr;
+        constexpr uint64_t kTileD = LY::kTile >> 4;
+        const uint64_t dq = tc::make_sdesc_sw128(tc::smem_u32(smem), 16, 1024);
+        const uint64_t dk = tc::make_sdesc_sw128(tc::smem_u32(kbase), 16, 1024);
         auto wait = [&](uint64_t* bar, uint32_t par) {
             if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(bar, par, tmo));
             return ok;
@@ -332,41 +350,51 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (leader) tc::mma_commit(bar);
             __syncwarp();
         };
-        auto one = [&](const unsigned char* q, const unsigned char* k) {
+        auto one = [&](uint64_t q, uint64_t k) {
             const int buf = step % kSBufs;
             if (!wait(&b.se[buf], ((step / kSBufs) & 1) ^ 1)) return;
             tc::fence_after_sync();
-            if (leader) issue_s<BF16, D>(tmem, buf, PASS == 0 ? q : k, PASS == 0 ? k : q);
+            if (leader) {
+                issue_s<BF16, D>(tmem, buf, PASS == 0 ? q : k, PASS == 0 ? k : q);
+                tc::mma_commit(&b.sf[buf]);
+            }
             __syncwarp();
-            commit(&b.sf[buf]);
             ++step;
         };
         if (!stream_q) wait(&b.qf[0], 0);
         if constexpr (PASS == 0) {
-            for (int kt = k0; kt < k1 && ok; ++kt, ++kt_n) {
-                const int s = kt_n % k_slots;
-                wait(&b.kf[s], (kt_n / k_slots) & 1);
-                for (int r = 0; r < n_q && ok; ++r) one(smem + r * LY::kTile, kbase + s * LY::kTile);
-                if (ok) commit(&b.ke[s]);
+            for (int kt = k0; kt < k1 && ok; ++kt) {
+                wait(&b.kf[kr.slot], kr.phase);
+                for (int r = 0; r < n_q && ok; ++r) one(dq + r * kTileD, dk + kr.slot * kTileD);
+                if (ok) commit(&b.ke[kr.slot]);
+                kr.next(k_slots);
             }
         } else {
             for (int g = k0; g < k1 && ok; g += p.b_splits) {
-                const int r0 = rt_from(g);
-                if (r0 >= n_q) continue;
-                const int nk = min(p.kg, p.n_kt - g * p.kg);
+                const int r0 = rt_from(g), nk = min(p.kg, p.n_kt - g * p.kg);
+                Ring k2 = kr;
+                k2.next(k_slots);
                 for (int rt = r0; rt < n_q && ok; ++rt) {
-                    const int qs = stream_q ? qt_n % q_slots : rt;
-                    if (stream_q) wait(&b.qf[qs], (qt_n / q_slots) & 1);
-                    for (int k = 0; k < nk && ok; ++k) {
-                        const int s = (kt_n + k) % k_slots;
-                        if (rt == r0) wait(&b.kf[s], ((kt_n + k) / k_slots) & 1);
-                        if (ok) one(smem + qs * LY::kTile, kbase + s * LY::kTile);
+                    const int qs = stream_q ? qr.slot : rt;
+                    if (stream_q) wait(&b.qf[qs], qr.phase);
+                    if (rt == r0) wait(&b.kf[kr.slot], kr.phase);
+                    if (ok) one(dq + qs * kTileD, dk + kr.slot * kTileD);
+                    if (nk == 2) {
+                        if (rt == r0) wait(&b.kf[k2.slot], k2.phase);
+                        if (ok) one(dq + qs * kTileD, dk + k2.slot * kTileD);
                     }
-                    if (stream_q && ok) commit(&b.qe[qs]);
-                    ++qt_n;
+                    if (stream_q) {
+                        if (ok) commit(&b.qe[qs]);
+                        qr.next(q_slots);
+                    }
                 }
-                for (int k = 0; k < nk && ok; ++k) commit(&b.ke[(kt_n + k) % k_slots]);
-                kt_n += nk;
+                if (!ok) break;
+                commit(&b.ke[kr.slot]);
+                kr.next(k_slots);
+                if (nk == 2) {
+                    commit(&b.ke[kr.slot]);
+                    kr.next(k_slots);
+                }
             }
         }
         if (!ok && lane == 0) report_error(a.err, kDevWaitWeights, 0xb2 + PASS, step);
@@ -377,7 +405,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else if (warp >= 4) {
         // ------------------------------------------------------- softmax --
         const int wg = (warp - 4) >> 2, odd = wg >> 1, half = wg & 1, wq = warp & 3, row = wq * 32 + lane;
-        const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
+        const uint32_t s_addr = tmem + ((uint32_t)(wq * 32) << 16) + half * 64;
         const float sl2 = a.kq_scale * 1.4426950408889634f;
         const float2 sl2_2 = make_float2(sl2, sl2);
         bool ok = true;
@@ -393,14 +421,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             float2* stat = stats + wg * kMaxGroup * BM + row;
             for (int r = 0; r < n_q; ++r) stat[r * BM] = make_float2(-INFINITY, 0.f);
             const int steps = (k1 - k0) * n_q;
-            int kt = k0, r = odd;
+            int kt = k0, r = odd, r_held = -1;
             if (r >= n_q) r -= n_q, ++kt;
+            float2 st = make_float2(-INFINITY, 0.f);  // of query tile r_held
             for (int step = odd; step < steps; step += 2) {
                 const int buf = step % kSBufs;
                 if (!wait(&b.sf[buf], (step / kSBufs) & 1, step)) break;
                 tc::fence_after_sync();
                 float s[64];
-                take_s(tmem, buf, half, lane_addr, b.se, lane, s);
+                take_s(s_addr + buf * BM, &b.se[buf], lane, s);
+                if (r != r_held) {
+                    if (r_held >= 0) stat[r_held * BM] = st;
+                    st = stat[r * BM];
+                    r_held = r;
+                }
                 const int tt = t_first + (rt0 + r) * p.T, key = kt * BM + half * 64;
                 if (key + 63 > tt) {
                     const int lim = tt + row / G - key;
@@ -415,7 +449,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], s[c + i], s[c + 4 + i]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], s[60 + i]);
-                const float2 st = stat[r * BM];
                 const float m = fmaxf(st.x, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
                 const float ms = m == -INFINITY ? 0.f : m;
                 const float2 nm = make_float2(-ms, -ms);
@@ -425,10 +458,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     acc[c & 1] = __fadd2_rn(
                         acc[c & 1], exp2_pair(__ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2_2, nm), c));
                 const float2 t = __fadd2_rn(acc[0], acc[1]);
-                stat[r * BM] = make_float2(m, st.y * ex2(st.x - ms) + (t.x + t.y));
+                st = make_float2(m, st.y * ex2(st.x - ms) + (t.x + t.y));
                 r += 2;
                 while (r >= n_q) r -= n_q, ++kt;
             }
+            if (r_held >= 0) stat[r_held * BM] = st;
             // the four warpgroups' statistics of each row
             tc::named_bar_sync(1, 512);
             const int sp = blockIdx.x % p.splits;
@@ -447,22 +481,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 out[i] = make_float2(m, l);
             }
         } else {
-            float* red = reinterpret_cast<float*>(smem + LY::kOffRed);  // [2 turns][3 warpgroups][2][BM]
-            int turn = 0, step = 0, qt_n = 0;
+            // sums of up to kBatch key tiles wait in shared memory for the
+            // other warpgroups': one barrier per batch
+            float* red = reinterpret_cast<float*>(smem + LY::kOffRed);  // [2 turns][kBatch][4 warpgroups][BM]
+            int turn = 0, step = 0, held = 0, g_first = k0;
+            Ring qr;
             if (!stream_q) wait(&b.qf[0], 0, 0);
             for (int g = k0; g < k1; g += p.b_splits) {
                 const int r0 = rt_from(g), nk = min(p.kg, p.n_kt - g * p.kg);
                 float sum0 = 0.f, sum1 = 0.f;
                 for (int rt = r0; rt < n_q && ok; ++rt) {
-                    const int qs = stream_q ? qt_n % q_slots : rt;
-                    if (stream_q) wait(&b.qf[qs], (qt_n / q_slots) & 1, step);
+                    const int qs = stream_q ? qr.slot : rt;
+                    if (stream_q) wait(&b.qf[qs], qr.phase, step);
                     for (int k = 0; k < nk; ++k, ++step) {
                         if ((step & 1) != odd) continue;
                         const int buf = step % kSBufs;
                         if (!wait(&b.sf[buf], (step / kSBufs) & 1, step)) break;
                         tc::fence_after_sync();
                         float s[64];
-                        take_s(tmem, buf, half, lane_addr, b.se, lane, s);
+                        take_s(s_addr + buf * BM, &b.se[buf], lane, s);
                         const float4* l4 = reinterpret_cast<const float4*>(lse_s + qs * BM + half * 64);
                         const int key = (g * p.kg + k) * BM + row, tt = t_first + rt * p.T;
                         if (key - row + BM - 1 > tt) {
@@ -492,25 +529,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (stream_q) {
                         __syncwarp();
                         if (lane == 0) tc::mbar_arrive(&b.qe[qs]);
+                        qr.next(q_slots);
                     }
-                    ++qt_n;
                 }
-                // the warpgroups' sums of each key
-                float* mine = red + (turn * 3 + wg - 1) * 2 * BM + row;
-                if (wg > 0) mine[0] = sum0, mine[BM] = sum1;
+                float* mine = red + ((turn * kBatch + held) * 4 + wg) * BM + row;
+                mine[0] = sum0;
+                if (p.kg == 2) mine[4 * BM] = sum1;
+                held += p.kg;
+                if (held < kBatch && g + p.b_splits < k1) continue;
                 tc::named_bar_sync(1, 512);
-                if (wg == 0 && ok) {
-                    for (int k = 0; k < nk; ++k) {
-                        const int key = (g * p.kg + k) * BM + row;
-                        if (key >= a.kv_len) break;
-                        float v = k == 0 ? sum0 : sum1;
-#pragma unroll
-                        for (int w = 0; w < 3; ++w) v += red[((turn * 3 + w) * 2 + k) * BM + row];
-                        float* out = a.acc + (int64_t)h * a.acc_stride + key;
-                        *out = a.accumulate ? *out + v : v;
-                    }
+                for (int i = wg * BM + row; i < held * BM && ok; i += 4 * BM) {
+                    // key tile i / BM of the batch
+                    const int j = i / BM, kt = (g_first + j / p.kg * p.b_splits) * p.kg + j % p.kg, key = kt * BM + row;
+                    if (key >= a.kv_len) continue;
+                    const float* from = red + (turn * kBatch + j) * 4 * BM + row;
+                    const float v = (from[0] + from[BM]) + (from[2 * BM] + from[3 * BM]);
+                    float* out = a.acc + (int64_t)h * a.acc_stride + key;
+                    *out = a.accumulate ? *out + v : v;
                 }
                 turn ^= 1;
+                held = 0;
+                g_first = g + p.b_splits;
             }
         }
     }
