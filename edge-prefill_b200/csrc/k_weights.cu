@@ -42,12 +42,12 @@ __device__ __forceinline__ float max3f(float x, float y, float z) {
     return r;
 }
 
-// 2^x of a pair on the FMA pipe.  x >= -126 (below: 2^-126; NaN stays) is split
+// acc + 2^x of a pair on the FMA pipe.  x >= -126 (below: 2^-126; NaN stays) is split
 // into n + r, n = round(x), r in [-0.5, 0.5]: adding 1.5 * 2^23 + 127 leaves
 // n + 127 in the low mantissa bits, which shifted up are 2^n's bits.  2^r is a
 // polynomial of degree 5, fitted here for the least relative error on that
 // interval (7.5e-8, 2.4e-7 with f32 coefficients and steps: ex2's own error).
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
+__device__ __forceinline__ float2 exp2_poly_add(float2 x, float2 acc) {
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
     const float2 t = __fadd2_rn(x, make_float2(12583039.f, 12583039.f));
@@ -59,17 +59,19 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
     p = __ffma2_rn(p, r, make_float2(0.24022120237350464f, 0.24022120237350464f));
     p = __ffma2_rn(p, r, make_float2(0.6931469440460205f, 0.6931469440460205f));
     p = __ffma2_rn(p, r, make_float2(1.0000001192092896f, 1.0000001192092896f));
-    return __fmul2_rn(p, make_float2(__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23)));
+    return __ffma2_rn(
+        p, make_float2(__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23)), acc);
 }
 
-// Exponentials of pair i of a run of pairs: one pair in kPolyEvery on the FMA
+// acc + 2^x of pair i of a run of pairs: one pair in kPolyEvery on the FMA
 // pipe, the rest on MUFU.
 #ifndef K7_POLY_EVERY
 #define K7_POLY_EVERY 3
 #endif
 constexpr int kPolyEvery = K7_POLY_EVERY;
-__device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
-    return i % kPolyEvery == kPolyEvery - 1 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+__device__ __forceinline__ float2 exp2_add(float2 x, int i, float2 acc) {
+    return i % kPolyEvery == kPolyEvery - 1 ? exp2_poly_add(x, acc)
+                                            : __fadd2_rn(acc, make_float2(ex2(x.x), ex2(x.y)));
 }
 
 // ---------------------------------------------------------- 16-bit: tcgen05 --
@@ -282,9 +284,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int q_bytes = D / 64 * 64 * 2 * p.T * G;
 
     // first query tile that sees any key of group kgi (sums pass)
+    // (on chip, all are taken: there are few)
     auto rt_from = [&](int kgi) {
         const int late = kgi * p.kg * BM - t_first;
-        return late < p.T ? 0 : late / p.T;
+        return !stream_q || late < p.T ? 0 : late / p.T;
     };
 
     if (warp == 0) {
@@ -455,8 +458,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int c = 0; c < 32; ++c)
-                    acc[c & 1] = __fadd2_rn(
-                        acc[c & 1], exp2_pair(__ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2_2, nm), c));
+                    acc[c & 1] = exp2_add(__ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2_2, nm), c, acc[c & 1]);
                 const float2 t = __fadd2_rn(acc[0], acc[1]);
                 st = make_float2(m, st.y * ex2(st.x - ms) + (t.x + t.y));
                 r += 2;
@@ -484,63 +486,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // sums of up to kBatch key tiles wait in shared memory for the
             // other warpgroups': one barrier per batch
             float* red = reinterpret_cast<float*>(smem + LY::kOffRed);  // [2 turns][kBatch][4 warpgroups][BM]
-            int turn = 0, step = 0, held = 0, g_first = k0;
-            Ring qr;
-            if (!stream_q) wait(&b.qf[0], 0, 0);
-            for (int g = k0; g < k1; g += p.b_splits) {
-                const int r0 = rt_from(g), nk = min(p.kg, p.n_kt - g * p.kg);
-                float sum0 = 0.f, sum1 = 0.f;
-                for (int rt = r0; rt < n_q && ok; ++rt) {
-                    const int qs = stream_q ? qr.slot : rt;
-                    if (stream_q) wait(&b.qf[qs], qr.phase, step);
-                    for (int k = 0; k < nk; ++k, ++step) {
-                        if ((step & 1) != odd) continue;
-                        const int buf = step % kSBufs;
-                        if (!wait(&b.sf[buf], (step / kSBufs) & 1, step)) break;
-                        tc::fence_after_sync();
-                        float s[64];
-                        take_s(s_addr + buf * BM, &b.se[buf], lane, s);
-                        const float4* l4 = reinterpret_cast<const float4*>(lse_s + qs * BM + half * 64);
-                        const int key = (g * p.kg + k) * BM + row, tt = t_first + rt * p.T;
-                        if (key - row + BM - 1 > tt) {
-                            // some of these rows come before some of these keys
-                            int tok = tt + half * 64 / G, rem = half * 64 % G;
-#pragma unroll
-                            for (int c = 0; c < 64; ++c) {
-                                if (key > tok) s[c] = -INFINITY;
-                                if (++rem == G) rem = 0, ++tok;
-                            }
-                        }
-                        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) {
-                            const float4 l = l4[c];
-                            acc[0] = __fadd2_rn(acc[0], exp2_pair(__ffma2_rn(make_float2(s[4 * c], s[4 * c + 1]), sl2_2,
-                                                                             make_float2(l.x, l.y)),
-                                                                  2 * c));
-                            acc[1] = __fadd2_rn(acc[1], exp2_pair(__ffma2_rn(make_float2(s[4 * c + 2], s[4 * c + 3]),
-                                                                             sl2_2, make_float2(l.z, l.w)),
-                                                                  2 * c + 1));
-                        }
-                        const float2 t = __fadd2_rn(acc[0], acc[1]);
-                        if (k == 0) sum0 += t.x + t.y;
-                        else sum1 += t.x + t.y;
-                    }
-                    if (stream_q) {
-                        __syncwarp();
-                        if (lane == 0) tc::mbar_arrive(&b.qe[qs]);
-                        qr.next(q_slots);
-                    }
-                }
-                float* mine = red + ((turn * kBatch + held) * 4 + wg) * BM + row;
-                mine[0] = sum0;
-                if (p.kg == 2) mine[4 * BM] = sum1;
-                held += p.kg;
-                if (held < kBatch && g + p.b_splits < k1) continue;
+            int turn = 0, held = 0;
+            auto put = [&](float v) { red[((turn * kBatch + held++) * 4 + wg) * BM + row] = v; };
+            auto flush = [&](int g_first) {
                 tc::named_bar_sync(1, 512);
                 for (int i = wg * BM + row; i < held * BM && ok; i += 4 * BM) {
-                    // key tile i / BM of the batch
-                    const int j = i / BM, kt = (g_first + j / p.kg * p.b_splits) * p.kg + j % p.kg, key = kt * BM + row;
+                    const int j = i / BM, gj = p.kg == 1 ? j : j >> 1;
+                    const int kt = (g_first + gj * p.b_splits) * p.kg + (p.kg == 1 ? 0 : j & 1), key = kt * BM + row;
                     if (key >= a.kv_len) continue;
                     const float* from = red + (turn * kBatch + j) * 4 * BM + row;
                     const float v = (from[0] + from[BM]) + (from[2 * BM] + from[3 * BM]);
@@ -549,7 +501,84 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 turn ^= 1;
                 held = 0;
-                g_first = g + p.b_splits;
+            };
+            // one step: the weights that the 64 rows of query tile rt (slot qs) in `half` give key tile kt, summed
+            auto take_step = [&](int step, int kt, int rt, int qs) -> float {
+                const int buf = step % kSBufs;
+                if (!wait(&b.sf[buf], (step / kSBufs) & 1, step)) return 0.f;
+                tc::fence_after_sync();
+                float s[64];
+                take_s(s_addr + buf * BM, &b.se[buf], lane, s);
+                const float4* l4 = reinterpret_cast<const float4*>(lse_s + qs * BM + half * 64);
+                const int key0 = kt * BM, tt = t_first + rt * p.T;
+                if (key0 + BM - 1 > tt) {
+                    // some of these rows come before some of these keys
+                    int tok = tt + half * 64 / G, rem = half * 64 % G;
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) {
+                        if (key0 + row > tok) s[c] = -INFINITY;
+                        if (++rem == G) rem = 0, ++tok;
+                    }
+                }
+                float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const float4 l = l4[c];
+                    acc[0] = exp2_add(__ffma2_rn(make_float2(s[4 * c], s[4 * c + 1]), sl2_2, make_float2(l.x, l.y)), 2 * c,
+                                      acc[0]);
+                    acc[1] = exp2_add(__ffma2_rn(make_float2(s[4 * c + 2], s[4 * c + 3]), sl2_2, make_float2(l.z, l.w)),
+                                      2 * c + 1, acc[1]);
+                }
+                const float2 t = __fadd2_rn(acc[0], acc[1]);
+                return t.x + t.y;
+            };
+            if (!stream_q) {
+                // steps (key tile, query tile) in turn; this pair of warpgroups has every other one
+                wait(&b.qf[0], 0, 0);
+                const int n_mine = k0 < k1 ? (k1 - 1 - k0) / p.b_splits + 1 : 0;
+                int i = 0, rt = odd, kt = k0, g_first = k0;
+                float sum = 0.f;
+                for (int step = odd; i < n_mine; step += 2) {
+                    while (rt >= n_q && i < n_mine) {
+                        put(sum);
+                        sum = 0.f;
+                        rt -= n_q;
+                        kt += p.b_splits;
+                        if (++i == n_mine || held == kBatch) {
+                            flush(g_first);
+                            g_first = kt;
+                        }
+                    }
+                    if (i == n_mine) break;
+                    sum += take_step(step, kt, rt, rt);
+                    rt += 2;
+                }
+            } else {
+                Ring qr;
+                int step = 0, g_first = k0;
+                for (int g = k0; g < k1; g += p.b_splits) {
+                    const int r0 = rt_from(g), nk = min(p.kg, p.n_kt - g * p.kg);
+                    float sum0 = 0.f, sum1 = 0.f;
+                    for (int rt = r0; rt < n_q && ok; ++rt) {
+                        const int qs = qr.slot;
+                        wait(&b.qf[qs], qr.phase, step);
+                        if ((step & 1) == odd) sum0 += take_step(step, g * p.kg, rt, qs);
+                        ++step;
+                        if (nk == 2) {
+                            if ((step & 1) == odd) sum1 += take_step(step, g * p.kg + 1, rt, qs);
+                            ++step;
+                        }
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&b.qe[qs]);
+                        qr.next(q_slots);
+                    }
+                    put(sum0);
+                    if (p.kg == 2) put(sum1);
+                    if (held == kBatch || g + p.b_splits >= k1) {
+                        flush(g_first);
+                        g_first = g + p.b_splits;
+                    }
+                }
             }
         }
     }
