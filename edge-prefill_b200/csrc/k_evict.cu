@@ -5,20 +5,18 @@
 // significant first) finds the weight of the last row that stays; then every
 // row above it, and the first of those equal to it, get their place by a
 // prefix sum in row order.  The rows of one head are split over a cluster of
-// up to 8 CTAs, which keep their slice of the weights in shared memory (one
-// read of the weights) and add their histograms through distributed shared
+// up to 8 CTAs, which keep their slice of the weights in registers (one read
+// of the weights) and add their histograms through distributed shared
 // memory; only counts are exchanged, so the result is exact and has no order.
 // Latency bounds it: three histogram rounds, each with one cluster barrier.
 //
-// K8b moves the listed rows, which the bytes bound: a warp takes 32 rows, K in
-// its lower half's lanes and V in the upper's.  In place there is an order to
+// K8b moves the listed rows, which the bytes bound: a warp takes as many rows
+// as fill its lanes with eight 16-byte loads each.  In place there is an order to
 // keep (a row may only be written once every row read from it has been), and
 // K8c gives each CTA a 32-byte column of one head, which it compacts from the
 // first row to the last: a kept row never moves up, so a step's loads need
 // only be done before its own stores.
 #include <cooperative_groups.h>
-
-#include <atomic>
 
 #include "epsp_kernels.h"
 
@@ -31,7 +29,10 @@ constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
-constexpr int kCacheRows = 32768;  // weights a CTA keeps in shared memory (128 KB)
+#ifndef K8_CLUSTER_ROWS
+#define K8_CLUSTER_ROWS 2048
+#endif
+constexpr int kClusterRows = K8_CLUSTER_ROWS;
 
 // Order-preserving key of a weight: larger weight, larger key; NaN as -inf;
 // +0 and -0 alike.
@@ -47,44 +48,45 @@ struct EvictPlan {
     int32_t* list;  // [n_seq][Hkv][cap] kept rows, ascending
     int32_t cap;
     int32_t cluster;
-    int32_t cached;  // the slices fit in shared memory
+    int32_t per_thread;  // weights a thread of K8a holds; 0: the slices are too long, read again each time
 };
 
-// Inclusive sum over the CTA's threads (two 32-bit counts in one word).
-__device__ __forceinline__ uint64_t scan_cta(uint64_t x, uint64_t* warp_sums, uint64_t& total) {
+// Inclusive sum over the CTA's threads.
+template <class T>
+__device__ __forceinline__ T scan_cta(T x, T* warp_sums, T& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const uint64_t u = __shfl_up_sync(0xffffffffu, x, d);
+        const T u = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += u;
     }
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        uint64_t w = warp_sums[lane];
+    T w = warp_sums[lane];
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint64_t u = __shfl_up_sync(0xffffffffu, w, d);
-            if (lane >= d) w += u;
-        }
-        warp_sums[lane] = w;
+    for (int d = 1; d < 32; d <<= 1) {
+        const T u = __shfl_up_sync(0xffffffffu, w, d);
+        if (lane >= d) w += u;
     }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const T before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
     __syncthreads();
-    if (warp > 0) x += warp_sums[warp - 1];
-    total = warp_sums[31];
-    __syncthreads();
-    return x;
+    return warp > 0 ? x + before : x;
 }
 
+// Thread t holds the KPT rows r0 + t, r0 + 1024 + t, ... of its CTA's slice
+// (KPT 0: any number of rows, read from memory each time).
+template <int KPT>
 __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, const EvictPlan p) {
-    extern __shared__ float cache[];  // this CTA's weights
-    __shared__ int hist[3][kBins];
+    __shared__ __align__(8) int hist[3][kBins];
     __shared__ uint64_t warp_sums[32], counts[kThreads], mine;
-    __shared__ int s_digit, s_above;
+    __shared__ int s_digit, s_above, warp_counts[32];
     cg::cluster_group cluster = cg::this_cluster();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int C = p.cluster, rank = blockIdx.x % C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int h = blockIdx.x / C % a.n_head_kv, s = blockIdx.x / C / a.n_head_kv;
+    for (int i = t; i < 3 * kBins / 2; i += kThreads) reinterpret_cast<int2*>(&hist[0][0])[i] = make_int2(0, 0);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int n = batch_len(a.src, s, a.err), m = min(n, a.n_keep);
     const int64_t sh = (int64_t)s * a.n_head_kv + h;
     const float* acc = a.acc + sh * a.acc_stride;
@@ -96,10 +98,22 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
     const int want = n > m ? m - a.sink_rows - a.recent_rows : 0;
     const bool ranked = want > 0;  // else no candidate stays (or there is none)
 
-    for (int i = t; i < 3 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
-    if (p.cached)
-        for (int r = r0 + t; r < r1; r += kThreads) cache[r - r0] = acc[r];
-    auto weight = [&](int r) { return p.cached ? cache[r - r0] : acc[r]; };
+    float w[KPT > 0 ? KPT : 1];
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+        const int r = r0 + i * kThreads + t;
+        w[i] = r < r1 ? acc[r] : 0.f;
+    }
+    // f(row, weight) for this thread's rows
+    auto each = [&](auto&& f) {
+        if constexpr (KPT > 0) {
+#pragma unroll
+            for (int i = 0; i < KPT; ++i)
+                if (r0 + i * kThreads + t < r1) f(r0 + i * kThreads + t, w[i]);
+        } else {
+            for (int r = r0 + t; r < r1; r += kThreads) f(r, acc[r]);
+        }
+    };
     __syncthreads();
     uint32_t key = 0;
     int ties = 0;
@@ -109,23 +123,26 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
 #pragma unroll
         for (int d = 0; d < 3; ++d) {
             const int shift = shifts[d], bins = 1 << bits[d];
-            for (int r = max(r0, lo) + t; r < min(r1, hi); r += kThreads) {
-                const uint32_t k = weight_key(weight(r));
+            each([&](int r, float x) {
+                if (r < lo || r >= hi) return;
+                const uint32_t k = weight_key(x);
                 if (d == 0 || (k >> (shift + bits[d])) == (key >> (shift + bits[d])))
                     atomicAdd(&hist[d][(k >> shift) & (bins - 1)], 1);
-            }
+            });
             cluster.sync();
             // thread t has bins b and b - 1, counted from the top
             const int b = bins - 1 - 2 * t;
+            int2 c[kMaxCluster];
+#pragma unroll
+            for (int k = 0; k < kMaxCluster; ++k)
+                c[k] = b > 0 && k < C
+                           ? *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[d][0], k) + b - 1)
+                           : make_int2(0, 0);
             int c0 = 0, c1 = 0;
-            if (b > 0)
-                for (int c = 0; c < C; ++c) {
-                    const int* other = cluster.map_shared_rank(&hist[d][0], c);
-                    c0 += other[b];
-                    c1 += other[b - 1];
-                }
-            uint64_t total;
-            const int upto = (int)scan_cta((uint64_t)(c0 + c1), warp_sums, total);
+#pragma unroll
+            for (int k = 0; k < kMaxCluster; ++k) c0 += c[k].y, c1 += c[k].x;
+            int total;
+            const int upto = scan_cta(c0 + c1, warp_counts, total);
             const int above = upto - c0 - c1;
             if (above < left && left <= upto) {
                 const bool first = left <= above + c0;
@@ -140,111 +157,152 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
         ties = left;  // rows equal to `key` that stay, the first ones
     }
     // 1 << 32: the row stays whatever comes before it; 1: it equals `key`
-    auto mark = [&](int r) -> uint64_t {
+    auto mark = [&](int r, float x) -> uint64_t {
         if (r >= r1) return 0;
         if (r < lo || r >= hi) return 1ull << 32;
         if (!ranked) return 0;
-        const uint32_t k = weight_key(weight(r));
+        const uint32_t k = weight_key(x);
         return k > key ? 1ull << 32 : k == key ? 1ull : 0ull;
     };
-    // this CTA's counts, then those of the CTAs before it
-    uint64_t sum = 0;
-    for (int r = r0 + t; r < r1; r += kThreads) sum += mark(r);
-    uint64_t total;
-    scan_cta(sum, warp_sums, total);
-    if (t == 0) mine = total;
-    cluster.sync();
-    uint64_t base = 0;
-    for (int c = 0; c < rank; ++c) base += *cluster.map_shared_rank(&mine, c);
-    // places, up to 1024 runs of 32 rows at a time
+    // both kinds of marks of a warp's 32 rows
+    auto votes = [&](uint64_t f, uint32_t& hard, uint32_t& eq) {
+        hard = __ballot_sync(0xffffffffu, f >> 32 != 0);
+        eq = __ballot_sync(0xffffffffu, f & 1);
+    };
     int32_t* list = p.list + sh * p.cap;
     int32_t* kept_rows = a.kept_rows ? a.kept_rows + sh * a.n_keep : nullptr;
-    float* acc_dst = a.acc_dst && (p.cached || a.acc_dst != a.acc) ? a.acc_dst + sh * a.acc_dst_stride : nullptr;
-    for (int c0 = r0; c0 < r1; c0 += kThreads * 32) {
-        const int runs = min(kThreads, (r1 - c0 + 31) / 32);
-        for (int g = warp; g < runs; g += kWarps) {
-            const uint64_t f = mark(c0 + g * 32 + lane);
-            const uint32_t hard = __ballot_sync(0xffffffffu, f >> 32 != 0), eq = __ballot_sync(0xffffffffu, f & 1);
-            if (lane == 0) counts[g] = ((uint64_t)__popc(hard) << 32) | (uint32_t)__popc(eq);
+    float* acc_dst = a.acc_dst && (KPT > 0 || a.acc_dst != a.acc) ? a.acc_dst + sh * a.acc_dst_stride : nullptr;
+    auto place = [&](int r, float x, uint64_t f, uint64_t before) {
+        uint32_t hard, eq;
+        votes(f, hard, eq);
+        const uint32_t below = (1u << lane) - 1;
+        const int n_hard = (int)(before >> 32) + __popc(hard & below);
+        const int n_eq = (int)(uint32_t)before + __popc(eq & below);
+        if (f >> 32 != 0 || ((f & 1) && n_eq < ties)) {
+            const int at = n_hard + min(n_eq, ties);
+            list[at] = r;
+            if (kept_rows) kept_rows[at] = r;
+            if (acc_dst) acc_dst[at] = x;
+        }
+    };
+    auto word = [](uint32_t hard, uint32_t eq) { return ((uint64_t)__popc(hard) << 32) | (uint32_t)__popc(eq); };
+    // the counts of the CTAs before this one
+    auto base_of = [&](uint64_t total) {
+        if (t == 0) mine = total;
+        cluster.sync();
+        uint64_t v[kMaxCluster], base = 0;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) v[k] = k < rank ? *cluster.map_shared_rank(&mine, k) : 0;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) base += v[k];
+        return base;
+    };
+    uint64_t total;
+    if constexpr (KPT > 0) {
+        // rows in order are runs of 32, run i * 32 + warp
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            uint32_t hard, eq;
+            votes(mark(r0 + i * kThreads + t, w[i]), hard, eq);
+            if (lane == 0) counts[i * kWarps + warp] = word(hard, eq);
         }
         __syncthreads();
-        const uint64_t own = t < runs ? counts[t] : 0;
+        const uint64_t own = t < KPT * kWarps ? counts[t] : 0;
         const uint64_t incl = scan_cta(own, warp_sums, total);
+        const uint64_t base = base_of(total);
         counts[t] = base + incl - own;
+        cluster.barrier_arrive();  // `mine` of the others has been read
         __syncthreads();
-        for (int g = warp; g < runs; g += kWarps) {
-            const int r = c0 + g * 32 + lane;
-            const uint64_t f = mark(r);
-            const uint32_t hard = __ballot_sync(0xffffffffu, f >> 32 != 0), eq = __ballot_sync(0xffffffffu, f & 1);
-            const uint32_t below = (1u << lane) - 1;
-            const uint64_t before = counts[g];
-            const int n_hard = (int)(before >> 32) + __popc(hard & below);
-            const int n_eq = (int)(uint32_t)before + __popc(eq & below);
-            if (f >> 32 != 0 || ((f & 1) && n_eq < ties)) {
-                const int at = n_hard + min(n_eq, ties);
-                list[at] = r;
-                if (kept_rows) kept_rows[at] = r;
-                if (acc_dst) acc_dst[at] = weight(r);
-            }
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const int r = r0 + i * kThreads + t;
+            place(r, w[i], mark(r, w[i]), counts[i * kWarps + warp]);
         }
-        base += total;
-        __syncthreads();
+    } else {
+        uint64_t sum = 0;
+        each([&](int r, float x) { sum += mark(r, x); });
+        scan_cta(sum, warp_sums, total);
+        uint64_t base = base_of(total);
+        cluster.barrier_arrive();
+        for (int c0 = r0; c0 < r1; c0 += kThreads * 32) {
+            const int runs = min(kThreads, (r1 - c0 + 31) / 32);
+            auto weight = [&](int r) { return r < r1 ? acc[r] : 0.f; };
+            for (int g = warp; g < runs; g += kWarps) {
+                uint32_t hard, eq;
+                votes(mark(c0 + g * 32 + lane, weight(c0 + g * 32 + lane)), hard, eq);
+                if (lane == 0) counts[g] = word(hard, eq);
+            }
+            __syncthreads();
+            const uint64_t own = t < runs ? counts[t] : 0;
+            const uint64_t incl = scan_cta(own, warp_sums, total);
+            counts[t] = base + incl - own;
+            __syncthreads();
+            for (int g = warp; g < runs; g += kWarps) {
+                const int r = c0 + g * 32 + lane;
+                const float x = weight(r);
+                place(r, x, mark(r, x), counts[g]);
+            }
+            base += total;
+            __syncthreads();
+        }
     }
     if (kept_rows)
         for (int i = m + rank * kThreads + t; i < a.n_keep; i += C * kThreads) kept_rows[i] = -1;
     if (acc_dst)
         for (int i = m + rank * kThreads + t; i < a.acc_dst_stride; i += C * kThreads) acc_dst[i] = 0.f;
-    cluster.sync();  // no CTA leaves while another reads its counts
+    cluster.barrier_wait();  // no CTA leaves while another reads its counts
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = kMoveThreads / 32 * 32;  // kept rows per CTA
+constexpr int kMoveUnroll = 8;  // a thread's loads under way
 
-// Grid (KV head, rows / kMoveRows, sequence): gathers into other rows than the
-// source's.
+// Kept rows a warp moves: a row of K and V is 2 NV 16-byte vectors.
+constexpr int move_rows(int nv) { return 2 * nv > 32 ? kMoveUnroll / 2 : kMoveUnroll * (32 / (2 * nv)); }
+
+// Grid (KV head, rows / (8 warps' rows), sequence): gathers into other rows
+// than the source's.
 template <int NV>  // 16-byte vectors of a row
 __global__ void __launch_bounds__(kMoveThreads) k8b_move(const EvictArgs a, const EvictPlan p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    constexpr int kRows = move_rows(NV);
+    constexpr int kTurns = 2 * NV > 32 ? 2 * NV / 32 : 1;
+    constexpr int kAtOnce = 2 * NV > 32 ? 1 : 32 / (2 * NV);
     const int h = blockIdx.x, s = blockIdx.z, lane = threadIdx.x & 31;
-    const int i0 = (blockIdx.y * (kMoveThreads / 32) + (threadIdx.x >> 5)) * 32;
+    const int i0 = (blockIdx.y * (kMoveThreads / 32) + (threadIdx.x >> 5)) * kRows;
+    const int i = i0 + lane;
+    // (the list's capacity, not the count, bounds this load: both arrive together)
+    const int row = lane < kRows && i < p.cap ? p.list[((int64_t)s * a.n_head_kv + h) * p.cap + i] : -1;
     const int m = p.kept[s];
     if (a.new_lens && h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_lens[s] = m;
     if (i0 >= m) return;
     int from = -1, to = -1;
-    if (i0 + lane < m) {
-        from = batch_row(a.src, s, p.list[((int64_t)s * a.n_head_kv + h) * p.cap + i0 + lane], a.err);
-        to = batch_row(a.dst, s, i0 + lane, a.err);
+    if (lane < kRows && i < m) {
+        from = batch_row(a.src, s, row, a.err);
+        to = batch_row(a.dst, s, i, a.err);
     }
-    // a row of K and V is 2 NV vectors: 32 / (2 NV) rows at a time (or 2 NV / 32 turns for one)
-    constexpr int kTurns = 2 * NV > 32 ? 2 * NV / 32 : 1;
-    constexpr int kAtOnce = 2 * NV > 32 ? 1 : 32 / (2 * NV);
-    const int cnt = min(32, m - i0);
-    constexpr int kUnroll = 8;
-    for (int j0 = 0; j0 < cnt; j0 += kAtOnce * kUnroll) {
-        uint4 x[kUnroll][kTurns];
-        int dst[kUnroll];
+    uint4 x[kRows / kAtOnce][kTurns];
+    int dst[kRows / kAtOnce];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int j = j0 + u * kAtOnce + (kAtOnce > 1 ? lane / (2 * NV) : 0);
-            const int f = __shfl_sync(0xffffffffu, from, j & 31), d = __shfl_sync(0xffffffffu, to, j & 31);
-            dst[u] = j < cnt && f >= 0 ? d : -1;
+    for (int u = 0; u < kRows / kAtOnce; ++u) {
+        const int j = u * kAtOnce + (kAtOnce > 1 ? lane / (2 * NV) : 0);
+        const int f = __shfl_sync(0xffffffffu, from, j), d = __shfl_sync(0xffffffffu, to, j);
+        dst[u] = f >= 0 ? d : -1;
 #pragma unroll
-            for (int v = 0; v < kTurns; ++v) {
-                const int c = (lane + v * 32) % (2 * NV);
-                const void* base = c < NV ? a.k : a.v;
-                if (dst[u] >= 0)
-                    x[u][v] = *(static_cast<const uint4*>(base) + ((int64_t)f * a.n_head_kv + h) * NV + c % NV);
-            }
+        for (int v = 0; v < kTurns; ++v) {
+            const int c = (lane + v * 32) % (2 * NV);
+            const void* base = c < NV ? a.k : a.v;
+            if (dst[u] >= 0) x[u][v] = *(static_cast<const uint4*>(base) + ((int64_t)f * a.n_head_kv + h) * NV + c % NV);
         }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int v = 0; v < kTurns; ++v) {
-                const int c = (lane + v * 32) % (2 * NV);
-                void* base = c < NV ? a.k_dst : a.v_dst;
-                if (dst[u] >= 0) *(static_cast<uint4*>(base) + ((int64_t)dst[u] * a.n_head_kv + h) * NV + c % NV) = x[u][v];
-            }
     }
+#pragma unroll
+    for (int u = 0; u < kRows / kAtOnce; ++u)
+#pragma unroll
+        for (int v = 0; v < kTurns; ++v) {
+            const int c = (lane + v * 32) % (2 * NV);
+            void* base = c < NV ? a.k_dst : a.v_dst;
+            if (dst[u] >= 0) *(static_cast<uint4*>(base) + ((int64_t)dst[u] * a.n_head_kv + h) * NV + c % NV) = x[u][v];
+        }
 }
 
 constexpr int kPlaceThreads = 512;
@@ -253,6 +311,7 @@ constexpr int kPlaceThreads = 512;
 // K or V where it is.
 __global__ void __launch_bounds__(kPlaceThreads) k8c_compact(const EvictArgs a, const EvictPlan p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int nv = a.head_dim * a.elem_bytes / 16, cols = nv / 2;  // 16-byte vectors, 32-byte columns of a row
     const int h = blockIdx.y, s = blockIdx.z, t = threadIdx.x;
     const int m = p.kept[s];
@@ -301,10 +360,11 @@ size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 size_t plan_of(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t n_head_kv, char* ws, EvictPlan* p) {
     p->cap = n_keep < max_kv_len ? n_keep : max_kv_len;
-    // a CTA per 2048 rows, up to 8 per head
+    // a CTA per kClusterRows rows, up to 8 per head
     p->cluster = 1;
-    while (p->cluster < kMaxCluster && p->cluster * 2048 < max_kv_len) p->cluster *= 2;
-    p->cached = (max_kv_len + p->cluster - 1) / p->cluster + 31 <= kCacheRows;
+    while (p->cluster < kMaxCluster && p->cluster * kClusterRows < max_kv_len) p->cluster *= 2;
+    const int each = ((max_kv_len + p->cluster - 1) / p->cluster + 31) & ~31;
+    p->per_thread = each <= 2 * kThreads ? 2 : each <= 8 * kThreads ? 8 : each <= 32 * kThreads ? 32 : 0;
     p->kept = reinterpret_cast<int32_t*>(ws);
     const size_t head = up16((size_t)n_seq * sizeof(int32_t));
     p->list = reinterpret_cast<int32_t*>(ws + head);
@@ -335,41 +395,36 @@ size_t evict_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t
 cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s) {
     EvictPlan p{};
     plan_of(a.src.n_seq, a.src.max_kv_len, a.n_keep, a.n_head_kv, static_cast<char*>(a.ws), &p);
-    const int smem = p.cached ? (((a.src.max_kv_len + p.cluster - 1) / p.cluster + 31) & ~31) * (int)sizeof(float) : 0;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    static std::atomic<unsigned> set_mask{0};
-    if (dev >= 32 || !(set_mask.load(std::memory_order_acquire) & (1u << dev))) {
-        const cudaError_t e = cudaFuncSetAttribute(k8a_select_rows, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   kCacheRows * (int)sizeof(float));
-        if (e != cudaSuccess) return e;
-        if (dev < 32) set_mask.fetch_or(1u << dev, std::memory_order_release);
-    }
     const int64_t ctas = (int64_t)a.src.n_seq * a.n_head_kv * p.cluster;
     if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = p.cluster;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, k8a_select_rows, a, p);
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = p.cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    cudaError_t e = p.per_thread == 2    ? cudaLaunchKernelEx(&cfg, k8a_select_rows<2>, a, p)
+                    : p.per_thread == 8  ? cudaLaunchKernelEx(&cfg, k8a_select_rows<8>, a, p)
+                    : p.per_thread == 32 ? cudaLaunchKernelEx(&cfg, k8a_select_rows<32>, a, p)
+                                         : cudaLaunchKernelEx(&cfg, k8a_select_rows<0>, a, p);
     if (e != cudaSuccess) return e;
     const int nv = a.head_dim * a.elem_bytes / 16;
     if (a.in_place) {
         e = launch_after(k8c_compact, dim3(nv, a.n_head_kv, a.src.n_seq), kPlaceThreads, s, a, p);
     } else {
-        const dim3 grid(a.n_head_kv, (p.cap + kMoveRows - 1) / kMoveRows, a.src.n_seq);
+        const int rows = move_rows(nv) * (kMoveThreads / 32);
+        const dim3 grid(a.n_head_kv, (p.cap + rows - 1) / rows, a.src.n_seq);
         if (nv == 8) e = launch_after(k8b_move<8>, grid, kMoveThreads, s, a, p);
         else if (nv == 16) e = launch_after(k8b_move<16>, grid, kMoveThreads, s, a, p);
         else e = launch_after(k8b_move<32>, grid, kMoveThreads, s, a, p);
     }
-    if (e == cudaSuccess && a.acc_dst == a.acc && !p.cached) {
+    if (e == cudaSuccess && a.acc_dst == a.acc && p.per_thread == 0) {
         k8d_compact_weights<<<dim3(a.n_head_kv, a.src.n_seq), kThreads, 0, s>>>(a, p);
         e = cudaGetLastError();
     }

@@ -635,45 +635,55 @@ struct F32Plan {
     float* nlse;     // [Hkv][n_rt * 64]: minus the lse, -inf for rows that are none
 };
 
-// 64 rows of `D` floats into shared memory, rows padded by 16 bytes (the 4 x 4
-// product reads 8 rows at once without a bank conflict).  src(r): the row's
-// address, null for zeros.
-template <int D, class F>
-__device__ __forceinline__ void load_rows_f32(float* dst, F&& src) {
-    for (int i = threadIdx.x; i < FT * (D / 4); i += kF32Threads) {
-        const int r = i / (D / 4), c = i % (D / 4);
-        const float* p = src(r);
-        *reinterpret_cast<float4*>(dst + r * (D + 4) + c * 4) =
-            p != nullptr ? *reinterpret_cast<const float4*>(p + c * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-}
-
+// 64 rows of D floats on their way into shared memory: fetch has all of a
+// thread's loads under way at once, store follows when the buffer is free.
+// Rows are padded by 16 bytes (the 4 x 4 product reads 8 rows at once without
+// a bank conflict).
 template <int D>
-__device__ __forceinline__ void load_queries_f32(const WeightArgs& a, const F32Plan& p, float* dst, int rt, int h) {
-    const int G = a.n_head / a.n_head_kv;
-    load_rows_f32<D>(dst, [&](int r) -> const float* {
-        const int i = rt * FT + r;
-        if (i >= p.n_rows) return nullptr;
-        const int tok = i / G;
-        return static_cast<const float*>(a.q) +
-               ((int64_t)(a.row_begin + tok) * a.n_head + h * G + (i - tok * G)) * D;
-    });
-}
-
-template <int D>
-__device__ __forceinline__ void load_keys_f32(const WeightArgs& a, float* dst, int kt, int h) {
-    load_rows_f32<D>(dst, [&](int r) -> const float* {
-        const int j = kt * FT + r;
-        if (j >= a.kv_len) return nullptr;
-        bool bad = false;
-        const int row = phys_row(a.paging, j, bad);
-        if (bad) {
-            report_error(a.err, kDevBadBlockTable, 0x92, j);
-            return nullptr;
+struct RowsF32 {
+    static constexpr int kN = FT * (D / 4) / kF32Threads;
+    float4 v[kN];
+    // src(r): the row's address, null for zeros
+    template <class F>
+    __device__ __forceinline__ void fetch(F&& src) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            const int i = threadIdx.x + n * kF32Threads;
+            const float* p = src(i / (D / 4));
+            v[n] = p != nullptr ? *reinterpret_cast<const float4*>(p + i % (D / 4) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        return static_cast<const float*>(a.k) + ((int64_t)row * a.n_head_kv + h) * D;
-    });
-}
+    }
+    __device__ __forceinline__ void store(float* dst) const {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            const int i = threadIdx.x + n * kF32Threads;
+            *reinterpret_cast<float4*>(dst + i / (D / 4) * (D + 4) + i % (D / 4) * 4) = v[n];
+        }
+    }
+    __device__ __forceinline__ void fetch_queries(const WeightArgs& a, int n_rows, int rt, int h) {
+        const int G = a.n_head / a.n_head_kv;
+        fetch([&](int r) -> const float* {
+            const int i = rt * FT + r;
+            if (i >= n_rows) return nullptr;
+            const int tok = i / G;
+            return static_cast<const float*>(a.q) +
+                   ((int64_t)(a.row_begin + tok) * a.n_head + h * G + (i - tok * G)) * D;
+        });
+    }
+    __device__ __forceinline__ void fetch_keys(const WeightArgs& a, int kt, int h) {
+        fetch([&](int r) -> const float* {
+            const int j = kt * FT + r;
+            if (j >= a.kv_len) return nullptr;
+            bool bad = false;
+            const int row = phys_row(a.paging, j, bad);
+            if (bad) {
+                report_error(a.err, kDevBadBlockTable, 0x92, j);
+                return nullptr;
+            }
+            return static_cast<const float*>(a.k) + ((int64_t)row * a.n_head_kv + h) * D;
+        });
+    }
+};
 
 // x[i][j] = q row (ty + 16 i) . k row (tx + 16 j)
 template <int D>
@@ -724,11 +734,18 @@ __global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, 
         m[i] = -INFINITY;
         l[i] = 0.f;
     }
-    load_queries_f32<D>(a, p, q, rt, h);
+    RowsF32<D> next;
+    {
+        RowsF32<D> rows;
+        rows.fetch_queries(a, p.n_rows, rt, h);
+        if (k0 < k1) next.fetch_keys(a, k0, h);
+        rows.store(q);
+    }
     for (int kt = k0; kt < k1; ++kt) {
         __syncthreads();
-        load_keys_f32<D>(a, k, kt, h);
+        next.store(k);
         __syncthreads();
+        if (kt + 1 < k1) next.fetch_keys(a, kt + 1, h);
         float x[4][4];
         scores_f32<D>(q, k, ty, tx, x);
 #pragma unroll
@@ -777,14 +794,21 @@ __global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, c
     const float sl2 = a.kq_scale * 1.4426950408889634f;
     tc::pdl_wait();
     tc::pdl_launch();
-    load_keys_f32<D>(a, k, kt, h);
     const float* nlse = p.nlse + (int64_t)h * p.n_rt * FT;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     const int r0 = max(0, (int)((int64_t)(kt * FT - t_first) * G / FT));  // first tile with a row that sees the keys
+    RowsF32<D> next;
+    {
+        RowsF32<D> rows;
+        rows.fetch_keys(a, kt, h);
+        if (r0 < p.n_rt) next.fetch_queries(a, p.n_rows, r0, h);
+        rows.store(k);
+    }
     for (int rt = r0; rt < p.n_rt; ++rt) {
         __syncthreads();
-        load_queries_f32<D>(a, p, q, rt, h);
+        next.store(q);
         __syncthreads();
+        if (rt + 1 < p.n_rt) next.fetch_queries(a, p.n_rows, rt + 1, h);
         float x[4][4];
         scores_f32<D>(q, k, ty, tx, x);
 #pragma unroll
@@ -819,9 +843,9 @@ size_t plan_f32(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv,
     p->n_rows = (int32_t)n_rows;
     p->n_rt = (p->n_rows + FT - 1) / FT;
     p->n_kt = (kv_len + FT - 1) / FT;
-    // three CTAs fit an SM: split the keys until the device is full
+    // two CTAs fit an SM: split the keys until the device is full
     const int64_t ctas = (int64_t)n_head_kv * p->n_rt;
-    p->splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_kt, 3 * kSms / ctas));
+    p->splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_kt, 2 * kSms / ctas));
     const size_t n = (size_t)n_head_kv * p->n_rt * FT, ml = up16(n * p->splits * sizeof(float2));
     p->ml = reinterpret_cast<float2*>(ws);
     p->nlse = reinterpret_cast<float*>(ws + ml);
