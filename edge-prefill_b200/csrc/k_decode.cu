@@ -58,7 +58,7 @@ constexpr int kMinUnits = K6_MIN_UNITS;
 // What a run costs a CTA besides its units (the merge of the warps' states),
 // in units: the ranges are equal in this measure.
 #ifndef K6_RUN_COST
-#define K6_RUN_COST 4
+#define K6_RUN_COST 6
 #endif
 constexpr int kRunCost = K6_RUN_COST;
 constexpr int kLensOnChip = 1024;  // lengths a CTA keeps in shared memory

@@ -8,7 +8,8 @@
 // up to 8 CTAs, which keep their slice of the weights in registers (one read
 // of the weights) and add their histograms through distributed shared
 // memory; only counts are exchanged, so the result is exact and has no order.
-// Latency bounds it: three histogram rounds, each with one cluster barrier.
+// Latency bounds it: a histogram round is one cluster barrier and a few block
+// ones; the third, and often the second, is skipped when the whole bin stays.
 //
 // K8b moves the listed rows, which the bytes bound: a warp takes as many rows
 // as fill its lanes with eight 16-byte loads each.  In place there is an order to
@@ -80,7 +81,7 @@ template <int KPT>
 __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, const EvictPlan p) {
     __shared__ __align__(8) int hist[3][kBins];
     __shared__ uint64_t warp_sums[32], counts[kThreads], mine;
-    __shared__ int s_digit, s_above, warp_counts[32];
+    __shared__ int s_digit, s_above, s_all, warp_counts[32];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = p.cluster, rank = blockIdx.x % C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int h = blockIdx.x / C % a.n_head_kv, s = blockIdx.x / C / a.n_head_kv;
@@ -116,7 +117,11 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
     };
     __syncthreads();
     uint32_t key = 0;
-    int ties = 0;
+    int ties = 0, known = 0;  // rows that share the key's bits from `known` on are equal
+    auto sync_all = [&]() {
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+    };
     if (ranked) {  // the same in the whole cluster
         int left = want;
         const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
@@ -129,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
                 if (d == 0 || (k >> (shift + bits[d])) == (key >> (shift + bits[d])))
                     atomicAdd(&hist[d][(k >> shift) & (bins - 1)], 1);
             });
-            cluster.sync();
+            sync_all();
             // thread t has bins b and b - 1, counted from the top
             const int b = bins - 1 - 2 * t;
             int2 c[kMaxCluster];
@@ -148,11 +153,15 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
                 const bool first = left <= above + c0;
                 s_digit = first ? b : b - 1;
                 s_above = first ? above : above + c0;
+                s_all = (first ? c0 : c1) == left - s_above;
             }
             __syncthreads();
             key |= (uint32_t)s_digit << shift;
             left -= s_above;
+            known = shift;
+            const bool all = s_all;  // the whole bin stays: no need to look into it
             __syncthreads();
+            if (all) break;
         }
         ties = left;  // rows equal to `key` that stay, the first ones
     }
@@ -161,8 +170,8 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
         if (r >= r1) return 0;
         if (r < lo || r >= hi) return 1ull << 32;
         if (!ranked) return 0;
-        const uint32_t k = weight_key(x);
-        return k > key ? 1ull << 32 : k == key ? 1ull : 0ull;
+        const uint32_t k = weight_key(x) >> known, edge = key >> known;
+        return k > edge ? 1ull << 32 : k == edge ? 1ull : 0ull;
     };
     // both kinds of marks of a warp's 32 rows
     auto votes = [&](uint64_t f, uint32_t& hard, uint32_t& eq) {
@@ -189,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
     // the counts of the CTAs before this one
     auto base_of = [&](uint64_t total) {
         if (t == 0) mine = total;
-        cluster.sync();
+        sync_all();
         uint64_t v[kMaxCluster], base = 0;
 #pragma unroll
         for (int k = 0; k < kMaxCluster; ++k) v[k] = k < rank ? *cluster.map_shared_rank(&mine, k) : 0;
