@@ -78,14 +78,17 @@ __device__ __forceinline__ T scan_cta(T x, T* warp_sums, T& total) {
 // Thread t holds the KPT rows r0 + t, r0 + 1024 + t, ... of its CTA's slice
 // (KPT 0: any number of rows, read from memory each time).
 template <int KPT>
-__global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, const EvictPlan p) {
-    __shared__ __align__(8) int hist[3][kBins];
+__global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a, const EvictPlan p) {
+    // counts of up to 32 K rows share a word with their neighbour's: half the
+    // bytes to read from the other CTAs
+    constexpr bool kPairs = KPT > 0;
+    __shared__ __align__(8) int hist[3][kPairs ? kBins / 2 : kBins];
     __shared__ uint64_t warp_sums[32], counts[kThreads], mine;
     __shared__ int s_digit, s_above, s_all, warp_counts[32];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = p.cluster, rank = blockIdx.x % C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int h = blockIdx.x / C % a.n_head_kv, s = blockIdx.x / C / a.n_head_kv;
-    for (int i = t; i < 3 * kBins / 2; i += kThreads) reinterpret_cast<int2*>(&hist[0][0])[i] = make_int2(0, 0);
+    for (int i = t; i < (int)(sizeof(hist) / 8); i += kThreads) reinterpret_cast<int2*>(&hist[0][0])[i] = make_int2(0, 0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int n = batch_len(a.src, s, a.err), m = min(n, a.n_keep);
@@ -131,21 +134,30 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
             each([&](int r, float x) {
                 if (r < lo || r >= hi) return;
                 const uint32_t k = weight_key(x);
-                if (d == 0 || (k >> (shift + bits[d])) == (key >> (shift + bits[d])))
-                    atomicAdd(&hist[d][(k >> shift) & (bins - 1)], 1);
+                if (d == 0 || (k >> (shift + bits[d])) == (key >> (shift + bits[d]))) {
+                    const int b = (k >> shift) & (bins - 1);
+                    if constexpr (kPairs) atomicAdd(&hist[d][b >> 1], b & 1 ? 65536 : 1);
+                    else atomicAdd(&hist[d][b], 1);
+                }
             });
             sync_all();
             // thread t has bins b and b - 1, counted from the top
             const int b = bins - 1 - 2 * t;
             int2 c[kMaxCluster];
 #pragma unroll
-            for (int k = 0; k < kMaxCluster; ++k)
-                c[k] = b > 0 && k < C
-                           ? *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[d][0], k) + b - 1)
-                           : make_int2(0, 0);
+            for (int k = 0; k < kMaxCluster; ++k) {
+                c[k] = make_int2(0, 0);
+                if (b < 0 || k >= C) continue;
+                const int* other = cluster.map_shared_rank(&hist[d][0], k);
+                if constexpr (kPairs) c[k].x = other[b >> 1];
+                else c[k] = *reinterpret_cast<const int2*>(other + b - 1);
+            }
             int c0 = 0, c1 = 0;
 #pragma unroll
-            for (int k = 0; k < kMaxCluster; ++k) c0 += c[k].y, c1 += c[k].x;
+            for (int k = 0; k < kMaxCluster; ++k) {
+                c0 += kPairs ? (int)((uint32_t)c[k].x >> 16) : c[k].y;
+                c1 += kPairs ? c[k].x & 0xffff : c[k].x;
+            }
             int total;
             const int upto = scan_cta(c0 + c1, warp_counts, total);
             const int above = upto - c0 - c1;
@@ -165,36 +177,34 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
         }
         ties = left;  // rows equal to `key` that stay, the first ones
     }
-    // 1 << 32: the row stays whatever comes before it; 1: it equals `key`
-    auto mark = [&](int r, float x) -> uint64_t {
-        if (r >= r1) return 0;
-        if (r < lo || r >= hi) return 1ull << 32;
-        if (!ranked) return 0;
-        const uint32_t k = weight_key(x) >> known, edge = key >> known;
-        return k > edge ? 1ull << 32 : k == edge ? 1ull : 0ull;
-    };
-    // both kinds of marks of a warp's 32 rows
-    auto votes = [&](uint64_t f, uint32_t& hard, uint32_t& eq) {
-        hard = __ballot_sync(0xffffffffu, f >> 32 != 0);
-        eq = __ballot_sync(0xffffffffu, f & 1);
+    // a row stays whatever comes before it, or it equals `key`
+    const uint32_t edge = key >> known;
+    auto mark = [&](int r, float x, bool& hard, bool& eq) {
+        const bool cand = r >= lo && r < hi;
+        const uint32_t k = weight_key(x) >> known;
+        hard = r < r1 && (!cand || (ranked && k > edge));
+        eq = r < r1 && cand && ranked && k == edge;
     };
     int32_t* list = p.list + sh * p.cap;
     int32_t* kept_rows = a.kept_rows ? a.kept_rows + sh * a.n_keep : nullptr;
     float* acc_dst = a.acc_dst && (KPT > 0 || a.acc_dst != a.acc) ? a.acc_dst + sh * a.acc_dst_stride : nullptr;
-    auto place = [&](int r, float x, uint64_t f, uint64_t before) {
-        uint32_t hard, eq;
-        votes(f, hard, eq);
+    auto place = [&](int r, float x, bool hard, bool eq, uint64_t before) {
+        const uint32_t all_hard = __ballot_sync(0xffffffffu, hard), all_eq = __ballot_sync(0xffffffffu, eq);
         const uint32_t below = (1u << lane) - 1;
-        const int n_hard = (int)(before >> 32) + __popc(hard & below);
-        const int n_eq = (int)(uint32_t)before + __popc(eq & below);
-        if (f >> 32 != 0 || ((f & 1) && n_eq < ties)) {
+        const int n_hard = (int)(before >> 32) + __popc(all_hard & below);
+        const int n_eq = (int)(uint32_t)before + __popc(all_eq & below);
+        if (hard || (eq && n_eq < ties)) {
             const int at = n_hard + min(n_eq, ties);
             list[at] = r;
             if (kept_rows) kept_rows[at] = r;
             if (acc_dst) acc_dst[at] = x;
         }
     };
-    auto word = [](uint32_t hard, uint32_t eq) { return ((uint64_t)__popc(hard) << 32) | (uint32_t)__popc(eq); };
+    // rows of a warp's 32 that stay in any case (upper half) and that equal `key`
+    auto count = [](bool hard, bool eq) {
+        const int n_hard = __popc(__ballot_sync(0xffffffffu, hard)), n_eq = __popc(__ballot_sync(0xffffffffu, eq));
+        return ((uint64_t)n_hard << 32) | (uint32_t)n_eq;
+    };
     // the counts of the CTAs before this one
     auto base_of = [&](uint64_t total) {
         if (t == 0) mine = total;
@@ -209,11 +219,15 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
     uint64_t total;
     if constexpr (KPT > 0) {
         // rows in order are runs of 32, run i * 32 + warp
+        uint32_t hards = 0, eqs = 0;  // bit i: this thread's row i
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
-            uint32_t hard, eq;
-            votes(mark(r0 + i * kThreads + t, w[i]), hard, eq);
-            if (lane == 0) counts[i * kWarps + warp] = word(hard, eq);
+            bool hard, eq;
+            mark(r0 + i * kThreads + t, w[i], hard, eq);
+            hards |= (uint32_t)hard << i;
+            eqs |= (uint32_t)eq << i;
+            const uint64_t c = count(hard, eq);
+            if (lane == 0) counts[i * kWarps + warp] = c;
         }
         __syncthreads();
         const uint64_t own = t < KPT * kWarps ? counts[t] : 0;
@@ -225,11 +239,15 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
             const int r = r0 + i * kThreads + t;
-            place(r, w[i], mark(r, w[i]), counts[i * kWarps + warp]);
+            place(r, w[i], hards >> i & 1, eqs >> i & 1, counts[i * kWarps + warp]);
         }
     } else {
         uint64_t sum = 0;
-        each([&](int r, float x) { sum += mark(r, x); });
+        each([&](int r, float x) {
+            bool hard, eq;
+            mark(r, x, hard, eq);
+            sum += ((uint64_t)hard << 32) | (uint32_t)eq;
+        });
         scan_cta(sum, warp_sums, total);
         uint64_t base = base_of(total);
         cluster.barrier_arrive();
@@ -237,9 +255,11 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
             const int runs = min(kThreads, (r1 - c0 + 31) / 32);
             auto weight = [&](int r) { return r < r1 ? acc[r] : 0.f; };
             for (int g = warp; g < runs; g += kWarps) {
-                uint32_t hard, eq;
-                votes(mark(c0 + g * 32 + lane, weight(c0 + g * 32 + lane)), hard, eq);
-                if (lane == 0) counts[g] = word(hard, eq);
+                const int r = c0 + g * 32 + lane;
+                bool hard, eq;
+                mark(r, weight(r), hard, eq);
+                const uint64_t c = count(hard, eq);
+                if (lane == 0) counts[g] = c;
             }
             __syncthreads();
             const uint64_t own = t < runs ? counts[t] : 0;
@@ -249,7 +269,9 @@ __global__ void __launch_bounds__(kThreads) k8a_select_rows(const EvictArgs a, c
             for (int g = warp; g < runs; g += kWarps) {
                 const int r = c0 + g * 32 + lane;
                 const float x = weight(r);
-                place(r, x, mark(r, x), counts[g]);
+                bool hard, eq;
+                mark(r, x, hard, eq);
+                place(r, x, hard, eq, counts[g]);
             }
             base += total;
             __syncthreads();
