@@ -64,9 +64,11 @@ int32_t ensure_device(ep_sp_ctx* c) {
         cudaGetLastError();
         return fail(c, kUnavailable, "no CUDA device " + std::to_string(c->cfg.device));
     }
-    cudaDeviceProp prop;
-    if (cudaGetDeviceProperties(&prop, c->cfg.device) != cudaSuccess) return fail(c, kUnavailable, "device query failed");
-    if (prop.major != 10) return fail(c, kUnsupported, std::string("not an sm_100 device: ") + prop.name);
+    int major = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, c->cfg.device) != cudaSuccess)
+        return fail(c, kUnavailable, "device query failed");
+    if (major != 10)
+        return fail(c, kUnsupported, "not an sm_100 device: compute capability " + std::to_string(major) + ".x");
     cudaError_t e = cudaSetDevice(c->cfg.device);
     if (e != cudaSuccess) return cuda_fail(c, e, "cudaSetDevice");
     const int32_t Hkv = c->cfg.n_head_kv, d = c->cfg.head_dim, nl = c->cfg.n_layer;

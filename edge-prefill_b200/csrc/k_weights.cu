@@ -24,6 +24,7 @@
 #include <atomic>
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "epsp_kernels.h"
 #include "tc100.cuh"
@@ -108,7 +109,9 @@ struct WeightPlan {
     int32_t resident;  // sums pass: every query tile stays on chip
     int32_t q_slots, k_slots;  // sums pass
     int32_t kg;        // sums pass: key tiles a CTA works on at a time (1, 2)
-    int32_t b_splits;  // sums pass: CTAs per KV head
+    int32_t b_splits;  // sums pass: CTAs per KV head (and row split)
+    int32_t r_splits;  // sums pass: parts the query tiles are split into
+    float* part;       // [r_splits][Hkv][n_kt * 128] sums of each part (r_splits > 1)
     float2* ml;        // [splits][Hkv][n_rt * 128]
     float* nlse;       // [Hkv][n_rt * 128]: minus the lse, log2 units, -inf for rows that are none
 };
@@ -234,9 +237,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         q_slots = p.group;
         k_slots = LY::kSlots - p.group;
     } else {
-        h = blockIdx.x / p.b_splits;
-        n_q = p.n_rt;
-        k0 = blockIdx.x % p.b_splits;  // groups of kg key tiles: k0, k0 + b_splits, ...
+        const int rs = blockIdx.x % p.r_splits, rest = blockIdx.x / p.r_splits;
+        h = rest / p.b_splits;
+        rt0 = (int)((int64_t)p.n_rt * rs / p.r_splits);
+        n_q = (int)((int64_t)p.n_rt * (rs + 1) / p.r_splits) - rt0;
+        k0 = rest % p.b_splits;  // groups of kg key tiles: k0, k0 + b_splits, ...
         k1 = (p.n_kt + p.kg - 1) / p.kg;
         q_slots = p.q_slots;
         k_slots = p.k_slots;
@@ -283,11 +288,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t tmem = *tmem_slot;
     const int q_bytes = D / 64 * 64 * 2 * p.T * G;
 
-    // first query tile that sees any key of group kgi (sums pass)
-    // (on chip, all are taken: there are few)
+    // first of the CTA's query tiles that sees any key of group kgi, n_q or
+    // more if none does (sums pass; on chip, all are taken: there are few)
     auto rt_from = [&](int kgi) {
         const int late = kgi * p.kg * BM - t_first;
-        return !stream_q || late < p.T ? 0 : late / p.T;
+        return !stream_q || late < p.T ? 0 : max(0, late / p.T - rt0);
     };
 
     if (warp == 0) {
@@ -308,21 +313,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int i = 0; i < n_q; ++i)
                     load_queries<D>(a, p, &tmQ, smem + i * LY::kTile, &b.qf[0], rt0 + i, h);
                 if constexpr (PASS == 1)
-                    tc::bulk_load(lse_s, p.nlse + (int64_t)h * p.n_rt * BM, BM * 4 * n_q, &b.qf[0]);
+                    tc::bulk_load(lse_s, p.nlse + ((int64_t)h * p.n_rt + rt0) * BM, BM * 4 * n_q, &b.qf[0]);
             }
             if constexpr (PASS == 0) {
                 for (int kt = k0; kt < k1 && ok; ++kt) keys(kt);
             } else {
                 for (int g = k0; g < k1 && ok; g += p.b_splits) {
+                    const int r0 = rt_from(g);
+                    if (r0 >= n_q) continue;
                     for (int k = 0; k < p.kg && g * p.kg + k < p.n_kt && ok; ++k) keys(g * p.kg + k);
                     if (!stream_q) continue;
-                    for (int rt = rt_from(g); rt < n_q && ok; ++rt) {
+                    for (int rt = r0; rt < n_q && ok; ++rt) {
                         const int s = qr.slot;
                         ok = tc::mbar_wait(&b.qe[s], qr.phase ^ 1, tmo);
                         if (!ok) break;
                         tc::mbar_arrive_expect_tx(&b.qf[s], q_bytes + BM * 4);
-                        load_queries<D>(a, p, &tmQ, smem + s * LY::kTile, &b.qf[s], rt, h);
-                        tc::bulk_load(lse_s + s * BM, p.nlse + ((int64_t)h * p.n_rt + rt) * BM, BM * 4, &b.qf[s]);
+                        load_queries<D>(a, p, &tmQ, smem + s * LY::kTile, &b.qf[s], rt0 + rt, h);
+                        tc::bulk_load(lse_s + s * BM, p.nlse + ((int64_t)h * p.n_rt + rt0 + rt) * BM, BM * 4, &b.qf[s]);
                         qr.next(q_slots);
                         ++qt_n;
                     }
@@ -375,6 +382,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         } else {
             for (int g = k0; g < k1 && ok; g += p.b_splits) {
                 const int r0 = rt_from(g), nk = min(p.kg, p.n_kt - g * p.kg);
+                if (r0 >= n_q) continue;
                 Ring k2 = kr;
                 k2.next(k_slots);
                 for (int rt = r0; rt < n_q && ok; ++rt) {
@@ -496,6 +504,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (key >= a.kv_len) continue;
                     const float* from = red + (turn * kBatch + j) * 4 * BM + row;
                     const float v = (from[0] + from[BM]) + (from[2 * BM] + from[3 * BM]);
+                    if (p.r_splits > 1) {
+                        p.part[((int64_t)(blockIdx.x % p.r_splits) * Hkv + h) * p.n_kt * BM + key] = v;
+                        continue;
+                    }
                     float* out = a.acc + (int64_t)h * a.acc_stride + key;
                     *out = a.accumulate ? *out + v : v;
                 }
@@ -510,7 +522,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 float s[64];
                 take_s(s_addr + buf * BM, &b.se[buf], lane, s);
                 const float4* l4 = reinterpret_cast<const float4*>(lse_s + qs * BM + half * 64);
-                const int key0 = kt * BM, tt = t_first + rt * p.T;
+                const int key0 = kt * BM, tt = t_first + (rt0 + rt) * p.T;
                 if (key0 + BM - 1 > tt) {
                     // some of these rows come before some of these keys
                     int tok = tt + half * 64 / G, rem = half * 64 % G;
@@ -614,6 +626,20 @@ __device__ __forceinline__ void join_rows(const float2* ml, float* nlse, int64_t
     if (part == 0) nlse[at] = there(at % n) ? -(ms + log2f(l)) : -INFINITY;
 }
 
+// The parts' sums of each key, in order, into acc; `stride`: keys of a row of
+// `part` [splits][Hkv][stride].
+__global__ void __launch_bounds__(kJoinThreads) k7_add(const WeightArgs a, const float* part, int stride, int splits) {
+    tc::pdl_wait();
+    tc::pdl_launch();
+    const int key = blockIdx.x * kJoinThreads + threadIdx.x, h = blockIdx.y;
+    if (key >= a.kv_len) return;
+    float v = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) v += part[((int64_t)s * a.n_head_kv + h) * stride + key];
+    float* out = a.acc + (int64_t)h * a.acc_stride + key;
+    *out = a.accumulate ? *out + v : v;
+}
+
 __global__ void __launch_bounds__(kJoinThreads) k7_join(const WeightArgs a, const WeightPlan p) {
     tc::pdl_wait();
     tc::pdl_launch();
@@ -630,7 +656,8 @@ constexpr int kF32Threads = 256;  // 16 x 16 threads, 4 rows x 4 keys each
 
 struct F32Plan {
     int32_t n_rows;  // (token, head) rows of the window per KV head
-    int32_t n_rt, n_kt, splits;
+    int32_t n_rt, n_kt, splits, r_splits;
+    float* part;     // [r_splits][Hkv][n_kt * 64] (r_splits > 1)
     float2* ml;      // [splits][Hkv][n_rt * 64]
     float* nlse;     // [Hkv][n_rt * 64]: minus the lse, -inf for rows that are none
 };
@@ -685,23 +712,22 @@ struct RowsF32 {
     }
 };
 
-// x[i][j] = q row (ty + 16 i) . k row (tx + 16 j)
-template <int D>
-__device__ __forceinline__ void scores_f32(const float* q, const float* k, int ty, int tx, float (&x)[4][4]) {
+// x[i][j] = q row (ty + 16 i) . k row (tx + 16 j), i < NI
+template <int D, int NI>
+__device__ __forceinline__ void scores_f32(const float* q, const float* k, int ty, int tx, float (&x)[NI][4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[i][j] = 0.f;
 #pragma unroll 4
     for (int c = 0; c < D; c += 4) {
-        float4 qq[4], kk[4];
+        float4 qq[NI], kk[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            qq[i] = *reinterpret_cast<const float4*>(q + (ty + 16 * i) * (D + 4) + c);
-            kk[i] = *reinterpret_cast<const float4*>(k + (tx + 16 * i) * (D + 4) + c);
-        }
+        for (int i = 0; i < NI; ++i) qq[i] = *reinterpret_cast<const float4*>(q + (ty + 16 * i) * (D + 4) + c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) kk[i] = *reinterpret_cast<const float4*>(k + (tx + 16 * i) * (D + 4) + c);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 x[i][j] = fmaf(qq[i].x, kk[j].x, x[i][j]);
@@ -734,6 +760,7 @@ __global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, 
         m[i] = -INFINITY;
         l[i] = 0.f;
     }
+    const bool few = p.n_rows - rt * FT <= 16;  // a small window: the rows past it cost nothing
     RowsF32<D> next;
     {
         RowsF32<D> rows;
@@ -746,22 +773,27 @@ __global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, 
         next.store(k);
         __syncthreads();
         if (kt + 1 < k1) next.fetch_keys(a, kt + 1, h);
-        float x[4][4];
-        scores_f32<D>(q, k, ty, tx, x);
+        auto tile = [&](auto ni) {
+            constexpr int NI = decltype(ni)::value;
+            float x[NI][4];
+            scores_f32<D, NI>(q, k, ty, tx, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float mx = m[i];
+            for (int i = 0; i < NI; ++i) {
+                float mx = m[i];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[i][j] = kt * FT + tx + 16 * j <= tok[i] ? x[i][j] * sl2 : -INFINITY;
-                mx = fmaxf(mx, x[i][j]);
+                for (int j = 0; j < 4; ++j) {
+                    x[i][j] = kt * FT + tx + 16 * j <= tok[i] ? x[i][j] * sl2 : -INFINITY;
+                    mx = fmaxf(mx, x[i][j]);
+                }
+                const float ms = mx == -INFINITY ? 0.f : mx;
+                l[i] *= ex2(m[i] - ms);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) l[i] += ex2(x[i][j] - ms);
+                m[i] = mx;
             }
-            const float ms = mx == -INFINITY ? 0.f : mx;
-            l[i] *= ex2(m[i] - ms);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) l[i] += ex2(x[i][j] - ms);
-            m[i] = mx;
-        }
+        };
+        if (few) tile(std::integral_constant<int, 1>{});
+        else tile(std::integral_constant<int, 4>{});
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -788,7 +820,9 @@ template <int D>
 __global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, const F32Plan p) {
     extern __shared__ __align__(16) float sm[];
     float *q = sm, *k = sm + FT * (D + 4);
-    const int kt = blockIdx.x % p.n_kt, h = blockIdx.x / p.n_kt;
+    const int rs = blockIdx.x % p.r_splits, rest = blockIdx.x / p.r_splits;
+    const int kt = rest % p.n_kt, h = rest / p.n_kt;
+    const int r1 = (int)((int64_t)p.n_rt * (rs + 1) / p.r_splits);  // this part's last row tile + 1
     const int G = a.n_head / a.n_head_kv, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     const int t_first = a.kv_len - a.n_tok + a.row_begin;
     const float sl2 = a.kq_scale * 1.4426950408889634f;
@@ -796,29 +830,35 @@ __global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, c
     tc::pdl_launch();
     const float* nlse = p.nlse + (int64_t)h * p.n_rt * FT;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    const int r0 = max(0, (int)((int64_t)(kt * FT - t_first) * G / FT));  // first tile with a row that sees the keys
+    // first of the part's row tiles with a row that sees the keys
+    const int r0 = max((int)((int64_t)p.n_rt * rs / p.r_splits), (int)((int64_t)(kt * FT - t_first) * G / FT));
     RowsF32<D> next;
     {
         RowsF32<D> rows;
         rows.fetch_keys(a, kt, h);
-        if (r0 < p.n_rt) next.fetch_queries(a, p.n_rows, r0, h);
+        if (r0 < r1) next.fetch_queries(a, p.n_rows, r0, h);
         rows.store(k);
     }
-    for (int rt = r0; rt < p.n_rt; ++rt) {
+    for (int rt = r0; rt < r1; ++rt) {
         __syncthreads();
         next.store(q);
         __syncthreads();
-        if (rt + 1 < p.n_rt) next.fetch_queries(a, p.n_rows, rt + 1, h);
-        float x[4][4];
-        scores_f32<D>(q, k, ty, tx, x);
+        if (rt + 1 < r1) next.fetch_queries(a, p.n_rows, rt + 1, h);
+        auto tile = [&](auto ni) {
+            constexpr int NI = decltype(ni)::value;
+            float x[NI][4];
+            scores_f32<D, NI>(q, k, ty, tx, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = rt * FT + ty + 16 * i, tok = t_first + r / G;
-            const float ls = nlse[r];
+            for (int i = 0; i < NI; ++i) {
+                const int r = rt * FT + ty + 16 * i, tok = t_first + r / G;
+                const float ls = nlse[r];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (kt * FT + tx + 16 * j <= tok) sum[j] += ex2(fmaf(x[i][j], sl2, ls));
-        }
+                for (int j = 0; j < 4; ++j)
+                    if (kt * FT + tx + 16 * j <= tok) sum[j] += ex2(fmaf(x[i][j], sl2, ls));
+            }
+        };
+        if (p.n_rows - rt * FT <= 16) tile(std::integral_constant<int, 1>{});
+        else tile(std::integral_constant<int, 4>{});
     }
     __syncthreads();
 #pragma unroll
@@ -827,6 +867,10 @@ __global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, c
     if (threadIdx.x < FT && kt * FT + (int)threadIdx.x < a.kv_len) {
         float v = 0.f;
         for (int i = 0; i < 16; ++i) v += q[i * FT + threadIdx.x];
+        if (p.r_splits > 1) {
+            p.part[(((int64_t)rs * a.n_head_kv + h) * p.n_kt + kt) * FT + threadIdx.x] = v;
+            return;
+        }
         float* out = a.acc + (int64_t)h * a.acc_stride + kt * FT + threadIdx.x;
         *out = a.accumulate ? *out + v : v;
     }
@@ -849,7 +893,11 @@ size_t plan_f32(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv,
     const size_t n = (size_t)n_head_kv * p->n_rt * FT, ml = up16(n * p->splits * sizeof(float2));
     p->ml = reinterpret_cast<float2*>(ws);
     p->nlse = reinterpret_cast<float*>(ws + ml);
-    return ml + up16(n * sizeof(float));
+    // few key tiles and many rows: split the rows of the sums pass too
+    p->r_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_rt / 2, 2 * kSms / ((int64_t)n_head_kv * p->n_kt)));
+    const size_t lse = up16(n * sizeof(float));
+    p->part = reinterpret_cast<float*>(ws + ml + lse);
+    return ml + lse + (p->r_splits > 1 ? up16((size_t)p->r_splits * n_head_kv * p->n_kt * FT * sizeof(float)) : 0);
 }
 
 size_t plan_tc(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, int32_t d, char* ws, WeightPlan* p) {
@@ -862,26 +910,35 @@ size_t plan_tc(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, 
     p->group = (p->n_rt + p->n_groups - 1) / p->n_groups;
     p->n_groups = (p->n_rt + p->group - 1) / p->group;
     p->splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_kt, kSms / ((int64_t)n_head_kv * p->n_groups)));
-    // sums pass: query tiles that leave two slots for keys stay on chip, more
-    // of them stream; then two key tiles share each query tile's load once
-    // there are enough key tiles to fill the device that way
-    p->resident = p->n_rt <= slots - 2;
-    p->q_slots = p->resident ? p->n_rt : slots / 2;
+    // sums pass: a CTA per key tile, the rows split too when there are few key
+    // tiles and many rows
+    p->r_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_rt / 4, kSms / ((int64_t)n_head_kv * p->n_kt)));
+    // query tiles that leave two slots for keys stay on chip, more of them
+    // stream; then two key tiles share each query tile's load once there are
+    // enough key tiles to fill the device that way
+    const int tiles = (p->n_rt + p->r_splits - 1) / p->r_splits;
+    p->resident = tiles <= slots - 2;
+    p->q_slots = p->resident ? tiles : slots / 2;
     p->k_slots = slots - p->q_slots;
     p->kg = !p->resident && (int64_t)n_head_kv * p->n_kt >= 2 * kSms ? 2 : 1;
     const int n_kg = (p->n_kt + p->kg - 1) / p->kg;
     p->b_splits = std::max(1, std::min(n_kg, kSms / n_head_kv));
     const size_t n = (size_t)n_head_kv * p->n_rt * BM, ml = up16(n * p->splits * sizeof(float2));
+    const size_t lse = up16(n * sizeof(float));
     p->ml = reinterpret_cast<float2*>(ws);
     p->nlse = reinterpret_cast<float*>(ws + ml);
-    return ml + up16(n * sizeof(float));
+    p->part = reinterpret_cast<float*>(ws + ml + lse);
+    return ml + lse + (p->r_splits > 1 ? up16((size_t)p->r_splits * n_head_kv * p->n_kt * BM * sizeof(float)) : 0);
 }
 
+// A launch that may start before what precedes it on the stream has ended (the
+// kernels wait for it on the device).
 template <class... P, class... A>
-cudaError_t launch_after(void (*k)(P...), int64_t grid, int threads, int smem, cudaStream_t s, const A&... args) {
+cudaError_t launch_after(void (*k)(P...), int64_t grid, int heads, int threads, int smem, cudaStream_t s,
+                         const A&... args) {
     if (grid < 1 || grid > INT_MAX) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)grid);
+    cfg.gridDim = dim3((unsigned)grid, heads);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -913,12 +970,13 @@ cudaError_t launch_f32(const WeightArgs& a, cudaStream_t s) {
     cudaError_t e = allow_smem(reinterpret_cast<const void*>(&k7_stats_f32<D>), smem, m0);
     if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_sums_f32<D>), smem, m1);
     if (e != cudaSuccess) return e;
-    const int64_t ctas = (int64_t)a.n_head_kv * p.n_rt * p.splits, rows = (int64_t)a.n_head_kv * p.n_rt * FT;
-    e = launch_after(k7_stats_f32<D>, ctas, kF32Threads, smem, s, a, p);
-    if (e == cudaSuccess)
-        e = launch_after(k7_join_f32, (rows + kJoinThreads / 16 - 1) / (kJoinThreads / 16), kJoinThreads, 0, s, a, p);
-    if (e != cudaSuccess) return e;
-    return launch_after(k7_sums_f32<D>, (int64_t)a.n_head_kv * p.n_kt, kF32Threads, smem, s, a, p);
+    const int64_t K = a.n_head_kv, rows = K * p.n_rt * FT;
+    e = launch_after(k7_stats_f32<D>, K * p.n_rt * p.splits, 1, kF32Threads, smem, s, a, p);
+    if (e == cudaSuccess) e = launch_after(k7_join_f32, rows / (kJoinThreads / 16), 1, kJoinThreads, 0, s, a, p);
+    if (e == cudaSuccess) e = launch_after(k7_sums_f32<D>, K * p.n_kt * p.r_splits, 1, kF32Threads, smem, s, a, p);
+    if (e != cudaSuccess || p.r_splits == 1) return e;
+    return launch_after(k7_add, (a.kv_len + kJoinThreads - 1) / kJoinThreads, a.n_head_kv, kJoinThreads, 0, s, a,
+                        (const float*)p.part, p.n_kt * FT, p.r_splits);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
@@ -962,12 +1020,14 @@ cudaError_t launch_tc(const WeightArgs& a, cudaStream_t s) {
     cudaError_t e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 0>), smem, m0);
     if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 1>), smem, m1);
     if (e != cudaSuccess) return e;
-    const int64_t ctas = (int64_t)a.n_head_kv * p.n_groups * p.splits, n = (int64_t)p.n_rt * BM;
-    e = launch_after(k7_pass<BF16, D, SEG, 0>, ctas, kTcThreads, smem, s, mq, mk, a, p);
+    const int64_t K = a.n_head_kv;
+    e = launch_after(k7_pass<BF16, D, SEG, 0>, K * p.n_groups * p.splits, 1, kTcThreads, smem, s, mq, mk, a, p);
+    if (e == cudaSuccess) e = launch_after(k7_join, K * p.n_rt * BM / (kJoinThreads / 16), 1, kJoinThreads, 0, s, a, p);
     if (e == cudaSuccess)
-        e = launch_after(k7_join, n * a.n_head_kv / (kJoinThreads / 16), kJoinThreads, 0, s, a, p);
-    if (e != cudaSuccess) return e;
-    return launch_after(k7_pass<BF16, D, SEG, 1>, (int64_t)a.n_head_kv * p.b_splits, kTcThreads, smem, s, mq, mk, a, p);
+        e = launch_after(k7_pass<BF16, D, SEG, 1>, K * p.b_splits * p.r_splits, 1, kTcThreads, smem, s, mq, mk, a, p);
+    if (e != cudaSuccess || p.r_splits == 1) return e;
+    return launch_after(k7_add, (a.kv_len + kJoinThreads - 1) / kJoinThreads, a.n_head_kv, kJoinThreads, 0, s, a,
+                        (const float*)p.part, p.n_kt * BM, p.r_splits);
 }
 
 template <bool BF16, int D>

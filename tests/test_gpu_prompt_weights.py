@@ -61,6 +61,16 @@ def test_whole_prompt(dtype):
     run_case(1111, 1111, 0, (8, 2, 64), dtype, 32, 32, seed=1)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("kv_len,n_tok,row_begin,heads", [
+    (257, 174, 100, (16, 1, 128)), (300, 290, 0, (48, 1, 64)), (130, 129, 0, (100, 1, 64)), (700, 700, 0, (64, 2, 128)),
+    (1000, 600, 0, (7, 1, 64))], ids=str)
+def test_many_rows_over_few_keys(kv_len, n_tok, row_begin, heads, dtype):
+    """The rows of the sums are split over the device, and their parts put together."""
+    run_case(kv_len, n_tok, row_begin, heads, dtype, 32, 32, seed=kv_len)
+    run_case(kv_len, n_tok, row_begin, heads, dtype, 32, 0, accumulate=True, pad=3, seed=kv_len + 1)
+
+
 def test_long_cache():
     run_case(30000, 64, 0, (32, 8, 128), BF16, 128, 128, accumulate=True, seed=2)
     run_case(20011, 700, 500, (28, 4, 128), F16, 64, 64, seed=3)
