@@ -475,8 +475,11 @@ typedef struct ep_sp_kv_batch {
  * softmax statistics and sums are f32; an f32 context multiplies in f32
  * whatever ep_sp_set_f32_attention says.  A sequence's result does not depend
  * on timing, only on the batch (the cache is split over the SMs by the lengths
- * of the whole batch).  rc 2 on bad arguments, 12 on a CUDA launch error; a
- * bounded wait that expired is rc 6 from ep_sp_sync_status.
+ * of the whole batch).  A call with k_new makes the context forget the layer's
+ * page sums and f16 shadows (only the device knows which rows were written),
+ * so a later gated prefill call pools the cache again; after replaying a
+ * captured one ep_sp_reset does that.  rc 2 on bad arguments, 12 on a CUDA
+ * launch error; a bounded wait that expired is rc 6 from ep_sp_sync_status.
  * ep_sp_decode_bytes gives the workspace size of a call with n_seq sequences
  * of up to max_kv_len rows, with_acc 1 when acc is given. */
 int32_t ep_sp_decode_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_len, int32_t with_acc, size_t* bytes);

@@ -92,6 +92,10 @@ def test_many_sequences_of_one_long_and_the_rest_short():
     run_case([6000] + [1 + i % 40 for i in range(300)], (8, 2, 64), F16, F16, 32, 32, False, True)
 
 
+def test_more_sequences_than_a_cta_keeps_the_lengths_of():
+    run_case([(7 * i) % 45 for i in range(2500)], (4, 2, 64), F16, F16, 32, 32, True, True)
+
+
 def test_long_cache_spread_over_the_device():
     run_case([40000, 25000], (28, 4, 128), BF16, BF16, 128, 256, True, True, seed=3)
 

@@ -117,3 +117,51 @@ def test_prefill_evict_decode_evict_prefill(dtype, heads, page):
     for a, b in zip(*outs):
         assert torch.equal(a, b)
     assert math.isfinite(float(outs[0][0].sum()))
+
+
+@pytest.mark.parametrize("dtype", [epsp.BF16, epsp.F32], ids=["bf16", "f32"])
+def test_prefill_after_decoding_over_a_cut_back_sequence(dtype):
+    """A sequence is cut back, continued by decode steps over rows whose pages were summed, then prefilled further:
+    the selection sees the new rows."""
+    H, K, d, P = 8, 2, 64, 32
+    n, back, t = 600, 300, 130
+    w = W.Workload("back", 1000, 1, H, K, d, dtype, 1000, P, 2, 2 * P)
+    q, k, v = (x.cuda() for x in W.gen_layer(w, 0))
+    outs = []
+    for fresh in (False, True):
+        ctx = context(H, K, d, dtype, epsp.F32, 1000, P)
+        ctx.check(ctx.set_ext(1, 0, 0))
+        ctx.check(ctx.set_qg_bound(1, 2, 2, 0))
+        ctx.set_prefill_mode(True)
+        kc, vc = torch.zeros_like(k), torch.zeros_like(v)
+        o = torch.zeros(n, H, d, device="cuda")
+        if fresh:
+            kc[:n], vc[:n] = k[:n], v[:n]
+        else:
+            ctx.check(ctx.append_kv(0, k[:n].contiguous(), v[:n].contiguous(), n, kc, vc, 0))
+            ctx.check(ctx.attend_layer(0, q[:n].contiguous(), kc, vc, n, n, o))
+        rows = range(back, back + 70)
+        if fresh:
+            for i, r in enumerate(rows):
+                kc[r], vc[r] = 3 * k[n + i], v[n + i]
+        else:
+            ws = workspace(ctx.decode_bytes(1, 1000, False))
+            lens = torch.tensor([back], dtype=torch.int32, device="cuda")
+            kv = epsp.KvBatch(lens, 1000, seq_rows=1000)
+            out = torch.zeros(1, H, d, device="cuda")
+            for i, r in enumerate(rows):
+                lens.add_(1)
+                ctx.check(ctx.decode_layer(0, kv, q[r][None].contiguous(), kc, vc, out, ws,
+                                           k_new=(3 * k[n + i])[None].contiguous(), v_new=v[n + i][None].contiguous()))
+        u0 = back + 70
+        kc[u0:u0 + t], vc[u0:u0 + t] = k[800:800 + t], v[800:800 + t]
+        o = torch.zeros(t, H, d, device="cuda")
+        sel = torch.full((1, K, 64), -1, dtype=torch.int32, device="cuda")
+        cnt = torch.zeros((1, K), dtype=torch.int32, device="cuda")
+        ctx.check(ctx.attend_layer(0, q[800:800 + t].contiguous(), kc, vc, u0 + t, t, o, sel, cnt, 64))
+        torch.cuda.synchronize()
+        ctx.check(ctx.sync_status())
+        outs.append((o, sel, cnt))
+    assert int(outs[0][2].sum()) > 0
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
