@@ -7,14 +7,14 @@
 // Storing the scores instead would cost 8 bytes a pair; recomputing them costs
 // 2 d flops, which the tensor cores do in a quarter of the time the pair's two
 // exponentials take.  The exponentials bound both passes (16 MUFU results per
-// clock and SM, a third of the pairs on the FMA pipe instead).  Every key has one writer and a fixed order of additions.
+// clock and SM, a fifth of the pairs on the FMA pipe instead).  Every key has one writer and a fixed order of additions.
 //
 // 16-bit (tcgen05): a query tile packs T = 128 / G tokens x G heads into 128
 // rows.  The two passes are one kernel with the MMA operands exchanged: with
 // queries as the M side a thread (TMEM lane) owns a query row and reduces over
 // keys; with keys as the M side it owns a key and reduces over queries.  Both
 // reductions stay in the thread's registers, no shuffles.  One warp loads
-// tiles by TMA, one issues MMAs into 4 S buffers in TMEM, and 16 warps take
+// tiles by TMA, one issues MMAs into 3 S buffers in TMEM, and 24 warps take
 // the exponentials.
 // f32: the same passes on the CUDA cores, 64 x 64 tiles, 4 x 4 per thread.
 #include <cuda.h>
@@ -67,7 +67,7 @@ __device__ __forceinline__ float2 exp2_poly_add(float2 x, float2 acc) {
 // acc + 2^x of pair i of a run of pairs: one pair in kPolyEvery on the FMA
 // pipe, the rest on MUFU.
 #ifndef K7_POLY_EVERY
-#define K7_POLY_EVERY 3
+#define K7_POLY_EVERY 5
 #endif
 constexpr int kPolyEvery = K7_POLY_EVERY;
 __device__ __forceinline__ float2 exp2_add(float2 x, int i, float2 acc) {
@@ -77,10 +77,15 @@ __device__ __forceinline__ float2 exp2_add(float2 x, int i, float2 acc) {
 
 // ---------------------------------------------------------- 16-bit: tcgen05 --
 constexpr int BM = 128;                 // rows of a query tile, keys of a key tile
-constexpr int kTcThreads = 640;         // producer, MMA, 2 idle warps, 4 x 4 softmax warps
+constexpr int kPairs = 3;               // pairs of softmax warpgroups
+constexpr int kWgs = 2 * kPairs;
+constexpr int kTcThreads = 128 + kWgs * 128;  // producer, MMA, 2 idle warps, the softmax warps
 constexpr int kHalfTile = BM * 128;     // [128][64 x 16-bit], 128-byte swizzled
 constexpr int kMaxGroup = 4;            // query tiles a statistics CTA keeps on chip
-constexpr int kSBufs = 4;               // S tiles in TMEM (128 columns each)
+// S tiles in TMEM (128 columns each), one per pair: a buffer's fills are all
+// awaited by the same warps, in order, as the barrier's one phase bit demands.
+constexpr int kSBufs = kPairs;
+constexpr int kTmemCols = 512;          // a power of two
 constexpr int kSms = 148;
 constexpr int kBatch = 4;               // key tiles whose sums are put together at a time
 
@@ -88,12 +93,12 @@ template <int D>
 struct TcLayout {
     static constexpr int kTile = D / 64 * kHalfTile;
     static constexpr int kSlots = D == 128 ? 6 : 12;  // query + key tiles on chip
-    // statistics pass: float2 [4][kMaxGroup * BM]; sums pass: float
-    // [kSlots][BM] lse of the query tiles on chip, then [2][kBatch][4][BM] sums
+    // statistics pass: float2 [kWgs][kMaxGroup * BM]; sums pass: float
+    // [kSlots][BM] lse of the query tiles on chip, then [2][kBatch][kWgs][BM] sums
     static constexpr int kOffStat = kSlots * kTile;
     static constexpr int kOffRed = kOffStat + kSlots * BM * 4;
-    static constexpr int kOffBar = kOffRed + 2 * kBatch * 4 * BM * 4;
-    static_assert(kOffStat + 4 * kMaxGroup * BM * 8 <= kOffBar, "statistics pass");
+    static constexpr int kOffBar = kOffRed + 2 * kBatch * kWgs * BM * 4;
+    static_assert(kOffStat + kWgs * kMaxGroup * BM * 8 <= kOffBar, "statistics pass");
     static constexpr int kBars = 2 * 12 + 2 * 12 + 2 * kSBufs + 1;
     static constexpr int kBytes = kOffBar + kBars * 8 + 32;
     static_assert(kBytes + 1024 <= 232448, "shared memory");
@@ -185,14 +190,16 @@ __device__ __forceinline__ void issue_s(uint32_t tmem, int buf, uint64_t da, uin
     }
 }
 
-// 64 columns of S of this thread's lane; the buffer is handed back at once.
-__device__ __forceinline__ void take_s(uint32_t addr, uint64_t* se, int lane, float (&s)[64]) {
-    uint32_t u[2][32];
-    tc::tmem_ld32(addr, u[0]);
-    tc::tmem_ld32(addr + 32, u[1]);
+// 32 columns of S of this thread's lane.
+__device__ __forceinline__ void take_s(uint32_t addr, float (&s)[32]) {
+    uint32_t u[32];
+    tc::tmem_ld32(addr, u);
     tc::tmem_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(u[i >> 5][i & 31]);
+    for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(u[i]);
+}
+// (once the last column has left it)
+__device__ __forceinline__ void give_back(uint64_t* se, int lane) {
     tc::fence_before_sync();
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(se);
@@ -205,9 +212,13 @@ __device__ __forceinline__ void take_s(uint32_t addr, uint64_t* se, int lane, fl
 // query rows, so each thread sums one key's weights in registers; key tiles
 // (kg at a time) against all query tiles, which stay when they fit and
 // stream otherwise.
-// A step is one (query tile, key tile), its S in buffer step % 4; two
-// warpgroups take the even steps, two the odd ones, each 64 of the 128 columns.
-template <bool BF16, int D, int SEG, int PASS>
+// A step is one (query tile, key tile); three pairs of warpgroups, an S buffer
+// each, take the steps in turn, each warpgroup 64 of the 128 columns, 32 at a
+// time (the buffer goes back to the MMA warp halfway).  Issue slots and MUFU together bound it: 24 warps hide more of
+// each other than 16 with 64 columns in registers (96 against 101 us for 64
+// rows of 32 heads over 64K keys), a warpgroup per step measured 99 us.
+// STREAM: the sums pass whose query tiles stream.
+template <bool BF16, int D, int SEG, int PASS, bool STREAM>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k7_pass(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
             const __grid_constant__ WeightArgs a, const __grid_constant__ WeightPlan p) {
@@ -223,7 +234,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     // the CTA's part
     int h, rt0 = 0, n_q, k0, k1, q_slots, k_slots;
-    bool stream_q = false;
+    constexpr bool stream_q = STREAM;
+    static_assert(PASS == 1 || !STREAM, "the statistics pass keeps its query tiles");
     if constexpr (PASS == 0) {
         const int sp = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
         h = rest / p.n_groups;
@@ -245,7 +257,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         k1 = (p.n_kt + p.kg - 1) / p.kg;
         q_slots = p.q_slots;
         k_slots = p.k_slots;
-        stream_q = !p.resident;
     }
     unsigned char* kbase = smem + q_slots * LY::kTile;
     float* lse_s = reinterpret_cast<float*>(smem + LY::kOffStat);
@@ -253,7 +264,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < q_slots; ++i) {
             tc::mbar_init(&b.qf[i], 1);
-            tc::mbar_init(&b.qe[i], 17);  // the MMAs' commit and the 16 softmax warps
+            tc::mbar_init(&b.qe[i], 1 + 4 * kWgs);  // the MMAs' commit and the softmax warps
         }
         for (int i = 0; i < k_slots; ++i) {
             tc::mbar_init(&b.kf[i], 1);
@@ -269,7 +280,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc::tma_prefetch_desc(&tmK);
     }
     if (warp == 1) {
-        tc::tmem_alloc(tmem_slot, kSBufs * BM);
+        tc::tmem_alloc(tmem_slot, kTmemCols);
         tc::tmem_relinquish();
     }
     // Query rows past T * G are never written by TMA: zeros, so that no stale
@@ -322,16 +333,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const int r0 = rt_from(g);
                     if (r0 >= n_q) continue;
                     for (int k = 0; k < p.kg && g * p.kg + k < p.n_kt && ok; ++k) keys(g * p.kg + k);
-                    if (!stream_q) continue;
-                    for (int rt = r0; rt < n_q && ok; ++rt) {
-                        const int s = qr.slot;
-                        ok = tc::mbar_wait(&b.qe[s], qr.phase ^ 1, tmo);
-                        if (!ok) break;
-                        tc::mbar_arrive_expect_tx(&b.qf[s], q_bytes + BM * 4);
-                        load_queries<D>(a, p, &tmQ, smem + s * LY::kTile, &b.qf[s], rt0 + rt, h);
-                        tc::bulk_load(lse_s + s * BM, p.nlse + ((int64_t)h * p.n_rt + rt0 + rt) * BM, BM * 4, &b.qf[s]);
-                        qr.next(q_slots);
-                        ++qt_n;
+                    if constexpr (STREAM) {
+                        for (int rt = r0; rt < n_q && ok; ++rt) {
+                            const int s = qr.slot;
+                            ok = tc::mbar_wait(&b.qe[s], qr.phase ^ 1, tmo);
+                            if (!ok) break;
+                            tc::mbar_arrive_expect_tx(&b.qf[s], q_bytes + BM * 4);
+                            load_queries<D>(a, p, &tmQ, smem + s * LY::kTile, &b.qf[s], rt0 + rt, h);
+                            tc::bulk_load(lse_s + s * BM, p.nlse + ((int64_t)h * p.n_rt + rt0 + rt) * BM, BM * 4, &b.qf[s]);
+                            qr.next(q_slots);
+                            ++qt_n;
+                        }
                     }
                 }
             }
@@ -415,7 +427,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
     } else if (warp >= 4) {
         // ------------------------------------------------------- softmax --
-        const int wg = (warp - 4) >> 2, odd = wg >> 1, half = wg & 1, wq = warp & 3, row = wq * 32 + lane;
+        const int wg = (warp - 4) >> 2, pair = wg >> 1, half = wg & 1, wq = warp & 3, row = wq * 32 + lane;
         const uint32_t s_addr = tmem + ((uint32_t)(wq * 32) << 16) + half * 64;
         const float sl2 = a.kq_scale * 1.4426950408889634f;
         const float2 sl2_2 = make_float2(sl2, sl2);
@@ -432,78 +444,84 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             float2* stat = stats + wg * kMaxGroup * BM + row;
             for (int r = 0; r < n_q; ++r) stat[r * BM] = make_float2(-INFINITY, 0.f);
             const int steps = (k1 - k0) * n_q;
-            int kt = k0, r = odd, r_held = -1;
-            if (r >= n_q) r -= n_q, ++kt;
+            int kt = k0, r = pair, r_held = -1;
+            while (r >= n_q) r -= n_q, ++kt;
             float2 st = make_float2(-INFINITY, 0.f);  // of query tile r_held
-            for (int step = odd; step < steps; step += 2) {
-                const int buf = step % kSBufs;
+            for (int step = pair; step < steps; step += kPairs) {
+                const int buf = pair;  // = step % kSBufs
                 if (!wait(&b.sf[buf], (step / kSBufs) & 1, step)) break;
                 tc::fence_after_sync();
-                float s[64];
-                take_s(s_addr + buf * BM, &b.se[buf], lane, s);
                 if (r != r_held) {
                     if (r_held >= 0) stat[r_held * BM] = st;
                     st = stat[r * BM];
                     r_held = r;
                 }
                 const int tt = t_first + (rt0 + r) * p.T, key = kt * BM + half * 64;
-                if (key + 63 > tt) {
-                    const int lim = tt + row / G - key;
+                const bool cut = key + 63 > tt;
+                const int lim = tt + row / G - key;
 #pragma unroll
-                    for (int c = 0; c < 64; ++c)
-                        if (c > lim) s[c] = -INFINITY;
+                for (int hc = 0; hc < 2; ++hc) {
+                    float s[32];
+                    take_s(s_addr + buf * BM + hc * 32, s);
+                    if (hc == 1) give_back(&b.se[buf], lane);
+                    if (cut) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (hc * 32 + c > lim) s[c] = -INFINITY;
+                    }
+                    float mx[2] = {s[0], s[1]};
+#pragma unroll
+                    for (int c = 2; c < 30; c += 4)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) mx[i] = max3f(mx[i], s[c + i], s[c + 2 + i]);
+                    mx[0] = max3f(mx[0], s[30], s[31]);
+                    const float m = fmaxf(st.x, fmaxf(mx[0], mx[1]) * sl2);
+                    const float ms = m == -INFINITY ? 0.f : m;
+                    const float2 nm = make_float2(-ms, -ms);
+                    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        acc[c & 1] = exp2_add(__ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2_2, nm), hc * 16 + c, acc[c & 1]);
+                    const float2 t = __fadd2_rn(acc[0], acc[1]);
+                    st = make_float2(m, st.y * ex2(st.x - ms) + (t.x + t.y));
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int c = 4; c < 60; c += 8)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], s[c + i], s[c + 4 + i]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], s[60 + i]);
-                const float m = fmaxf(st.x, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
-                const float ms = m == -INFINITY ? 0.f : m;
-                const float2 nm = make_float2(-ms, -ms);
-                float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                for (int c = 0; c < 32; ++c)
-                    acc[c & 1] = exp2_add(__ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2_2, nm), c, acc[c & 1]);
-                const float2 t = __fadd2_rn(acc[0], acc[1]);
-                st = make_float2(m, st.y * ex2(st.x - ms) + (t.x + t.y));
-                r += 2;
+                r += kPairs;
                 while (r >= n_q) r -= n_q, ++kt;
             }
             if (r_held >= 0) stat[r_held * BM] = st;
-            // the four warpgroups' statistics of each row
-            tc::named_bar_sync(1, 512);
+            // the warpgroups' statistics of each row
+            tc::named_bar_sync(1, kWgs * 128);
             const int sp = blockIdx.x % p.splits;
             float2* out = p.ml + ((int64_t)sp * Hkv + h) * p.n_rt * BM + rt0 * BM;
-            for (int i = wg * BM + row; i < n_q * BM; i += 4 * BM) {
-                float2 v[4];
+            for (int i = wg * BM + row; i < n_q * BM; i += kWgs * BM) {
+                float2 v[kWgs];
                 float m = -INFINITY, l = 0.f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
+                for (int w = 0; w < kWgs; ++w) {
                     v[w] = stats[w * kMaxGroup * BM + i];
                     m = fmaxf(m, v[w].x);
                 }
                 const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) l += v[w].y * ex2(v[w].x - ms);
+                for (int w = 0; w < kWgs; ++w) l += v[w].y * ex2(v[w].x - ms);
                 out[i] = make_float2(m, l);
             }
         } else {
             // sums of up to kBatch key tiles wait in shared memory for the
             // other warpgroups': one barrier per batch
-            float* red = reinterpret_cast<float*>(smem + LY::kOffRed);  // [2 turns][kBatch][4 warpgroups][BM]
+            float* red = reinterpret_cast<float*>(smem + LY::kOffRed);  // [2 turns][kBatch][kWgs][BM]
             int turn = 0, held = 0;
-            auto put = [&](float v) { red[((turn * kBatch + held++) * 4 + wg) * BM + row] = v; };
+            auto put = [&](float v) { red[((turn * kBatch + held++) * kWgs + wg) * BM + row] = v; };
             auto flush = [&](int g_first) {
-                tc::named_bar_sync(1, 512);
-                for (int i = wg * BM + row; i < held * BM && ok; i += 4 * BM) {
+                tc::named_bar_sync(1, kWgs * 128);
+                for (int i = wg * BM + row; i < held * BM && ok; i += kWgs * BM) {
                     const int j = i / BM, gj = p.kg == 1 ? j : j >> 1;
                     const int kt = (g_first + gj * p.b_splits) * p.kg + (p.kg == 1 ? 0 : j & 1), key = kt * BM + row;
                     if (key >= a.kv_len) continue;
-                    const float* from = red + (turn * kBatch + j) * 4 * BM + row;
-                    const float v = (from[0] + from[BM]) + (from[2 * BM] + from[3 * BM]);
+                    const float* from = red + (turn * kBatch + j) * kWgs * BM + row;
+                    float v = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWgs; ++w) v += from[w * BM];
                     if (p.r_splits > 1) {
                         p.part[((int64_t)(blockIdx.x % p.r_splits) * Hkv + h) * p.n_kt * BM + key] = v;
                         continue;
@@ -514,43 +532,46 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 turn ^= 1;
                 held = 0;
             };
-            // one step: the weights that the 64 rows of query tile rt (slot qs) in `half` give key tile kt, summed
+            // one step: the weights that the 64 rows of query tile rt (slot qs) in `half` give this thread's key of tile kt, summed
             auto take_step = [&](int step, int kt, int rt, int qs) -> float {
-                const int buf = step % kSBufs;
+                const int buf = pair;  // = step % kSBufs
                 if (!wait(&b.sf[buf], (step / kSBufs) & 1, step)) return 0.f;
                 tc::fence_after_sync();
-                float s[64];
-                take_s(s_addr + buf * BM, &b.se[buf], lane, s);
                 const float4* l4 = reinterpret_cast<const float4*>(lse_s + qs * BM + half * 64);
                 const int key0 = kt * BM, tt = t_first + (rt0 + rt) * p.T;
-                if (key0 + BM - 1 > tt) {
-                    // some of these rows come before some of these keys
-                    int tok = tt + half * 64 / G, rem = half * 64 % G;
-#pragma unroll
-                    for (int c = 0; c < 64; ++c) {
-                        if (key0 + row > tok) s[c] = -INFINITY;
-                        if (++rem == G) rem = 0, ++tok;
-                    }
-                }
                 float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    const float4 l = l4[c];
-                    acc[0] = exp2_add(__ffma2_rn(make_float2(s[4 * c], s[4 * c + 1]), sl2_2, make_float2(l.x, l.y)), 2 * c,
-                                      acc[0]);
-                    acc[1] = exp2_add(__ffma2_rn(make_float2(s[4 * c + 2], s[4 * c + 3]), sl2_2, make_float2(l.z, l.w)),
-                                      2 * c + 1, acc[1]);
+                for (int hc = 0; hc < 2; ++hc) {
+                    float s[32];
+                    take_s(s_addr + buf * BM + hc * 32, s);
+                    if (hc == 1) give_back(&b.se[buf], lane);
+                    if (key0 + BM - 1 > tt) {
+                        int tok = tt + (half * 64 + hc * 32) / G, rem = (half * 64 + hc * 32) % G;
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            if (key0 + row > tok) s[c] = -INFINITY;
+                            if (++rem == G) rem = 0, ++tok;
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float4 l = l4[hc * 8 + c];
+                        acc[0] = exp2_add(__ffma2_rn(make_float2(s[4 * c], s[4 * c + 1]), sl2_2, make_float2(l.x, l.y)), hc * 16 + 2 * c,
+                                          acc[0]);
+                        acc[1] = exp2_add(__ffma2_rn(make_float2(s[4 * c + 2], s[4 * c + 3]), sl2_2, make_float2(l.z, l.w)),
+                                          hc * 16 + 2 * c + 1, acc[1]);
+                    }
                 }
                 const float2 t = __fadd2_rn(acc[0], acc[1]);
                 return t.x + t.y;
             };
-            if (!stream_q) {
-                // steps (key tile, query tile) in turn; this pair of warpgroups has every other one
+            if constexpr (!STREAM) {
+                // steps (key tile, query tile) in turn; this pair of warpgroups has every third one
                 wait(&b.qf[0], 0, 0);
                 const int n_mine = k0 < k1 ? (k1 - 1 - k0) / p.b_splits + 1 : 0;
-                int i = 0, rt = odd, kt = k0, g_first = k0;
+                int i = 0, rt = pair, kt = k0, g_first = k0;
                 float sum = 0.f;
-                for (int step = odd; i < n_mine; step += 2) {
+                for (int step = pair; i < n_mine; step += kPairs) {
                     while (rt >= n_q && i < n_mine) {
                         put(sum);
                         sum = 0.f;
@@ -563,7 +584,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     if (i == n_mine) break;
                     sum += take_step(step, kt, rt, rt);
-                    rt += 2;
+                    rt += kPairs;
                 }
             } else {
                 Ring qr;
@@ -574,11 +595,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int rt = r0; rt < n_q && ok; ++rt) {
                         const int qs = qr.slot;
                         wait(&b.qf[qs], qr.phase, step);
-                        if ((step & 1) == odd) sum0 += take_step(step, g * p.kg, rt, qs);
-                        ++step;
-                        if (nk == 2) {
-                            if ((step & 1) == odd) sum1 += take_step(step, g * p.kg + 1, rt, qs);
-                            ++step;
+                        for (int k = 0; k < nk; ++k, ++step) {
+                            if (step % kPairs != pair) continue;
+                            const float v = take_step(step, g * p.kg + k, rt, qs);
+                            if (k == 0) sum0 += v;
+                            else sum1 += v;
                         }
                         __syncwarp();
                         if (lane == 0) tc::mbar_arrive(&b.qe[qs]);
@@ -599,7 +620,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == 1) {
         __syncwarp();
         tc::fence_after_sync();
-        tc::tmem_dealloc(tmem, kSBufs * BM);
+        tc::tmem_dealloc(tmem, kTmemCols);
     }
 }
 
@@ -1016,15 +1037,17 @@ cudaError_t launch_tc(const WeightArgs& a, cudaStream_t s) {
         !make_map(&mk, a.k, BF16, D, a.n_head_kv, rows, 1, SEG))
         return cudaErrorInvalidValue;
     const int smem = TcLayout<D>::kBytes + 1024;
-    static std::atomic<unsigned> m0{0}, m1{0};
-    cudaError_t e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 0>), smem, m0);
-    if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 1>), smem, m1);
+    static std::atomic<unsigned> m0{0}, m1{0}, m2{0};
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 0, false>), smem, m0);
+    if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 1, false>), smem, m1);
+    if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 1, true>), smem, m2);
     if (e != cudaSuccess) return e;
     const int64_t K = a.n_head_kv;
-    e = launch_after(k7_pass<BF16, D, SEG, 0>, K * p.n_groups * p.splits, 1, kTcThreads, smem, s, mq, mk, a, p);
+    e = launch_after(k7_pass<BF16, D, SEG, 0, false>, K * p.n_groups * p.splits, 1, kTcThreads, smem, s, mq, mk, a, p);
     if (e == cudaSuccess) e = launch_after(k7_join, K * p.n_rt * BM / (kJoinThreads / 16), 1, kJoinThreads, 0, s, a, p);
     if (e == cudaSuccess)
-        e = launch_after(k7_pass<BF16, D, SEG, 1>, K * p.b_splits * p.r_splits, 1, kTcThreads, smem, s, mq, mk, a, p);
+        e = launch_after(p.resident ? k7_pass<BF16, D, SEG, 1, false> : k7_pass<BF16, D, SEG, 1, true>,
+                         K * p.b_splits * p.r_splits, 1, kTcThreads, smem, s, mq, mk, a, p);
     if (e != cudaSuccess || p.r_splits == 1) return e;
     return launch_after(k7_add, (a.kv_len + kJoinThreads - 1) / kJoinThreads, a.n_head_kv, kJoinThreads, 0, s, a,
                         (const float*)p.part, p.n_kt * BM, p.r_splits);
