@@ -26,15 +26,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
+// Slices of up to 2048 rows are held by 512 threads, 4 rows each (batches of
+// short sequences: 14 against 16 us with 1024 threads), longer ones by 1024
+// threads, 8 or 32 rows each (64 K rows: 26 against 28 us with 512).
+constexpr int kSliceS = 2048, kSliceM = 8192, kSliceL = 32768;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
-#ifndef K8_CLUSTER_ROWS
-#define K8_CLUSTER_ROWS 2048
-#endif
-constexpr int kClusterRows = K8_CLUSTER_ROWS;
-
+constexpr int kSms = 148;
 // Order-preserving key of a weight: larger weight, larger key; NaN as -inf;
 // +0 and -0 alike.
 __device__ __forceinline__ uint32_t weight_key(float x) {
@@ -49,11 +47,11 @@ struct EvictPlan {
     int32_t* list;  // [n_seq][Hkv][cap] kept rows, ascending
     int32_t cap;
     int32_t cluster;
-    int32_t per_thread;  // weights a thread of K8a holds; 0: the slices are too long, read again each time
+    int32_t slice;  // rows that a CTA of K8a holds, at most; 0: the slices are too long, read again each time
 };
 
 // Inclusive sum over the CTA's threads.
-template <class T>
+template <int kWarps, class T>
 __device__ __forceinline__ T scan_cta(T x, T* warp_sums, T& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -63,7 +61,7 @@ __device__ __forceinline__ T scan_cta(T x, T* warp_sums, T& total) {
     }
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    T w = warp_sums[lane];
+    T w = lane < kWarps ? warp_sums[lane] : 0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const T u = __shfl_up_sync(0xffffffffu, w, d);
@@ -75,15 +73,18 @@ __device__ __forceinline__ T scan_cta(T x, T* warp_sums, T& total) {
     return warp > 0 ? x + before : x;
 }
 
-// Thread t holds the KPT rows r0 + t, r0 + 1024 + t, ... of its CTA's slice
+// Thread t holds the KPT rows r0 + t, r0 + kThreads + t, ... of its CTA's slice
 // (KPT 0: any number of rows, read from memory each time).
-template <int KPT>
+template <int KPT, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a, const EvictPlan p) {
+    constexpr int kWarps = kThreads / 32;
     // counts of up to 32 K rows share a word with their neighbour's: half the
     // bytes to read from the other CTAs
     constexpr bool kPairs = KPT > 0;
     __shared__ __align__(8) int hist[3][kPairs ? kBins / 2 : kBins];
-    __shared__ uint64_t warp_sums[32], counts[kThreads], mine;
+    constexpr int kRuns = KPT > 0 ? KPT * kWarps : 1024;  // runs of 32 rows placed at a time
+    constexpr int kRunsEach = (kRuns + kThreads - 1) / kThreads;
+    __shared__ uint64_t warp_sums[32], counts[kRunsEach * kThreads], mine;
     __shared__ int s_digit, s_above, s_all, warp_counts[32];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = p.cluster, rank = blockIdx.x % C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -141,31 +142,42 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
                 }
             });
             sync_all();
-            // thread t has bins b and b - 1, counted from the top
-            const int b = bins - 1 - 2 * t;
-            int2 c[kMaxCluster];
+            // thread t has per_t pairs of bins, counted from the top
+            constexpr int kMost = kBins / 2 / kThreads > 0 ? kBins / 2 / kThreads : 1;
+            const int per_t = bins / 2 / kThreads > 0 ? bins / 2 / kThreads : 1;
+            int c0[kMost], c1[kMost], sum = 0;  // upper and lower bin of each pair, over the cluster
 #pragma unroll
-            for (int k = 0; k < kMaxCluster; ++k) {
-                c[k] = make_int2(0, 0);
-                if (b < 0 || k >= C) continue;
-                const int* other = cluster.map_shared_rank(&hist[d][0], k);
-                if constexpr (kPairs) c[k].x = other[b >> 1];
-                else c[k] = *reinterpret_cast<const int2*>(other + b - 1);
-            }
-            int c0 = 0, c1 = 0;
+            for (int q = 0; q < kMost; ++q) {
+                const int b = bins - 1 - 2 * (t * per_t + q);
+                int2 c[kMaxCluster];
 #pragma unroll
-            for (int k = 0; k < kMaxCluster; ++k) {
-                c0 += kPairs ? (int)((uint32_t)c[k].x >> 16) : c[k].y;
-                c1 += kPairs ? c[k].x & 0xffff : c[k].x;
+                for (int k = 0; k < kMaxCluster; ++k) {
+                    c[k] = make_int2(0, 0);
+                    if (q >= per_t || b < 0 || k >= C) continue;
+                    const int* other = cluster.map_shared_rank(&hist[d][0], k);
+                    if constexpr (kPairs) c[k].x = other[b >> 1];
+                    else c[k] = *reinterpret_cast<const int2*>(other + b - 1);
+                }
+                c0[q] = c1[q] = 0;
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; ++k) {
+                    c0[q] += kPairs ? (int)((uint32_t)c[k].x >> 16) : c[k].y;
+                    c1[q] += kPairs ? c[k].x & 0xffff : c[k].x;
+                }
+                sum += c0[q] + c1[q];
             }
             int total;
-            const int upto = scan_cta(c0 + c1, warp_counts, total);
-            const int above = upto - c0 - c1;
-            if (above < left && left <= upto) {
-                const bool first = left <= above + c0;
-                s_digit = first ? b : b - 1;
-                s_above = first ? above : above + c0;
-                s_all = (first ? c0 : c1) == left - s_above;
+            int above = scan_cta<kWarps>(sum, warp_counts, total) - sum;
+#pragma unroll
+            for (int q = 0; q < kMost; ++q) {
+                const int b = bins - 1 - 2 * (t * per_t + q), upto = above + c0[q] + c1[q];
+                if (above < left && left <= upto) {
+                    const bool first = left <= above + c0[q];
+                    s_digit = first ? b : b - 1;
+                    s_above = first ? above : above + c0[q];
+                    s_all = (first ? c0[q] : c1[q]) == left - s_above;
+                }
+                above = upto;
             }
             __syncthreads();
             key |= (uint32_t)s_digit << shift;
@@ -219,6 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
     uint64_t total;
     if constexpr (KPT > 0) {
         // rows in order are runs of 32, run i * 32 + warp
+        static_assert(KPT <= 32, "a bit per row");
         uint32_t hards = 0, eqs = 0;  // bit i: this thread's row i
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
@@ -230,10 +243,19 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
             if (lane == 0) counts[i * kWarps + warp] = c;
         }
         __syncthreads();
-        const uint64_t own = t < KPT * kWarps ? counts[t] : 0;
-        const uint64_t incl = scan_cta(own, warp_sums, total);
-        const uint64_t base = base_of(total);
-        counts[t] = base + incl - own;
+        uint64_t own[kRunsEach], sum = 0;
+#pragma unroll
+        for (int e = 0; e < kRunsEach; ++e) {
+            own[e] = t * kRunsEach + e < kRuns ? counts[t * kRunsEach + e] : 0;
+            sum += own[e];
+        }
+        uint64_t before = scan_cta<kWarps>(sum, warp_sums, total) - sum;
+        before += base_of(total);
+#pragma unroll
+        for (int e = 0; e < kRunsEach; ++e) {
+            counts[t * kRunsEach + e] = before;
+            before += own[e];
+        }
         cluster.barrier_arrive();  // `mine` of the others has been read
         __syncthreads();
 #pragma unroll
@@ -248,11 +270,11 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
             mark(r, x, hard, eq);
             sum += ((uint64_t)hard << 32) | (uint32_t)eq;
         });
-        scan_cta(sum, warp_sums, total);
+        scan_cta<kWarps>(sum, warp_sums, total);
         uint64_t base = base_of(total);
         cluster.barrier_arrive();
-        for (int c0 = r0; c0 < r1; c0 += kThreads * 32) {
-            const int runs = min(kThreads, (r1 - c0 + 31) / 32);
+        for (int c0 = r0; c0 < r1; c0 += kRuns * 32) {
+            const int runs = min(kRuns, (r1 - c0 + 31) / 32);
             auto weight = [&](int r) { return r < r1 ? acc[r] : 0.f; };
             for (int g = warp; g < runs; g += kWarps) {
                 const int r = c0 + g * 32 + lane;
@@ -262,9 +284,18 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
                 if (lane == 0) counts[g] = c;
             }
             __syncthreads();
-            const uint64_t own = t < runs ? counts[t] : 0;
-            const uint64_t incl = scan_cta(own, warp_sums, total);
-            counts[t] = base + incl - own;
+            uint64_t own[kRunsEach], sum = 0;
+#pragma unroll
+            for (int e = 0; e < kRunsEach; ++e) {
+                own[e] = t * kRunsEach + e < runs ? counts[t * kRunsEach + e] : 0;
+                sum += own[e];
+            }
+            uint64_t before = base + scan_cta<kWarps>(sum, warp_sums, total) - sum;
+#pragma unroll
+            for (int e = 0; e < kRunsEach; ++e) {
+                counts[t * kRunsEach + e] = before;
+                before += own[e];
+            }
             __syncthreads();
             for (int g = warp; g < runs; g += kWarps) {
                 const int r = c0 + g * 32 + lane;
@@ -371,14 +402,16 @@ __global__ void __launch_bounds__(kPlaceThreads) k8c_compact(const EvictArgs a, 
     }
 }
 
-// Grid (KV head, sequence): the weights of a slice too long for shared memory,
-// where they are.
-__global__ void __launch_bounds__(kThreads) k8d_compact_weights(const EvictArgs a, const EvictPlan p) {
+constexpr int kWeightThreads = 1024;
+
+// Grid (KV head, sequence): the weights of slices too long for registers,
+// compacted where they are.
+__global__ void __launch_bounds__(kWeightThreads) k8d_compact_weights(const EvictArgs a, const EvictPlan p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t sh = (int64_t)blockIdx.y * a.n_head_kv + blockIdx.x;
     const int m = p.kept[blockIdx.y];
     float* acc = a.acc_dst + sh * a.acc_dst_stride;
-    for (int i0 = 0; i0 < a.acc_dst_stride; i0 += kThreads) {
+    for (int i0 = 0; i0 < a.acc_dst_stride; i0 += kWeightThreads) {
         const int i = i0 + threadIdx.x;
         const float x = i < m ? acc[p.list[sh * p.cap + i]] : 0.f;
         __syncthreads();
@@ -391,11 +424,17 @@ size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 size_t plan_of(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t n_head_kv, char* ws, EvictPlan* p) {
     p->cap = n_keep < max_kv_len ? n_keep : max_kv_len;
-    // a CTA per kClusterRows rows, up to 8 per head
+    // One CTA per head when that fills the device; more for slices over 8 K
+    // rows, and where few heads leave SMs idle, down to 2 K rows.  (64 heads of
+    // 16 K rows: 67 us with clusters of 8, 35 with 4, 24 with 2.)
+    const int64_t runs = (int64_t)n_seq * n_head_kv;
+    auto slice = [&](int cluster) { return ((max_kv_len + cluster - 1) / cluster + 31) & ~31; };
     p->cluster = 1;
-    while (p->cluster < kMaxCluster && p->cluster * kClusterRows < max_kv_len) p->cluster *= 2;
-    const int each = ((max_kv_len + p->cluster - 1) / p->cluster + 31) & ~31;
-    p->per_thread = each <= 2 * kThreads ? 2 : each <= 8 * kThreads ? 8 : each <= 32 * kThreads ? 32 : 0;
+    while (p->cluster < kMaxCluster &&
+           (slice(p->cluster) > kSliceM || (slice(p->cluster) > kSliceS && runs * p->cluster * 2 <= kSms)))
+        p->cluster *= 2;
+    const int each = slice(p->cluster);
+    p->slice = each <= kSliceS ? kSliceS : each <= kSliceM ? kSliceM : each <= kSliceL ? kSliceL : 0;
     p->kept = reinterpret_cast<int32_t*>(ws);
     const size_t head = up16((size_t)n_seq * sizeof(int32_t));
     p->list = reinterpret_cast<int32_t*>(ws + head);
@@ -430,7 +469,7 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s) {
     if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(p.slice == kSliceS ? 512 : 1024);
     cfg.stream = s;
     cudaLaunchAttribute at[2]{};
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -440,10 +479,10 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s) {
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    cudaError_t e = p.per_thread == 2    ? cudaLaunchKernelEx(&cfg, k8a_select_rows<2>, a, p)
-                    : p.per_thread == 8  ? cudaLaunchKernelEx(&cfg, k8a_select_rows<8>, a, p)
-                    : p.per_thread == 32 ? cudaLaunchKernelEx(&cfg, k8a_select_rows<32>, a, p)
-                                         : cudaLaunchKernelEx(&cfg, k8a_select_rows<0>, a, p);
+    cudaError_t e = p.slice == kSliceS   ? cudaLaunchKernelEx(&cfg, k8a_select_rows<4, 512>, a, p)
+                    : p.slice == kSliceM ? cudaLaunchKernelEx(&cfg, k8a_select_rows<8, 1024>, a, p)
+                    : p.slice == kSliceL ? cudaLaunchKernelEx(&cfg, k8a_select_rows<32, 1024>, a, p)
+                                         : cudaLaunchKernelEx(&cfg, k8a_select_rows<0, 1024>, a, p);
     if (e != cudaSuccess) return e;
     const int nv = a.head_dim * a.elem_bytes / 16;
     if (a.in_place) {
@@ -455,8 +494,8 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s) {
         else if (nv == 16) e = launch_after(k8b_move<16>, grid, kMoveThreads, s, a, p);
         else e = launch_after(k8b_move<32>, grid, kMoveThreads, s, a, p);
     }
-    if (e == cudaSuccess && a.acc_dst == a.acc && p.per_thread == 0) {
-        k8d_compact_weights<<<dim3(a.n_head_kv, a.src.n_seq), kThreads, 0, s>>>(a, p);
+    if (e == cudaSuccess && a.acc_dst == a.acc && p.slice == 0) {
+        k8d_compact_weights<<<dim3(a.n_head_kv, a.src.n_seq), kWeightThreads, 0, s>>>(a, p);
         e = cudaGetLastError();
     }
     return e;

@@ -82,6 +82,14 @@ def test_query_heads_per_kv_head(heads, dtype):
     run_case([5, 0, 129, 700], heads, dtype, F32, 32, 32, True, True, seed=heads[0])
 
 
+@pytest.mark.parametrize("heads", [(7, 1, 128), (17, 1, 64), (65, 1, 128), (128, 1, 64), (256, 2, 128)], ids=str)
+@pytest.mark.parametrize("dtype,out", [(BF16, BF16), (BF16, F32), (F16, F16), (F32, F32)], ids=["bf16", "bf16_f32", "f16", "f32"])
+def test_few_rows_without_a_split(heads, dtype, out):
+    """Up to 512 rows and as many runs as SMs: a CTA per run, no second kernel unless weights are kept."""
+    run_case([3, 0, 300, 512], heads, dtype, out, 32, 32, True, False, seed=heads[0])
+    run_case([33], heads, dtype, out, 32, 0, False, True, seed=heads[0])
+
+
 def test_empty_batch_and_capacity_above_the_lengths():
     run_case([0, 0, 0], (32, 8, 128), BF16, BF16, 128, 128, True, True, cap=5000)
     run_case([3, 0, 70], (32, 8, 128), BF16, BF16, 128, 128, True, True, cap=5000, extra_stride=13)

@@ -64,7 +64,7 @@ def test_whole_prompt(dtype):
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("kv_len,n_tok,row_begin,heads", [
     (257, 174, 100, (16, 1, 128)), (300, 290, 0, (48, 1, 64)), (130, 129, 0, (100, 1, 64)), (700, 700, 0, (64, 2, 128)),
-    (1000, 600, 0, (7, 1, 64))], ids=str)
+    (1000, 600, 0, (7, 1, 64)), (2000, 2000, 0, (16, 1, 128)), (7680, 320, 0, (16, 1, 128))], ids=str)
 def test_many_rows_over_few_keys(kv_len, n_tok, row_begin, heads, dtype):
     """The rows of the sums are split over the device, and their parts put together."""
     run_case(kv_len, n_tok, row_begin, heads, dtype, 32, 32, seed=kv_len)

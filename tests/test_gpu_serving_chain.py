@@ -8,7 +8,7 @@ import torch
 
 import epsp
 import workloads as W
-from serving_util import context, decode64, kept64, prompt64, rounding, workspace
+from serving_util import Cache, context, decode64, kept64, prompt64, rounding, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -165,3 +165,83 @@ def test_prefill_after_decoding_over_a_cut_back_sequence(dtype):
     assert int(outs[0][2].sum()) > 0
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+def test_blocks_past_32_bit_offsets():
+    """Pools of 2.2 M rows of 8 heads x 128 bf16 (4.5 GB each): the sequence's blocks lie at the end, past 2^31 elements
+    and 2^32 bytes."""
+    H, K, d, P, n, keep = 32, 8, 128, 128, 700, 256
+    rows = 17200 * P
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(n, K, d, generator=g).bfloat16().cuda() for _ in range(2))
+    kp, vp = (torch.empty(rows, K, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    used = -(-n // P)
+    table = torch.tensor([17199 - 3 * i for i in range(used)], dtype=torch.int32, device="cuda")
+    far = torch.tensor([17198, 17195], dtype=torch.int32, device="cuda")
+    at = table.long()[torch.arange(n, device="cuda") // P] * P + torch.arange(n, device="cuda") % P
+    assert int(at.min()) * K * d > 2 ** 31
+    kp[at], vp[at] = k, v
+    ctx = context(H, K, d, epsp.BF16, epsp.F32, 1024, P)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    kv = epsp.KvBatch(lens, n, table[None], P, rows)
+    q = torch.randn(40, H, d, generator=g).bfloat16().cuda()
+    out, acc = torch.zeros(1, H, d, device="cuda"), torch.zeros(1, K, n, device="cuda")
+    new = torch.randn(2, 1, K, d, generator=g).bfloat16().cuda()
+    ws = workspace(max(ctx.decode_bytes(1, n, True), ctx.prompt_weights_bytes(n, 40, 0), ctx.evict_bytes(1, n, keep)))
+    ctx.check(ctx.decode_layer(0, kv, q[:1].contiguous(), kp, vp, out, ws, k_new=new[0], v_new=new[1], acc=acc))
+    k[-1], v[-1] = new[0, 0], new[1, 0]
+    ref, tol, add, add_tol = decode64(Plain(k, v), q[:1])
+    assert ((out.double() - ref).abs() <= tol + rounding(ref, epsp.F32)).all()
+    assert ((acc.double() - add).abs() <= add_tol).all()
+    assert torch.equal(kp[at[-1]], new[0, 0]) and torch.equal(vp[at[-1]], new[1, 0])
+    ctx.check(ctx.set_paged_kv(P, table, used, rows))
+    acc2 = torch.zeros(K, n, device="cuda")
+    ctx.check(ctx.prompt_weights(0, q, kp, n, 40, 0, acc2, ws))
+    ref, tol = prompt64(q, k, n, 40, 0)
+    assert ((acc2.double() - ref).abs() <= tol).all()
+    dst = epsp.KvBatch(None, keep, far[None], P, rows, n_seq=1)
+    ctx.check(ctx.evict_layer(0, kv, kp, vp, acc2[None], keep, 4, 30, dst, kp, vp, ws))
+    ctx.check(ctx.sync_status())
+    a_host = acc2.cpu().tolist()
+    to = far.long()[torch.arange(keep, device="cuda") // P] * P + torch.arange(keep, device="cuda") % P
+    for h in range(K):
+        idx = torch.tensor(kept64(a_host[h], n, keep, 4, 30), device="cuda")
+        assert torch.equal(kp[to, h], k[idx, h]) and torch.equal(vp[to, h], v[idx, h])
+
+
+def test_calls_on_two_streams_at_once():
+    """Two sequences' steps on two streams of one context, each with its own workspace and caches."""
+    H, K, d, n = 8, 2, 64, 3000
+    ctx = context(H, K, d, epsp.F16, epsp.F32, n, 32)
+    sides = []
+    for seed in (1, 2):
+        g = torch.Generator().manual_seed(seed)
+        c = Cache([n], K, d, epsp.F16, 32, seed)
+        q = torch.randn(30, H, d, generator=g).half().cuda()
+        small = Cache([500], K, d, epsp.F16, 32, seed + 9)
+        need = max(ctx.decode_bytes(1, n, True), ctx.evict_bytes(1, n, 500), ctx.prompt_weights_bytes(n, 30, 0))
+        sides.append(dict(c=c, q=q, q1=q[:1].contiguous(), out=torch.zeros(1, H, d, device="cuda"), small=small,
+                          acc=torch.zeros(1, K, n, device="cuda"), ws=workspace(need), s=torch.cuda.Stream(),
+                          wacc=torch.zeros(K, n, device="cuda"),
+                          kept=torch.zeros(1, K, 500, dtype=torch.int32, device="cuda")))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for x in sides:
+            with torch.cuda.stream(x["s"]):
+                x["acc"].zero_()
+                c = x["c"]
+                ctx.check(ctx.decode_layer(0, c.batch, x["q1"], c.k, c.v, x["out"], x["ws"], acc=x["acc"]))
+                ctx.check(ctx.set_paged_kv(32, c.d_table[0], c.d_table.shape[1], c.rows))
+                ctx.check(ctx.prompt_weights(0, x["q"], c.k, n, 30, 0, x["wacc"], x["ws"]))
+                ctx.check(ctx.evict_layer(0, c.batch, c.k, c.v, x["acc"], 500, 4, 30, x["small"].batch, x["small"].k,
+                                          x["small"].v, x["ws"], kept_rows=x["kept"]))
+    torch.cuda.synchronize()
+    ctx.check(ctx.sync_status())
+    for x in sides:
+        ref, tol, add, add_tol = decode64(x["c"], x["q1"])
+        assert ((x["out"].double() - ref).abs() <= tol + rounding(ref, epsp.F32)).all()
+        assert ((x["acc"].double() - add).abs() <= add_tol).all()
+        ref, tol = prompt64(x["q"], x["c"].seq(0)[0], n, 30, 0)
+        assert ((x["wacc"].double() - ref).abs() <= tol).all()
+        a_host = x["acc"][0].cpu().tolist()
+        assert x["kept"][0].tolist() == [kept64(a_host[h], n, 500, 4, 30) for h in range(K)]
