@@ -72,30 +72,30 @@ int32_t launch(ep_sp_ctx* c, Family f, void* stream, const char* what, F&& go) {
 // Layout rules of one batch; `min_rows` is what each sequence must have room for.
 int32_t check_batch(ep_sp_ctx* c, const ep_sp_kv_batch* b, int32_t min_rows, bool need_lens, const char* who,
                     epsp::BatchKv* out) {
-    const std::string w = std::string(who) + ": ";
-    if (!b) return ctx_fail(c, kInvalid, w + "null batch");
-    if (b->n_seq < 1 || b->n_seq > 65535) return ctx_fail(c, kInvalid, w + "n_seq must lie in [1, 65535]");
+    auto bad = [&](const char* what) { return ctx_fail(c, kInvalid, std::string(who) + ": " + what); };
+    if (!b) return bad("null batch");
+    if (b->n_seq < 1 || b->n_seq > 65535) return bad("n_seq must lie in [1, 65535]");
     if (b->max_kv_len < 1 || b->max_kv_len > c->cfg.max_ctx)
-        return ctx_fail(c, kInvalid, w + "max_kv_len must lie in [1, max_ctx]");
-    if (need_lens && !b->kv_lens) return ctx_fail(c, kInvalid, w + "null kv_lens");
+        return bad("max_kv_len must lie in [1, max_ctx]");
+    if (need_lens && !b->kv_lens) return bad("null kv_lens");
     const int32_t rows = std::max(min_rows, 1);
     out->n_seq = b->n_seq;
     out->max_kv_len = b->max_kv_len;
     out->lens = b->kv_lens;
     if (b->block_rows == 0) {
-        if (b->seq_rows < rows) return ctx_fail(c, kInvalid, w + "seq_rows does not cover max_kv_len rows");
+        if (b->seq_rows < rows) return bad("seq_rows does not cover max_kv_len rows");
         const int64_t all = (int64_t)b->n_seq * b->seq_rows;
-        if (all > INT_MAX) return ctx_fail(c, kInvalid, w + "more than 2^31 - 1 cache rows");
+        if (all > INT_MAX) return bad("more than 2^31 - 1 cache rows");
         out->seq_rows = b->seq_rows;
         out->rows = (int32_t)all;
         return kOk;
     }
     if (b->block_rows < 0 || b->block_rows % c->cfg.page_size)
-        return ctx_fail(c, kInvalid, w + "block_rows must be a multiple of the page size");
+        return bad("block_rows must be a multiple of the page size");
     if (!b->block_tables || b->pool_rows < b->block_rows || b->pool_rows % b->block_rows)
-        return ctx_fail(c, kInvalid, w + "block tables and a pool of whole blocks are needed");
+        return bad("block tables and a pool of whole blocks are needed");
     if (b->table_stride < 1 || (int64_t)b->table_stride * b->block_rows < rows)
-        return ctx_fail(c, kInvalid, w + "the block tables do not cover max_kv_len rows");
+        return bad("the block tables do not cover max_kv_len rows");
     out->tables = b->block_tables;
     out->table_stride = b->table_stride;
     out->block_rows = b->block_rows;

@@ -209,12 +209,17 @@ def _torch_dtypes():
 _DTYPES: dict = {}  # the torch types of F32, F16, BF16 and "i32", filled by the first batch or context call
 
 
-def _current_stream(device):
-    """The raw current stream of a device (the direct query where torch has it: a tenth of the time)."""
-    import torch
+_RAW_STREAM = []  # torch's direct query of a device's current stream, where it has one
 
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+def _current_stream(device):
+    """The raw current stream of a device (the direct query takes a tenth of the time)."""
+    if not _RAW_STREAM:
+        import torch
+
+        _RAW_STREAM.append(getattr(torch._C, "_cuda_getCurrentRawStream", None)
+                           or (lambda d: torch.cuda.current_stream(d).cuda_stream))
+    return _RAW_STREAM[0](device)
 
 
 def _dtype(code):
@@ -224,17 +229,16 @@ def _dtype(code):
 
 
 def _check(name, t, dtype, shape, device):
-    """The library sees plain pointers: what a tensor is must be checked here.  The trailing dimensions are `shape`
-    (an entry None is any size)."""
+    """The library sees plain pointers: what a tensor is must be checked here."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return
     if t.dtype is not dtype:
         raise ValueError(f"{name} is {t.dtype}, not {dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name} is not contiguous (strides {tuple(t.stride())})")
     if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, not cuda:{device}")
-    if t.shape != shape and (len(t.shape) != len(shape)
-                             or any(w is not None and h != w for h, w in zip(t.shape, shape))):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
+    raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
 
 
 class KvBatch:
@@ -256,7 +260,7 @@ class KvBatch:
         if block_rows:
             if block_tables is None:
                 raise ValueError("block_rows without block_tables")
-            _check("block_tables", block_tables, _dtype("i32"), (self.n_seq, None), self.device)
+            _check("block_tables", block_tables, _dtype("i32"), (self.n_seq, block_tables.shape[-1]), self.device)
             entries = block_tables.shape[1]
         self.rows = pool_rows if block_rows else self.n_seq * seq_rows
         self.desc = KvBatchDesc(self.n_seq, max_kv_len, _ptr(kv_lens), _ptr(block_tables) if block_rows else None,
@@ -272,6 +276,7 @@ class Context:
         self.cfg = Config(n_layer, n_head, n_head_kv, head_dim, dtype, dtype if out_dtype is None else out_dtype,
                           max_ctx, page_size, device, kv_head_offset, n_head_kv_total, kq_scale)
         self._pool_rows = 0  # rows of the pools of set_paged_kv
+        self._facts = None   # see _fast
         self.h = c_void_p()
         rc = lib.ep_sp_create(ctypes.byref(self.cfg), ctypes.byref(self.h))
         if rc != OK:
@@ -423,23 +428,32 @@ class Context:
         return rc
 
     # ------------------------------- answering from and shrinking the cache
+    def _fast(self):
+        """(torch type, output type, f32, int32, device, n_head, n_head_kv, head_dim), read once: a ctypes field costs
+        as much as a check."""
+        f = self._facts
+        if f is None:
+            c = self.cfg
+            f = self._facts = (_dtype(c.dtype), _dtype(c.out_dtype), _dtype(F32), _dtype("i32"), c.device, c.n_head,
+                               c.n_head_kv, c.head_dim)
+        return f
+
     def _cache_tensors(self, kv, k, v, what=("k", "v")):
-        c = self.cfg
-        if kv.device is not None and kv.device != c.device:
-            raise ValueError(f"the batch is on cuda:{kv.device}, not cuda:{c.device}")
-        dt, heads, d, need = _dtype(c.dtype), c.n_head_kv, c.head_dim, kv.rows * c.n_head_kv * c.head_dim
+        dt, _, _, _, dev, _, heads, d = self._fast()
+        if kv.device is not None and kv.device != dev:
+            raise ValueError(f"the batch is on cuda:{kv.device}, not cuda:{dev}")
+        need = kv.rows * heads * d
         for name, t in zip(what, (k, v)):
             # rows in any number of leading dimensions
-            if (t.dtype is not dt or t.get_device() != c.device or not t.is_contiguous()
-                    or t.shape[-2:] != (heads, d)):
-                _check(name, t, dt, t.shape[:-2] + (heads, d), c.device)
+            if t.dtype is not dt or t.get_device() != dev or not t.is_contiguous() or t.shape[-2:] != (heads, d):
+                _check(name, t, dt, t.shape[:-2] + (heads, d), dev)
             if t.numel() < need:
                 raise ValueError(f"{name} holds fewer than the batch's {kv.rows} rows")
 
     def _workspace(self, t):
         if t is None:
             return None, 0
-        if not t.is_contiguous() or t.get_device() != self.cfg.device:
+        if not t.is_contiguous() or t.get_device() != self._fast()[4]:
             raise ValueError(f"the workspace must be a contiguous tensor on cuda:{self.cfg.device}")
         return t.data_ptr(), t.numel() * t.element_size()
 
@@ -452,16 +466,17 @@ class Context:
         """kv: KvBatch; q, out [n_seq][n_head][head_dim]; k, v the cache's rows; k_new, v_new [n_seq][n_head_kv]
         [head_dim]; acc f32 [n_seq][n_head_kv][stride].  Raises ValueError for a tensor of another type, shape,
         layout or device; returns the status code."""
-        c = self.cfg
-        dt = _dtype(c.dtype)
+        dt, odt, f32, _, dev, heads, kvh, d = self._fast()
         self._cache_tensors(kv, k, v)
-        _check("q", q, dt, (kv.n_seq, c.n_head, c.head_dim), c.device)
-        _check("out", out, _dtype(c.out_dtype), (kv.n_seq, c.n_head, c.head_dim), c.device)
-        for name, t in (("k_new", k_new), ("v_new", v_new)):
-            if t is not None:
-                _check(name, t, dt, (kv.n_seq, c.n_head_kv, c.head_dim), c.device)
+        n_seq = kv.n_seq
+        _check("q", q, dt, (n_seq, heads, d), dev)
+        _check("out", out, odt, (n_seq, heads, d), dev)
+        if k_new is not None:
+            _check("k_new", k_new, dt, (n_seq, kvh, d), dev)
+        if v_new is not None:
+            _check("v_new", v_new, dt, (n_seq, kvh, d), dev)
         if acc is not None:
-            _check("acc", acc, _dtype(F32), (kv.n_seq, c.n_head_kv, None), c.device)
+            _check("acc", acc, f32, (n_seq, kvh, acc.shape[-1]), dev)
         ws, n = self._workspace(workspace)
         return lib.ep_sp_decode_layer(self.h, layer, kv.ref, q.data_ptr(), _ptr(k_new), _ptr(v_new), k.data_ptr(),
                                       v.data_ptr(), out.data_ptr(), _ptr(acc), 0 if acc is None else acc.shape[-1],
@@ -474,13 +489,12 @@ class Context:
 
     def prompt_weights(self, layer, q, k, kv_len, n_tok, row_begin, acc, workspace, accumulate=False, stream=None):
         """q [n_tok][n_head][head_dim]; k the cache (paged under set_paged_kv); acc f32 [n_head_kv][stride]."""
-        c = self.cfg
-        dt = _dtype(c.dtype)
-        _check("q", q, dt, (n_tok, c.n_head, c.head_dim), c.device)
-        _check("k", k, dt, (None, c.n_head_kv, c.head_dim), c.device)
+        dt, _, f32, _, dev, heads, kvh, d = self._fast()
+        _check("q", q, dt, (n_tok, heads, d), dev)
+        _check("k", k, dt, (k.shape[0], kvh, d), dev)
         if k.shape[0] < (self._pool_rows or kv_len):
             raise ValueError(f"k holds {k.shape[0]} rows, the call reads {self._pool_rows or kv_len}")
-        _check("acc", acc, _dtype(F32), (c.n_head_kv, None), c.device)
+        _check("acc", acc, f32, (kvh, acc.shape[-1]), dev)
         ws, n = self._workspace(workspace)
         return lib.ep_sp_prompt_weights(self.h, layer, q.data_ptr(), k.data_ptr(), kv_len, n_tok, row_begin,
                                         1 if accumulate else 0, acc.data_ptr(), acc.shape[-1], ws, n,
@@ -495,16 +509,17 @@ class Context:
                     acc_dst=None, new_lens=None, kept_rows=None, stream=None):
         """src, dst: KvBatch (the same object and tensors compact in place); acc f32 [n_seq][n_head_kv][stride];
         acc_dst likewise; new_lens int32 [n_seq]; kept_rows int32 [n_seq][n_head_kv][n_keep]."""
-        c = self.cfg
+        _, _, f32, i32, dev, _, kvh, _ = self._fast()
         self._cache_tensors(src, k, v)
         self._cache_tensors(dst, k_dst, v_dst, ("k_dst", "v_dst"))
-        _check("acc", acc, _dtype(F32), (src.n_seq, c.n_head_kv, None), c.device)
+        n_seq = src.n_seq
+        _check("acc", acc, f32, (n_seq, kvh, acc.shape[-1]), dev)
         if acc_dst is not None:
-            _check("acc_dst", acc_dst, _dtype(F32), (src.n_seq, c.n_head_kv, None), c.device)
+            _check("acc_dst", acc_dst, f32, (n_seq, kvh, acc_dst.shape[-1]), dev)
         if new_lens is not None:
-            _check("new_lens", new_lens, _dtype("i32"), (src.n_seq,), c.device)
+            _check("new_lens", new_lens, i32, (n_seq,), dev)
         if kept_rows is not None:
-            _check("kept_rows", kept_rows, _dtype("i32"), (src.n_seq, c.n_head_kv, n_keep), c.device)
+            _check("kept_rows", kept_rows, i32, (n_seq, kvh, n_keep), dev)
         ws, n = self._workspace(workspace)
         return lib.ep_sp_evict_layer(self.h, layer, src.ref, k.data_ptr(), v.data_ptr(), acc.data_ptr(),
                                      acc.shape[-1], n_keep, sink_rows, recent_rows, dst.ref, k_dst.data_ptr(),
@@ -520,7 +535,7 @@ class Context:
     def _stream(self, stream):
         """The given stream, or the current one of the context's device."""
         if stream is None:
-            return _current_stream(self.cfg.device)
+            return _current_stream(self._fast()[4])
         return stream if isinstance(stream, int) else stream.cuda_stream
 
     def set_head_routing(self, mode, threshold):
