@@ -78,6 +78,7 @@ struct DecodeSplit {
     // workspace
     int32_t* per;        // cost per CTA
     int32_t* run_start;  // [n_seq][Hkv][passes] where each run starts in the cost of all
+    int32_t* lens;       // [n_seq] this call's view of the lengths (more sequences than a CTA keeps on chip)
     int4* cut;           // [ctas] (sequence, run, start, units) of a run that goes on past the CTA it began in; -1: none
     float* part_o;       // [2 ctas][groups * 8][D]
     float2* part_ml;     // [2 ctas][groups * 8] (maximum, sum), log2 units
@@ -180,7 +181,9 @@ struct Layout {
 
 static_assert(kUnit == 32, "a lane per row, a page holds whole units");
 
-// The sequences' lengths: on chip when there are few.
+// The sequences' lengths: on chip when there are few, else the copy that
+// k6_lengths made.  Either way a CTA reads each once, or from memory that
+// nobody else writes: its warps must agree on the segments they meet at.
 struct Lens {
     const int32_t* chip;
     __device__ __forceinline__ int32_t at(const DecodeArgs& a, int s) const {
@@ -344,10 +347,11 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
         w0.s = blockIdx.x / runs;
         w0.run = blockIdx.x % runs;
         w0.u = 0;
-        w0.n = batch_len(a.kv, w0.s, a.err);
+        if (threadIdx.x == 0) lens_s[0] = batch_len(a.kv, w0.s, a.err);
+        __syncthreads();
+        w0.n = lens_s[0];
         w0.units = units_of(w0.n);
         w0.left = w0.units;
-        __syncthreads();
     } else {
         if (a.kv.n_seq <= kLensOnChip) {
             for (int s = threadIdx.x; s < a.kv.n_seq; s += kThreads) lens_s[s] = batch_len(a.kv, s, a.err);
@@ -758,9 +762,11 @@ struct Shares {
         return 2 * c + (i == 0 && start > c * per ? 1 : 0);
     }
 };
-__device__ __forceinline__ Shares shares_of(int32_t per, int32_t start, int units) {
-    const int u0 = start + kRunCost, c0 = u0 / per;  // the first unit comes after the run's cost
-    return {per, start, c0, (u0 + units - 1) / per - c0 + 1};
+// (Lengths that change under the call give wrong shares, never ones past the
+// last CTA.)
+__device__ __forceinline__ Shares shares_of(const DecodeSplit& sp, int32_t per, int32_t start, int units) {
+    const int u0 = start + kRunCost, c0 = min(u0 / per, sp.ctas - 1);  // the first unit comes after the run's cost
+    return {per, start, c0, min((u0 + units - 1) / per, sp.ctas - 1) - c0 + 1};
 }
 
 // Maximum and sum of one head over its shares (a warp; the same in every lane).
@@ -780,6 +786,13 @@ __device__ __forceinline__ float2 join_ml(const DecodeSplit& sp, const Shares& s
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
     return make_float2(ms, l);
+}
+
+__global__ void k6_lengths(const DecodeArgs a, int32_t* lens) {
+    tc::pdl_wait();
+    tc::pdl_launch();
+    const int s = blockIdx.x * blockDim.x + threadIdx.x;
+    if (s < a.kv.n_seq) lens[s] = batch_len(a.kv, s, a.err);
 }
 
 constexpr int kJoinThreads = 256;
@@ -807,7 +820,7 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
         const int gi = blockIdx.x % heads, h = cut.y / sp.passes, g = cut.y % sp.passes * sp.pass_heads + gi;
         if (g >= G) return;
         const int64_t out = ((int64_t)cut.x * a.n_head + h * G + g) * D;
-        const Shares sh = shares_of(per, cut.z, cut.w);
+        const Shares sh = shares_of(sp, per, cut.z, cut.w);
         constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes, kHeld = 4;
         const int c = threadIdx.x % kLanes, r = threadIdx.x / kLanes;
         auto part_of = [&](int i) {
@@ -855,7 +868,7 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
     for (int g = warp; g < G; g += kJoinThreads / 32) {
         const int pass = g / sp.pass_heads;
         const Shares sh = sp.direct ? Shares{1, 0, 0, 1}
-                                    : shares_of(per, sp.run_start[(int64_t)s * runs + h * sp.passes + pass], units);
+                                    : shares_of(sp, per, sp.run_start[(int64_t)s * runs + h * sp.passes + pass], units);
         float x;
         if (sh.count == 1) {
             x = sp.lse[(int64_t)s * a.n_head + h * G + g];
@@ -964,6 +977,7 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
     if (!sp->direct) {
         sp->run_start = reinterpret_cast<int32_t*>(take(all_runs * sizeof(int32_t)));
         sp->cut = reinterpret_cast<int4*>(take(sp->ctas * sizeof(int4)));
+        if (n_seq > kLensOnChip) sp->lens = reinterpret_cast<int32_t*>(take(n_seq * sizeof(int32_t)));
         sp->part_ml = reinterpret_cast<float2*>(take((size_t)2 * sp->ctas * stride * sizeof(float2)));
         sp->part_o = reinterpret_cast<float*>(take((size_t)2 * sp->ctas * stride * d * sizeof(float)));
     }
@@ -975,7 +989,7 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
 }
 
 template <int ET, int D, int W, bool P3, int GH>
-cudaError_t launch_t(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s) {
+cudaError_t launch_t(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     constexpr int kThreads = (W + 1) * 32;
     CUtensorMap mk, mv;
     if (!cache_map(&mk, a.k, a.dtype, D, a.n_head_kv, a.kv.rows) ||
@@ -1001,6 +1015,13 @@ cudaError_t launch_t(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s)
     cfg.attrs = &at;
     cfg.numAttrs = 1;
     cfg.stream = s;
+    if (sp.lens) {
+        cfg.gridDim = dim3((a.kv.n_seq + 255) / 256);
+        cfg.blockDim = dim3(256);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, k6_lengths, a, sp.lens);
+        if (e != cudaSuccess) return e;
+        a.kv.lens = sp.lens;
+    }
     cfg.gridDim = dim3(sp.ctas);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;

@@ -85,14 +85,26 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
     constexpr int kRuns = KPT > 0 ? KPT * kWarps : 1024;  // runs of 32 rows placed at a time
     constexpr int kRunsEach = (kRuns + kThreads - 1) / kThreads;
     __shared__ uint64_t warp_sums[32], counts[kRunsEach * kThreads], mine;
-    __shared__ int s_digit, s_above, s_all, warp_counts[32];
+    __shared__ int s_len, s_digit, s_above, s_all, warp_counts[32];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = p.cluster, rank = blockIdx.x % C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int h = blockIdx.x / C % a.n_head_kv, s = blockIdx.x / C / a.n_head_kv;
     for (int i = t; i < (int)(sizeof(hist) / 8); i += kThreads) reinterpret_cast<int2*>(&hist[0][0])[i] = make_int2(0, 0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int n = batch_len(a.src, s, a.err), m = min(n, a.n_keep);
+    // one reading of the length for the whole cluster: its CTAs must take the
+    // same turns
+    int n;
+    if (C > 1) {
+        if (rank == 0 && t == 0) s_len = batch_len(a.src, s, a.err);
+        cluster.sync();
+        n = *cluster.map_shared_rank(&s_len, 0);
+    } else {
+        if (t == 0) s_len = batch_len(a.src, s, a.err);
+        __syncthreads();
+        n = s_len;
+    }
+    const int m = min(n, a.n_keep);
     const int64_t sh = (int64_t)s * a.n_head_kv + h;
     const float* acc = a.acc + sh * a.acc_stride;
     if (h == 0 && rank == 0 && t == 0) p.kept[s] = m;
