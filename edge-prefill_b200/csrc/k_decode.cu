@@ -30,7 +30,11 @@
 // lane for O.
 //
 // Weights: the scores are kept in the workspace (4 bytes per query head and
-// row against the 4 d / G of K and V) and k6b_join adds exp(x - lse).
+// row against the 4 d / G of K and V) and k6b_join adds exp(x - lse).  They are
+// written with evict_last, so that the cache streaming past leaves them in L2,
+// and given up there once read, so that they never go out to memory (8 x 16-32 K
+// rows, 28 heads, 22 MB of scores: 95.5 us without either, 90 with the first, 85
+// with both).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -50,17 +54,10 @@ namespace {
 constexpr int kUnit = 32;      // cache rows per unit
 constexpr int kCtas = 148;     // one per SM
 constexpr int kChunk = kUnit * 128;  // one 128-byte column block of a unit
-// Fewest units dealt to a CTA.
-#ifndef K6_MIN_UNITS
-#define K6_MIN_UNITS 4
-#endif
-constexpr int kMinUnits = K6_MIN_UNITS;
+constexpr int kMinUnits = 4;  // fewest units dealt to a CTA
 // What a run costs a CTA besides its units (the merge of the warps' states),
 // in units: the ranges are equal in this measure.
-#ifndef K6_RUN_COST
-#define K6_RUN_COST 6
-#endif
-constexpr int kRunCost = K6_RUN_COST;
+constexpr int kRunCost = 6;
 constexpr int kLensOnChip = 1024;  // lengths a CTA keeps in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 // A call of at most this many units per run and one CTA per run skips the
@@ -70,6 +67,8 @@ constexpr int kDirectUnits = 16;
 struct DecodeSplit {
     int32_t ctas;      // grid
     int32_t direct;    // one CTA per run
+    int32_t by_run;    // cut has a place per run (no more runs than CTAs), not one per CTA
+    int32_t joins;     // places of cut
     int32_t pass_heads;  // query heads of a pass, at most
     int32_t passes;    // passes per KV head
     int32_t groups;    // warps that share a unit (1, 2, 4, 8)
@@ -79,7 +78,7 @@ struct DecodeSplit {
     int32_t* per;        // cost per CTA
     int32_t* run_start;  // [n_seq][Hkv][passes] where each run starts in the cost of all
     int32_t* lens;       // [n_seq] this call's view of the lengths (more sequences than a CTA keeps on chip)
-    int4* cut;           // [ctas] (sequence, run, start, units) of a run that goes on past the CTA it began in; -1: none
+    int4* cut;           // [joins] (sequence, run, start, units) of a run that goes on past the CTA it began in; -1: none
     float* part_o;       // [2 ctas][groups * 8][D]
     float2* part_ml;     // [2 ctas][groups * 8] (maximum, sum), log2 units
     float* lse;          // [n_seq][n_head] log2 units, runs finished by one CTA
@@ -361,10 +360,13 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
         w0 = share_of(a, sp, lens, runs, lane);
         // sequences without rows, dealt out to the CTAs
         for (int s = blockIdx.x; s < a.kv.n_seq; s += gridDim.x)
-            if (lens.at(a, s) == 0)
+            if (lens.at(a, s) == 0) {
                 for (int i = threadIdx.x; i < a.n_head * (D / 4); i += kThreads)
                     store4(a.out, a.out_dtype, (int64_t)s * a.n_head * D + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-        if (w0.left <= 0 && threadIdx.x == 0) sp.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+                if (sp.by_run)
+                    for (int i = threadIdx.x; i < runs; i += kThreads) sp.cut[s * runs + i] = make_int4(-1, 0, 0, 0);
+            }
+        if (w0.left <= 0 && !sp.by_run && threadIdx.x == 0) sp.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
     if (w0.left <= 0) {
         if (sp.direct) {  // a sequence without rows
@@ -446,6 +448,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
     const int groups = sp.groups, streams = kWarps / groups;
     const int grp = warp & (groups - 1), stream = warp / groups;
     const float sl2 = a.kq_scale * kLog2e;
+    const uint64_t keep = tc::policy_evict_last();  // scores: read once more, by k6b_join
     float* om = reinterpret_cast<float*>(smem + LY::kOffO);
     float* om_w = om + warp * kHeads * D;
     float* ps = reinterpret_cast<float*>(smem + LY::kOffP) + warp * kUnit * kHeads;
@@ -538,7 +541,9 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                     float* sc = sp.scores + (q_row + g0 + hd) * sp.score_stride + u * kUnit + qc;
 #pragma unroll
                     for (int t = 0; t < 4; ++t)
-                        *reinterpret_cast<float2*>(sc + t * 8) = make_float2(s4[t][0], s4[t][1]);
+                        asm volatile("st.global.L2::cache_hint.v2.f32 [%0], {%1, %2}, %3;" ::"l"(sc + t * 8),
+                                     "f"(s4[t][0]), "f"(s4[t][1]), "l"(keep)
+                                     : "memory");
                 }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -611,7 +616,10 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                 for (int g = 0; g < GH; ++g) {
                     x[g] = lane < lim ? x[g] * sl2 : -INFINITY;
                     if (a.acc != nullptr && g0 + g < G)
-                        sp.scores[(q_row + g0 + g) * sp.score_stride + u * kUnit + lane] = x[g];
+                        asm volatile("st.global.L2::cache_hint.f32 [%0], %1, %2;" ::"l"(
+                                         sp.scores + (q_row + g0 + g) * sp.score_stride + u * kUnit + lane),
+                                     "f"(x[g]), "l"(keep)
+                                     : "memory");
                     mx[g] = x[g];
 #pragma unroll
                     for (int d = 16; d > 0; d >>= 1) mx[g] = fmaxf(mx[g], __shfl_xor_sync(0xffffffffu, mx[g], d));
@@ -746,8 +754,12 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
         }
         if (!sp.direct && threadIdx.x == 0) {
             if (w.u == 0) sp.run_start[(int64_t)w.s * runs + w.run] = w.at;
-            // the CTA's last segment has the last word
-            sp.cut[blockIdx.x] = w.u == 0 && n_seg < w.units ? make_int4(w.s, w.run, w.at, w.units) : make_int4(-1, 0, 0, 0);
+            const int4 c =
+                w.u == 0 && n_seg < w.units ? make_int4(w.s, w.run, w.at, w.units) : make_int4(-1, 0, 0, 0);
+            if (!sp.by_run)
+                sp.cut[blockIdx.x] = c;  // the CTA's last segment has the last word
+            else if (w.u == 0)
+                sp.cut[w.s * runs + w.run] = c;
         }
         it += n_seg;
         w.advance(a, lens, runs, n_seg);
@@ -762,11 +774,11 @@ struct Shares {
         return 2 * c + (i == 0 && start > c * per ? 1 : 0);
     }
 };
-// (Lengths that change under the call give wrong shares, never ones past the
-// last CTA.)
+// (Lengths that change under the call give wrong shares, never ones outside
+// the CTAs.)
 __device__ __forceinline__ Shares shares_of(const DecodeSplit& sp, int32_t per, int32_t start, int units) {
-    const int u0 = start + kRunCost, c0 = min(u0 / per, sp.ctas - 1);  // the first unit comes after the run's cost
-    return {per, start, c0, min((u0 + units - 1) / per, sp.ctas - 1) - c0 + 1};
+    const int u0 = start + kRunCost, c0 = min(max(u0 / per, 0), sp.ctas - 1);  // the first unit comes after the run's cost
+    return {per, start, c0, max(min((u0 + units - 1) / per, sp.ctas - 1) - c0, 0) + 1};
 }
 
 // Maximum and sum of one head over its shares (a warp; the same in every lane).
@@ -796,27 +808,29 @@ __global__ void k6_lengths(const DecodeArgs a, int32_t* lens) {
 }
 
 constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 1024;  // cache rows per weights CTA
+constexpr int kJoinRows = 4 * kJoinThreads;  // cache rows per weights CTA
+constexpr int kJoinHeads = 8;    // query heads whose scores a thread holds at a time
 
-// The first ctas * heads CTAs put together the outputs of the runs that several
+// The first joins * heads CTAs put together the outputs of the runs that several
 // CTAs shared (one CTA per query head of a run; at most one such run begins in
 // a CTA of k6a); the others, [n_seq][Hkv][chunks], add the weights of kJoinRows
-// rows of one KV head.
+// rows of one KV head.  Latency bounds it (lengths, then ranges, then sums, then
+// weights), so registers are held to four CTAs per SM.
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, const DecodeSplit sp, int heads,
+__global__ void __launch_bounds__(kJoinThreads, 4) k6b_join(const DecodeArgs a, const DecodeSplit sp, int heads,
                                                          int chunks) {
     __shared__ float wgt[kCtas];
     __shared__ float part[kJoinThreads * 4];
     __shared__ float lse[128];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = a.n_head / a.n_head_kv, runs = a.n_head_kv * sp.passes, stride = sp.groups * sp.heads;
-    const int joins = sp.direct ? 0 : sp.ctas * heads;
+    const int joins = sp.joins * heads;
     tc::pdl_wait();
     tc::pdl_launch();
     if ((int)blockIdx.x < joins) {
         const int4 cut = sp.cut[blockIdx.x / heads];
         const int32_t per = *sp.per;
-        if (cut.x < 0) return;
+        if (cut.x < 0 || cut.x >= a.kv.n_seq || cut.y < 0 || cut.y >= runs) return;
         const int gi = blockIdx.x % heads, h = cut.y / sp.passes, g = cut.y % sp.passes * sp.pass_heads + gi;
         if (g >= G) return;
         const int64_t out = ((int64_t)cut.x * a.n_head + h * G + g) * D;
@@ -862,6 +876,18 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
     }
     const int id = blockIdx.x - joins, s = id / chunks / a.n_head_kv;
     const int h = id / chunks % a.n_head_kv, j0 = (id % chunks) * kJoinRows;
+    // the first heads' scores are on their way while the sums are put together
+    // (rows past the length are read where there are any, and not used)
+    const int r0 = j0 + 4 * threadIdx.x;
+    const float* sc = sp.scores + ((int64_t)s * a.n_head + (int64_t)h * G) * sp.score_stride +
+                      min(r0, sp.score_stride - 4);
+    float4 x[kJoinHeads];
+    auto fetch = [&](int g0) {
+#pragma unroll
+        for (int g = 0; g < kJoinHeads; ++g)
+            if (g0 + g < G) x[g] = *reinterpret_cast<const float4*>(sc + (int64_t)(g0 + g) * sp.score_stride);
+    };
+    fetch(0);
     const int n = batch_len(a.kv, s, a.err), units = units_of(n);
     if (j0 >= n) return;
     const int32_t per = sp.direct ? 1 : *sp.per;
@@ -869,37 +895,54 @@ __global__ void __launch_bounds__(kJoinThreads) k6b_join(const DecodeArgs a, con
         const int pass = g / sp.pass_heads;
         const Shares sh = sp.direct ? Shares{1, 0, 0, 1}
                                     : shares_of(sp, per, sp.run_start[(int64_t)s * runs + h * sp.passes + pass], units);
-        float x;
+        float v;
         if (sh.count == 1) {
-            x = sp.lse[(int64_t)s * a.n_head + h * G + g];
+            v = sp.lse[(int64_t)s * a.n_head + h * G + g];
         } else {
-            const float2 v = join_ml(sp, sh, stride, g % sp.pass_heads, lane);
-            x = v.x + log2f(v.y);
+            const float2 t = join_ml(sp, sh, stride, g % sp.pass_heads, lane);
+            v = t.x + log2f(t.y);
         }
-        if (lane == 0) lse[g] = x;
+        if (lane == 0) lse[g] = v;
+    }
+    float* acc = a.acc + ((int64_t)s * a.n_head_kv + h) * a.acc_stride;
+    acc += r0;
+    const bool quad = r0 + 4 <= n && (reinterpret_cast<uintptr_t>(acc) & 15) == 0;
+    float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (quad) {
+        w = *reinterpret_cast<const float4*>(acc);
+    } else {
+        if (r0 < n) w.x = acc[0];
+        if (r0 + 1 < n) w.y = acc[1];
+        if (r0 + 2 < n) w.z = acc[2];
+        if (r0 + 3 < n) w.w = acc[3];
     }
     __syncthreads();
-    const float* sc = sp.scores + ((int64_t)s * a.n_head + (int64_t)h * G) * sp.score_stride;
-    float* acc = a.acc + ((int64_t)s * a.n_head_kv + h) * a.acc_stride;
-    // four rows a thread, two heads at a time: eight loads under way
-    constexpr int kR = kJoinRows / kJoinThreads;
-    const int end = min(n, j0 + kJoinRows);
-    float w[kR] = {};
-    int j[kR];
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g0 = 0;;) {
 #pragma unroll
-    for (int k = 0; k < kR; ++k) j[k] = min(j0 + (int)threadIdx.x + k * kJoinThreads, end - 1);
-#pragma unroll 2
-    for (int g = 0; g < G; ++g) {
-        float x[kR];
-#pragma unroll
-        for (int k = 0; k < kR; ++k) x[k] = sc[(int64_t)g * sp.score_stride + j[k]];
-#pragma unroll
-        for (int k = 0; k < kR; ++k) w[k] += ex2(x[k] - lse[g]);
+        for (int g = 0; g < kJoinHeads; ++g)
+            if (g0 + g < G) {
+                const float z = lse[g0 + g];
+                sum.x += ex2(x[g].x - z), sum.y += ex2(x[g].y - z);
+                sum.z += ex2(x[g].z - z), sum.w += ex2(x[g].w - z);
+            }
+        // the warp has all it wants of these lines: they need not go to memory
+        __syncwarp();
+        if (lane % 8 == 0 && r0 < sp.score_stride)
+            for (int g = 0; g < kJoinHeads && g0 + g < G; ++g)
+                asm volatile("discard.global.L2 [%0], 128;" ::"l"(sc + (int64_t)(g0 + g) * sp.score_stride) : "memory");
+        g0 += kJoinHeads;
+        if (g0 >= G) break;
+        fetch(g0);
     }
-#pragma unroll
-    for (int k = 0; k < kR; ++k) {
-        const int r = j0 + threadIdx.x + k * kJoinThreads;
-        if (r < end) acc[r] += w[k];
+    w.x += sum.x, w.y += sum.y, w.z += sum.z, w.w += sum.w;
+    if (quad) {
+        *reinterpret_cast<float4*>(acc) = w;
+    } else {
+        if (r0 < n) acc[0] = w.x;
+        if (r0 + 1 < n) acc[1] = w.y;
+        if (r0 + 2 < n) acc[2] = w.z;
+        if (r0 + 3 < n) acc[3] = w.w;
     }
 }
 
@@ -965,6 +1008,8 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
     sp->direct = all_runs <= kCtas && units <= kDirectUnits;
     const int64_t ctas = sp->direct ? all_runs : (total + kMinUnits - 1) / kMinUnits;
     sp->ctas = (int32_t)(ctas < kCtas ? ctas : kCtas);
+    sp->by_run = !sp->direct && all_runs <= sp->ctas;
+    sp->joins = sp->direct ? 0 : sp->by_run ? (int32_t)all_runs : sp->ctas;
     sp->score_stride = (int32_t)(units * kUnit);
     size_t at = 16;
     auto take = [&](size_t bytes) {
@@ -976,14 +1021,17 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
     const int stride = sp->groups * sp->heads;
     if (!sp->direct) {
         sp->run_start = reinterpret_cast<int32_t*>(take(all_runs * sizeof(int32_t)));
-        sp->cut = reinterpret_cast<int4*>(take(sp->ctas * sizeof(int4)));
+        sp->cut = reinterpret_cast<int4*>(take(sp->joins * sizeof(int4)));
         if (n_seq > kLensOnChip) sp->lens = reinterpret_cast<int32_t*>(take(n_seq * sizeof(int32_t)));
         sp->part_ml = reinterpret_cast<float2*>(take((size_t)2 * sp->ctas * stride * sizeof(float2)));
         sp->part_o = reinterpret_cast<float*>(take((size_t)2 * sp->ctas * stride * d * sizeof(float)));
     }
     if (weights) {
         sp->lse = reinterpret_cast<float*>(take((size_t)n_seq * n_head * sizeof(float)));
-        sp->scores = reinterpret_cast<float*>(take((size_t)n_seq * n_head * sp->score_stride * sizeof(float)));
+        // whole 128-byte lines, which k6b_join gives up
+        const uintptr_t sc = reinterpret_cast<uintptr_t>(
+            take((size_t)n_seq * n_head * sp->score_stride * sizeof(float) + 112));
+        sp->scores = reinterpret_cast<float*>((sc + 127) & ~(uintptr_t)127);
     }
     return at;
 }
@@ -1029,7 +1077,7 @@ cudaError_t launch_t(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     if (e != cudaSuccess || (sp.direct && !a.acc)) return e;
     const int chunks = a.acc ? (a.kv.max_kv_len + kJoinRows - 1) / kJoinRows : 0;
     const int heads = std::min(a.n_head / a.n_head_kv, sp.pass_heads);
-    const int64_t grid = (sp.direct ? 0 : sp.ctas * heads) + (int64_t)a.kv.n_seq * a.n_head_kv * chunks;
+    const int64_t grid = (int64_t)sp.joins * heads + (int64_t)a.kv.n_seq * a.n_head_kv * chunks;
     if (grid > INT_MAX) return cudaErrorInvalidValue;
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kJoinThreads);

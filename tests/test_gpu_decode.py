@@ -211,6 +211,32 @@ def test_bad_table_entries_and_lengths_are_reported():
         assert ((out[1].double() - ref[1]).abs() <= tol[1] + rounding(ref[1], BF16)).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shift", [16, 48, 112])
+def test_any_16_byte_workspace_and_4_byte_weights(dtype, shift):
+    """The workspace may start at any multiple of 16 bytes and the weights at any of 4; nothing around either of them
+    changes, and the results are the same."""
+    heads, lens = (20, 2, 64), [2300, 0, 129, 1025]
+    ctx = context(*heads, dtype, dtype, 4096, 64)
+    cache = Cache(lens, heads[1], heads[2], dtype, 0, 5)
+    q = torch.randn(len(lens), heads[0], heads[2], generator=torch.Generator().manual_seed(1)).to(TORCH[dtype]).cuda()
+    n = ctx.decode_bytes(len(lens), cache.cap, True)
+
+    def run(before, first):
+        raw = torch.full((before + n + 256,), 0xAB, dtype=torch.uint8, device="cuda")
+        flat = torch.full((first + len(lens) * heads[1] * cache.cap + 8,), 3.0, device="cuda")
+        acc = flat[first:-8].view(len(lens), heads[1], cache.cap)
+        out = torch.empty_like(q)
+        ctx.check(ctx.decode_layer(0, cache.batch, q, cache.k, cache.v, out, raw[before:before + n], acc=acc))
+        torch.cuda.synchronize()
+        assert (raw[:before] == 0xAB).all() and (raw[before + n:] == 0xAB).all()
+        assert (flat[:first] == 3).all() and (flat[-8:] == 3).all()
+        return out, acc.clone()
+
+    for x, y in zip(run(0, 0), run(shift, shift // 16)):
+        assert torch.equal(x, y)
+
+
 def test_same_result_every_time_and_on_another_stream():
     H, K, d = 32, 8, 128
     cache = Cache([3000, 17, 900, 0, 2222], K, d, BF16, 128, 4)
