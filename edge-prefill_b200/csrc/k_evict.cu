@@ -19,6 +19,8 @@
 // only be done before its own stores.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "epsp_kernels.h"
 
 namespace epsp {
@@ -47,10 +49,12 @@ struct EvictPlan {
     int32_t* list;  // [n_seq][Hkv][cap] kept rows, ascending
     int32_t cap;
     int32_t cluster;
-    int32_t slice;  // rows that a CTA of K8a holds, at most; 0: the slices are too long, read again each time
+    int32_t per;    // rows of a CTA of K8a
+    int32_t slice;  // rows that it can hold; 0: they are too many, read again each time
 };
 
-// Inclusive sum over the CTA's threads.
+// Inclusive sum over the CTA's threads.  `warp_sums` is this call's alone: no
+// barrier comes after its last reading.
 template <int kWarps, class T>
 __device__ __forceinline__ T scan_cta(T x, T* warp_sums, T& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -69,252 +73,249 @@ __device__ __forceinline__ T scan_cta(T x, T* warp_sums, T& total) {
     }
     total = __shfl_sync(0xffffffffu, w, 31);
     const T before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
-    __syncthreads();
     return warp > 0 ? x + before : x;
 }
 
-// Thread t holds the KPT rows r0 + t, r0 + kThreads + t, ... of its CTA's slice
-// (KPT 0: any number of rows, read from memory each time).
+// Address of `p`, a variable in shared memory, in CTA k of the cluster.
+__device__ __forceinline__ uint32_t peer_of(const void* p, int k) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(k));
+    return r;
+}
+
+struct Choice {
+    int digit, above, all;
+};
+
+// Thread t holds the KPT rows from r0 + t KPT on of its CTA's slice (KPT 0:
+// any number of rows, read from memory each time).
 template <int KPT, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a, const EvictPlan p) {
     constexpr int kWarps = kThreads / 32;
-    // counts of up to 32 K rows share a word with their neighbour's: half the
-    // bytes to read from the other CTAs
-    constexpr bool kPairs = KPT > 0;
-    __shared__ __align__(8) int hist[3][kPairs ? kBins / 2 : kBins];
-    constexpr int kRuns = KPT > 0 ? KPT * kWarps : 1024;  // runs of 32 rows placed at a time
-    constexpr int kRunsEach = (kRuns + kThreads - 1) / kThreads;
-    __shared__ uint64_t warp_sums[32], counts[kRunsEach * kThreads], mine;
-    __shared__ int s_len, s_digit, s_above, s_all, warp_counts[32];
+    // counts of the cluster's rows per bin and digit; a cluster's CTAs count in
+    // `own` first and then add the bins that are not empty, mostly few, to the
+    // counts of all
+    __shared__ __align__(16) int bins_of[3][kBins], own[kBins];
+    constexpr int kRuns = KPT > 0 ? 1 : 1024;  // KPT 0: runs of 32 rows placed at a time
+    __shared__ uint64_t run_counts[kRuns], totals[kMaxCluster], run_sums[2][32];
+    __shared__ int digit_sums[3][32];
+    __shared__ uint32_t place_sums[32];
+    __shared__ Choice choice[3];
+    __shared__ int s_len;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = p.cluster, rank = blockIdx.x % C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int h = blockIdx.x / C % a.n_head_kv, s = blockIdx.x / C / a.n_head_kv;
-    for (int i = t; i < (int)(sizeof(hist) / 8); i += kThreads) reinterpret_cast<int2*>(&hist[0][0])[i] = make_int2(0, 0);
+    for (int i = t; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<int4*>(bins_of)[i] = make_int4(0, 0, 0, 0);
+    if (C > 1)
+        for (int i = t; i < kBins / 4; i += kThreads) reinterpret_cast<int4*>(own)[i] = make_int4(0, 0, 0, 0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int64_t sh = (int64_t)s * a.n_head_kv + h;
+    const float* acc = a.acc + sh * a.acc_stride;
+    const int r0 = rank * p.per, mine = r0 + t * KPT;
+    float w[KPT > 0 ? KPT : 1] = {};
+    auto load = [&](int end) {
+        if constexpr (KPT > 0) {
+            const bool quads = (reinterpret_cast<uintptr_t>(acc + r0) & 15) == 0;
+#pragma unroll
+            for (int i = 0; i < KPT; i += 4) {
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (quads && mine + i + 4 <= end) {
+                    x = *reinterpret_cast<const float4*>(acc + mine + i);
+                } else {
+                    if (mine + i < end) x.x = acc[mine + i];
+                    if (mine + i + 1 < end) x.y = acc[mine + i + 1];
+                    if (mine + i + 2 < end) x.z = acc[mine + i + 2];
+                    if (mine + i + 3 < end) x.w = acc[mine + i + 3];
+                }
+                w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+            }
+        }
+    };
     // one reading of the length for the whole cluster: its CTAs must take the
-    // same turns
+    // same turns.  (Weights of rows past it come along where the CTA would have
+    // nothing else to do.)
     int n;
     if (C > 1) {
-        if (rank == 0 && t == 0) s_len = batch_len(a.src, s, a.err);
+        if (t == 0 && rank == 0) s_len = batch_len(a.src, s, a.err);
+        load(min(a.src.max_kv_len, r0 + p.per));
         cluster.sync();
         n = *cluster.map_shared_rank(&s_len, 0);
     } else {
         if (t == 0) s_len = batch_len(a.src, s, a.err);
         __syncthreads();
         n = s_len;
+        load(n);
     }
     const int m = min(n, a.n_keep);
-    const int64_t sh = (int64_t)s * a.n_head_kv + h;
-    const float* acc = a.acc + sh * a.acc_stride;
     if (h == 0 && rank == 0 && t == 0) p.kept[s] = m;
     // rows [r0, r1) are this CTA's; [lo, hi) the candidates, of which `want` stay
-    const int per = ((n + C - 1) / C + 31) & ~31;
-    const int r0 = min(n, rank * per), r1 = min(n, r0 + per);
+    const int r1 = min(n, r0 + p.per);
     const int lo = n > m ? a.sink_rows : n, hi = n > m ? n - a.recent_rows : n;
     const int want = n > m ? m - a.sink_rows - a.recent_rows : 0;
     const bool ranked = want > 0;  // else no candidate stays (or there is none)
 
-    float w[KPT > 0 ? KPT : 1];
+    constexpr bool kKeys = KPT > 0 && KPT <= 8;  // registers for the keys too
+    uint32_t keys[kKeys ? KPT : 1];
+    if constexpr (kKeys) {
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-        const int r = r0 + i * kThreads + t;
-        w[i] = r < r1 ? acc[r] : 0.f;
+        for (int i = 0; i < KPT; ++i) keys[i] = weight_key(w[i]);
     }
-    // f(row, weight) for this thread's rows
-    auto each = [&](auto&& f) {
-        if constexpr (KPT > 0) {
-#pragma unroll
-            for (int i = 0; i < KPT; ++i)
-                if (r0 + i * kThreads + t < r1) f(r0 + i * kThreads + t, w[i]);
-        } else {
-            for (int r = r0 + t; r < r1; r += kThreads) f(r, acc[r]);
-        }
+    auto key_of = [&](int i) {
+        if constexpr (kKeys) return keys[i];
+        else return weight_key(w[i]);
     };
-    __syncthreads();
+    uint32_t cands = 0;  // bit i: this thread's row i is a candidate
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) cands |= (uint32_t)(mine + i >= lo && mine + i < min(r1, hi)) << i;
     uint32_t key = 0;
     int ties = 0, known = 0;  // rows that share the key's bits from `known` on are equal
-    auto sync_all = [&]() {
-        if (C > 1) cluster.sync();
-        else __syncthreads();
-    };
     if (ranked) {  // the same in the whole cluster
         int left = want;
-        const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+        // one digit; true when all of its bin stays
+        auto round = [&](auto digit) {
+            constexpr int d = decltype(digit)::value, shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d < 2 ? 11 : 10;
+            constexpr int bins = 1 << bits;
+            int* hist = C > 1 ? own : bins_of[d];
+            auto add = [&](uint32_t k) {
+                if (d == 0 || (k >> (shift + bits) % 32) == (key >> (shift + bits) % 32))
+                    atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+            };
+            if constexpr (KPT > 0) {
 #pragma unroll
-        for (int d = 0; d < 3; ++d) {
-            const int shift = shifts[d], bins = 1 << bits[d];
-            each([&](int r, float x) {
-                if (r < lo || r >= hi) return;
-                const uint32_t k = weight_key(x);
-                if (d == 0 || (k >> (shift + bits[d])) == (key >> (shift + bits[d]))) {
-                    const int b = (k >> shift) & (bins - 1);
-                    if constexpr (kPairs) atomicAdd(&hist[d][b >> 1], b & 1 ? 65536 : 1);
-                    else atomicAdd(&hist[d][b], 1);
+                for (int i = 0; i < KPT; ++i)
+                    if (cands >> i & 1) add(key_of(i));
+            } else {
+                for (int r = max(r0, lo) + t; r < min(r1, hi); r += kThreads) add(weight_key(acc[r]));
+            }
+            __syncthreads();
+            if (C > 1) {
+                for (int b = t; b < bins; b += kThreads) {
+                    const int c = own[b];
+                    if (c == 0) continue;
+                    own[b] = 0;
+                    for (int k = 0; k < C; ++k)
+                        asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(
+                                         peer_of(&bins_of[d][b], k)),
+                                     "r"(c)
+                                     : "memory");
                 }
-            });
-            sync_all();
-            // thread t has per_t pairs of bins, counted from the top
-            constexpr int kMost = kBins / 2 / kThreads > 0 ? kBins / 2 / kThreads : 1;
-            const int per_t = bins / 2 / kThreads > 0 ? bins / 2 / kThreads : 1;
-            int c0[kMost], c1[kMost], sum = 0;  // upper and lower bin of each pair, over the cluster
+                cluster.sync();
+            }
+            // thread t has kEach bins, counted from the top
+            constexpr int kEach = bins / kThreads > 0 ? bins / kThreads : 1;
+            int c[kEach], sum = 0;
 #pragma unroll
-            for (int q = 0; q < kMost; ++q) {
-                const int b = bins - 1 - 2 * (t * per_t + q);
-                int2 c[kMaxCluster];
-#pragma unroll
-                for (int k = 0; k < kMaxCluster; ++k) {
-                    c[k] = make_int2(0, 0);
-                    if (q >= per_t || b < 0 || k >= C) continue;
-                    const int* other = cluster.map_shared_rank(&hist[d][0], k);
-                    if constexpr (kPairs) c[k].x = other[b >> 1];
-                    else c[k] = *reinterpret_cast<const int2*>(other + b - 1);
-                }
-                c0[q] = c1[q] = 0;
-#pragma unroll
-                for (int k = 0; k < kMaxCluster; ++k) {
-                    c0[q] += kPairs ? (int)((uint32_t)c[k].x >> 16) : c[k].y;
-                    c1[q] += kPairs ? c[k].x & 0xffff : c[k].x;
-                }
-                sum += c0[q] + c1[q];
+            for (int q = 0; q < kEach; ++q) {
+                c[q] = bins_of[d][bins - 1 - (t * kEach + q)];
+                sum += c[q];
             }
             int total;
-            int above = scan_cta<kWarps>(sum, warp_counts, total) - sum;
+            int above = scan_cta<kWarps>(sum, digit_sums[d], total) - sum;
 #pragma unroll
-            for (int q = 0; q < kMost; ++q) {
-                const int b = bins - 1 - 2 * (t * per_t + q), upto = above + c0[q] + c1[q];
-                if (above < left && left <= upto) {
-                    const bool first = left <= above + c0[q];
-                    s_digit = first ? b : b - 1;
-                    s_above = first ? above : above + c0[q];
-                    s_all = (first ? c0[q] : c1[q]) == left - s_above;
-                }
-                above = upto;
+            for (int q = 0; q < kEach; ++q) {
+                if (above < left && left <= above + c[q])
+                    choice[d] = {bins - 1 - (t * kEach + q), above, c[q] == left - above};
+                above += c[q];
             }
             __syncthreads();
-            key |= (uint32_t)s_digit << shift;
-            left -= s_above;
+            key |= (uint32_t)choice[d].digit << shift;
+            left -= choice[d].above;
             known = shift;
-            const bool all = s_all;  // the whole bin stays: no need to look into it
-            __syncthreads();
-            if (all) break;
-        }
+            return choice[d].all != 0;  // the whole bin stays: no need to look into it
+        };
+        if (!round(std::integral_constant<int, 0>()) && !round(std::integral_constant<int, 1>()))
+            round(std::integral_constant<int, 2>());
         ties = left;  // rows equal to `key` that stay, the first ones
     }
     // a row stays whatever comes before it, or it equals `key`
     const uint32_t edge = key >> known;
-    auto mark = [&](int r, float x, bool& hard, bool& eq) {
-        const bool cand = r >= lo && r < hi;
-        const uint32_t k = weight_key(x) >> known;
-        hard = r < r1 && (!cand || (ranked && k > edge));
-        eq = r < r1 && cand && ranked && k == edge;
-    };
     int32_t* list = p.list + sh * p.cap;
     int32_t* kept_rows = a.kept_rows ? a.kept_rows + sh * a.n_keep : nullptr;
     float* acc_dst = a.acc_dst && (KPT > 0 || a.acc_dst != a.acc) ? a.acc_dst + sh * a.acc_dst_stride : nullptr;
-    auto place = [&](int r, float x, bool hard, bool eq, uint64_t before) {
-        const uint32_t all_hard = __ballot_sync(0xffffffffu, hard), all_eq = __ballot_sync(0xffffffffu, eq);
-        const uint32_t below = (1u << lane) - 1;
-        const int n_hard = (int)(before >> 32) + __popc(all_hard & below);
-        const int n_eq = (int)(uint32_t)before + __popc(all_eq & below);
-        if (hard || (eq && n_eq < ties)) {
-            const int at = n_hard + min(n_eq, ties);
-            list[at] = r;
-            if (kept_rows) kept_rows[at] = r;
-            if (acc_dst) acc_dst[at] = x;
-        }
+    auto put = [&](int at, int r, float x) {
+        list[at] = r;
+        if (kept_rows) kept_rows[at] = r;
+        if (acc_dst) acc_dst[at] = x;
     };
-    // rows of a warp's 32 that stay in any case (upper half) and that equal `key`
-    auto count = [](bool hard, bool eq) {
-        const int n_hard = __popc(__ballot_sync(0xffffffffu, hard)), n_eq = __popc(__ballot_sync(0xffffffffu, eq));
-        return ((uint64_t)n_hard << 32) | (uint32_t)n_eq;
-    };
-    // the counts of the CTAs before this one
+    // the counts of the CTAs before this one (the last that CTAs have of one
+    // another: they may leave when they like)
     auto base_of = [&](uint64_t total) {
-        if (t == 0) mine = total;
-        sync_all();
-        uint64_t v[kMaxCluster], base = 0;
-#pragma unroll
-        for (int k = 0; k < kMaxCluster; ++k) v[k] = k < rank ? *cluster.map_shared_rank(&mine, k) : 0;
-#pragma unroll
-        for (int k = 0; k < kMaxCluster; ++k) base += v[k];
+        uint64_t base = 0;
+        if (C > 1) {
+            if (t < C)
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_of(&totals[rank], t)), "l"(total) : "memory");
+            cluster.sync();
+            for (int k = 0; k < rank; ++k) base += totals[k];
+        }
         return base;
     };
-    uint64_t total;
     if constexpr (KPT > 0) {
-        // rows in order are runs of 32, run i * 32 + warp
-        static_assert(KPT <= 32, "a bit per row");
-        uint32_t hards = 0, eqs = 0;  // bit i: this thread's row i
+        static_assert(KPT <= 32 && KPT * kThreads < 65536, "a bit per row, 16 bits per count");
+        uint32_t hards = 0, eqs = 0;
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) hards |= (uint32_t)(mine + i < r1) << i;
+        hards &= ~cands;
+        if (ranked) {
+#pragma unroll
+            for (int i = 0; i < KPT; ++i) {
+                const uint32_t k = key_of(i) >> known;
+                hards |= (cands >> i & 1 & (uint32_t)(k > edge)) << i;
+                eqs |= (cands >> i & 1 & (uint32_t)(k == edge)) << i;
+            }
+        }
+        const uint32_t sum = (uint32_t)__popc(hards) << 16 | (uint32_t)__popc(eqs);
+        uint32_t total;
+        const uint32_t before = scan_cta<kWarps>(sum, place_sums, total) - sum;
+        const uint64_t base = base_of((uint64_t)(total >> 16) << 32 | (total & 0xffff));
+        int n_hard = (int)(base >> 32) + (int)(before >> 16), n_eq = (int)(uint32_t)base + (int)(before & 0xffff);
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
-            bool hard, eq;
-            mark(r0 + i * kThreads + t, w[i], hard, eq);
-            hards |= (uint32_t)hard << i;
-            eqs |= (uint32_t)eq << i;
-            const uint64_t c = count(hard, eq);
-            if (lane == 0) counts[i * kWarps + warp] = c;
-        }
-        __syncthreads();
-        uint64_t own[kRunsEach], sum = 0;
-#pragma unroll
-        for (int e = 0; e < kRunsEach; ++e) {
-            own[e] = t * kRunsEach + e < kRuns ? counts[t * kRunsEach + e] : 0;
-            sum += own[e];
-        }
-        uint64_t before = scan_cta<kWarps>(sum, warp_sums, total) - sum;
-        before += base_of(total);
-#pragma unroll
-        for (int e = 0; e < kRunsEach; ++e) {
-            counts[t * kRunsEach + e] = before;
-            before += own[e];
-        }
-        cluster.barrier_arrive();  // `mine` of the others has been read
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < KPT; ++i) {
-            const int r = r0 + i * kThreads + t;
-            place(r, w[i], hards >> i & 1, eqs >> i & 1, counts[i * kWarps + warp]);
+            const bool hard = hards >> i & 1, eq = eqs >> i & 1;
+            if (hard || (eq && n_eq < ties)) put(n_hard + min(n_eq, ties), mine + i, w[i]);
+            n_hard += hard;
+            n_eq += eq;
         }
     } else {
-        uint64_t sum = 0;
-        each([&](int r, float x) {
+        auto mark = [&](int r, float x, bool& hard, bool& eq) {
+            const bool cand = r >= lo && r < hi;
+            const uint32_t k = weight_key(x) >> known;
+            hard = r < r1 && (!cand || (ranked && k > edge));
+            eq = r < r1 && cand && ranked && k == edge;
+        };
+        uint64_t sum = 0, total;
+        for (int r = r0 + t; r < r1; r += kThreads) {
             bool hard, eq;
-            mark(r, x, hard, eq);
+            mark(r, acc[r], hard, eq);
             sum += ((uint64_t)hard << 32) | (uint32_t)eq;
-        });
-        scan_cta<kWarps>(sum, warp_sums, total);
+        }
+        scan_cta<kWarps>(sum, run_sums[0], total);
         uint64_t base = base_of(total);
-        cluster.barrier_arrive();
+        static_assert(kRuns <= kThreads || KPT > 0, "a run per thread");
         for (int c0 = r0; c0 < r1; c0 += kRuns * 32) {
             const int runs = min(kRuns, (r1 - c0 + 31) / 32);
-            auto weight = [&](int r) { return r < r1 ? acc[r] : 0.f; };
             for (int g = warp; g < runs; g += kWarps) {
                 const int r = c0 + g * 32 + lane;
                 bool hard, eq;
-                mark(r, weight(r), hard, eq);
-                const uint64_t c = count(hard, eq);
-                if (lane == 0) counts[g] = c;
+                mark(r, r < r1 ? acc[r] : 0.f, hard, eq);
+                const uint32_t all_hard = __ballot_sync(0xffffffffu, hard), all_eq = __ballot_sync(0xffffffffu, eq);
+                if (lane == 0) run_counts[g] = (uint64_t)__popc(all_hard) << 32 | (uint32_t)__popc(all_eq);
             }
             __syncthreads();
-            uint64_t own[kRunsEach], sum = 0;
-#pragma unroll
-            for (int e = 0; e < kRunsEach; ++e) {
-                own[e] = t * kRunsEach + e < runs ? counts[t * kRunsEach + e] : 0;
-                sum += own[e];
-            }
-            uint64_t before = base + scan_cta<kWarps>(sum, warp_sums, total) - sum;
-#pragma unroll
-            for (int e = 0; e < kRunsEach; ++e) {
-                counts[t * kRunsEach + e] = before;
-                before += own[e];
-            }
+            const uint64_t mine_sum = t < runs ? run_counts[t] : 0;
+            const uint64_t before = base + scan_cta<kWarps>(mine_sum, run_sums[1], total) - mine_sum;
+            if (t < runs) run_counts[t] = before;
             __syncthreads();
             for (int g = warp; g < runs; g += kWarps) {
                 const int r = c0 + g * 32 + lane;
-                const float x = weight(r);
+                const float x = r < r1 ? acc[r] : 0.f;
                 bool hard, eq;
                 mark(r, x, hard, eq);
-                place(r, x, hard, eq, counts[g]);
+                const uint32_t all_hard = __ballot_sync(0xffffffffu, hard), all_eq = __ballot_sync(0xffffffffu, eq);
+                const uint32_t below = (1u << lane) - 1;
+                const int n_hard = (int)(run_counts[g] >> 32) + __popc(all_hard & below);
+                const int n_eq = (int)(uint32_t)run_counts[g] + __popc(all_eq & below);
+                if (hard || (eq && n_eq < ties)) put(n_hard + min(n_eq, ties), r, x);
             }
             base += total;
             __syncthreads();
@@ -324,7 +325,6 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
         for (int i = m + rank * kThreads + t; i < a.n_keep; i += C * kThreads) kept_rows[i] = -1;
     if (acc_dst)
         for (int i = m + rank * kThreads + t; i < a.acc_dst_stride; i += C * kThreads) acc_dst[i] = 0.f;
-    cluster.barrier_wait();  // no CTA leaves while another reads its counts
 }
 
 constexpr int kMoveThreads = 256;
@@ -445,7 +445,7 @@ size_t plan_of(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t n_head
     while (p->cluster < kMaxCluster &&
            (slice(p->cluster) > kSliceM || (slice(p->cluster) > kSliceS && runs * p->cluster * 2 <= kSms)))
         p->cluster *= 2;
-    const int each = slice(p->cluster);
+    const int each = p->per = slice(p->cluster);
     p->slice = each <= kSliceS ? kSliceS : each <= kSliceM ? kSliceM : each <= kSliceL ? kSliceL : 0;
     p->kept = reinterpret_cast<int32_t*>(ws);
     const size_t head = up16((size_t)n_seq * sizeof(int32_t));
