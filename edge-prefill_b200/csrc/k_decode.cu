@@ -12,7 +12,8 @@
 // lengths), so ragged batches and one long sequence load the SMs alike.  A run
 // inside one CTA is finished there; one that several CTAs share leaves its
 // running (maximum, sum, output) in the workspace, two slots per CTA, and
-// k6b_join puts them together in a fixed order.
+// k6b_join puts them together in a fixed order.  Calls of few short runs give
+// each a cluster of CTAs, which join in shared memory: one launch.
 //
 // CTA: one warp streams K and V units into a ring by TMA (128-byte swizzled
 // rows); units go round robin to the streams of the 8 other warps (4 for f32 rows of 512 bytes), each warp with its
@@ -60,13 +61,24 @@ constexpr int kMinUnits = 4;  // fewest units dealt to a CTA
 constexpr int kRunCost = 6;
 constexpr int kLensOnChip = 1024;  // lengths a CTA keeps in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
-// A call of at most this many units per run and one CTA per run skips the
-// split (and the join).
+// Calls that skip the split and the join: one CTA per run of at most
+// kDirectUnits units, or a cluster of up to 8 CTAs per run, joined in shared
+// memory, with kClusterUnits units for each CTA (twice as many where the
+// cluster may not grow, but for weights, which then pay: 1500 rows, 12 us
+// against 10 by the split).  1000 rows, 14 heads: 8 us against 10 by the
+// split, f32 11.5 against 14.3, with weights 10 against 12.
 constexpr int kDirectUnits = 16;
+constexpr int kMaxCluster = 8;
+constexpr int kClusterUnits = 4;
+// CTAs of all clusters together: 14 clusters of 8 run at once (8 us), 16 do
+// not (12 us).
+constexpr int kClusterCtas = 112;
 
 struct DecodeSplit {
     int32_t ctas;      // grid
-    int32_t direct;    // one CTA per run
+    int32_t direct;    // a cluster per run, of
+    int32_t cluster;   // so many CTAs
+    int32_t fused;     // direct, and the weights are added by the same CTAs
     int32_t by_run;    // cut has a place per run (no more runs than CTAs), not one per CTA
     int32_t joins;     // places of cut
     int32_t pass_heads;  // query heads of a pass, at most
@@ -304,6 +316,82 @@ __device__ __forceinline__ void patch_unit(unsigned char* stage, int lane, int l
     __syncwarp();
 }
 
+// Joins what the CTAs of a cluster (or this one alone) have of a run: outputs
+// [head][D], then (maximum, sum) [head], at the start of each one's shared
+// memory; and adds the weights of this CTA's rows.  `lse_s`: [heads] of scratch.
+template <int D, int kThreads, int kPass>
+__device__ __forceinline__ void join_cluster(const DecodeArgs& a, const DecodeSplit& sp, const unsigned char* smem,
+                                             float* lse_s, const Walk& w, int n_seg, int64_t q_row, int n_heads, int h,
+                                             int rank) {
+    const int C = sp.cluster, lane = threadIdx.x & 31;
+    if (C > 1) tc::cluster_sync();
+    else tc::named_bar_sync(1, kThreads);
+    // weight of each CTA's part of head g, and log2 of the sum over all
+    auto weigh = [&](int g, float (&f)[kMaxCluster]) {
+        float2 v[kMaxCluster];
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k)
+            if (k < C) {
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                             : "=f"(v[k].x), "=f"(v[k].y)
+                             : "r"(tc::peer_of(smem + kPass * D * 4 + g * 8, k))
+                             : "memory");
+            } else {
+                v[k] = make_float2(0.f, 0.f);
+            }
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k)
+            if (v[k].y != 0.f) m = fmaxf(m, v[k].x);
+        const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) {
+            f[k] = v[k].y != 0.f ? ex2(v[k].x - ms) : 0.f;  // 0: nothing but -inf there, its sums may be anything
+            l += v[k].y * f[k];
+        }
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) f[k] *= inv;
+        return ms + log2f(l);
+    };
+    float f[kMaxCluster];
+    for (int j = rank * kThreads + threadIdx.x; j < n_heads * (D / 4); j += C * kThreads) {
+        const int g = j / (D / 4), c = j % (D / 4);
+        float4 t[kMaxCluster];
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k)
+            if (k < C)
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(t[k].x), "=f"(t[k].y), "=f"(t[k].z), "=f"(t[k].w)
+                             : "r"(tc::peer_of(smem + (g * D + c * 4) * 4, k))
+                             : "memory");
+        const float lse = weigh(g, f);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (w.n > 0) {
+#pragma unroll
+            for (int k = 0; k < kMaxCluster; ++k)
+                if (k < C && f[k] != 0.f) o.x += f[k] * t[k].x, o.y += f[k] * t[k].y, o.z += f[k] * t[k].z, o.w += f[k] * t[k].w;
+        }
+        store4(a.out, a.out_dtype, (q_row + g) * D + c * 4, o);
+        if (c == 0 && a.acc != nullptr && !sp.fused) sp.lse[q_row + g] = lse;
+    }
+    if (!sp.fused) return;
+    for (int g = threadIdx.x; g < n_heads; g += kThreads) lse_s[g] = weigh(g, f);
+    tc::named_bar_sync(1, kThreads);
+    float* acc = a.acc + ((int64_t)w.s * a.n_head_kv + h) * a.acc_stride;
+    for (int r = w.u * kUnit + threadIdx.x; r < (w.u + n_seg) * kUnit; r += kThreads) {
+        const float* sc = sp.scores + q_row * sp.score_stride + r;
+        const float was = r < w.n ? acc[r] : 0.f;
+        float sum = 0.f;
+#pragma unroll 8
+        for (int g = 0; g < n_heads; ++g) sum += ex2(sc[(int64_t)g * sp.score_stride] - lse_s[g]);
+        if (r < w.n) acc[r] = was + sum;
+        __syncwarp();
+        for (int g = lane; g < n_heads; g += 32)
+            asm volatile("discard.global.L2 [%0], 128;" ::"l"(sc - lane + (int64_t)g * sp.score_stride) : "memory");
+    }
+}
+
 template <int ET, int D, int W, bool P3, int GH>
 __global__ void __launch_bounds__((W + 1) * 32, 1)
     k6a_decode(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
@@ -342,15 +430,18 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
     // ----------------------------------------- this CTA's range of the units
     Walk w0;
     Lens lens{nullptr};
+    const int C = sp.cluster, rank = blockIdx.x & (C - 1);
     if (sp.direct) {
-        w0.s = blockIdx.x / runs;
-        w0.run = blockIdx.x % runs;
-        w0.u = 0;
+        const int id = blockIdx.x >> (__ffs(C) - 1);
+        w0.s = id / runs;
+        w0.run = id % runs;
         if (threadIdx.x == 0) lens_s[0] = batch_len(a.kv, w0.s, a.err);
         __syncthreads();
         w0.n = lens_s[0];
         w0.units = units_of(w0.n);
-        w0.left = w0.units;
+        const int per = (w0.units + C - 1) >> (__ffs(C) - 1);
+        w0.u = min(rank * per, w0.units);
+        w0.left = min(per, w0.units - w0.u);
     } else {
         if (a.kv.n_seq <= kLensOnChip) {
             for (int s = threadIdx.x; s < a.kv.n_seq; s += kThreads) lens_s[s] = batch_len(a.kv, s, a.err);
@@ -368,7 +459,8 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
             }
         if (w0.left <= 0 && !sp.by_run && threadIdx.x == 0) sp.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
-    if (w0.left <= 0) {
+    // (a cluster's CTAs meet whatever their lengths)
+    if (w0.left <= 0 && C == 1) {
         if (sp.direct) {  // a sequence without rows
             const int g0 = (w0.run % sp.passes) * kPass, n = min(kPass, G - g0) * (D / 4);
             const int64_t at = ((int64_t)w0.s * a.n_head + (w0.run / sp.passes) * G + g0) * D;
@@ -387,7 +479,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
         bool ok = true;
         int seg = 0;
         const uint64_t policy = tc::policy_evict_first();  // the cache is read once
-        for (; w.left > 0 && ok; ++seg) {
+        for (; (w.left > 0 || (C > 1 && seg == 0)) && ok; ++seg) {
             const int n_seg = w.segment();
             const int h = w.run / sp.passes, pass = w.run % sp.passes;
             if (lane == 0) {
@@ -455,7 +547,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
     Walk w = w0;
     int it = 0;
     bool ok = true;
-    for (int seg = 0; w.left > 0; ++seg) {
+    for (int seg = 0; w.left > 0 || (C > 1 && seg == 0); ++seg) {
         const int n_seg = w.segment();
         const int h = w.run / sp.passes, pass = w.run % sp.passes;
         const int g0 = pass * kPass + grp * kHeads;  // this warp's first query head of the group
@@ -741,7 +833,11 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                     lt += v[r].y * ex2(v[r].x - ms);
                     ot.x += t[r].x, ot.y += t[r].y, ot.z += t[r].z, ot.w += t[r].w;
                 }
-            if (whole) {
+            if (C > 1 || sp.fused) {
+                // (the ring: this CTA's last copy has landed)
+                *reinterpret_cast<float4*>(smem + (g * D + c * 4) * 4) = ot;
+                if (c == 0) *reinterpret_cast<float2*>(smem + kPass * D * 4 + g * 8) = make_float2(ms, lt);
+            } else if (whole) {
                 const float inv = 1.f / lt;
                 store4(a.out, a.out_dtype, (q_row + pass * kPass + g) * D + c * 4,
                        make_float4(ot.x * inv, ot.y * inv, ot.z * inv, ot.w * inv));
@@ -751,6 +847,10 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                 *reinterpret_cast<float4*>(sp.part_o + p * D + c * 4) = ot;
                 if (c == 0) sp.part_ml[p] = make_float2(ms, lt);
             }
+        }
+        if (C > 1 || sp.fused) {
+            join_cluster<D, kWarps * 32, kPass>(a, sp, smem, om, w, n_seg, q_row + pass * kPass, n_heads, h, rank);
+            if (C > 1) tc::cluster_sync();  // nobody reads this CTA's part any more
         }
         if (!sp.direct && threadIdx.x == 0) {
             if (w.u == 0) sp.run_start[(int64_t)w.s * runs + w.run] = w.at;
@@ -1005,8 +1105,16 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
     const int64_t all_runs = (int64_t)n_seq * n_head_kv * sp->passes;
     const int64_t units = units_of(max_kv_len), total = all_runs * (units + kRunCost);
     if (total > INT_MAX) return SIZE_MAX;
+    sp->cluster = 1;
     sp->direct = all_runs <= kCtas && units <= kDirectUnits;
-    const int64_t ctas = sp->direct ? all_runs : (total + kMinUnits - 1) / kMinUnits;
+    if (!sp->direct) {
+        while (sp->cluster < kMaxCluster && units > sp->cluster * kClusterUnits && all_runs * sp->cluster * 2 <= kClusterCtas)
+            sp->cluster *= 2;
+        sp->direct = sp->cluster > 1 && units <= sp->cluster * (weights ? 1 : 2) * kClusterUnits;
+        if (!sp->direct) sp->cluster = 1;
+    }
+    sp->fused = sp->direct && weights && sp->passes == 1;  // (several passes would add to the same rows)
+    const int64_t ctas = sp->direct ? all_runs * sp->cluster : (total + kMinUnits - 1) / kMinUnits;
     sp->ctas = (int32_t)(ctas < kCtas ? ctas : kCtas);
     sp->by_run = !sp->direct && all_runs <= sp->ctas;
     sp->joins = sp->direct ? 0 : sp->by_run ? (int32_t)all_runs : sp->ctas;
@@ -1027,7 +1135,7 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
         sp->part_o = reinterpret_cast<float*>(take((size_t)2 * sp->ctas * stride * d * sizeof(float)));
     }
     if (weights) {
-        sp->lse = reinterpret_cast<float*>(take((size_t)n_seq * n_head * sizeof(float)));
+        if (!sp->fused) sp->lse = reinterpret_cast<float*>(take((size_t)n_seq * n_head * sizeof(float)));
         // whole 128-byte lines, which k6b_join gives up
         const uintptr_t sc = reinterpret_cast<uintptr_t>(
             take((size_t)n_seq * n_head * sp->score_stride * sizeof(float) + 112));
@@ -1056,11 +1164,14 @@ cudaError_t launch_t(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     }
     // both kernels may start before what precedes them on the stream has
     // ended: they wait for it on the device
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = sp.cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.attrs = &at;
+    cfg.attrs = at;
     cfg.numAttrs = 1;
     cfg.stream = s;
     if (sp.lens) {
@@ -1073,8 +1184,9 @@ cudaError_t launch_t(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     cfg.gridDim = dim3(sp.ctas);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
+    cfg.numAttrs = sp.cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, k6a_decode<ET, D, W, P3, GH>, mk, mv, a, sp);
-    if (e != cudaSuccess || (sp.direct && !a.acc)) return e;
+    if (e != cudaSuccess || (sp.direct && (!a.acc || sp.fused))) return e;
     const int chunks = a.acc ? (a.kv.max_kv_len + kJoinRows - 1) / kJoinRows : 0;
     const int heads = std::min(a.n_head / a.n_head_kv, sp.pass_heads);
     const int64_t grid = (int64_t)sp.joins * heads + (int64_t)a.kv.n_seq * a.n_head_kv * chunks;
@@ -1082,6 +1194,7 @@ cudaError_t launch_t(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, k6b_join<D>, a, sp, heads, chunks);
 }
 

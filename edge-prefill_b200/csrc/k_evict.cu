@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "epsp_kernels.h"
+#include "tc100.cuh"
 
 namespace epsp {
 namespace {
@@ -74,13 +75,6 @@ __device__ __forceinline__ T scan_cta(T x, T* warp_sums, T& total) {
     total = __shfl_sync(0xffffffffu, w, 31);
     const T before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
     return warp > 0 ? x + before : x;
-}
-
-// Address of `p`, a variable in shared memory, in CTA k of the cluster.
-__device__ __forceinline__ uint32_t peer_of(const void* p, int k) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(k));
-    return r;
 }
 
 struct Choice {
@@ -196,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
                     own[b] = 0;
                     for (int k = 0; k < C; ++k)
                         asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(
-                                         peer_of(&bins_of[d][b], k)),
+                                         tc::peer_of(&bins_of[d][b], k)),
                                      "r"(c)
                                      : "memory");
                 }
@@ -244,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
         uint64_t base = 0;
         if (C > 1) {
             if (t < C)
-                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_of(&totals[rank], t)), "l"(total) : "memory");
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(tc::peer_of(&totals[rank], t)), "l"(total) : "memory");
             cluster.sync();
             for (int k = 0; k < rank; ++k) base += totals[k];
         }

@@ -91,6 +91,18 @@ __device__ __forceinline__ uint64_t policy_evict_last() {
     return p;
 }
 
+// Address of `p`, a variable in shared memory, in CTA k of the cluster.
+__device__ __forceinline__ uint32_t peer_of(const void* p, int k) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(k));
+    return r;
+}
+// Waits for every thread of the cluster that has not ended, and for what it
+// wrote to shared memory.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // `bytes` contiguous bytes (both addresses and the size multiples of 16) into
 // this CTA's shared memory, completing on `bar`.
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {

@@ -90,6 +90,17 @@ def test_few_rows_without_a_split(heads, dtype, out):
     run_case([33], heads, dtype, out, 32, 0, False, True, seed=heads[0])
 
 
+@pytest.mark.parametrize("weights", [False, True], ids=["plain", "weights"])
+@pytest.mark.parametrize("dtype,heads,out", [
+    (BF16, (8, 2, 128), BF16), (F16, (14, 2, 64), F16), (BF16, (28, 2, 64), F32), (F32, (7, 1, 64), F32),
+    (F32, (4, 2, 128), F32), (BF16, (128, 1, 128), BF16), (F32, (40, 1, 64), F32)], ids=str)
+@pytest.mark.parametrize("lens", [[513], [900, 0, 1, 33], [1024, 40, 0], [1500, 1], [2048, 1025, 31]], ids=str)
+def test_short_runs_joined_in_a_cluster(lens, dtype, heads, out, weights):
+    """Few runs of up to 2048 rows: a cluster of 2 to 8 CTAs each, some of them without rows."""
+    run_case(lens, heads, dtype, out, 32, 32, True, weights, seed=lens[0])
+    run_case(lens, heads, dtype, out, 32, 0, False, weights, seed=lens[0], extra_stride=3)
+
+
 def test_empty_batch_and_capacity_above_the_lengths():
     run_case([0, 0, 0], (32, 8, 128), BF16, BF16, 128, 128, True, True, cap=5000)
     run_case([3, 0, 70], (32, 8, 128), BF16, BF16, 128, 128, True, True, cap=5000, extra_stride=13)
