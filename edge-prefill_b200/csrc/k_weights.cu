@@ -16,7 +16,9 @@
 // reductions stay in the thread's registers, no shuffles.  One warp loads
 // tiles by TMA, one issues MMAs into 3 S buffers in TMEM, and 24 warps take
 // the exponentials.
-// f32: the same passes on the CUDA cores, 64 x 64 tiles, 4 x 4 per thread.
+// f32: the same passes on the CUDA cores, 64 x 64 tiles, 4 x 4 per thread; few
+// scores are kept by the first pass instead, and the second only adds up their
+// exponentials.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -681,7 +683,15 @@ struct F32Plan {
     float* part;     // [r_splits][Hkv][n_kt * 64] (r_splits > 1)
     float2* ml;      // [splits][Hkv][n_rt * 64]
     float* nlse;     // [Hkv][n_rt * 64]: minus the lse, -inf for rows that are none
+    float* scores;   // [Hkv][n_rt * 64][n_kt * 64] log2 units, of the tiles with a visible key (null: not kept)
 };
+
+// Scores that fit L2 next to everything else are written and read once instead
+// of being computed twice, and given up there once read: 2 launches, not 3 or 4.
+// (14 heads of 64, 32 rows over 4096 keys: 25 us against 30; 32 heads of 128,
+// 128 rows, 64 MB of scores: 165 against 287.)
+constexpr int64_t kKeptScores = 16 << 20;
+constexpr int kKeptCtas = 4 * kSms;  // of the second pass, at once
 
 // 64 rows of D floats on their way into shared memory: fetch has all of a
 // thread's loads under way at once, store follows when the buffer is free.
@@ -691,22 +701,20 @@ template <int D>
 struct RowsF32 {
     static constexpr int kN = FT * (D / 4) / kF32Threads;
     float4 v[kN];
-    // src(r): the row's address, null for zeros
+    // src(r): the row's address, null for zeros; four threads to a row
     template <class F>
     __device__ __forceinline__ void fetch(F&& src) {
+        static_assert(kF32Threads == 4 * FT, "four threads to a row");
+        const float* p = src(threadIdx.x / 4);
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
-            const int i = threadIdx.x + n * kF32Threads;
-            const float* p = src(i / (D / 4));
-            v[n] = p != nullptr ? *reinterpret_cast<const float4*>(p + i % (D / 4) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+        for (int n = 0; n < kN; ++n)
+            v[n] = p != nullptr ? *reinterpret_cast<const float4*>(p + threadIdx.x % 4 * 4 + n * 16)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __device__ __forceinline__ void store(float* dst) const {
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
-            const int i = threadIdx.x + n * kF32Threads;
-            *reinterpret_cast<float4*>(dst + i / (D / 4) * (D + 4) + i % (D / 4) * 4) = v[n];
-        }
+        for (int n = 0; n < kN; ++n)
+            *reinterpret_cast<float4*>(dst + threadIdx.x / 4 * (D + 4) + threadIdx.x % 4 * 4 + n * 16) = v[n];
     }
     __device__ __forceinline__ void fetch_queries(const WeightArgs& a, int n_rows, int rt, int h) {
         const int G = a.n_head / a.n_head_kv;
@@ -782,6 +790,9 @@ __global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, 
         l[i] = 0.f;
     }
     const bool few = p.n_rows - rt * FT <= 16;  // a small window: the rows past it cost nothing
+    const uint64_t keep = tc::policy_evict_last();
+    const int64_t wide = (int64_t)p.n_kt * FT;
+    float* scores = p.scores + (((int64_t)h * p.n_rt + rt) * FT + ty) * wide + tx;
     RowsF32<D> next;
     {
         RowsF32<D> rows;
@@ -805,6 +816,14 @@ __global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, 
                 for (int j = 0; j < 4; ++j) {
                     x[i][j] = kt * FT + tx + 16 * j <= tok[i] ? x[i][j] * sl2 : -INFINITY;
                     mx = fmaxf(mx, x[i][j]);
+                }
+                if (p.scores != nullptr) {
+                    const float* to = scores + 16 * i * wide + kt * FT;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        asm volatile("st.global.L2::cache_hint.f32 [%0], %1, %2;" ::"l"(to + 16 * j), "f"(x[i][j]),
+                                     "l"(keep)
+                                     : "memory");
                 }
                 const float ms = mx == -INFINITY ? 0.f : mx;
                 l[i] *= ex2(m[i] - ms);
@@ -897,6 +916,103 @@ __global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, c
     }
 }
 
+// Sums pass over kept scores: a cluster of CTAs per 64 keys of a head, which
+// share its rows (3500 rows over 8 tiles of 2 heads: one CTA each 57 us, 8 each
+// 33).  The rows' sums are put together from the splits' by every cluster (L2
+// holds them), a thread to a row and a part of the splits.
+constexpr int kKeptThreads = 256;
+constexpr int kKeptRows = 1024;  // rows whose sums a CTA holds
+__global__ void __launch_bounds__(kKeptThreads) k7_kept_f32(const WeightArgs a, const F32Plan p) {
+    __shared__ float nlse[kKeptRows];
+    __shared__ float4 part[kKeptThreads];
+    __shared__ float2 halves[kKeptThreads];
+    __shared__ float sums[FT];
+    tc::pdl_wait();
+    tc::pdl_launch();
+    const int C = p.r_splits, rank = blockIdx.x % C, kt = blockIdx.x / C % p.n_kt, h = blockIdx.x / C / p.n_kt;
+    const int G = a.n_head / a.n_head_kv, t_first = a.kv_len - a.n_tok + a.row_begin;
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int64_t rows = (int64_t)p.n_rt * FT, stride = rows * a.n_head_kv, wide = (int64_t)p.n_kt * FT;
+    const float* scores = p.scores + h * rows * wide + kt * FT + 4 * tx;
+    const float2* ml = p.ml + h * rows;
+    // from the first row that sees a key of the tile
+    const int first = (int)max((int64_t)0, (int64_t)(kt * FT - t_first) * G), n_rows = max(0, p.n_rows - first);
+    const int b1 = first + (int)((int64_t)n_rows * (rank + 1) / C);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int b = first + (int)((int64_t)n_rows * rank / C); b < b1; b += kKeptRows) {
+        const int n = min(kKeptRows, b1 - b);
+        for (int r0 = 0; r0 < n; r0 += kKeptThreads) {
+            const int here = min(n - r0, kKeptThreads), lanes = (here + 31) & ~31, parts = kKeptThreads / lanes;
+            const int r = threadIdx.x % lanes, part_of = threadIdx.x / lanes;
+            float m = -INFINITY, l = 0.f;
+            if (r < here && part_of < parts) {
+                constexpr int kAtOnce = 8;
+                for (int s = part_of; s < p.splits; s += parts * kAtOnce) {
+                    float2 v[kAtOnce];
+                    float mx = m;
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i)
+                        v[i] = s + i * parts < p.splits ? ml[(s + i * parts) * stride + b + r0 + r]
+                                                        : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) mx = fmaxf(mx, v[i].x);
+                    const float ms = mx == -INFINITY ? 0.f : mx;
+                    l *= ex2(m - ms);
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) l += v[i].y * ex2(v[i].x - ms);
+                    m = mx;
+                }
+            }
+            halves[threadIdx.x] = make_float2(m, l);
+            __syncthreads();
+            if (part_of == 0 && r < here) {
+                for (int i = 1; i < parts; ++i) {
+                    const float2 u = halves[i * lanes + r];
+                    const float mx = fmaxf(m, u.x), ms = mx == -INFINITY ? 0.f : mx;
+                    l = l * ex2(m - ms) + u.y * ex2(u.x - ms);
+                    m = mx;
+                }
+                nlse[r0 + r] = -(m + log2f(l));
+            }
+            __syncthreads();
+        }
+#pragma unroll 8
+        for (int r = ty; r < n; r += kKeptThreads / 16) {
+            const float4 x = *reinterpret_cast<const float4*>(scores + (b + r) * wide);
+            const float ls = nlse[r];
+            sum.x += ex2(x.x + ls), sum.y += ex2(x.y + ls), sum.z += ex2(x.z + ls), sum.w += ex2(x.w + ls);
+        }
+        __syncthreads();
+        if (tx % 8 == 0)
+            for (int r = ty; r < n; r += kKeptThreads / 16)
+                asm volatile("discard.global.L2 [%0], 128;" ::"l"(scores + (b + r) * wide) : "memory");
+    }
+    part[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x < FT) {
+        const float* of = reinterpret_cast<const float*>(part) + threadIdx.x;
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < kKeptThreads / 16; ++i) v += of[i * FT];
+        sums[threadIdx.x] = v;
+    }
+    if (C > 1) tc::cluster_sync();
+    if (rank == 0 && threadIdx.x < FT && kt * FT + (int)threadIdx.x < a.kv_len) {
+        float v = sums[threadIdx.x];
+        for (int k = 1; k < C; ++k) {
+            float u;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                         : "=f"(u)
+                         : "r"(tc::peer_of(&sums[threadIdx.x], k))
+                         : "memory");
+            v += u;
+        }
+        float* out = a.acc + (int64_t)h * a.acc_stride + kt * FT + threadIdx.x;
+        *out = a.accumulate ? *out + v : v;
+    }
+    if (C > 1) tc::cluster_sync();  // nobody reads this CTA's sums any more
+}
+
 // ---------------------------------------------------------------- host side --
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
@@ -913,6 +1029,14 @@ size_t plan_f32(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv,
     p->splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_kt, 2 * kSms / ctas));
     const size_t n = (size_t)n_head_kv * p->n_rt * FT, ml = up16(n * p->splits * sizeof(float2));
     p->ml = reinterpret_cast<float2*>(ws);
+    if ((int64_t)n * p->n_kt * FT <= kKeptScores) {  // whole lines of 128 bytes
+        p->scores = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(ws + ml) + 127) & ~(uintptr_t)127);
+        p->r_splits = 1;
+        while (p->r_splits < 8 && p->n_rows >= 64 * p->r_splits &&
+               (int64_t)n_head_kv * p->n_kt * p->r_splits * 2 <= kKeptCtas)
+            p->r_splits *= 2;
+        return ml + n * p->n_kt * FT * sizeof(float) + 112;
+    }
     p->nlse = reinterpret_cast<float*>(ws + ml);
     // few key tiles and many rows: split the rows of the sums pass too
     p->r_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_rt / 2, 2 * kSms / ((int64_t)n_head_kv * p->n_kt)));
@@ -955,7 +1079,7 @@ size_t plan_tc(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, 
 // A launch that may start before what precedes it on the stream has ended (the
 // kernels wait for it on the device).
 template <class... P, class... A>
-cudaError_t launch_after(void (*k)(P...), int64_t grid, int heads, int threads, int smem, cudaStream_t s,
+cudaError_t launch_after(void (*k)(P...), int64_t grid, int heads, int threads, int smem, cudaStream_t s, int cluster,
                          const A&... args) {
     if (grid < 1 || grid > INT_MAX) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
@@ -963,11 +1087,14 @@ cudaError_t launch_after(void (*k)(P...), int64_t grid, int heads, int threads, 
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
@@ -992,11 +1119,13 @@ cudaError_t launch_f32(const WeightArgs& a, cudaStream_t s) {
     if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_sums_f32<D>), smem, m1);
     if (e != cudaSuccess) return e;
     const int64_t K = a.n_head_kv, rows = K * p.n_rt * FT;
-    e = launch_after(k7_stats_f32<D>, K * p.n_rt * p.splits, 1, kF32Threads, smem, s, a, p);
-    if (e == cudaSuccess) e = launch_after(k7_join_f32, rows / (kJoinThreads / 16), 1, kJoinThreads, 0, s, a, p);
-    if (e == cudaSuccess) e = launch_after(k7_sums_f32<D>, K * p.n_kt * p.r_splits, 1, kF32Threads, smem, s, a, p);
+    e = launch_after(k7_stats_f32<D>, K * p.n_rt * p.splits, 1, kF32Threads, smem, s, 1, a, p);
+    if (e == cudaSuccess && p.scores != nullptr)
+        return launch_after(k7_kept_f32, K * p.n_kt * p.r_splits, 1, kKeptThreads, 0, s, p.r_splits, a, p);
+    if (e == cudaSuccess) e = launch_after(k7_join_f32, rows / (kJoinThreads / 16), 1, kJoinThreads, 0, s, 1, a, p);
+    if (e == cudaSuccess) e = launch_after(k7_sums_f32<D>, K * p.n_kt * p.r_splits, 1, kF32Threads, smem, s, 1, a, p);
     if (e != cudaSuccess || p.r_splits == 1) return e;
-    return launch_after(k7_add, (a.kv_len + kJoinThreads - 1) / kJoinThreads, a.n_head_kv, kJoinThreads, 0, s, a,
+    return launch_after(k7_add, (a.kv_len + kJoinThreads - 1) / kJoinThreads, a.n_head_kv, kJoinThreads, 0, s, 1, a,
                         (const float*)p.part, p.n_kt * FT, p.r_splits);
 }
 
@@ -1043,13 +1172,13 @@ cudaError_t launch_tc(const WeightArgs& a, cudaStream_t s) {
     if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(&k7_pass<BF16, D, SEG, 1, true>), smem, m2);
     if (e != cudaSuccess) return e;
     const int64_t K = a.n_head_kv;
-    e = launch_after(k7_pass<BF16, D, SEG, 0, false>, K * p.n_groups * p.splits, 1, kTcThreads, smem, s, mq, mk, a, p);
-    if (e == cudaSuccess) e = launch_after(k7_join, K * p.n_rt * BM / (kJoinThreads / 16), 1, kJoinThreads, 0, s, a, p);
+    e = launch_after(k7_pass<BF16, D, SEG, 0, false>, K * p.n_groups * p.splits, 1, kTcThreads, smem, s, 1, mq, mk, a, p);
+    if (e == cudaSuccess) e = launch_after(k7_join, K * p.n_rt * BM / (kJoinThreads / 16), 1, kJoinThreads, 0, s, 1, a, p);
     if (e == cudaSuccess)
         e = launch_after(p.resident ? k7_pass<BF16, D, SEG, 1, false> : k7_pass<BF16, D, SEG, 1, true>,
-                         K * p.b_splits * p.r_splits, 1, kTcThreads, smem, s, mq, mk, a, p);
+                         K * p.b_splits * p.r_splits, 1, kTcThreads, smem, s, 1, mq, mk, a, p);
     if (e != cudaSuccess || p.r_splits == 1) return e;
-    return launch_after(k7_add, (a.kv_len + kJoinThreads - 1) / kJoinThreads, a.n_head_kv, kJoinThreads, 0, s, a,
+    return launch_after(k7_add, (a.kv_len + kJoinThreads - 1) / kJoinThreads, a.n_head_kv, kJoinThreads, 0, s, 1, a,
                         (const float*)p.part, p.n_kt * BM, p.r_splits);
 }
 

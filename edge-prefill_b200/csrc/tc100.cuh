@@ -100,6 +100,7 @@ __device__ __forceinline__ uint32_t peer_of(const void* p, int k) {
 // Waits for every thread of the cluster that has not ended, and for what it
 // wrote to shared memory.
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
