@@ -241,8 +241,10 @@ struct BatchKv {
 
 #if defined(__CUDACC__)
 // Length of sequence s; one outside [0, max_kv_len] is recorded and read as 0.
+// (An ordinary load: the kernel before may still have been writing the lengths
+// when this one started, so they are not read-only for its whole life.)
 __device__ __forceinline__ int32_t batch_len(const BatchKv& b, int32_t s, int32_t* err) {
-    const int32_t n = __ldg(b.lens + s);
+    const int32_t n = b.lens[s];
     if (n < 0 || n > b.max_kv_len) {
         report_error(err, kDevBadLength, 0x90, s);
         return 0;
@@ -255,7 +257,7 @@ __device__ __forceinline__ int32_t batch_len(const BatchKv& b, int32_t s, int32_
 __device__ __forceinline__ int32_t batch_row(const BatchKv& b, int32_t s, int32_t r, int32_t* err) {
     if (b.block_rows <= 0) return s * b.seq_rows + r;
     const int32_t i = r / b.block_rows;
-    const int64_t blk = __ldg(b.tables + (int64_t)s * b.table_stride + i);
+    const int64_t blk = b.tables[(int64_t)s * b.table_stride + i];
     const int64_t row = blk * b.block_rows + (r - i * b.block_rows);
     if (blk < 0 || row >= b.rows) {
         report_error(err, kDevBadBlockTable, 0x91, s);

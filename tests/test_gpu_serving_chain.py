@@ -8,7 +8,7 @@ import torch
 
 import epsp
 import workloads as W
-from serving_util import Cache, context, decode64, kept64, prompt64, rounding, workspace
+from serving_util import Cache, TORCH, context, decode64, kept64, prompt64, rounding, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -245,3 +245,37 @@ def test_calls_on_two_streams_at_once():
         assert ((x["wacc"].double() - ref).abs() <= tol).all()
         a_host = x["acc"][0].cpu().tolist()
         assert x["kept"][0].tolist() == [kept64(a_host[h], n, 500, 4, 30) for h in range(K)]
+
+
+@pytest.mark.parametrize("dtype", [epsp.BF16, epsp.F32], ids=["bf16", "f32"])
+def test_calls_that_follow_each_other_without_a_wait(dtype):
+    """Evictions in place that rewrite the lengths the next call reads, and decode steps on the rows they leave: back to
+    back the same as with a wait after each call."""
+    H, K, d, B = 8, 2, 64, 64
+    lens0 = [1500, 900, 64, 0, 301]
+    n_seq = len(lens0)
+
+    def run(wait):
+        cache = Cache(lens0, K, d, dtype, B, 9)
+        ctx = context(H, K, d, dtype, dtype, 2048, B)
+        g = torch.Generator().manual_seed(3)
+        q = torch.randn(12, n_seq, H, d, generator=g).to(TORCH[dtype]).cuda()
+        acc = torch.rand(n_seq, K, cache.cap, generator=g).cuda()
+        ws = workspace(max(ctx.decode_bytes(n_seq, cache.cap, True), ctx.evict_bytes(n_seq, cache.cap, 1400)))
+        out = torch.zeros(12, n_seq, H, d, dtype=TORCH[dtype], device="cuda")
+        torch.cuda.synchronize()
+        for i in range(12):
+            keep = 1400 - 110 * i
+            ctx.check(ctx.evict_layer(0, cache.batch, cache.k, cache.v, acc, keep, 3, 17, cache.batch, cache.k, cache.v,
+                                      ws, acc_dst=acc, new_lens=cache.d_lens))
+            if wait:
+                torch.cuda.synchronize()
+            ctx.check(ctx.decode_layer(0, cache.batch, q[i], cache.k, cache.v, out[i], ws, acc=acc))
+            if wait:
+                torch.cuda.synchronize()
+        ctx.check(ctx.sync_status())
+        assert cache.d_lens.tolist() == [min(n, 1400 - 110 * 11) for n in lens0]
+        return out, acc
+
+    for x, y in zip(run(False), run(True)):
+        assert torch.equal(x, y)
