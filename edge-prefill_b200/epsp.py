@@ -439,7 +439,7 @@ class Context:
         return f
 
     def _cache_tensors(self, kv, k, v, what=("k", "v")):
-        dt, _, _, _, dev, _, heads, d = self._fast()
+        dt, _, _, _, dev, _, heads, d = self._facts or self._fast()
         if kv.device is not None and kv.device != dev:
             raise ValueError(f"the batch is on cuda:{kv.device}, not cuda:{dev}")
         need = kv.rows * heads * d
@@ -471,22 +471,26 @@ class Context:
         """kv: KvBatch; q, out [n_seq][n_head][head_dim]; k, v the cache's rows; k_new, v_new [n_seq][n_head_kv]
         [head_dim]; acc f32 [n_seq][n_head_kv][stride].  Raises ValueError for a tensor of another type, shape,
         layout or device; returns the status code."""
-        dt, odt, f32, _, dev, heads, kvh, d = self._fast()
+        dt, odt, f32, _, dev, heads, kvh, d = self._facts or self._fast()
         self._cache_tensors(kv, k, v)
         n_seq = kv.n_seq
         _check("q", q, dt, (n_seq, heads, d), dev)
         _check("out", out, odt, (n_seq, heads, d), dev)
+        p_k, p_v, p_acc, wide = None, None, None, 0
         if k_new is not None:
             _check("k_new", k_new, dt, (n_seq, kvh, d), dev)
+            p_k = k_new.data_ptr()
         if v_new is not None:
             _check("v_new", v_new, dt, (n_seq, kvh, d), dev)
-        wide = 0
+            p_v = v_new.data_ptr()
         if acc is not None:
             wide = acc.shape[-1]
             _check("acc", acc, f32, (n_seq, kvh, wide), dev)
+            p_acc = acc.data_ptr()
         ws, n = self._workspace(workspace)
-        return lib.ep_sp_decode_layer(self.h, layer, kv.ref, q.data_ptr(), _ptr(k_new), _ptr(v_new), k.data_ptr(),
-                                      v.data_ptr(), out.data_ptr(), _ptr(acc), wide, ws, n, self._stream(stream))
+        return lib.ep_sp_decode_layer(self.h, layer, kv.ref, q.data_ptr(), p_k, p_v, k.data_ptr(), v.data_ptr(),
+                                      out.data_ptr(), p_acc, wide, ws, n,
+                                      _current_stream(dev) if stream is None else self._stream(stream))
 
     def prompt_weights_bytes(self, kv_len, n_tok, row_begin):
         n = c_size_t()
@@ -516,24 +520,28 @@ class Context:
                     acc_dst=None, new_lens=None, kept_rows=None, stream=None):
         """src, dst: KvBatch (the same object and tensors compact in place); acc f32 [n_seq][n_head_kv][stride];
         acc_dst likewise; new_lens int32 [n_seq]; kept_rows int32 [n_seq][n_head_kv][n_keep]."""
-        _, _, f32, i32, dev, _, kvh, _ = self._fast()
+        _, _, f32, i32, dev, _, kvh, _ = self._facts or self._fast()
         self._cache_tensors(src, k, v)
         self._cache_tensors(dst, k_dst, v_dst, ("k_dst", "v_dst"))
         n_seq = src.n_seq
-        wide, wide_dst = acc.shape[-1], 0
+        wide = acc.shape[-1]
         _check("acc", acc, f32, (n_seq, kvh, wide), dev)
+        p_acc, wide_dst, p_lens, p_kept = None, 0, None, None
         if acc_dst is not None:
             wide_dst = acc_dst.shape[-1]
             _check("acc_dst", acc_dst, f32, (n_seq, kvh, wide_dst), dev)
+            p_acc = acc_dst.data_ptr()
         if new_lens is not None:
             _check("new_lens", new_lens, i32, (n_seq,), dev)
+            p_lens = new_lens.data_ptr()
         if kept_rows is not None:
             _check("kept_rows", kept_rows, i32, (n_seq, kvh, n_keep), dev)
+            p_kept = kept_rows.data_ptr()
         ws, n = self._workspace(workspace)
         return lib.ep_sp_evict_layer(self.h, layer, src.ref, k.data_ptr(), v.data_ptr(), acc.data_ptr(), wide,
                                      n_keep, sink_rows, recent_rows, dst.ref, k_dst.data_ptr(), v_dst.data_ptr(),
-                                     _ptr(acc_dst), wide_dst, _ptr(new_lens), _ptr(kept_rows), ws, n,
-                                     self._stream(stream))
+                                     p_acc, wide_dst, p_lens, p_kept, ws, n,
+                                     _current_stream(dev) if stream is None else self._stream(stream))
 
     def profile_families(self):
         """{family name: (milliseconds, launches)} since the last ep_sp_profile_enable."""
