@@ -7,7 +7,8 @@
 // Storing the scores instead would cost 8 bytes a pair; recomputing them costs
 // 2 d flops, which the tensor cores do in a quarter of the time the pair's two
 // exponentials take.  The exponentials bound both passes (16 MUFU results per
-// clock and SM, a fifth of the pairs on the FMA pipe instead).  Every key has one writer and a fixed order of additions.
+// clock and SM, a fifth of the pairs on the FMA pipe instead).  Every key has one
+// writer (k7_add where the rows are split) and a fixed order of additions.
 //
 // 16-bit (tcgen05): a query tile packs T = 128 / G tokens x G heads into 128
 // rows.  The two passes are one kernel with the MMA operands exchanged: with
@@ -68,10 +69,7 @@ __device__ __forceinline__ float2 exp2_poly_add(float2 x, float2 acc) {
 
 // acc + 2^x of pair i of a run of pairs: one pair in kPolyEvery on the FMA
 // pipe, the rest on MUFU.
-#ifndef K7_POLY_EVERY
-#define K7_POLY_EVERY 5
-#endif
-constexpr int kPolyEvery = K7_POLY_EVERY;
+constexpr int kPolyEvery = 5;
 __device__ __forceinline__ float2 exp2_add(float2 x, int i, float2 acc) {
     return i % kPolyEvery == kPolyEvery - 1 ? exp2_poly_add(x, acc)
                                             : __fadd2_rn(acc, make_float2(ex2(x.x), ex2(x.y)));
@@ -216,8 +214,8 @@ __device__ __forceinline__ void give_back(uint64_t* se, int lane) {
 // stream otherwise.
 // A step is one (query tile, key tile); three pairs of warpgroups, an S buffer
 // each, take the steps in turn, each warpgroup 64 of the 128 columns, 32 at a
-// time (the buffer goes back to the MMA warp halfway).  Issue slots and MUFU together bound it: 24 warps hide more of
-// each other than 16 with 64 columns in registers (96 against 101 us for 64
+// time (the buffer goes back to the MMA warp halfway).  Issue slots and MUFU
+// together bound it: 24 warps hide more of each other than 16 with 64 columns in registers (96 against 101 us for 64
 // rows of 32 heads over 64K keys), a warpgroup per step measured 99 us.
 // STREAM: the sums pass whose query tiles stream.
 template <bool BF16, int D, int SEG, int PASS, bool STREAM>
@@ -235,7 +233,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint64_t tmo = a.timeout_ns;
 
     // the CTA's part
-    int h, rt0 = 0, n_q, k0, k1, q_slots, k_slots;
+    int h, rs = 0, rt0 = 0, n_q, k0, k1, q_slots, k_slots;
     constexpr bool stream_q = STREAM;
     static_assert(PASS == 1 || !STREAM, "the statistics pass keeps its query tiles");
     if constexpr (PASS == 0) {
@@ -251,12 +249,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         q_slots = p.group;
         k_slots = LY::kSlots - p.group;
     } else {
-        const int rs = blockIdx.x % p.r_splits, rest = blockIdx.x / p.r_splits;
+        const int rest = blockIdx.x / p.r_splits;
+        rs = p.r_splits - 1 - blockIdx.x % p.r_splits;  // late rows first
         h = rest / p.b_splits;
         rt0 = (int)((int64_t)p.n_rt * rs / p.r_splits);
         n_q = (int)((int64_t)p.n_rt * (rs + 1) / p.r_splits) - rt0;
         k0 = rest % p.b_splits;  // groups of kg key tiles: k0, k0 + b_splits, ...
-        k1 = (p.n_kt + p.kg - 1) / p.kg;
+        // (no row of the part sees the key tiles after its last)
+        k1 = ((min(t_first + (rt0 + n_q) * p.T, a.kv_len) - 1) / BM + p.kg) / p.kg;
         q_slots = p.q_slots;
         k_slots = p.k_slots;
     }
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int w = 0; w < kWgs; ++w) v += from[w * BM];
                     if (p.r_splits > 1) {
-                        p.part[((int64_t)(blockIdx.x % p.r_splits) * Hkv + h) * p.n_kt * BM + key] = v;
+                        p.part[((int64_t)rs * Hkv + h) * p.n_kt * BM + key] = v;
                         continue;
                     }
                     float* out = a.acc + (int64_t)h * a.acc_stride + key;
@@ -650,15 +650,20 @@ __device__ __forceinline__ void join_rows(const float2* ml, float* nlse, int64_t
 }
 
 // The parts' sums of each key, in order, into acc; `stride`: keys of a row of
-// `part` [splits][Hkv][stride].
-__global__ void __launch_bounds__(kJoinThreads) k7_add(const WeightArgs a, const float* part, int stride, int splits) {
+// `part` [splits][Hkv][stride].  T > 0: parts of n_rt query tiles of T tokens,
+// which only wrote the key tiles that they see.
+__global__ void __launch_bounds__(kJoinThreads) k7_add(const WeightArgs a, const float* part, int stride, int splits,
+                                                       int T, int n_rt) {
     tc::pdl_wait();
     tc::pdl_launch();
     const int key = blockIdx.x * kJoinThreads + threadIdx.x, h = blockIdx.y;
     if (key >= a.kv_len) return;
+    int first = 0;
+    if (const int late = key / BM * BM - (a.kv_len - a.n_tok + a.row_begin); T > 0 && late > 0)
+        while (first + 1 < splits && (int)((int64_t)n_rt * (first + 1) / splits) * T <= late) ++first;
     float v = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < splits; ++s) v += part[((int64_t)s * a.n_head_kv + h) * stride + key];
+    for (int s = first; s < splits; ++s) v += part[((int64_t)s * a.n_head_kv + h) * stride + key];
     float* out = a.acc + (int64_t)h * a.acc_stride + key;
     *out = a.accumulate ? *out + v : v;
 }
@@ -1045,6 +1050,8 @@ size_t plan_f32(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv,
     return ml + lse + (p->r_splits > 1 ? up16((size_t)p->r_splits * n_head_kv * p->n_kt * FT * sizeof(float)) : 0);
 }
 
+constexpr int64_t kPartSums = 16 << 20;  // sums of all parts, at most
+
 size_t plan_tc(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, int32_t d, char* ws, WeightPlan* p) {
     const int slots = d == 128 ? TcLayout<128>::kSlots : TcLayout<64>::kSlots;
     p->T = BM / (n_head / n_head_kv);
@@ -1058,16 +1065,29 @@ size_t plan_tc(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, 
     // sums pass: a CTA per key tile, the rows split too when there are few key
     // tiles and many rows
     p->r_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(p->n_rt / 4, kSms / ((int64_t)n_head_kv * p->n_kt)));
-    // query tiles that leave two slots for keys stay on chip, more of them
-    // stream; then two key tiles share each query tile's load once there are
-    // enough key tiles to fill the device that way
-    const int tiles = (p->n_rt + p->r_splits - 1) / p->r_splits;
-    p->resident = tiles <= slots - 2;
-    p->q_slots = p->resident ? tiles : slots / 2;
+    // Query tiles that leave two slots for keys stay on chip.  More of them are
+    // split until they do (the split with the fewest steps for a CTA), as long
+    // as the parts' sums stay small; else they stream, and two key tiles share
+    // each query tile's load once there are enough key tiles to fill the
+    // device that way.  (14 heads of 64, 512 rows over 8192 keys: 61 us split, 66
+    // streaming; 32 heads of 128, 256 over 65536: 316 and 363.)
+    auto tiles = [&](int r) { return (p->n_rt + r - 1) / r; };
+    auto ctas = [&](int r) { return std::max(1, std::min(p->n_kt, kSms / (n_head_kv * r))); };
+    if (const int least = tiles(slots - 2); tiles(p->r_splits) > slots - 2 &&
+                                            (int64_t)least * n_head_kv * p->n_kt * BM <= kPartSums) {
+        int64_t best = INT64_MAX;
+        for (int r = least; r <= 2 * least && (int64_t)r * n_head_kv * p->n_kt * BM <= kPartSums; ++r) {
+            const int64_t waves = ((int64_t)n_head_kv * r * ctas(r) + kSms - 1) / kSms;
+            const int64_t steps = waves * ((p->n_kt + ctas(r) - 1) / ctas(r)) * tiles(r);
+            if (steps < best) best = steps, p->r_splits = r;
+        }
+    }
+    p->resident = tiles(p->r_splits) <= slots - 2;
+    p->q_slots = p->resident ? tiles(p->r_splits) : slots / 2;
     p->k_slots = slots - p->q_slots;
     p->kg = !p->resident && (int64_t)n_head_kv * p->n_kt >= 2 * kSms ? 2 : 1;
     const int n_kg = (p->n_kt + p->kg - 1) / p->kg;
-    p->b_splits = std::max(1, std::min(n_kg, kSms / n_head_kv));
+    p->b_splits = std::max(1, std::min(n_kg, kSms / (n_head_kv * p->r_splits)));
     const size_t n = (size_t)n_head_kv * p->n_rt * BM, ml = up16(n * p->splits * sizeof(float2));
     const size_t lse = up16(n * sizeof(float));
     p->ml = reinterpret_cast<float2*>(ws);
@@ -1126,7 +1146,7 @@ cudaError_t launch_f32(const WeightArgs& a, cudaStream_t s) {
     if (e == cudaSuccess) e = launch_after(k7_sums_f32<D>, K * p.n_kt * p.r_splits, 1, kF32Threads, smem, s, 1, a, p);
     if (e != cudaSuccess || p.r_splits == 1) return e;
     return launch_after(k7_add, (a.kv_len + kJoinThreads - 1) / kJoinThreads, a.n_head_kv, kJoinThreads, 0, s, 1, a,
-                        (const float*)p.part, p.n_kt * FT, p.r_splits);
+                        (const float*)p.part, p.n_kt * FT, p.r_splits, 0, 0);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
@@ -1179,7 +1199,7 @@ cudaError_t launch_tc(const WeightArgs& a, cudaStream_t s) {
                          K * p.b_splits * p.r_splits, 1, kTcThreads, smem, s, 1, mq, mk, a, p);
     if (e != cudaSuccess || p.r_splits == 1) return e;
     return launch_after(k7_add, (a.kv_len + kJoinThreads - 1) / kJoinThreads, a.n_head_kv, kJoinThreads, 0, s, 1, a,
-                        (const float*)p.part, p.n_kt * BM, p.r_splits);
+                        (const float*)p.part, p.n_kt * BM, p.r_splits, p.T, p.n_rt);
 }
 
 template <bool BF16, int D>

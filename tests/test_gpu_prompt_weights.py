@@ -71,6 +71,21 @@ def test_many_rows_over_few_keys(kv_len, n_tok, row_begin, heads, dtype):
     run_case(kv_len, n_tok, row_begin, heads, dtype, 32, 0, accumulate=True, pad=3, seed=kv_len + 1)
 
 
+def test_more_rows_than_parts_are_kept_of():
+    """So many rows and keys that the sums are not split over the rows: the query tiles stream past the keys."""
+    run_case(8250, 8250, 0, (128, 1, 128), BF16, 64, 64, seed=4)
+    run_case(19000, 1800, 0, (256, 2, 128), F16, 128, 0, accumulate=True, pad=5, seed=5)
+
+
+@pytest.mark.parametrize("kv_len,n_tok,row_begin,heads", [
+    (5000, 600, 0, (14, 2, 64)), (3000, 3000, 17, (7, 1, 64)), (4300, 900, 0, (8, 1, 128)), (9000, 260, 3, (32, 8, 128))],
+    ids=str)
+def test_rows_split_over_parts(kv_len, n_tok, row_begin, heads):
+    """More query tiles than stay on chip: parts of the rows, of which the early ones do not see the last keys."""
+    run_case(kv_len, n_tok, row_begin, heads, BF16, 64, 64, seed=kv_len)
+    run_case(kv_len, n_tok, row_begin, heads, F16, 32, 0, accumulate=True, pad=3, seed=kv_len + 1)
+
+
 def test_long_cache():
     run_case(30000, 64, 0, (32, 8, 128), BF16, 128, 128, accumulate=True, seed=2)
     run_case(20011, 700, 500, (28, 4, 128), F16, 64, 64, seed=3)
