@@ -6,10 +6,12 @@
 // row above it, and the first of those equal to it, get their place by a
 // prefix sum in row order.  The rows of one head are split over a cluster of
 // up to 8 CTAs, which keep their slice of the weights in registers (one read
-// of the weights) and add their histograms through distributed shared
-// memory; only counts are exchanged, so the result is exact and has no order.
-// Latency bounds it: a histogram round is one cluster barrier and a few block
-// ones; the third, and often the second, is skipped when the whole bin stays.
+// of the weights), count in their own shared memory and add the bins that are
+// not empty to every CTA's counts; only counts are exchanged, so the result is
+// exact and has no order.  Latency bounds it: a histogram round is one cluster
+// barrier and a few block ones; the third, and often the second, is skipped
+// when the whole bin stays.  (Reading all bins of all CTAs instead: 64 K rows
+// 24 us against 22; each CTA summing a share of the bins, two barriers: 23.)
 //
 // K8b moves the listed rows, which the bytes bound: a warp takes as many rows
 // as fill its lanes with eight 16-byte loads each.  In place there is an order to
@@ -30,8 +32,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 // Slices of up to 2048 rows are held by 512 threads, 4 rows each (batches of
-// short sequences: 14 against 16 us with 1024 threads), longer ones by 1024
-// threads, 8 or 32 rows each (64 K rows: 26 against 28 us with 512).
+// short sequences: 11 against 14 us with 1024 threads), longer ones by 1024
+// threads, 8 or 32 rows each (64 heads of 16 K rows: 20 against 22 us with 512).
 constexpr int kSliceS = 2048, kSliceM = 8192, kSliceL = 32768;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
@@ -432,7 +434,7 @@ size_t plan_of(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t n_head
     p->cap = n_keep < max_kv_len ? n_keep : max_kv_len;
     // One CTA per head when that fills the device; more for slices over 8 K
     // rows, and where few heads leave SMs idle, down to 2 K rows.  (64 heads of
-    // 16 K rows: 67 us with clusters of 8, 35 with 4, 24 with 2.)
+    // 16 K rows: 40 us with clusters of 8, 28 with 4, 20 with 2.)
     const int64_t runs = (int64_t)n_seq * n_head_kv;
     auto slice = [&](int cluster) { return ((max_kv_len + cluster - 1) / cluster + 31) & ~31; };
     p->cluster = 1;
