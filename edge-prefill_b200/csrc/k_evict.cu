@@ -480,13 +480,13 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s) {
     cfg.blockDim = dim3(p.slice == kSliceS ? 512 : 1024);
     cfg.stream = s;
     cudaLaunchAttribute at[2]{};
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = p.cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = p.cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = p.cluster > 1 ? 2 : 1;
     cudaError_t e = p.slice == kSliceS   ? cudaLaunchKernelEx(&cfg, k8a_select_rows<4, 512>, a, p)
                     : p.slice == kSliceM ? cudaLaunchKernelEx(&cfg, k8a_select_rows<8, 1024>, a, p)
                     : p.slice == kSliceL ? cudaLaunchKernelEx(&cfg, k8a_select_rows<32, 1024>, a, p)

@@ -1083,7 +1083,7 @@ size_t plan_tc(int32_t kv_len, int32_t rows, int32_t n_head, int32_t n_head_kv, 
     if (const int least = tiles(slots - 2); tiles(p->r_splits) > slots - 2 &&
                                             (int64_t)least * n_head_kv * p->n_kt * BM <= kPartSums) {
         best = INT64_MAX;
-        for (int r = least; r <= 2 * least && (int64_t)r * n_head_kv * p->n_kt * BM <= kPartSums; ++r) {
+        for (int r = least; r <= std::min(2 * least, least + 16) && (int64_t)r * n_head_kv * p->n_kt * BM <= kPartSums; ++r) {
             const int64_t waves = ((int64_t)n_head_kv * r * ctas(r) + kSms - 1) / kSms;
             const int64_t steps = waves * ((p->n_kt + ctas(r) - 1) / ctas(r)) * tiles(r);
             if (steps < best) best = steps, p->r_splits = r;

@@ -446,9 +446,9 @@ class Context:
         tail = (heads, d)
         # rows in any number of leading dimensions; both at once when all is well (an attribute of a tensor takes
         # 50 to 150 ns)
+        shape = k.shape
         if (k.dtype is dt and v.dtype is dt and k.get_device() == dev and v.get_device() == dev and k.is_contiguous()
-                and v.is_contiguous() and k.shape[-2:] == tail and v.shape[-2:] == tail and k.numel() >= need
-                and v.numel() >= need):
+                and v.is_contiguous() and shape[-2:] == tail and v.shape == shape and k.numel() >= need):
             return
         for name, t in zip(what, (k, v)):
             _check(name, t, dt, t.shape[:-2] + tail, dev)
