@@ -19,8 +19,6 @@
 // K8c gives each CTA a 32-byte column of one head, which it compacts from the
 // first row to the last: a kept row never moves up, so a step's loads need
 // only be done before its own stores.
-#include <cooperative_groups.h>
-
 #include <type_traits>
 
 #include "epsp_kernels.h"
@@ -28,8 +26,6 @@
 
 namespace epsp {
 namespace {
-
-namespace cg = cooperative_groups;
 
 // Slices of up to 2048 rows are held by 512 threads, 4 rows each (batches of
 // short sequences: 11 against 14 us with 1024 threads), longer ones by 1024
@@ -98,7 +94,6 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
     __shared__ uint32_t place_sums[32];
     __shared__ Choice choice[3];
     __shared__ int s_len;
-    cg::cluster_group cluster = cg::this_cluster();
     const int C = p.cluster, rank = blockIdx.x % C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int h = blockIdx.x / C % a.n_head_kv, s = blockIdx.x / C / a.n_head_kv;
     for (int i = t; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<int4*>(bins_of)[i] = make_int4(0, 0, 0, 0);
@@ -135,8 +130,8 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
     if (C > 1) {
         if (t == 0 && rank == 0) s_len = batch_len(a.src, s, a.err);
         load(min(a.src.max_kv_len, r0 + p.per));
-        cluster.sync();
-        n = *cluster.map_shared_rank(&s_len, 0);
+        tc::cluster_sync();
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(tc::peer_of(&s_len, 0)) : "memory");
     } else {
         if (t == 0) s_len = batch_len(a.src, s, a.err);
         __syncthreads();
@@ -196,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
                                      "r"(c)
                                      : "memory");
                 }
-                cluster.sync();
+                tc::cluster_sync();
             }
             // thread t has kEach bins, counted from the top
             constexpr int kEach = bins / kThreads > 0 ? bins / kThreads : 1;
@@ -241,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
         if (C > 1) {
             if (t < C)
                 asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(tc::peer_of(&totals[rank], t)), "l"(total) : "memory");
-            cluster.sync();
+            tc::cluster_sync();
             for (int k = 0; k < rank; ++k) base += totals[k];
         }
         return base;
