@@ -392,7 +392,9 @@ __device__ __forceinline__ void join_cluster(const DecodeArgs& a, const DecodeSp
     }
 }
 
-template <int ET, int D, int W, bool P3, int GH>
+// JOIN: the calls that join_cluster finishes (kept apart: 64 runs of up to
+// 4096 rows, 90 us without its code and 92 with it).
+template <int ET, int D, int W, bool P3, int GH, bool JOIN>
 __global__ void __launch_bounds__((W + 1) * 32, 1)
     k6a_decode(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
                const DecodeSplit sp) {
@@ -430,8 +432,8 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
     // ----------------------------------------- this CTA's range of the units
     Walk w0;
     Lens lens{nullptr};
-    const int C = sp.cluster, rank = blockIdx.x & (C - 1);
-    if (sp.direct) {
+    const int C = JOIN ? sp.cluster : 1, rank = blockIdx.x & (C - 1);
+    if (JOIN || sp.direct) {
         const int id = blockIdx.x >> (__ffs(C) - 1);
         w0.s = id / runs;
         w0.run = id % runs;
@@ -833,7 +835,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                     lt += v[r].y * ex2(v[r].x - ms);
                     ot.x += t[r].x, ot.y += t[r].y, ot.z += t[r].z, ot.w += t[r].w;
                 }
-            if (C > 1 || sp.fused) {
+            if constexpr (JOIN) {
                 // (the ring: this CTA's last copy has landed)
                 *reinterpret_cast<float4*>(smem + (g * D + c * 4) * 4) = ot;
                 if (c == 0) *reinterpret_cast<float2*>(smem + kPass * D * 4 + g * 8) = make_float2(ms, lt);
@@ -848,7 +850,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                 if (c == 0) sp.part_ml[p] = make_float2(ms, lt);
             }
         }
-        if (C > 1 || sp.fused) {
+        if constexpr (JOIN) {
             join_cluster<D, kWarps * 32, kPass>(a, sp, smem, om, w, n_seg, q_row + pass * kPass, n_heads, h, rank);
             if (C > 1) tc::cluster_sync();  // nobody reads this CTA's part any more
         }
@@ -1144,8 +1146,8 @@ size_t split_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_hea
     return at;
 }
 
-template <int ET, int D, int W, bool P3, int GH>
-cudaError_t launch_t(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
+template <int ET, int D, int W, bool P3, int GH, bool JOIN>
+cudaError_t launch_join(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     constexpr int kThreads = (W + 1) * 32;
     CUtensorMap mk, mv;
     if (!cache_map(&mk, a.k, a.dtype, D, a.n_head_kv, a.kv.rows) ||
@@ -1157,7 +1159,7 @@ cudaError_t launch_t(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     // one bit per device ordinal < 32 whose attribute is set
     static std::atomic<unsigned> set_mask{0};
     if (dev >= 32 || !(set_mask.load(std::memory_order_acquire) & (1u << dev))) {
-        const cudaError_t e = cudaFuncSetAttribute(k6a_decode<ET, D, W, P3, GH>,
+        const cudaError_t e = cudaFuncSetAttribute(k6a_decode<ET, D, W, P3, GH, JOIN>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         if (dev < 32) set_mask.fetch_or(1u << dev, std::memory_order_release);
@@ -1185,7 +1187,7 @@ cudaError_t launch_t(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.numAttrs = sp.cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k6a_decode<ET, D, W, P3, GH>, mk, mv, a, sp);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k6a_decode<ET, D, W, P3, GH, JOIN>, mk, mv, a, sp);
     if (e != cudaSuccess || (sp.direct && (!a.acc || sp.fused))) return e;
     const int chunks = a.acc ? (a.kv.max_kv_len + kJoinRows - 1) / kJoinRows : 0;
     const int heads = std::min(a.n_head / a.n_head_kv, sp.pass_heads);
@@ -1196,6 +1198,12 @@ cudaError_t launch_t(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, k6b_join<D>, a, sp, heads, chunks);
+}
+
+template <int ET, int D, int W, bool P3, int GH>
+cudaError_t launch_t(const DecodeArgs& a, const DecodeSplit& sp, cudaStream_t s) {
+    return sp.cluster > 1 || sp.fused ? launch_join<ET, D, W, P3, GH, true>(a, sp, s)
+                                      : launch_join<ET, D, W, P3, GH, false>(a, sp, s);
 }
 
 template <int ET, int D, int W>
