@@ -22,6 +22,7 @@
 // exponentials.
 #include <cuda.h>
 #include <cudaTypedefs.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <atomic>
@@ -203,6 +204,47 @@ __device__ __forceinline__ void give_back(uint64_t* se, int lane) {
     tc::fence_before_sync();
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(se);
+}
+
+// What rows [c0, c1) of the query tile whose first token is `tok0` of the window
+// give one key.  Rows of a tile that are none are zeros with an lse of -inf:
+// they add nothing to a finite key, but 0 * inf to one with an infinity.  A NaN
+// sum of a tile that has such rows is therefore taken again, here, without
+// them; `lse`: minus the tile's lse.  (In line and in loops that stay loops: as
+// a call, 64 rows of 32 heads over 64K keys 114 us, so 107, without it 107;
+// masking the columns in every step instead 114 to 117.)
+template <bool BF16, int D>
+__device__ __forceinline__ float weigh_again(const WeightArgs& a, const float* lse, int c0, int c1, int tok0, int h, int key) {
+    const int G = a.n_head / a.n_head_kv, at = a.kv_len - a.n_tok + a.row_begin + tok0;  // cache row of the first token
+    const float sl2 = a.kq_scale * 1.4426950408889634f;
+    bool bad = false;
+    const int kr = phys_row(a.paging, key, bad);
+    if (bad) return 0.f;  // (reported when the tile was loaded)
+    auto two = [](uint32_t u) {
+        if constexpr (BF16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+        else return __half22float2(*reinterpret_cast<const __half2*>(&u));
+    };
+    const uint4* k = static_cast<const uint4*>(a.k) + ((int64_t)kr * a.n_head_kv + h) * (D / 8);
+    float sum = 0.f;
+#pragma unroll 1
+    for (int c = max(c0, (key - at) * G); c < c1 && sum == sum; ++c) {  // from the first row that sees the key
+        const uint4* q = static_cast<const uint4*>(a.q) +
+                         ((int64_t)(a.row_begin + tok0 + c / G) * a.n_head + h * G + c % G) * (D / 8);
+        float x = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < D / 8; ++i) {
+            const uint4 u = q[i], v = k[i];
+            const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 y = two(us[j]), z = two(vs[j]);
+                x = fmaf(y.x, z.x, x);
+                x = fmaf(y.y, z.y, x);
+            }
+        }
+        sum += ex2(fmaf(x, sl2, lse[c]));
+    }
+    return sum;
 }
 
 // PASS 0: statistics.  CTA (key split, group of query tiles, KV head): the
@@ -565,7 +607,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
                 const float2 t = __fadd2_rn(acc[0], acc[1]);
-                return t.x + t.y;
+                float v = t.x + t.y;
+                if (__any_sync(0xffffffffu, v != v)) {
+                    const int live = min(p.T, a.kv_len - tt) * G - half * 64;  // of this thread's 64 columns
+                    if (v != v && live < 64 && key0 + row < a.kv_len)
+                        v = weigh_again<BF16, D>(a, lse_s + qs * BM, half * 64, half * 64 + live, (rt0 + rt) * p.T, h, key0 + row);
+                    __syncwarp();
+                }
+                return v;
             };
             if constexpr (!STREAM) {
                 // steps (key tile, query tile) in turn; this pair of warpgroups has every third one
@@ -895,7 +944,8 @@ __global__ void __launch_bounds__(kF32Threads) k7_sums_f32(const WeightArgs a, c
             scores_f32<D, NI>(q, k, ty, tx, x);
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int r = rt * FT + ty + 16 * i, tok = t_first + r / G;
+                // (a row that is none sees no key: its query is zeros, and a key may hold infinities)
+                const int r = rt * FT + ty + 16 * i, tok = r < p.n_rows ? t_first + r / G : -1;
                 const float ls = nlse[r];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)

@@ -496,7 +496,9 @@ int32_t ep_sp_decode_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* 
  * [head_dim], k the cache, paged under ep_sp_set_paged_kv); acc is
  * [n_head_kv][acc_stride] f32 with acc_stride >= kv_len.  q, k and the
  * workspace are 16-byte aligned.  Each row's weights are added in a fixed
- * order.  rc 2 on bad arguments. */
+ * order.  A cache row whose scores are all -inf weighs nothing, also where an
+ * infinity in it makes them so; a NaN in a query row of the window may make
+ * any of its KV head's sums NaN.  rc 2 on bad arguments. */
 int32_t ep_sp_prompt_weights_bytes(const ep_sp_ctx* ctx, int32_t kv_len, int32_t n_tok, int32_t row_begin,
                                    size_t* bytes);
 int32_t ep_sp_prompt_weights(ep_sp_ctx* ctx, int32_t layer, const void* q, const void* k, int32_t kv_len,

@@ -1,0 +1,95 @@
+"""The cache-serving calls on values that are no ordinary numbers, and on weights far apart: infinities in the rows of a
+cache, rows whose weight is nothing, one row that outweighs all others."""
+import pytest
+import torch
+
+import epsp
+from serving_util import Cache, TORCH, context, score_error, workspace
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = epsp.F32, epsp.F16, epsp.BF16
+
+
+def with_dead_keys(kv_len, n_tok, row_begin, heads, dtype, page, block, seed):
+    """Sums over a cache in which some rows hold an infinity that makes all of their scores -inf (elements of q of one
+    sign meet an infinity of the other), their 64-bit reference, its tolerance, and the dead rows."""
+    H, K, d = heads
+    g = torch.Generator().manual_seed(seed)
+    k = torch.randn(1, kv_len, K, d, generator=g)
+    dead = torch.rand(kv_len, generator=g) < 0.1
+    dead[0] = False  # every query sees a key that counts
+    dead[kv_len // 2] = dead[-1] = True
+    minus = torch.rand(kv_len, generator=g) < 0.5
+    k[0, dead & minus, :, 5] = float("-inf")
+    k[0, dead & ~minus, :, 9] = float("inf")
+    cache = Cache([kv_len], K, d, dtype, block, seed, k=k.to(TORCH[dtype]))
+    q = torch.randn(n_tok, H, d, generator=g)
+    q[..., 5] = q[..., 5].abs() + 0.1
+    q[..., 9] = -q[..., 9].abs() - 0.1
+    q = q.to(TORCH[dtype]).cuda()
+    ctx = context(H, K, d, dtype, dtype, kv_len, page)
+    if block:
+        ctx.check(ctx.set_paged_kv(block, cache.d_table[0], cache.d_table.shape[1], cache.rows))
+    acc = torch.full((K, kv_len), 5.0, device="cuda")
+    ws = workspace(ctx.prompt_weights_bytes(kv_len, n_tok, row_begin))
+    ctx.check(ctx.prompt_weights(0, q, cache.k, kv_len, n_tok, row_begin, acc, ws))
+    torch.cuda.synchronize()
+    ctx.check(ctx.sync_status())
+    # the same with the dead rows taken out of each query's softmax
+    dead = dead.cuda()
+    alive = cache.seq(0)[0].clone()
+    alive[dead] = 0
+    ref, tol = torch.zeros((K, kv_len), dtype=torch.float64, device="cuda"), 0.0
+    late = torch.arange(kv_len, device="cuda")[None, :] > torch.arange(kv_len - n_tok + row_begin, kv_len, device="cuda")[:, None]
+    for hq in range(H):
+        a, b = q[row_begin:, hq].double(), alive[:, hq // (H // K)].double()
+        x = (a @ b.T / d ** 0.5).masked_fill(late | dead, float("-inf"))
+        ref[hq // (H // K)] += torch.softmax(x, -1).sum(0)
+        tol = max(tol, 2 * score_error(a.abs() @ b.abs().T / d ** 0.5, d))
+    return acc, ref, ref * (tol + (n_tok - row_begin) * (H // K) * 2.0 ** -24), dead
+
+
+# windows that fill their last query tile and that do not, groups that divide it and that do not, query tiles that stay
+# on chip, are split into parts and stream; in f32, scores that are kept and that are computed twice
+DEAD_KEYS = [(500, 64, 0, (14, 2, 64)), (300, 36, 0, (7, 1, 128)), (1000, 37, 5, (8, 1, 64)), (129, 1, 0, (4, 4, 128)),
+             (700, 32, 0, (32, 8, 128)), (260, 30, 0, (65, 1, 64)), (5000, 600, 0, (14, 2, 64)),
+             (4300, 900, 0, (8, 1, 128)), (2000, 2000, 0, (16, 1, 128)), (17200, 4100, 0, (100, 1, 128))]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("kv_len,n_tok,row_begin,heads", DEAD_KEYS, ids=str)
+def test_prompt_weights_of_rows_of_infinities(kv_len, n_tok, row_begin, heads, dtype):
+    """A cache row whose scores are all -inf has weight 0, whatever the columns that hold no query make of it."""
+    if dtype == F32 and kv_len > 10000:
+        kv_len, n_tok = 4500, 500
+    for block in (0, 32):
+        acc, ref, tol, dead = with_dead_keys(kv_len, n_tok, row_begin, heads, dtype, 32, block, kv_len + block)
+        assert torch.isfinite(acc).all()
+        assert (acc[:, dead].abs() <= 2.0 ** -100).all()
+        over = (acc.double() - ref).abs() - tol - 2.0 ** -100
+        assert (over <= 0).all(), float(over.max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("kv_len,n_tok,heads", [(65536, 36, (28, 4, 128)), (17200, 2050, (100, 1, 128))], ids=str)
+def test_prompt_weights_of_a_query_that_is_none(kv_len, n_tok, heads, dtype):
+    """A NaN query, or a NaN cache row, ends in NaN sums and in time: no wait runs out."""
+    H, K, d = heads
+    if dtype == F32:
+        kv_len //= 8
+    g = torch.Generator().manual_seed(1)
+    cache = Cache([kv_len], K, d, dtype, 0, 2)
+    ctx = context(H, K, d, dtype, dtype, kv_len, 32)
+    ws = workspace(ctx.prompt_weights_bytes(kv_len, n_tok, 0))
+    for what in ("query", "key"):
+        q = torch.randn(n_tok, H, d, generator=g).to(TORCH[dtype]).cuda()
+        k = cache.k.clone()
+        if what == "query":
+            q[-1, -1, 3] = float("nan")
+        else:
+            k[7, -1, 3] = float("nan")
+        acc = torch.zeros(K, kv_len, device="cuda")
+        ctx.check(ctx.prompt_weights(0, q, k, kv_len, n_tok, 0, acc, ws))
+        ctx.check(ctx.sync_status())
+        assert torch.isnan(acc[-1]).all() and torch.isfinite(acc[:-1]).all()
