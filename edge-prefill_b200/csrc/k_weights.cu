@@ -47,14 +47,15 @@ __device__ __forceinline__ float max3f(float x, float y, float z) {
     return r;
 }
 
-// acc + 2^x of a pair on the FMA pipe.  x >= -126 (below: 2^-126; NaN stays) is split
-// into n + r, n = round(x), r in [-0.5, 0.5]: adding 1.5 * 2^23 + 127 leaves
-// n + 127 in the low mantissa bits, which shifted up are 2^n's bits.  2^r is a
-// polynomial of degree 5, fitted here for the least relative error on that
-// interval (7.5e-8, 2.4e-7 with f32 coefficients and steps: ex2's own error).
+// acc + 2^x of a pair on the FMA pipe.  x >= -126.5 (below: 0, as ex2 has it;
+// the exponent's bits come out 0 at -127; NaN stays) is split into n + r,
+// n = round(x), r in [-0.5, 0.5]: adding 1.5 * 2^23 + 127 leaves n + 127 in the
+// low mantissa bits, which shifted up are 2^n's bits.  2^r is a polynomial of
+// degree 5, fitted here for the least relative error on that interval (7.5e-8,
+// 2.4e-7 with f32 coefficients and steps: ex2's own error).
 __device__ __forceinline__ float2 exp2_poly_add(float2 x, float2 acc) {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
     const float2 t = __fadd2_rn(x, make_float2(12583039.f, 12583039.f));
     const float2 n = __fadd2_rn(t, make_float2(-12583039.f, -12583039.f));
     const float2 r = __ffma2_rn(n, make_float2(-1.f, -1.f), x);

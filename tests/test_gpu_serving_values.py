@@ -93,3 +93,24 @@ def test_prompt_weights_of_a_query_that_is_none(kv_len, n_tok, heads, dtype):
         ctx.check(ctx.prompt_weights(0, q, k, kv_len, n_tok, 0, acc, ws))
         ctx.check(ctx.sync_status())
         assert torch.isnan(acc[-1]).all() and torch.isfinite(acc[:-1]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("kv_len,n_tok,row_begin,heads", DEAD_KEYS, ids=str)
+def test_prompt_weights_of_nothing_are_zero(kv_len, n_tok, row_begin, heads, dtype):
+    """A weight of nothing is 0 itself, so that an eviction ranks such rows by their place alone; so is one that
+    underflows in every query (scores 200 and more below the others)."""
+    if dtype == F32 and kv_len > 10000:
+        kv_len, n_tok = 4500, 500
+    acc, _, _, dead = with_dead_keys(kv_len, n_tok, row_begin, heads, dtype, 32, 0, kv_len)
+    assert (acc[:, dead] == 0).all()
+    H, K, d = heads
+    q = torch.full((n_tok, H, d), 4.0).to(TORCH[dtype]).cuda()
+    k = torch.zeros(kv_len, K, d, dtype=TORCH[dtype], device="cuda")
+    k[dead] = -200.0 / (4 * d ** 0.5)
+    ctx = context(H, K, d, dtype, dtype, kv_len, 32)
+    ctx.check(ctx.prompt_weights(0, q, k, kv_len, n_tok, row_begin, acc,
+                                 workspace(ctx.prompt_weights_bytes(kv_len, n_tok, row_begin))))
+    torch.cuda.synchronize()
+    ctx.check(ctx.sync_status())
+    assert (acc[:, dead] == 0).all()
