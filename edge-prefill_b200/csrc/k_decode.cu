@@ -26,7 +26,11 @@
 // take, and the fragments come straight from the ring by ldmatrix; tcgen05
 // would want 128 rows where there are 8.  Rows 8-15 of the P operand carry
 // P - round16(P), so P keeps 16 bits of mantissa (bf16; 22 in f16) at no extra
-// MMA; f32 outputs of bf16 caches add a third part.
+// MMA; f32 outputs of bf16 caches add a third part.  f16 has few exponents: P
+// is 2^7 times the weight against the running maximum there (2^15 at most), and
+// the remainder, summed in accumulators of its own, 2^12 times itself.  A
+// weight keeps 2^-16 of itself down to 2^-28 of the largest, and an absolute
+// step of 2^-44 of it below.
 // f32: FMA on the CUDA cores, one key per lane for S, 4 (or 2) columns per
 // lane for O.
 //
@@ -401,6 +405,8 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
     constexpr int kHeads = ET == 0 ? GH : 8;  // query heads per warp
     using LY = Layout<ET, D, W, kHeads>;
     constexpr bool BF16 = ET == 2;
+    constexpr float kUp = ET == 1 ? 7.f : 0.f;         // the maximum is kept this much lower, in log2 units
+    constexpr float kLow = ET == 1 ? 4096.f : 1.f;     // factor of P's remainder
     constexpr int kWarps = LY::kWarps, kThreads = (W + 1) * 32, kPass = LY::kPass;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
@@ -641,11 +647,11 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                 }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                // the running maximum follows when it is 2^8 behind: p stays below 2^8
-                const bool need = mx > m[0] + 8.f;
+                // the running maximum follows when it is 2^8 behind: p stays below 2^8 (f16: 2^15)
+                const bool need = mx > m[0] + (8.f + kUp);
                 if (__any_sync(0xffffffffu, need)) {
-                    const float alpha = need ? ex2(m[0] - mx) : 1.f;
-                    if (need) m[0] = mx;
+                    const float alpha = need ? ex2(m[0] - (mx - kUp)) : 1.f;
+                    if (need) m[0] = mx - kUp;
                     l[0] *= alpha;
 #pragma unroll
                     for (int j = 0; j < NO; ++j) o[j] *= alpha;
@@ -663,6 +669,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                     float* p0 = s4[2 * kb16];
                     float* p1 = s4[2 * kb16 + 1];
                     const uint32_t a0 = split2<BF16>(p0[0], p0[1]), a2 = split2<BF16>(p1[0], p1[1]);
+                    if constexpr (kLow != 1.f) p0[0] *= kLow, p0[1] *= kLow, p1[0] *= kLow, p1[1] *= kLow;
                     const uint32_t a1 = split2<BF16>(p0[0], p0[1]), a3 = split2<BF16>(p1[0], p1[1]);
                     uint32_t t0 = 0, t2 = 0;
                     if constexpr (P3) {
@@ -799,7 +806,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
 #pragma unroll
             for (int c = 0; c < D / 8; ++c)  // rows 8-15 hold the P remainders' part
                 *reinterpret_cast<float2*>(om_w + hd * D + c * 8 + qc) =
-                    make_float2((o[4 * c] + o[4 * c + 2]) * f, (o[4 * c + 1] + o[4 * c + 3]) * f);
+                    make_float2(fmaf(o[4 * c + 2], 1.f / kLow, o[4 * c]) * f, fmaf(o[4 * c + 3], 1.f / kLow, o[4 * c + 1]) * f);
         } else {
             constexpr int NC = D / 32;
 #pragma unroll

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import epsp
-from serving_util import Cache, TORCH, context, score_error, workspace
+from serving_util import Cache, TORCH, context, decode64, rounding, score_error, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,57 @@ def test_prompt_weights_of_nothing_are_zero(kv_len, n_tok, row_begin, heads, dty
     torch.cuda.synchronize()
     ctx.check(ctx.sync_status())
     assert (acc[:, dead] == 0).all()
+
+
+TYPES = [(F16, F16), (F16, F32), (BF16, BF16), (BF16, F32), (F32, F32)]
+TYPE_IDS = ["f16", "f16_f32", "bf16", "bf16_f32", "f32"]
+
+
+def decode_once(cache, q, dtype, out_dtype, page=32):
+    n_seq, H, d = q.shape
+    K = cache.k.shape[1]
+    ctx = context(H, K, d, dtype, out_dtype, cache.cap, page)
+    out = torch.full((n_seq, H, d), 7.0, dtype=TORCH[out_dtype], device="cuda")
+    acc = torch.zeros(n_seq, K, cache.cap, device="cuda")
+    ctx.check(ctx.decode_layer(0, cache.batch, q, cache.k, cache.v, out,
+                               workspace(ctx.decode_bytes(n_seq, cache.cap, True)), acc=acc))
+    plain = torch.full_like(out, 7.0)  # without weights the rows may be split over CTAs in another way
+    ctx.check(ctx.decode_layer(0, cache.batch, q, cache.k, cache.v, plain,
+                               workspace(ctx.decode_bytes(n_seq, cache.cap, False))))
+    torch.cuda.synchronize()
+    ctx.check(ctx.sync_status())
+    return out, plain, acc
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("heads", [(4, 2, 64), (20, 1, 128)], ids=str)
+@pytest.mark.parametrize("n", [200, 1000, 5000])
+def test_decode_of_one_row_that_outweighs_all(n, heads, dtype, out_dtype):
+    """One row's weight is e^10 to e^18 times each other's and its V row is zero, so that the output comes from the light
+    rows alone: their weights have to keep their bits."""
+    H, K, d = heads
+    g = torch.Generator().manual_seed(n)
+    for gap in (10.0, 14.0, 16.0, 17.5, 18.0):
+        for at in (5, n // 2, n - 1):
+            for spread in (0.0, 0.3):
+                k = torch.randn(1, n, K, d, generator=g) * spread
+                k[..., 0] = 0
+                k[0, at] = 0
+                k[0, at, :, 0] = gap * d ** 0.5 / 8
+                v = torch.ones(1, n, K, d) if spread == 0 else torch.rand(1, n, K, d, generator=g)
+                v[0, at] = 0
+                q = torch.randn(1, H, d, generator=g)
+                q[..., 0] = 8
+                cache = Cache([n], K, d, dtype, 32, 1, k=k.to(TORCH[dtype]), v=v.to(TORCH[dtype]))
+                q = q.to(TORCH[dtype]).cuda()
+                outs = decode_once(cache, q, dtype, out_dtype)
+                ref, tol, add, add_tol = decode64(cache, q)
+                if spread == 0:
+                    # every score is one exact product, and its scaling in log2 units off by half a step of a value under
+                    # 32, 2^-20, once above and once below: 2^-18 of the ratio with the exponentials' own; 2^-16 for the
+                    # weights' parts; and 200 additions in f32 of a warp's, its CTA's and the joined sums
+                    tol = ref.abs() * (2.0 ** -18 + 2.0 ** -16 + 200 * 2.0 ** -24)
+                for out in outs[:2]:
+                    over = (out.double() - ref).abs() - tol - rounding(ref, out_dtype)
+                    assert (over <= 0).all(), (gap, at, spread, float(((out.double() - ref) / ref).abs().max()))
+                assert ((outs[2].double() - add).abs() <= add_tol).all()
