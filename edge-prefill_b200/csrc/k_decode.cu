@@ -686,9 +686,9 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
                         float(&o1)[4] = *reinterpret_cast<float(*)[4]>(&o[8 * c + 4]);
                         mma16816<BF16>(o0, a0, a1, a2, a3, b[0], b[1]);
                         mma16816<BF16>(o1, a0, a1, a2, a3, b[2], b[3]);
-                        if constexpr (P3) {
-                            mma16816<BF16>(o0, t0, 0, t2, 0, b[0], b[1]);
-                            mma16816<BF16>(o1, t0, 0, t2, 0, b[2], b[3]);
+                        if constexpr (P3) {  // (P again in rows 0-7: a zero or a third part there would spoil an infinite V)
+                            mma16816<BF16>(o0, a0, t0, a2, t2, b[0], b[1]);
+                            mma16816<BF16>(o1, a0, t0, a2, t2, b[2], b[3]);
                         }
                     }
                 }
@@ -802,11 +802,17 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
             return mt == -INFINITY ? 0.f : mt;
         };
         if constexpr (ET != 0) {
+            // the sum over P and that over its remainders, which says nothing
+            // where V is infinite: a remainder may be 0 or negative
+            auto whole_sum = [](float hi, float lo) {
+                if constexpr (P3) hi *= 0.5f;  // added twice
+                return isinf(hi) ? hi : fmaf(lo, 1.f / kLow, hi);
+            };
             const float f = ex2(m[0] - top(hd));
 #pragma unroll
             for (int c = 0; c < D / 8; ++c)  // rows 8-15 hold the P remainders' part
                 *reinterpret_cast<float2*>(om_w + hd * D + c * 8 + qc) =
-                    make_float2(fmaf(o[4 * c + 2], 1.f / kLow, o[4 * c]) * f, fmaf(o[4 * c + 3], 1.f / kLow, o[4 * c + 1]) * f);
+                    make_float2(whole_sum(o[4 * c], o[4 * c + 2]) * f, whole_sum(o[4 * c + 1], o[4 * c + 3]) * f);
         } else {
             constexpr int NC = D / 32;
 #pragma unroll

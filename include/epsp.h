@@ -471,6 +471,10 @@ typedef struct ep_sp_kv_batch {
  *   acc           NULL, or [n_seq][n_head_kv][acc_stride] f32 (acc_stride >=
  *                 max_kv_len): acc[s][h][r] += the row's softmax weights
  *                 summed over the query heads of KV head h, r < kv_lens[s].
+ * A row whose score is -inf weighs nothing.  An infinite element of V makes its
+ * column of the output infinite; the column is NaN where infinities of both
+ * signs meet, and where such a row's weight is nothing (in an f16 cache: under
+ * 2^-32 of the largest).
  * q, k, v, k_new, v_new, out and the workspace are 16-byte aligned.  Scores,
  * softmax statistics and sums are f32; an f32 context multiplies in f32
  * whatever ep_sp_set_f32_attention says.  A sequence's result does not depend

@@ -168,3 +168,37 @@ def test_decode_of_one_row_that_outweighs_all(n, heads, dtype, out_dtype):
                     over = (out.double() - ref).abs() - tol - rounding(ref, out_dtype)
                     assert (over <= 0).all(), (gap, at, spread, float(((out.double() - ref) / ref).abs().max()))
                 assert ((outs[2].double() - add).abs() <= add_tol).all()
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("heads", [(14, 2, 64), (20, 1, 128)], ids=str)
+@pytest.mark.parametrize("n", [1, 33, 200, 1000, 5000])
+def test_decode_of_infinite_values(n, heads, dtype, out_dtype):
+    """An infinite element of V makes its column of the output infinite, infinities of both signs or a NaN make it NaN,
+    and the other columns are as they were."""
+    H, K, d = heads
+    g = torch.Generator().manual_seed(n)
+    inf = float("inf")
+    for rows in ([0], [n // 2, n - 1], sorted({0, n // 3, n - 1})):
+        k, v = torch.randn(1, n, K, d, generator=g), torch.randn(1, n, K, d, generator=g)
+        for i, r in enumerate(rows):
+            v[0, r, :, 3] = inf
+            v[0, r, :, 7 + 2 * i] = -inf
+            v[0, r, :, d - 1] = inf if i % 2 else -inf
+        v[0, rows[-1], 0, 20] = float("nan")
+        cache = Cache([n], K, d, dtype, 32, 1, k=k.to(TORCH[dtype]), v=v.to(TORCH[dtype]))
+        q = torch.randn(1, H, d, generator=g).to(TORCH[dtype]).cuda()
+        outs = decode_once(cache, q, dtype, out_dtype)
+        vals = cache.seq(0)[1].float()
+        up, down, nan = (x.any(0).repeat_interleave(H // K, 0)[None] for x in (vals == inf, vals == -inf, vals.isnan()))
+        cache.v = torch.where(torch.isfinite(cache.v), cache.v, torch.zeros_like(cache.v))
+        ref, tol, add, add_tol = decode64(cache, q)
+        ref[up], ref[down] = inf, -inf
+        ref[nan | (up & down)] = float("nan")
+        plain = torch.isfinite(ref)
+        for out in outs[:2]:
+            assert torch.equal(torch.isnan(out), torch.isnan(ref))
+            assert torch.equal(torch.isinf(out), torch.isinf(ref)) and torch.equal(out[torch.isinf(ref)] > 0, ref[torch.isinf(ref)] > 0)
+            over = (out.double() - ref).abs() - tol - rounding(ref, out_dtype)
+            assert (over[plain] <= 0).all(), float(over[plain].max())
+        assert ((outs[2].double() - add).abs() <= add_tol).all()
