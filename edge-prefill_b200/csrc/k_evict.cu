@@ -324,7 +324,7 @@ constexpr int kMoveUnroll = 8;  // a thread's loads under way
 // Kept rows a warp moves: a row of K and V is 2 NV 16-byte vectors.
 constexpr int move_rows(int nv) { return 2 * nv > 32 ? kMoveUnroll / 2 : kMoveUnroll * (32 / (2 * nv)); }
 
-// Grid (KV head, rows / (8 warps' rows), sequence): gathers into other rows
+// Grid (rows / (8 warps' rows) * KV heads, 1, sequence): gathers into other rows
 // than the source's.
 template <int NV>  // 16-byte vectors of a row
 __global__ void __launch_bounds__(kMoveThreads) k8b_move(const EvictArgs a, const EvictPlan p) {
@@ -333,13 +333,13 @@ __global__ void __launch_bounds__(kMoveThreads) k8b_move(const EvictArgs a, cons
     constexpr int kRows = move_rows(NV);
     constexpr int kTurns = 2 * NV > 32 ? 2 * NV / 32 : 1;
     constexpr int kAtOnce = 2 * NV > 32 ? 1 : 32 / (2 * NV);
-    const int h = blockIdx.x, s = blockIdx.z, lane = threadIdx.x & 31;
-    const int i0 = (blockIdx.y * (kMoveThreads / 32) + (threadIdx.x >> 5)) * kRows;
+    const int h = blockIdx.x % a.n_head_kv, s = blockIdx.z, lane = threadIdx.x & 31;
+    const int i0 = (blockIdx.x / a.n_head_kv * (kMoveThreads / 32) + (threadIdx.x >> 5)) * kRows;
     const int i = i0 + lane;
     // (the list's capacity, not the count, bounds this load: both arrive together)
     const int row = lane < kRows && i < p.cap ? p.list[((int64_t)s * a.n_head_kv + h) * p.cap + i] : -1;
     const int m = p.kept[s];
-    if (a.new_lens && h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_lens[s] = m;
+    if (a.new_lens && blockIdx.x == 0 && threadIdx.x == 0) a.new_lens[s] = m;
     if (i0 >= m) return;
     int from = -1, to = -1;
     if (lane < kRows && i < m) {
@@ -468,8 +468,10 @@ size_t evict_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t
 cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s) {
     EvictPlan p{};
     plan_of(a.src.n_seq, a.src.max_kv_len, a.n_keep, a.n_head_kv, static_cast<char*>(a.ws), &p);
+    const int nv = a.head_dim * a.elem_bytes / 16, rows = move_rows(nv) * (kMoveThreads / 32);
     const int64_t ctas = (int64_t)a.src.n_seq * a.n_head_kv * p.cluster;
-    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+    const int64_t moves = ((int64_t)p.cap + rows - 1) / rows * a.n_head_kv;  // in x: y and z hold 65535
+    if (ctas > 0x7fffffff || moves > 0x7fffffff || a.n_head_kv > 65535) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(p.slice == kSliceS ? 512 : 1024);
@@ -487,12 +489,10 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s) {
                     : p.slice == kSliceL ? cudaLaunchKernelEx(&cfg, k8a_select_rows<32, 1024>, a, p)
                                          : cudaLaunchKernelEx(&cfg, k8a_select_rows<0, 1024>, a, p);
     if (e != cudaSuccess) return e;
-    const int nv = a.head_dim * a.elem_bytes / 16;
     if (a.in_place) {
         e = launch_after(k8c_compact, dim3(nv, a.n_head_kv, a.src.n_seq), kPlaceThreads, s, a, p);
     } else {
-        const int rows = move_rows(nv) * (kMoveThreads / 32);
-        const dim3 grid(a.n_head_kv, (p.cap + rows - 1) / rows, a.src.n_seq);
+        const dim3 grid((unsigned)moves, 1, a.src.n_seq);
         if (nv == 8) e = launch_after(k8b_move<8>, grid, kMoveThreads, s, a, p);
         else if (nv == 16) e = launch_after(k8b_move<16>, grid, kMoveThreads, s, a, p);
         else e = launch_after(k8b_move<32>, grid, kMoveThreads, s, a, p);

@@ -1,5 +1,5 @@
-"""The cache-serving calls on values that are no ordinary numbers, and on weights far apart: infinities in the rows of a
-cache, rows whose weight is nothing, one row that outweighs all others."""
+"""The cache-serving calls on values that are no ordinary numbers, and on weights and sizes far apart: infinities in the
+rows of a cache, rows whose weight is nothing, one row that outweighs all others, millions of rows kept."""
 import pytest
 import torch
 
@@ -202,3 +202,27 @@ def test_decode_of_infinite_values(n, heads, dtype, out_dtype):
             over = (out.double() - ref).abs() - tol - rounding(ref, out_dtype)
             assert (over[plain] <= 0).all(), float(over[plain].max())
         assert ((outs[2].double() - add).abs() <= add_tol).all()
+
+
+def test_eviction_that_keeps_millions_of_rows():
+    """More chunks of rows than a grid's y and z can count: 2,100,000 rows of 512 bytes are gathered."""
+    K, d, n, keep = 1, 128, 2_200_003, 2_100_001
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(n, K, d, generator=g, device="cuda") for _ in range(2))
+    acc = torch.randint(0, 1 << 20, (1, K, n), generator=g, device="cuda").float()
+    kd, vd = (torch.full((keep + 5, K, d), 3.0, device="cuda") for _ in range(2))
+    ctx = context(2, K, d, F32, F32, n, 128)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    new, kept = torch.zeros_like(lens), torch.zeros(1, K, keep, dtype=torch.int32, device="cuda")
+    src, dst = epsp.KvBatch(lens, n, seq_rows=n), epsp.KvBatch(None, keep, seq_rows=keep, n_seq=1)
+    rc = ctx.evict_layer(0, src, k, v, acc, keep, 4, 1000, dst, kd, vd, workspace(ctx.evict_bytes(1, n, keep)),
+                         new_lens=new, kept_rows=kept)
+    assert rc == epsp.OK, ctx.last_error()
+    torch.cuda.synchronize()
+    ctx.check(ctx.sync_status())
+    rank = acc[0, 0].clone()
+    rank[:4] = rank[n - 1000:] = float("inf")
+    rows = torch.sort(torch.sort(rank, descending=True, stable=True)[1][:keep])[0]
+    assert int(new) == keep and torch.equal(kept[0, 0].long(), rows)
+    assert torch.equal(kd[:keep], k[rows]) and torch.equal(vd[:keep], v[rows])
+    assert (kd[keep:] == 3).all() and (vd[keep:] == 3).all()
