@@ -836,11 +836,13 @@ __global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, 
     const int last_row = min(rt * FT + FT, p.n_rows) - 1;
     const int n_kt = (t_first + last_row / G) / FT + 1;
     const int k0 = (int)((int64_t)n_kt * sp / p.splits), k1 = (int)((int64_t)n_kt * (sp + 1) / p.splits);
-    int tok[4];
+    int tok[4], seen_to[4];
     float m[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        tok[i] = t_first + (rt * FT + ty + 16 * i) / G;
+        const int r = rt * FT + ty + 16 * i;
+        tok[i] = t_first + r / G;
+        seen_to[i] = r < p.n_rows ? tok[i] / FT : -1;  // a row that is none is not kept
         m[i] = -INFINITY;
         l[i] = 0.f;
     }
@@ -872,7 +874,8 @@ __global__ void __launch_bounds__(kF32Threads) k7_stats_f32(const WeightArgs a, 
                     x[i][j] = kt * FT + tx + 16 * j <= tok[i] ? x[i][j] * sl2 : -INFINITY;
                     mx = fmaxf(mx, x[i][j]);
                 }
-                if (p.scores != nullptr) {
+                // (only scores that are read, and given up, by the second pass: others would stay in L2)
+                if (p.scores != nullptr && kt <= seen_to[i]) {
                     const float* to = scores + 16 * i * wide + kt * FT;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import epsp
-from serving_util import Cache, TORCH, context, decode64, rounding, score_error, workspace
+from serving_util import Cache, TORCH, context, decode64, prompt64, rounding, score_error, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -226,3 +226,24 @@ def test_eviction_that_keeps_millions_of_rows():
     assert int(new) == keep and torch.equal(kept[0, 0].long(), rows)
     assert torch.equal(kd[:keep], k[rows]) and torch.equal(vd[:keep], v[rows])
     assert (kd[keep:] == 3).all() and (vd[keep:] == 3).all()
+
+
+@pytest.mark.parametrize("kv_len,window,heads", [(4096, 17, (1, 1, 64)), (3000, 1, (3, 1, 128)), (2048, 2048, (2, 2, 64))],
+                         ids=str)
+def test_prompt_weights_keep_only_scores_that_are_read(kv_len, window, heads):
+    """f32: scores wait in the cache between the passes at its highest priority, so only those of rows that see a key of
+    their 64 are written."""
+    H, K, d = heads
+    cache = Cache([kv_len], K, d, F32, 0, 1)
+    q = torch.randn(window, H, d, generator=torch.Generator().manual_seed(2)).cuda()
+    ctx = context(H, K, d, F32, F32, kv_len, 32)
+    acc = torch.zeros(K, kv_len, device="cuda")
+    ws = workspace(ctx.prompt_weights_bytes(kv_len, window, 0))
+    ctx.check(ctx.prompt_weights(0, q, cache.k, kv_len, window, 0, acc, ws))
+    torch.cuda.synchronize()
+    written = int((ws[:ws.numel() // 4 * 4].view(torch.int32) != -0x54545455).sum())  # 0xABABABAB: as it was
+    sees = torch.arange(kv_len - window, kv_len) // 64 + 1  # tiles of 64 keys that each query row sees
+    tiles = -(-window * (H // K) // 64) * -(-kv_len // 64) * K  # a maximum and a sum of 64 rows each, at most
+    assert written <= int(sees.sum()) * 64 * H + tiles * 64 * 2
+    ref, tol = prompt64(q, cache.k, kv_len, window, 0)
+    assert ((acc.double() - ref).abs() <= tol).all()
