@@ -78,6 +78,8 @@ int32_t check_batch(ep_sp_ctx* c, const ep_sp_kv_batch* b, int32_t min_rows, boo
     if (b->max_kv_len < 1 || b->max_kv_len > c->cfg.max_ctx)
         return bad("max_kv_len must lie in [1, max_ctx]");
     if (need_lens && !b->kv_lens) return bad("null kv_lens");
+    if (!aligned(b->kv_lens, 4) || (b->block_rows != 0 && !aligned(b->block_tables, 4)))
+        return bad("kv_lens and block_tables must be 4-byte aligned");
     const int32_t rows = std::max(min_rows, 1);
     out->n_seq = b->n_seq;
     out->max_kv_len = b->max_kv_len;
@@ -290,6 +292,8 @@ int32_t ep_sp_evict_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* s
             return ctx_fail(ctx, kInvalid, "acc_stride smaller than max_kv_len");
         if (acc_dst && (acc_dst_stride < most || !aligned(acc_dst, 4)))
             return ctx_fail(ctx, kInvalid, "acc_dst_stride smaller than the rows kept");
+        if (!aligned(new_lens, 4) || !aligned(kept_rows, 4))
+            return ctx_fail(ctx, kInvalid, "new_lens and kept_rows must be 4-byte aligned");
         if (acc_dst == acc && acc_dst_stride != acc_stride)
             return ctx_fail(ctx, kInvalid, "acc_dst may be acc only with the same stride");
         const bool same_layout = a.src.block_rows == a.dst.block_rows && a.src.tables == a.dst.tables &&
