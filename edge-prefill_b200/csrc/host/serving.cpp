@@ -299,6 +299,7 @@ int32_t ep_sp_evict_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* s
         const bool same_layout = a.src.block_rows == a.dst.block_rows && a.src.tables == a.dst.tables &&
                                  a.src.table_stride == a.dst.table_stride && a.src.seq_rows == a.dst.seq_rows &&
                                  a.src.rows == a.dst.rows;
+        if (k_dst == v_dst && k != v) return ctx_fail(ctx, kInvalid, "K and V would go to the same rows");
         if ((k_dst == k) != (v_dst == v) || k_dst == v || v_dst == k)
             return ctx_fail(ctx, kInvalid, "K and V are either both compacted in place or both gathered elsewhere");
         a.in_place = k_dst == k && same_layout;

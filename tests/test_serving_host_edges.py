@@ -18,3 +18,8 @@ def test_lengths_and_tables_off_their_alignment_are_refused(bad):
 def test_outputs_of_an_eviction_off_their_alignment_are_refused(bad):
     c = make()
     assert evict(c, desc(), dst(), **bad) == I and "aligned" in c.last_error()
+
+
+def test_k_and_v_into_the_same_rows_is_refused():
+    c = make()
+    assert evict(c, desc(), dst(), k_dst=3 * PTR, v_dst=3 * PTR) == I and "same rows" in c.last_error()
