@@ -40,6 +40,10 @@ private:
     bool ok_ = false;
 };
 
+// Rows of a sequence, at most: kernels round lengths up to tiles, and step past
+// them, in 32 bits.
+constexpr int32_t kMaxRows = INT_MAX - 65536;
+
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // Device state and current device of a compute call.  Reserving allocates and
@@ -77,6 +81,7 @@ int32_t check_batch(ep_sp_ctx* c, const ep_sp_kv_batch* b, int32_t min_rows, boo
     if (b->n_seq < 1 || b->n_seq > 65535) return bad("n_seq must lie in [1, 65535]");
     if (b->max_kv_len < 1 || b->max_kv_len > c->cfg.max_ctx)
         return bad("max_kv_len must lie in [1, max_ctx]");
+    if (b->max_kv_len > kMaxRows) return bad("max_kv_len is more than 32 bits can round up");
     if (need_lens && !b->kv_lens) return bad("null kv_lens");
     if (!aligned(b->kv_lens, 4) || (b->block_rows != 0 && !aligned(b->block_tables, 4)))
         return bad("kv_lens and block_tables must be 4-byte aligned");
@@ -144,7 +149,7 @@ int32_t guarded(F&& f) noexcept {
 extern "C" {
 
 int32_t ep_sp_decode_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_len, int32_t with_acc, size_t* bytes) {
-    if (!ctx || !bytes || n_seq < 1 || n_seq > 65535 || max_kv_len < 1 || max_kv_len > ctx->cfg.max_ctx ||
+    if (!ctx || !bytes || n_seq < 1 || n_seq > 65535 || max_kv_len < 1 || max_kv_len > std::min(ctx->cfg.max_ctx, kMaxRows) ||
         (with_acc != 0 && with_acc != 1))
         return kInvalid;
     const ep_sp_config& c = ctx->cfg;
@@ -202,7 +207,7 @@ int32_t ep_sp_decode_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* 
 
 int32_t ep_sp_prompt_weights_bytes(const ep_sp_ctx* ctx, int32_t kv_len, int32_t n_tok, int32_t row_begin,
                                    size_t* bytes) {
-    if (!ctx || !bytes || n_tok < 1 || kv_len < n_tok || kv_len > ctx->cfg.max_ctx || row_begin < 0 ||
+    if (!ctx || !bytes || n_tok < 1 || kv_len < n_tok || kv_len > std::min(ctx->cfg.max_ctx, kMaxRows) || row_begin < 0 ||
         row_begin >= n_tok)
         return kInvalid;
     *bytes = epsp::weights_ws_bytes(kv_len, n_tok - row_begin, ctx->cfg.n_head, ctx->cfg.n_head_kv, ctx->cfg.head_dim,
@@ -221,7 +226,8 @@ int32_t ep_sp_prompt_weights(ep_sp_ctx* ctx, int32_t layer, const void* q, const
         if (!q || !k || !acc) return ctx_fail(ctx, kInvalid, "null tensor");
         if (!aligned(q, 16) || !aligned(k, 16) || !aligned(acc, 4))
             return ctx_fail(ctx, kInvalid, "q and k must be 16-byte aligned");
-        if (n_tok < 1 || kv_len < n_tok || kv_len > c.max_ctx) return ctx_fail(ctx, kInvalid, "bad kv_len / n_tok");
+        if (n_tok < 1 || kv_len < n_tok || kv_len > std::min(c.max_ctx, kMaxRows))
+            return ctx_fail(ctx, kInvalid, "bad kv_len / n_tok");
         if (row_begin < 0 || row_begin >= n_tok) return ctx_fail(ctx, kInvalid, "row_begin must lie in [0, n_tok)");
         if (accumulate != 0 && accumulate != 1) return ctx_fail(ctx, kInvalid, "accumulate must be 0 or 1");
         if (acc_stride < kv_len) return ctx_fail(ctx, kInvalid, "acc_stride smaller than kv_len");
@@ -258,7 +264,7 @@ int32_t ep_sp_prompt_weights(ep_sp_ctx* ctx, int32_t layer, const void* q, const
 }
 
 int32_t ep_sp_evict_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_len, int32_t n_keep, size_t* bytes) {
-    if (!ctx || !bytes || n_seq < 1 || n_seq > 65535 || max_kv_len < 1 || max_kv_len > ctx->cfg.max_ctx ||
+    if (!ctx || !bytes || n_seq < 1 || n_seq > 65535 || max_kv_len < 1 || max_kv_len > std::min(ctx->cfg.max_ctx, kMaxRows) ||
         n_keep < 1 || n_keep > ctx->cfg.max_ctx)
         return kInvalid;
     *bytes = epsp::evict_ws_bytes(n_seq, max_kv_len, n_keep, ctx->cfg.n_head_kv);

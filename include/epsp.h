@@ -452,7 +452,7 @@ int32_t ep_sp_ffn_scatter(ep_sp_ctx* ctx, int32_t layer, const void* ffn_out, vo
  * (NaN too).  Two sequences may share blocks that no call writes. */
 typedef struct ep_sp_kv_batch {
     int32_t n_seq;
-    int32_t max_kv_len;          /* 1..max_ctx */
+    int32_t max_kv_len;          /* 1..max_ctx, under 2^31 - 65536 */
     const int32_t* kv_lens;      /* DEVICE [n_seq] */
     const int32_t* block_tables; /* DEVICE [n_seq][table_stride] block ids */
     int32_t table_stride;
