@@ -19,7 +19,6 @@ namespace {
 
 constexpr int32_t kOk = 0;
 constexpr int32_t kInvalid = static_cast<int32_t>(ErrorCode::InvalidArgument);
-constexpr int32_t kUnsupported = static_cast<int32_t>(ErrorCode::Unsupported);
 constexpr int32_t kInternal = static_cast<int32_t>(ErrorCode::Internal);
 
 // Families of ep_sp_profile_read_families.
@@ -68,7 +67,6 @@ int32_t launch(ep_sp_ctx* c, Family f, void* stream, const char* what, F&& go) {
     void* ev = ctx_profile_begin(c, f, stream);
     const cudaError_t e = go();
     ctx_profile_end(c, f, ev, stream);
-    if (e == cudaErrorNotSupported) return ctx_fail(c, kUnsupported, std::string(what) + ": shape not supported");
     if (e != cudaSuccess) return ctx_fail(c, kInternal, std::string(what) + ": " + cudaGetErrorString(e));
     return kOk;
 }
