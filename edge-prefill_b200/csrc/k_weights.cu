@@ -6,8 +6,8 @@
 // (maximum, sum) per key split, k7_join its lse, the sums pass each key's sum.
 // Storing the scores instead would cost 8 bytes a pair; recomputing them costs
 // 2 d flops, which the tensor cores do in a quarter of the time the pair's two
-// exponentials take.  The exponentials bound both passes (16 MUFU results per
-// clock and SM, a fifth of the pairs on the FMA pipe instead).  Every key has one
+// exponentials take.  Those take most of both passes (16 MUFU results per clock
+// and SM, a fifth of the pairs on the FMA pipe instead).  Every key has one
 // writer (k7_add where the rows are split) and a fixed order of additions.
 //
 // 16-bit (tcgen05): a query tile packs T = 128 / G tokens x G heads into 128
@@ -211,9 +211,9 @@ __device__ __forceinline__ void give_back(uint64_t* se, int lane) {
 // give one key.  Rows of a tile that are none are zeros with an lse of -inf:
 // they add nothing to a finite key, but 0 * inf to one with an infinity.  A NaN
 // sum of a tile that has such rows is therefore taken again, here, without
-// them; `lse`: minus the tile's lse.  (In line and in loops that stay loops: as
-// a call, 64 rows of 32 heads over 64K keys 114 us, so 107, without it 107;
-// masking the columns in every step instead 114 to 117.)
+// them; `lse`: minus the tile's lse.  (In line and in loops that stay loops, 64
+// rows of 32 heads over 64K keys 107.2 us, 107.0 without it; as a call 3 % more,
+// with the columns masked in every step 4 to 6 %.)
 template <bool BF16, int D>
 __device__ __forceinline__ float weigh_again(const WeightArgs& a, const float* lse, int c0, int c1, int tok0, int h, int key) {
     const int G = a.n_head / a.n_head_kv, at = a.kv_len - a.n_tok + a.row_begin + tok0;  // cache row of the first token
@@ -257,9 +257,10 @@ __device__ __forceinline__ float weigh_again(const WeightArgs& a, const float* l
 // stream otherwise.
 // A step is one (query tile, key tile); three pairs of warpgroups, an S buffer
 // each, take the steps in turn, each warpgroup 64 of the 128 columns, 32 at a
-// time (the buffer goes back to the MMA warp halfway).  Issue slots and MUFU
-// together bound it: 24 warps hide more of each other than 16 with 64 columns in registers (96 against 101 us for 64
-// rows of 32 heads over 64K keys), a warpgroup per step measured 99 us.
+// time (the buffer goes back to the MMA warp halfway).  MUFU (57 to 68 %) and
+// the issue slots (53 to 56 %) are the busiest units: 24 warps hide more of each
+// other's waits than 16 with 64 columns in registers (96 against 101 us for 64
+// rows of 32 heads over 64K keys); a warpgroup per step measured 99 us.
 // STREAM: the sums pass whose query tiles stream.
 template <bool BF16, int D, int SEG, int PASS, bool STREAM>
 __global__ void __launch_bounds__(kTcThreads, 1)
