@@ -1,0 +1,84 @@
+// cache8.cuh -- the arithmetic of the 8-bit cache, one place for every kernel
+// that writes it.
+//
+// A page's scale is 2^e, e the least integer with amax <= M 2^e (M = 448 for
+// e4m3, 127 for integers) and at least -100, and a value's byte the nearest to
+// x / 2^e, ties to even.  A power of two costs e4m3 nothing (its steps are
+// relative), half a bit of an integer's on average; it makes x / s exact, so
+// that the rounding to 8 bits is the only one, that every order of the same
+// work gives the same bytes, and that a page whose scale grows under appended
+// rows loses only what falls below the new last place.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cstdint>
+
+#include "epsp_kernels.h"
+
+namespace epsp {
+namespace {
+
+constexpr int kLeastExp8 = -100;  // exponent of the smallest scale
+
+// Scale of a page whose largest finite magnitude has these f32 bits.
+template <bool I8>
+__device__ __forceinline__ float scale8(uint32_t amax_bits) {
+    constexpr uint32_t top = I8 ? 0x42fe0000u : 0x43e00000u;  // 127, 448
+    // both are m 2^x with x = 6, 8: the exponents' difference, one more where amax's mantissa is the larger
+    const int e = (int)(amax_bits >> 23) - (int)(top >> 23) + ((amax_bits & 0x7fffffu) > (top & 0x7fffffu) ? 1 : 0);
+    return __uint_as_float((uint32_t)(max(e, kLeastExp8) + 127) << 23);
+}
+
+// 1 / s where that is exact (a power of two), else 0.
+__device__ __forceinline__ float exact_inverse(float s) {
+    const uint32_t b = __float_as_uint(s), e = b >> 23;
+    return (b & 0x7fffffu) == 0 && e >= 1 && e <= 253 ? __uint_as_float((254 - e) << 23) : 0.f;
+}
+
+// Four values, already divided by their scale, to bytes.  An infinity becomes
+// the largest magnitude, a NaN 0 (both are reported by the caller).
+template <bool I8>
+__device__ __forceinline__ uint32_t to8(float x0, float x1, float x2, float x3) {
+    if constexpr (I8) {
+        auto q = [](float x) { return (uint32_t)__float2int_rn(fminf(fmaxf(x == x ? x : 0.f, -127.f), 127.f)) & 0xffu; };
+        return q(x0) | q(x1) << 8 | q(x2) << 16 | q(x3) << 24;
+    } else {
+        auto n = [](float x) { return x == x ? x : 0.f; };
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(n(x0), n(x1)), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(n(x2), n(x3)), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
+    }
+}
+
+// Four bytes to the numbers they hold, exactly.
+template <bool I8>
+__device__ __forceinline__ void from8(uint32_t w, float (&x)[4]) {
+    if constexpr (I8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
+            const float2 f = __half22float2(__half2(h));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+}
+
+// x / s: by its exact inverse where it has one.
+__device__ __forceinline__ float over(float x, float s, float inv) { return inv != 0.f ? x * inv : x / s; }
+
+// f32 bits of |x| where x is finite, else 0; `odd` is set where it is not.
+__device__ __forceinline__ uint32_t magnitude(float x, bool& odd) {
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    if (b < 0x7f800000u) return b;
+    odd = true;
+    return 0;
+}
+
+}  // namespace
+}  // namespace epsp

@@ -24,8 +24,11 @@ enum DeviceError : int32_t {
     kDevWaitPoolProducer = 0x107,  // K1's producer waited too long for a free stage
     kDevBadSelection = 0x201,
     kDevF16Range = 0x301,      // an f32 input is outside the f16 range of the tensor-core mode
+    kDevNotFinite8 = 0x302,    // a row that went into an 8-bit cache held an infinity or a NaN
     kDevBadBlockTable = 0x401, // a paged-KV block table entry lies outside the pool
     kDevBadLength = 0x501,     // a sequence length of a batch lies outside [0, max_kv_len]
+    kDevBadParent = 0x502,     // a fork's parent or length lies outside what there is
+    kDevNoBlocks = 0x503,      // the pool has fewer free blocks than a resize needs
     kDevWaitDecode = 0x601,    // a decode KV unit did not arrive (or leave) in time
     kDevWaitWeights = 0x602,   // a prompt-weight tile did not arrive (or leave) in time
 };
@@ -332,6 +335,72 @@ struct EvictArgs {
 };
 size_t evict_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_keep, int32_t n_head_kv);
 cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s);
+
+// ---------------------------------------------------------------------------
+// The cache in 8 bits: per page (page_size rows of one sequence) and KV head one
+// scale, a value is its byte (e4m3 or a signed integer) times the scale.
+struct Cache8 {
+    int32_t i8 = 0;            // 0 e4m3, 1 signed integers
+    int32_t page_size = 0;
+    uint8_t* k = nullptr;      // cache rows [rows][Hkv][d]
+    uint8_t* v = nullptr;
+    float* k_scale = nullptr;  // [rows / page_size][Hkv]
+    float* v_scale = nullptr;
+};
+
+// Rows [first[s], src.lens[s]) of each sequence from one cache to the same rows
+// of the other: pack from k / v (src) into the 8-bit cache (dst), unpack back.
+struct PackArgs {
+    BatchKv src, dst;      // dst.lens unused
+    const int32_t* first;  // [n_seq] or null: 0
+    const void* k;         // pack: read; unpack: written
+    const void* v;
+    Cache8 c;
+    int32_t dtype, n_head_kv, head_dim;
+    int32_t* err;
+};
+cudaError_t launch_pack(const PackArgs& a, cudaStream_t s);
+cudaError_t launch_unpack(const PackArgs& a, cudaStream_t s);
+
+// One token's K and V row per sequence into row lens[s] - 1 of the 8-bit cache.
+struct AppendArgs {
+    BatchKv kv;
+    const void* k_new;  // [n_seq][Hkv][d]
+    const void* v_new;
+    Cache8 c;
+    int32_t dtype, n_head_kv, head_dim;
+    int32_t* err;
+};
+cudaError_t launch_append8(const AppendArgs& a, cudaStream_t s);
+
+// Attention of one token per sequence over an 8-bit cache (a.k / a.v / a.acc are
+// not used; k_new / v_new are quantised into the cache first).
+size_t decode8_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                        int32_t dtype);
+cudaError_t launch_decode8(const DecodeArgs& a, const Cache8& c, cudaStream_t s);
+
+// ---------------------------------------------------------------------------
+// Blocks of paged caches, held by sequences.
+struct PagesArgs {
+    int32_t n_seq, table_stride, block_rows, pool_blocks;
+    int32_t* lens;    // [n_seq]
+    int32_t* tables;  // [n_seq][table_stride]
+    int32_t* refs;    // [pool_blocks]
+    int32_t* err;
+};
+struct Pool {
+    void* rows;          // [pool_blocks][bytes]
+    size_t bytes;        // of a block, a multiple of 4
+};
+cudaError_t launch_count_refs(const PagesArgs& a, cudaStream_t s);
+size_t fork_ws_bytes(const PagesArgs& a);
+cudaError_t launch_fork(const PagesArgs& a, const int32_t* parents, const int32_t* lens, void* ws, cudaStream_t s);
+size_t resize_ws_bytes(const PagesArgs& a);
+cudaError_t launch_resize(const PagesArgs& a, const int32_t* new_lens, const Pool* pools, int32_t n_pools, void* ws,
+                          cudaStream_t s);
+size_t compact_ws_bytes(const PagesArgs& a);
+cudaError_t launch_compact(const PagesArgs& a, const Pool* pools, int32_t n_pools, int32_t* n_used, void* ws,
+                           cudaStream_t s);
 
 // Reads and clears the device error word of the no-allocation selection path
 // on the current device (0 when that device never ran it).

@@ -430,9 +430,16 @@ int32_t ep_sp_sync_status(ep_sp_ctx* ctx, void* stream) {
             return fail(ctx, kUnsupported,
                         "an f32 input lies outside the f16 range of the tensor-core mode (ep_sp_set_f32_attention 0 "
                         "attends it in f32)");
+        if (err == epsp::kDevNotFinite8)
+            return fail(ctx, kUnsupported,
+                        "a row that went into an 8-bit cache held an infinity (kept as the largest magnitude) or a NaN "
+                        "(kept as 0)");
+        if (err == epsp::kDevNoBlocks)
+            return fail(ctx, kOom, "a resize needed " + std::to_string(rec[3]) +
+                                       " more free blocks than the pool had; it changed nothing");
         char buf[160];
         std::snprintf(buf, sizeof buf,
-                      "device error word 0x%x (bounded wait expired, bad selection, block table or length); where 0x%x, "
+                      "device error word 0x%x (bounded wait expired, bad selection, block table, length or parent); where 0x%x, "
                       "block %d, tile %d",
                       err, rec[1], rec[2], rec[3]);
         return fail(ctx, kPrefill, buf);
@@ -834,7 +841,7 @@ int32_t ep_sp_profile_enable(ep_sp_ctx* ctx, int32_t on) {
         ctx->event_pool.push_back(ev.stop);
     }
     ctx->events.clear();
-    for (int i = 0; i < EP_SP_NUM_FAMILIES; ++i) ctx->launches[i] = 0;
+    for (int64_t& n : ctx->launches) n = 0;
     ctx->profiling = on != 0;
     return kOk;
 }
@@ -853,6 +860,22 @@ int32_t ep_sp_profile_read_families(ep_sp_ctx* ctx, int32_t n, double* ms, int64
         e = cudaEventElapsedTime(&t, static_cast<cudaEvent_t>(ev.start), static_cast<cudaEvent_t>(ev.stop));
         if (e != cudaSuccess) return cuda_fail(ctx, e, "profile elapsed");
         ms[ev.kind] += t;
+    }
+    return kOk;
+}
+
+int32_t ep_sp_profile_read_family(ep_sp_ctx* ctx, int32_t family, double* ms, int64_t* launches) {
+    if (!ctx || !ms || !launches || family < 0 || family > EP_SP_FAMILY_PAGES) return kInvalid;
+    *ms = 0.0;
+    *launches = ctx->launches[family];
+    for (auto& ev : ctx->events) {
+        if (ev.kind != family) continue;
+        cudaError_t e = cudaEventSynchronize(static_cast<cudaEvent_t>(ev.stop));
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "profile event");
+        float t = 0.f;
+        e = cudaEventElapsedTime(&t, static_cast<cudaEvent_t>(ev.start), static_cast<cudaEvent_t>(ev.stop));
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "profile elapsed");
+        *ms += t;
     }
     return kOk;
 }

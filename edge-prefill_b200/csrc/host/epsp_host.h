@@ -157,7 +157,7 @@ struct ep_sp_ctx {
     };
     std::vector<Ev> events;       // recorded since the last enable
     std::vector<void*> event_pool;
-    int64_t launches[EP_SP_NUM_FAMILIES] = {};
+    int64_t launches[EP_SP_FAMILY_PAGES + 1] = {};
 
     // head-parallel output exchange (ep_sp_xchg_*)
     void* xchg_base = nullptr;            // this rank's buffer: [header][slots]

@@ -1,0 +1,341 @@
+// k_pack8.cu -- K9: rows into the 8-bit cache and out of it.
+//
+//   pack    q = round8(x / s), s = scale of the page's rows and KV head
+//   unpack  x = q s
+//   append  one token's row per sequence (before K10 attends it)
+//
+// Every element is read once and written once: memory bounds them.
+//
+// pack: a CTA takes the rows of one page and KV head, of K or of V, into
+// registers (16 bytes a load, all in flight before the first is used), so that
+// the maximum and the bytes come from one read.  The CTAs of a page's heads
+// follow one another, so the whole rows of the source are read at about one
+// time.  A page that holds rows before `first` keeps its scale, or has it grown
+// and those rows' bytes follow, by the same CTA.
+// unpack: 16 bytes a thread, four times, in the order they lie in.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "cache8.cuh"
+#include "epsp_kernels.h"
+#include "tc100.cuh"
+
+namespace epsp {
+namespace {
+
+constexpr int kThreads = 256;
+
+// The 4 values of 8 bytes (16-bit types) or 16 bytes (f32).
+template <int ET>
+__device__ __forceinline__ void values4(const uint32_t* w, float (&x)[4]) {
+    if constexpr (ET == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    } else if constexpr (ET == 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+}
+
+// Rows [first, len) of a sequence; an empty range where `first` is none.
+__device__ __forceinline__ int2 span_of(const PackArgs& a, int s) {
+    const int n = batch_len(a.src, s, a.err), f = a.first ? a.first[s] : 0;
+    if (f < 0 || f > n) {
+        report_error(a.err, kDevBadLength, 0x92, s);
+        return make_int2(0, 0);
+    }
+    return make_int2(f, n);
+}
+
+// Largest of the CTA's values, and whether any thread saw something odd.
+__device__ __forceinline__ uint32_t cta_max(uint32_t m, bool& odd, uint32_t* box) {
+    m = __reduce_max_sync(0xffffffffu, m);
+    const bool any = __any_sync(0xffffffffu, odd);
+    if ((threadIdx.x & 31) == 0) box[threadIdx.x >> 5] = m | (any ? 0x80000000u : 0u);
+    __syncthreads();
+    m = 0;
+    odd = false;
+    for (int i = 0; i < (int)blockDim.x / 32; ++i) {
+        odd |= (box[i] & 0x80000000u) != 0;
+        m = max(m, box[i] & 0x7fffffffu);
+    }
+    __syncthreads();  // (the box is written again)
+    return m;
+}
+
+// The bytes of rows [0, rows) of one head at `p` follow their page's scale from
+// `was` to `s`.
+template <bool I8>
+__device__ __forceinline__ void rescale(uint8_t* p, int64_t stride, int rows, int d, float was, float s) {
+    const float f = was / s;
+    for (int i = threadIdx.x; i < rows * (d / 4); i += blockDim.x) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(p + (int64_t)(i / (d / 4)) * stride) + i % (d / 4);
+        float x[4];
+        from8<I8>(*w, x);
+        *w = to8<I8>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+    }
+}
+
+// C: 16-byte chunks of a page and head per thread.
+template <int ET, bool I8, int C>
+__global__ void __launch_bounds__(kThreads) k9_pack(const PackArgs a) {
+    constexpr int kEs = ET == 0 ? 4 : 2, kPer = 16 / kEs;
+    __shared__ uint32_t box[kThreads / 32];
+    __shared__ int2 span_s;
+    tc::pdl_wait();
+    tc::pdl_launch();
+    const int s = blockIdx.y, P = a.c.page_size, d = a.head_dim, Hkv = a.n_head_kv;
+    if (threadIdx.x == 0) span_s = span_of(a, s);
+    __syncthreads();
+    const int f = span_s.x, n = span_s.y;
+    if (f >= n) return;
+    const int p0 = f / P;
+    const int64_t tiles = (int64_t)((n + P - 1) / P - p0) * Hkv * 2;
+    const int lg = __ffs(d * kEs / 16) - 1;  // chunks per row, a power of two
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const bool is_v = t & 1;
+        const int h = (int)((t >> 1) % Hkv), r0 = (p0 + (int)((t >> 1) / Hkv)) * P;
+        const int lo = max(f, r0) - r0, hi = min(n - r0, P);  // rows of the page to write
+        const int from = batch_row(a.src, s, r0, a.err), to = batch_row(a.dst, s, r0, a.err);
+        const bool there = from >= 0 && to >= 0;
+        const char* src = static_cast<const char*>(is_v ? a.v : a.k) + ((int64_t)from * Hkv + h) * d * kEs;
+        uint8_t* dst = (is_v ? a.c.v : a.c.k) + ((int64_t)to * Hkv + h) * d;
+        float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + (int64_t)(to / P) * Hkv + h;
+        uint4 v[C];
+        uint32_t m = 0;
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const int i = threadIdx.x + j * kThreads, r = i >> lg, c = i & ((1 << lg) - 1);
+            v[j] = make_uint4(0, 0, 0, 0);
+            if (there && r >= lo && r < hi)
+                v[j] = __ldcs(reinterpret_cast<const uint4*>(src + (int64_t)r * Hkv * d * kEs + c * 16));
+        }
+        const float was = there && lo > 0 ? *scale : 0.f;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[j]);
+#pragma unroll
+            for (int e = 0; e < kPer / 4; ++e) {
+                float x[4];
+                values4<ET>(w + 2 * e, x);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) m = max(m, magnitude(x[i], odd));
+            }
+        }
+        m = cta_max(m, odd, box);
+        if (!there) continue;
+        // (the values are made from the rows again, not held: twice the registers)
+#pragma unroll
+        for (int j = 0; j < C; ++j) asm volatile("" : "+r"(v[j].x), "+r"(v[j].y), "+r"(v[j].z), "+r"(v[j].w));
+        if (odd && threadIdx.x == 0) report_error(a.err, kDevNotFinite8, 0x93, r0 / P);
+        float sc = scale8<I8>(m);
+        if (was >= sc) sc = was;
+        else {
+            if (lo > 0) rescale<I8>(dst, (int64_t)Hkv * d, lo, d, was, sc);
+            if (threadIdx.x == 0) *scale = sc;
+        }
+        const float inv = exact_inverse(sc);
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const int i = threadIdx.x + j * kThreads, r = i >> lg, c = i & ((1 << lg) - 1);
+            if (r < lo || r >= hi) continue;
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[j]);
+            uint32_t q[kPer / 4];
+#pragma unroll
+            for (int e = 0; e < kPer / 4; ++e) {
+                float x[4];
+                values4<ET>(w + 2 * e, x);
+                q[e] = to8<I8>(over(x[0], sc, inv), over(x[1], sc, inv), over(x[2], sc, inv), over(x[3], sc, inv));
+            }
+            uint8_t* o = dst + (int64_t)r * Hkv * d + c * kPer;
+            if constexpr (kPer == 8) *reinterpret_cast<uint2*>(o) = make_uint2(q[0], q[1]);
+            else *reinterpret_cast<uint32_t*>(o) = q[0];
+        }
+    }
+}
+
+constexpr int kUnpack = 4;  // 16-byte chunks of the 8-bit cache per thread and turn
+
+template <int ET, bool I8>
+__global__ void __launch_bounds__(kThreads) k9_unpack(const PackArgs a) {
+    tc::pdl_wait();
+    tc::pdl_launch();
+    const int s = blockIdx.y, P = a.c.page_size, d = a.head_dim, Hkv = a.n_head_kv;
+    const int2 span = span_of(a, s);
+    const int f = span.x, n = span.y, per_row = Hkv * d / 16;
+    const int64_t end = (int64_t)n * per_row;
+    for (int64_t t = (int64_t)f * per_row + (int64_t)blockIdx.x * kThreads * kUnpack + threadIdx.x; t < end;
+         t += (int64_t)gridDim.x * kThreads * kUnpack) {
+        uint4 q[2][kUnpack];
+        float sc[2][kUnpack];
+        int64_t to[kUnpack];  // element in the destination, -1: none
+#pragma unroll
+        for (int j = 0; j < kUnpack; ++j) {
+            const int64_t i = t + j * kThreads;
+            to[j] = -1;
+            if (i >= end) continue;
+            const int r = (int)(i / per_row), c = (int)(i - (int64_t)r * per_row);
+            const int from = batch_row(a.src, s, r, a.err), row = batch_row(a.dst, s, r, a.err);
+            if (from < 0 || row < 0) continue;
+            to[j] = ((int64_t)row * per_row + c) * 16;
+            const int64_t at = (int64_t)from * per_row + c, page = (int64_t)(from / P) * Hkv + c / (d / 16);
+            q[0][j] = __ldcs(reinterpret_cast<const uint4*>(a.c.k) + at);
+            q[1][j] = __ldcs(reinterpret_cast<const uint4*>(a.c.v) + at);
+            sc[0][j] = a.c.k_scale[page];
+            sc[1][j] = a.c.v_scale[page];
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int j = 0; j < kUnpack; ++j) {
+                if (to[j] < 0) continue;
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(&q[kv][j]);
+                void* out = const_cast<void*>(kv ? a.v : a.k);
+                uint32_t o[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x[4];
+                    from8<I8>(w[e], x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] *= sc[kv][j];
+                    if constexpr (ET == 0) {
+                        reinterpret_cast<float4*>(static_cast<float*>(out) + to[j])[e] = make_float4(x[0], x[1], x[2], x[3]);
+                    } else if constexpr (ET == 1) {
+                        const __half2 p = __floats2half2_rn(x[0], x[1]), r = __floats2half2_rn(x[2], x[3]);
+                        o[2 * e] = *reinterpret_cast<const uint32_t*>(&p);
+                        o[2 * e + 1] = *reinterpret_cast<const uint32_t*>(&r);
+                    } else {
+                        const __nv_bfloat162 p = __floats2bfloat162_rn(x[0], x[1]), r = __floats2bfloat162_rn(x[2], x[3]);
+                        o[2 * e] = *reinterpret_cast<const uint32_t*>(&p);
+                        o[2 * e + 1] = *reinterpret_cast<const uint32_t*>(&r);
+                    }
+                }
+                if constexpr (ET != 0) {
+                    uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + to[j]);
+                    p[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                    p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+                }
+            }
+    }
+}
+
+// One CTA of 128 threads per (sequence, KV head, K or V), an element per thread.
+// Latency bounds it: the length, then the block table, then the page's scale.
+template <int ET, bool I8>
+__global__ void __launch_bounds__(128) k9_append(const AppendArgs a) {
+    __shared__ uint32_t box[4];
+    __shared__ int n_s;
+    tc::pdl_wait();
+    tc::pdl_launch();
+    const int P = a.c.page_size, d = a.head_dim, Hkv = a.n_head_kv;
+    const bool is_v = blockIdx.x & 1;
+    const int s = (int)(blockIdx.x >> 1) / Hkv, h = (int)(blockIdx.x >> 1) % Hkv, t = threadIdx.x;
+    float x = 0.f;
+    if (t < d) {
+        const int64_t i = ((int64_t)s * Hkv + h) * d + t;
+        const void* src = is_v ? a.v_new : a.k_new;
+        if constexpr (ET == 0) x = static_cast<const float*>(src)[i];
+        else if constexpr (ET == 1) x = __half2float(static_cast<const __half*>(src)[i]);
+        else x = __bfloat162float(static_cast<const __nv_bfloat16*>(src)[i]);
+    }
+    if (t == 0) n_s = batch_len(a.kv, s, a.err);
+    __syncthreads();
+    const int n = n_s;
+    if (n == 0) return;
+    const int r0 = (n - 1) / P * P, lo = n - 1 - r0;
+    const int row = batch_row(a.kv, s, r0, a.err);
+    bool odd = false;
+    uint32_t m = magnitude(x, odd);
+    float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + (int64_t)(max(row, 0) / P) * Hkv + h;
+    const float was = row >= 0 && lo > 0 ? *scale : 0.f;
+    m = cta_max(m, odd, box);
+    if (row < 0) return;
+    if (odd && t == 0) report_error(a.err, kDevNotFinite8, 0x94, s);
+    uint8_t* dst = (is_v ? a.c.v : a.c.k) + ((int64_t)row * Hkv + h) * d;
+    float sc = scale8<I8>(m);
+    if (was >= sc) sc = was;
+    else {
+        if (lo > 0) rescale<I8>(dst, (int64_t)Hkv * d, lo, d, was, sc);
+        if (t == 0) *scale = sc;
+    }
+    if (t < d) dst[(int64_t)lo * Hkv * d + t] = (uint8_t)to8<I8>(over(x, sc, exact_inverse(sc)), 0.f, 0.f, 0.f);
+}
+
+// Kernels here may start before what precedes them on the stream has ended:
+// they wait for it on the device.
+template <class... P, class... A>
+cudaError_t go(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t s, A... args) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// CTAs for `work` pieces per sequence: more than the device holds at once do
+// not help.
+unsigned grid_x(int64_t work, int32_t n_seq) {
+    const int64_t most = std::max<int64_t>(1, 148 * 64 / n_seq);
+    return (unsigned)std::min(work, most);
+}
+
+template <int ET, bool I8>
+cudaError_t pack_t(const PackArgs& a, cudaStream_t s) {
+    const int64_t pages = (a.src.max_kv_len + (int64_t)a.c.page_size - 1) / a.c.page_size;
+    const dim3 grid(grid_x(pages * a.n_head_kv * 2, a.src.n_seq), a.src.n_seq);
+    const int chunks = a.c.page_size * a.head_dim * (ET == 0 ? 4 : 2) / (16 * kThreads);
+    switch (chunks) {
+        case 1: return go(k9_pack<ET, I8, 1>, grid, kThreads, s, a);
+        case 2: return go(k9_pack<ET, I8, 2>, grid, kThreads, s, a);
+        case 4: return go(k9_pack<ET, I8, 4>, grid, kThreads, s, a);
+        case 8: return go(k9_pack<ET, I8, 8>, grid, kThreads, s, a);
+        default: return go(k9_pack<ET, I8, 16>, grid, kThreads, s, a);
+    }
+}
+
+template <int ET, bool I8>
+cudaError_t unpack_t(const PackArgs& a, cudaStream_t s) {
+    const int64_t chunks = (int64_t)a.src.max_kv_len * a.n_head_kv * a.head_dim / 16;
+    const dim3 grid(grid_x((chunks + kThreads * kUnpack - 1) / (kThreads * kUnpack), a.src.n_seq), a.src.n_seq);
+    return go(k9_unpack<ET, I8>, grid, kThreads, s, a);
+}
+
+template <int ET, bool I8>
+cudaError_t append_t(const AppendArgs& a, cudaStream_t s) {
+    const int64_t ctas = (int64_t)a.kv.n_seq * a.n_head_kv * 2;
+    if (ctas > INT_MAX) return cudaErrorInvalidValue;
+    return go(k9_append<ET, I8>, dim3((unsigned)ctas), 128, s, a);
+}
+
+#define EPSP_BY_TYPES(fn, a, s)                                             \
+    switch ((a).dtype) {                                                    \
+        case 0: return (a).c.i8 ? fn<0, true>(a, s) : fn<0, false>(a, s);   \
+        case 1: return (a).c.i8 ? fn<1, true>(a, s) : fn<1, false>(a, s);   \
+        default: return (a).c.i8 ? fn<2, true>(a, s) : fn<2, false>(a, s);  \
+    }
+
+}  // namespace
+
+cudaError_t launch_pack(const PackArgs& a, cudaStream_t s) { EPSP_BY_TYPES(pack_t, a, s) }
+cudaError_t launch_unpack(const PackArgs& a, cudaStream_t s) { EPSP_BY_TYPES(unpack_t, a, s) }
+cudaError_t launch_append8(const AppendArgs& a, cudaStream_t s) { EPSP_BY_TYPES(append_t, a, s) }
+
+}  // namespace epsp

@@ -113,6 +113,15 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                  : "memory");
 }
 
+// 4 bytes of global memory into this CTA's shared memory; copies_arrive arrives
+// once on `bar` when this thread's copies so far have landed.
+__device__ __forceinline__ void copy4_async(void* smem_dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem_dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // Programmatic dependent launch: what the kernels before this one on the
 // stream wrote may be read, and written over, after pdl_wait; pdl_launch lets
 // the next kernel's CTAs start (up to their own pdl_wait).

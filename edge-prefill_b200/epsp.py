@@ -18,6 +18,7 @@ LIB_PATH = os.environ.get("EPSP_LIB") or os.path.join(HERE, "libepsp.so")
 
 OK, INVALID_ARGUMENT, PREFILL, UNSUPPORTED, OUT_OF_MEMORY, IO, INTERNAL, UNAVAILABLE = 0, 2, 6, 9, 10, 11, 12, 13
 F32, F16, BF16 = 0, 1, 2
+E4M3, I8 = 3, 4  # of an 8-bit cache
 
 # Every symbol include/epsp.h declares.
 EXPORTS = [
@@ -35,12 +36,16 @@ EXPORTS = [
     "ep_sp_get_head_routing", "ep_sp_set_paged_kv", "ep_sp_xchg_attach_buffers", "ep_sp_xchg_bytes",
     "ep_sp_decode_bytes", "ep_sp_decode_layer", "ep_sp_prompt_weights_bytes", "ep_sp_prompt_weights",
     "ep_sp_evict_bytes", "ep_sp_evict_layer", "ep_sp_profile_read_families",
+    "ep_sp_pack_kv", "ep_sp_unpack_kv", "ep_sp_decode8_bytes", "ep_sp_decode8_layer", "ep_sp_count_refs",
+    "ep_sp_fork_bytes", "ep_sp_fork_seqs", "ep_sp_resize_bytes", "ep_sp_resize_seqs", "ep_sp_compact_bytes",
+    "ep_sp_compact_pool", "ep_sp_profile_read_family",
 ]
 NUM_KERNELS = 6  # EP_SP_NUM_KERNELS
 KERNEL_NAMES = ["k1_pool_pages", "k2_select_pages", "k3_sparse_attention", "k4_compact", "k4_scatter",
                 "k5_exchange_wait"]
 NUM_FAMILIES = 9  # EP_SP_NUM_FAMILIES
 FAMILY_NAMES = KERNEL_NAMES + ["k6_decode", "k7_prompt_weights", "k8_evict"]
+FAMILY_PACK, FAMILY_PAGES = 9, 10  # of profile_family alone
 XCHG_HANDLE_BYTES = 64
 
 
@@ -73,6 +78,27 @@ class KvBatchDesc(ctypes.Structure):
         ("n_seq", c_int32), ("max_kv_len", c_int32), ("kv_lens", c_void_p), ("block_tables", c_void_p),
         ("table_stride", c_int32), ("block_rows", c_int32), ("pool_rows", c_int32), ("seq_rows", c_int32),
     ]
+
+
+class Kv8Desc(ctypes.Structure):
+    """ep_sp_kv8."""
+
+    _fields_ = [("type", c_int32), ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p)]
+
+
+class PagesDesc(ctypes.Structure):
+    """ep_sp_pages."""
+
+    _fields_ = [
+        ("n_seq", c_int32), ("table_stride", c_int32), ("block_rows", c_int32), ("pool_blocks", c_int32),
+        ("kv_lens", c_void_p), ("block_tables", c_void_p), ("refs", c_void_p),
+    ]
+
+
+class PoolDesc(ctypes.Structure):
+    """ep_sp_pool."""
+
+    _fields_ = [("rows", c_void_p), ("block_bytes", c_size_t)]
 
 
 def _load() -> ctypes.CDLL:
@@ -149,6 +175,21 @@ def _load() -> ctypes.CDLL:
         "ep_sp_evict_layer": (c_int32, [P, c_int32, POINTER(KvBatchDesc), P, P, P, c_int32, c_int32, c_int32, c_int32,
                                         POINTER(KvBatchDesc), P, P, P, c_int32, P, P, P, c_size_t, P]),
         "ep_sp_profile_read_families": (c_int32, [P, c_int32, POINTER(c_double), POINTER(ctypes.c_int64)]),
+        "ep_sp_profile_read_family": (c_int32, [P, c_int32, POINTER(c_double), POINTER(ctypes.c_int64)]),
+        "ep_sp_pack_kv": (c_int32, [P, c_int32, POINTER(KvBatchDesc), P, P, P, POINTER(KvBatchDesc), POINTER(Kv8Desc),
+                                    P]),
+        "ep_sp_unpack_kv": (c_int32, [P, c_int32, POINTER(KvBatchDesc), POINTER(Kv8Desc), P, POINTER(KvBatchDesc), P, P,
+                                      P]),
+        "ep_sp_decode8_bytes": (c_int32, [P, c_int32, c_int32, POINTER(c_size_t)]),
+        "ep_sp_decode8_layer": (c_int32, [P, c_int32, POINTER(KvBatchDesc), P, P, P, POINTER(Kv8Desc), P, P, c_size_t,
+                                          P]),
+        "ep_sp_count_refs": (c_int32, [P, POINTER(PagesDesc), P]),
+        "ep_sp_fork_bytes": (c_int32, [P, POINTER(PagesDesc), POINTER(c_size_t)]),
+        "ep_sp_fork_seqs": (c_int32, [P, POINTER(PagesDesc), P, P, P, c_size_t, P]),
+        "ep_sp_resize_bytes": (c_int32, [P, POINTER(PagesDesc), POINTER(c_size_t)]),
+        "ep_sp_resize_seqs": (c_int32, [P, POINTER(PagesDesc), P, POINTER(PoolDesc), c_int32, P, c_size_t, P]),
+        "ep_sp_compact_bytes": (c_int32, [P, POINTER(PagesDesc), POINTER(c_size_t)]),
+        "ep_sp_compact_pool": (c_int32, [P, POINTER(PagesDesc), POINTER(PoolDesc), c_int32, P, P, c_size_t, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -266,6 +307,68 @@ class KvBatch:
         self.desc = KvBatchDesc(self.n_seq, max_kv_len, _ptr(kv_lens), _ptr(block_tables) if block_rows else None,
                                 entries, block_rows, pool_rows, seq_rows)
         self.ref = ctypes.byref(self.desc)
+
+
+def _code8(dtype):
+    import torch
+
+    code = {torch.float8_e4m3fn: E4M3, torch.int8: I8}.get(dtype)
+    if code is None:
+        raise ValueError(f"an 8-bit cache is torch.float8_e4m3fn or torch.int8, not {dtype}")
+    return code
+
+
+class Kv8:
+    """One layer's cache in 8 bits (ep_sp_kv8): k, v [rows][n_head_kv][head_dim] of torch.float8_e4m3fn or torch.int8,
+    k_scale, v_scale f32 [rows / page_size][n_head_kv].  Keeps its tensors alive."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.type, self.device = _code8(k.dtype), k.get_device()
+        if k.dim() != 3 or k_scale.dim() != 2 or k.shape[0] % max(1, k_scale.shape[0]):
+            raise ValueError("k is [rows][n_head_kv][head_dim], k_scale [rows / page_size][n_head_kv]")
+        _check("v", v, k.dtype, k.shape, self.device)
+        _check("k", k, k.dtype, k.shape, self.device)
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            _check(name, t, _dtype(F32), (k_scale.shape[0], k.shape[1]), self.device)
+        self.rows = k.shape[0]
+        self.page = self.rows // k_scale.shape[0] if k_scale.shape[0] else 0
+        self.desc = Kv8Desc(self.type, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self.ref = ctypes.byref(self.desc)
+
+
+class Pages:
+    """Sequences and the blocks they hold (ep_sp_pages): kv_lens int32 [n_seq], block_tables int32 [n_seq][entries],
+    refs int32 [pool_blocks], all on the device and rewritten by the calls.  Keeps its tensors alive."""
+
+    def __init__(self, kv_lens, block_tables, refs, block_rows):
+        i32, self.device = _dtype("i32"), kv_lens.get_device()
+        self.kv_lens, self.block_tables, self.refs, self.n_seq = kv_lens, block_tables, refs, kv_lens.shape[0]
+        _check("kv_lens", kv_lens, i32, (self.n_seq,), self.device)
+        _check("block_tables", block_tables, i32, (self.n_seq, block_tables.shape[-1]), self.device)
+        _check("refs", refs, i32, (refs.shape[0],), self.device)
+        self.blocks = refs.shape[0]
+        self.desc = PagesDesc(self.n_seq, block_tables.shape[1], block_rows, self.blocks, kv_lens.data_ptr(),
+                              block_tables.data_ptr(), refs.data_ptr())
+        self.ref = ctypes.byref(self.desc)
+
+
+class Pools:
+    """The pools that follow a set of block tables: tensors (K, V, scales, of any layers and types) whose storage is
+    [blocks][bytes of a block].  Keeps its tensors alive."""
+
+    def __init__(self, tensors, blocks):
+        self.tensors, self.blocks = list(tensors), blocks
+        if not self.tensors:
+            raise ValueError("no pools")
+        self.device = self.tensors[0].get_device()
+        self.desc = (PoolDesc * len(self.tensors))()
+        for i, t in enumerate(self.tensors):
+            if not t.is_contiguous() or t.get_device() != self.device:
+                raise ValueError(f"pool {i} must be contiguous and on the device of the others")
+            if t.nbytes == 0 or t.nbytes % (4 * blocks):
+                raise ValueError(f"pool {i} is not {blocks} blocks of whole 4-byte words")
+            self.desc[i] = PoolDesc(t.data_ptr(), t.nbytes // blocks)
 
 
 class Context:
@@ -542,6 +645,122 @@ class Context:
                                      n_keep, sink_rows, recent_rows, dst.ref, k_dst.data_ptr(), v_dst.data_ptr(),
                                      p_acc, wide_dst, p_lens, p_kept, ws, n,
                                      _current_stream(dev) if stream is None else self._stream(stream))
+
+    # ------------------------------------------------- the cache in 8 bits
+    def _cache8_tensors(self, kv, c8, what="the 8-bit cache"):
+        _, _, _, _, dev, _, heads, d = self._facts or self._fast()
+        if c8.device != dev or (kv.device is not None and kv.device != dev):
+            raise ValueError(f"{what} or its batch is not on cuda:{dev}")
+        if c8.k.shape[1:] != (heads, d):
+            raise ValueError(f"{what} has rows of shape {tuple(c8.k.shape[1:])}, not {(heads, d)}")
+        if c8.rows != c8.page * c8.k_scale.shape[0] or c8.page != self.cfg.page_size:
+            raise ValueError(f"{what} has {c8.k_scale.shape[0]} scales for {c8.rows} rows in pages of {self.cfg.page_size}")
+        if c8.rows < kv.rows:
+            raise ValueError(f"{what} holds fewer than the batch's {kv.rows} rows")
+
+    def _first(self, first, n_seq):
+        if first is None:
+            return None
+        _check("first", first, self._fast()[3], (n_seq,), self._fast()[4])
+        return first.data_ptr()
+
+    def pack_kv(self, layer, src, k, v, dst, cache, first=None, stream=None):
+        """Rows [first, src.kv_lens) of k, v (src: KvBatch) into cache (Kv8, laid out by dst: KvBatch)."""
+        self._cache_tensors(src, k, v)
+        self._cache8_tensors(dst, cache)
+        return lib.ep_sp_pack_kv(self.h, layer, src.ref, k.data_ptr(), v.data_ptr(), self._first(first, src.n_seq),
+                                 dst.ref, cache.ref, self._stream(stream))
+
+    def unpack_kv(self, layer, src, cache, dst, k, v, first=None, stream=None):
+        """Rows [first, src.kv_lens) of cache (Kv8, src: KvBatch) into k, v (dst: KvBatch)."""
+        self._cache8_tensors(src, cache)
+        self._cache_tensors(dst, k, v)
+        return lib.ep_sp_unpack_kv(self.h, layer, src.ref, cache.ref, self._first(first, src.n_seq), dst.ref,
+                                   k.data_ptr(), v.data_ptr(), self._stream(stream))
+
+    def decode8_bytes(self, n_seq, max_kv_len):
+        n = c_size_t()
+        self.check(lib.ep_sp_decode8_bytes(self.h, n_seq, max_kv_len, ctypes.byref(n)))
+        return n.value
+
+    def decode8_layer(self, layer, kv, q, cache, out, workspace, k_new=None, v_new=None, stream=None):
+        """decode_layer over a Kv8; k_new, v_new go into it first."""
+        dt, odt, _, _, dev, heads, kvh, d = self._facts or self._fast()
+        self._cache8_tensors(kv, cache)
+        n_seq = kv.n_seq
+        _check("q", q, dt, (n_seq, heads, d), dev)
+        _check("out", out, odt, (n_seq, heads, d), dev)
+        p_k, p_v = None, None
+        if k_new is not None:
+            _check("k_new", k_new, dt, (n_seq, kvh, d), dev)
+            p_k = k_new.data_ptr()
+        if v_new is not None:
+            _check("v_new", v_new, dt, (n_seq, kvh, d), dev)
+            p_v = v_new.data_ptr()
+        ws, n = self._workspace(workspace)
+        return lib.ep_sp_decode8_layer(self.h, layer, kv.ref, q.data_ptr(), p_k, p_v, cache.ref, out.data_ptr(), ws, n,
+                                       _current_stream(dev) if stream is None else self._stream(stream))
+
+    # --------------------------------------------- blocks of paged caches
+    def _pages(self, pages, pools=None):
+        dev = self._fast()[4]
+        if pages.device != dev or (pools is not None and pools.device != dev):
+            raise ValueError(f"the pages or pools are not on cuda:{dev}")
+        if pools is not None and pools.blocks != pages.blocks:
+            raise ValueError(f"the pools have {pools.blocks} blocks, the counts {pages.blocks}")
+
+    def _seq_ints(self, name, t, n_seq):
+        _check(name, t, self._fast()[3], (n_seq,), self._fast()[4])
+        return t.data_ptr()
+
+    def _bytes(self, fn, pages):
+        n = c_size_t()
+        rc = fn(self.h, pages.ref, ctypes.byref(n))
+        if rc != OK:
+            raise EpspError(rc, "pages")
+        return n.value
+
+    def count_refs(self, pages, stream=None):
+        self._pages(pages)
+        return lib.ep_sp_count_refs(self.h, pages.ref, self._stream(stream))
+
+    def fork_bytes(self, pages):
+        return self._bytes(lib.ep_sp_fork_bytes, pages)
+
+    def fork_seqs(self, pages, parents, workspace, lens=None, stream=None):
+        """parents int32 [n_seq] (-1: empty the sequence); lens int32 [n_seq] or None: all of the parent's rows."""
+        self._pages(pages)
+        ws, n = self._workspace(workspace)
+        return lib.ep_sp_fork_seqs(self.h, pages.ref, self._seq_ints("parents", parents, pages.n_seq),
+                                   None if lens is None else self._seq_ints("lens", lens, pages.n_seq), ws, n,
+                                   self._stream(stream))
+
+    def resize_bytes(self, pages):
+        return self._bytes(lib.ep_sp_resize_bytes, pages)
+
+    def resize_seqs(self, pages, new_lens, pools, workspace, stream=None):
+        """new_lens int32 [n_seq]; pools: Pools."""
+        self._pages(pages, pools)
+        ws, n = self._workspace(workspace)
+        return lib.ep_sp_resize_seqs(self.h, pages.ref, self._seq_ints("new_lens", new_lens, pages.n_seq), pools.desc,
+                                     len(pools.tensors), ws, n, self._stream(stream))
+
+    def compact_bytes(self, pages):
+        return self._bytes(lib.ep_sp_compact_bytes, pages)
+
+    def compact_pool(self, pages, pools, workspace, n_used=None, stream=None):
+        """n_used int32 [1] or None: receives the number of blocks in use."""
+        self._pages(pages, pools)
+        p_used = None if n_used is None else self._seq_ints("n_used", n_used, 1)
+        ws, n = self._workspace(workspace)
+        return lib.ep_sp_compact_pool(self.h, pages.ref, pools.desc, len(pools.tensors), p_used, ws, n,
+                                      self._stream(stream))
+
+    def profile_family(self, family):
+        """(milliseconds, launches) of one family since the last ep_sp_profile_enable."""
+        ms, n = c_double(), ctypes.c_int64()
+        self.check(lib.ep_sp_profile_read_family(self.h, family, ctypes.byref(ms), ctypes.byref(n)))
+        return ms.value, n.value
 
     def profile_families(self):
         """{family name: (milliseconds, launches)} since the last ep_sp_profile_enable."""

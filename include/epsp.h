@@ -540,12 +540,149 @@ int32_t ep_sp_evict_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* s
                           int32_t acc_dst_stride, int32_t* new_lens, int32_t* kept_rows, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The cache in 8 bits: half the bytes of a 16-bit one, which bound a decode
+ * step.  No reference counterpart.  The conventions of the calls above hold
+ * (batches, workspaces, capture, devices).
+ *
+ * k, v hold a byte per element in the layout of the batch's tensors; each page
+ * (page_size rows of a sequence; block_rows is a multiple of it, and without
+ * blocks seq_rows must be one here) has a scale per KV head in k_scale and
+ * v_scale, DEVICE [rows / page_size][n_head_kv] f32 with `rows` the tensors' row
+ * count, so the page of row x is x / page_size.  A value is byte * scale, the
+ * byte read as e4m3 or as a signed integer.
+ *
+ * The calls write scales 2^e with e the least integer for which the page's
+ * largest magnitude is at most M * 2^e (M = 448 for e4m3, 127 for integers) and
+ * at least -100, and bytes rounded to nearest, ties to even.  Rows written
+ * behind others of a page grow its scale where they need to; the bytes that
+ * were there are then rounded again to the new one.  Scales of rows that these
+ * calls read must be positive and finite; the calls that only read (unpack,
+ * decode) take any such scale, those that write behind rows want a power of
+ * two, as they leave it themselves.  An infinity goes into the cache as the
+ * largest magnitude, a NaN as 0; either is reported by ep_sp_sync_status (rc 9).
+ * All four pointers are 16-byte aligned (the scales 4-byte). */
+#define EP_SP_E4M3 3
+#define EP_SP_I8 4
+typedef struct ep_sp_kv8 {
+    int32_t type; /* EP_SP_E4M3 or EP_SP_I8 */
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+} ep_sp_kv8;
+
+/* Rows [first[s], src->kv_lens[s]) of every sequence into the same rows of the
+ * 8-bit cache (first: DEVICE [n_seq], or NULL for 0; one outside
+ * [0, kv_lens[s]] is reported, rc 6, and its sequence left out).  Rows of dst
+ * outside that range keep their values (those before first[s] in its page are
+ * rounded to a grown scale).  src is a cache of the context's dtype as a
+ * prefill leaves it; dst has the same n_seq, room for src->max_kv_len rows and
+ * its own layout, its kv_lens is not read.  No page of dst may be written
+ * through two sequences.  rc 2 on bad arguments. */
+int32_t ep_sp_pack_kv(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* src, const void* k, const void* v,
+                      const int32_t* first, const ep_sp_kv_batch* dst, const ep_sp_kv8* cache, void* stream);
+
+/* The way back: rows [first[s], src->kv_lens[s]) of the 8-bit cache (src) into
+ * the same rows of a cache of the context's dtype (dst), rounded to it.  The
+ * context forgets the layer's page sums and f16 shadows, so a gated prefill
+ * call on those rows pools them (after replaying a captured call ep_sp_reset
+ * does that). */
+int32_t ep_sp_unpack_kv(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* src, const ep_sp_kv8* cache,
+                        const int32_t* first, const ep_sp_kv_batch* dst, void* k, void* v, void* stream);
+
+/* ep_sp_decode_layer over an 8-bit cache: out[s] = softmax(q[s] . K^T *
+ * kq_scale) V per query head, K and V the values the cache holds; a sequence of
+ * length 0 gets a zero row.  k_new, v_new: NULL, or [n_seq][n_head_kv][head_dim]
+ * of the context's dtype, which go into row kv_lens[s] - 1 of the cache first
+ * and are attended as what the cache then holds of them (no two sequences may
+ * then share the page of that row).  The products are exact, their sums, the
+ * scores and the softmax statistics f32; an f32 q is taken to 22 bits of its
+ * head's largest element.  A query head with an infinity or a NaN has a row of
+ * NaN, a NaN code of e4m3 makes NaN of what it reaches.  A sequence's result
+ * depends on the batch alone, not on timing. */
+int32_t ep_sp_decode8_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_len, size_t* bytes);
+int32_t ep_sp_decode8_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* kv, const void* q, const void* k_new,
+                            const void* v_new, const ep_sp_kv8* cache, void* out, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Blocks of paged caches, shared between sequences, taken, given back and moved
+ * on the device (no reference counterpart).  A sequence holds the first
+ * ceil(kv_lens[s] / block_rows) entries of its table; refs counts for each block
+ * of the pool how many sequences hold it, 0 for a free one.  Lengths, tables and
+ * counts stay on the device: a captured serving step can fork, grow and free
+ * sequences.  One set of tables serves every layer; the pools are what has to
+ * follow when a block is copied or moved: K and V of each layer, in whatever
+ * type, and the scales of an 8-bit cache.
+ * Results do not depend on timing.  Table entries that a call does not write
+ * stay as they are.  A length that its table cannot hold is reported by
+ * ep_sp_sync_status (rc 6) and read as 0, a table entry outside the pool is
+ * reported and not followed. */
+typedef struct ep_sp_pages {
+    int32_t n_seq;
+    int32_t table_stride;
+    int32_t block_rows;    /* a multiple of the page size */
+    int32_t pool_blocks;
+    int32_t* kv_lens;      /* DEVICE [n_seq] */
+    int32_t* block_tables; /* DEVICE [n_seq][table_stride] */
+    int32_t* refs;         /* DEVICE [pool_blocks] */
+} ep_sp_pages;
+
+/* [pool_blocks][block_bytes], block_bytes a multiple of 4; the rows of one
+ * block lie together in all of the pools that belong to a set of tables. */
+typedef struct ep_sp_pool {
+    void* rows;
+    size_t block_bytes;
+} ep_sp_pool;
+
+/* refs from the lengths and tables (to adopt tables made elsewhere). */
+int32_t ep_sp_count_refs(ep_sp_ctx* ctx, const ep_sp_pages* pages, void* stream);
+
+/* Every sequence s becomes a copy of the first lens[s] rows (lens NULL: all
+ * rows) of what sequence parents[s] was before the call, by holding the same
+ * blocks; parents[s] = -1 empties it and gives its blocks back.  parents[s] = s
+ * with its own length leaves it.  A parent outside [-1, n_seq) or a length
+ * outside the parent's rows is reported (rc 6) and leaves its sequence as it
+ * is.  Nothing is copied yet: ep_sp_resize_seqs does that where a sequence goes
+ * on to write into a block that others hold.  parents, lens: DEVICE [n_seq].
+ * The context forgets all layers' page sums.  rc 2 on bad arguments. */
+int32_t ep_sp_fork_bytes(const ep_sp_ctx* ctx, const ep_sp_pages* pages, size_t* bytes);
+int32_t ep_sp_fork_seqs(ep_sp_ctx* ctx, const ep_sp_pages* pages, const int32_t* parents, const int32_t* lens,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Lengths become new_lens (DEVICE [n_seq], 0 to table_stride * block_rows; one
+ * outside is reported, rc 6, and its sequence left).  First the blocks past the
+ * shorter lengths are given back, then the longer sequences, in order, take the
+ * lowest free blocks: one for the copy of a partly filled last block that other
+ * sequences hold too, then those for the rows to come.  Where every holder of
+ * such a block grows in this call, the last of them keeps it.  After the call no
+ * other sequence holds a block that has rows [old length, new length) of this
+ * one; what those rows hold is undefined.  With fewer free blocks than needed
+ * nothing changes and ep_sp_sync_status reports rc 10.  Only lengths are changed
+ * here: call it before the step that writes the rows.  pools: HOST [n_pools],
+ * n_pools in [1, 4096]. */
+int32_t ep_sp_resize_bytes(const ep_sp_ctx* ctx, const ep_sp_pages* pages, size_t* bytes);
+int32_t ep_sp_resize_seqs(ep_sp_ctx* ctx, const ep_sp_pages* pages, const int32_t* new_lens, const ep_sp_pool* pools,
+                          int32_t n_pools, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Moves the blocks in use to the front of the pools: with n blocks in use, the
+ * i-th of them at or past block n goes to the i-th free block below it; refs and
+ * every sequence's table follow.  The pools can then be cut to n blocks.  n_used:
+ * NULL, or DEVICE [1] receiving n.  The moved blocks' old places are free and
+ * keep their contents. */
+int32_t ep_sp_compact_bytes(const ep_sp_ctx* ctx, const ep_sp_pages* pages, size_t* bytes);
+int32_t ep_sp_compact_pool(ep_sp_ctx* ctx, const ep_sp_pages* pages, const ep_sp_pool* pools, int32_t n_pools,
+                           int32_t* n_used, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Synchronises the stream and reads the context's device error word: rc 6
  * (Prefill) when a kernel's bounded wait expired or a selection was out of
  * range or a paged-KV block table entry lay outside the pool or a batch's
- * sequence length outside its range since the last check, rc 9 (Unsupported) when an f32 input left the
- * f16 range of the tensor-core mode (the word is then cleared), 12 on a CUDA
- * error.
+ * sequence length outside its range (or a fork's parent) since the last check,
+ * rc 9 (Unsupported) when an f32 input left the f16 range of the tensor-core
+ * mode or a row with an infinity or a NaN went into an 8-bit cache, rc 10 when a
+ * resize found too few free blocks (the word is then cleared; the first of
+ * several failures is the one reported), 12 on a CUDA error.
  * It also reads and clears the error word of ep_sp_select_pages_noalloc on
  * the context's device.  The compute calls themselves never synchronise. */
 int32_t ep_sp_sync_status(ep_sp_ctx* ctx, void* stream);
@@ -563,6 +700,11 @@ int32_t ep_sp_profile_read(ep_sp_ctx* ctx, double* ms, int64_t* launches);
  * prompt weights, 8 eviction (n <= EP_SP_NUM_FAMILIES; rc 2 otherwise). */
 #define EP_SP_NUM_FAMILIES 9
 int32_t ep_sp_profile_read_families(ep_sp_ctx* ctx, int32_t n, double* ms, int64_t* launches);
+/* One family: any of those (6 counts decode steps over 8-bit caches, too), or
+ * one of the two below. */
+#define EP_SP_FAMILY_PACK 9   /* pack and unpack */
+#define EP_SP_FAMILY_PAGES 10 /* fork, resize, compact, counting */
+int32_t ep_sp_profile_read_family(ep_sp_ctx* ctx, int32_t family, double* ms, int64_t* launches);
 
 /* Algorithmic work of one ep_sp_attend_layer(layer, kv_len, n_tok) call with
  * the context's current settings, from the same block plan the kernels use:
