@@ -37,27 +37,39 @@ __device__ __forceinline__ float exact_inverse(float s) {
     return (b & 0x7fffffu) == 0 && e >= 1 && e <= 253 ? __uint_as_float((254 - e) << 23) : 0.f;
 }
 
-// Four values, already divided by their scale, to bytes.  An infinity becomes
-// the largest magnitude, a NaN 0 (both are reported by the caller).
+// Four values, already divided by their scale and at most its M, to bytes.  The
+// integers are the low bits of a sum with 1.5 * 2^23, which rounds as wanted.
 template <bool I8>
 __device__ __forceinline__ uint32_t to8(float x0, float x1, float x2, float x3) {
     if constexpr (I8) {
-        auto q = [](float x) { return (uint32_t)__float2int_rn(fminf(fmaxf(x == x ? x : 0.f, -127.f), 127.f)) & 0xffu; };
-        return q(x0) | q(x1) << 8 | q(x2) << 16 | q(x3) << 24;
+        auto q = [](float x) { return __float_as_uint(x + 12582912.f); };
+        return __byte_perm(__byte_perm(q(x0), q(x1), 0x0040), __byte_perm(q(x2), q(x3), 0x0040), 0x5410);
     } else {
-        auto n = [](float x) { return x == x ? x : 0.f; };
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(n(x0), n(x1)), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(n(x2), n(x3)), __NV_SATFINITE, __NV_E4M3);
-        return lo | hi << 16;
+        uint32_t r;
+        asm("{\n .reg .b16 l, h;\n cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n"
+            " mov.b32 %0, {l, h};\n}"
+            : "=r"(r)
+            : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
+        return r;
     }
+}
+
+// What a value that is not finite goes into the cache as, already divided: an
+// infinity as the largest magnitude, a NaN as 0.
+template <bool I8>
+__device__ __forceinline__ float tame8(float x) {
+    constexpr float top = I8 ? 127.f : 448.f;
+    return x == x ? fminf(fmaxf(x, -top), top) : 0.f;
 }
 
 // Four bytes to the numbers they hold, exactly.
 template <bool I8>
 __device__ __forceinline__ void from8(uint32_t w, float (&x)[4]) {
     if constexpr (I8) {
+        // b + 128 as the low bits of 2^23
+        const uint32_t u = w ^ 0x80808080u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)) - 8388736.f;
     } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {

@@ -85,15 +85,13 @@ __device__ __forceinline__ void pairs8(uint32_t w, uint32_t& p01, uint32_t& p23)
     }
 }
 
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint2 lds8(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-    return v;
+// D += A B in f16 with f32 sums.  (Not volatile: the products may be put in any
+// order that keeps each sum's.)
+__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                     uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // Four neighbouring query elements.
@@ -196,6 +194,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
         bool ok = true;
         int seg = 0;
         const uint64_t policy = tc::policy_evict_first();  // the cache is read once
+        const int lg_page = __ffs(c8.page_size) - 1;
         for (; (w.left > 0 || (C > 1 && seg == 0)) && ok; ++seg) {
             const int n_seg = w.segment();
             const int h = w.run / sp.passes, pass = w.run % sp.passes;
@@ -231,7 +230,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
                             tc::tma_load_3d(base, &tmK, &full[st], 0, h, r, policy);
                             tc::tma_load_3d(base + LY::kHalf, &tmV, &full[st], 0, h, r, policy);
                             if (r < a.kv.rows) {
-                                const int64_t page = (int64_t)(r / c8.page_size) * Hkv + h;
+                                const int64_t page = (int64_t)(r >> lg_page) * Hkv + h;
                                 tc::copy4_async(&scale_s[st].x, c8.k_scale + page);
                                 tc::copy4_async(&scale_s[st].y, c8.v_scale + page);
                                 tc::copies_arrive(&full[st]);
@@ -321,7 +320,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
             if (!ok) break;
             unsigned char* stage = smem + st * LY::kStage;
             const int u = w.u + i, lim = min(kUnit, w.n - u * kUnit);
-            const uint32_t kb = tc::smem_u32(stage), vb = kb + LY::kHalf;
+            const unsigned char* vb = stage + LY::kHalf;
             if (!I8 && lim < kUnit) {
                 // V rows past the length may hold NaN codes: their P is 0, and 0 * NaN is not 0
                 for (int j = lane; j < (kUnit - lim) * (D / 16); j += 32)
@@ -330,23 +329,25 @@ __global__ void __launch_bounds__(kThreads8, 1)
                 __syncwarp();
             }
             const float2 sc = scale_s[st];
+            // (the four tiles of keys in turn: each one's products wait for one another)
             float s4[4][4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                s4[t][0] = s4[t][1] = s4[t][2] = s4[t][3] = 0.f;
+            for (int t = 0; t < 4; ++t) s4[t][0] = s4[t][1] = s4[t][2] = s4[t][3] = 0.f;
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) {
-                    const uint4 b = lds16(kb + tile_at<D>(t * 8 + hd, (D / 64) * tq + c));
-                    const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+            for (int c = 0; c < D / 64; ++c) {
+                uint4 b[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                for (int t = 0; t < 4; ++t) b[t] = *reinterpret_cast<const uint4*>(stage + tile_at<D>(t * 8 + hd, (D / 64) * tq + c));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
                         const int j = 4 * c + e;
                         uint32_t b0, b1;
-                        pairs8<I8>(bw[e], b0, b1);
-                        mma16816<false>(s4[t], qh[2 * j], LO ? ql[LO ? 2 * j : 0] : 0u, qh[2 * j + 1],
+                        pairs8<I8>(e == 0 ? b[t].x : e == 1 ? b[t].y : e == 2 ? b[t].z : b[t].w, b0, b1);
+                        mma8(s4[t], qh[2 * j], LO ? ql[LO ? 2 * j : 0] : 0u, qh[2 * j + 1],
                                         LO ? ql[LO ? 2 * j + 1 : 0] : 0u, b0, b1);
                     }
-                }
             }
             const float slk = sl * sc.x;
             float mx = -INFINITY;
@@ -391,10 +392,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
                     for (int e = 0; e < 2; ++e) {
                         const int r = 16 * b + 8 * t + 2 * tq + e;
                         if constexpr (D == 128) {
-                            const uint4 x = lds16(vb + tile_at<D>(r, hd));
+                            const uint4 x = *reinterpret_cast<const uint4*>(vb + tile_at<D>(r, hd));
                             v[b][t][e][0] = x.x, v[b][t][e][1] = x.y, v[b][t][e][2] = x.z, v[b][t][e][3] = x.w;
                         } else {
-                            const uint2 x = lds8(vb + tile_at<D>(r, hd >> 1) + (hd & 1) * 8);
+                            const uint2 x = *reinterpret_cast<const uint2*>(vb + tile_at<D>(r, hd >> 1) + (hd & 1) * 8);
                             v[b][t][e][0] = x.x, v[b][t][e][1] = x.y;
                         }
                     }
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
                     pairs8<I8>(prmt(v[b][1][0][x], v[b][1][1][x], 0x7362), b1[2], b1[3]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        mma16816<false>(t4[j], p[b][0], p[b][1], p[b][2], p[b][3], b0[j], b1[j]);
+                        mma8(t4[j], p[b][0], p[b][1], p[b][2], p[b][3], b0[j], b1[j]);
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j)

@@ -59,20 +59,25 @@ __device__ __forceinline__ int2 span_of(const PackArgs& a, int s) {
     return make_int2(f, n);
 }
 
-// Largest of the CTA's values, and whether any thread saw something odd.
-__device__ __forceinline__ uint32_t cta_max(uint32_t m, bool& odd, uint32_t* box) {
+// Largest of the CTA's values.
+__device__ __forceinline__ uint32_t cta_max(uint32_t m, uint32_t* box) {
     m = __reduce_max_sync(0xffffffffu, m);
-    const bool any = __any_sync(0xffffffffu, odd);
-    if ((threadIdx.x & 31) == 0) box[threadIdx.x >> 5] = m | (any ? 0x80000000u : 0u);
+    if ((threadIdx.x & 31) == 0) box[threadIdx.x >> 5] = m;
     __syncthreads();
     m = 0;
-    odd = false;
-    for (int i = 0; i < (int)blockDim.x / 32; ++i) {
-        odd |= (box[i] & 0x80000000u) != 0;
-        m = max(m, box[i] & 0x7fffffffu);
-    }
+    for (int i = 0; i < (int)blockDim.x / 32; ++i) m = max(m, box[i]);
     __syncthreads();  // (the box is written again)
     return m;
+}
+
+// Largest bit pattern without its sign of a register's values, as f32 bits: the
+// patterns of one type are in the order of the magnitudes, a NaN's above all.
+template <int ET>
+__device__ __forceinline__ uint32_t top_of(uint32_t m) {
+    if constexpr (ET == 0) return m;
+    m = max(m & 0xffffu, m >> 16);
+    if constexpr (ET == 2) return m << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
 }
 
 // The bytes of rows [0, rows) of one head at `p` follow their page's scale from
@@ -90,7 +95,7 @@ __device__ __forceinline__ void rescale(uint8_t* p, int64_t stride, int rows, in
 
 // C: 16-byte chunks of a page and head per thread.
 template <int ET, bool I8, int C>
-__global__ void __launch_bounds__(kThreads) k9_pack(const PackArgs a) {
+__global__ void __launch_bounds__(kThreads, C <= 2 ? 6 : C <= 8 ? 4 : 2) k9_pack(const PackArgs a) {
     constexpr int kEs = ET == 0 ? 4 : 2, kPer = 16 / kEs;
     __shared__ uint32_t box[kThreads / 32];
     __shared__ int2 span_s;
@@ -115,7 +120,6 @@ __global__ void __launch_bounds__(kThreads) k9_pack(const PackArgs a) {
         float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + (int64_t)(to / P) * Hkv + h;
         uint4 v[C];
         uint32_t m = 0;
-        bool odd = false;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const int i = threadIdx.x + j * kThreads, r = i >> lg, c = i & ((1 << lg) - 1);
@@ -128,19 +132,26 @@ __global__ void __launch_bounds__(kThreads) k9_pack(const PackArgs a) {
         for (int j = 0; j < C; ++j) {
             const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[j]);
 #pragma unroll
-            for (int e = 0; e < kPer / 4; ++e) {
-                float x[4];
-                values4<ET>(w + 2 * e, x);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) m = max(m, magnitude(x[i], odd));
-            }
+            for (int e = 0; e < 4; ++e) m = ET == 0 ? max(m, w[e] & 0x7fffffffu) : __vmaxu2(m, w[e] & 0x7fff7fffu);
         }
-        m = cta_max(m, odd, box);
+        m = cta_max(top_of<ET>(m), box);
         if (!there) continue;
-        // (the values are made from the rows again, not held: twice the registers)
-#pragma unroll
-        for (int j = 0; j < C; ++j) asm volatile("" : "+r"(v[j].x), "+r"(v[j].y), "+r"(v[j].z), "+r"(v[j].w));
-        if (odd && threadIdx.x == 0) report_error(a.err, kDevNotFinite8, 0x93, r0 / P);
+        const bool odd = m >= 0x7f800000u;
+        if (odd) {  // (rare) again, without what is not finite
+            m = 0;
+            bool any = false;
+#pragma unroll 1
+            for (int i = threadIdx.x; i < (hi - lo) * d; i += kThreads) {
+                const char* p = src + ((int64_t)(lo + i / d) * Hkv * d + i % d) * kEs;
+                float x;
+                if constexpr (ET == 0) x = *reinterpret_cast<const float*>(p);
+                else if constexpr (ET == 1) x = __half2float(*reinterpret_cast<const __half*>(p));
+                else x = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p));
+                m = max(m, magnitude(x, any));
+            }
+            m = cta_max(m, box);
+            if (threadIdx.x == 0) report_error(a.err, kDevNotFinite8, 0x93, r0 / P);
+        }
         float sc = scale8<I8>(m);
         if (was >= sc) sc = was;
         else {
@@ -148,6 +159,7 @@ __global__ void __launch_bounds__(kThreads) k9_pack(const PackArgs a) {
             if (threadIdx.x == 0) *scale = sc;
         }
         const float inv = exact_inverse(sc);
+        const bool slow = odd || inv == 0.f;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const int i = threadIdx.x + j * kThreads, r = i >> lg, c = i & ((1 << lg) - 1);
@@ -158,7 +170,14 @@ __global__ void __launch_bounds__(kThreads) k9_pack(const PackArgs a) {
             for (int e = 0; e < kPer / 4; ++e) {
                 float x[4];
                 values4<ET>(w + 2 * e, x);
-                q[e] = to8<I8>(over(x[0], sc, inv), over(x[1], sc, inv), over(x[2], sc, inv), over(x[3], sc, inv));
+                if (slow) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = tame8<I8>(over(x[k], sc, inv));
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] *= inv;
+                }
+                q[e] = to8<I8>(x[0], x[1], x[2], x[3]);
             }
             uint8_t* o = dst + (int64_t)r * Hkv * d + c * kPer;
             if constexpr (kPer == 8) *reinterpret_cast<uint2*>(o) = make_uint2(q[0], q[1]);
@@ -261,7 +280,8 @@ __global__ void __launch_bounds__(128) k9_append(const AppendArgs a) {
     uint32_t m = magnitude(x, odd);
     float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + (int64_t)(max(row, 0) / P) * Hkv + h;
     const float was = row >= 0 && lo > 0 ? *scale : 0.f;
-    m = cta_max(m, odd, box);
+    m = cta_max(m, box);
+    odd = __syncthreads_or(odd);
     if (row < 0) return;
     if (odd && t == 0) report_error(a.err, kDevNotFinite8, 0x94, s);
     uint8_t* dst = (is_v ? a.c.v : a.c.k) + ((int64_t)row * Hkv + h) * d;
@@ -271,7 +291,7 @@ __global__ void __launch_bounds__(128) k9_append(const AppendArgs a) {
         if (lo > 0) rescale<I8>(dst, (int64_t)Hkv * d, lo, d, was, sc);
         if (t == 0) *scale = sc;
     }
-    if (t < d) dst[(int64_t)lo * Hkv * d + t] = (uint8_t)to8<I8>(over(x, sc, exact_inverse(sc)), 0.f, 0.f, 0.f);
+    if (t < d) dst[(int64_t)lo * Hkv * d + t] = (uint8_t)to8<I8>(tame8<I8>(over(x, sc, exact_inverse(sc))), 0.f, 0.f, 0.f);
 }
 
 // Kernels here may start before what precedes them on the stream has ended:
