@@ -7,10 +7,11 @@
 // the ring and the joins are K6's (decode_common.cuh).  A new token's row is
 // quantised into the cache by k9_append first.
 //
-// CTA: one warp streams K and V units (32 rows of one head, so one scale each)
-// into a ring by TMA, the two scales by cp.async on the same barrier; units go
-// round robin to the streams of 8 warps, each with its own online softmax over
-// 8 query heads (groups of more than 8 heads give a unit to 2, 4 or 8 warps).
+// CTA: units (32 rows of one head, so one scale each of K and V) go round robin
+// to the streams of 8 warps, each with its own online softmax over 8 query heads
+// (groups of more than 8 heads give a unit to 2, 4 or 8 warps).  A stream has
+// its own stages and fetches for itself: K and V by TMA, the two scales by
+// cp.async on the same barrier.
 //
 // S = Q K^T and O = P V on mma.sync m16n8k16 in f16, which holds both 8-bit
 // types exactly.  The order of the contracted dimension is free, so a lane
@@ -38,7 +39,7 @@ namespace epsp {
 namespace {
 
 constexpr int kWarps8 = 8;
-constexpr int kThreads8 = (kWarps8 + 1) * 32;
+constexpr int kThreads8 = kWarps8 * 32;
 constexpr float kUp8 = 7.f;       // P is 2^7 times the weight against the running maximum (2^15 at most)
 constexpr float kLow8 = 4096.f;   // factor of a remainder
 constexpr int kPass8 = 64;        // query heads of a pass, at most
@@ -47,14 +48,14 @@ template <int D>
 struct Layout8 {
     static constexpr int kHalf = kUnit * D;      // K (or V) of a unit
     static constexpr int kStage = 2 * kHalf;
-    static constexpr int kStages = 131072 / kStage;  // a multiple of the streams, as in K6
+    static constexpr int kStages = 131072 / kStage;  // dealt to the streams in equal parts
     static constexpr int kOffQ = kStages * kStage;   // [2] queries of a segment
     static constexpr int kQBytes = 16384;
     static constexpr int kOffO = kOffQ + 2 * kQBytes;  // [kWarps8][8][D] merge buffer
     static constexpr int kOffMl = kOffO + kWarps8 * 8 * D * 4;
     static constexpr int kOffScale = kOffMl + 2 * kWarps8 * 8 * 8;  // [kStages] (ks, vs)
     static constexpr int kOffBar = kOffScale + kStages * 8;
-    static constexpr int kOffLens = kOffBar + (2 * kStages + 4) * 8;
+    static constexpr int kOffLens = kOffBar + (2 * kStages + 2) * 8;
     static constexpr int kBytes = kOffLens + kLensOnChip * 4;
     static_assert(kStages % kWarps8 == 0 && kBytes + 1024 <= 232448, "shared memory");
 };
@@ -107,6 +108,36 @@ __device__ __forceinline__ float4 q_of(const unsigned char* q, int32_t dtype, in
                        __uint_as_float(w.y & 0xffff0000u));
 }
 
+// What a stream of warps fetches next: the units of the CTA's range that fall to
+// it, one segment after the other.
+struct Fetch {
+    Walk w;          // the segment
+    int32_t before;  // units of the CTA's range before it
+    int32_t at;      // the unit, counted from the range's start
+    int32_t entry;   // its table entry, on its way
+
+    __device__ __forceinline__ bool more() const { return w.left > 0; }
+    // To the segment that holds unit `at`, and for its table entry.
+    __device__ __forceinline__ void find(const DecodeArgs& a, const Lens& lens, int runs) {
+        while (w.left > 0 && at - before >= w.segment()) {
+            before += w.segment();
+            w.advance(a, lens, runs, w.segment());
+        }
+        if (w.left > 0 && a.kv.block_rows > 0)
+            entry = a.kv.tables[(int64_t)w.s * a.kv.table_stride + (w.u + at - before) * kUnit / a.kv.block_rows];
+    }
+    // Cache row of the unit; the tensors' row count (zeros are read there) for a
+    // table entry outside the pool, which is recorded.
+    __device__ __forceinline__ int row(const DecodeArgs& a, int32_t e) const {
+        const int r = (w.u + at - before) * kUnit;
+        if (a.kv.block_rows <= 0) return w.s * a.kv.seq_rows + r;
+        const int64_t x = (int64_t)e * a.kv.block_rows + r % a.kv.block_rows;
+        if (e >= 0 && x < a.kv.rows) return (int)x;
+        report_error(a.err, kDevBadBlockTable, 0x95, w.s);
+        return a.kv.rows;
+    }
+};
+
 // LO: q has remainders (f32).  JOIN: the calls that join_cluster finishes.
 template <int D, bool I8, bool LO, bool JOIN>
 __global__ void __launch_bounds__(kThreads8, 1)
@@ -119,7 +150,6 @@ __global__ void __launch_bounds__(kThreads8, 1)
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
     uint64_t* empty = full + LY::kStages;
     uint64_t* q_full = empty + LY::kStages;
-    uint64_t* q_empty = q_full + 2;
     int32_t* lens_s = reinterpret_cast<int32_t*>(smem + LY::kOffLens);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int Hkv = a.n_head_kv, G = a.n_head / Hkv, es = a.dtype == 0 ? 4 : 2;
@@ -130,10 +160,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
             tc::mbar_init(&full[i], 2);  // the bytes' announcement, and the scales
             tc::mbar_init(&empty[i], sp.groups);
         }
-        for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(&q_full[i], 1);
-            tc::mbar_init(&q_empty[i], kWarps8);
-        }
+        for (int i = 0; i < 2; ++i) tc::mbar_init(&q_full[i], 1);
         tc::fence_mbar_init();
         tc::tma_prefetch_desc(&tmK);
         tc::tma_prefetch_desc(&tmV);
@@ -186,89 +213,76 @@ __global__ void __launch_bounds__(kThreads8, 1)
     const uint64_t tmo = a.timeout_ns;
     float2* scale_s = reinterpret_cast<float2*>(smem + LY::kOffScale);
 
-    if (warp == kWarps8) {
-        // ------------------------------------------------------- producer --
-        // 32 units' rows at a time (one table entry per lane), lane 0 issues.
-        Walk w = w0;
-        int it = 0;
-        bool ok = true;
-        int seg = 0;
-        const uint64_t policy = tc::policy_evict_first();  // the cache is read once
-        const int lg_page = __ffs(c8.page_size) - 1;
-        for (; (w.left > 0 || (C > 1 && seg == 0)) && ok; ++seg) {
-            const int n_seg = w.segment();
-            const int h = w.run / sp.passes, pass = w.run % sp.passes;
-            if (lane == 0) {
-                const int b = seg & 1;
-                ok = tc::mbar_wait(&q_empty[b], ((seg >> 1) & 1) ^ 1, tmo);
-                if (ok) {
-                    const uint32_t bytes = min(sp.pass_heads, G - pass * sp.pass_heads) * D * es;
-                    tc::mbar_arrive_expect_tx(&q_full[b], bytes);
-                    tc::bulk_load(smem + LY::kOffQ + b * LY::kQBytes,
-                                  static_cast<const char*>(a.q) +
-                                      ((int64_t)w.s * a.n_head + (int64_t)h * G + pass * sp.pass_heads) * D * es,
-                                  bytes, &q_full[b]);
-                }
-            }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (!ok) break;
-            for (int i0 = 0; i0 < n_seg && ok; i0 += 32) {
-                int row = a.kv.rows;  // past the end: zeros
-                if (i0 + lane < n_seg) {
-                    const int r = batch_row(a.kv, w.s, (w.u + i0 + lane) * kUnit, a.err);
-                    if (r >= 0) row = r;
-                }
-                const int cnt = min(32, n_seg - i0);
-                for (int i = 0; i < cnt; ++i, ++it) {
-                    const int st = it % LY::kStages;
-                    const int r = __shfl_sync(0xffffffffu, row, i);
-                    if (lane == 0) {
-                        ok = tc::mbar_wait(&empty[st], ((it / LY::kStages) & 1) ^ 1, tmo);
-                        if (ok) {
-                            tc::mbar_arrive_expect_tx(&full[st], LY::kStage);
-                            unsigned char* base = smem + st * LY::kStage;
-                            tc::tma_load_3d(base, &tmK, &full[st], 0, h, r, policy);
-                            tc::tma_load_3d(base + LY::kHalf, &tmV, &full[st], 0, h, r, policy);
-                            if (r < a.kv.rows) {
-                                const int64_t page = (int64_t)(r >> lg_page) * Hkv + h;
-                                tc::copy4_async(&scale_s[st].x, c8.k_scale + page);
-                                tc::copy4_async(&scale_s[st].y, c8.v_scale + page);
-                                tc::copies_arrive(&full[st]);
-                            } else {
-                                scale_s[st] = make_float2(0.f, 0.f);
-                                tc::mbar_arrive(&full[st]);
-                            }
-                        }
-                    }
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
-                    if (!ok) break;
-                }
-            }
-            w.advance(a, lens, runs, n_seg);
-        }
-        if (!ok) {
-            if (lane == 0) report_error(a.err, kDevWaitDecode, 0xb1, it);
-            // copies still in flight land before the CTA ends
-            for (int j = max(0, it - LY::kStages); j < it; ++j)
-                tc::mbar_wait(&full[j % LY::kStages], (j / LY::kStages) & 1, tmo);
-            for (int j = max(0, seg - 1); j <= seg; ++j) tc::mbar_wait(&q_full[j & 1], (j >> 1) & 1, tmo);
-        }
-        return;
-    }
-
-    // ---------------------------------------------------------- consumers --
     const int groups = sp.groups, streams = kWarps8 / groups;
     const int grp = warp & (groups - 1), stream = warp / groups;
+    const int depth = LY::kStages / streams, st0 = stream * depth;  // this stream's stages
+    const uint64_t policy = tc::policy_evict_first();               // the cache is read once
+    const int lg_page = __ffs(c8.page_size) - 1;
+    bool ok = true;
+
+    // The stream's first warp fetches for it, a stage as soon as its warps are
+    // done with it: eight warps issue copies, which one alone does at no more
+    // than 5.2 TB/s (over all SMs, 8 KB units).
+    Fetch f{w0, 0, stream, 0};
+    int fetched = 0;
+    if (grp == 0) f.find(a, lens, runs);
+    auto fetch = [&]() {
+        const Fetch x = f;
+        f.at += streams;
+        f.find(a, lens, runs);  // (the next entry is on its way while this one's copies are issued)
+        const int st = st0 + fetched % depth, r = x.row(a, x.entry), h = x.w.run / sp.passes;
+        if (groups > 1) {
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&empty[st], ((fetched / depth) & 1) ^ 1, tmo));
+            if (!ok) return;
+        }
+        ++fetched;
+        if (lane == 0) {
+            tc::mbar_arrive_expect_tx(&full[st], LY::kStage);
+            unsigned char* base = smem + st * LY::kStage;
+            tc::tma_load_3d(base, &tmK, &full[st], 0, h, r, policy);
+            tc::tma_load_3d(base + LY::kHalf, &tmV, &full[st], 0, h, r, policy);
+            if (r < a.kv.rows) {
+                const int64_t page = (int64_t)(r >> lg_page) * Hkv + h;
+                tc::copy4_async(&scale_s[st].x, c8.k_scale + page);
+                tc::copy4_async(&scale_s[st].y, c8.v_scale + page);
+                tc::copies_arrive(&full[st]);
+            } else {
+                scale_s[st] = make_float2(0.f, 0.f);
+                tc::mbar_arrive(&full[st]);
+            }
+        }
+        __syncwarp();
+    };
+    // The queries of segment n_q, by thread 0, while the segment before is
+    // attended (its buffer's readers met at the end of the one before that).
+    Walk wq = w0;
+    int n_q = 0;
+    auto fetch_q = [&]() {
+        if (threadIdx.x == 0 && (wq.left > 0 || (C > 1 && n_q == 0))) {
+            const int h = wq.run / sp.passes, pass = wq.run % sp.passes, b = n_q & 1;
+            const uint32_t bytes = min(sp.pass_heads, G - pass * sp.pass_heads) * D * es;
+            tc::mbar_arrive_expect_tx(&q_full[b], bytes);
+            tc::bulk_load(smem + LY::kOffQ + b * LY::kQBytes,
+                          static_cast<const char*>(a.q) +
+                              ((int64_t)wq.s * a.n_head + (int64_t)h * G + pass * sp.pass_heads) * D * es,
+                          bytes, &q_full[b]);
+            ++n_q;
+            if (wq.left > 0) wq.advance(a, lens, runs, wq.segment());
+        }
+    };
+    fetch_q();
+    for (int i = 0; i < depth && grp == 0 && f.more(); ++i) fetch();
+
     float* om = reinterpret_cast<float*>(smem + LY::kOffO);
     float* om_w = om + warp * 8 * D;
     Walk w = w0;
-    int it = 0;
-    bool ok = true;
+    int it = 0, used = 0;  // units of the range before the segment; units that this warp is done with
     for (int seg = 0; w.left > 0 || (C > 1 && seg == 0); ++seg) {
         const int n_seg = w.segment();
         const int h = w.run / sp.passes, pass = w.run % sp.passes;
         const int g0 = pass * sp.pass_heads + grp * 8;  // this warp's first query head of the group
         const int64_t q_row = (int64_t)w.s * a.n_head + (int64_t)h * G;
+        fetch_q();
         const int hd = lane >> 2, tq = lane & 3;  // this lane's head (or column block of V) and quarter
         float o[2 * kCols];  // head hd, columns kCols (2 tq + e) + j at [2 j + e]
 #pragma unroll
@@ -311,13 +325,13 @@ __global__ void __launch_bounds__(kThreads8, 1)
         // first unit of the segment that falls to this stream
         int i = (stream - it) & (streams - 1);
         for (; i < n_seg; i += streams) {
-            const int at = it + i, st = at % LY::kStages;
+            const int st = st0 + used % depth;
             if (ok) {
-                ok = tc::mbar_wait(&full[st], (at / LY::kStages) & 1, tmo);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb2, at);
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[st], (used / depth) & 1, tmo));
+                if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb2, it + i);
             }
             if (!ok) break;
+            ++used;
             unsigned char* stage = smem + st * LY::kStage;
             const int u = w.u + i, lim = min(kUnit, w.n - u * kUnit);
             const unsigned char* vb = stage + LY::kHalf;
@@ -425,14 +439,13 @@ __global__ void __launch_bounds__(kThreads8, 1)
                     }
             }
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&empty[st]);
+            if (groups > 1 && lane == 0) tc::mbar_arrive(&empty[st]);
+            if (grp == 0 && f.more()) fetch();
         }
 
         // ------------------------------------------- merge the warps' states
         // (ml alternates between two buffers: a warp may write the next
         // segment's before another has read this one's sums)
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&q_empty[seg & 1]);
         float2* ml = reinterpret_cast<float2*>(smem + LY::kOffMl) + (seg & 1) * kWarps8 * 8;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -509,6 +522,12 @@ __global__ void __launch_bounds__(kThreads8, 1)
         it += n_seg;
         w.advance(a, lens, runs, n_seg);
     }
+    if (!ok) {
+        // copies still in flight land before the CTA ends
+        if (lane == 0) report_error(a.err, kDevWaitDecode, 0xb1, used);
+        for (int j = max(0, fetched - depth); j < fetched; ++j) tc::mbar_wait(&full[st0 + j % depth], (j / depth) & 1, tmo);
+        for (int j = max(0, n_q - 2); j < n_q; ++j) tc::mbar_wait(&q_full[j & 1], (j >> 1) & 1, tmo);
+    }
 }
 
 // ---------------------------------------------------------------- host side --
@@ -522,7 +541,7 @@ bool cache8_map(CUtensorMap* m, const void* base, int32_t d, int32_t n_head_kv, 
     const cuuint32_t estr[3] = {1, 1, 1};
     return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Split of a call and its workspace layout; returns the bytes (SIZE_MAX: more
