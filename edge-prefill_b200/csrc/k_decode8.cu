@@ -20,8 +20,11 @@
 // a transpose, and one byte permutation pairs two rows of V.  q is scaled to a
 // largest magnitude of 2^14 to 2^15 by a power of two, so f16 takes its 16-bit
 // types as they are; an f32 q has its rounding remainder (times 2^12) in rows
-// 8-15.  Rows 8-15 of the P operand carry P's remainder, times 2^12 too: P
-// keeps 22 bits.  A unit's product goes into O in f32, by its scale.
+// 8-15.  P is the weight times V's scale, against the running maximum of just
+// that, so that units of other scales add up in the accumulators as they are;
+// the weights' sum takes P over the scale.  P is held 2^7 up (2^15 at most);
+// rows 8-15 of its operand carry its rounding remainder, times 2^12: an element
+// keeps 22 bits of itself and an absolute 2^-44 of the largest.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -94,6 +97,13 @@ __device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, ui
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// D = A B.
+__device__ __forceinline__ void mma8_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                           uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 
 // Four neighbouring query elements.
 __device__ __forceinline__ float4 q_of(const unsigned char* q, int32_t dtype, int i) {
@@ -108,31 +118,53 @@ __device__ __forceinline__ float4 q_of(const unsigned char* q, int32_t dtype, in
                        __uint_as_float(w.y & 0xffff0000u));
 }
 
+// Units of a block, and the place of a unit: dividing by a number that is known
+// at run time only costs forty instructions, by its reciprocal five.
+struct Blocks {
+    int32_t units;   // of a block; 0: no blocks
+    uint32_t inverse;
+    __device__ __forceinline__ explicit Blocks(int block_rows) {
+        units = block_rows / kUnit;
+        inverse = units > 0 ? 0xffffffffu / (uint32_t)units : 0;
+    }
+    // Block of unit u (under 2^26), and the unit's place in it.  The product is
+    // short of u / units by less than 2^-5.
+    __device__ __forceinline__ int2 of(int u) const {
+        int q = (int)__umulhi((uint32_t)u, inverse), r = u - q * units;
+        if (r >= units) ++q, r -= units;
+        return make_int2(q, r);
+    }
+};
+
 // What a stream of warps fetches next: the units of the CTA's range that fall to
 // it, one segment after the other.
 struct Fetch {
     Walk w;          // the segment
+    int32_t h;       // its KV head
     int32_t before;  // units of the CTA's range before it
     int32_t at;      // the unit, counted from the range's start
+    int32_t place;   // of the unit in its block
     int32_t entry;   // its table entry, on its way
 
     __device__ __forceinline__ bool more() const { return w.left > 0; }
     // To the segment that holds unit `at`, and for its table entry.
-    __device__ __forceinline__ void find(const DecodeArgs& a, const Lens& lens, int runs) {
+    __device__ __forceinline__ void find(const DecodeArgs& a, const Blocks& bl, const Lens& lens, int runs, int passes) {
         while (w.left > 0 && at - before >= w.segment()) {
             before += w.segment();
             w.advance(a, lens, runs, w.segment());
+            h = w.run / passes;
         }
-        if (w.left > 0 && a.kv.block_rows > 0)
-            entry = a.kv.tables[(int64_t)w.s * a.kv.table_stride + (w.u + at - before) * kUnit / a.kv.block_rows];
+        if (w.left <= 0 || bl.units == 0) return;
+        const int2 b = bl.of(w.u + at - before);
+        place = b.y;
+        entry = a.kv.tables[(int64_t)w.s * a.kv.table_stride + b.x];
     }
     // Cache row of the unit; the tensors' row count (zeros are read there) for a
     // table entry outside the pool, which is recorded.
-    __device__ __forceinline__ int row(const DecodeArgs& a, int32_t e) const {
-        const int r = (w.u + at - before) * kUnit;
-        if (a.kv.block_rows <= 0) return w.s * a.kv.seq_rows + r;
-        const int64_t x = (int64_t)e * a.kv.block_rows + r % a.kv.block_rows;
-        if (e >= 0 && x < a.kv.rows) return (int)x;
+    __device__ __forceinline__ int row(const DecodeArgs& a, const Blocks& bl) const {
+        if (bl.units == 0) return w.s * a.kv.seq_rows + (w.u + at - before) * kUnit;
+        const int64_t x = (int64_t)entry * a.kv.block_rows + place * kUnit;
+        if (entry >= 0 && x < a.kv.rows) return (int)x;
         report_error(a.err, kDevBadBlockTable, 0x95, w.s);
         return a.kv.rows;
     }
@@ -215,7 +247,9 @@ __global__ void __launch_bounds__(kThreads8, 1)
 
     const int groups = sp.groups, streams = kWarps8 / groups;
     const int grp = warp & (groups - 1), stream = warp / groups;
-    const int depth = LY::kStages / streams, st0 = stream * depth;  // this stream's stages
+    // this stream's stages
+    const int lg_depth = __ffs(LY::kStages / kWarps8 * groups) - 1, depth = 1 << lg_depth, st0 = stream << lg_depth;
+    const Blocks blocks(a.kv.block_rows);
     const uint64_t policy = tc::policy_evict_first();               // the cache is read once
     const int lg_page = __ffs(c8.page_size) - 1;
     bool ok = true;
@@ -223,31 +257,31 @@ __global__ void __launch_bounds__(kThreads8, 1)
     // The stream's first warp fetches for it, a stage as soon as its warps are
     // done with it: eight warps issue copies, which one alone does at no more
     // than 5.2 TB/s (over all SMs, 8 KB units).
-    Fetch f{w0, 0, stream, 0};
+    Fetch f{w0, w0.run / sp.passes, 0, stream, 0, 0};
     int fetched = 0;
-    if (grp == 0) f.find(a, lens, runs);
+    if (grp == 0) f.find(a, blocks, lens, runs, sp.passes);
     auto fetch = [&]() {
         const Fetch x = f;
         f.at += streams;
-        f.find(a, lens, runs);  // (the next entry is on its way while this one's copies are issued)
-        const int st = st0 + fetched % depth, r = x.row(a, x.entry), h = x.w.run / sp.passes;
+        f.find(a, blocks, lens, runs, sp.passes);  // (the next entry is on its way while this one's copies are issued)
+        const int st = st0 + (fetched & (depth - 1)), r = x.row(a, blocks);
         if (groups > 1) {
-            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&empty[st], ((fetched / depth) & 1) ^ 1, tmo));
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&empty[st], ((fetched >> lg_depth) & 1) ^ 1, tmo));
             if (!ok) return;
         }
         ++fetched;
         if (lane == 0) {
             tc::mbar_arrive_expect_tx(&full[st], LY::kStage);
             unsigned char* base = smem + st * LY::kStage;
-            tc::tma_load_3d(base, &tmK, &full[st], 0, h, r, policy);
-            tc::tma_load_3d(base + LY::kHalf, &tmV, &full[st], 0, h, r, policy);
+            tc::tma_load_3d(base, &tmK, &full[st], 0, x.h, r, policy);
+            tc::tma_load_3d(base + LY::kHalf, &tmV, &full[st], 0, x.h, r, policy);
             if (r < a.kv.rows) {
-                const int64_t page = (int64_t)(r >> lg_page) * Hkv + h;
+                const int64_t page = (int64_t)(r >> lg_page) * Hkv + x.h;
                 tc::copy4_async(&scale_s[st].x, c8.k_scale + page);
                 tc::copy4_async(&scale_s[st].y, c8.v_scale + page);
                 tc::copies_arrive(&full[st]);
             } else {
-                scale_s[st] = make_float2(0.f, 0.f);
+                scale_s[st] = make_float2(0.f, 1.f);
                 tc::mbar_arrive(&full[st]);
             }
         }
@@ -284,9 +318,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
         const int64_t q_row = (int64_t)w.s * a.n_head + (int64_t)h * G;
         fetch_q();
         const int hd = lane >> 2, tq = lane & 3;  // this lane's head (or column block of V) and quarter
-        float o[2 * kCols];  // head hd, columns kCols (2 tq + e) + j at [2 j + e]
+        // head hd, columns kCols (2 tq + e) + j: the sum over P at [j][e], over its remainders at [j][2 + e]
+        float o[kCols][4];
 #pragma unroll
-        for (int i = 0; i < 2 * kCols; ++i) o[i] = 0.f;
+        for (int j = 0; j < kCols; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
         float m = -INFINITY, l = 0.f;
         if (ok) {
             ok = __all_sync(0xffffffffu, tc::mbar_wait(&q_full[seg & 1], (seg >> 1) & 1, tmo));
@@ -325,9 +360,9 @@ __global__ void __launch_bounds__(kThreads8, 1)
         // first unit of the segment that falls to this stream
         int i = (stream - it) & (streams - 1);
         for (; i < n_seg; i += streams) {
-            const int st = st0 + used % depth;
+            const int st = st0 + (used & (depth - 1));
             if (ok) {
-                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[st], (used / depth) & 1, tmo));
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[st], (used >> lg_depth) & 1, tmo));
                 if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb2, it + i);
             }
             if (!ok) break;
@@ -346,8 +381,6 @@ __global__ void __launch_bounds__(kThreads8, 1)
             // (the four tiles of keys in turn: each one's products wait for one another)
             float s4[4][4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) s4[t][0] = s4[t][1] = s4[t][2] = s4[t][3] = 0.f;
-#pragma unroll
             for (int c = 0; c < D / 64; ++c) {
                 uint4 b[4];
 #pragma unroll
@@ -359,18 +392,20 @@ __global__ void __launch_bounds__(kThreads8, 1)
                         const int j = 4 * c + e;
                         uint32_t b0, b1;
                         pairs8<I8>(e == 0 ? b[t].x : e == 1 ? b[t].y : e == 2 ? b[t].z : b[t].w, b0, b1);
-                        mma8(s4[t], qh[2 * j], LO ? ql[LO ? 2 * j : 0] : 0u, qh[2 * j + 1],
-                                        LO ? ql[LO ? 2 * j + 1 : 0] : 0u, b0, b1);
+                        const uint32_t a1 = LO ? ql[LO ? 2 * j : 0] : 0u, a3 = LO ? ql[LO ? 2 * j + 1 : 0] : 0u;
+                        if (j == 0) mma8_first(s4[t], qh[0], a1, qh[1], a3, b0, b1);
+                        else mma8(s4[t], qh[2 * j], a1, qh[2 * j + 1], a3, b0, b1);
                     }
             }
-            const float slk = sl * sc.x;
+            // log2 of the weight times V's scale: that is what O is the sum of
+            const float slk = sl * sc.x, lv = __log2f(sc.y);
             float mx = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     if constexpr (LO) s4[t][e] = fmaf(s4[t][e + 2], 1.f / kLow8, s4[t][e]);
-                    s4[t][e] = t * 8 + 2 * tq + e < lim ? s4[t][e] * slk : -INFINITY;
+                    s4[t][e] = t * 8 + 2 * tq + e < lim ? fmaf(s4[t][e], slk, lv) : -INFINITY;
                     mx = fmaxf(mx, s4[t][e]);
                 }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -382,20 +417,24 @@ __global__ void __launch_bounds__(kThreads8, 1)
                 if (need) m = mx - kUp8;
                 l *= alpha;
 #pragma unroll
-                for (int j = 0; j < 2 * kCols; ++j) o[j] *= alpha;
+                for (int j = 0; j < kCols; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] *= alpha;
             }
             const float ms = m == -INFINITY ? 0.f : m;
             uint32_t p[2][4];
+            float sum = 0.f;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     float x = ex2(s4[2 * b + t][0] - ms), y = ex2(s4[2 * b + t][1] - ms);
-                    l += x + y;
+                    sum += x + y;
                     p[b][2 * t] = split2<false>(x, y);
                     x *= kLow8, y *= kLow8;
                     p[b][2 * t + 1] = split2<false>(x, y);
                 }
+            l = fmaf(sum, ex2(-lv), l);  // (the weights alone)
             // rows 16 b + 8 t + 2 tq + {0, 1} of V, D / 8 columns from D / 8 hd
             uint32_t v[2][2][2][D / 32];
 #pragma unroll
@@ -413,12 +452,8 @@ __global__ void __launch_bounds__(kThreads8, 1)
                             v[b][t][e][0] = x.x, v[b][t][e][1] = x.y;
                         }
                     }
-            const float lo = sc.y * (1.f / kLow8);
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-                float t4[4][4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) t4[j][0] = t4[j][1] = t4[j][2] = t4[j][3] = 0.f;
+            for (int x = 0; x < D / 32; ++x)
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     uint32_t b0[4], b1[4];
@@ -427,17 +462,8 @@ __global__ void __launch_bounds__(kThreads8, 1)
                     pairs8<I8>(prmt(v[b][1][0][x], v[b][1][1][x], 0x5140), b1[0], b1[1]);
                     pairs8<I8>(prmt(v[b][1][0][x], v[b][1][1][x], 0x7362), b1[2], b1[3]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        mma8(t4[j], p[b][0], p[b][1], p[b][2], p[b][3], b0[j], b1[j]);
+                    for (int j = 0; j < 4; ++j) mma8(o[4 * x + j], p[b][0], p[b][1], p[b][2], p[b][3], b0[j], b1[j]);
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& y = o[2 * (4 * x + j) + e];
-                        y = fmaf(t4[j][e], sc.y, fmaf(t4[j][e + 2], lo, y));
-                    }
-            }
             __syncwarp();
             if (groups > 1 && lane == 0) tc::mbar_arrive(&empty[st]);
             if (grp == 0 && f.more()) fetch();
@@ -458,12 +484,14 @@ __global__ void __launch_bounds__(kThreads8, 1)
             for (int r = 0; r < kWarps8; ++r)
                 if (r < streams) mt = fmaxf(mt, ml[(r * groups + grp) * 8 + hd].x);
             const float f = ex2(m - (mt == -INFINITY ? 0.f : mt));
+            auto whole_sum = [](const float (&x)[4], int e) { return fmaf(x[2 + e], 1.f / kLow8, x[e]); };
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int j = 0; j < kCols; j += 4)
                     *reinterpret_cast<float4*>(om_w + hd * D + kCols * (2 * tq + e) + j) =
-                        make_float4(o[2 * j + e] * f, o[2 * j + 2 + e] * f, o[2 * j + 4 + e] * f, o[2 * j + 6 + e] * f);
+                        make_float4(whole_sum(o[j], e) * f, whole_sum(o[j + 1], e) * f, whole_sum(o[j + 2], e) * f,
+                                    whole_sum(o[j + 3], e) * f);
         }
         tc::named_bar_sync(1, kWarps8 * 32);
         const bool whole = w.u == 0 && n_seg == w.units;
@@ -525,7 +553,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
     if (!ok) {
         // copies still in flight land before the CTA ends
         if (lane == 0) report_error(a.err, kDevWaitDecode, 0xb1, used);
-        for (int j = max(0, fetched - depth); j < fetched; ++j) tc::mbar_wait(&full[st0 + j % depth], (j / depth) & 1, tmo);
+        for (int j = max(0, fetched - depth); j < fetched; ++j) tc::mbar_wait(&full[st0 + (j & (depth - 1))], (j >> lg_depth) & 1, tmo);
         for (int j = max(0, n_q - 2); j < n_q; ++j) tc::mbar_wait(&q_full[j & 1], (j >> 1) & 1, tmo);
     }
 }
