@@ -8,23 +8,26 @@
 // quantised into the cache by k9_append first.
 //
 // CTA: units (32 rows of one head, so one scale each of K and V) go round robin
-// to the streams of 8 warps, each with its own online softmax over 8 query heads
+// to the streams of 16 warps, each with its own online softmax over 8 query heads
 // (groups of more than 8 heads give a unit to 2, 4 or 8 warps).  A stream has
-// its own stages and fetches for itself: K and V by TMA, the two scales by
-// cp.async on the same barrier.
+// its own stages and fetches for itself, K as soon as the scores are made, V
+// once it is summed: by TMA, the two scales by cp.async on K's barrier.
 //
-// S = Q K^T and O = P V on mma.sync m16n8k16 in f16, which holds both 8-bit
-// types exactly.  The order of the contracted dimension is free, so a lane
-// takes 16 neighbouring bytes of a K row (its fragments of four steps) and the
-// bytes of one column block of V from the rows it needs: 16-byte reads without
-// a transpose, and one byte permutation pairs two rows of V.  q is scaled to a
+// S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16 in f16, which holds both
+// 8-bit types exactly: keys, then columns of V, on the 16 side and 8 query heads
+// on the other, so no row of the tensor work is empty, and O takes 32 registers,
+// which leaves room for 16 warps (8 with heads on the 16 side: 38.8 us for 64 K
+// rows, issue slots 37 % busy).  The order of the contracted dimension is free, so a lane takes
+// 16 neighbouring bytes of a K row (its fragments of four steps) and the bytes
+// of one column block of V from the rows it needs: 16-byte reads without a
+// transpose, and one byte permutation pairs two rows of V.  q is scaled to a
 // largest magnitude of 2^14 to 2^15 by a power of two, so f16 takes its 16-bit
-// types as they are; an f32 q has its rounding remainder (times 2^12) in rows
-// 8-15.  P is the weight times V's scale, against the running maximum of just
-// that, so that units of other scales add up in the accumulators as they are;
-// the weights' sum takes P over the scale.  P is held 2^7 up (2^15 at most);
-// rows 8-15 of its operand carry its rounding remainder, times 2^12: an element
-// keeps 22 bits of itself and an absolute 2^-44 of the largest.
+// types as they are; an f32 q is two f16 (a second product).  P is the weight
+// times V's scale, against the running maximum of just that, so that units of
+// other scales add up in the accumulators as they are; the weights' sum takes P
+// over the scale.  The largest P is held between 2^14 and 2^15, and P is two
+// f16: an element keeps 22 bits of itself and an absolute 2^-39 of the largest
+// (half of f16's smallest step).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -43,8 +46,8 @@ namespace {
 
 constexpr int kWarps8 = 8;
 constexpr int kThreads8 = kWarps8 * 32;
-constexpr float kUp8 = 7.f;       // P is 2^7 times the weight against the running maximum (2^15 at most)
-constexpr float kLow8 = 4096.f;   // factor of a remainder
+constexpr float kUp8 = 14.f;      // P is 2^14 times what it is against the running maximum,
+constexpr float kSlack8 = 1.f;    // which follows when it is twice that behind: 2^15 at most
 constexpr int kPass8 = 64;        // query heads of a pass, at most
 
 template <int D>
@@ -58,7 +61,7 @@ struct Layout8 {
     static constexpr int kOffMl = kOffO + kWarps8 * 8 * D * 4;
     static constexpr int kOffScale = kOffMl + 2 * kWarps8 * 8 * 8;  // [kStages] (ks, vs)
     static constexpr int kOffBar = kOffScale + kStages * 8;
-    static constexpr int kOffLens = kOffBar + (2 * kStages + 2) * 8;
+    static constexpr int kOffLens = kOffBar + (4 * kStages + 2) * 8;
     static constexpr int kBytes = kOffLens + kLensOnChip * 4;
     static_assert(kStages % kWarps8 == 0 && kBytes + 1024 <= 232448, "shared memory");
 };
@@ -96,6 +99,12 @@ __device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, ui
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The 8 x 8 tile of 16-bit values (row lane / 4, columns 2 (lane % 4) + {0, 1}) turned over.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 // D = A B.
 __device__ __forceinline__ void mma8_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -176,12 +185,15 @@ __global__ void __launch_bounds__(kThreads8, 1)
     k10_decode8(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
                 const Cache8 c8, const DecodeSplit sp) {
     using LY = Layout8<D>;
-    constexpr int kSteps = D / 16, kCols = D / 8;  // steps of a score, columns (of 8 lanes) of an output
+    constexpr int kSteps = D / 16, kCols = D / 8;  // steps of a score; columns of an output that a lane has
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
-    uint64_t* empty = full + LY::kStages;
-    uint64_t* q_full = empty + LY::kStages;
+    // of a stage's K and V each: landed, and (where warps share a stage) done with
+    uint64_t* full_k = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
+    uint64_t* full_v = full_k + LY::kStages;
+    uint64_t* empty_k = full_v + LY::kStages;
+    uint64_t* empty_v = empty_k + LY::kStages;
+    uint64_t* q_full = empty_v + LY::kStages;
     int32_t* lens_s = reinterpret_cast<int32_t*>(smem + LY::kOffLens);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int Hkv = a.n_head_kv, G = a.n_head / Hkv, es = a.dtype == 0 ? 4 : 2;
@@ -189,8 +201,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < LY::kStages; ++i) {
-            tc::mbar_init(&full[i], 2);  // the bytes' announcement, and the scales
-            tc::mbar_init(&empty[i], sp.groups);
+            tc::mbar_init(&full_k[i], 2);  // the bytes' announcement, and the scales
+            tc::mbar_init(&full_v[i], 1);
+            tc::mbar_init(&empty_k[i], sp.groups);
+            tc::mbar_init(&empty_v[i], sp.groups);
         }
         for (int i = 0; i < 2; ++i) tc::mbar_init(&q_full[i], 1);
         tc::fence_mbar_init();
@@ -255,35 +269,46 @@ __global__ void __launch_bounds__(kThreads8, 1)
     bool ok = true;
 
     // The stream's first warp fetches for it, a stage as soon as its warps are
-    // done with it: eight warps issue copies, which one alone does at no more
-    // than 5.2 TB/s (over all SMs, 8 KB units).
+    // done with it: all issue copies, which one alone does at no more than
+    // 5.2 TB/s (over all SMs, 8 KB units).
     Fetch f{w0, w0.run / sp.passes, 0, stream, 0, 0};
-    int fetched = 0;
+    int fetched = 0, row_v = 0, head_v = 0;  // units whose K was asked for; the last one's place, for V
     if (grp == 0) f.find(a, blocks, lens, runs, sp.passes);
-    auto fetch = [&]() {
+    auto fetch_k = [&]() {
         const Fetch x = f;
         f.at += streams;
         f.find(a, blocks, lens, runs, sp.passes);  // (the next entry is on its way while this one's copies are issued)
-        const int st = st0 + (fetched & (depth - 1)), r = x.row(a, blocks);
-        if (groups > 1) {
-            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&empty[st], ((fetched >> lg_depth) & 1) ^ 1, tmo));
-            if (!ok) return;
-        }
+        const int st = st0 + (fetched & (depth - 1));
+        row_v = x.row(a, blocks), head_v = x.h;
+        if (groups > 1)
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&empty_k[st], ((fetched >> lg_depth) & 1) ^ 1, tmo));
+        if (!ok) return;
         ++fetched;
         if (lane == 0) {
-            tc::mbar_arrive_expect_tx(&full[st], LY::kStage);
-            unsigned char* base = smem + st * LY::kStage;
-            tc::tma_load_3d(base, &tmK, &full[st], 0, x.h, r, policy);
-            tc::tma_load_3d(base + LY::kHalf, &tmV, &full[st], 0, x.h, r, policy);
-            if (r < a.kv.rows) {
-                const int64_t page = (int64_t)(r >> lg_page) * Hkv + x.h;
+            tc::mbar_arrive_expect_tx(&full_k[st], LY::kHalf);
+            tc::tma_load_3d(smem + st * LY::kStage, &tmK, &full_k[st], 0, head_v, row_v, policy);
+            if (row_v < a.kv.rows) {
+                const int64_t page = (int64_t)(row_v >> lg_page) * Hkv + head_v;
                 tc::copy4_async(&scale_s[st].x, c8.k_scale + page);
                 tc::copy4_async(&scale_s[st].y, c8.v_scale + page);
-                tc::copies_arrive(&full[st]);
+                tc::copies_arrive(&full_k[st]);
             } else {
                 scale_s[st] = make_float2(0.f, 1.f);
-                tc::mbar_arrive(&full[st]);
+                tc::mbar_arrive(&full_k[st]);
             }
+        }
+        __syncwarp();
+    };
+    int fetched_v = 0;
+    auto fetch_v = [&]() {  // of the unit whose K was asked for last
+        const int st = st0 + (fetched_v & (depth - 1));
+        if (groups > 1)
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&empty_v[st], ((fetched_v >> lg_depth) & 1) ^ 1, tmo));
+        if (!ok) return;
+        ++fetched_v;
+        if (lane == 0) {
+            tc::mbar_arrive_expect_tx(&full_v[st], LY::kHalf);
+            tc::tma_load_3d(smem + st * LY::kStage + LY::kHalf, &tmV, &full_v[st], 0, head_v, row_v, policy);
         }
         __syncwarp();
     };
@@ -305,7 +330,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
         }
     };
     fetch_q();
-    for (int i = 0; i < depth && grp == 0 && f.more(); ++i) fetch();
+    for (int i = 0; i < depth && grp == 0 && f.more(); ++i) {
+        fetch_k();
+        fetch_v();
+    }
 
     float* om = reinterpret_cast<float*>(smem + LY::kOffO);
     float* om_w = om + warp * 8 * D;
@@ -317,19 +345,20 @@ __global__ void __launch_bounds__(kThreads8, 1)
         const int g0 = pass * sp.pass_heads + grp * 8;  // this warp's first query head of the group
         const int64_t q_row = (int64_t)w.s * a.n_head + (int64_t)h * G;
         fetch_q();
-        const int hd = lane >> 2, tq = lane & 3;  // this lane's head (or column block of V) and quarter
-        // head hd, columns kCols (2 tq + e) + j: the sum over P at [j][e], over its remainders at [j][2 + e]
-        float o[kCols][4];
+        // lane: row hd of a 16-row tile and of its second half; columns 2 tq + {0, 1}
+        const int hd = lane >> 2, tq = lane & 3;
+        // columns D / 8 hd + 2 i + {0, 1} of heads 2 tq + {0, 1}: [i][column * 2 + head]
+        float o[D / 16][4];
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-        float m = -INFINITY, l = 0.f;
+        for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of heads 2 tq + {0, 1}
         if (ok) {
             ok = __all_sync(0xffffffffu, tc::mbar_wait(&q_full[seg & 1], (seg >> 1) & 1, tmo));
             if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb3, seg);
         }
         // q in f16, dims D / 4 tq + 4 j + {0, 1, 2, 3} for step j
         uint32_t qh[2 * kSteps], ql[LO ? 2 * kSteps : 1];
-        float sl;
+        float sl[2];  // factor of the scores of heads 2 tq + {0, 1}
         {
             const unsigned char* qs = smem + LY::kOffQ + (seg & 1) * LY::kQBytes + (grp * 8 + hd) * D * es;
             float4 x[kSteps];
@@ -344,14 +373,15 @@ __global__ void __launch_bounds__(kThreads8, 1)
             const int e = (int)(__float_as_uint(top) >> 23) - 127;
             const int up = e < 128 ? min(14 - e, 126) : 0;  // (at least -113)
             const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-            sl = a.kq_scale * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23);
+            const float back = a.kq_scale * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23);
+            sl[0] = __shfl_sync(0xffffffffu, back, 8 * tq);
+            sl[1] = __shfl_sync(0xffffffffu, back, 8 * tq + 4);
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) {
                 x[j].x *= f, x[j].y *= f, x[j].z *= f, x[j].w *= f;
                 qh[2 * j] = split2<false>(x[j].x, x[j].y);
                 qh[2 * j + 1] = split2<false>(x[j].z, x[j].w);
                 if constexpr (LO) {
-                    x[j].x *= kLow8, x[j].y *= kLow8, x[j].z *= kLow8, x[j].w *= kLow8;
                     ql[2 * j] = split2<false>(x[j].x, x[j].y);
                     ql[2 * j + 1] = split2<false>(x[j].z, x[j].w);
                 }
@@ -361,15 +391,96 @@ __global__ void __launch_bounds__(kThreads8, 1)
         int i = (stream - it) & (streams - 1);
         for (; i < n_seg; i += streams) {
             const int st = st0 + (used & (depth - 1));
+            const uint32_t phase = (used >> lg_depth) & 1;
             if (ok) {
-                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[st], (used >> lg_depth) & 1, tmo));
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full_k[st], phase, tmo));
                 if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb2, it + i);
             }
             if (!ok) break;
-            ++used;
             unsigned char* stage = smem + st * LY::kStage;
-            const int u = w.u + i, lim = min(kUnit, w.n - u * kUnit);
             const unsigned char* vb = stage + LY::kHalf;
+            const int u = w.u + i, lim = min(kUnit, w.n - u * kUnit);
+            const float2 sc = scale_s[st];
+            // scores of keys 16 b + hd and 16 b + 8 + hd: [b][half * 2 + head]; the sum of even steps and that of
+            // odd ones (each one's products wait for one another)
+            float s4[2][4], s5[2][4];
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                uint4 k4[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    k4[t] = *reinterpret_cast<const uint4*>(stage + tile_at<D>(t * 8 + hd, (D / 64) * tq + c));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const int j = 4 * c + e;
+                        auto word = [&](const uint4& x) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; };
+                        uint32_t a0, a1, a2, a3;
+                        pairs8<I8>(word(k4[2 * b]), a0, a2);
+                        pairs8<I8>(word(k4[2 * b + 1]), a1, a3);
+                        float(&x)[4] = j & 1 ? s5[b] : s4[b];
+                        if (j < 2) mma8_first(x, a0, a1, a2, a3, qh[2 * j], qh[2 * j + 1]);
+                        else mma8(x, a0, a1, a2, a3, qh[2 * j], qh[2 * j + 1]);
+                        if constexpr (LO) mma8(x, a0, a1, a2, a3, ql[2 * j], ql[2 * j + 1]);
+                    }
+            }
+            __syncwarp();
+            if (groups > 1 && lane == 0) tc::mbar_arrive(&empty_k[st]);
+            if (grp == 0 && f.more()) fetch_k();
+            // log2 of the weight times V's scale: that is what O is the sum of
+            const float lv = __log2f(sc.y);
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s4[b][e] = fmaf(s4[b][e] + s5[b][e], sl[e & 1] * sc.x, lv);
+            if (lim < kUnit) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (16 * b + 8 * (e >> 1) + hd >= lim) s4[b][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e & 1] = fmaxf(mx[e & 1], s4[b][e]);
+            // (the maximum over the lanes is wanted where one of them is past the running one only)
+            if (__any_sync(0xffffffffu, mx[0] > m[0] + (kUp8 + kSlack8) || mx[1] > m[1] + (kUp8 + kSlack8))) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+                const bool need0 = mx[0] > m[0] + (kUp8 + kSlack8), need1 = mx[1] > m[1] + (kUp8 + kSlack8);
+                const float alpha0 = need0 ? ex2(m[0] - (mx[0] - kUp8)) : 1.f;
+                const float alpha1 = need1 ? ex2(m[1] - (mx[1] - kUp8)) : 1.f;
+                if (need0) m[0] = mx[0] - kUp8;
+                if (need1) m[1] = mx[1] - kUp8;
+                l[0] *= alpha0, l[1] *= alpha1;
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) o[j][0] *= alpha0, o[j][1] *= alpha1, o[j][2] *= alpha0, o[j][3] *= alpha1;
+            }
+            const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+            uint32_t ph[2][2], pl[2][2];  // keys 16 b + 8 half + 2 tq + {0, 1} of head hd
+            float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    float x = ex2(s4[b][2 * t] - m0), y = ex2(s4[b][2 * t + 1] - m1);
+                    sum0 += x, sum1 += y;
+                    ph[b][t] = turned(split2<false>(x, y));
+                    pl[b][t] = turned(split2<false>(x, y));
+                }
+            const float rv = ex2(-lv);
+            l[0] = fmaf(sum0, rv, l[0]), l[1] = fmaf(sum1, rv, l[1]);  // (the weights alone)
+            if (ok) {
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full_v[st], phase, tmo));
+                if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb4, it + i);
+            }
+            ++used;
+            if (!ok) break;
             if (!I8 && lim < kUnit) {
                 // V rows past the length may hold NaN codes: their P is 0, and 0 * NaN is not 0
                 for (int j = lane; j < (kUnit - lim) * (D / 16); j += 32)
@@ -377,68 +488,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes the stage next
                 __syncwarp();
             }
-            const float2 sc = scale_s[st];
-            // (the four tiles of keys in turn: each one's products wait for one another)
-            float s4[4][4];
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-                uint4 b[4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) b[t] = *reinterpret_cast<const uint4*>(stage + tile_at<D>(t * 8 + hd, (D / 64) * tq + c));
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const int j = 4 * c + e;
-                        uint32_t b0, b1;
-                        pairs8<I8>(e == 0 ? b[t].x : e == 1 ? b[t].y : e == 2 ? b[t].z : b[t].w, b0, b1);
-                        const uint32_t a1 = LO ? ql[LO ? 2 * j : 0] : 0u, a3 = LO ? ql[LO ? 2 * j + 1 : 0] : 0u;
-                        if (j == 0) mma8_first(s4[t], qh[0], a1, qh[1], a3, b0, b1);
-                        else mma8(s4[t], qh[2 * j], a1, qh[2 * j + 1], a3, b0, b1);
-                    }
-            }
-            // log2 of the weight times V's scale: that is what O is the sum of
-            const float slk = sl * sc.x, lv = __log2f(sc.y);
-            float mx = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    if constexpr (LO) s4[t][e] = fmaf(s4[t][e + 2], 1.f / kLow8, s4[t][e]);
-                    s4[t][e] = t * 8 + 2 * tq + e < lim ? fmaf(s4[t][e], slk, lv) : -INFINITY;
-                    mx = fmaxf(mx, s4[t][e]);
-                }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // the running maximum follows when it is 2^8 behind
-            const bool need = mx > m + (8.f + kUp8);
-            if (__any_sync(0xffffffffu, need)) {
-                const float alpha = need ? ex2(m - (mx - kUp8)) : 1.f;
-                if (need) m = mx - kUp8;
-                l *= alpha;
-#pragma unroll
-                for (int j = 0; j < kCols; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] *= alpha;
-            }
-            const float ms = m == -INFINITY ? 0.f : m;
-            uint32_t p[2][4];
-            float sum = 0.f;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    float x = ex2(s4[2 * b + t][0] - ms), y = ex2(s4[2 * b + t][1] - ms);
-                    sum += x + y;
-                    p[b][2 * t] = split2<false>(x, y);
-                    x *= kLow8, y *= kLow8;
-                    p[b][2 * t + 1] = split2<false>(x, y);
-                }
-            l = fmaf(sum, ex2(-lv), l);  // (the weights alone)
-            // rows 16 b + 8 t + 2 tq + {0, 1} of V, D / 8 columns from D / 8 hd
-            uint32_t v[2][2][2][D / 32];
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < 2; ++b) {
+                // rows 16 b + 8 t + 2 tq + {0, 1} of V, D / 8 columns from D / 8 hd
+                uint32_t v[2][2][D / 32];
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -446,78 +499,88 @@ __global__ void __launch_bounds__(kThreads8, 1)
                         const int r = 16 * b + 8 * t + 2 * tq + e;
                         if constexpr (D == 128) {
                             const uint4 x = *reinterpret_cast<const uint4*>(vb + tile_at<D>(r, hd));
-                            v[b][t][e][0] = x.x, v[b][t][e][1] = x.y, v[b][t][e][2] = x.z, v[b][t][e][3] = x.w;
+                            v[t][e][0] = x.x, v[t][e][1] = x.y, v[t][e][2] = x.z, v[t][e][3] = x.w;
                         } else {
                             const uint2 x = *reinterpret_cast<const uint2*>(vb + tile_at<D>(r, hd >> 1) + (hd & 1) * 8);
-                            v[b][t][e][0] = x.x, v[b][t][e][1] = x.y;
+                            v[t][e][0] = x.x, v[t][e][1] = x.y;
                         }
                     }
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x)
+                for (int x = 0; x < D / 32; ++x) {
+                    uint32_t a0[4], a1[4];  // [tile * 2 + column]
+                    pairs8<I8>(prmt(v[0][0][x], v[0][1][x], 0x5140), a0[0], a0[1]);
+                    pairs8<I8>(prmt(v[0][0][x], v[0][1][x], 0x7362), a0[2], a0[3]);
+                    pairs8<I8>(prmt(v[1][0][x], v[1][1][x], 0x5140), a1[0], a1[1]);
+                    pairs8<I8>(prmt(v[1][0][x], v[1][1][x], 0x7362), a1[2], a1[3]);
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    uint32_t b0[4], b1[4];
-                    pairs8<I8>(prmt(v[b][0][0][x], v[b][0][1][x], 0x5140), b0[0], b0[1]);
-                    pairs8<I8>(prmt(v[b][0][0][x], v[b][0][1][x], 0x7362), b0[2], b0[3]);
-                    pairs8<I8>(prmt(v[b][1][0][x], v[b][1][1][x], 0x5140), b1[0], b1[1]);
-                    pairs8<I8>(prmt(v[b][1][0][x], v[b][1][1][x], 0x7362), b1[2], b1[3]);
+                    for (int j = 0; j < 2; ++j)
+                        mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], ph[b][0], ph[b][1]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma8(o[4 * x + j], p[b][0], p[b][1], p[b][2], p[b][3], b0[j], b1[j]);
+                    for (int j = 0; j < 2; ++j)
+                        mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], pl[b][0], pl[b][1]);
                 }
+            }
             __syncwarp();
-            if (groups > 1 && lane == 0) tc::mbar_arrive(&empty[st]);
-            if (grp == 0 && f.more()) fetch();
+            if (groups > 1 && lane == 0) tc::mbar_arrive(&empty_v[st]);
+            if (grp == 0 && fetched_v < fetched) fetch_v();
         }
 
         // ------------------------------------------- merge the warps' states
         // (ml alternates between two buffers: a warp may write the next
         // segment's before another has read this one's sums)
         float2* ml = reinterpret_cast<float2*>(smem + LY::kOffMl) + (seg & 1) * kWarps8 * 8;
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (tq == 0) ml[warp * 8 + hd] = make_float2(m, l);
-        tc::named_bar_sync(1, kWarps8 * 32);
-        {
-            // the streams' common maximum of this lane's head
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+        if (hd == 0) {
+            ml[warp * 8 + 2 * tq] = make_float2(m[0], l[0]);
+            ml[warp * 8 + 2 * tq + 1] = make_float2(m[1], l[1]);
+        }
+        tc::named_bar_sync(1, kThreads8);
+        // against the streams' common maximum
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
             float mt = -INFINITY;
 #pragma unroll
             for (int r = 0; r < kWarps8; ++r)
-                if (r < streams) mt = fmaxf(mt, ml[(r * groups + grp) * 8 + hd].x);
-            const float f = ex2(m - (mt == -INFINITY ? 0.f : mt));
-            auto whole_sum = [](const float (&x)[4], int e) { return fmaf(x[2 + e], 1.f / kLow8, x[e]); };
+                if (r < streams) mt = fmaxf(mt, ml[(r * groups + grp) * 8 + 2 * tq + e].x);
+            const float f = ex2(m[e] - (mt == -INFINITY ? 0.f : mt));
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int j = 0; j < kCols; j += 4)
-                    *reinterpret_cast<float4*>(om_w + hd * D + kCols * (2 * tq + e) + j) =
-                        make_float4(whole_sum(o[j], e) * f, whole_sum(o[j + 1], e) * f, whole_sum(o[j + 2], e) * f,
-                                    whole_sum(o[j + 3], e) * f);
+            for (int j = 0; j < D / 16; ++j) o[j][e] *= f, o[j][2 + e] *= f;
         }
-        tc::named_bar_sync(1, kWarps8 * 32);
+        auto place = [&](int e, int j) {
+            return reinterpret_cast<float4*>(om_w + (2 * tq + e) * D + kCols * hd + 2 * j);
+        };
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < D / 16; j += 2)
+                *place(e, j) = make_float4(o[j][e], o[j][2 + e], o[j + 1][e], o[j + 1][2 + e]);
+        tc::named_bar_sync(1, kThreads8);
         const bool whole = w.u == 0 && n_seg == w.units;
         const int n_heads = min(min(groups * 8, sp.pass_heads), G - pass * sp.pass_heads);
         const int slot = blockIdx.x * 2 + (seg == 0 ? 0 : 1);
-        for (int j = threadIdx.x; j < n_heads * (D / 4); j += kWarps8 * 32) {
+        for (int j = threadIdx.x; j < n_heads * (D / 4); j += kThreads8) {
             const int g = j / (D / 4), c = j % (D / 4), gw = g >> 3, gh = g & 7;
-            float2 v[kWarps8];
-            float4 t[kWarps8];
             float mt = -INFINITY;
 #pragma unroll
             for (int r = 0; r < kWarps8; ++r)
-                if (r < streams) {
-                    const int wr = (r * groups + gw) * 8 + gh;
-                    v[r] = ml[wr];
-                    t[r] = *reinterpret_cast<const float4*>(om + wr * D + c * 4);
-                    mt = fmaxf(mt, v[r].x);
-                }
+                if (r < streams) mt = fmaxf(mt, ml[(r * groups + gw) * 8 + gh].x);
             const float ms = mt == -INFINITY ? 0.f : mt;
             float lt = 0.f;
             float4 ot = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int r = 0; r < kWarps8; ++r)
                 if (r < streams) {
-                    lt += v[r].y * ex2(v[r].x - ms);
-                    ot.x += t[r].x, ot.y += t[r].y, ot.z += t[r].z, ot.w += t[r].w;
+                    const float2 v = ml[(r * groups + gw) * 8 + gh];
+                    lt += v.y * ex2(v.x - ms);
+                }
+#pragma unroll
+            for (int r = 0; r < kWarps8; ++r)
+                if (r < streams) {
+                    const float4 t = *reinterpret_cast<const float4*>(om + ((r * groups + gw) * 8 + gh) * D + c * 4);
+                    ot.x += t.x, ot.y += t.y, ot.z += t.z, ot.w += t.w;
                 }
             if constexpr (JOIN) {
                 // (the ring: this CTA's last copy has landed)
@@ -534,7 +597,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
             }
         }
         if constexpr (JOIN) {
-            join_cluster<D, kWarps8 * 32, kPass8>(a, sp, smem, om, w, n_seg, q_row + pass * sp.pass_heads, n_heads, h,
+            join_cluster<D, kThreads8, kPass8>(a, sp, smem, om, w, n_seg, q_row + pass * sp.pass_heads, n_heads, h,
                                                   rank);
             if (C > 1) tc::cluster_sync();  // nobody reads this CTA's part any more
         }
@@ -553,7 +616,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
     if (!ok) {
         // copies still in flight land before the CTA ends
         if (lane == 0) report_error(a.err, kDevWaitDecode, 0xb1, used);
-        for (int j = max(0, fetched - depth); j < fetched; ++j) tc::mbar_wait(&full[st0 + (j & (depth - 1))], (j >> lg_depth) & 1, tmo);
+        for (int j = max(0, fetched - depth); j < fetched; ++j) {
+            tc::mbar_wait(&full_k[st0 + (j & (depth - 1))], (j >> lg_depth) & 1, tmo);
+            if (j < fetched_v) tc::mbar_wait(&full_v[st0 + (j & (depth - 1))], (j >> lg_depth) & 1, tmo);
+        }
         for (int j = max(0, n_q - 2); j < n_q; ++j) tc::mbar_wait(&q_full[j & 1], (j >> 1) & 1, tmo);
     }
 }

@@ -131,12 +131,15 @@ def decode64(cache, q, scale=None):
             qq = q[i, h * G:(h + 1) * G]
             p, mag = softmax64(qq, k[:, h], scale)
             lost = float((qq.double().abs().amax(1) * part).max() * k[:, h].abs().sum(1).max() * scale)
-            # numerator and denominator each carry one score error; weights keep 2^-22 of themselves and an absolute
-            # 2^-44 of the largest; a unit's sum of 32 and the sums over units (in f32) cut at most a step each
+            # numerator and denominator each carry one score error; a unit's sum of 32 and the sums over units (in f32)
+            # cut at most a step each.  Weights (times V's scale) are two f16: 2^-22 of themselves, and no finer than
+            # half of f16's smallest step, 2^-25, where the largest is 2^14 at least: n times 2^-39 of the largest
+            # meets bytes of at most TOP
             e = 2 * (score_error(mag, d) + lost)
             out[i, h * G:(h + 1) * G] = p @ v[:, h]
+            vs = cache.vs[cache.at(i, n).cuda() // cache.page, h].double()
             tol[i, h * G:(h + 1) * G] = ((p @ v[:, h].abs()) * (e + 2.0 ** -21 + (64 + n / 32) * 2.0 ** -23)
-                                         + n * 2.0 ** -43 * v[:, h].abs().max())
+                                         + n * 2.0 ** -39 * TOP[cache.q8] * (p * vs).amax(1, keepdim=True))
     return out, tol
 
 
