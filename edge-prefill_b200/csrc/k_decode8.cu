@@ -8,19 +8,18 @@
 // quantised into the cache by k9_append first.
 //
 // CTA: units (32 rows of one head, so one scale each of K and V) go round robin
-// to the streams of 16 warps, each with its own online softmax over 8 query heads
+// to the streams of 8 warps, each with its own online softmax over 8 query heads
 // (groups of more than 8 heads give a unit to 2, 4 or 8 warps).  A stream has
-// its own stages and fetches for itself, K as soon as the scores are made, V
-// once it is summed: by TMA, the two scales by cp.async on K's barrier.
+// its own stages; four more warps fetch, a lane for each stream: K and V by TMA,
+// the two scales by cp.async on the same barrier.
 //
 // S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16 in f16, which holds both
 // 8-bit types exactly: keys, then columns of V, on the 16 side and 8 query heads
-// on the other, so no row of the tensor work is empty, and O takes 32 registers,
-// which leaves room for 16 warps (8 with heads on the 16 side: 38.8 us for 64 K
-// rows, issue slots 37 % busy).  The order of the contracted dimension is free, so a lane takes
-// 16 neighbouring bytes of a K row (its fragments of four steps) and the bytes
-// of one column block of V from the rows it needs: 16-byte reads without a
-// transpose, and one byte permutation pairs two rows of V.  q is scaled to a
+// on the other, so no row of the tensor work is empty and O takes 32 registers.
+// The order of the contracted dimension is free, so a lane takes 16 neighbouring
+// bytes of a K row (its fragments of four steps) and the bytes of one column
+// block of V from the rows it needs: 16-byte reads without a transpose, and one
+// byte permutation pairs two rows of V.  q is scaled to a
 // largest magnitude of 2^14 to 2^15 by a power of two, so f16 takes its 16-bit
 // types as they are; an f32 q is two f16 (a second product).  P is the weight
 // times V's scale, against the running maximum of just that, so that units of
@@ -45,25 +44,40 @@ namespace epsp {
 namespace {
 
 constexpr int kWarps8 = 8;
-constexpr int kThreads8 = kWarps8 * 32;
+constexpr int kThreads8 = kWarps8 * 32;  // that attend
+constexpr int kFetchers = 4;             // warps that fetch
 constexpr float kUp8 = 14.f;      // P is 2^14 times what it is against the running maximum,
 constexpr float kSlack8 = 1.f;    // which follows when it is twice that behind: 2^15 at most
 constexpr int kPass8 = 64;        // query heads of a pass, at most
 
+// Shared memory: the stages, then what follows by offset.
 template <int D>
 struct Layout8 {
     static constexpr int kHalf = kUnit * D;      // K (or V) of a unit
     static constexpr int kStage = 2 * kHalf;
-    static constexpr int kStages = 131072 / kStage;  // dealt to the streams in equal parts
-    static constexpr int kOffQ = kStages * kStage;   // [2] queries of a segment
-    static constexpr int kQBytes = 16384;
-    static constexpr int kOffO = kOffQ + 2 * kQBytes;  // [kWarps8][8][D] merge buffer
-    static constexpr int kOffMl = kOffO + kWarps8 * 8 * D * 4;
-    static constexpr int kOffScale = kOffMl + 2 * kWarps8 * 8 * 8;  // [kStages] (ks, vs)
-    static constexpr int kOffBar = kOffScale + kStages * 8;
-    static constexpr int kOffLens = kOffBar + (4 * kStages + 2) * 8;
-    static constexpr int kBytes = kOffLens + kLensOnChip * 4;
-    static_assert(kStages % kWarps8 == 0 && kBytes + 1024 <= 232448, "shared memory");
+    static constexpr int kMost = 196608 / kStage;  // stages, at most
+    static constexpr int kMl = 2 * kWarps8 * 8 * 8;
+    int32_t stages;   // a multiple of the streams
+    int32_t q_bytes;  // of a segment's queries: two buffers
+    int32_t slots;    // of the merge buffer, [slots][8][D]
+    __host__ __device__ int off_q() const { return stages * kStage; }
+    __host__ __device__ int off_o() const { return off_q() + 2 * q_bytes; }
+    __host__ __device__ int off_ml() const { return off_o() + slots * 8 * D * 4; }
+    __host__ __device__ int off_scale() const { return off_ml() + kMl; }  // [stages] (ks, vs)
+    __host__ __device__ int off_bar() const { return off_scale() + kMost * 8; }
+    __host__ __device__ int off_lens() const { return off_bar() + (2 * kMost + 2) * 8; }
+    __host__ __device__ int bytes() const { return off_lens() + kLensOnChip * 4; }
+    // For `pass` query heads of `es` bytes and units shared by `groups` warps:
+    // as many stages as 227 KB hold.
+    static Layout8 make(int pass, int es, int groups) {
+        Layout8 l;
+        l.stages = 0;
+        l.q_bytes = pass * D * es;
+        l.slots = groups == kWarps8 ? kWarps8 : kWarps8 / 2;
+        const int streams = kWarps8 / groups;
+        l.stages = std::min(kMost, (232448 - 1024 - l.bytes()) / kStage) / streams * streams;
+        return l;
+    }
 };
 
 // Byte of row r, 16-byte chunk ch, in a swizzled tile of rows of D bytes.
@@ -181,30 +195,26 @@ struct Fetch {
 
 // LO: q has remainders (f32).  JOIN: the calls that join_cluster finishes.
 template <int D, bool I8, bool LO, bool JOIN>
-__global__ void __launch_bounds__(kThreads8, 1)
+__global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     k10_decode8(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
-                const Cache8 c8, const DecodeSplit sp) {
+                const Cache8 c8, const DecodeSplit sp, const Layout8<D> ly) {
     using LY = Layout8<D>;
+    constexpr int kAll = kThreads8 + 32 * kFetchers;
     constexpr int kSteps = D / 16, kCols = D / 8;  // steps of a score; columns of an output that a lane has
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
-    // of a stage's K and V each: landed, and (where warps share a stage) done with
-    uint64_t* full_k = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
-    uint64_t* full_v = full_k + LY::kStages;
-    uint64_t* empty_k = full_v + LY::kStages;
-    uint64_t* empty_v = empty_k + LY::kStages;
-    uint64_t* q_full = empty_v + LY::kStages;
-    int32_t* lens_s = reinterpret_cast<int32_t*>(smem + LY::kOffLens);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + ly.off_bar());
+    uint64_t* empty = full + LY::kMost;
+    uint64_t* q_full = empty + LY::kMost;
+    int32_t* lens_s = reinterpret_cast<int32_t*>(smem + ly.off_lens());
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int Hkv = a.n_head_kv, G = a.n_head / Hkv, es = a.dtype == 0 ? 4 : 2;
     const int runs = Hkv * sp.passes;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < LY::kStages; ++i) {
-            tc::mbar_init(&full_k[i], 2);  // the bytes' announcement, and the scales
-            tc::mbar_init(&full_v[i], 1);
-            tc::mbar_init(&empty_k[i], sp.groups);
-            tc::mbar_init(&empty_v[i], sp.groups);
+        for (int i = 0; i < ly.stages; ++i) {
+            tc::mbar_init(&full[i], 2);  // the bytes' announcement, and the scales
+            tc::mbar_init(&empty[i], sp.groups);
         }
         for (int i = 0; i < 2; ++i) tc::mbar_init(&q_full[i], 1);
         tc::fence_mbar_init();
@@ -231,7 +241,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
         w0.left = min(per, w0.units - w0.u);
     } else {
         if (a.kv.n_seq <= kLensOnChip) {
-            for (int s = threadIdx.x; s < a.kv.n_seq; s += kThreads8) lens_s[s] = batch_len(a.kv, s, a.err);
+            for (int s = threadIdx.x; s < a.kv.n_seq; s += kAll) lens_s[s] = batch_len(a.kv, s, a.err);
             lens.chip = lens_s;
         }
         __syncthreads();
@@ -239,10 +249,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
         // sequences without rows, dealt out to the CTAs
         for (int s = blockIdx.x; s < a.kv.n_seq; s += gridDim.x)
             if (lens.at(a, s) == 0) {
-                for (int i = threadIdx.x; i < a.n_head * (D / 4); i += kThreads8)
+                for (int i = threadIdx.x; i < a.n_head * (D / 4); i += kAll)
                     store4(a.out, a.out_dtype, (int64_t)s * a.n_head * D + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
                 if (sp.by_run)
-                    for (int i = threadIdx.x; i < runs; i += kThreads8) sp.cut[s * runs + i] = make_int4(-1, 0, 0, 0);
+                    for (int i = threadIdx.x; i < runs; i += kAll) sp.cut[s * runs + i] = make_int4(-1, 0, 0, 0);
             }
         if (w0.left <= 0 && !sp.by_run && threadIdx.x == 0) sp.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
@@ -251,67 +261,75 @@ __global__ void __launch_bounds__(kThreads8, 1)
         if (sp.direct) {  // a sequence without rows
             const int g0 = (w0.run % sp.passes) * sp.pass_heads, n = min(sp.pass_heads, G - g0) * (D / 4);
             const int64_t at = ((int64_t)w0.s * a.n_head + (w0.run / sp.passes) * G + g0) * D;
-            for (int i = threadIdx.x; i < n; i += kThreads8)
+            for (int i = threadIdx.x; i < n; i += kAll)
                 store4(a.out, a.out_dtype, at + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
         }
         return;
     }
     const uint64_t tmo = a.timeout_ns;
-    float2* scale_s = reinterpret_cast<float2*>(smem + LY::kOffScale);
+    float2* scale_s = reinterpret_cast<float2*>(smem + ly.off_scale());
 
-    const int groups = sp.groups, streams = kWarps8 / groups;
-    const int grp = warp & (groups - 1), stream = warp / groups;
-    // this stream's stages
-    const int lg_depth = __ffs(LY::kStages / kWarps8 * groups) - 1, depth = 1 << lg_depth, st0 = stream << lg_depth;
-    const Blocks blocks(a.kv.block_rows);
-    const uint64_t policy = tc::policy_evict_first();               // the cache is read once
-    const int lg_page = __ffs(c8.page_size) - 1;
-    bool ok = true;
+    const int groups = sp.groups, streams = kWarps8 / groups, depth = ly.stages / streams;
 
-    // The stream's first warp fetches for it, a stage as soon as its warps are
-    // done with it: all issue copies, which one alone does at no more than
-    // 5.2 TB/s (over all SMs, 8 KB units).
-    Fetch f{w0, w0.run / sp.passes, 0, stream, 0, 0};
-    int fetched = 0, row_v = 0, head_v = 0;  // units whose K was asked for; the last one's place, for V
-    if (grp == 0) f.find(a, blocks, lens, runs, sp.passes);
-    auto fetch_k = [&]() {
-        const Fetch x = f;
-        f.at += streams;
-        f.find(a, blocks, lens, runs, sp.passes);  // (the next entry is on its way while this one's copies are issued)
-        const int st = st0 + (fetched & (depth - 1));
-        row_v = x.row(a, blocks), head_v = x.h;
-        if (groups > 1)
-            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&empty_k[st], ((fetched >> lg_depth) & 1) ^ 1, tmo));
-        if (!ok) return;
-        ++fetched;
-        if (lane == 0) {
-            tc::mbar_arrive_expect_tx(&full_k[st], LY::kHalf);
-            tc::tma_load_3d(smem + st * LY::kStage, &tmK, &full_k[st], 0, head_v, row_v, policy);
-            if (row_v < a.kv.rows) {
-                const int64_t page = (int64_t)(row_v >> lg_page) * Hkv + head_v;
-                tc::copy4_async(&scale_s[st].x, c8.k_scale + page);
-                tc::copy4_async(&scale_s[st].y, c8.v_scale + page);
-                tc::copies_arrive(&full_k[st]);
-            } else {
-                scale_s[st] = make_float2(0.f, 1.f);
-                tc::mbar_arrive(&full_k[st]);
+    if (warp >= kWarps8) {
+        // ------------------------------------------------------ fetchers --
+        // A lane fetches for one stream whenever a stage of it is free.  Asking for a
+        // unit takes a thread some 290 cycles, so that a unit every 220 takes
+        // several warps (one warp: 33.0 us for 64 K rows; those that attend do it
+        // themselves: 36.4).
+        const uint64_t policy = tc::policy_evict_first();  // the cache is read once
+        const int lg_page = __ffs(c8.page_size) - 1;
+        const Blocks blocks(a.kv.block_rows);
+        const int mine = warp - kWarps8 + lane * kFetchers;  // the stream
+        Fetch f{w0, w0.run / sp.passes, 0, mine, 0, 0};
+        if (mine >= streams) f.w.left = 0;
+        f.find(a, blocks, lens, runs, sp.passes);
+        int st = 0, fetched = 0;
+        uint32_t phase = 1;  // (a stage's first fill waits for nobody)
+        uint64_t since = 0;
+        for (uint32_t idle = 0; __any_sync(0xffffffffu, f.more());) {
+            const int at = mine * depth + st;
+            const bool go = f.more() && tc::mbar_test(&empty[at], phase);
+            if (go) {
+                const int r = f.row(a, blocks), h = f.h;
+                unsigned char* base = smem + at * LY::kStage;
+                tc::mbar_arrive_expect_tx(&full[at], LY::kStage);
+                tc::tma_load_3d(base, &tmK, &full[at], 0, h, r, policy);
+                tc::tma_load_3d(base + LY::kHalf, &tmV, &full[at], 0, h, r, policy);
+                if (r < a.kv.rows) {
+                    const int64_t page = (int64_t)(r >> lg_page) * Hkv + h;
+                    tc::copy4_async(&scale_s[at].x, c8.k_scale + page);
+                    tc::copy4_async(&scale_s[at].y, c8.v_scale + page);
+                    tc::copies_arrive(&full[at]);
+                } else {
+                    scale_s[at] = make_float2(0.f, 1.f);
+                    tc::mbar_arrive(&full[at]);
+                }
+                ++fetched;
+                if (++st == depth) st = 0, phase ^= 1;
+                f.at += streams;
+                f.find(a, blocks, lens, runs, sp.passes);
+            }
+            if (__any_sync(0xffffffffu, go)) {
+                idle = 0;
+            } else if (++idle == 64) {
+                since = tc::globaltimer_ns();
+            } else if ((idle & 63) == 0 && __any_sync(0xffffffffu, tc::globaltimer_ns() - since > tmo)) {
+                if (lane == 0) report_error(a.err, kDevWaitDecode, 0xb1, fetched);
+                break;
             }
         }
-        __syncwarp();
-    };
-    int fetched_v = 0;
-    auto fetch_v = [&]() {  // of the unit whose K was asked for last
-        const int st = st0 + (fetched_v & (depth - 1));
-        if (groups > 1)
-            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&empty_v[st], ((fetched_v >> lg_depth) & 1) ^ 1, tmo));
-        if (!ok) return;
-        ++fetched_v;
-        if (lane == 0) {
-            tc::mbar_arrive_expect_tx(&full_v[st], LY::kHalf);
-            tc::tma_load_3d(smem + st * LY::kStage + LY::kHalf, &tmV, &full_v[st], 0, head_v, row_v, policy);
+        // copies still in flight land before the CTA ends
+        for (int i = 0; i < min(fetched, depth); ++i) {
+            if (--st < 0) st = depth - 1, phase ^= 1;
+            tc::mbar_wait(&full[mine * depth + st], phase ^ 1, tmo);
         }
-        __syncwarp();
-    };
+        return;
+    }
+
+    // ---------------------------------------------------------- consumers --
+    const int grp = warp & (groups - 1), stream = warp / groups, st0 = stream * depth;
+    bool ok = true;
     // The queries of segment n_q, by thread 0, while the segment before is
     // attended (its buffer's readers met at the end of the one before that).
     Walk wq = w0;
@@ -321,7 +339,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
             const int h = wq.run / sp.passes, pass = wq.run % sp.passes, b = n_q & 1;
             const uint32_t bytes = min(sp.pass_heads, G - pass * sp.pass_heads) * D * es;
             tc::mbar_arrive_expect_tx(&q_full[b], bytes);
-            tc::bulk_load(smem + LY::kOffQ + b * LY::kQBytes,
+            tc::bulk_load(smem + ly.off_q() + b * ly.q_bytes,
                           static_cast<const char*>(a.q) +
                               ((int64_t)wq.s * a.n_head + (int64_t)h * G + pass * sp.pass_heads) * D * es,
                           bytes, &q_full[b]);
@@ -330,15 +348,12 @@ __global__ void __launch_bounds__(kThreads8, 1)
         }
     };
     fetch_q();
-    for (int i = 0; i < depth && grp == 0 && f.more(); ++i) {
-        fetch_k();
-        fetch_v();
-    }
-
-    float* om = reinterpret_cast<float*>(smem + LY::kOffO);
-    float* om_w = om + warp * 8 * D;
+    float* om = reinterpret_cast<float*>(smem + ly.off_o());
+    float* om_w = om + warp % ly.slots * 8 * D;
     Walk w = w0;
-    int it = 0, used = 0;  // units of the range before the segment; units that this warp is done with
+    int it = 0;  // units of the range before the segment
+    int st = 0;  // the next stage, and the phase of its barrier
+    uint32_t phase = 0;
     for (int seg = 0; w.left > 0 || (C > 1 && seg == 0); ++seg) {
         const int n_seg = w.segment();
         const int h = w.run / sp.passes, pass = w.run % sp.passes;
@@ -360,7 +375,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
         uint32_t qh[2 * kSteps], ql[LO ? 2 * kSteps : 1];
         float sl[2];  // factor of the scores of heads 2 tq + {0, 1}
         {
-            const unsigned char* qs = smem + LY::kOffQ + (seg & 1) * LY::kQBytes + (grp * 8 + hd) * D * es;
+            const unsigned char* qs = smem + ly.off_q() + (seg & 1) * ly.q_bytes + (grp * 8 + hd) * D * es;
             float4 x[kSteps];
             float top = 0.f;
 #pragma unroll
@@ -390,17 +405,17 @@ __global__ void __launch_bounds__(kThreads8, 1)
         // first unit of the segment that falls to this stream
         int i = (stream - it) & (streams - 1);
         for (; i < n_seg; i += streams) {
-            const int st = st0 + (used & (depth - 1));
-            const uint32_t phase = (used >> lg_depth) & 1;
+            const int at = st0 + st;
             if (ok) {
-                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full_k[st], phase, tmo));
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[at], phase, tmo));
                 if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb2, it + i);
             }
             if (!ok) break;
-            unsigned char* stage = smem + st * LY::kStage;
+            if (++st == depth) st = 0, phase ^= 1;
+            unsigned char* stage = smem + at * LY::kStage;
             const unsigned char* vb = stage + LY::kHalf;
             const int u = w.u + i, lim = min(kUnit, w.n - u * kUnit);
-            const float2 sc = scale_s[st];
+            const float2 sc = scale_s[at];
             // scores of keys 16 b + hd and 16 b + 8 + hd: [b][half * 2 + head]; the sum of even steps and that of
             // odd ones (each one's products wait for one another)
             float s4[2][4], s5[2][4];
@@ -425,9 +440,6 @@ __global__ void __launch_bounds__(kThreads8, 1)
                         if constexpr (LO) mma8(x, a0, a1, a2, a3, ql[2 * j], ql[2 * j + 1]);
                     }
             }
-            __syncwarp();
-            if (groups > 1 && lane == 0) tc::mbar_arrive(&empty_k[st]);
-            if (grp == 0 && f.more()) fetch_k();
             // log2 of the weight times V's scale: that is what O is the sum of
             const float lv = __log2f(sc.y);
             float mx[2] = {-INFINITY, -INFINITY};
@@ -475,12 +487,6 @@ __global__ void __launch_bounds__(kThreads8, 1)
                 }
             const float rv = ex2(-lv);
             l[0] = fmaf(sum0, rv, l[0]), l[1] = fmaf(sum1, rv, l[1]);  // (the weights alone)
-            if (ok) {
-                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full_v[st], phase, tmo));
-                if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb4, it + i);
-            }
-            ++used;
-            if (!ok) break;
             if (!I8 && lim < kUnit) {
                 // V rows past the length may hold NaN codes: their P is 0, and 0 * NaN is not 0
                 for (int j = lane; j < (kUnit - lim) * (D / 16); j += 32)
@@ -505,30 +511,33 @@ __global__ void __launch_bounds__(kThreads8, 1)
                             v[t][e][0] = x.x, v[t][e][1] = x.y;
                         }
                     }
+                // (four tiles of columns at a time: a tile's second product waits for its first)
 #pragma unroll
-                for (int x = 0; x < D / 32; ++x) {
-                    uint32_t a0[4], a1[4];  // [tile * 2 + column]
-                    pairs8<I8>(prmt(v[0][0][x], v[0][1][x], 0x5140), a0[0], a0[1]);
-                    pairs8<I8>(prmt(v[0][0][x], v[0][1][x], 0x7362), a0[2], a0[3]);
-                    pairs8<I8>(prmt(v[1][0][x], v[1][1][x], 0x5140), a1[0], a1[1]);
-                    pairs8<I8>(prmt(v[1][0][x], v[1][1][x], 0x7362), a1[2], a1[3]);
+                for (int x = 0; x < D / 32; x += 2) {
+                    uint32_t a0[8], a1[8];  // [tile * 2 + column]
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int y = 0; y < 2; ++y) {
+                        pairs8<I8>(prmt(v[0][0][x + y], v[0][1][x + y], 0x5140), a0[4 * y], a0[4 * y + 1]);
+                        pairs8<I8>(prmt(v[0][0][x + y], v[0][1][x + y], 0x7362), a0[4 * y + 2], a0[4 * y + 3]);
+                        pairs8<I8>(prmt(v[1][0][x + y], v[1][1][x + y], 0x5140), a1[4 * y], a1[4 * y + 1]);
+                        pairs8<I8>(prmt(v[1][0][x + y], v[1][1][x + y], 0x7362), a1[4 * y + 2], a1[4 * y + 3]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
                         mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], ph[b][0], ph[b][1]);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < 4; ++j)
                         mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], pl[b][0], pl[b][1]);
                 }
             }
             __syncwarp();
-            if (groups > 1 && lane == 0) tc::mbar_arrive(&empty_v[st]);
-            if (grp == 0 && fetched_v < fetched) fetch_v();
+            if (lane == 0) tc::mbar_arrive(&empty[at]);
         }
 
         // ------------------------------------------- merge the warps' states
         // (ml alternates between two buffers: a warp may write the next
         // segment's before another has read this one's sums)
-        float2* ml = reinterpret_cast<float2*>(smem + LY::kOffMl) + (seg & 1) * kWarps8 * 8;
+        float2* ml = reinterpret_cast<float2*>(smem + ly.off_ml()) + (seg & 1) * kWarps8 * 8;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -552,11 +561,27 @@ __global__ void __launch_bounds__(kThreads8, 1)
         auto place = [&](int e, int j) {
             return reinterpret_cast<float4*>(om_w + (2 * tq + e) * D + kCols * hd + 2 * j);
         };
+        // the upper half of the warps hands its sums to the lower half, whose warps have the same heads (not where all
+        // share a unit: there each has its own)
+        const bool hand = groups < kWarps8 && warp >= kWarps8 / 2, take = groups < kWarps8 && warp < kWarps8 / 2;
+        if (hand) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int j = 0; j < D / 16; j += 2)
-                *place(e, j) = make_float4(o[j][e], o[j][2 + e], o[j + 1][e], o[j + 1][2 + e]);
+                for (int j = 0; j < D / 16; j += 2)
+                    *place(e, j) = make_float4(o[j][e], o[j][2 + e], o[j + 1][e], o[j + 1][2 + e]);
+        }
+        tc::named_bar_sync(1, kThreads8);
+        if (!hand) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < D / 16; j += 2) {
+                    float4 x = take ? *place(e, j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x.x += o[j][e], x.y += o[j][2 + e], x.z += o[j + 1][e], x.w += o[j + 1][2 + e];
+                    *place(e, j) = x;
+                }
+        }
         tc::named_bar_sync(1, kThreads8);
         const bool whole = w.u == 0 && n_seg == w.units;
         const int n_heads = min(min(groups * 8, sp.pass_heads), G - pass * sp.pass_heads);
@@ -577,8 +602,8 @@ __global__ void __launch_bounds__(kThreads8, 1)
                     lt += v.y * ex2(v.x - ms);
                 }
 #pragma unroll
-            for (int r = 0; r < kWarps8; ++r)
-                if (r < streams) {
+            for (int r = 0; r < kWarps8 / 2; ++r)
+                if (r * groups < ly.slots) {
                     const float4 t = *reinterpret_cast<const float4*>(om + ((r * groups + gw) * 8 + gh) * D + c * 4);
                     ot.x += t.x, ot.y += t.y, ot.z += t.z, ot.w += t.w;
                 }
@@ -613,15 +638,9 @@ __global__ void __launch_bounds__(kThreads8, 1)
         it += n_seg;
         w.advance(a, lens, runs, n_seg);
     }
-    if (!ok) {
-        // copies still in flight land before the CTA ends
-        if (lane == 0) report_error(a.err, kDevWaitDecode, 0xb1, used);
-        for (int j = max(0, fetched - depth); j < fetched; ++j) {
-            tc::mbar_wait(&full_k[st0 + (j & (depth - 1))], (j >> lg_depth) & 1, tmo);
-            if (j < fetched_v) tc::mbar_wait(&full_v[st0 + (j & (depth - 1))], (j >> lg_depth) & 1, tmo);
-        }
+    // (after a wait that ran out, queries asked for may still be on their way)
+    if (!ok && threadIdx.x == 0)
         for (int j = max(0, n_q - 2); j < n_q; ++j) tc::mbar_wait(&q_full[j & 1], (j >> 1) & 1, tmo);
-    }
 }
 
 // ---------------------------------------------------------------- host side --
@@ -688,7 +707,8 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
     CUtensorMap mk, mv;
     if (!cache8_map(&mk, c.k, D, a.n_head_kv, a.kv.rows) || !cache8_map(&mv, c.v, D, a.n_head_kv, a.kv.rows))
         return cudaErrorInvalidValue;
-    const int smem = Layout8<D>::kBytes + 1024;
+    const Layout8<D> ly = Layout8<D>::make(sp.pass_heads, a.dtype == 0 ? 4 : 2, sp.groups);
+    const int smem = 232448;  // all there is: the stages take what is left
     int dev = 0;
     cudaGetDevice(&dev);
     // one bit per device ordinal < 32 whose attribute is set
@@ -719,10 +739,10 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
         a.kv.lens = sp.lens;
     }
     cfg.gridDim = dim3(sp.ctas);
-    cfg.blockDim = dim3(kThreads8);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(kThreads8 + 32 * kFetchers);
+    cfg.dynamicSmemBytes = ly.bytes() + 1024;
     cfg.numAttrs = sp.cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k10_decode8<D, I8, LO, JOIN>, mk, mv, a, c, sp);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k10_decode8<D, I8, LO, JOIN>, mk, mv, a, c, sp, ly);
     if (e != cudaSuccess || sp.direct) return e;
     const int heads = std::min(a.n_head / a.n_head_kv, sp.pass_heads);
     const int64_t grid = (int64_t)sp.joins * heads;
