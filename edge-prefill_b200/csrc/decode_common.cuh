@@ -21,8 +21,12 @@ constexpr int kUnit = 32;      // cache rows per unit
 constexpr int kCtas = 148;     // one per SM
 constexpr int kMinUnits = 4;  // fewest units dealt to a CTA
 // What a run costs a CTA besides its units (the merge of the warps' states),
-// in units: the ranges are equal in this measure.
-constexpr int kRunCost = 6;
+// in units: the ranges are equal in this measure.  (EPSP_RUN_COST: the file that
+// includes this one has another.)
+#ifndef EPSP_RUN_COST
+#define EPSP_RUN_COST 6
+#endif
+constexpr int kRunCost = EPSP_RUN_COST;
 constexpr int kLensOnChip = 1024;  // lengths a CTA keeps in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 // Calls that skip the split and the join: one CTA per run of at most

@@ -35,7 +35,10 @@
 #include <atomic>
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
+// (in units of 32 rows of 8 bits; 64 sequences of up to 4096 rows: 6 72 us, 10 64.2, 14 63.7, 20 64.5)
+#define EPSP_RUN_COST 14
 #include "decode_common.cuh"
 #include "epsp_kernels.h"
 #include "tc100.cuh"
@@ -56,26 +59,21 @@ struct Layout8 {
     static constexpr int kHalf = kUnit * D;      // K (or V) of a unit
     static constexpr int kStage = 2 * kHalf;
     static constexpr int kMost = 196608 / kStage;  // stages, at most
-    static constexpr int kMl = 2 * kWarps8 * 8 * 8;
-    int32_t stages;   // a multiple of the streams
+    int32_t stages;   // dealt to the streams as evenly as they go
     int32_t q_bytes;  // of a segment's queries: two buffers
-    int32_t slots;    // of the merge buffer, [slots][8][D]
     __host__ __device__ int off_q() const { return stages * kStage; }
-    __host__ __device__ int off_o() const { return off_q() + 2 * q_bytes; }
-    __host__ __device__ int off_ml() const { return off_o() + slots * 8 * D * 4; }
-    __host__ __device__ int off_scale() const { return off_ml() + kMl; }  // [stages] (ks, vs)
+    __host__ __device__ int off_o() const { return off_q() + 2 * q_bytes; }        // [kWarps8][8][D] the warps' sums
+    __host__ __device__ int off_ml() const { return off_o() + kWarps8 * 8 * D * 4; }  // [kWarps8][8] (maximum, sum)
+    __host__ __device__ int off_scale() const { return off_ml() + kWarps8 * 8 * 8; }  // [stages] (ks, vs)
     __host__ __device__ int off_bar() const { return off_scale() + kMost * 8; }
-    __host__ __device__ int off_lens() const { return off_bar() + (2 * kMost + 2) * 8; }
+    __host__ __device__ int off_lens() const { return off_bar() + (2 * kMost + 6) * 8; }
     __host__ __device__ int bytes() const { return off_lens() + kLensOnChip * 4; }
-    // For `pass` query heads of `es` bytes and units shared by `groups` warps:
-    // as many stages as 227 KB hold.
-    static Layout8 make(int pass, int es, int groups) {
+    // For `pass` query heads of `es` bytes: as many stages as 227 KB hold.
+    static Layout8 make(int pass, int es) {
         Layout8 l;
         l.stages = 0;
         l.q_bytes = pass * D * es;
-        l.slots = groups == kWarps8 ? kWarps8 : kWarps8 / 2;
-        const int streams = kWarps8 / groups;
-        l.stages = std::min(kMost, (232448 - 1024 - l.bytes()) / kStage) / streams * streams;
+        l.stages = std::min(kMost, (232448 - 1024 - l.bytes()) / kStage);
         return l;
     }
 };
@@ -128,19 +126,6 @@ __device__ __forceinline__ void mma8_first(float (&c)[4], uint32_t a0, uint32_t 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// Four neighbouring query elements.
-__device__ __forceinline__ float4 q_of(const unsigned char* q, int32_t dtype, int i) {
-    if (dtype == 0) return *reinterpret_cast<const float4*>(q + i * 4);
-    const uint2 w = *reinterpret_cast<const uint2*>(q + i * 2);
-    if (dtype == 1) {
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-        return make_float4(a.x, a.y, b.x, b.y);
-    }
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                       __uint_as_float(w.y & 0xffff0000u));
-}
-
 // Units of a block, and the place of a unit: dividing by a number that is known
 // at run time only costs forty instructions, by its reciprocal five.
 struct Blocks {
@@ -175,7 +160,7 @@ struct Fetch {
         while (w.left > 0 && at - before >= w.segment()) {
             before += w.segment();
             w.advance(a, lens, runs, w.segment());
-            h = w.run / passes;
+            h = passes == 1 ? w.run : w.run / passes;
         }
         if (w.left <= 0 || bl.units == 0) return;
         const int2 b = bl.of(w.u + at - before);
@@ -193,6 +178,16 @@ struct Fetch {
     }
 };
 
+__device__ __forceinline__ void store2(void* out, int32_t dtype, int64_t i, float x, float y) {
+    if (dtype == 0) {
+        *reinterpret_cast<float2*>(static_cast<float*>(out) + i) = make_float2(x, y);
+    } else if (dtype == 1) {
+        *reinterpret_cast<__half2*>(static_cast<__half*>(out) + i) = __floats2half2_rn(x, y);
+    } else {
+        *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(out) + i) = __floats2bfloat162_rn(x, y);
+    }
+}
+
 // LO: q has remainders (f32).  JOIN: the calls that join_cluster finishes.
 template <int D, bool I8, bool LO, bool JOIN>
 __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
@@ -205,18 +200,27 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + ly.off_bar());
     uint64_t* empty = full + LY::kMost;
-    uint64_t* q_full = empty + LY::kMost;
+    uint64_t* q_full = empty + LY::kMost;  // [2] queries are there, and every warp has read them
+    uint64_t* q_empty = q_full + 2;
+    uint64_t* written = q_empty + 2;       // the warps' sums of a segment are in shared memory,
+    uint64_t* merged = written + 1;        // and out of it
     int32_t* lens_s = reinterpret_cast<int32_t*>(smem + ly.off_lens());
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int Hkv = a.n_head_kv, G = a.n_head / Hkv, es = a.dtype == 0 ? 4 : 2;
     const int runs = Hkv * sp.passes;
 
+    if (threadIdx.x < ly.stages) {
+        tc::mbar_init(&full[threadIdx.x], 2);  // the bytes' announcement, and the scales
+        tc::mbar_init(&empty[threadIdx.x], sp.groups);
+        tc::fence_mbar_init();
+    }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < ly.stages; ++i) {
-            tc::mbar_init(&full[i], 2);  // the bytes' announcement, and the scales
-            tc::mbar_init(&empty[i], sp.groups);
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&q_full[i], 1);
+            tc::mbar_init(&q_empty[i], kWarps8);
         }
-        for (int i = 0; i < 2; ++i) tc::mbar_init(&q_full[i], 1);
+        tc::mbar_init(written, kWarps8);
+        tc::mbar_init(merged, kWarps8);
         tc::fence_mbar_init();
         tc::tma_prefetch_desc(&tmK);
         tc::tma_prefetch_desc(&tmV);
@@ -269,7 +273,10 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     const uint64_t tmo = a.timeout_ns;
     float2* scale_s = reinterpret_cast<float2*>(smem + ly.off_scale());
 
-    const int groups = sp.groups, streams = kWarps8 / groups, depth = ly.stages / streams;
+    const int groups = sp.groups, streams = kWarps8 / groups;
+    // stages of stream i: the first few have one more
+    const int base = ly.stages / streams, more = ly.stages % streams;
+    auto first_of = [&](int i) { return i * base + min(i, more); };
 
     if (warp >= kWarps8) {
         // ------------------------------------------------------ fetchers --
@@ -281,21 +288,38 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         const int lg_page = __ffs(c8.page_size) - 1;
         const Blocks blocks(a.kv.block_rows);
         const int mine = warp - kWarps8 + lane * kFetchers;  // the stream
+        const int st0 = first_of(mine), depth = base + (mine < more ? 1 : 0);
+        // (the last lane of all: the queries, a segment ahead)
+        const bool asks = warp == kWarps8 + kFetchers - 1 && lane == 31;
         Fetch f{w0, w0.run / sp.passes, 0, mine, 0, 0};
-        if (mine >= streams) f.w.left = 0;
-        f.find(a, blocks, lens, runs, sp.passes);
+        if (mine >= streams && !asks) f.w.left = 0;
+        if (!asks) f.find(a, blocks, lens, runs, sp.passes);
         int st = 0, fetched = 0;
         uint32_t phase = 1;  // (a stage's first fill waits for nobody)
         uint64_t since = 0;
-        for (uint32_t idle = 0; __any_sync(0xffffffffu, f.more());) {
-            const int at = mine * depth + st;
-            const bool go = f.more() && tc::mbar_test(&empty[at], phase);
-            if (go) {
+        bool more_q = asks && (w0.left > 0 || C > 1);
+        auto left = [&]() { return asks ? more_q : f.more(); };
+        for (uint32_t idle = 0; __any_sync(0xffffffffu, left());) {
+            const int at = st0 + st;
+            const bool go = left() && tc::mbar_test(asks ? &q_empty[st] : &empty[at], phase);
+            if (go && asks) {
+                const int pass = f.w.run % sp.passes;
+                const uint32_t bytes = min(sp.pass_heads, G - pass * sp.pass_heads) * D * es;
+                tc::mbar_arrive_expect_tx(&q_full[st], bytes);
+                tc::bulk_load(smem + ly.off_q() + st * ly.q_bytes,
+                              static_cast<const char*>(a.q) +
+                                  ((int64_t)f.w.s * a.n_head + (int64_t)(f.w.run / sp.passes) * G + pass * sp.pass_heads) * D * es,
+                              bytes, &q_full[st]);
+                ++fetched;
+                if (++st == 2) st = 0, phase ^= 1;
+                if (f.w.left > 0) f.w.advance(a, lens, runs, f.w.segment());
+                more_q = f.w.left > 0;
+            } else if (go) {
                 const int r = f.row(a, blocks), h = f.h;
-                unsigned char* base = smem + at * LY::kStage;
+                unsigned char* to = smem + at * LY::kStage;
                 tc::mbar_arrive_expect_tx(&full[at], LY::kStage);
-                tc::tma_load_3d(base, &tmK, &full[at], 0, h, r, policy);
-                tc::tma_load_3d(base + LY::kHalf, &tmV, &full[at], 0, h, r, policy);
+                tc::tma_load_3d(to, &tmK, &full[at], 0, h, r, policy);
+                tc::tma_load_3d(to + LY::kHalf, &tmV, &full[at], 0, h, r, policy);
                 if (r < a.kv.rows) {
                     const int64_t page = (int64_t)(r >> lg_page) * Hkv + h;
                     tc::copy4_async(&scale_s[at].x, c8.k_scale + page);
@@ -320,46 +344,108 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
             }
         }
         // copies still in flight land before the CTA ends
-        for (int i = 0; i < min(fetched, depth); ++i) {
-            if (--st < 0) st = depth - 1, phase ^= 1;
-            tc::mbar_wait(&full[mine * depth + st], phase ^ 1, tmo);
+        const int turn = asks ? 2 : depth;
+        for (int i = 0; i < min(fetched, turn); ++i) {
+            if (--st < 0) st = turn - 1, phase ^= 1;
+            tc::mbar_wait(asks ? &q_full[st] : &full[st0 + st], phase ^ 1, tmo);
         }
         return;
     }
 
     // ---------------------------------------------------------- consumers --
-    const int grp = warp & (groups - 1), stream = warp / groups, st0 = stream * depth;
+    const int grp = warp & (groups - 1), stream = warp / groups;
+    const int st0 = first_of(stream), depth = base + (stream < more ? 1 : 0);
     bool ok = true;
-    // The queries of segment n_q, by thread 0, while the segment before is
-    // attended (its buffer's readers met at the end of the one before that).
-    Walk wq = w0;
-    int n_q = 0;
-    auto fetch_q = [&]() {
-        if (threadIdx.x == 0 && (wq.left > 0 || (C > 1 && n_q == 0))) {
-            const int h = wq.run / sp.passes, pass = wq.run % sp.passes, b = n_q & 1;
-            const uint32_t bytes = min(sp.pass_heads, G - pass * sp.pass_heads) * D * es;
-            tc::mbar_arrive_expect_tx(&q_full[b], bytes);
-            tc::bulk_load(smem + ly.off_q() + b * ly.q_bytes,
-                          static_cast<const char*>(a.q) +
-                              ((int64_t)wq.s * a.n_head + (int64_t)h * G + pass * sp.pass_heads) * D * es,
-                          bytes, &q_full[b]);
-            ++n_q;
-            if (wq.left > 0) wq.advance(a, lens, runs, wq.segment());
-        }
-    };
-    fetch_q();
+
     float* om = reinterpret_cast<float*>(smem + ly.off_o());
-    float* om_w = om + warp % ly.slots * 8 * D;
+    float* om_w = om + warp * 8 * D;
+    float2* ml = reinterpret_cast<float2*>(smem + ly.off_ml());
+    // Place of 16 bytes in a warp's sums of one head: turned by the head, so that
+    // lanes of one column block and four heads meet different banks.
+    auto chunk = [&](int g, int c) { return c ^ (D == 128 ? g >> 1 & 3 : (g >> 2 & 1) << 2 | (g >> 1 & 1)); };
+    // What is left to do of the segment before: its sums are put together once all
+    // warps have left theirs, each warp a head (or as many as there are groups),
+    // between two units of the next.
+    bool pending = false, whole = false;
+    int64_t head_row = 0;  // row of the pass's first query head
+    int pass_n = 0, part = 0;  // its heads; the segment's slot in the workspace
+    int segs = 0;          // segments whose sums this warp has left
+    auto merge = [&]() {
+        constexpr int kC = D / 32;  // columns of a lane
+        for (int g = warp; g < pass_n; g += kWarps8) {
+            const int gw = g >> 3, gh = g & 7;
+            // lane r: stream r
+            const float2 v = lane < streams ? ml[(lane * groups + gw) * 8 + gh] : make_float2(-INFINITY, 0.f);
+            const float* from = om + gw * 8 * D + gh * D + chunk(gh, lane * kC / 4) * 4 + lane * kC % 4;
+            float t[kWarps8][kC];
+#pragma unroll
+            for (int r = 0; r < kWarps8; ++r) {
+                const float* x = from + (r < streams ? r * groups * 8 * D : 0);
+                if constexpr (kC == 4) *reinterpret_cast<float4*>(t[r]) = *reinterpret_cast<const float4*>(x);
+                else *reinterpret_cast<float2*>(t[r]) = *reinterpret_cast<const float2*>(x);
+            }
+            float mt = v.x;
+#pragma unroll
+            for (int x = 1; x < 8; x <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+            mt = __shfl_sync(0xffffffffu, mt, 0);
+            const float ms = mt == -INFINITY ? 0.f : mt, f = ex2(v.x - ms);
+            float lt = v.y * f;
+#pragma unroll
+            for (int x = 1; x < 8; x <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, x);
+            lt = __shfl_sync(0xffffffffu, lt, 0);
+            float acc[kC];
+#pragma unroll
+            for (int c = 0; c < kC; ++c) acc[c] = 0.f;
+#pragma unroll
+            for (int r = 0; r < kWarps8; ++r) {
+                const float fr = __shfl_sync(0xffffffffu, f, r);
+#pragma unroll
+                for (int c = 0; c < kC; ++c) acc[c] = r < streams ? fmaf(fr, t[r][c], acc[c]) : acc[c];
+            }
+            if constexpr (JOIN) {
+                // (the ring: this CTA's last copy has landed)
+                float* to = reinterpret_cast<float*>(smem) + g * D + lane * kC;
+#pragma unroll
+                for (int c = 0; c < kC; ++c) to[c] = acc[c];
+                if (lane == 0) *reinterpret_cast<float2*>(smem + kPass8 * D * 4 + g * 8) = make_float2(ms, lt);
+            } else if (whole) {
+                const float inv = 1.f / lt;
+                const int64_t to = (head_row + g) * D + lane * kC;
+                if constexpr (kC == 4)
+                    store4(a.out, a.out_dtype, to, make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv));
+                else
+                    store2(a.out, a.out_dtype, to, acc[0] * inv, acc[1] * inv);
+            } else {
+                const int64_t to = (int64_t)part * groups * 8 + g;
+                if constexpr (kC == 4)
+                    *reinterpret_cast<float4*>(sp.part_o + to * D + lane * kC) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                else
+                    *reinterpret_cast<float2*>(sp.part_o + to * D + lane * kC) = make_float2(acc[0], acc[1]);
+                if (lane == 0) sp.part_ml[to] = make_float2(ms, lt);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(merged);
+        pending = false;
+    };
+    // Waits for all warps' sums, then does this one's share.
+    auto finish = [&]() {
+        if (!pending) return;
+        if (ok) {
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(written, (segs - 1) & 1, tmo));
+            if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb4, segs);
+        }
+        merge();
+    };
     Walk w = w0;
     int it = 0;  // units of the range before the segment
     int st = 0;  // the next stage, and the phase of its barrier
     uint32_t phase = 0;
     for (int seg = 0; w.left > 0 || (C > 1 && seg == 0); ++seg) {
         const int n_seg = w.segment();
-        const int h = w.run / sp.passes, pass = w.run % sp.passes;
+        const int h = sp.passes == 1 ? w.run : w.run / sp.passes, pass = w.run - h * sp.passes;
         const int g0 = pass * sp.pass_heads + grp * 8;  // this warp's first query head of the group
         const int64_t q_row = (int64_t)w.s * a.n_head + (int64_t)h * G;
-        fetch_q();
         // lane: row hd of a 16-row tile and of its second half; columns 2 tq + {0, 1}
         const int hd = lane >> 2, tq = lane & 3;
         // columns D / 8 hd + 2 i + {0, 1} of heads 2 tq + {0, 1}: [i][column * 2 + head]
@@ -375,33 +461,63 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         uint32_t qh[2 * kSteps], ql[LO ? 2 * kSteps : 1];
         float sl[2];  // factor of the scores of heads 2 tq + {0, 1}
         {
-            const unsigned char* qs = smem + ly.off_q() + (seg & 1) * ly.q_bytes + (grp * 8 + hd) * D * es;
-            float4 x[kSteps];
-            float top = 0.f;
+            const unsigned char* qs = smem + ly.off_q() + (seg & 1) * ly.q_bytes + ((grp * 8 + hd) * D + D / 4 * tq) * es;
+            const bool in = g0 + hd < G;
+            float back = a.kq_scale * kLog2e;
+            // factor that takes elements of a head whose largest is `top` to 2^14 .. 2^15; `back` takes it back
+            auto scaled = [&](float top) {
+                const int e = (int)(__float_as_uint(top) >> 23) - 127;
+                const int up = e < 128 ? min(14 - e, 126) : 0;  // (at least -113)
+                back *= __uint_as_float((uint32_t)(127 - up) << 23);
+                return __uint_as_float((uint32_t)(up + 127) << 23);
+            };
+            if constexpr (LO) {
+                float4 x[kSteps];
+                float top = 0.f;
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-                x[j] = g0 + hd < G ? q_of(qs, a.dtype, D / 4 * tq + 4 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                top = fmaxf(fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))), top);
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = (int)(__float_as_uint(top) >> 23) - 127;
-            const int up = e < 128 ? min(14 - e, 126) : 0;  // (at least -113)
-            const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-            const float back = a.kq_scale * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23);
-            sl[0] = __shfl_sync(0xffffffffu, back, 8 * tq);
-            sl[1] = __shfl_sync(0xffffffffu, back, 8 * tq + 4);
+                for (int j = 0; j < kSteps; ++j) {
+                    x[j] = in ? *reinterpret_cast<const float4*>(qs + 16 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    top = fmaxf(fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))), top);
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float f = scaled(top);
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-                x[j].x *= f, x[j].y *= f, x[j].z *= f, x[j].w *= f;
-                qh[2 * j] = split2<false>(x[j].x, x[j].y);
-                qh[2 * j + 1] = split2<false>(x[j].z, x[j].w);
-                if constexpr (LO) {
+                for (int j = 0; j < kSteps; ++j) {
+                    x[j].x *= f, x[j].y *= f, x[j].z *= f, x[j].w *= f;
+                    qh[2 * j] = split2<false>(x[j].x, x[j].y);
+                    qh[2 * j + 1] = split2<false>(x[j].z, x[j].w);
                     ql[2 * j] = split2<false>(x[j].x, x[j].y);
                     ql[2 * j + 1] = split2<false>(x[j].z, x[j].w);
                 }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kSteps / 2; ++j) {
+                    const uint4 x = in ? *reinterpret_cast<const uint4*>(qs + 16 * j) : make_uint4(0, 0, 0, 0);
+                    qh[4 * j] = x.x, qh[4 * j + 1] = x.y, qh[4 * j + 2] = x.z, qh[4 * j + 3] = x.w;
+                }
+                if (a.dtype == 2) {
+                    // (a pattern without its sign is in the order of the magnitudes)
+                    uint32_t t = 0;
+#pragma unroll
+                    for (int j = 0; j < 2 * kSteps; ++j) t = __vmaxu2(t, qh[j] & 0x7fff7fffu);
+                    t = max(t & 0xffffu, t >> 16);
+                    t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
+                    t = max(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                    const float f = scaled(__uint_as_float(t << 16));
+#pragma unroll
+                    for (int j = 0; j < 2 * kSteps; ++j) {
+                        const __half2 x = __floats2half2_rn(__uint_as_float(qh[j] << 16) * f,
+                                                            __uint_as_float(qh[j] & 0xffff0000u) * f);
+                        qh[j] = *reinterpret_cast<const uint32_t*>(&x);
+                    }
+                }
             }
+            sl[0] = __shfl_sync(0xffffffffu, back, 8 * tq);
+            sl[1] = __shfl_sync(0xffffffffu, back, 8 * tq + 4);
         }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&q_empty[seg & 1]);
         // first unit of the segment that falls to this stream
         int i = (stream - it) & (streams - 1);
         for (; i < n_seg; i += streams) {
@@ -532,98 +648,37 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
             }
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&empty[at]);
+            if (pending && __all_sync(0xffffffffu, tc::mbar_test(written, (segs - 1) & 1))) merge();
         }
 
-        // ------------------------------------------- merge the warps' states
-        // (ml alternates between two buffers: a warp may write the next
-        // segment's before another has read this one's sums)
-        float2* ml = reinterpret_cast<float2*>(smem + ly.off_ml()) + (seg & 1) * kWarps8 * 8;
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
-        if (hd == 0) {
-            ml[warp * 8 + 2 * tq] = make_float2(m[0], l[0]);
-            ml[warp * 8 + 2 * tq + 1] = make_float2(m[1], l[1]);
+        // Each warp leaves its sums in shared memory and goes on.
+        finish();
+        if (segs > 0 && ok) {
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(merged, (segs - 1) & 1, tmo));
+            if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb5, segs);
         }
-        tc::named_bar_sync(1, kThreads8);
-        // against the streams' common maximum
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float mt = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < kWarps8; ++r)
-                if (r < streams) mt = fmaxf(mt, ml[(r * groups + grp) * 8 + 2 * tq + e].x);
-            const float f = ex2(m[e] - (mt == -INFINITY ? 0.f : mt));
+            for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+            const int g = 2 * tq + e;
+            if (hd == 0) ml[warp * 8 + g] = make_float2(m[e], l[e]);
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) o[j][e] *= f, o[j][2 + e] *= f;
+            for (int j = 0; j < D / 16; j += 2)
+                *reinterpret_cast<float4*>(om_w + g * D + chunk(g, kCols / 4 * hd + j / 2) * 4) =
+                    make_float4(o[j][e], o[j][2 + e], o[j + 1][e], o[j + 1][2 + e]);
         }
-        auto place = [&](int e, int j) {
-            return reinterpret_cast<float4*>(om_w + (2 * tq + e) * D + kCols * hd + 2 * j);
-        };
-        // the upper half of the warps hands its sums to the lower half, whose warps have the same heads (not where all
-        // share a unit: there each has its own)
-        const bool hand = groups < kWarps8 && warp >= kWarps8 / 2, take = groups < kWarps8 && warp < kWarps8 / 2;
-        if (hand) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int j = 0; j < D / 16; j += 2)
-                    *place(e, j) = make_float4(o[j][e], o[j][2 + e], o[j + 1][e], o[j + 1][2 + e]);
-        }
-        tc::named_bar_sync(1, kThreads8);
-        if (!hand) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int j = 0; j < D / 16; j += 2) {
-                    float4 x = take ? *place(e, j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    x.x += o[j][e], x.y += o[j][2 + e], x.z += o[j + 1][e], x.w += o[j + 1][2 + e];
-                    *place(e, j) = x;
-                }
-        }
-        tc::named_bar_sync(1, kThreads8);
-        const bool whole = w.u == 0 && n_seg == w.units;
-        const int n_heads = min(min(groups * 8, sp.pass_heads), G - pass * sp.pass_heads);
-        const int slot = blockIdx.x * 2 + (seg == 0 ? 0 : 1);
-        for (int j = threadIdx.x; j < n_heads * (D / 4); j += kThreads8) {
-            const int g = j / (D / 4), c = j % (D / 4), gw = g >> 3, gh = g & 7;
-            float mt = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < kWarps8; ++r)
-                if (r < streams) mt = fmaxf(mt, ml[(r * groups + gw) * 8 + gh].x);
-            const float ms = mt == -INFINITY ? 0.f : mt;
-            float lt = 0.f;
-            float4 ot = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int r = 0; r < kWarps8; ++r)
-                if (r < streams) {
-                    const float2 v = ml[(r * groups + gw) * 8 + gh];
-                    lt += v.y * ex2(v.x - ms);
-                }
-#pragma unroll
-            for (int r = 0; r < kWarps8 / 2; ++r)
-                if (r * groups < ly.slots) {
-                    const float4 t = *reinterpret_cast<const float4*>(om + ((r * groups + gw) * 8 + gh) * D + c * 4);
-                    ot.x += t.x, ot.y += t.y, ot.z += t.z, ot.w += t.w;
-                }
-            if constexpr (JOIN) {
-                // (the ring: this CTA's last copy has landed)
-                *reinterpret_cast<float4*>(smem + (g * D + c * 4) * 4) = ot;
-                if (c == 0) *reinterpret_cast<float2*>(smem + kPass8 * D * 4 + g * 8) = make_float2(ms, lt);
-            } else if (whole) {
-                const float inv = 1.f / lt;
-                store4(a.out, a.out_dtype, (q_row + pass * sp.pass_heads + g) * D + c * 4,
-                       make_float4(ot.x * inv, ot.y * inv, ot.z * inv, ot.w * inv));
-            } else {
-                const int64_t p = (int64_t)slot * groups * 8 + g;
-                *reinterpret_cast<float4*>(sp.part_o + p * D + c * 4) = ot;
-                if (c == 0) sp.part_ml[p] = make_float2(ms, lt);
-            }
-        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(written);
+        pending = true;
+        ++segs;
+        whole = w.u == 0 && n_seg == w.units;
+        head_row = q_row + pass * sp.pass_heads;
+        pass_n = min(min(groups * 8, sp.pass_heads), G - pass * sp.pass_heads);
+        part = blockIdx.x * 2 + (seg == 0 ? 0 : 1);
         if constexpr (JOIN) {
-            join_cluster<D, kThreads8, kPass8>(a, sp, smem, om, w, n_seg, q_row + pass * sp.pass_heads, n_heads, h,
-                                                  rank);
+            finish();
+            join_cluster<D, kThreads8, kPass8>(a, sp, smem, om, w, n_seg, head_row, pass_n, h, rank);
             if (C > 1) tc::cluster_sync();  // nobody reads this CTA's part any more
         }
         if (!sp.direct && threadIdx.x == 0) {
@@ -638,9 +693,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         it += n_seg;
         w.advance(a, lens, runs, n_seg);
     }
-    // (after a wait that ran out, queries asked for may still be on their way)
-    if (!ok && threadIdx.x == 0)
-        for (int j = max(0, n_q - 2); j < n_q; ++j) tc::mbar_wait(&q_full[j & 1], (j >> 1) & 1, tmo);
+    finish();
 }
 
 // ---------------------------------------------------------------- host side --
@@ -707,7 +760,7 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
     CUtensorMap mk, mv;
     if (!cache8_map(&mk, c.k, D, a.n_head_kv, a.kv.rows) || !cache8_map(&mv, c.v, D, a.n_head_kv, a.kv.rows))
         return cudaErrorInvalidValue;
-    const Layout8<D> ly = Layout8<D>::make(sp.pass_heads, a.dtype == 0 ? 4 : 2, sp.groups);
+    const Layout8<D> ly = Layout8<D>::make(sp.pass_heads, a.dtype == 0 ? 4 : 2);
     const int smem = 232448;  // all there is: the stages take what is left
     int dev = 0;
     cudaGetDevice(&dev);
