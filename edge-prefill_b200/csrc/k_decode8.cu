@@ -431,10 +431,11 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     // Waits for all warps' sums, then does this one's share.
     auto finish = [&]() {
         if (!pending) return;
-        if (ok) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(written, (segs - 1) & 1, tmo));
-            if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb4, segs);
+        if (ok && !tc::mbar_wait(written, (segs - 1) & 1, tmo)) {
+            ok = false;
+            report_error(a.err, kDevWaitDecode, 0xb4, segs);
         }
+        __syncwarp();
         merge();
     };
     Walk w = w0;
@@ -453,10 +454,11 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of heads 2 tq + {0, 1}
-        if (ok) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(&q_full[seg & 1], (seg >> 1) & 1, tmo));
-            if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb3, seg);
+        if (ok && !tc::mbar_wait(&q_full[seg & 1], (seg >> 1) & 1, tmo)) {
+            ok = false;
+            report_error(a.err, kDevWaitDecode, 0xb3, seg);
         }
+        __syncwarp();
         // q in f16, dims D / 4 tq + 4 j + {0, 1, 2, 3} for step j
         uint32_t qh[2 * kSteps], ql[LO ? 2 * kSteps : 1];
         float sl[2];  // factor of the scores of heads 2 tq + {0, 1}
@@ -522,16 +524,24 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         int i = (stream - it) & (streams - 1);
         for (; i < n_seg; i += streams) {
             const int at = st0 + st;
-            if (ok) {
-                ok = __all_sync(0xffffffffu, tc::mbar_wait(&full[at], phase, tmo));
-                if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb2, it + i);
+            // (a lane whose wait runs out waits no more; nothing is skipped, so that the lanes stay together)
+            if (ok && !tc::mbar_wait(&full[at], phase, tmo)) {
+                ok = false;
+                report_error(a.err, kDevWaitDecode, 0xb2, it + i);
             }
-            if (!ok) break;
+            __syncwarp();
             if (++st == depth) st = 0, phase ^= 1;
             unsigned char* stage = smem + at * LY::kStage;
             const unsigned char* vb = stage + LY::kHalf;
             const int u = w.u + i, lim = min(kUnit, w.n - u * kUnit);
             const float2 sc = scale_s[at];
+            if (!I8 && lim < kUnit) {
+                // V rows past the length may hold NaN codes: their P is 0, and 0 * NaN is not 0
+                for (int j = lane; j < (kUnit - lim) * (D / 16); j += 32)
+                    *reinterpret_cast<uint4*>(stage + LY::kHalf + lim * D + j * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes the stage next
+                __syncwarp();
+            }
             // scores of keys 16 b + hd and 16 b + 8 + hd: [b][half * 2 + head]; the sum of even steps and that of
             // odd ones (each one's products wait for one another)
             float s4[2][4], s5[2][4];
@@ -556,6 +566,23 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                         if constexpr (LO) mma8(x, a0, a1, a2, a3, ql[2 * j], ql[2 * j + 1]);
                     }
             }
+            // rows 16 b + 8 t + 2 tq + {0, 1} of V, D / 8 columns from D / 8 hd (asked for before they are wanted)
+            uint32_t v[2][2][2][D / 32];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = 16 * b + 8 * t + 2 * tq + e;
+                        if constexpr (D == 128) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(vb + tile_at<D>(r, hd));
+                            v[b][t][e][0] = x.x, v[b][t][e][1] = x.y, v[b][t][e][2] = x.z, v[b][t][e][3] = x.w;
+                        } else {
+                            const uint2 x = *reinterpret_cast<const uint2*>(vb + tile_at<D>(r, hd >> 1) + (hd & 1) * 8);
+                            v[b][t][e][0] = x.x, v[b][t][e][1] = x.y;
+                        }
+                    }
             // log2 of the weight times V's scale: that is what O is the sum of
             const float lv = __log2f(sc.y);
             float mx[2] = {-INFINITY, -INFINITY};
@@ -603,40 +630,18 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                 }
             const float rv = ex2(-lv);
             l[0] = fmaf(sum0, rv, l[0]), l[1] = fmaf(sum1, rv, l[1]);  // (the weights alone)
-            if (!I8 && lim < kUnit) {
-                // V rows past the length may hold NaN codes: their P is 0, and 0 * NaN is not 0
-                for (int j = lane; j < (kUnit - lim) * (D / 16); j += 32)
-                    *reinterpret_cast<uint4*>(stage + LY::kHalf + lim * D + j * 16) = make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes the stage next
-                __syncwarp();
-            }
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                // rows 16 b + 8 t + 2 tq + {0, 1} of V, D / 8 columns from D / 8 hd
-                uint32_t v[2][2][D / 32];
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int r = 16 * b + 8 * t + 2 * tq + e;
-                        if constexpr (D == 128) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(vb + tile_at<D>(r, hd));
-                            v[t][e][0] = x.x, v[t][e][1] = x.y, v[t][e][2] = x.z, v[t][e][3] = x.w;
-                        } else {
-                            const uint2 x = *reinterpret_cast<const uint2*>(vb + tile_at<D>(r, hd >> 1) + (hd & 1) * 8);
-                            v[t][e][0] = x.x, v[t][e][1] = x.y;
-                        }
-                    }
                 // (four tiles of columns at a time: a tile's second product waits for its first)
 #pragma unroll
                 for (int x = 0; x < D / 32; x += 2) {
                     uint32_t a0[8], a1[8];  // [tile * 2 + column]
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        pairs8<I8>(prmt(v[0][0][x + y], v[0][1][x + y], 0x5140), a0[4 * y], a0[4 * y + 1]);
-                        pairs8<I8>(prmt(v[0][0][x + y], v[0][1][x + y], 0x7362), a0[4 * y + 2], a0[4 * y + 3]);
-                        pairs8<I8>(prmt(v[1][0][x + y], v[1][1][x + y], 0x5140), a1[4 * y], a1[4 * y + 1]);
-                        pairs8<I8>(prmt(v[1][0][x + y], v[1][1][x + y], 0x7362), a1[4 * y + 2], a1[4 * y + 3]);
+                        pairs8<I8>(prmt(v[b][0][0][x + y], v[b][0][1][x + y], 0x5140), a0[4 * y], a0[4 * y + 1]);
+                        pairs8<I8>(prmt(v[b][0][0][x + y], v[b][0][1][x + y], 0x7362), a0[4 * y + 2], a0[4 * y + 3]);
+                        pairs8<I8>(prmt(v[b][1][0][x + y], v[b][1][1][x + y], 0x5140), a1[4 * y], a1[4 * y + 1]);
+                        pairs8<I8>(prmt(v[b][1][0][x + y], v[b][1][1][x + y], 0x7362), a1[4 * y + 2], a1[4 * y + 3]);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -653,10 +658,11 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
 
         // Each warp leaves its sums in shared memory and goes on.
         finish();
-        if (segs > 0 && ok) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(merged, (segs - 1) & 1, tmo));
-            if (!ok && lane == 0) report_error(a.err, kDevWaitDecode, 0xb5, segs);
+        if (segs > 0 && ok && !tc::mbar_wait(merged, (segs - 1) & 1, tmo)) {
+            ok = false;
+            report_error(a.err, kDevWaitDecode, 0xb5, segs);
         }
+        __syncwarp();
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
