@@ -84,6 +84,19 @@ __device__ __forceinline__ void from8(uint32_t w, float (&x)[4]) {
 // x / s: by its exact inverse where it has one.
 __device__ __forceinline__ float over(float x, float s, float inv) { return inv != 0.f ? x * inv : x / s; }
 
+// The bytes of rows [0, rows) of one head at `p` follow their page's scale from
+// `was` to `s`: thread `first` of `step` threads.
+template <bool I8>
+__device__ __forceinline__ void rescale8(uint8_t* p, int64_t stride, int rows, int d, float was, float s, int first, int step) {
+    const float f = was / s;
+    for (int i = first; i < rows * (d / 4); i += step) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(p + (int64_t)(i / (d / 4)) * stride) + i % (d / 4);
+        float x[4];
+        from8<I8>(*w, x);
+        *w = to8<I8>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+    }
+}
+
 // f32 bits of |x| where x is finite, else 0; `odd` is set where it is not.
 __device__ __forceinline__ uint32_t magnitude(float x, bool& odd) {
     const uint32_t b = __float_as_uint(x) & 0x7fffffffu;

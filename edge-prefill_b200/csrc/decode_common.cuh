@@ -118,7 +118,7 @@ __device__ __forceinline__ void store4(void* out, int32_t dtype, int64_t i, floa
             make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
     }
 }
-static_assert(kUnit == 32, "a lane per row, a page holds whole units");
+static_assert(kUnit == 32, "a lane per row, a page holds whole units of 2^5 rows");
 
 // The sequences' lengths: on chip when there are few, else the copy that
 // k6_lengths made.  Either way a CTA reads each once, or from memory that
@@ -135,8 +135,16 @@ struct Walk {
     int32_t s, run, u, n, units;  // sequence, run within it (h * passes + pass), next unit, length, units of the run
     int32_t left;                 // cost of the CTA's range from here on
     int32_t at;                   // where the run starts in the cost of all
+    int32_t per;                  // cost of a CTA's range
+    int32_t whole;                // log2 of the rows of a page that one CTA attends (the last page of a run, which the
+                                  // call writes a row into); 0: any unit may end a CTA's range
 
-    __device__ __forceinline__ int segment() const { return min(units - u, left); }
+    // First unit of the run's last page where one CTA attends it (else no unit is in it).
+    __device__ __forceinline__ int last_page() const { return whole > 0 ? (n - 1) >> whole << (whole - 5) : units; }
+    __device__ __forceinline__ int segment() const {
+        const int k = min(units - u, left);
+        return whole > 0 && u + k > last_page() ? units - u : k;
+    }
     __device__ __forceinline__ void advance(const DecodeArgs& a, const Lens& lens, int runs, int n_seg) {
         left -= n_seg + kRunCost;
         if (left <= 0) return;
@@ -160,24 +168,41 @@ __device__ __forceinline__ int cost_of(int units) { return units > 0 ? units + k
 __device__ __forceinline__ Walk share_of(const DecodeArgs& a, const DecodeSplit& sp, const Lens& lens, int runs,
                                          int lane) {
     Walk w{};
-    const int n_seq = a.kv.n_seq, part = (n_seq + 31) / 32;
+    const int n_seq = a.kv.n_seq;
+    if (n_seq == 1) {  // (the same without the search)
+        w.n = lens.at(a, 0);
+        w.units = units_of(w.n);
+        const int32_t cost = cost_of(w.units), total = cost * runs;
+        const int32_t per = max((int32_t)(((uint32_t)total + sp.ctas - 1) / (uint32_t)sp.ctas), kMinUnits);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *sp.per = per;
+        w.per = per;
+        const int64_t first = (int64_t)per * blockIdx.x;
+        if (first >= total) return w;
+        w.left = min(per, total - (int32_t)first);
+        w.run = (int32_t)((uint32_t)first / (uint32_t)cost);
+        const int32_t off = (int32_t)first - w.run * cost;
+        w.at = (int32_t)first - off;
+        w.u = max(0, off - kRunCost);
+        w.left -= max(0, kRunCost - off);
+        return w;
+    }
+    const int part = (n_seq + 31) / 32;
     const int s0 = min(n_seq, lane * part), s1 = min(n_seq, s0 + part);
     int32_t mine = 0;
     for (int s = s0; s < s1; ++s) mine += cost_of(units_of(lens.at(a, s)));
     mine *= runs;
     int32_t incl = mine;
-    if (n_seq > 1) {
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int32_t v = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += v;
-        }
+    for (int d = 1; d < 32; d <<= 1) {
+        const int32_t v = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += v;
     }
-    const int32_t total = __shfl_sync(0xffffffffu, incl, n_seq > 1 ? 31 : 0);
+    const int32_t total = __shfl_sync(0xffffffffu, incl, 31);
     const int32_t per = max((int32_t)(((uint32_t)total + sp.ctas - 1) / (uint32_t)sp.ctas), kMinUnits);
     if (blockIdx.x == 0 && threadIdx.x == 0) *sp.per = per;
     if (total / per < (int)blockIdx.x) return w;  // (the product below stays under total)
     const int32_t first = per * blockIdx.x;
+    w.per = per;
     if (first >= total) return w;
     w.left = min(per, total - first);
     const bool here = mine > 0 && first >= incl - mine && first < incl;

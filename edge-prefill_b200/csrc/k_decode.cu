@@ -173,7 +173,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1)
     tc::pdl_launch();
 
     // ----------------------------------------- this CTA's range of the units
-    Walk w0;
+    Walk w0{};
     Lens lens{nullptr};
     const int C = JOIN ? sp.cluster : 1, rank = blockIdx.x & (C - 1);
     if (JOIN || sp.direct) {

@@ -5,7 +5,9 @@
 //
 // Half the bytes of K6, and they bound it; the split of the rows over the CTAs,
 // the ring and the joins are K6's (decode_common.cuh).  A new token's row is
-// quantised into the cache by k9_append first.
+// quantised into the cache by the CTA that attends it: the last page of a run is
+// never split, and its copies wait for the row (as a kernel before, k9_append,
+// it took 3 to 4 us more; calls of several passes still have that).
 //
 // CTA: units (32 rows of one head, so one scale each of K and V) go round robin
 // to the streams of 8 warps, each with its own online softmax over 8 query heads
@@ -26,7 +28,7 @@
 // other scales add up in the accumulators as they are; the weights' sum takes P
 // over the scale.  The largest P is held between 2^14 and 2^15, and P is two
 // f16: an element keeps 22 bits of itself and an absolute 2^-39 of the largest
-// (half of f16's smallest step).
+// (half of f16's smallest step); one f16 where the output is bf16.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -39,6 +41,7 @@
 
 // (in units of 32 rows of 8 bits; 64 sequences of up to 4096 rows: 6 72 us, 10 64.2, 14 63.7, 20 64.5)
 #define EPSP_RUN_COST 14
+#include "cache8.cuh"
 #include "decode_common.cuh"
 #include "epsp_kernels.h"
 #include "tc100.cuh"
@@ -66,7 +69,7 @@ struct Layout8 {
     __host__ __device__ int off_ml() const { return off_o() + kWarps8 * 8 * D * 4; }  // [kWarps8][8] (maximum, sum)
     __host__ __device__ int off_scale() const { return off_ml() + kWarps8 * 8 * 8; }  // [stages] (ks, vs)
     __host__ __device__ int off_bar() const { return off_scale() + kMost * 8; }
-    __host__ __device__ int off_lens() const { return off_bar() + (2 * kMost + 6) * 8; }
+    __host__ __device__ int off_lens() const { return off_bar() + (2 * kMost + 7) * 8; }
     __host__ __device__ int bytes() const { return off_lens() + kLensOnChip * 4; }
     // For `pass` query heads of `es` bytes: as many stages as 227 KB hold.
     static Layout8 make(int pass, int es) {
@@ -188,8 +191,55 @@ __device__ __forceinline__ void store2(void* out, int32_t dtype, int64_t i, floa
     }
 }
 
-// LO: q has remainders (f32).  JOIN: the calls that join_cluster finishes.
-template <int D, bool I8, bool LO, bool JOIN>
+// A warp puts the new token's K and V row of one head into row n - 1 of the cache.
+template <int D, bool I8>
+__device__ __forceinline__ void append_row(const DecodeArgs& a, const Cache8& c, int s, int h, int n, int lane) {
+    constexpr int E = D / 32;  // elements of a lane
+    const int Hkv = a.n_head_kv, r0 = (n - 1) / c.page_size * c.page_size, lo = n - 1 - r0;
+    const int row = batch_row(a.kv, s, r0, a.err);
+    float x[2][E], was[2];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const int64_t i = ((int64_t)s * Hkv + h) * D + lane * E;
+        const void* src = v ? a.v_new : a.k_new;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            x[v][e] = a.dtype == 0   ? static_cast<const float*>(src)[i + e]
+                      : a.dtype == 1 ? __half2float(static_cast<const __half*>(src)[i + e])
+                                     : __bfloat162float(static_cast<const __nv_bfloat16*>(src)[i + e]);
+        was[v] = row >= 0 && lo > 0 ? (v ? c.v_scale : c.k_scale)[(int64_t)(row / c.page_size) * Hkv + h] : 0.f;
+    }
+    if (row < 0) return;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        bool odd = false;
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = max(m, magnitude(x[v][e], odd));
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (odd) report_error(a.err, kDevNotFinite8, 0x94, s);
+        uint8_t* dst = (v ? c.v : c.k) + ((int64_t)row * Hkv + h) * D;
+        float sc = scale8<I8>(m);
+        if (was[v] >= sc) sc = was[v];
+        else {
+            if (lo > 0) rescale8<I8>(dst, (int64_t)Hkv * D, lo, D, was[v], sc, lane, 32);
+            if (lane == 0) (v ? c.v_scale : c.k_scale)[(int64_t)(row / c.page_size) * Hkv + h] = sc;
+        }
+        const float inv = exact_inverse(sc);
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = tame8<I8>(over(x[v][e], sc, inv));
+        const uint32_t q = to8<I8>(y[0], y[1], y[2], y[3]);
+        uint8_t* to = dst + (int64_t)lo * Hkv * D + lane * E;
+        if constexpr (E == 4) *reinterpret_cast<uint32_t*>(to) = q;
+        else *reinterpret_cast<uint16_t*>(to) = (uint16_t)q;
+    }
+}
+
+// LO: q has remainders (f32).  P2: P has remainders (for outputs of 11 bits and
+// more; bf16's half step is eight times that of the f16 that P then is).
+// JOIN: the calls that join_cluster finishes.
+template <int D, bool I8, bool LO, bool P2, bool JOIN>
 __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     k10_decode8(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
                 const Cache8 c8, const DecodeSplit sp, const Layout8<D> ly) {
@@ -204,6 +254,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     uint64_t* q_empty = q_full + 2;
     uint64_t* written = q_empty + 2;       // the warps' sums of a segment are in shared memory,
     uint64_t* merged = written + 1;        // and out of it
+    uint64_t* appended = merged + 1;       // the CTA's new rows are in the cache
     int32_t* lens_s = reinterpret_cast<int32_t*>(smem + ly.off_lens());
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int Hkv = a.n_head_kv, G = a.n_head / Hkv, es = a.dtype == 0 ? 4 : 2;
@@ -221,6 +272,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         }
         tc::mbar_init(written, kWarps8);
         tc::mbar_init(merged, kWarps8);
+        tc::mbar_init(appended, kWarps8);
         tc::fence_mbar_init();
         tc::tma_prefetch_desc(&tmK);
         tc::tma_prefetch_desc(&tmV);
@@ -229,9 +281,11 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     tc::pdl_launch();
 
     // ----------------------------------------- this CTA's range of the units
-    Walk w0;
+    Walk w0{};
     Lens lens{nullptr};
     const int C = JOIN ? sp.cluster : 1, rank = blockIdx.x & (C - 1);
+    // the new rows are put into the cache by the CTAs that attend them
+    const int lg_whole = a.k_new != nullptr ? __ffs(c8.page_size) - 1 : 0;
     if (JOIN || sp.direct) {
         const int id = blockIdx.x >> (__ffs(C) - 1);
         w0.s = id / runs;
@@ -241,8 +295,11 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         w0.n = lens_s[0];
         w0.units = units_of(w0.n);
         const int per = (w0.units + C - 1) >> (__ffs(C) - 1);
-        w0.u = min(rank * per, w0.units);
-        w0.left = min(per, w0.units - w0.u);
+        w0.whole = lg_whole;
+        const int lp = w0.n > 0 ? w0.last_page() : 0;
+        auto cut_at = [&](int r) { return r * per > lp ? w0.units : min(r * per, w0.units); };
+        w0.u = cut_at(rank);
+        w0.left = cut_at(rank + 1) - w0.u;
     } else {
         if (a.kv.n_seq <= kLensOnChip) {
             for (int s = threadIdx.x; s < a.kv.n_seq; s += kAll) lens_s[s] = batch_len(a.kv, s, a.err);
@@ -250,6 +307,9 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         }
         __syncthreads();
         w0 = share_of(a, sp, lens, runs, lane);
+        w0.whole = lg_whole;
+        // (the CTA before has taken the rest of that page)
+        if (w0.left > 0 && w0.u > 0 && w0.u > w0.last_page()) w0.advance(a, lens, runs, w0.units - w0.u);
         // sequences without rows, dealt out to the CTAs
         for (int s = blockIdx.x; s < a.kv.n_seq; s += gridDim.x)
             if (lens.at(a, s) == 0) {
@@ -297,11 +357,16 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         int st = 0, fetched = 0;
         uint32_t phase = 1;  // (a stage's first fill waits for nobody)
         uint64_t since = 0;
-        bool more_q = asks && (w0.left > 0 || C > 1);
+        bool more_q = asks && (w0.left > 0 || C > 1), in_cache = a.k_new == nullptr;
         auto left = [&]() { return asks ? more_q : f.more(); };
         for (uint32_t idle = 0; __any_sync(0xffffffffu, left());) {
             const int at = st0 + st;
-            const bool go = left() && tc::mbar_test(asks ? &q_empty[st] : &empty[at], phase);
+            bool go = left() && tc::mbar_test(asks ? &q_empty[st] : &empty[at], phase);
+            if (go && !in_cache && !asks && f.w.u + f.at - f.before >= f.w.last_page()) {
+                go = in_cache = tc::mbar_test(appended, 0);
+                // (what was written there by stores is read by copies)
+                if (go) asm volatile("fence.proxy.async;" ::: "memory");
+            }
             if (go && asks) {
                 const int pass = f.w.run % sp.passes;
                 const uint32_t bytes = min(sp.pass_heads, G - pass * sp.pass_heads) * D * es;
@@ -353,6 +418,19 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     }
 
     // ---------------------------------------------------------- consumers --
+    if (a.k_new != nullptr) {
+        // the ends of runs in this CTA's range, dealt out to the warps, which have nothing to attend yet (done by the
+        // fetchers: 64 us for 64 sequences of up to 4096 rows, by a kernel before 65, here 60.8)
+        Walk x = w0;
+        for (int i = 0; x.left > 0;) {
+            const int n = x.segment();
+            if (x.u + n == x.units && (i++ & (kWarps8 - 1)) == warp) append_row<D, I8>(a, c8, x.s, x.run, x.n, lane);
+            x.advance(a, lens, runs, n);
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(appended);
+    }
     const int grp = warp & (groups - 1), stream = warp / groups;
     const int st0 = first_of(stream), depth = base + (stream < more ? 1 : 0);
     bool ok = true;
@@ -617,7 +695,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                 for (int j = 0; j < D / 16; ++j) o[j][0] *= alpha0, o[j][1] *= alpha1, o[j][2] *= alpha0, o[j][3] *= alpha1;
             }
             const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-            uint32_t ph[2][2], pl[2][2];  // keys 16 b + 8 half + 2 tq + {0, 1} of head hd
+            uint32_t ph[2][2], pl[P2 ? 2 : 1][2];  // keys 16 b + 8 half + 2 tq + {0, 1} of head hd
             float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -626,7 +704,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                     float x = ex2(s4[b][2 * t] - m0), y = ex2(s4[b][2 * t + 1] - m1);
                     sum0 += x, sum1 += y;
                     ph[b][t] = turned(split2<false>(x, y));
-                    pl[b][t] = turned(split2<false>(x, y));
+                    if constexpr (P2) pl[b][t] = turned(split2<false>(x, y));
                 }
             const float rv = ex2(-lv);
             l[0] = fmaf(sum0, rv, l[0]), l[1] = fmaf(sum1, rv, l[1]);  // (the weights alone)
@@ -646,9 +724,11 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], ph[b][0], ph[b][1]);
+                    if constexpr (P2) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], pl[b][0], pl[b][1]);
+                        for (int j = 0; j < 4; ++j)
+                            mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], pl[b][0], pl[b][1]);
+                    }
                 }
             }
             __syncwarp();
@@ -681,7 +761,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         whole = w.u == 0 && n_seg == w.units;
         head_row = q_row + pass * sp.pass_heads;
         pass_n = min(min(groups * 8, sp.pass_heads), G - pass * sp.pass_heads);
-        part = blockIdx.x * 2 + (seg == 0 ? 0 : 1);
+        part = blockIdx.x * 2 + (w.u == 0 && w.at > w.per * (int)blockIdx.x ? 1 : 0);
         if constexpr (JOIN) {
             finish();
             join_cluster<D, kThreads8, kPass8>(a, sp, smem, om, w, n_seg, head_row, pass_n, h, rank);
@@ -690,7 +770,9 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         if (!sp.direct && threadIdx.x == 0) {
             if (w.u == 0) sp.run_start[(int64_t)w.s * runs + w.run] = w.at;
             const int4 c =
-                w.u == 0 && n_seg < w.units ? make_int4(w.s, w.run, w.at, w.units) : make_int4(-1, 0, 0, 0);
+                w.u == 0 && n_seg < w.units
+                    ? make_int4(w.s, w.run, w.at, lg_whole > 0 ? w.last_page() + 1 : w.units)  // (whose is the last unit?)
+                    : make_int4(-1, 0, 0, 0);
             if (!sp.by_run)
                 sp.cut[blockIdx.x] = c;  // the CTA's last segment has the last word
             else if (w.u == 0)
@@ -761,7 +843,7 @@ size_t split8_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_he
     return at;
 }
 
-template <int D, bool I8, bool LO, bool JOIN>
+template <int D, bool I8, bool LO, bool P2, bool JOIN>
 cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, cudaStream_t s) {
     CUtensorMap mk, mv;
     if (!cache8_map(&mk, c.k, D, a.n_head_kv, a.kv.rows) || !cache8_map(&mv, c.v, D, a.n_head_kv, a.kv.rows))
@@ -774,7 +856,7 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
     static std::atomic<unsigned> set_mask{0};
     if (dev >= 32 || !(set_mask.load(std::memory_order_acquire) & (1u << dev))) {
         const cudaError_t e =
-            cudaFuncSetAttribute(k10_decode8<D, I8, LO, JOIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            cudaFuncSetAttribute(k10_decode8<D, I8, LO, P2, JOIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         if (dev < 32) set_mask.fetch_or(1u << dev, std::memory_order_release);
     }
@@ -801,7 +883,7 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
     cfg.blockDim = dim3(kThreads8 + 32 * kFetchers);
     cfg.dynamicSmemBytes = ly.bytes() + 1024;
     cfg.numAttrs = sp.cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k10_decode8<D, I8, LO, JOIN>, mk, mv, a, c, sp, ly);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k10_decode8<D, I8, LO, P2, JOIN>, mk, mv, a, c, sp, ly);
     if (e != cudaSuccess || sp.direct) return e;
     const int heads = std::min(a.n_head / a.n_head_kv, sp.pass_heads);
     const int64_t grid = (int64_t)sp.joins * heads;
@@ -814,9 +896,13 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
 
 template <int D, bool I8>
 cudaError_t launch8_t(const DecodeArgs& a, const Cache8& c, const DecodeSplit& sp, cudaStream_t s) {
+    const bool join = sp.cluster > 1;
     if (a.dtype == 0)
-        return sp.cluster > 1 ? launch8_join<D, I8, true, true>(a, c, sp, s) : launch8_join<D, I8, true, false>(a, c, sp, s);
-    return sp.cluster > 1 ? launch8_join<D, I8, false, true>(a, c, sp, s) : launch8_join<D, I8, false, false>(a, c, sp, s);
+        return join ? launch8_join<D, I8, true, true, true>(a, c, sp, s) : launch8_join<D, I8, true, true, false>(a, c, sp, s);
+    if (a.out_dtype == 2)
+        return join ? launch8_join<D, I8, false, false, true>(a, c, sp, s)
+                    : launch8_join<D, I8, false, false, false>(a, c, sp, s);
+    return join ? launch8_join<D, I8, false, true, true>(a, c, sp, s) : launch8_join<D, I8, false, true, false>(a, c, sp, s);
 }
 
 }  // namespace
@@ -827,14 +913,17 @@ size_t decode8_ws_bytes(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32
     return split8_of(n_seq, max_kv_len, n_head, n_head_kv, head_dim, dtype, nullptr, &sp);
 }
 
-cudaError_t launch_decode8(const DecodeArgs& a, const Cache8& c, cudaStream_t s) {
-    if (a.k_new) {
+cudaError_t launch_decode8(const DecodeArgs& args, const Cache8& c, cudaStream_t s) {
+    DecodeArgs a = args;
+    DecodeSplit sp{};
+    split8_of(a.kv.n_seq, a.kv.max_kv_len, a.n_head, a.n_head_kv, a.head_dim, a.dtype, static_cast<char*>(a.ws), &sp);
+    if (a.k_new && sp.passes > 1) {
+        // (several runs read the row: no one of them can write it)
         const AppendArgs w{a.kv, a.k_new, a.v_new, c, a.dtype, a.n_head_kv, a.head_dim, a.err};
         const cudaError_t e = launch_append8(w, s);
         if (e != cudaSuccess) return e;
+        a.k_new = a.v_new = nullptr;
     }
-    DecodeSplit sp{};
-    split8_of(a.kv.n_seq, a.kv.max_kv_len, a.n_head, a.n_head_kv, a.head_dim, a.dtype, static_cast<char*>(a.ws), &sp);
     if (a.head_dim == 128) return c.i8 ? launch8_t<128, true>(a, c, sp, s) : launch8_t<128, false>(a, c, sp, s);
     return c.i8 ? launch8_t<64, true>(a, c, sp, s) : launch8_t<64, false>(a, c, sp, s);
 }

@@ -80,19 +80,6 @@ __device__ __forceinline__ uint32_t top_of(uint32_t m) {
     return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
 }
 
-// The bytes of rows [0, rows) of one head at `p` follow their page's scale from
-// `was` to `s`.
-template <bool I8>
-__device__ __forceinline__ void rescale(uint8_t* p, int64_t stride, int rows, int d, float was, float s) {
-    const float f = was / s;
-    for (int i = threadIdx.x; i < rows * (d / 4); i += blockDim.x) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(p + (int64_t)(i / (d / 4)) * stride) + i % (d / 4);
-        float x[4];
-        from8<I8>(*w, x);
-        *w = to8<I8>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
-    }
-}
-
 // C: 16-byte chunks of a page and head per thread.
 template <int ET, bool I8, int C>
 __global__ void __launch_bounds__(kThreads, C <= 2 ? 6 : C <= 8 ? 4 : 2) k9_pack(const PackArgs a) {
@@ -155,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, C <= 2 ? 6 : C <= 8 ? 4 : 2) k9_pack
         float sc = scale8<I8>(m);
         if (was >= sc) sc = was;
         else {
-            if (lo > 0) rescale<I8>(dst, (int64_t)Hkv * d, lo, d, was, sc);
+            if (lo > 0) rescale8<I8>(dst, (int64_t)Hkv * d, lo, d, was, sc, threadIdx.x, blockDim.x);
             if (threadIdx.x == 0) *scale = sc;
         }
         const float inv = exact_inverse(sc);
@@ -288,7 +275,7 @@ __global__ void __launch_bounds__(128) k9_append(const AppendArgs a) {
     float sc = scale8<I8>(m);
     if (was >= sc) sc = was;
     else {
-        if (lo > 0) rescale<I8>(dst, (int64_t)Hkv * d, lo, d, was, sc);
+        if (lo > 0) rescale8<I8>(dst, (int64_t)Hkv * d, lo, d, was, sc, threadIdx.x, blockDim.x);
         if (t == 0) *scale = sc;
     }
     if (t < d) dst[(int64_t)lo * Hkv * d + t] = (uint8_t)to8<I8>(tame8<I8>(over(x, sc, exact_inverse(sc))), 0.f, 0.f, 0.f);

@@ -113,7 +113,7 @@ def write64(cache, state, i, x, a, t):
             s[p, h] = sc
 
 
-def decode64(cache, q, scale=None):
+def decode64(cache, q, scale=None, bf16_out=False):
     """Per sequence: out and its tolerance before the output's rounding, over what the cache holds."""
     n_seq, H, d = q.shape
     G = H // cache.K
@@ -134,11 +134,11 @@ def decode64(cache, q, scale=None):
             # numerator and denominator each carry one score error; a unit's sum of 32 and the sums over units (in f32)
             # cut at most a step each.  Weights (times V's scale) are two f16: 2^-22 of themselves, and no finer than
             # half of f16's smallest step, 2^-25, where the largest is 2^14 at least: n times 2^-39 of the largest
-            # meets bytes of at most TOP
+            # meets bytes of at most TOP.  For bf16 outputs of 16-bit models they are one f16: half a step, 2^-11
             e = 2 * (score_error(mag, d) + lost)
             out[i, h * G:(h + 1) * G] = p @ v[:, h]
             vs = cache.vs[cache.at(i, n).cuda() // cache.page, h].double()
-            tol[i, h * G:(h + 1) * G] = ((p @ v[:, h].abs()) * (e + 2.0 ** -21 + (64 + n / 32) * 2.0 ** -23)
+            tol[i, h * G:(h + 1) * G] = ((p @ v[:, h].abs()) * (e + (2.0 ** -11 if bf16_out else 2.0 ** -21) + (64 + n / 32) * 2.0 ** -23)
                                          + n * 2.0 ** -39 * TOP[cache.q8] * (p * vs).amax(1, keepdim=True))
     return out, tol
 

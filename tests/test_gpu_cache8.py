@@ -200,7 +200,7 @@ def run(ctx, c, q, out_dtype=epsp.F32, ws=None, kn=None, vn=None, stream=None):
 
 
 def held(out, c, q, out_dtype, scale=None):
-    ref, tol = decode64(c, q, scale)
+    ref, tol = decode64(c, q, scale, out_dtype == epsp.BF16 and q.dtype != torch.float32)
     err = (out.double() - ref).abs()
     assert bool((err <= tol + rounding(ref, out_dtype)).all()), float((err - tol).max())
 
