@@ -11,11 +11,13 @@
 // depend on timing.
 //
 // The planning is latency (a few dependent passes over refs and tables), the
-// copies are bandwidth.  A plan runs in one cluster of CTAs: its passes meet at
-// cluster barriers, a launch would cost more than a pass.  What is copied (pairs
+// copies are bandwidth.  A plan runs in one CTA, on arrays in shared memory, or in
+// one cluster of CTAs, on arrays in the workspace: its passes meet at barriers, a
+// launch would cost more than a pass.  What is copied (pairs
 // of blocks) is known on the device only; the copies of all pools follow in one
-// launch that reads the pairs, 4 KB to a warp, eight 16-byte loads a lane in
-// flight.
+// launch that reads the pairs.  One thread per SM moves 16 KB pieces through
+// shared memory by bulk copies, eleven in flight; what is not made of 16-byte
+// pieces (scales) goes through registers.
 #include <algorithm>
 #include <climits>
 
@@ -27,14 +29,39 @@ namespace {
 
 constexpr int kPlan = 1024;       // threads of a planning CTA
 constexpr int kPlanCtas = 8;      // CTAs of its cluster, at most
-constexpr int kPlanItems = 4096;  // sequences and blocks up to which one CTA plans
+// What one CTA plans in shared memory (blocks and sequences, tables' entries);
+// more is planned in the workspace by a cluster.  400 blocks: 4 us against 8.
+constexpr int kSmallBlocks = 8192;
+constexpr int kSmallSeqs = 4096;
+constexpr int kSmallEntries = 16384;
 constexpr int kPoolsPerLaunch = 128;
-constexpr int kChunk = 4096;      // bytes a warp copies at a time
+constexpr int kBulk = 16384;      // bytes of a bulk copy
+constexpr int kStages = 12;
+constexpr int kPlain = 512;       // bytes a warp copies at a time
+constexpr int kCopyThreads = 128;
 
+// The pools that bulk copies take come first.
 struct PoolList {
     Pool p[kPoolsPerLaunch];
-    int32_t end[kPoolsPerLaunch];  // chunks of a block in the pools up to this one
-    int32_t n;
+    int32_t end[kPoolsPerLaunch];  // pieces of a block in the pools of its kind up to this one
+    int32_t n_bulk, n;
+};
+
+// Piece c of a block in the pools [lo, hi].
+struct Piece {
+    char* rows;
+    size_t bytes, at;  // of a block; where the piece begins
+    __device__ __forceinline__ Piece(const PoolList& l, int lo, int hi, int c, int size) {
+        const int first = lo;
+        while (lo < hi) {  // the pool whose pieces hold c
+            const int mid = (lo + hi) >> 1;
+            if (l.end[mid] > c) hi = mid;
+            else lo = mid + 1;
+        }
+        rows = static_cast<char*>(l.p[lo].rows);
+        bytes = l.p[lo].bytes;
+        at = (size_t)(c - (lo > first ? l.end[lo - 1] : 0)) * size;
+    }
 };
 
 __host__ __device__ __forceinline__ int blocks_of(int rows, int block_rows) {
@@ -126,6 +153,51 @@ __global__ void k11_fork_write(const PagesArgs a, const ForkWs w) {
     }
 }
 
+// Both in one CTA, with what the tables held in shared memory.
+__global__ void __launch_bounds__(kPlan, 1) k11_fork(const PagesArgs a, const int32_t* parents, const int32_t* lens) {
+    extern __shared__ int32_t tables_s[];  // [n_seq][table_stride], then [n_seq] lengths and new lengths
+    int32_t *was_s = tables_s + a.n_seq * a.table_stride, *now_s = was_s + a.n_seq, *parent_s = now_s + a.n_seq;
+    tc::pdl_wait();
+    tc::pdl_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int s = threadIdx.x; s < a.n_seq; s += kPlan) {
+        was_s[s] = rows_of(a, a.lens[s], s);
+        parent_s[s] = parents[s];
+        now_s[s] = lens ? lens[s] : -1;
+    }
+    __syncthreads();
+    for (int s = warp; s < a.n_seq; s += kPlan / 32) {
+        const int held = blocks_of(was_s[s], a.block_rows);
+        for (int i = lane; i < held; i += 32) tables_s[s * a.table_stride + i] = a.tables[(int64_t)s * a.table_stride + i];
+    }
+    __syncthreads();
+    for (int s = warp; s < a.n_seq; s += kPlan / 32) {
+        int p = parent_s[s], now = -1;
+        const int was = was_s[s];
+        if (p >= -1 && p < a.n_seq) {
+            const int have = p < 0 ? 0 : was_s[p];
+            now = lens ? now_s[s] : have;
+            if (now < 0 || now > have) now = -1;
+        }
+        if (now < 0) {  // stays as it is
+            if (lane == 0) report_error(a.err, kDevBadParent, 0xc2, s);
+            continue;
+        }
+        if (p == s && now == was) continue;
+        const int held = blocks_of(was, a.block_rows), want = blocks_of(now, a.block_rows);
+        for (int i = lane; i < max(held, want); i += 32) {
+            const int old = i < held ? tables_s[s * a.table_stride + i] : -1, b = i < want ? tables_s[p * a.table_stride + i] : -1;
+            if (i < held && i < want && old == b) continue;
+            if (i < held && entry(a, old, s) >= 0) atomicAdd(&a.refs[old], -1);
+            if (i < want) {
+                if (entry(a, b, s) >= 0) atomicAdd(&a.refs[b], 1);
+                a.tables[(int64_t)s * a.table_stride + i] = b;
+            }
+        }
+        if (lane == 0) a.lens[s] = now;
+    }
+}
+
 // ----------------------------------------------------------------- planning --
 __device__ __forceinline__ int cluster_rank() {
     uint32_t r;
@@ -137,11 +209,20 @@ __device__ __forceinline__ int cluster_size() {
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return (int)r;
 }
-// All threads of the plan, and what they wrote to global memory.  (Reads of what
-// another CTA wrote go past the L1: __ldcg.)
+// SMALL: one CTA, the plan's arrays in shared memory.  All threads of the plan
+// meet, and see what they wrote; reads of what another CTA wrote go past the L1.
+template <bool SMALL>
 __device__ __forceinline__ void meet() {
-    __threadfence();
-    tc::cluster_sync();
+    if constexpr (SMALL) {
+        __syncthreads();
+    } else {
+        __threadfence();
+        tc::cluster_sync();
+    }
+}
+template <bool SMALL>
+__device__ __forceinline__ int32_t at(const int32_t* p) {
+    return SMALL ? *p : __ldcg(p);
 }
 
 // Exclusive sum over the CTA's threads of two counts; the totals in `all`.
@@ -173,7 +254,12 @@ __device__ __forceinline__ int2 cta_scan(int2 x, int2& all, int2* box) {
 
 // Totals of all CTAs from those of this one (what the CTAs before it have in
 // `before`).
+template <bool SMALL>
 __device__ __forceinline__ int2 cluster_scan(int2 mine, int2& before, int2* shared) {
+    if constexpr (SMALL) {
+        before = make_int2(0, 0);
+        return mine;
+    }
     if (threadIdx.x == 0) *shared = mine;
     tc::cluster_sync();
     int2 all = make_int2(0, 0);
@@ -202,21 +288,33 @@ __device__ __forceinline__ Part part_of(int64_t n) {
 struct ResizeWs {
     int32_t* n_pairs;  // [4] the count first
     int2* pairs;       // [n_seq] (from, to)
-    int32_t *refs, *growers, *keeper;  // [pool_blocks]; growers and keeper: of a shared last block
-    int32_t *was, *now, *need, *off;   // [n_seq]
-    int32_t* free;                     // [pool_blocks] free blocks taken, in order
+    // the rest in the workspace, or in shared memory
+    int32_t *refs, *growers, *keeper;        // [pool_blocks]; growers and keeper: of a shared last block
+    int32_t* free;                           // [pool_blocks] free blocks taken, in order
+    int32_t *was, *now, *last, *need, *off;  // [n_seq]; last: a block that a sequence grows in, -1 where it is its own
 };
 
-// Sequence s's last block where it grows inside one that others hold too, else -1.
-__device__ __forceinline__ int shared_last(const PagesArgs& a, const ResizeWs& w, int s) {
-    const int was = __ldcg(&w.was[s]), now = __ldcg(&w.now[s]);
-    if (now <= was || was % a.block_rows == 0) return -1;
-    const int b = a.tables[(int64_t)s * a.table_stride + was / a.block_rows];
-    return b >= 0 && b < a.pool_blocks && __ldcg(&w.refs[b]) > 1 ? b : -1;
+// Lays out the arrays that a plan works on; returns the bytes.
+__host__ __device__ inline size_t plan_arrays(const PagesArgs& a, char* base, ResizeWs* w) {
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        int32_t* p = reinterpret_cast<int32_t*>(base + at);
+        at += (n * 4 + 15) & ~(size_t)15;
+        return p;
+    };
+    w->refs = take(a.pool_blocks), w->growers = take(a.pool_blocks), w->keeper = take(a.pool_blocks);
+    w->free = take(a.pool_blocks);
+    w->was = take(a.n_seq), w->now = take(a.n_seq), w->last = take(a.n_seq);
+    w->need = take(a.n_seq), w->off = take(a.n_seq);
+    return at;
 }
 
-__global__ void __launch_bounds__(kPlan, 1) k11_resize(const PagesArgs a, const int32_t* new_lens, const ResizeWs w) {
+template <bool SMALL>
+__global__ void __launch_bounds__(kPlan, 1) k11_resize(const PagesArgs a, const int32_t* new_lens, ResizeWs w) {
     __shared__ int2 box[32], mine_s;
+    __shared__ int pairs_s;
+    extern __shared__ __align__(16) char plan_s[];
+    if constexpr (SMALL) plan_arrays(a, plan_s, &w);
     tc::pdl_wait();
     tc::pdl_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -236,36 +334,43 @@ __global__ void __launch_bounds__(kPlan, 1) k11_resize(const PagesArgs a, const 
         }
         w.was[s] = n;
         w.now[s] = now;
+        // (held by others or not is known once all have given back)
+        const int b = now > n && n % a.block_rows ? a.tables[s * a.table_stride + n / a.block_rows] : -1;
+        w.last[s] = b >= 0 && b < a.pool_blocks ? b : -1;
     }
-    if (me == 0 && lane == 0) *w.n_pairs = 0;
-    meet();
+    if (me == 0 && lane == 0) *(SMALL ? &pairs_s : w.n_pairs) = 0;
+    meet<SMALL>();
     // blocks given back
     for (int s = me; s < a.n_seq; s += warps) {
-        const int held = blocks_of(__ldcg(&w.was[s]), a.block_rows), want = blocks_of(__ldcg(&w.now[s]), a.block_rows);
+        const int held = blocks_of(at<SMALL>(&w.was[s]), a.block_rows), want = blocks_of(at<SMALL>(&w.now[s]), a.block_rows);
         for (int i = want + lane; i < held; i += 32) {
             const int b = entry(a, a.tables[(int64_t)s * a.table_stride + i], s);
             if (b >= 0) atomicAdd(&w.refs[b], -1);
         }
     }
-    meet();
+    meet<SMALL>();
     // who grows inside a block that others hold too
     for (int64_t s = seqs.begin + threadIdx.x; s < seqs.end; s += kPlan) {
-        const int b = shared_last(a, w, (int)s);
-        if (b >= 0) {
+        const int b = w.last[s];
+        if (b < 0) continue;
+        if (at<SMALL>(&w.refs[b]) > 1) {
             atomicAdd(&w.growers[b], 1);
             atomicMax(&w.keeper[b], (int)s);
+        } else {
+            w.last[s] = -1;
         }
     }
-    meet();
+    meet<SMALL>();
     // what each sequence takes; where all holders of a block grow, the last one keeps it
     int2 run = make_int2(0, 0);
     for (int64_t s0 = seqs.begin; s0 < seqs.end; s0 += kPlan) {
         const int64_t s = s0 + threadIdx.x;
         int need = 0;
         if (s < seqs.end) {
-            const int b = shared_last(a, w, (int)s);
-            const bool copy = b >= 0 && !(__ldcg(&w.growers[b]) == __ldcg(&w.refs[b]) && __ldcg(&w.keeper[b]) == (int)s);
-            need = max(0, blocks_of(__ldcg(&w.now[s]), a.block_rows) - blocks_of(__ldcg(&w.was[s]), a.block_rows)) + (copy ? 1 : 0);
+            const int b = w.last[s];
+            const bool copy =
+                b >= 0 && !(at<SMALL>(&w.growers[b]) == at<SMALL>(&w.refs[b]) && at<SMALL>(&w.keeper[b]) == (int)s);
+            need = max(0, blocks_of(w.now[s], a.block_rows) - blocks_of(w.was[s], a.block_rows)) + (copy ? 1 : 0);
             w.need[s] = copy ? -need : need;  // (negative: its first block is the copy)
         }
         int2 all;
@@ -275,12 +380,15 @@ __global__ void __launch_bounds__(kPlan, 1) k11_resize(const PagesArgs a, const 
     }
     for (int64_t b0 = blocks.begin; b0 < blocks.end; b0 += kPlan) {
         const int64_t b = b0 + threadIdx.x;
-        run.y += __syncthreads_count(b < blocks.end && __ldcg(&w.refs[b]) == 0);
+        run.y += __syncthreads_count(b < blocks.end && at<SMALL>(&w.refs[b]) == 0);
     }
     int2 before;
-    const int2 all = cluster_scan(run, before, &mine_s);
+    const int2 all = cluster_scan<SMALL>(run, before, &mine_s);
     if (all.x > all.y) {  // too few: nothing changes
-        if (me == 0 && lane == 0) report_error(a.err, kDevNoBlocks, 0xc4, all.x - all.y);
+        if (me == 0 && lane == 0) {
+            *w.n_pairs = 0;
+            report_error(a.err, kDevNoBlocks, 0xc4, all.x - all.y);
+        }
         return;
     }
     // this CTA's sequences take from here; its free blocks have these places
@@ -289,35 +397,37 @@ __global__ void __launch_bounds__(kPlan, 1) k11_resize(const PagesArgs a, const 
     for (int64_t b0 = blocks.begin; b0 < blocks.end; b0 += kPlan) {
         const int64_t b = b0 + threadIdx.x;
         const bool in = b < blocks.end;
-        const int refs = in ? __ldcg(&w.refs[b]) : 1;
+        const int refs = in ? at<SMALL>(&w.refs[b]) : 1;
         int2 here;
         const int2 at = cta_scan(make_int2(0, refs == 0 ? 1 : 0), here, box);
         if (refs == 0 && place + at.y < all.x) w.free[place + at.y] = (int)b;
         if (in) a.refs[b] = refs;
         place += here.y;
     }
-    meet();
+    meet<SMALL>();
     for (int s = me; s < a.n_seq; s += warps) {
-        const int was = __ldcg(&w.was[s]), now = __ldcg(&w.now[s]), off = __ldcg(&w.off[s]), need = __ldcg(&w.need[s]);
+        const int was = at<SMALL>(&w.was[s]), now = at<SMALL>(&w.now[s]), off = at<SMALL>(&w.off[s]), need = at<SMALL>(&w.need[s]);
         const int held = blocks_of(was, a.block_rows), want = blocks_of(now, a.block_rows), copy = need < 0;
         int32_t* table = a.tables + (int64_t)s * a.table_stride;
         for (int i = held + lane; i < want; i += 32) {
-            const int b = __ldcg(&w.free[off + copy + i - held]);
+            const int b = at<SMALL>(&w.free[off + copy + i - held]);
             table[i] = b;
             a.refs[b] = 1;
         }
         if (lane == 0) {
             if (copy) {
-                const int from = entry(a, table[held - 1], s), to = __ldcg(&w.free[off]);
+                const int from = at<SMALL>(&w.last[s]), to = at<SMALL>(&w.free[off]);
                 table[held - 1] = to;
                 a.refs[to] = 1;
-                if (from >= 0) {
-                    atomicAdd(&a.refs[from], -1);
-                    w.pairs[atomicAdd(w.n_pairs, 1)] = make_int2(from, to);  // (their order does not matter)
-                }
+                atomicAdd(&a.refs[from], -1);
+                w.pairs[atomicAdd(SMALL ? &pairs_s : w.n_pairs, 1)] = make_int2(from, to);  // (their order does not matter)
             }
             a.lens[s] = now;
         }
+    }
+    if constexpr (SMALL) {
+        __syncthreads();
+        if (threadIdx.x == 0) *w.n_pairs = pairs_s;
     }
 }
 
@@ -327,46 +437,60 @@ struct CompactWs {
     int32_t* map;      // [pool_blocks] where a moved block went
 };
 
+template <bool SMALL>
 __global__ void __launch_bounds__(kPlan, 1) k11_compact(const PagesArgs a, int32_t* n_used, const CompactWs w) {
     __shared__ int2 box[32], mine_s;
+    extern __shared__ __align__(16) char plan_s[];
+    int32_t* refs_s = reinterpret_cast<int32_t*>(plan_s);  // SMALL: [pool_blocks], then the pairs
+    int2* pairs = SMALL ? reinterpret_cast<int2*>(plan_s + ((size_t)a.pool_blocks * 4 + 15) / 16 * 16) : w.pairs;
     tc::pdl_wait();
     tc::pdl_launch();
     const Part blocks = part_of(a.pool_blocks);
     int2 run = make_int2(0, 0);
     for (int64_t b0 = blocks.begin; b0 < blocks.end; b0 += kPlan) {
         const int64_t b = b0 + threadIdx.x;
-        run.x += __syncthreads_count(b < blocks.end && a.refs[b] > 0);
+        const int refs = b < blocks.end ? a.refs[b] : 0;
+        if (SMALL && b < blocks.end) refs_s[b] = refs;
+        run.x += __syncthreads_count(refs > 0);
     }
     int2 before;
-    const int used = cluster_scan(run, before, &mine_s).x;
+    const int used = cluster_scan<SMALL>(run, before, &mine_s).x;
+    const int32_t* refs = SMALL ? refs_s : a.refs;
     // holes below, blocks in use at or past `used`: as many of each
     auto what = [&](int64_t b) {
-        const bool live = b < blocks.end && a.refs[b] > 0;
+        const bool live = b < blocks.end && refs[b] > 0;
         return make_int2(b < blocks.end && b < used && !live, b >= used && live);
     };
-    run = make_int2(0, 0);
-    for (int64_t b0 = blocks.begin; b0 < blocks.end; b0 += kPlan) {
-        const int2 x = what(b0 + threadIdx.x);
-        run.x += __syncthreads_count(x.x);
-        run.y += __syncthreads_count(x.y);
+    int2 all;
+    if constexpr (!SMALL) {
+        run = make_int2(0, 0);
+        for (int64_t b0 = blocks.begin; b0 < blocks.end; b0 += kPlan) {
+            const int2 x = what(b0 + threadIdx.x);
+            run.x += __syncthreads_count(x.x);
+            run.y += __syncthreads_count(x.y);
+        }
+        all = cluster_scan<SMALL>(run, before, &mine_s);
+    } else {
+        before = make_int2(0, 0);
     }
-    const int2 all = cluster_scan(run, before, &mine_s);
     for (int64_t b0 = blocks.begin; b0 < blocks.end; b0 += kPlan) {
         const int64_t b = b0 + threadIdx.x;
         const int2 x = what(b);
         int2 here;
         const int2 at = cta_scan(x, here, box);
-        if (x.x) w.pairs[before.x + at.x].y = (int)b;
-        if (x.y) w.pairs[before.y + at.y].x = (int)b;
+        if (x.x) pairs[before.x + at.x].y = (int)b;
+        if (x.y) pairs[before.y + at.y].x = (int)b;
         else if (b < blocks.end && b >= used) w.map[b] = (int)b;
         before.x += here.x;
         before.y += here.y;
     }
-    meet();
+    if constexpr (SMALL) all = before;
+    meet<SMALL>();
     for (int i = cluster_rank() * kPlan + threadIdx.x; i < all.y; i += cluster_size() * kPlan) {
-        const int2 p = __ldcg(&w.pairs[i]);
+        const int2 p = SMALL ? pairs[i] : __ldcg(&pairs[i]);
         w.map[p.x] = p.y;
-        a.refs[p.y] = a.refs[p.x];
+        if constexpr (SMALL) w.pairs[i] = p;
+        a.refs[p.y] = refs[p.x];
         a.refs[p.x] = 0;
     }
     if (cluster_rank() == 0 && threadIdx.x == 0) {
@@ -378,14 +502,79 @@ __global__ void __launch_bounds__(kPlan, 1) k11_compact(const PagesArgs a, int32
 
 // Copies the pairs' blocks in every pool; `used` (not null): tables follow the
 // map, too.
-__global__ void __launch_bounds__(256) k11_copy(const PagesArgs a, const __grid_constant__ PoolList pools,
-                                                const int32_t* n_pairs, const int2* pairs, const int32_t* used,
-                                                const int32_t* map) {
+__global__ void __launch_bounds__(kCopyThreads) k11_copy(const PagesArgs a, const __grid_constant__ PoolList pools,
+                                                         const int32_t* n_pairs, const int2* pairs, const int32_t* used,
+                                                         const int32_t* map, uint64_t timeout_ns) {
+    extern __shared__ __align__(128) char stage_s[];
+    __shared__ uint64_t full[kStages];
+    __shared__ char* dst_s[kStages];
+    __shared__ uint32_t bytes_s[kStages];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) tc::mbar_init(&full[i], 1);
+        tc::fence_mbar_init();
+    }
     tc::pdl_wait();
     tc::pdl_launch();
-    const int lane = threadIdx.x & 31;
-    const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32), me = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
-    const int n = *n_pairs, per = pools.n ? pools.end[pools.n - 1] : 0;
+    const int n = *n_pairs;
+    if (warp == 0) {
+        if (pools.n_bulk == 0) return;
+        const int per = pools.end[pools.n_bulk - 1];
+        const int64_t items = (int64_t)n * per;
+        const int mine = (int)((items - blockIdx.x + gridDim.x - 1) / gridDim.x);  // (0 or less: none)
+        // Piece k is asked for when piece k - (kStages - 1) is sent on; 32 pieces' places at a time, one per lane
+        // (one thread for all of it: 113 us for 264 MB).
+        const char* src = nullptr;
+        char* dst = nullptr;
+        uint32_t bytes = 0;
+        bool ok = true;
+        auto send = [&](int k) {
+            if (lane == 0) {
+                ok = tc::mbar_wait(&full[k % kStages], (k / kStages) & 1, timeout_ns);
+                if (ok) {
+                    tc::bulk_store(dst_s[k % kStages], stage_s + k % kStages * kBulk, bytes_s[k % kStages]);
+                    tc::bulk_commit();
+                    tc::bulk_wait_read<1>();  // the stage of the piece before is free
+                } else {
+                    report_error(a.err, kDevWaitPages, 0xc5, k);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+        };
+        int k = 0, sent = 0;
+        for (; k < mine && ok; ++k) {
+            if ((k & 31) == 0 && k + lane < mine) {
+                const int64_t t = blockIdx.x + (int64_t)(k + lane) * gridDim.x;
+                const int2 pair = pairs[t / per];
+                const Piece x(pools, 0, pools.n_bulk - 1, (int)(t % per), kBulk);
+                src = x.rows + pair.x * x.bytes + x.at;
+                dst = x.rows + pair.y * x.bytes + x.at;
+                bytes = (uint32_t)min((size_t)kBulk, x.bytes - x.at);
+            }
+            if (k >= kStages - 1) {
+                send(sent++);
+                if (!ok) break;
+            }
+            const char* from = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(src), k & 31));
+            char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), k & 31));
+            const uint32_t size = __shfl_sync(0xffffffffu, bytes, k & 31);
+            if (lane == 0) {
+                dst_s[k % kStages] = to;
+                bytes_s[k % kStages] = size;
+                tc::mbar_arrive_expect_tx(&full[k % kStages], size);
+                tc::bulk_load(stage_s + k % kStages * kBulk, from, size, &full[k % kStages]);
+            }
+        }
+        while (sent < k && ok) send(sent++);
+        if (lane == 0) {
+            // (after a wait that ran out: copies still in flight land before the CTA ends)
+            if (!ok)
+                for (int j = sent; j < k; ++j) tc::mbar_wait(&full[j % kStages], (j / kStages) & 1, timeout_ns);
+            tc::bulk_wait_read<0>();
+        }
+        return;
+    }
+    const int64_t warps = (int64_t)gridDim.x * (kCopyThreads / 32 - 1), me = (int64_t)blockIdx.x * (kCopyThreads / 32 - 1) + warp - 1;
     if (used && n > 0) {
         const int from = *used;
         for (int64_t s = me; s < a.n_seq; s += warps) {
@@ -397,36 +586,27 @@ __global__ void __launch_bounds__(256) k11_copy(const PagesArgs a, const __grid_
             }
         }
     }
+    if (pools.n_bulk == pools.n) return;
+    const int per = pools.end[pools.n - 1];
     for (int64_t t = me; t < (int64_t)n * per; t += warps) {
         const int2 pair = pairs[t / per];
-        const int c = (int)(t % per);
-        int lo = 0, hi = pools.n - 1;  // the pool whose chunks hold c
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (pools.end[mid] > c) hi = mid;
-            else lo = mid + 1;
-        }
-        const size_t bytes = pools.p[lo].bytes, at = (size_t)(c - (lo ? pools.end[lo - 1] : 0)) * kChunk;
-        const char* src = static_cast<const char*>(pools.p[lo].rows) + pair.x * bytes + at;
-        char* dst = static_cast<char*>(pools.p[lo].rows) + pair.y * bytes + at;
-        const int here = (int)min((size_t)kChunk, bytes - at);
-        if (((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | here) & 15) == 0) {
-            uint4 v[kChunk / 512];
+        const Piece x(pools, pools.n_bulk, pools.n - 1, (int)(t % per), kPlain);
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(x.rows + pair.x * x.bytes + x.at);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(x.rows + pair.y * x.bytes + x.at);
+        const int words = (int)min((size_t)kPlain, x.bytes - x.at) / 4;
+        uint32_t v[kPlain / 128];
 #pragma unroll
-            for (int j = 0; j < kChunk / 512; ++j)
-                if ((j * 32 + lane) * 16 < here) v[j] = __ldcs(reinterpret_cast<const uint4*>(src) + j * 32 + lane);
+        for (int j = 0; j < kPlain / 128; ++j)
+            if (j * 32 + lane < words) v[j] = src[j * 32 + lane];
 #pragma unroll
-            for (int j = 0; j < kChunk / 512; ++j)
-                if ((j * 32 + lane) * 16 < here) __stcs(reinterpret_cast<uint4*>(dst) + j * 32 + lane, v[j]);
-        } else {
-            for (int i = lane * 4; i < here; i += 128) *reinterpret_cast<uint32_t*>(dst + i) = *reinterpret_cast<const uint32_t*>(src + i);
-        }
+        for (int j = 0; j < kPlain / 128; ++j)
+            if (j * 32 + lane < words) dst[j * 32 + lane] = v[j];
     }
 }
 
 // ---------------------------------------------------------------- host side --
 template <class... P, class... A>
-cudaError_t go(void (*kernel)(P...), dim3 grid, int threads, int cluster, cudaStream_t s, A&&... args) {
+cudaError_t go(void (*kernel)(P...), dim3 grid, int threads, int cluster, size_t smem, cudaStream_t s, A&&... args) {
     cudaLaunchAttribute at[2]{};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -436,13 +616,19 @@ cudaError_t go(void (*kernel)(P...), dim3 grid, int threads, int cluster, cudaSt
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = at;
     cfg.numAttrs = cluster ? 2 : 1;
+    if (smem > 48 * 1024) {
+        // (the same for all calls: two threads may be here with different sizes)
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        if (e != cudaSuccess) return e;
+    }
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
-int plan_ctas(const PagesArgs& a) { return std::max(a.n_seq, a.pool_blocks) <= kPlanItems ? 1 : kPlanCtas; }
+bool small_plan(const PagesArgs& a) { return a.n_seq <= kSmallSeqs && a.pool_blocks <= kSmallBlocks; }
 
 // Lays out `n` bytes at the workspace's next 16-byte boundary.
 struct Space {
@@ -469,14 +655,7 @@ size_t resize_ws(const PagesArgs& a, void* ws, ResizeWs* w) {
     Space sp{static_cast<char*>(ws)};
     w->n_pairs = sp.take<int32_t>(4);
     w->pairs = sp.take<int2>(a.n_seq);
-    w->refs = sp.take<int32_t>(a.pool_blocks);
-    w->growers = sp.take<int32_t>(a.pool_blocks);
-    w->keeper = sp.take<int32_t>(a.pool_blocks);
-    w->free = sp.take<int32_t>(a.pool_blocks);
-    w->was = sp.take<int32_t>(a.n_seq);
-    w->now = sp.take<int32_t>(a.n_seq);
-    w->need = sp.take<int32_t>(a.n_seq);
-    w->off = sp.take<int32_t>(a.n_seq);
+    sp.at += plan_arrays(a, sp.base + sp.at, w);
     return sp.at;
 }
 
@@ -493,18 +672,28 @@ size_t compact_ws(const PagesArgs& a, void* ws, CompactWs* w) {
 cudaError_t copy_pools(const PagesArgs& a, const Pool* pools, int32_t n_pools, int64_t most, const int32_t* n_pairs,
                        const int2* pairs, const int32_t* used, const int32_t* map, cudaStream_t s) {
     for (int32_t i0 = 0; i0 < n_pools; i0 += kPoolsPerLaunch) {
-        PoolList l{};
-        l.n = std::min(kPoolsPerLaunch, n_pools - i0);
-        int64_t chunks = 0;
-        for (int i = 0; i < l.n; ++i) {
-            l.p[i] = pools[i0 + i];
-            chunks += (int64_t)((l.p[i].bytes + kChunk - 1) / kChunk);
-            if (chunks > INT_MAX) return cudaErrorInvalidValue;
-            l.end[i] = (int32_t)chunks;
+        const int32_t n = std::min(kPoolsPerLaunch, n_pools - i0);
+        PoolList l;
+        l.n = 0;
+        int64_t pieces[2] = {0, 0};
+        for (int plain = 0; plain < 2; ++plain) {
+            for (int32_t i = i0; i < i0 + n; ++i) {
+                const bool by_bulk = ((reinterpret_cast<uintptr_t>(pools[i].rows) | pools[i].bytes) & 15) == 0;
+                if (by_bulk == (plain != 0)) continue;
+                const size_t size = plain ? kPlain : kBulk;
+                pieces[plain] += (int64_t)((pools[i].bytes + size - 1) / size);
+                if (pieces[plain] > INT_MAX) return cudaErrorInvalidValue;
+                l.p[l.n] = pools[i];
+                l.end[l.n++] = (int32_t)pieces[plain];
+            }
+            if (!plain) l.n_bulk = l.n;
         }
-        const int64_t ctas = std::min<int64_t>(148 * 8, (chunks * std::max<int64_t>(most, 1) + 7) / 8);
-        const cudaError_t e = go(k11_copy, dim3((unsigned)std::max<int64_t>(ctas, 1)), 256, 0, s, a, l, n_pairs, pairs,
-                                 i0 == 0 ? used : nullptr, map);
+        const int64_t pairs_most = std::max<int64_t>(most, 1), warps = kCopyThreads / 32 - 1;
+        const int64_t ctas = std::max({pieces[0] * pairs_most, (pieces[1] * pairs_most + warps - 1) / warps,
+                                       used && i0 == 0 ? (int64_t)(a.n_seq + warps - 1) / warps : 0});
+        const cudaError_t e = go(k11_copy, dim3((unsigned)std::min<int64_t>(ctas, 148)), kCopyThreads, 0,
+                                 l.n_bulk ? (size_t)kStages * kBulk : 0, s, a, l, n_pairs, pairs, i0 == 0 ? used : nullptr, map,
+                                 a.timeout_ns);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -513,8 +702,8 @@ cudaError_t copy_pools(const PagesArgs& a, const Pool* pools, int32_t n_pools, i
 }  // namespace
 
 cudaError_t launch_count_refs(const PagesArgs& a, cudaStream_t s) {
-    const cudaError_t e = go(k11_zero, dim3(std::min(592, (a.pool_blocks + 255) / 256)), 256, 0, s, a.refs, (int64_t)a.pool_blocks);
-    return e != cudaSuccess ? e : go(k11_count, dim3(std::min(a.n_seq, 1184)), 128, 0, s, a);
+    const cudaError_t e = go(k11_zero, dim3(std::min(592, (a.pool_blocks + 255) / 256)), 256, 0, 0, s, a.refs, (int64_t)a.pool_blocks);
+    return e != cudaSuccess ? e : go(k11_count, dim3(std::min(a.n_seq, 1184)), 128, 0, 0, s, a);
 }
 
 size_t fork_ws_bytes(const PagesArgs& a) {
@@ -523,11 +712,13 @@ size_t fork_ws_bytes(const PagesArgs& a) {
 }
 
 cudaError_t launch_fork(const PagesArgs& a, const int32_t* parents, const int32_t* lens, void* ws, cudaStream_t s) {
+    if ((int64_t)a.n_seq * a.table_stride <= kSmallEntries && a.n_seq <= kSmallSeqs)
+        return go(k11_fork, dim3(1), kPlan, 0, (size_t)a.n_seq * (a.table_stride + 3) * 4, s, a, parents, lens);
     ForkWs w;
     fork_ws(a, ws, &w);
     const dim3 grid(std::min(a.n_seq, 4096), std::min(16, (a.table_stride + 255) / 256));
-    const cudaError_t e = go(k11_fork_read, grid, 256, 0, s, a, parents, lens, w);
-    return e != cudaSuccess ? e : go(k11_fork_write, grid, 256, 0, s, a, w);
+    const cudaError_t e = go(k11_fork_read, grid, 256, 0, 0, s, a, parents, lens, w);
+    return e != cudaSuccess ? e : go(k11_fork_write, grid, 256, 0, 0, s, a, w);
 }
 
 size_t resize_ws_bytes(const PagesArgs& a) {
@@ -539,8 +730,10 @@ cudaError_t launch_resize(const PagesArgs& a, const int32_t* new_lens, const Poo
                           cudaStream_t s) {
     ResizeWs w;
     resize_ws(a, ws, &w);
-    const int ctas = plan_ctas(a);
-    const cudaError_t e = go(k11_resize, dim3(ctas), kPlan, ctas, s, a, new_lens, w);
+    ResizeWs none;
+    const cudaError_t e = small_plan(a)
+                              ? go(k11_resize<true>, dim3(1), kPlan, 0, plan_arrays(a, nullptr, &none), s, a, new_lens, w)
+                              : go(k11_resize<false>, dim3(kPlanCtas), kPlan, kPlanCtas, 0, s, a, new_lens, w);
     if (e != cudaSuccess) return e;
     return copy_pools(a, pools, n_pools, a.n_seq, w.n_pairs, w.pairs, nullptr, nullptr, s);
 }
@@ -554,8 +747,9 @@ cudaError_t launch_compact(const PagesArgs& a, const Pool* pools, int32_t n_pool
                            cudaStream_t s) {
     CompactWs w;
     compact_ws(a, ws, &w);
-    const int ctas = plan_ctas(a);
-    const cudaError_t e = go(k11_compact, dim3(ctas), kPlan, ctas, s, a, n_used, w);
+    const size_t smem = ((size_t)a.pool_blocks * 4 + 15) / 16 * 16 + ((size_t)a.pool_blocks / 2 + 1) * 8;
+    const cudaError_t e = small_plan(a) ? go(k11_compact<true>, dim3(1), kPlan, 0, smem, s, a, n_used, w)
+                                        : go(k11_compact<false>, dim3(kPlanCtas), kPlan, kPlanCtas, 0, s, a, n_used, w);
     if (e != cudaSuccess) return e;
     return copy_pools(a, pools, n_pools, a.pool_blocks / 2, w.n_pairs, w.pairs, w.n_pairs + 1, w.map, s);
 }

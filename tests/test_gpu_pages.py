@@ -80,7 +80,8 @@ class Both:
 
 
 @pytest.mark.parametrize("n_seq,stride,B,blocks", [(1, 1, 32, 1), (5, 4, 32, 17), (40, 6, 64, 150), (300, 3, 32, 700),
-                                                   (70, 5, 32, 5000), (5000, 2, 32, 6000)], ids=str)
+                                                   (70, 5, 32, 5000), (70, 5, 32, 9000),
+                                                   (5000, 2, 32, 6000)], ids=str)
 def test_a_server_s_life(n_seq, stride, B, blocks):
     """Sequences grow, fork, are cut back, freed and compacted in a random order."""
     x = Both(n_seq, stride, B, blocks, n_seq, sizes=None if blocks < 1000 else [4, 20, 4100])
