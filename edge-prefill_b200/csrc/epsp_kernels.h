@@ -31,7 +31,6 @@ enum DeviceError : int32_t {
     kDevNoBlocks = 0x503,      // the pool has fewer free blocks than a resize needs
     kDevWaitDecode = 0x601,    // a decode KV unit did not arrive (or leave) in time
     kDevWaitWeights = 0x602,   // a prompt-weight tile did not arrive (or leave) in time
-    kDevWaitPages = 0x603,     // a piece of a block did not arrive in time
 };
 
 // The device error word is err[0] of a 4-word record: the kernel whose
@@ -388,7 +387,6 @@ struct PagesArgs {
     int32_t* tables;  // [n_seq][table_stride]
     int32_t* refs;    // [pool_blocks]
     int32_t* err;
-    uint64_t timeout_ns;
 };
 struct Pool {
     void* rows;          // [pool_blocks][bytes]

@@ -30,7 +30,7 @@ const char* wrong_pages(const ep_sp_config& c, const ep_sp_pages* p) {
 }
 
 epsp::PagesArgs args_of(const ep_sp_pages* p) {
-    return {p->n_seq, p->table_stride, p->block_rows, p->pool_blocks, p->kv_lens, p->block_tables, p->refs, nullptr, 0};
+    return {p->n_seq, p->table_stride, p->block_rows, p->pool_blocks, p->kv_lens, p->block_tables, p->refs, nullptr};
 }
 
 int32_t check_pages(ep_sp_ctx* ctx, const ep_sp_pages* p, const char* who, epsp::PagesArgs* a) {
@@ -68,7 +68,6 @@ int32_t run(ep_sp_ctx* ctx, epsp::PagesArgs& a, void* stream, const char* what, 
     const int32_t rc = enter(ctx, s);
     if (rc) return rc;
     a.err = ctx->d_err;
-    a.timeout_ns = ctx->timeout_ns;
     return launch(ctx, kPages, stream, what, [&] { return go(s); });
 }
 

@@ -15,9 +15,9 @@
 // one cluster of CTAs, on arrays in the workspace: its passes meet at barriers, a
 // launch would cost more than a pass.  What is copied (pairs
 // of blocks) is known on the device only; the copies of all pools follow in one
-// launch that reads the pairs.  One thread per SM moves 16 KB pieces through
-// shared memory by bulk copies, eleven in flight; what is not made of 16-byte
-// pieces (scales) goes through registers.
+// launch that reads the pairs, 4 KB to a warp, eight 16-byte loads a lane in
+// flight (16 KB pieces through shared memory by bulk copies, eleven in flight per
+// SM: 107 us against 103 for 264 MB, 26 against 23 for 38).
 #include <algorithm>
 #include <climits>
 
@@ -35,33 +35,12 @@ constexpr int kSmallBlocks = 8192;
 constexpr int kSmallSeqs = 4096;
 constexpr int kSmallEntries = 16384;
 constexpr int kPoolsPerLaunch = 128;
-constexpr int kBulk = 16384;      // bytes of a bulk copy
-constexpr int kStages = 12;
-constexpr int kPlain = 512;       // bytes a warp copies at a time
-constexpr int kCopyThreads = 128;
+constexpr int kChunk = 4096;      // bytes a warp copies at a time
 
-// The pools that bulk copies take come first.
 struct PoolList {
     Pool p[kPoolsPerLaunch];
-    int32_t end[kPoolsPerLaunch];  // pieces of a block in the pools of its kind up to this one
-    int32_t n_bulk, n;
-};
-
-// Piece c of a block in the pools [lo, hi].
-struct Piece {
-    char* rows;
-    size_t bytes, at;  // of a block; where the piece begins
-    __device__ __forceinline__ Piece(const PoolList& l, int lo, int hi, int c, int size) {
-        const int first = lo;
-        while (lo < hi) {  // the pool whose pieces hold c
-            const int mid = (lo + hi) >> 1;
-            if (l.end[mid] > c) hi = mid;
-            else lo = mid + 1;
-        }
-        rows = static_cast<char*>(l.p[lo].rows);
-        bytes = l.p[lo].bytes;
-        at = (size_t)(c - (lo > first ? l.end[lo - 1] : 0)) * size;
-    }
+    int32_t end[kPoolsPerLaunch];  // chunks of a block in the pools up to this one
+    int32_t n;
 };
 
 __host__ __device__ __forceinline__ int blocks_of(int rows, int block_rows) {
@@ -502,79 +481,14 @@ __global__ void __launch_bounds__(kPlan, 1) k11_compact(const PagesArgs a, int32
 
 // Copies the pairs' blocks in every pool; `used` (not null): tables follow the
 // map, too.
-__global__ void __launch_bounds__(kCopyThreads) k11_copy(const PagesArgs a, const __grid_constant__ PoolList pools,
-                                                         const int32_t* n_pairs, const int2* pairs, const int32_t* used,
-                                                         const int32_t* map, uint64_t timeout_ns) {
-    extern __shared__ __align__(128) char stage_s[];
-    __shared__ uint64_t full[kStages];
-    __shared__ char* dst_s[kStages];
-    __shared__ uint32_t bytes_s[kStages];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) tc::mbar_init(&full[i], 1);
-        tc::fence_mbar_init();
-    }
+__global__ void __launch_bounds__(256) k11_copy(const PagesArgs a, const __grid_constant__ PoolList pools,
+                                                const int32_t* n_pairs, const int2* pairs, const int32_t* used,
+                                                const int32_t* map) {
     tc::pdl_wait();
     tc::pdl_launch();
-    const int n = *n_pairs;
-    if (warp == 0) {
-        if (pools.n_bulk == 0) return;
-        const int per = pools.end[pools.n_bulk - 1];
-        const int64_t items = (int64_t)n * per;
-        const int mine = (int)((items - blockIdx.x + gridDim.x - 1) / gridDim.x);  // (0 or less: none)
-        // Piece k is asked for when piece k - (kStages - 1) is sent on; 32 pieces' places at a time, one per lane
-        // (one thread for all of it: 113 us for 264 MB).
-        const char* src = nullptr;
-        char* dst = nullptr;
-        uint32_t bytes = 0;
-        bool ok = true;
-        auto send = [&](int k) {
-            if (lane == 0) {
-                ok = tc::mbar_wait(&full[k % kStages], (k / kStages) & 1, timeout_ns);
-                if (ok) {
-                    tc::bulk_store(dst_s[k % kStages], stage_s + k % kStages * kBulk, bytes_s[k % kStages]);
-                    tc::bulk_commit();
-                    tc::bulk_wait_read<1>();  // the stage of the piece before is free
-                } else {
-                    report_error(a.err, kDevWaitPages, 0xc5, k);
-                }
-            }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-        };
-        int k = 0, sent = 0;
-        for (; k < mine && ok; ++k) {
-            if ((k & 31) == 0 && k + lane < mine) {
-                const int64_t t = blockIdx.x + (int64_t)(k + lane) * gridDim.x;
-                const int2 pair = pairs[t / per];
-                const Piece x(pools, 0, pools.n_bulk - 1, (int)(t % per), kBulk);
-                src = x.rows + pair.x * x.bytes + x.at;
-                dst = x.rows + pair.y * x.bytes + x.at;
-                bytes = (uint32_t)min((size_t)kBulk, x.bytes - x.at);
-            }
-            if (k >= kStages - 1) {
-                send(sent++);
-                if (!ok) break;
-            }
-            const char* from = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(src), k & 31));
-            char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(dst), k & 31));
-            const uint32_t size = __shfl_sync(0xffffffffu, bytes, k & 31);
-            if (lane == 0) {
-                dst_s[k % kStages] = to;
-                bytes_s[k % kStages] = size;
-                tc::mbar_arrive_expect_tx(&full[k % kStages], size);
-                tc::bulk_load(stage_s + k % kStages * kBulk, from, size, &full[k % kStages]);
-            }
-        }
-        while (sent < k && ok) send(sent++);
-        if (lane == 0) {
-            // (after a wait that ran out: copies still in flight land before the CTA ends)
-            if (!ok)
-                for (int j = sent; j < k; ++j) tc::mbar_wait(&full[j % kStages], (j / kStages) & 1, timeout_ns);
-            tc::bulk_wait_read<0>();
-        }
-        return;
-    }
-    const int64_t warps = (int64_t)gridDim.x * (kCopyThreads / 32 - 1), me = (int64_t)blockIdx.x * (kCopyThreads / 32 - 1) + warp - 1;
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32), me = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
+    const int n = *n_pairs, per = pools.n ? pools.end[pools.n - 1] : 0;
     if (used && n > 0) {
         const int from = *used;
         for (int64_t s = me; s < a.n_seq; s += warps) {
@@ -586,21 +500,30 @@ __global__ void __launch_bounds__(kCopyThreads) k11_copy(const PagesArgs a, cons
             }
         }
     }
-    if (pools.n_bulk == pools.n) return;
-    const int per = pools.end[pools.n - 1];
     for (int64_t t = me; t < (int64_t)n * per; t += warps) {
         const int2 pair = pairs[t / per];
-        const Piece x(pools, pools.n_bulk, pools.n - 1, (int)(t % per), kPlain);
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(x.rows + pair.x * x.bytes + x.at);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(x.rows + pair.y * x.bytes + x.at);
-        const int words = (int)min((size_t)kPlain, x.bytes - x.at) / 4;
-        uint32_t v[kPlain / 128];
+        const int c = (int)(t % per);
+        int lo = 0, hi = pools.n - 1;  // the pool whose chunks hold c
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (pools.end[mid] > c) hi = mid;
+            else lo = mid + 1;
+        }
+        const size_t bytes = pools.p[lo].bytes, at = (size_t)(c - (lo ? pools.end[lo - 1] : 0)) * kChunk;
+        const char* src = static_cast<const char*>(pools.p[lo].rows) + pair.x * bytes + at;
+        char* dst = static_cast<char*>(pools.p[lo].rows) + pair.y * bytes + at;
+        const int here = (int)min((size_t)kChunk, bytes - at);
+        if (((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | here) & 15) == 0) {
+            uint4 v[kChunk / 512];
 #pragma unroll
-        for (int j = 0; j < kPlain / 128; ++j)
-            if (j * 32 + lane < words) v[j] = src[j * 32 + lane];
+            for (int j = 0; j < kChunk / 512; ++j)
+                if ((j * 32 + lane) * 16 < here) v[j] = __ldcs(reinterpret_cast<const uint4*>(src) + j * 32 + lane);
 #pragma unroll
-        for (int j = 0; j < kPlain / 128; ++j)
-            if (j * 32 + lane < words) dst[j * 32 + lane] = v[j];
+            for (int j = 0; j < kChunk / 512; ++j)
+                if ((j * 32 + lane) * 16 < here) __stcs(reinterpret_cast<uint4*>(dst) + j * 32 + lane, v[j]);
+        } else {
+            for (int i = lane * 4; i < here; i += 128) *reinterpret_cast<uint32_t*>(dst + i) = *reinterpret_cast<const uint32_t*>(src + i);
+        }
     }
 }
 
@@ -668,32 +591,24 @@ size_t compact_ws(const PagesArgs& a, void* ws, CompactWs* w) {
 }
 
 // The copies of all pools, kPoolsPerLaunch a launch; the first also rewrites the
-// tables.
-cudaError_t copy_pools(const PagesArgs& a, const Pool* pools, int32_t n_pools, int64_t most, const int32_t* n_pairs,
+// tables.  `over`: CTAs per SM at most.  More even out the copies' ends (264 MB:
+// 8 103 us, 32 98, 64 97), and cost a call that copies nothing: a step's growth
+// within its blocks takes 8.4 us with 8, 12 with 32.
+cudaError_t copy_pools(const PagesArgs& a, const Pool* pools, int32_t n_pools, int64_t most, int32_t over, const int32_t* n_pairs,
                        const int2* pairs, const int32_t* used, const int32_t* map, cudaStream_t s) {
     for (int32_t i0 = 0; i0 < n_pools; i0 += kPoolsPerLaunch) {
-        const int32_t n = std::min(kPoolsPerLaunch, n_pools - i0);
-        PoolList l;
-        l.n = 0;
-        int64_t pieces[2] = {0, 0};
-        for (int plain = 0; plain < 2; ++plain) {
-            for (int32_t i = i0; i < i0 + n; ++i) {
-                const bool by_bulk = ((reinterpret_cast<uintptr_t>(pools[i].rows) | pools[i].bytes) & 15) == 0;
-                if (by_bulk == (plain != 0)) continue;
-                const size_t size = plain ? kPlain : kBulk;
-                pieces[plain] += (int64_t)((pools[i].bytes + size - 1) / size);
-                if (pieces[plain] > INT_MAX) return cudaErrorInvalidValue;
-                l.p[l.n] = pools[i];
-                l.end[l.n++] = (int32_t)pieces[plain];
-            }
-            if (!plain) l.n_bulk = l.n;
+        PoolList l{};
+        l.n = std::min(kPoolsPerLaunch, n_pools - i0);
+        int64_t chunks = 0;
+        for (int i = 0; i < l.n; ++i) {
+            l.p[i] = pools[i0 + i];
+            chunks += (int64_t)((l.p[i].bytes + kChunk - 1) / kChunk);
+            if (chunks > INT_MAX) return cudaErrorInvalidValue;
+            l.end[i] = (int32_t)chunks;
         }
-        const int64_t pairs_most = std::max<int64_t>(most, 1), warps = kCopyThreads / 32 - 1;
-        const int64_t ctas = std::max({pieces[0] * pairs_most, (pieces[1] * pairs_most + warps - 1) / warps,
-                                       used && i0 == 0 ? (int64_t)(a.n_seq + warps - 1) / warps : 0});
-        const cudaError_t e = go(k11_copy, dim3((unsigned)std::min<int64_t>(ctas, 148)), kCopyThreads, 0,
-                                 l.n_bulk ? (size_t)kStages * kBulk : 0, s, a, l, n_pairs, pairs, i0 == 0 ? used : nullptr, map,
-                                 a.timeout_ns);
+        const int64_t ctas = std::min<int64_t>(148 * over, (chunks * std::max<int64_t>(most, 1) + 7) / 8);
+        const cudaError_t e = go(k11_copy, dim3((unsigned)std::max<int64_t>(ctas, 1)), 256, 0, 0, s, a, l, n_pairs, pairs,
+                                 i0 == 0 ? used : nullptr, map);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -735,7 +650,7 @@ cudaError_t launch_resize(const PagesArgs& a, const int32_t* new_lens, const Poo
                               ? go(k11_resize<true>, dim3(1), kPlan, 0, plan_arrays(a, nullptr, &none), s, a, new_lens, w)
                               : go(k11_resize<false>, dim3(kPlanCtas), kPlan, kPlanCtas, 0, s, a, new_lens, w);
     if (e != cudaSuccess) return e;
-    return copy_pools(a, pools, n_pools, a.n_seq, w.n_pairs, w.pairs, nullptr, nullptr, s);
+    return copy_pools(a, pools, n_pools, a.n_seq, 8, w.n_pairs, w.pairs, nullptr, nullptr, s);
 }
 
 size_t compact_ws_bytes(const PagesArgs& a) {
@@ -751,7 +666,7 @@ cudaError_t launch_compact(const PagesArgs& a, const Pool* pools, int32_t n_pool
     const cudaError_t e = small_plan(a) ? go(k11_compact<true>, dim3(1), kPlan, 0, smem, s, a, n_used, w)
                                         : go(k11_compact<false>, dim3(kPlanCtas), kPlan, kPlanCtas, 0, s, a, n_used, w);
     if (e != cudaSuccess) return e;
-    return copy_pools(a, pools, n_pools, a.pool_blocks / 2, w.n_pairs, w.pairs, w.n_pairs + 1, w.map, s);
+    return copy_pools(a, pools, n_pools, a.pool_blocks / 2, 32, w.n_pairs, w.pairs, w.n_pairs + 1, w.map, s);
 }
 
 }  // namespace epsp

@@ -125,18 +125,6 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                  : "memory");
 }
 
-// The way back: completes with the bulk group that bulk_commit closes.
-__device__ __forceinline__ void bulk_store(void* dst, const void* smem_src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(smem_src)), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// Waits until at most N of this thread's latest groups have still to read shared memory.
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() {
-    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
-
 // 4 bytes of global memory into this CTA's shared memory; copies_arrive arrives
 // once on `bar` when this thread's copies so far have landed.
 __device__ __forceinline__ void copy4_async(void* smem_dst, const void* src) {
