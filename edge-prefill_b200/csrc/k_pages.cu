@@ -128,7 +128,7 @@ __global__ void k11_fork_write(const PagesArgs a, const ForkWs w) {
                 a.tables[row + i] = b;
             }
         }
-        if (blockIdx.y == 0 && threadIdx.x == 0) a.lens[s] = now;
+        if (blockIdx.y == 0 && threadIdx.x == 0 && (p != s || now != w.was[s])) a.lens[s] = now;
     }
 }
 

@@ -280,6 +280,66 @@ def test_steps_of_decoding(dtype, q8):
     ctx.check(ctx.sync_status())
 
 
+@pytest.mark.parametrize("q8", [E, Q], ids=name)
+@pytest.mark.parametrize("heads,page,dtype", [((8, 2, 128), 128, epsp.BF16), ((7, 1, 64), 32, epsp.F16),
+                                              ((12, 4, 128), 64, epsp.F32), ((34, 2, 64), 128, epsp.BF16)], ids=str)
+def test_new_rows_of_ragged_batches(heads, page, dtype, q8):
+    """Batches that are split over the device anywhere but in the page that a new row goes into: lengths that end
+    pages, begin them, lie in the first or fill several, and rows that make scales grow."""
+    H, K, d = heads
+    lens = [(i * 977) % 2300 for i in range(37)] + [page, page + 1, 1, 2299, 2 * page - 1]
+    c = Cache8(lens, K, d, q8, page, page, 1)
+    ctx = context(H, K, d, dtype, epsp.F32, max(lens), page)
+    n = len(lens)
+    q, kn, vn = randq(n, H, d, dtype), randq(n, K, d, dtype, 6), randq(n, K, d, dtype, 7)
+    kn[::3] *= 8
+    vn[1::3] *= 8
+    want = c.state()
+    for i, m in enumerate(lens):
+        if m:
+            for t, x in enumerate((kn, vn)):
+                write64(c, want, i, x[i].expand(m, K, d), m - 1, t)
+    out = run(ctx, c, q, kn=kn, vn=vn)
+    ctx.check(ctx.sync_status())
+    assert same(c.state(), want)
+    held(out, c, q, epsp.F32)
+    assert torch.equal(run(ctx, c, q, kn=kn, vn=vn), out)  # (the same rows again: the same bytes)
+
+
+def test_captured_packs_and_unpacks():
+    """Replayed as lengths and rows change; on another stream than the current one."""
+    K, d, page = 2, 64, 32
+    src = Cache([150, 90], K, d, epsp.F16, 0, 1)
+    dst = Cache8([150, 90], K, d, E, page, page, 2, capacity=150)
+    out = Cache([150, 90], K, d, epsp.F16, page, 3)
+    ctx = context(K, K, d, epsp.F16, epsp.F16, 150, page)
+    first, s, g = ints([0, 0]), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    batch8 = epsp.KvBatch(src.d_lens, 150, dst.d_table, page, dst.rows)
+    was = dst.state()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        ctx.check(ctx.pack_kv(0, src.batch, src.k, src.v, dst.batch, dst.kv8, first=first, stream=s))
+        ctx.check(ctx.unpack_kv(0, batch8, dst.kv8, out.batch, out.k, out.v, first=first, stream=s))
+    torch.cuda.synchronize()
+    assert same(dst.state(), was)
+    for lens, at in (([40, 90], [0, 0]), ([150, 64], [40, 3]), ([0, 1], [0, 1])):
+        src.d_lens.copy_(ints(lens)), first.copy_(ints(at))
+        want, refs = dst.state(), [out.k.clone(), out.v.clone()]
+        for i, n in enumerate(lens):
+            for t, x in enumerate((src.k, src.v)):
+                write64(dst, want, i, x[i * 150:i * 150 + n], at[i], t)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert same(dst.state(), want)
+        for i, n in enumerate(lens):
+            dst.lens[i] = n
+            for t, x in enumerate(dst.seq(i)):
+                refs[t][out.at(i, n)[at[i]:].cuda()] = x[at[i]:].half()
+        assert same([out.k, out.v], refs)
+    ctx.check(ctx.sync_status())
+
+
 @pytest.mark.parametrize("dtype", [epsp.BF16, epsp.F16, epsp.F32], ids=name)
 def test_magnitudes_of_queries_scales_and_weights(dtype):
     """Scales of neighbouring pages far apart, a large and a tiny query, weights that underflow."""
