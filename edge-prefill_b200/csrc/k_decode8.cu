@@ -55,6 +55,12 @@ constexpr int kFetchers = 4;             // warps that fetch
 constexpr float kUp8 = 14.f;      // P is 2^14 times what it is against the running maximum,
 constexpr float kSlack8 = 1.f;    // which follows when it is twice that behind: 2^15 at most
 constexpr int kPass8 = 64;        // query heads of a pass, at most
+// Units for each CTA of a cluster up to which a run is joined in shared memory
+// instead of being split over the device: one launch. One sequence of 6000, 12,000,
+// 16,000 and 24,000 rows, split 13.0, 15.1, 16.5 and 18.2 us, in clusters of 8 10.1,
+// 13.5, 15.5 and 19.8 (32 heads on 8); split 13.3, 14.5, 16.2 and 17.4, in clusters
+// 10.8, 15.0, 17.4 and 22.9 (28 on 4).
+constexpr int kClusterMost8 = 48;
 
 // Shared memory: the stages, then what follows by offset.
 template <int D>
@@ -818,7 +824,7 @@ size_t split8_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_he
     if (!sp->direct) {
         while (sp->cluster < kMaxCluster && units > sp->cluster * kClusterUnits && all_runs * sp->cluster * 2 <= kClusterCtas)
             sp->cluster *= 2;
-        sp->direct = sp->cluster > 1 && units <= sp->cluster * 2 * kClusterUnits;
+        sp->direct = sp->cluster > 1 && units <= sp->cluster * kClusterMost8;
         if (!sp->direct) sp->cluster = 1;
     }
     const int64_t ctas = sp->direct ? all_runs * sp->cluster : (total + kMinUnits - 1) / kMinUnits;

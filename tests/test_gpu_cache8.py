@@ -404,16 +404,17 @@ def test_table_entries_outside_the_pool_and_lengths_are_reported():
     assert ctx.sync_status() == epsp.PREFILL and same(c.state(), was)
 
 
-def test_captured_steps_streams_and_workspaces():
+@pytest.mark.parametrize("capacity", [3000, 40000])  # joined in a cluster, and by the second kernel
+def test_captured_steps_streams_and_workspaces(capacity):
     """A captured step replayed as lengths, rows and queries change, next to another one on its own workspace."""
     H, K, d, page = 14, 2, 64, 64
-    ctx = context(H, K, d, epsp.F16, epsp.F32, 3000, page)
+    ctx = context(H, K, d, epsp.F16, epsp.F32, capacity, page)
     runs = []
     for seed in (1, 2):
-        c = Cache8([700, 2500, 64], K, d, E, page, page, seed, capacity=3000)
+        c = Cache8([700, 2500, 64], K, d, E, page, page, seed, capacity=capacity)
         x = dict(q=randq(3, H, d, epsp.F16, seed), kn=randq(3, K, d, epsp.F16, seed + 10),
                  vn=randq(3, K, d, epsp.F16, seed + 20), out=torch.zeros(3, H, d, device="cuda"),
-                 ws=workspace(ctx.decode8_bytes(3, 3000)), s=torch.cuda.Stream())
+                 ws=workspace(ctx.decode8_bytes(3, capacity)), s=torch.cuda.Stream())
         g = torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
         was = c.state()
