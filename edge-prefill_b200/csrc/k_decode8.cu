@@ -54,6 +54,11 @@ constexpr int kThreads8 = kWarps8 * 32;  // that attend
 constexpr int kFetchers = 4;             // warps that fetch
 constexpr float kUp8 = 14.f;      // P is 2^14 times what it is against the running maximum,
 constexpr float kSlack8 = 1.f;    // which follows when it is twice that behind: 2^15 at most
+// log2 of V's scale in P is this at least (a page of zeros has a scale of 2^-100):
+// a weight is in the sum of weights while P is above f32's smallest, so that the
+// scales of a run may differ by 2^116, and the sum stays below 2^110.  What is
+// missing goes into P when it is f16 already.
+constexpr float kLeastV8 = -64.f;
 constexpr int kPass8 = 64;        // query heads of a pass, at most
 // Units for each CTA of a cluster up to which a run is joined in shared memory
 // instead of being split over the device: one launch. One sequence of 6000, 12,000,
@@ -133,6 +138,12 @@ __device__ __forceinline__ void mma8_first(float (&c)[4], uint32_t a0, uint32_t 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Two f16 times two.
+__device__ __forceinline__ uint32_t times2(uint32_t x, uint32_t y) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // Units of a block, and the place of a unit: dividing by a number that is known
@@ -668,7 +679,15 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                         }
                     }
             // log2 of the weight times V's scale: that is what O is the sum of
-            const float lv = __log2f(sc.y);
+            float lv = __log2f(sc.y);
+            uint32_t down = 0;  // factor of P for a scale below 2^kLeastV8
+            if (lv < kLeastV8) {
+                lv = fmaxf(lv, -200.f);
+                const float k = ceilf(kLeastV8 - lv);
+                lv += k;
+                const __half2 f = __float2half2_rn(ex2(-k));
+                down = *reinterpret_cast<const uint32_t*>(&f) | 0x80008000u;
+            }
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -712,6 +731,16 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                     ph[b][t] = turned(split2<false>(x, y));
                     if constexpr (P2) pl[b][t] = turned(split2<false>(x, y));
                 }
+            if (down) {
+                const uint32_t f = down & 0x7fff7fffu;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        ph[b][t] = times2(ph[b][t], f);
+                        if constexpr (P2) pl[b][t] = times2(pl[b][t], f);
+                    }
+            }
             const float rv = ex2(-lv);
             l[0] = fmaf(sum0, rv, l[0]), l[1] = fmaf(sum1, rv, l[1]);  // (the weights alone)
 #pragma unroll

@@ -361,6 +361,50 @@ def test_magnitudes_of_queries_scales_and_weights(dtype):
     ctx.check(ctx.sync_status())
 
 
+@pytest.mark.parametrize("dtype", [epsp.F16, epsp.F32], ids=name)
+def test_pages_of_zeros_next_to_large_values(dtype):
+    """A page of zeros has the smallest scale there is; its weights count all the same."""
+    H, K, d, page = 4, 2, 64, 32
+    c = Cache8([700, 90], K, d, E, page, 0, 1)
+    p = torch.arange(c.ks.shape[0], device="cuda") % 3
+    c.ks[:] = 2.0 ** -8
+    c.vs[:] = torch.exp2(torch.tensor([-100.0, 40.0, -8.0], device="cuda")[p])[:, None]
+    c.v8.view(torch.uint8).view(-1, page, K, d)[p == 0] = 0
+    ctx = context(H, K, d, dtype, epsp.F32, 700, page)
+    q = randq(2, H, d, dtype, 3)
+    ref, tol = decode64(c, q)
+    # scores carry log2 of V's scale, 64 and their own few at most: half a step of [64, 128) is 2^-18, times ln 2, in
+    # numerator and denominator: under 2^-17 of the sum of magnitudes, 16 times what the tolerance has of them at least
+    assert bool(((run(ctx, c, q).double() - ref).abs() <= 17 * tol).all())
+    ctx.check(ctx.sync_status())
+
+
+def test_long_caches_of_zeros():
+    """40,000 rows of zeros, all one block, before a page that is not: the sum of the weights stays finite."""
+    page, d, n_seq, n = 32, 64, 160, 40000
+    each = n // page
+    table = torch.zeros(n_seq, each, dtype=torch.int32, device="cuda")
+    table[:, -1] = torch.arange(1, n_seq + 1, device="cuda")
+    k = torch.zeros((n_seq + 1) * page, 1, d, dtype=torch.float8_e4m3fn, device="cuda")
+    v = torch.zeros_like(k)
+    scale = torch.full((n_seq + 1, 1), 2.0 ** -100, device="cuda")
+    g = torch.Generator().manual_seed(1)
+    v[page:] = torch.randn(n_seq * page, 1, d, generator=g).cuda().to(v.dtype)
+    v_scale = scale.clone()
+    v_scale[1:] = 0.5
+    ctx = context(1, 1, d, epsp.F16, epsp.F32, n, page)
+    batch = epsp.KvBatch(torch.full((n_seq,), n, dtype=torch.int32, device="cuda"), n, table, page, k.shape[0], 0)
+    out = torch.full((n_seq, 1, d), float("nan"), device="cuda")
+    ctx.check(ctx.decode8_layer(0, batch, randq(n_seq, 1, d, epsp.F16), epsp.Kv8(k, v, scale, v_scale), out,
+                                workspace(ctx.decode8_bytes(n_seq, n))))
+    ctx.check(ctx.sync_status())
+    x = v[page:].view(n_seq, page, d).double() * 0.5
+    # equal weights, exact; the sums of units over units in f32 (half a step each, numerator and denominator), a weight
+    # that is two f16 (2^-22), the exponent's error (2^-17 as above)
+    tol = x.abs().sum(1) / n * (2.0 ** -16 + 2 * n / 32 * 2.0 ** -24)
+    assert bool(((out[:, 0].double() - x.sum(1) / n).abs() <= tol).all())
+
+
 def test_not_finite_queries_and_codes_stay_with_their_heads():
     H, K, d, page = 8, 2, 128, 32
     for dtype in (epsp.BF16, epsp.F32):
