@@ -22,6 +22,8 @@ const char* wrong_pages(const ep_sp_config& c, const ep_sp_pages* p) {
     if (p->block_rows < 1 || p->block_rows % c.page_size) return "block_rows must be a multiple of the page size";
     if (p->table_stride < 1 || (int64_t)p->table_stride * p->block_rows > kMaxRows)
         return "table_stride must be at least 1, and a table's rows fit 32 bits";
+    // (the blocks that all sequences take are summed in 32 bits)
+    if ((int64_t)p->n_seq * p->table_stride > INT_MAX) return "the tables have more than 2^31 - 1 entries";
     if (p->pool_blocks < 1 || p->pool_blocks > kMaxRows) return "pool_blocks must be at least 1";
     if (!p->kv_lens || !p->block_tables || !p->refs) return "null lengths, tables or counts";
     if (!aligned(p->kv_lens, 4) || !aligned(p->block_tables, 4) || !aligned(p->refs, 4))

@@ -624,7 +624,7 @@ int32_t ep_sp_decode8_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch*
  * reported and not followed. */
 typedef struct ep_sp_pages {
     int32_t n_seq;
-    int32_t table_stride;
+    int32_t table_stride;  /* n_seq * table_stride < 2^31 */
     int32_t block_rows;    /* a multiple of the page size */
     int32_t pool_blocks;
     int32_t* kv_lens;      /* DEVICE [n_seq] */

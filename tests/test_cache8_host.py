@@ -109,7 +109,8 @@ def pages(**kw):
 BAD_PAGES = [dict(n_seq=0), dict(n_seq=65536), dict(table_stride=0), dict(block_rows=0), dict(block_rows=48),
              dict(block_rows=-32), dict(pool_blocks=0), dict(pool_blocks=2 ** 31 - 1), dict(kv_lens=None),
              dict(block_tables=None), dict(refs=None), dict(kv_lens=PTR + 2), dict(block_tables=PTR + 1),
-             dict(refs=PTR + 3), dict(table_stride=2 ** 27)]
+             dict(refs=PTR + 3), dict(table_stride=2 ** 27),
+             dict(n_seq=65535, table_stride=32769)]  # the blocks wanted would not fit 32 bits
 
 
 def calls(c, p, **kw):
