@@ -85,21 +85,21 @@ __device__ __forceinline__ void from8(uint32_t w, float (&x)[4]) {
 __device__ __forceinline__ float over(float x, float s, float inv) { return inv != 0.f ? x * inv : x / s; }
 
 // The bytes of rows [0, rows) of one head at `p` follow their page's scale from
-// `was` to `s`: thread `first` of `step` threads.  Eight 16-byte pieces a thread
-// are on their way at a time (a step of 64 sequences in which every page grows
-// takes 88 us; by 4 bytes, one row after the other, 264).
-template <bool I8>
+// `was` to `s`: thread `first` of `step` threads, A 16-byte pieces of each on
+// their way at a time.  (A warp wants eight: a step of 64 sequences in which every
+// page grows takes 88 us; by 4 bytes, one row after the other, 264.)
+template <bool I8, int A>
 __device__ __forceinline__ void rescale8(uint8_t* p, int64_t stride, int rows, int d, float was, float s, int first, int step) {
     const float f = was / s;
     const int lg = __ffs(d / 16) - 1, n = rows << lg;
     auto at = [&](int i) { return reinterpret_cast<uint4*>(p + (int64_t)(i >> lg) * stride + (i & ((1 << lg) - 1)) * 16); };
-    for (int i0 = first; i0 < n; i0 += 8 * step) {
-        uint4 w[8];
+    for (int i0 = first; i0 < n; i0 += A * step) {
+        uint4 w[A];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < A; ++j)
             if (i0 + j * step < n) w[j] = *at(i0 + j * step);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < A; ++j) {
             if (i0 + j * step >= n) break;
             uint32_t* q = reinterpret_cast<uint32_t*>(&w[j]);
 #pragma unroll

@@ -239,7 +239,7 @@ __device__ __forceinline__ void append_row(const DecodeArgs& a, const Cache8& c,
         float sc = scale8<I8>(m);
         if (was[v] >= sc) sc = was[v];
         else {
-            if (lo > 0) rescale8<I8>(dst, (int64_t)Hkv * D, lo, D, was[v], sc, lane, 32);
+            if (lo > 0) rescale8<I8, 8>(dst, (int64_t)Hkv * D, lo, D, was[v], sc, lane, 32);
             if (lane == 0) (v ? c.v_scale : c.k_scale)[(int64_t)(row / c.page_size) * Hkv + h] = sc;
         }
         const float inv = exact_inverse(sc);

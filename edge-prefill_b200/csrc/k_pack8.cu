@@ -120,9 +120,11 @@ __device__ __forceinline__ uint32_t quantised(const uint32_t* w, float inv) {
     }
 }
 
-// C: 16-byte chunks of a page and head per thread, of T threads.
+// C: 16-byte chunks of a page and head per thread, of T threads.  As many threads an
+// SM as leave each the registers it needs: with 1024 of C = 8 some are spilled (64 K
+// rows 81.6 us, of 768 80.1; a wider rescaling, eight pieces ahead, 154).
 template <int ET, bool I8, int C, int T>
-__global__ void __launch_bounds__(T, (C <= 2 ? 1536 : C <= 4 ? 1280 : 1024) / T) k9_pack(const PackArgs a) {
+__global__ void __launch_bounds__(T, (C == 1 ? 1536 : C == 2 ? 1280 : C == 4 || T > 256 ? 1024 : 768) / T) k9_pack(const PackArgs a) {
     constexpr int kEs = ET == 0 ? 4 : 2, kPer = 16 / kEs;
     __shared__ uint32_t box[4][T / 32];
     __shared__ int2 span_s, place_s[2];
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(T, (C <= 2 ? 1536 : C <= 4 ? 1280 : 1024) / T)
         float sc = scale8<I8>(m);
         if (was >= sc) sc = was;
         else {
-            if (lo > 0) rescale8<I8>(dst, (int64_t)Hkv * d, lo, d, was, sc, threadIdx.x, blockDim.x);
+            if (lo > 0) rescale8<I8, 1>(dst, (int64_t)Hkv * d, lo, d, was, sc, threadIdx.x, blockDim.x);
             if (threadIdx.x == 0) *scale = sc;
         }
         const float inv = exact_inverse(sc);
@@ -220,13 +222,20 @@ __global__ void __launch_bounds__(T, (C <= 2 ? 1536 : C <= 4 ? 1280 : 1024) / T)
         if (plain) {
             store([&](const uint32_t* w) { return quantised<ET, I8>(w, inv); });
         } else {
-            store([&](const uint32_t* w) {
+            // (rare) from the source again, four values at a time
+#pragma unroll 1
+            for (int i = threadIdx.x; i < (hi - lo) * d / 4; i += T) {
+                const int64_t el = (int64_t)(lo + i * 4 / d) * stride + i * 4 % d;
+                uint32_t w[4];
+                const uint2* p = reinterpret_cast<const uint2*>(src + el * kEs);
+                *reinterpret_cast<uint2*>(w) = p[0];
+                if constexpr (kEs == 4) *reinterpret_cast<uint2*>(w + 2) = p[1];
                 float x[4];
                 values4<ET>(w, x);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) x[k] = tame8<I8>(over(x[k], sc, inv));
-                return to8<I8>(x[0], x[1], x[2], x[3]);
-            });
+                *reinterpret_cast<uint32_t*>(dst + el) = to8<I8>(x[0], x[1], x[2], x[3]);
+            }
         }
     }
 }
@@ -336,7 +345,7 @@ __global__ void __launch_bounds__(128) k9_append(const AppendArgs a) {
     float sc = scale8<I8>(m);
     if (was >= sc) sc = was;
     else {
-        if (lo > 0) rescale8<I8>(dst, (int64_t)Hkv * d, lo, d, was, sc, threadIdx.x, blockDim.x);
+        if (lo > 0) rescale8<I8, 8>(dst, (int64_t)Hkv * d, lo, d, was, sc, threadIdx.x, blockDim.x);
         if (t == 0) *scale = sc;
     }
     if (t < d) dst[(int64_t)lo * Hkv * d + t] = (uint8_t)to8<I8>(tame8<I8>(over(x, sc, exact_inverse(sc))), 0.f, 0.f, 0.f);
