@@ -3,8 +3,11 @@
 //
 //   x_j = q . kq_j ks * scale,  out = sum_j exp(x_j - m) vq_j vs / sum_j exp(x_j - m)
 //
-// Half the bytes of K6, and they bound it; the split of the rows over the CTAs,
-// the ring and the joins are K6's (decode_common.cuh).  A new token's row is
+// Half the bytes of K6; the split of the rows over the CTAs, the ring and the
+// joins are K6's (decode_common.cuh).  64 K rows (8 heads of 128) take 32 us, 4.1
+// TB/s, 64 sequences of up to 4096 rows 60, 4.5 TB/s; without the arithmetic 26 and
+// 52: the bytes bound it first, then the attending warps, two a scheduler, whose
+// products and conversions wait for one another (issue slots 34 to 45 % busy).  A new token's row is
 // quantised into the cache by the CTA that attends it: the last page of a run is
 // never split, and its copies wait for the row (as a kernel before, k9_append,
 // it took 3 to 4 us more; calls of several passes still have that).

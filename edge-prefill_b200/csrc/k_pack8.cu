@@ -12,8 +12,8 @@
 // follow one another, so the whole rows of the source are read at about one
 // time.  A page that holds rows before `first` keeps its scale, or has it grown
 // and those rows' bytes follow, by the same CTA.  64 K rows (8 heads of 128,
-// bf16 to e4m3) 80 us, 5.0 TB/s: its instructions (12 a value: issue slots 62 %
-// busy) and the waits at a tile's ends bound it, not memory.
+// bf16 to e4m3) 80 us, 5.0 TB/s: the waits within a tile, for its rows and for its
+// maximum, bound it (issue slots 52 % busy, 24 warps an SM).
 // unpack: tiles of 32 rows, which lie together in both caches, 16 bytes a
 // thread.  32 K rows (4 heads of 128, to bf16) 24 us, 4.2 TB/s with the launch.
 #include <cuda_bf16.h>
@@ -377,7 +377,7 @@ template <int ET, bool I8>
 cudaError_t pack_t(const PackArgs& a, cudaStream_t s) {
     const int64_t pages = (a.src.max_kv_len + (int64_t)a.c.page_size - 1) / a.c.page_size;
     const dim3 grid(grid_x(pages * a.n_head_kv * 2, a.src.n_seq), a.src.n_seq);
-    // (8 chunks a thread: 80 us for 64 K rows in pages of 128; 4, of twice the threads, 89; 16, of half of them, 102)
+    // (8 chunks a thread: 80 us for 64 K rows in pages of 128; 4, of twice the threads, 94; 16, of half of them, 93)
     const int chunks = a.c.page_size * a.head_dim * (ET == 0 ? 4 : 2) / (16 * kThreads);
     switch (chunks) {
         case 1: return go(k9_pack<ET, I8, 1, 256>, grid, 256, s, a);
