@@ -217,13 +217,14 @@ HEADS = [(14, 2, 64), (32, 8, 128), (28, 4, 128), (8, 8, 64), (9, 1, 128), (16, 
 @pytest.mark.parametrize("q8", [E, Q], ids=name)
 @pytest.mark.parametrize("dtype", [epsp.BF16, epsp.F16, epsp.F32], ids=name)
 @pytest.mark.parametrize("heads", HEADS, ids=str)
-def test_decode8_heads(heads, dtype, q8):
+@pytest.mark.parametrize("capacity", [1111, 13000])  # joined in clusters, and split over the device
+def test_decode8_heads(capacity, heads, dtype, q8):
     """Every number of query heads per KV head that takes another path, ragged lengths, a row appended."""
     H, K, d = heads
     page = 64
     lens = [0, 1, 33, 64, 500, 1111]
-    c = Cache8(lens, K, d, q8, page, page, 1)
-    ctx = context(H, K, d, dtype, epsp.F32, max(lens), page)
+    c = Cache8(lens, K, d, q8, page, page, 1, capacity=capacity)
+    ctx = context(H, K, d, dtype, epsp.F32, capacity, page)
     q, kn, vn = randq(6, H, d, dtype), randq(6, K, d, dtype, 6, 3.0), randq(6, K, d, dtype, 7)
     want = c.state()
     for i, n in enumerate(lens):
