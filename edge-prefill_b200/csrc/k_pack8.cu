@@ -12,7 +12,7 @@
 // follow one another, so the whole rows of the source are read at about one
 // time.  A page that holds rows before `first` keeps its scale, or has it grown
 // and those rows' bytes follow, by the same CTA.  64 K rows (8 heads of 128,
-// bf16 to e4m3) 80 us, 5.0 TB/s: the waits within a tile, for its rows and for its
+// bf16 to e4m3) 79 us, 5.1 TB/s: the waits within a tile, for its rows and for its
 // maximum, bound it (issue slots 52 % busy, 24 warps an SM).
 // unpack: tiles of 32 rows, which lie together in both caches, 16 bytes a
 // thread.  32 K rows (4 heads of 128, to bf16) 24 us, 4.2 TB/s with the launch.
@@ -30,7 +30,7 @@ namespace epsp {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kOver = 32;  // CTAs per SM that a grid has at most (64 K rows packed: 8 89 us, 16 81, 32 80, 64 85)
+constexpr int kOver = 16;  // CTAs per SM that a grid has at most (64 K rows packed: 8 79.3 us, 16 78.9, 32 79.6, 64 87)
 
 // The 4 values of 8 bytes (16-bit types) or 16 bytes (f32).
 template <int ET>
