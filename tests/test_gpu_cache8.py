@@ -380,6 +380,25 @@ def test_pages_of_zeros_next_to_large_values(dtype):
     ctx.check(ctx.sync_status())
 
 
+@pytest.mark.parametrize("q8", [E, Q], ids=name)
+@pytest.mark.parametrize("dtype", [epsp.F16, epsp.F32], ids=name)
+def test_tiny_values(dtype, q8):
+    """V scales below 2^-64: what they are short of it goes into the weights when those are f16."""
+    H, K, d, page = 4, 2, 128, 32
+    lens = [700, 90]
+    c = Cache8(lens, K, d, q8, page, 0, 1)
+    p = torch.arange(c.vs.shape[0], device="cuda") % 3
+    c.vs[:] = torch.exp2(torch.tensor([-70.0, -65.0, -71.0], device="cuda")[p])[:, None]
+    ctx = context(H, K, d, dtype, epsp.F32, 700, page)
+    q = randq(2, H, d, dtype, 3)
+    ref, tol = decode64(c, q)
+    # 17: as above.  The weights' absolute part, 2^-39 of the largest where that is 2^14, is 2^-39 of the largest weight
+    # times 2^-64 here: in all at most rows * 2^-39 * 2^-64 * the largest byte
+    floor = torch.tensor(lens, device="cuda").double().view(2, 1, 1) * 2.0 ** -103 * 448
+    assert bool(((run(ctx, c, q).double() - ref).abs() <= 17 * tol + floor).all())
+    ctx.check(ctx.sync_status())
+
+
 def test_long_caches_of_zeros():
     """40,000 rows of zeros, all one block, before a page that is not: the sum of the weights stays finite."""
     page, d, n_seq, n = 32, 64, 160, 40000
