@@ -31,7 +31,7 @@
 // other scales add up in the accumulators as they are; the weights' sum takes P
 // over the scale.  The largest P is held between 2^14 and 2^15, and P is two
 // f16: an element keeps 22 bits of itself and an absolute 2^-39 of the largest
-// (half of f16's smallest step); one f16 where the output is bf16.
+// (half of f16's smallest step).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -256,10 +256,9 @@ __device__ __forceinline__ void append_row(const DecodeArgs& a, const Cache8& c,
     }
 }
 
-// LO: q has remainders (f32).  P2: P has remainders (for outputs of 11 bits and
-// more; bf16's half step is eight times that of the f16 that P then is).
-// JOIN: the calls that join_cluster finishes.
-template <int D, bool I8, bool LO, bool P2, bool JOIN>
+// LO: q has remainders (f32).  (P always has: where V's terms cancel, the 11 bits of
+// one f16 show in a bf16 output too.)  JOIN: the calls that join_cluster finishes.
+template <int D, bool I8, bool LO, bool JOIN>
 __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     k10_decode8(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
                 const Cache8 c8, const DecodeSplit sp, const Layout8<D> ly) {
@@ -723,7 +722,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                 for (int j = 0; j < D / 16; ++j) o[j][0] *= alpha0, o[j][1] *= alpha1, o[j][2] *= alpha0, o[j][3] *= alpha1;
             }
             const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-            uint32_t ph[2][2], pl[P2 ? 2 : 1][2];  // keys 16 b + 8 half + 2 tq + {0, 1} of head hd
+            uint32_t ph[2][2], pl[2][2];  // keys 16 b + 8 half + 2 tq + {0, 1} of head hd
             float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -732,7 +731,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                     float x = ex2(s4[b][2 * t] - m0), y = ex2(s4[b][2 * t + 1] - m1);
                     sum0 += x, sum1 += y;
                     ph[b][t] = turned(split2<false>(x, y));
-                    if constexpr (P2) pl[b][t] = turned(split2<false>(x, y));
+                    pl[b][t] = turned(split2<false>(x, y));
                 }
             if (down) {
                 const uint32_t f = down & 0x7fff7fffu;
@@ -741,7 +740,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         ph[b][t] = times2(ph[b][t], f);
-                        if constexpr (P2) pl[b][t] = times2(pl[b][t], f);
+                        pl[b][t] = times2(pl[b][t], f);
                     }
             }
             const float rv = ex2(-lv);
@@ -762,11 +761,9 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], ph[b][0], ph[b][1]);
-                    if constexpr (P2) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], pl[b][0], pl[b][1]);
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], pl[b][0], pl[b][1]);
                 }
             }
             __syncwarp();
@@ -881,7 +878,7 @@ size_t split8_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_he
     return at;
 }
 
-template <int D, bool I8, bool LO, bool P2, bool JOIN>
+template <int D, bool I8, bool LO, bool JOIN>
 cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, cudaStream_t s) {
     CUtensorMap mk, mv;
     if (!cache8_map(&mk, c.k, D, a.n_head_kv, a.kv.rows) || !cache8_map(&mv, c.v, D, a.n_head_kv, a.kv.rows))
@@ -894,7 +891,7 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
     static std::atomic<unsigned> set_mask{0};
     if (dev >= 32 || !(set_mask.load(std::memory_order_acquire) & (1u << dev))) {
         const cudaError_t e =
-            cudaFuncSetAttribute(k10_decode8<D, I8, LO, P2, JOIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            cudaFuncSetAttribute(k10_decode8<D, I8, LO, JOIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         if (dev < 32) set_mask.fetch_or(1u << dev, std::memory_order_release);
     }
@@ -921,7 +918,7 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
     cfg.blockDim = dim3(kThreads8 + 32 * kFetchers);
     cfg.dynamicSmemBytes = ly.bytes() + 1024;
     cfg.numAttrs = sp.cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k10_decode8<D, I8, LO, P2, JOIN>, mk, mv, a, c, sp, ly);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k10_decode8<D, I8, LO, JOIN>, mk, mv, a, c, sp, ly);
     if (e != cudaSuccess || sp.direct) return e;
     const int heads = std::min(a.n_head / a.n_head_kv, sp.pass_heads);
     const int64_t grid = (int64_t)sp.joins * heads;
@@ -935,12 +932,8 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
 template <int D, bool I8>
 cudaError_t launch8_t(const DecodeArgs& a, const Cache8& c, const DecodeSplit& sp, cudaStream_t s) {
     const bool join = sp.cluster > 1;
-    if (a.dtype == 0)
-        return join ? launch8_join<D, I8, true, true, true>(a, c, sp, s) : launch8_join<D, I8, true, true, false>(a, c, sp, s);
-    if (a.out_dtype == 2)
-        return join ? launch8_join<D, I8, false, false, true>(a, c, sp, s)
-                    : launch8_join<D, I8, false, false, false>(a, c, sp, s);
-    return join ? launch8_join<D, I8, false, true, true>(a, c, sp, s) : launch8_join<D, I8, false, true, false>(a, c, sp, s);
+    if (a.dtype == 0) return join ? launch8_join<D, I8, true, true>(a, c, sp, s) : launch8_join<D, I8, true, false>(a, c, sp, s);
+    return join ? launch8_join<D, I8, false, true>(a, c, sp, s) : launch8_join<D, I8, false, false>(a, c, sp, s);
 }
 
 }  // namespace

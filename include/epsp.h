@@ -599,9 +599,8 @@ int32_t ep_sp_unpack_kv(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* src
  * then share the page of that row).  The products are exact, their sums, the
  * scores and the softmax statistics f32; an f32 q is taken to 22 bits of its
  * head's largest element.  A weight times its page's V scale (one below 2^-64
- * counts as that) is held to 2^-39 of the head's largest, with bf16 outputs of a
- * 16-bit model to 11 bits as well; V scales of one sequence are to lie within
- * 2^116 of one another.  A query head with an infinity or a NaN has a row of
+ * counts as that) is held to 22 bits and to 2^-39 of the head's largest; V scales
+ * of one sequence are to lie within 2^116 of one another.  A query head with an infinity or a NaN has a row of
  * NaN, a NaN code of e4m3 makes NaN of what it reaches.  A sequence's result
  * depends on the batch alone, not on timing. */
 int32_t ep_sp_decode8_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_len, size_t* bytes);
