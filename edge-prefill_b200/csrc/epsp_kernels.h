@@ -33,10 +33,19 @@ enum DeviceError : int32_t {
     kDevWaitWeights = 0x602,   // a prompt-weight tile did not arrive (or leave) in time
 };
 
-// The device error word is err[0] of a 4-word record: the kernel whose
+// The device error word is err[0] of a record of kErrWords: the kernel whose
 // atomicCAS on err[0] wins also writes err[1] = where (role * 16 + barrier),
-// err[2] = its block index, err[3] = its KV tile, for ep_sp_sync_status.
+// err[2] = its block index, err[3] = its KV tile, for ep_sp_sync_status.  err[4]
+// is not 0 once a resize was refused (kDevNoBlocks), until that is reported.
+constexpr int kErrWords = 5, kErrRefused = 4;
 #if defined(__CUDACC__)
+// After a refused resize the tables do not hold the rows that the calls behind it
+// were to write: the row of a length that did not grow is a sequence's last one,
+// perhaps another's too, and entries past it are anybody's.  Those calls write
+// nothing through block tables.
+__device__ __forceinline__ bool resize_refused(const int32_t* err) {
+    return err[kErrRefused] != 0;
+}
 __device__ __forceinline__ void report_error(int32_t* err, int32_t code, int32_t where, int32_t tile) {
     if (atomicCAS(err, 0, code) == 0) {
         err[1] = where;
@@ -267,6 +276,11 @@ __device__ __forceinline__ int32_t batch_row(const BatchKv& b, int32_t s, int32_
         return -1;
     }
     return (int32_t)row;
+}
+
+// Whether rows of this batch must not be written.
+__device__ __forceinline__ bool held_back(const BatchKv& b, const int32_t* err) {
+    return b.block_rows > 0 && resize_refused(err);
 }
 #endif
 

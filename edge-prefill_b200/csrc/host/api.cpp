@@ -77,10 +77,10 @@ int32_t ensure_device(ep_sp_ctx* c) {
     if ((e = cudaMalloc(&c->psum, psum_bytes)) != cudaSuccess) return cuda_fail(c, e, "cudaMalloc page sums");
     if ((e = cudaMalloc(&c->d_budget, sizeof(int32_t) * nl * Hkv)) != cudaSuccess) return cuda_fail(c, e, "cudaMalloc");
     if ((e = cudaMalloc(&c->d_dense, sizeof(int32_t) * Hkv)) != cudaSuccess) return cuda_fail(c, e, "cudaMalloc");
-    if ((e = cudaMalloc(&c->d_err, 4 * sizeof(int32_t))) != cudaSuccess) return cuda_fail(c, e, "cudaMalloc");
+    if ((e = cudaMalloc(&c->d_err, epsp::kErrWords * sizeof(int32_t))) != cudaSuccess) return cuda_fail(c, e, "cudaMalloc");
     std::vector<int32_t> dense(Hkv, -1);
     cudaMemcpy(c->d_dense, dense.data(), sizeof(int32_t) * Hkv, cudaMemcpyHostToDevice);
-    cudaMemset(c->d_err, 0, 4 * sizeof(int32_t));
+    cudaMemset(c->d_err, 0, epsp::kErrWords * sizeof(int32_t));
     if ((e = cudaDeviceSynchronize()) != cudaSuccess) return cuda_fail(c, e, "device init");
     c->pooled.assign((size_t)nl * Hkv, 0);
     c->v_pooled.assign((size_t)nl * Hkv, 0);
@@ -420,28 +420,36 @@ int32_t ep_sp_sync_status(ep_sp_ctx* ctx, void* stream) {
         return fail(ctx, kPrefill, buf);
     }
     if (!ctx->reserved) return kOk;
-    int32_t rec[4] = {0, 0, 0, 0};  // code, where, block, tile
+    int32_t rec[epsp::kErrWords] = {};  // code, where, block, tile, refused
     e = cudaMemcpy(rec, ctx->d_err, sizeof rec, cudaMemcpyDeviceToHost);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "error word");
-    const int32_t err = rec[0];
+    const bool refused = rec[epsp::kErrRefused] != 0;
+    const int32_t err = rec[0] == 0 && refused ? epsp::kDevNoBlocks : rec[0];
     if (err != 0) {
-        cudaMemset(ctx->d_err, 0, sizeof rec);
+        // (cleared before the caller's next launch can read it, on whatever stream)
+        e = cudaMemsetAsync(ctx->d_err, 0, sizeof rec, s);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "error word");
+        // rows that calls did not write since may be in page sums and f16 shadows
+        if (refused)
+            for (int32_t l = 0; l < ctx->cfg.n_layer; ++l) forget_layer(ctx, l);
+        const char* held = refused ? "; calls since a refused resize wrote no rows through block tables" : "";
         if (err == epsp::kDevF16Range)
             return fail(ctx, kUnsupported,
                         "an f32 input lies outside the f16 range of the tensor-core mode (ep_sp_set_f32_attention 0 "
-                        "attends it in f32)");
+                        "attends it in f32)" + std::string(held));
         if (err == epsp::kDevNotFinite8)
             return fail(ctx, kUnsupported,
                         "a row that went into an 8-bit cache held an infinity (kept as the largest magnitude) or a NaN "
-                        "(kept as 0)");
+                        "(kept as 0)" + std::string(held));
         if (err == epsp::kDevNoBlocks)
             return fail(ctx, kOom, "a resize needed " + std::to_string(rec[3]) +
-                                       " more free blocks than the pool had; it changed nothing");
-        char buf[160];
+                                       " more free blocks than the pool had; it changed nothing" + held);
+        char buf[240];
         std::snprintf(buf, sizeof buf,
                       "device error word 0x%x (bounded wait expired, bad selection, block table, length or parent); where 0x%x, "
-                      "block %d, tile %d",
-                      err, rec[1], rec[2], rec[3]);
+                      "block %d, tile %d%s",
+                      err, rec[1], rec[2], rec[3], held);
         return fail(ctx, kPrefill, buf);
     }
     return kOk;

@@ -9,6 +9,7 @@
 // cparams (patch :567-584, :504-517).
 #pragma once
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 #include <vector>
@@ -181,5 +182,14 @@ int32_t ctx_ensure_device(ep_sp_ctx* ctx);
 // the launch, give after it; nothing is recorded on a capturing stream).
 void* ctx_profile_begin(ep_sp_ctx* ctx, int kind, void* stream);
 void ctx_profile_end(ep_sp_ctx* ctx, int kind, void* start, void* stream);
+// Rows of the layer have moved or been written past the context's knowledge:
+// page sums, V sums and f16 shadows start over at its next prefill call.
+inline void forget_layer(ep_sp_ctx* c, int32_t layer) {
+    const size_t at = (size_t)layer * c->cfg.n_head_kv;
+    std::fill_n(c->pooled.begin() + at, c->cfg.n_head_kv, 0);
+    std::fill_n(c->v_pooled.begin() + at, c->cfg.n_head_kv, 0);
+    c->shadowed[layer] = 0;
+    c->sel_valid = false;
+}
 
 }  // namespace edge_prefill_b200

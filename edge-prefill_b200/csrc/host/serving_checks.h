@@ -126,16 +126,6 @@ inline int32_t check_workspace(ep_sp_ctx* c, const void* ws, size_t have, size_t
 
 inline int32_t elem_bytes(int32_t dtype) { return dtype == EP_SP_F32 ? 4 : 2; }
 
-// Rows of the layer have moved or been written past the context's knowledge:
-// page sums, V sums and f16 shadows start over at its next prefill call.
-inline void forget_layer(ep_sp_ctx* c, int32_t layer) {
-    const size_t at = (size_t)layer * c->cfg.n_head_kv;
-    std::fill_n(c->pooled.begin() + at, c->cfg.n_head_kv, 0);
-    std::fill_n(c->v_pooled.begin() + at, c->cfg.n_head_kv, 0);
-    c->shadowed[layer] = 0;
-    c->sel_valid = false;
-}
-
 // No exception crosses the ABI.
 template <class F>
 int32_t guarded(F&& f) noexcept {

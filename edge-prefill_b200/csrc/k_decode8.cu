@@ -216,7 +216,7 @@ template <int D, bool I8>
 __device__ __forceinline__ void append_row(const DecodeArgs& a, const Cache8& c, int s, int h, int n, int lane) {
     constexpr int E = D / 32;  // elements of a lane
     const int Hkv = a.n_head_kv, r0 = (n - 1) / c.page_size * c.page_size, lo = n - 1 - r0;
-    const int row = batch_row(a.kv, s, r0, a.err);
+    const int row = held_back(a.kv, a.err) ? -1 : batch_row(a.kv, s, r0, a.err);
     float x[2][E], was[2];
 #pragma unroll
     for (int v = 0; v < 2; ++v) {

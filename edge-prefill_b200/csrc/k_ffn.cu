@@ -216,6 +216,7 @@ unsigned stream_grid(cudaStream_t) {
 // error and skips the row.
 __global__ void k_copy_rows_paged(const uint4* __restrict__ src, uint4* __restrict__ dst, int32_t row_begin,
                                   int32_t n_rows, int32_t cpr, KvPaging pg, int32_t* err) {
+    if (err && resize_refused(err)) return;
     const int64_t total = (int64_t)n_rows * cpr;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         const int32_t r = (int32_t)(i / cpr), c = (int32_t)(i % cpr);

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kPoolThreads) k1_pool_pages(PoolArgs a) {
                                           : *reinterpret_cast<const uint4*>(base + (prow0 + i) * row_bytes + col);
             }
             char* out = static_cast<char*>(a.k_store);
-            if (!bad) {
+            if (!bad && !(a.paging.block_rows > 0 && a.err && resize_refused(a.err))) {
 #pragma unroll
                 for (int i = 0; i < kPageSumGroupRows; ++i)
                     if (row0 + i >= a.new_begin) *reinterpret_cast<uint4*>(out + (prow0 + i) * row_bytes + col) = raw[i];

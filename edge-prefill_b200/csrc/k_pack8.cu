@@ -53,14 +53,16 @@ __device__ __forceinline__ void values4(const uint32_t* w, float (&x)[4]) {
     }
 }
 
-// Rows [first, len) of a sequence; an empty range where `first` is none.
+// Rows [first, len) of a sequence; an empty range where `first` is none, or no
+// rows may be written.
 __device__ __forceinline__ int2 span_of(const PackArgs& a, int s) {
+    const bool held = held_back(a.dst, a.err);
     const int n = batch_len(a.src, s, a.err), f = a.first ? a.first[s] : 0;
     if (f < 0 || f > n) {
         report_error(a.err, kDevBadLength, 0x92, s);
         return make_int2(0, 0);
     }
-    return make_int2(f, n);
+    return held ? make_int2(0, 0) : make_int2(f, n);
 }
 
 // Largest of the CTA's values.  (Two calls in a row want two boxes: a warp may
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(128) k9_append(const AppendArgs a) {
     const int n = n_s;
     if (n == 0) return;
     const int r0 = (n - 1) / P * P, lo = n - 1 - r0;
-    const int row = batch_row(a.kv, s, r0, a.err);
+    const int row = held_back(a.kv, a.err) ? -1 : batch_row(a.kv, s, r0, a.err);
     bool odd = false;
     uint32_t m = magnitude(x, odd);
     float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + (int64_t)(max(row, 0) / P) * Hkv + h;

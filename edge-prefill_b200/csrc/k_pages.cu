@@ -366,6 +366,7 @@ __global__ void __launch_bounds__(kPlan, 1) k11_resize(const PagesArgs a, const 
     if (all.x > all.y) {  // too few: nothing changes
         if (me == 0 && lane == 0) {
             *w.n_pairs = 0;
+            a.err[kErrRefused] = 1;
             report_error(a.err, kDevNoBlocks, 0xc4, all.x - all.y);
         }
         return;

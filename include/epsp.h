@@ -660,9 +660,18 @@ int32_t ep_sp_fork_seqs(ep_sp_ctx* ctx, const ep_sp_pages* pages, const int32_t*
  * sequences hold too, then those for the rows to come.  Where every holder of
  * such a block grows in this call, the last of them keeps it.  After the call no
  * other sequence holds a block that has rows [old length, new length) of this
- * one; what those rows hold is undefined.  With fewer free blocks than needed
- * nothing changes and ep_sp_sync_status reports rc 10.  Only lengths are changed
- * here: call it before the step that writes the rows.  pools: HOST [n_pools],
+ * one; what those rows hold is undefined.  Only lengths are changed here: call it
+ * before the step that writes the rows.
+ * With fewer free blocks than needed nothing changes and ep_sp_sync_status
+ * reports rc 10.  The steps that follow on the device do not know: row
+ * kv_lens[s] - 1 is then a row from before, which others may hold, and table
+ * entries past the lengths are anybody's.  So from there until
+ * ep_sp_sync_status has reported it no call of the context writes a row through
+ * block tables (ep_sp_decode_layer and ep_sp_decode8_layer with new rows,
+ * ep_sp_pack_kv, ep_sp_unpack_kv, ep_sp_append_kv, ep_sp_evict_layer into other
+ * rows, which leaves new_lens and acc_dst too): the caches stay as they are, what these
+ * calls answer means nothing, and the steps since have to be made again.
+ * ep_sp_sync_status then forgets all layers' page sums and f16 shadows.  pools: HOST [n_pools],
  * n_pools in [1, 4096]. */
 int32_t ep_sp_resize_bytes(const ep_sp_ctx* ctx, const ep_sp_pages* pages, size_t* bytes);
 int32_t ep_sp_resize_seqs(ep_sp_ctx* ctx, const ep_sp_pages* pages, const int32_t* new_lens, const ep_sp_pool* pools,
@@ -684,7 +693,8 @@ int32_t ep_sp_compact_pool(ep_sp_ctx* ctx, const ep_sp_pages* pages, const ep_sp
  * rc 9 (Unsupported) when an f32 input left the f16 range of the tensor-core
  * mode or a row with an infinity or a NaN went into an 8-bit cache, rc 10 when a
  * resize found too few free blocks (the word is then cleared; the first of
- * several failures is the one reported), 12 on a CUDA error.
+ * several failures is the one reported, ep_sp_last_error says whether a resize
+ * was refused, too), 12 on a CUDA error.
  * It also reads and clears the error word of ep_sp_select_pages_noalloc on
  * the context's device.  The compute calls themselves never synchronise. */
 int32_t ep_sp_sync_status(ep_sp_ctx* ctx, void* stream);
