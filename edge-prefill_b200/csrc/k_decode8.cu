@@ -27,11 +27,13 @@
 // byte permutation pairs two rows of V.  q is scaled to a
 // largest magnitude of 2^14 to 2^15 by a power of two, so f16 takes its 16-bit
 // types as they are; an f32 q is two f16 (a second product).  P is the weight
-// times V's scale, against the running maximum of just that, so that units of
-// other scales add up in the accumulators as they are; the weights' sum takes P
-// over the scale.  The largest P is held between 2^14 and 2^15, and P is two
-// f16: an element keeps 22 bits of itself and an absolute 2^-39 of the largest
-// (half of f16's smallest step).
+// times V's scale, so that units of any scales add up in the accumulators as they
+// are.  Two running maxima, in whole powers of two: that of the scores, for the
+// weights and their sum, and that of score and scale, for P; a unit's weights
+// become P by one factor.  (Of the products alone, the sum would lose the weights
+// of pages with small scales and the range of large ones.)  The largest P is held
+// between 2^14 and 2^15, and P is two f16: an element keeps 22 bits of itself and
+// an absolute 2^-39 of the largest (half of f16's smallest step).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -55,13 +57,11 @@ namespace {
 constexpr int kWarps8 = 8;
 constexpr int kThreads8 = kWarps8 * 32;  // that attend
 constexpr int kFetchers = 4;             // warps that fetch
-constexpr float kUp8 = 14.f;      // P is 2^14 times what it is against the running maximum,
-constexpr float kSlack8 = 1.f;    // which follows when it is twice that behind: 2^15 at most
-// log2 of V's scale in P is this at least (a page of zeros has a scale of 2^-100):
-// a weight is in the sum of weights while P is above f32's smallest, so that the
-// scales of a run may differ by 2^116, and the sum stays below 2^110.  What is
-// missing goes into P when it is f16 already.
-constexpr float kLeastV8 = -64.f;
+// Either maximum follows once something would pass 2^15: that of the weights to
+// where the largest is 1 to 2, P's to where it is 2^14 to 2^15.
+constexpr float kUp8 = 14.f;
+constexpr float kMost8 = 15.f;
+constexpr float kNone8 = -3.402823466e38f;  // either of no rows: a number, so that -inf lies below it
 constexpr int kPass8 = 64;        // query heads of a pass, at most
 // Units for each CTA of a cluster up to which a run is joined in shared memory
 // instead of being split over the device: one launch. One sequence of 6000, 12,000,
@@ -81,7 +81,8 @@ struct Layout8 {
     __host__ __device__ int off_q() const { return stages * kStage; }
     __host__ __device__ int off_o() const { return off_q() + 2 * q_bytes; }        // [kWarps8][8][D] the warps' sums
     __host__ __device__ int off_ml() const { return off_o() + kWarps8 * 8 * D * 4; }  // [kWarps8][8] (maximum, sum)
-    __host__ __device__ int off_scale() const { return off_ml() + kWarps8 * 8 * 8; }  // [stages] (ks, vs)
+    __host__ __device__ int off_mp() const { return off_ml() + kWarps8 * 8 * 8; }     // [kWarps8][8] P's maximum
+    __host__ __device__ int off_scale() const { return off_mp() + kWarps8 * 8 * 4; }  // [stages] (ks, vs)
     __host__ __device__ int off_bar() const { return off_scale() + kMost * 8; }
     __host__ __device__ int off_lens() const { return off_bar() + (2 * kMost + 7) * 8; }
     __host__ __device__ int bytes() const { return off_lens() + kLensOnChip * 4; }
@@ -143,10 +144,9 @@ __device__ __forceinline__ void mma8_first(float (&c)[4], uint32_t a0, uint32_t 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// Two f16 times two.
-__device__ __forceinline__ uint32_t times2(uint32_t x, uint32_t y) {
-    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
-    return *reinterpret_cast<const uint32_t*>(&r);
+// 2^t of a whole t in [-126, 127].
+__device__ __forceinline__ float pow2(float t) {
+    return __uint_as_float((__float_as_uint(t + 12582912.f) << 23) + 0x3f800000u);  // (the sum's low bits are t)
 }
 
 // Units of a block, and the place of a unit: dividing by a number that is known
@@ -457,6 +457,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     float* om = reinterpret_cast<float*>(smem + ly.off_o());
     float* om_w = om + warp * 8 * D;
     float2* ml = reinterpret_cast<float2*>(smem + ly.off_ml());
+    float* mps = reinterpret_cast<float*>(smem + ly.off_mp());
     // Place of 16 bytes in a warp's sums of one head: turned by the head, so that
     // lanes of one column block and four heads meet different banks.
     auto chunk = [&](int g, int c) { return c ^ (D == 128 ? g >> 1 & 3 : (g >> 2 & 1) << 2 | (g >> 1 & 1)); };
@@ -472,7 +473,9 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         for (int g = warp; g < pass_n; g += kWarps8) {
             const int gw = g >> 3, gh = g & 7;
             // lane r: stream r
-            const float2 v = lane < streams ? ml[(lane * groups + gw) * 8 + gh] : make_float2(-INFINITY, 0.f);
+            const int at = (lane * groups + gw) * 8 + gh;
+            const float2 v = lane < streams ? ml[at] : make_float2(-INFINITY, 0.f);
+            const float mp = lane < streams ? mps[at] : -INFINITY;
             const float* from = om + gw * 8 * D + gh * D + chunk(gh, lane * kC / 4) * 4 + lane * kC % 4;
             float t[kWarps8][kC];
 #pragma unroll
@@ -481,12 +484,13 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                 if constexpr (kC == 4) *reinterpret_cast<float4*>(t[r]) = *reinterpret_cast<const float4*>(x);
                 else *reinterpret_cast<float2*>(t[r]) = *reinterpret_cast<const float2*>(x);
             }
-            float mt = v.x;
+            // relative to the power of two that the largest sum is under: what goes on is never beyond V's largest
+            float mt = v.x + (float)((int)(__float_as_uint(v.y) >> 23) - 126);
 #pragma unroll
             for (int x = 1; x < 8; x <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
             mt = __shfl_sync(0xffffffffu, mt, 0);
-            const float ms = mt == -INFINITY ? 0.f : mt, f = ex2(v.x - ms);
-            float lt = v.y * f;
+            const float f = ex2(mp - mt);
+            float lt = v.y * ex2(v.x - mt);
 #pragma unroll
             for (int x = 1; x < 8; x <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, x);
             lt = __shfl_sync(0xffffffffu, lt, 0);
@@ -504,7 +508,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                 float* to = reinterpret_cast<float*>(smem) + g * D + lane * kC;
 #pragma unroll
                 for (int c = 0; c < kC; ++c) to[c] = acc[c];
-                if (lane == 0) *reinterpret_cast<float2*>(smem + kPass8 * D * 4 + g * 8) = make_float2(ms, lt);
+                if (lane == 0) *reinterpret_cast<float2*>(smem + kPass8 * D * 4 + g * 8) = make_float2(mt, lt);
             } else if (whole) {
                 const float inv = 1.f / lt;
                 const int64_t to = (head_row + g) * D + lane * kC;
@@ -518,7 +522,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                     *reinterpret_cast<float4*>(sp.part_o + to * D + lane * kC) = make_float4(acc[0], acc[1], acc[2], acc[3]);
                 else
                     *reinterpret_cast<float2*>(sp.part_o + to * D + lane * kC) = make_float2(acc[0], acc[1]);
-                if (lane == 0) sp.part_ml[to] = make_float2(ms, lt);
+                if (lane == 0) sp.part_ml[to] = make_float2(mt, lt);
             }
         }
         __syncwarp();
@@ -550,7 +554,8 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         float o[D / 16][4];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of heads 2 tq + {0, 1}
+        // of heads 2 tq + {0, 1}: log2 of what the weights (l: their sum) and P are relative to, and 2 to their difference
+        float m[2] = {kNone8, kNone8}, mp[2] = {kNone8, kNone8}, up[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
         if (ok && !tc::mbar_wait(&q_full[seg & 1], (seg >> 1) & 1, tmo)) {
             ok = false;
             report_error(a.err, kDevWaitDecode, 0xb3, seg);
@@ -680,21 +685,13 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                             v[b][t][e][0] = x.x, v[b][t][e][1] = x.y;
                         }
                     }
-            // log2 of the weight times V's scale: that is what O is the sum of
-            float lv = __log2f(sc.y);
-            uint32_t down = 0;  // factor of P for a scale below 2^kLeastV8
-            if (lv < kLeastV8) {
-                lv = fmaxf(lv, -200.f);
-                const float k = ceilf(kLeastV8 - lv);
-                lv += k;
-                const __half2 f = __float2half2_rn(ex2(-k));
-                down = *reinterpret_cast<const uint32_t*>(&f) | 0x80008000u;
-            }
+            // log2 of V's scale, rounded up (a number's exponent as the low bits of 2^23)
+            const float lv = __uint_as_float(0x4b000000u + ((__float_as_uint(sc.y) + 0x7fffffu) >> 23)) - (8388608.f + 127.f);
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s4[b][e] = fmaf(s4[b][e] + s5[b][e], sl[e & 1] * sc.x, lv);
+                for (int e = 0; e < 4; ++e) s4[b][e] = (s4[b][e] + s5[b][e]) * (sl[e & 1] * sc.x);
             if (lim < kUnit) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
@@ -706,45 +703,37 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx[e & 1] = fmaxf(mx[e & 1], s4[b][e]);
-            // (the maximum over the lanes is wanted where one of them is past the running one only)
-            if (__any_sync(0xffffffffu, mx[0] > m[0] + (kUp8 + kSlack8) || mx[1] > m[1] + (kUp8 + kSlack8))) {
+            // (the maximum over the lanes is wanted where one of them is past a running one only)
+            auto past = [&](int e) { return mx[e] > m[e] + kMost8 || mx[e] + lv > mp[e] + kMost8; };
+            if (__any_sync(0xffffffffu, past(0) || past(1))) {
+                float alpha[2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 2; ++e) {
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-                const bool need0 = mx[0] > m[0] + (kUp8 + kSlack8), need1 = mx[1] > m[1] + (kUp8 + kSlack8);
-                const float alpha0 = need0 ? ex2(m[0] - (mx[0] - kUp8)) : 1.f;
-                const float alpha1 = need1 ? ex2(m[1] - (mx[1] - kUp8)) : 1.f;
-                if (need0) m[0] = mx[0] - kUp8;
-                if (need1) m[1] = mx[1] - kUp8;
-                l[0] *= alpha0, l[1] *= alpha1;
+                    const float to = fmaxf(m[e], floorf(mx[e]));
+                    // (at most 2^127 for the factor: scales below 2^-112 keep fewer bits; 2^-115 at least)
+                    const float tp = fmaxf(fmaxf(mp[e], floorf(mx[e] + lv) - kUp8), to - 127.f);
+                    l[e] *= ex2(m[e] - to);
+                    alpha[e] = ex2(mp[e] - tp);
+                    m[e] = to, mp[e] = tp, up[e] = pow2(to - tp);
+                }
 #pragma unroll
-                for (int j = 0; j < D / 16; ++j) o[j][0] *= alpha0, o[j][1] *= alpha1, o[j][2] *= alpha0, o[j][3] *= alpha1;
+                for (int j = 0; j < D / 16; ++j)
+                    o[j][0] *= alpha[0], o[j][1] *= alpha[1], o[j][2] *= alpha[0], o[j][3] *= alpha[1];
             }
-            const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+            const float up0 = up[0] * sc.y, up1 = up[1] * sc.y;
             uint32_t ph[2][2], pl[2][2];  // keys 16 b + 8 half + 2 tq + {0, 1} of head hd
-            float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    float x = ex2(s4[b][2 * t] - m0), y = ex2(s4[b][2 * t + 1] - m1);
-                    sum0 += x, sum1 += y;
+                    float x = ex2(s4[b][2 * t] - m[0]), y = ex2(s4[b][2 * t + 1] - m[1]);
+                    l[0] += x, l[1] += y;
+                    x *= up0, y *= up1;
                     ph[b][t] = turned(split2<false>(x, y));
                     pl[b][t] = turned(split2<false>(x, y));
                 }
-            if (down) {
-                const uint32_t f = down & 0x7fff7fffu;
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        ph[b][t] = times2(ph[b][t], f);
-                        pl[b][t] = times2(pl[b][t], f);
-                    }
-            }
-            const float rv = ex2(-lv);
-            l[0] = fmaf(sum0, rv, l[0]), l[1] = fmaf(sum1, rv, l[1]);  // (the weights alone)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 // (four tiles of columns at a time: a tile's second product waits for its first)
@@ -778,12 +767,26 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
             report_error(a.err, kDevWaitDecode, 0xb5, segs);
         }
         __syncwarp();
+        if (__any_sync(0xffffffffu, mp[0] < m[0] - 60.f || mp[1] < m[1] - 60.f)) {
+            // (small scales alone: the factor 2^(mp - m) that takes sums of P to those of the weights, over up to 2^42, stays
+            // a number)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (mp[e] < m[e] - 60.f) {
+                    mp[e] += 100.f;
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) o[j][e] *= 0x1p-100f, o[j][2 + e] *= 0x1p-100f;
+                }
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
             const int g = 2 * tq + e;
-            if (hd == 0) ml[warp * 8 + g] = make_float2(m[e], l[e]);
+            if (hd == 0) {
+                ml[warp * 8 + g] = make_float2(m[e], l[e]);
+                mps[warp * 8 + g] = mp[e];
+            }
 #pragma unroll
             for (int j = 0; j < D / 16; j += 2)
                 *reinterpret_cast<float4*>(om_w + g * D + chunk(g, kCols / 4 * hd + j / 2) * 4) =

@@ -596,12 +596,13 @@ int32_t ep_sp_unpack_kv(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* src
  * length 0 gets a zero row.  k_new, v_new: NULL, or [n_seq][n_head_kv][head_dim]
  * of the context's dtype, which go into row kv_lens[s] - 1 of the cache first
  * and are attended as what the cache then holds of them (no two sequences may
- * then share the page of that row).  The products are exact, their sums, the
- * scores and the softmax statistics f32; an f32 q is taken to 22 bits of its
- * head's largest element.  A weight times its page's V scale (one below 2^-64
- * counts as that) is held to 22 bits and to 2^-39 of the head's largest; V scales
- * of one sequence are to lie within 2^116 of one another.  A query head with an infinity or a NaN has a row of
- * NaN, a NaN code of e4m3 makes NaN of what it reaches.  A sequence's result
+ * then share the page of that row).  The products are exact but for what is taken
+ * off q (an f32 q is held to 22 bits of its head's largest element, a bf16 q's
+ * elements below 2^-31 of it to 2^-39), their sums, the scores and the softmax
+ * statistics f32.  A weight times its page's V scale is held to 22 bits and to
+ * 2^-39 of the head's largest, whatever the scales (below 2^-112 to fewer), the
+ * sum of the weights is taken before the scales.  A query head with an infinity
+ * or a NaN has a row of NaN, a NaN code of e4m3 makes NaN of what it reaches.  A sequence's result
  * depends on the batch alone, not on timing. */
 int32_t ep_sp_decode8_bytes(const ep_sp_ctx* ctx, int32_t n_seq, int32_t max_kv_len, size_t* bytes);
 int32_t ep_sp_decode8_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* kv, const void* q, const void* k_new,

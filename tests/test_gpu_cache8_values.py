@@ -55,3 +55,61 @@ def test_bf16_outputs_of_terms_that_cancel(heads, dtype, q8):
     ctx.check(ctx.sync_status())
     # what is rounded to bf16 is off by tol at most
     assert bool(((out.double() - ref).abs() <= tol * (1 + 2.0 ** -8) + rounding(ref, epsp.BF16)).all())
+
+
+@pytest.mark.parametrize("q8", [E, Q], ids=name)
+@pytest.mark.parametrize("dtype", [epsp.BF16, epsp.F32], ids=name)
+@pytest.mark.parametrize("capacity", [64, 13000])  # joined in a CTA, and split over the device
+@pytest.mark.parametrize("v_scale", [2.0 ** -126, 2.0 ** -100, 2.0 ** -64, 1.0, 2.0 ** 126, 2.0 ** 127, 1.3 * 2.0 ** 126], ids=str)
+def test_weights_do_not_depend_on_the_scale_of_v(v_scale, capacity, dtype, q8):
+    """V the unit matrix, so that an output element is one weight times V's scale: the scale, wherever it lies, costs it
+    nothing."""
+    d, n = 64, 32
+    c = Cache8([n], 1, d, q8, 32, 0, 1, capacity=capacity)
+    at, one = c.at(0, n), 1 if q8 == Q else 0x38
+    k = torch.randint(-127, 128, (n,), generator=torch.Generator().manual_seed(1))
+    c.k8.view(torch.uint8).zero_(), c.v8.view(torch.uint8).zero_()
+    c.k8[at.cuda(), 0, 0] = k.cuda().to(c.k8.dtype)
+    c.v8.view(torch.uint8)[at.cuda(), 0, torch.arange(n)] = one
+    c.ks.fill_(2.0 ** -5), c.vs.fill_(v_scale)
+    ctx = context(1, 1, d, dtype, epsp.F32, capacity, 32)
+    q = torch.zeros(1, 1, d, device="cuda").to(TORCH[dtype])
+    q[0, 0, 0] = 3.0
+    out = run(ctx, c, q)[0, 0].double()
+    ctx.check(ctx.sync_status())
+    x = c.k8[at.cuda(), 0, 0].float().double() * 2.0 ** -5 * 3 / 8
+    want = torch.zeros(d, dtype=torch.float64, device="cuda")
+    want[:n] = torch.softmax(x, 0) * float(torch.tensor(v_scale, dtype=torch.float32))
+    # In units of 2^-24.  The score is one exact product, times the factor, log2 e in it and V's own: 4 roundings of
+    # |x| <= 1.5, so 6 of a weight; the subtraction of a maximum that is 16 off at most, 2^-21 ln 2, 5.5; the exponential
+    # 2^-22, 4: 16 of a weight, 32 with its sum's.  The weight as two f16 4, its products with the byte 4, a scale that is
+    # no power of two 1; the sum of weights 7, the quotient 2, the joins' factors 2 (of 2^-22 each, in one part)
+    tol = want * (32 + 4 + 4 + 1 + 7 + 2 + 8) * 2.0 ** -24
+    # Below f32's normal numbers (scales near 2^-126) steps are 2^-149: half a one in the sum, which the quotient by a sum
+    # of weights of 1/2 or more can double, and half a one in the quotient
+    tiny = 1.5 * 2.0 ** -149
+    assert bool(((out - want).abs() <= tol + tiny).all()), float(((out - want).abs() / (want + tiny)).max() * 2 ** 24)
+
+
+@pytest.mark.parametrize("q8", [E, Q], ids=name)
+@pytest.mark.parametrize("dtype", [epsp.F16, epsp.F32], ids=name)
+@pytest.mark.parametrize("scales", [(-100, -100, -100), (-100, -90, -89), (-80, -60, -88), (-126, -120, -110),
+                                    (-100, 40, -8), (-100, 110, 0), (126, 120, 100), (115, -126, 115)], ids=str)
+def test_scales_of_v_from_end_to_end(scales, dtype, q8):
+    """Pages of three scales in turn, far apart or all at one end, within the usual tolerance; pages of the smallest of
+    far scales hold zeros, as pack makes them."""
+    H, K, d, page, lens = 4, 2, 64, 32, [700, 90, 1, 33]
+    c = Cache8(lens, K, d, q8, page, 0, 1)
+    p = torch.arange(c.vs.shape[0], device="cuda") % 3
+    c.vs[:] = torch.exp2(torch.tensor(scales, dtype=torch.float64, device="cuda")[p])[:, None].float()
+    b = c.v8.view(-1, page, K, d)
+    b.copy_(torch.sign(b.float()).to(b.dtype))  # (448 * 2^126 is no f32)
+    if max(scales) - min(scales) > 100:
+        b.view(torch.uint8)[p == scales.index(min(scales))] = 0
+    ctx = context(H, K, d, dtype, epsp.F32, 700, page)
+    q = randq(4, H, d, dtype, 3)
+    ref, tol = decode64(c, q)
+    out = run(ctx, c, q)
+    ctx.check(ctx.sync_status())
+    assert bool(((out.double() - ref).abs() <= tol + rounding(ref, epsp.F32)).all())
+    assert torch.isfinite(out).all() and bool((out != 0).any(2).all())
