@@ -711,6 +711,8 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                 for (int e = 0; e < 2; ++e) {
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+                    // (each head for itself: no result depends on the other heads)
+                    if (!past(e)) mx[e] = -INFINITY;
                     const float to = fmaxf(m[e], floorf(mx[e]));
                     // (at most 2^127 for the factor: scales below 2^-112 keep fewer bits; 2^-115 at least)
                     const float tp = fmaxf(fmaxf(mp[e], floorf(mx[e] + lv) - kUp8), to - 127.f);

@@ -113,3 +113,19 @@ def test_scales_of_v_from_end_to_end(scales, dtype, q8):
     ctx.check(ctx.sync_status())
     assert bool(((out.double() - ref).abs() <= tol + rounding(ref, epsp.F32)).all())
     assert torch.isfinite(out).all() and bool((out != 0).any(2).all())
+
+
+@pytest.mark.parametrize("dtype", [epsp.BF16, epsp.F32], ids=name)
+@pytest.mark.parametrize("lens", [[20, 7], [1500, 700], [40000, 9]], ids=["a CTA", "a cluster", "split"])
+def test_a_head_does_not_depend_on_the_others(lens, dtype):
+    """One head of a group asks with queries far larger than the others': their bits stay."""
+    H, K, d, page = 8, 2, 64, 64
+    c = Cache8(lens, K, d, E, page, page, 1)
+    ctx = context(H, K, d, dtype, epsp.F32, max(lens), page)
+    q = randq(2, H, d, dtype)
+    clean = run(ctx, c, q)
+    q[:, 2] *= 40
+    out = run(ctx, c, q)
+    ctx.check(ctx.sync_status())
+    keep = torch.arange(H, device="cuda") != 2
+    assert torch.equal(out[:, keep], clean[:, keep]) and not torch.equal(out, clean)
