@@ -356,8 +356,9 @@ constexpr int kJoinHeads = 8;    // query heads whose scores a thread holds at a
 // CTAs shared (one CTA per query head of a run; at most one such run begins in
 // a CTA of k6a); the others, [n_seq][Hkv][chunks], add the weights of kJoinRows
 // rows of one KV head.  Latency bounds it (lengths, then ranges, then sums, then
-// weights), so registers are held to four CTAs per SM.
-template <int D>
+// weights), so registers are held to four CTAs per SM.  NAN_NONE: a head whose
+// scores are all -inf gets NaN, as the quotient 0 / 0 of a run in one CTA gives.
+template <int D, bool NAN_NONE>
 __global__ void __launch_bounds__(kJoinThreads, 4) k6b_join(const DecodeArgs a, const DecodeSplit sp, int heads,
                                                          int chunks) {
     __shared__ float wgt[kCtas];
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) k6b_join(const DecodeArgs a, 
             const float2 v = join_ml(sp, sh, stride, gi, lane);
             for (int i = lane; i < sh.count; i += 32) {
                 const float2 p = sp.part_ml[(int64_t)sh.slot(i) * stride + gi];
-                wgt[i] = p.y != 0.f ? ex2(p.x - v.x) / v.y : 0.f;
+                wgt[i] = p.y != 0.f ? ex2(p.x - v.x) / v.y : NAN_NONE && v.y == 0.f ? __int_as_float(0x7fffffff) : 0.f;
             }
         }
         __syncthreads();

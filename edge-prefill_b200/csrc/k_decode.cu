@@ -751,7 +751,7 @@ cudaError_t launch_join(DecodeArgs a, const DecodeSplit& sp, cudaStream_t s) {
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k6b_join<D>, a, sp, heads, chunks);
+    return cudaLaunchKernelEx(&cfg, k6b_join<D, false>, a, sp, heads, chunks);
 }
 
 template <int ET, int D, int W, bool P3, int GH>

@@ -931,7 +931,7 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k6b_join<D>, a, sp, heads, 0);
+    return cudaLaunchKernelEx(&cfg, k6b_join<D, true>, a, sp, heads, 0);
 }
 
 template <int D, bool I8>

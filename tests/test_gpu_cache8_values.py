@@ -129,3 +129,24 @@ def test_a_head_does_not_depend_on_the_others(lens, dtype):
     ctx.check(ctx.sync_status())
     keep = torch.arange(H, device="cuda") != 2
     assert torch.equal(out[:, keep], clean[:, keep]) and not torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("q8", [E, Q], ids=name)
+@pytest.mark.parametrize("dtype", [epsp.BF16, epsp.F16, epsp.F32], ids=name)
+@pytest.mark.parametrize("lens", [[20, 7], [1500, 700], [40000, 9]], ids=["a CTA", "a cluster", "split"])
+def test_a_query_of_minus_infinity_on_keys_of_one_sign(lens, dtype, q8):
+    """Every score of the head is -inf: a row of NaN, however a run is finished; other heads as without it."""
+    H, K, d, page = 8, 2, 64, 64
+    c = Cache8(lens, K, d, q8, page, page, 1)
+    b = c.k8.view(torch.uint8)
+    for i, n in enumerate(lens):
+        b[c.at(i, n).cuda(), :, 5] = 0x30  # positive in both types
+    ctx = context(H, K, d, dtype, epsp.F32, max(lens), page)
+    q = randq(2, H, d, dtype)
+    clean = run(ctx, c, q)
+    bad = torch.zeros(2, H, dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[0, 6] = bad[1, 3] = True
+    q[..., 5][bad] = -float("inf")
+    out = run(ctx, c, q)
+    ctx.check(ctx.sync_status())
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[~bad])
