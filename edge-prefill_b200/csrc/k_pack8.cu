@@ -242,6 +242,12 @@ __global__ void __launch_bounds__(T, (C == 1 ? 1536 : C == 2 ? 1280 : C == 4 || 
     }
 }
 
+// Largest finite value of the context's type.
+template <int ET>
+__device__ __forceinline__ float largest() {
+    return ET == 0 ? 3.402823466e38f : ET == 1 ? 65504.f : __uint_as_float(0x7f7f0000u);
+}
+
 constexpr int kTile = 32;   // rows of a tile: a page holds whole ones, so a tile's rows lie together in both caches
 constexpr int kUnpack = 2;  // 16-byte chunks of K and of V per thread and turn
 
@@ -288,6 +294,12 @@ __global__ void __launch_bounds__(kThreads) k9_unpack(const PackArgs a) {
                         from8<I8>(w[e], x);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) x[k] *= sc[kv][j];
+                        if (sc[kv][j] > largest<ET>() / (I8 ? 128.f : 448.f)) {
+                            // (rare) a value near the type's largest may have been rounded past it; a NaN stays
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (fabsf(x[k]) > largest<ET>()) x[k] = copysignf(largest<ET>(), x[k]);
+                        }
                         if constexpr (ET == 0) {
                             reinterpret_cast<float4*>(static_cast<float*>(out) + el)[e] = make_float4(x[0], x[1], x[2], x[3]);
                         } else if constexpr (ET == 1) {

@@ -584,7 +584,9 @@ int32_t ep_sp_pack_kv(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* src, 
                       const int32_t* first, const ep_sp_kv_batch* dst, const ep_sp_kv8* cache, void* stream);
 
 /* The way back: rows [first[s], src->kv_lens[s]) of the 8-bit cache (src) into
- * the same rows of a cache of the context's dtype (dst), rounded to it.  The
+ * the same rows of a cache of the context's dtype (dst), rounded to it (a value
+ * past its largest, which the rounding to 8 bits can make of one near it, becomes
+ * the largest; a NaN code of e4m3 a NaN).  The
  * context forgets the layer's page sums and f16 shadows, so a gated prefill
  * call on those rows pools them (after replaying a captured call ep_sp_reset
  * does that). */
