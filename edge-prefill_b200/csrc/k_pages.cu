@@ -314,8 +314,7 @@ __global__ void __launch_bounds__(kPlan, 1) k11_resize(const PagesArgs a, const 
         w.was[s] = n;
         w.now[s] = now;
         // (held by others or not is known once all have given back)
-        const int b = now > n && n % a.block_rows ? a.tables[s * a.table_stride + n / a.block_rows] : -1;
-        w.last[s] = b >= 0 && b < a.pool_blocks ? b : -1;
+        w.last[s] = now > n && n % a.block_rows ? entry(a, a.tables[s * a.table_stride + n / a.block_rows], (int)s) : -1;
     }
     if (me == 0 && lane == 0) *(SMALL ? &pairs_s : w.n_pairs) = 0;
     meet<SMALL>();
