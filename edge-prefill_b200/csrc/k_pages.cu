@@ -543,7 +543,7 @@ cudaError_t go(void (*kernel)(P...), dim3 grid, int threads, int cluster, size_t
     cfg.stream = s;
     cfg.attrs = at;
     cfg.numAttrs = cluster ? 2 : 1;
-    if (smem > 48 * 1024) {
+    if (smem > 47 * 1024) {  // (48 KB with the kernel's static part)
         // (the same for all calls: two threads may be here with different sizes)
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
         if (e != cudaSuccess) return e;

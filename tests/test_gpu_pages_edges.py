@@ -25,3 +25,15 @@ def test_growth_in_a_block_that_is_none_is_reported(n_seq, blocks):
         x.tables[0, 1] = was
         x.book.resize([n, 33, 64])
         x.check()
+
+
+@pytest.mark.parametrize("n_seq,blocks", [(3, 3060), (55, 3000), (3, 6120), (2, 6143), (3, 6144), (4096, 8192), (3, 8193)],
+                         ids=str)
+def test_sizes_around_what_a_plan_holds_on_chip(n_seq, blocks):
+    """Plans of 48 KB, a little less and a little more, of all that one CTA holds, and one more."""
+    x = Both(n_seq, 2, 32, blocks, 2, sizes=[4])
+    assert x.resize([(40 if s % 3 else 20) if s < 3000 else 0 for s in range(n_seq)])
+    x.fork([s if s % 4 else min(s + 1, n_seq - 1) for s in range(n_seq)])
+    assert x.resize([min(n + 1, 64) if n else 0 for n in x.book.lens])
+    assert x.resize([0 if s % 2 else n for s, n in enumerate(x.book.lens)])
+    x.compact()
