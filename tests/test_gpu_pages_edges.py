@@ -37,3 +37,13 @@ def test_sizes_around_what_a_plan_holds_on_chip(n_seq, blocks):
     assert x.resize([min(n + 1, 64) if n else 0 for n in x.book.lens])
     assert x.resize([0 if s % 2 else n for s, n in enumerate(x.book.lens)])
     x.compact()
+
+
+def test_the_last_holder_keeps_a_block_that_all_grow_in():
+    x = Both(4, 4, 32, 20, 1)
+    x.resize([40, 0, 0, 0])
+    kept = x.book.tables[0][1]
+    x.fork([0, 0, 0, 0])
+    x.resize([41, 41, 41, 41])
+    last = x.tables[:, 1].tolist()
+    assert last[3] == kept and len(set(last)) == 4
