@@ -347,7 +347,7 @@ class Pages:
         _check("kv_lens", kv_lens, i32, (self.n_seq,), self.device)
         _check("block_tables", block_tables, i32, (self.n_seq, block_tables.shape[-1]), self.device)
         _check("refs", refs, i32, (refs.shape[0],), self.device)
-        self.blocks = refs.shape[0]
+        self.blocks, self.block_rows = refs.shape[0], block_rows
         self.desc = PagesDesc(self.n_seq, block_tables.shape[1], block_rows, self.blocks, kv_lens.data_ptr(),
                               block_tables.data_ptr(), refs.data_ptr())
         self.ref = ctypes.byref(self.desc)
@@ -358,7 +358,7 @@ class Pools:
     [blocks][bytes of a block].  Keeps its tensors alive."""
 
     def __init__(self, tensors, blocks):
-        self.tensors, self.blocks = list(tensors), blocks
+        self.tensors, self.blocks, self.fits = list(tensors), blocks, None
         if not self.tensors:
             raise ValueError("no pools")
         self.device = self.tensors[0].get_device()
@@ -704,10 +704,26 @@ class Context:
     # --------------------------------------------- blocks of paged caches
     def _pages(self, pages, pools=None):
         dev = self._fast()[4]
+        if pools is not None and pools.fits != (self._facts, pages.blocks, pages.block_rows):
+            self._pool_rows_fit(pages, pools)
         if pages.device != dev or (pools is not None and pools.device != dev):
             raise ValueError(f"the pages or pools are not on cuda:{dev}")
         if pools is not None and pools.blocks != pages.blocks:
             raise ValueError(f"the pools have {pools.blocks} blocks, the counts {pages.blocks}")
+
+    def _pool_rows_fit(self, pages, pools):
+        """A tensor that is seen to hold cache rows or pages' scales has as many as the blocks (or one a block); looked
+        at once, the shapes stay."""
+        _, _, f32, _, _, _, heads, d = self._fast()
+        rows = pages.blocks * pages.block_rows
+        for i, t in enumerate(pools.tensors):
+            n = t.numel() // (heads * d) if t.dim() > 2 and t.shape[-2:] == (heads, d) else None
+            if t.dim() == 2 and t.dtype == f32 and t.shape[1] == heads:
+                n = t.shape[0]
+            if n is not None and n not in (rows, rows // self.cfg.page_size, pages.blocks):
+                raise ValueError(f"pool {i} of shape {tuple(t.shape)} is not {pages.blocks} blocks of "
+                                 f"{pages.block_rows} rows")
+        pools.fits = (self._facts, pages.blocks, pages.block_rows)
 
     def _seq_ints(self, name, t, n_seq):
         _check(name, t, self._fast()[3], (n_seq,), self._fast()[4])
