@@ -36,7 +36,8 @@ enum DeviceError : int32_t {
 // The device error word is err[0] of a record of kErrWords: the kernel whose
 // atomicCAS on err[0] wins also writes err[1] = where (role * 16 + barrier),
 // err[2] = its block index, err[3] = its KV tile, for ep_sp_sync_status.  err[4]
-// is not 0 once a resize was refused (kDevNoBlocks), until that is reported.
+// is not 0 once a resize was refused (kDevNoBlocks, or one sequence's length),
+// until that is reported.
 constexpr int kErrWords = 5, kErrRefused = 4;
 #if defined(__CUDACC__)
 // After a refused resize the tables do not hold the rows that the calls behind it

@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(kPlan, 1) k11_resize(const PagesArgs a, const 
         const int n = rows_of(a, a.lens[s], (int)s);
         int now = new_lens[s];
         if (now < 0 || now > (int64_t)a.table_stride * a.block_rows) {
+            a.err[kErrRefused] = 1;
             report_error(a.err, kDevBadLength, 0xc3, (int)s);
             now = n;
         }

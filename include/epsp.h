@@ -651,13 +651,14 @@ int32_t ep_sp_count_refs(ep_sp_ctx* ctx, const ep_sp_pages* pages, void* stream)
  * outside the parent's rows is reported (rc 6) and leaves its sequence as it
  * is.  Nothing is copied yet: ep_sp_resize_seqs does that where a sequence goes
  * on to write into a block that others hold.  parents, lens: DEVICE [n_seq].
- * The context forgets all layers' page sums.  rc 2 on bad arguments. */
+ * The context forgets all layers' page sums (after replaying a captured call
+ * ep_sp_reset does that).  rc 2 on bad arguments. */
 int32_t ep_sp_fork_bytes(const ep_sp_ctx* ctx, const ep_sp_pages* pages, size_t* bytes);
 int32_t ep_sp_fork_seqs(ep_sp_ctx* ctx, const ep_sp_pages* pages, const int32_t* parents, const int32_t* lens,
                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* Lengths become new_lens (DEVICE [n_seq], 0 to table_stride * block_rows; one
- * outside is reported, rc 6, and its sequence left).  First the blocks past the
+ * outside is refused, rc 6, and its sequence left).  First the blocks past the
  * shorter lengths are given back, then the longer sequences, in order, take the
  * lowest free blocks: one for the copy of a partly filled last block that other
  * sequences hold too, then those for the rows to come.  Where every holder of
@@ -666,16 +667,16 @@ int32_t ep_sp_fork_seqs(ep_sp_ctx* ctx, const ep_sp_pages* pages, const int32_t*
  * one; what those rows hold is undefined.  Only lengths are changed here: call it
  * before the step that writes the rows.
  * With fewer free blocks than needed nothing changes and ep_sp_sync_status
- * reports rc 10.  The steps that follow on the device do not know: row
- * kv_lens[s] - 1 is then a row from before, which others may hold, and table
- * entries past the lengths are anybody's.  So from there until
- * ep_sp_sync_status has reported it no call of the context writes a row through
- * block tables (ep_sp_decode_layer and ep_sp_decode8_layer with new rows,
+ * reports rc 10.  The steps that follow on the device do not know of that, nor of
+ * a refused length: row kv_lens[s] - 1 is then a row from before, which others
+ * may hold, and table entries past the lengths are anybody's.  So from a refusal
+ * until ep_sp_sync_status has reported it no call of the context writes a row
+ * through block tables (ep_sp_decode_layer and ep_sp_decode8_layer with new rows,
  * ep_sp_pack_kv, ep_sp_unpack_kv, ep_sp_append_kv, ep_sp_evict_layer into other
- * rows, which leaves new_lens and acc_dst too): the caches stay as they are, what these
+ * rows, which leaves new_lens and acc_dst too): the caches' rows stay, what these
  * calls answer means nothing, and the steps since have to be made again.
- * ep_sp_sync_status then forgets all layers' page sums and f16 shadows.  pools: HOST [n_pools],
- * n_pools in [1, 4096]. */
+ * ep_sp_sync_status then forgets all layers' page sums and f16 shadows.
+ * pools: HOST [n_pools], n_pools in [1, 4096]. */
 int32_t ep_sp_resize_bytes(const ep_sp_ctx* ctx, const ep_sp_pages* pages, size_t* bytes);
 int32_t ep_sp_resize_seqs(ep_sp_ctx* ctx, const ep_sp_pages* pages, const int32_t* new_lens, const ep_sp_pool* pools,
                           int32_t n_pools, void* workspace, size_t workspace_bytes, void* stream);

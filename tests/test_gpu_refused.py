@@ -134,3 +134,21 @@ def test_a_refusal_behind_another_failure_is_told_too():
     ctx.check(ctx.resize_seqs(pages, ints([70, 40]), pools, ws))
     assert ctx.sync_status() == epsp.PREFILL and "refused" in ctx.last_error()
     assert ctx.sync_status() == epsp.OK
+
+
+def test_a_refused_length_holds_the_step_back():
+    """One sequence's new length is more than its table holds, and its last row one that another sequence holds too."""
+    H, K, d, page, n = 8, 2, 64, 32, 96
+    c = Cache8([n, 0, 40], K, d, epsp.E4M3, page, page, 1, capacity=96)
+    ctx = context(H, K, d, epsp.BF16, epsp.F32, 96, page)
+    pages, pools = book_of(c, [c.k8, c.v8, c.ks, c.vs], c.lens, 2)
+    ws = workspace(max(ctx.fork_bytes(pages), ctx.resize_bytes(pages), ctx.decode8_bytes(3, 96)))
+    ctx.check(ctx.fork_seqs(pages, ints([0, 0, 2]), ws))
+    q = torch.randn(3, H, d, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    was, out = c.state(), torch.zeros(3, H, d, device="cuda")
+    ctx.check(ctx.resize_seqs(pages, ints([n + 1, n, 41]), pools, ws))
+    ctx.check(ctx.decode8_layer(0, c.batch, q, c.kv8, out, ws, k_new=q[:, :K].contiguous(), v_new=q[:, :K].contiguous()))
+    torch.cuda.synchronize()
+    assert same(c.state(), was) and c.d_lens.tolist() == [n, n, 41]
+    assert ctx.sync_status() == epsp.PREFILL and "refused" in ctx.last_error()
+    assert ctx.sync_status() == epsp.OK
