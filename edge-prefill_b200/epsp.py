@@ -358,7 +358,7 @@ class Pools:
     [blocks][bytes of a block].  Keeps its tensors alive."""
 
     def __init__(self, tensors, blocks):
-        self.tensors, self.blocks, self.fits = list(tensors), blocks, None
+        self.tensors, self.blocks, self.fits, self.shapes = list(tensors), blocks, None, {}
         if not self.tensors:
             raise ValueError("no pools")
         self.device = self.tensors[0].get_device()
@@ -369,6 +369,7 @@ class Pools:
             if t.nbytes == 0 or t.nbytes % (4 * blocks):
                 raise ValueError(f"pool {i} is not {blocks} blocks of whole 4-byte words")
             self.desc[i] = PoolDesc(t.data_ptr(), t.nbytes // blocks)
+            self.shapes.setdefault((t.shape, t.dtype), i)
 
 
 class Context:
@@ -716,12 +717,12 @@ class Context:
         at once, the shapes stay."""
         _, _, f32, _, _, _, heads, d = self._fast()
         rows = pages.blocks * pages.block_rows
-        for i, t in enumerate(pools.tensors):
-            n = t.numel() // (heads * d) if t.dim() > 2 and t.shape[-2:] == (heads, d) else None
-            if t.dim() == 2 and t.dtype == f32 and t.shape[1] == heads:
-                n = t.shape[0]
+        for (shape, dtype), i in pools.shapes.items():
+            n = shape.numel() // (heads * d) if len(shape) > 2 and shape[-2:] == (heads, d) else None
+            if len(shape) == 2 and dtype == f32 and shape[1] == heads:
+                n = shape[0]
             if n is not None and n not in (rows, rows // self.cfg.page_size, pages.blocks):
-                raise ValueError(f"pool {i} of shape {tuple(t.shape)} is not {pages.blocks} blocks of "
+                raise ValueError(f"pool {i} of shape {tuple(shape)} is not {pages.blocks} blocks of "
                                  f"{pages.block_rows} rows")
         pools.fits = (self._facts, pages.blocks, pages.block_rows)
 
