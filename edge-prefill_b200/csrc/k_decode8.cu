@@ -4,10 +4,10 @@
 //   x_j = q . kq_j ks * scale,  out = sum_j exp(x_j - m) vq_j vs / sum_j exp(x_j - m)
 //
 // Half the bytes of K6; the split of the rows over the CTAs, the ring and the
-// joins are K6's (decode_common.cuh).  64 K rows (8 heads of 128) take 32 us, 4.1
-// TB/s, 64 sequences of up to 4096 rows 60, 4.5 TB/s; without the arithmetic 26 and
+// joins are K6's (decode_common.cuh).  64 K rows (8 heads of 128) take 33 us, 4.1
+// TB/s, 64 sequences of up to 4096 rows 61, 4.4 TB/s; without the arithmetic 26 and
 // 52: the bytes bound it first, then the attending warps, two a scheduler, whose
-// products and conversions wait for one another (issue slots 34 to 45 % busy).  A new token's row is
+// products and conversions wait for one another (issue slots 35 to 47 % busy).  A new token's row is
 // quantised into the cache by the CTA that attends it: the last page of a run is
 // never split, and its copies wait for the row (as a kernel before, k9_append,
 // it took 3 to 4 us more; calls of several passes still have that).
@@ -31,7 +31,7 @@
 // are.  Two running maxima, in whole powers of two: that of the scores, for the
 // weights and their sum, and that of score and scale, for P; a unit's weights
 // become P by one factor.  (Of the products alone, the sum would lose the weights
-// of pages with small scales and the range of large ones.)  The largest P is held
+// of pages with small scales and the range of large ones; 1 to 2 % faster.)  The largest P is held
 // between 2^14 and 2^15, and P is two f16: an element keeps 22 bits of itself and
 // an absolute 2^-39 of the largest (half of f16's smallest step).
 #include <cuda.h>
@@ -44,7 +44,8 @@
 #include <cstdint>
 #include <type_traits>
 
-// (in units of 32 rows of 8 bits; 64 sequences of up to 4096 rows: 6 72 us, 10 64.2, 14 63.7, 20 64.5)
+// (in units of 32 rows of 8 bits; 64 sequences of up to 4096 rows: 6 71.5 us, 10
+// 64.7, 14 61.0, 20 60.7; 64 K rows: 10 32.3, 14 32.4, 20 32.5)
 #define EPSP_RUN_COST 14
 #include "cache8.cuh"
 #include "decode_common.cuh"
@@ -65,9 +66,10 @@ constexpr float kNone8 = -3.402823466e38f;  // either of no rows: a number, so t
 constexpr int kPass8 = 64;        // query heads of a pass, at most
 // Units for each CTA of a cluster up to which a run is joined in shared memory
 // instead of being split over the device: one launch. One sequence of 6000, 12,000,
-// 16,000 and 24,000 rows, split 13.0, 15.1, 16.5 and 18.2 us, in clusters of 8 10.1,
-// 13.5, 15.5 and 19.8 (32 heads on 8); split 13.3, 14.5, 16.2 and 17.4, in clusters
-// 10.8, 15.0, 17.4 and 22.9 (28 on 4).
+// 16,000 and 24,000 rows, split 14.1, 16.3, 17.9 and 20.2 us, in clusters of 8 11.4,
+// 15.6, 17.7 and 22.8 (32 heads on 8); split 13.5, 14.9, 16.1 and 17.8, in clusters
+// 11.8, 16.4, 19.1 and 24.9 (28 on 4); f32, 14 on 2, split 11.8, 12.6, 14.4 and 13.9, in
+// clusters 9.7, 13.0, 15.0 and 19.0.
 constexpr int kClusterMost8 = 48;
 
 // Shared memory: the stages, then what follows by offset.
@@ -257,7 +259,8 @@ __device__ __forceinline__ void append_row(const DecodeArgs& a, const Cache8& c,
 }
 
 // LO: q has remainders (f32).  (P always has: where V's terms cancel, the 11 bits of
-// one f16 show in a bf16 output too.)  JOIN: the calls that join_cluster finishes.
+// one f16 show in a bf16 output too; 8 sequences of 16 to 32 K rows 47.1 us, with one
+// f16 45.2.)  JOIN: the calls that join_cluster finishes.
 template <int D, bool I8, bool LO, bool JOIN>
 __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     k10_decode8(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,

@@ -12,10 +12,10 @@
 // follow one another, so the whole rows of the source are read at about one
 // time.  A page that holds rows before `first` keeps its scale, or has it grown
 // and those rows' bytes follow, by the same CTA.  64 K rows (8 heads of 128,
-// bf16 to e4m3) 79 us, 5.1 TB/s: the waits within a tile, for its rows and for its
-// maximum, bound it (issue slots 52 % busy, 24 warps an SM).
+// bf16 to e4m3) 80 us, 5.0 TB/s: the waits within a tile, for its rows and for its
+// maximum, bound it (issue slots 50 % busy, 24 warps an SM).
 // unpack: tiles of 32 rows, which lie together in both caches, 16 bytes a
-// thread.  32 K rows (4 heads of 128, to bf16) 24 us, 4.2 TB/s with the launch.
+// thread.  32 K rows (4 heads of 128, to bf16) 23 us, 4.3 TB/s with the launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
