@@ -83,7 +83,7 @@ struct Layout8 {
     __host__ __device__ int off_q() const { return stages * kStage; }
     __host__ __device__ int off_o() const { return off_q() + 2 * q_bytes; }        // [kWarps8][8][D] the warps' sums
     __host__ __device__ int off_ml() const { return off_o() + kWarps8 * 8 * D * 4; }  // [kWarps8][8] (maximum, sum)
-    __host__ __device__ int off_mp() const { return off_ml() + kWarps8 * 8 * 8; }     // [kWarps8][8] P's maximum
+    __host__ __device__ int off_mp() const { return off_ml() + kWarps8 * 8 * 8; }     // [kWarps8][8] P's over it
     __host__ __device__ int off_scale() const { return off_mp() + kWarps8 * 8 * 4; }  // [stages] (ks, vs)
     __host__ __device__ int off_bar() const { return off_scale() + kMost * 8; }
     __host__ __device__ int off_lens() const { return off_bar() + (2 * kMost + 7) * 8; }
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
             // lane r: stream r
             const int at = (lane * groups + gw) * 8 + gh;
             const float2 v = lane < streams ? ml[at] : make_float2(-INFINITY, 0.f);
-            const float mp = lane < streams ? mps[at] : -INFINITY;
+            const float mp = lane < streams ? mps[at] : 0.f;
             const float* from = om + gw * 8 * D + gh * D + chunk(gh, lane * kC / 4) * 4 + lane * kC % 4;
             float t[kWarps8][kC];
 #pragma unroll
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
 #pragma unroll
             for (int x = 1; x < 8; x <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
             mt = __shfl_sync(0xffffffffu, mt, 0);
-            const float f = ex2(mp - mt);
+            const float f = ex2(v.x - mt + mp);
             float lt = v.y * ex2(v.x - mt);
 #pragma unroll
             for (int x = 1; x < 8; x <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, x);
@@ -557,8 +557,9 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
         float o[D / 16][4];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        // of heads 2 tq + {0, 1}: log2 of what the weights (l: their sum) and P are relative to, and 2 to their difference
-        float m[2] = {kNone8, kNone8}, mp[2] = {kNone8, kNone8}, up[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
+        // of heads 2 tq + {0, 1}: log2 of what the weights (l: their sum) are relative to, that of P over it (a small whole
+        // number, however large the scores), and the factor from the ones to the other
+        float m[2] = {kNone8, kNone8}, mp[2] = {0.f, 0.f}, up[2] = {1.f, 1.f}, l[2] = {0.f, 0.f};
         if (ok && !tc::mbar_wait(&q_full[seg & 1], (seg >> 1) & 1, tmo)) {
             ok = false;
             report_error(a.err, kDevWaitDecode, 0xb3, seg);
@@ -707,7 +708,7 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx[e & 1] = fmaxf(mx[e & 1], s4[b][e]);
             // (the maximum over the lanes is wanted where one of them is past a running one only)
-            auto past = [&](int e) { return mx[e] > m[e] + kMost8 || mx[e] + lv > mp[e] + kMost8; };
+            auto past = [&](int e) { return mx[e] - m[e] > kMost8 || mx[e] - m[e] + lv > mp[e] + kMost8; };
             if (__any_sync(0xffffffffu, past(0) || past(1))) {
                 float alpha[2];
 #pragma unroll
@@ -716,12 +717,12 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                     for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
                     // (each head for itself: no result depends on the other heads)
                     if (!past(e)) mx[e] = -INFINITY;
-                    const float to = fmaxf(m[e], floorf(mx[e]));
+                    const float to = fmaxf(m[e], floorf(mx[e])), was = mp[e] + (m[e] - to);
                     // (at most 2^127 for the factor: scales below 2^-112 keep fewer bits; 2^-115 at least)
-                    const float tp = fmaxf(fmaxf(mp[e], floorf(mx[e] + lv) - kUp8), to - 127.f);
+                    const float tp = fmaxf(fmaxf(was, floorf(mx[e] - to + lv) - kUp8), -127.f);
                     l[e] *= ex2(m[e] - to);
-                    alpha[e] = ex2(mp[e] - tp);
-                    m[e] = to, mp[e] = tp, up[e] = pow2(to - tp);
+                    alpha[e] = ex2(was - tp);
+                    m[e] = to, mp[e] = tp, up[e] = pow2(-tp);
                 }
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j)
@@ -772,12 +773,12 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
             report_error(a.err, kDevWaitDecode, 0xb5, segs);
         }
         __syncwarp();
-        if (__any_sync(0xffffffffu, mp[0] < m[0] - 60.f || mp[1] < m[1] - 60.f)) {
-            // (small scales alone: the factor 2^(mp - m) that takes sums of P to those of the weights, over up to 2^42, stays
-            // a number)
+        if (__any_sync(0xffffffffu, mp[0] < -60.f || mp[1] < -60.f)) {
+            // (small scales alone: the factor 2^mp that takes sums of P to those of the weights, over up to 2^42, stays a
+            // number)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                if (mp[e] < m[e] - 60.f) {
+                if (mp[e] < -60.f) {
                     mp[e] += 100.f;
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j) o[j][e] *= 0x1p-100f, o[j][2 + e] *= 0x1p-100f;

@@ -150,3 +150,30 @@ def test_a_query_of_minus_infinity_on_keys_of_one_sign(lens, dtype, q8):
     out = run(ctx, c, q)
     ctx.check(ctx.sync_status())
     assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("q8", [E, Q], ids=name)
+@pytest.mark.parametrize("dtype", [epsp.BF16, epsp.F16, epsp.F32], ids=name)
+@pytest.mark.parametrize("lens", [[70, 1], [1500, 700], [40000, 9]], ids=["a CTA", "a cluster", "split"])
+@pytest.mark.parametrize("v_scale", [2.0 ** -100, 2.0 ** -40, 1.0, 2.0 ** 100], ids=str)
+def test_scores_beyond_whole_numbers(v_scale, lens, dtype, q8):
+    """Scores of up to 2^37 and more, where f32 has no fractions: the row of the largest is all there is, whatever V's
+    scale."""
+    K, d, page = 1, 64, 32
+    c = Cache8(lens, K, d, q8, page, page, 1)
+    g = torch.Generator().manual_seed(2)
+    c.k8.view(torch.uint8).zero_()
+    want = torch.zeros(len(lens), 1, d, device="cuda")
+    for i, n in enumerate(lens):
+        at, top = c.at(i, n).cuda(), int(torch.randint(n, (1,), generator=g))
+        k = torch.randint(-112, 97, (n,), generator=g).float()
+        k[top] = 112.0
+        c.k8[at, 0, 3] = k.cuda().to(c.k8.dtype)
+        want[i, 0] = c.v8[at[top], 0].float() * v_scale
+    c.ks.fill_(2.0 ** 12), c.vs.fill_(v_scale)
+    ctx = context(1, K, d, dtype, epsp.F32, max(lens), page)
+    q = torch.zeros(len(lens), 1, d, device="cuda").to(TORCH[dtype])
+    q[:, :, 3] = 2.0 ** 15 if dtype == epsp.F16 else 2.0 ** 40
+    out = run(ctx, c, q)
+    ctx.check(ctx.sync_status())
+    assert torch.equal(out, want)
