@@ -7,10 +7,11 @@
 // joins are K6's (decode_common.cuh).  64 K rows (8 heads of 128) take 33 us, 4.1
 // TB/s, 64 sequences of up to 4096 rows 61, 4.4 TB/s; without the arithmetic 26 and
 // 52: the bytes bound it first, then the attending warps, two a scheduler, whose
-// products and conversions wait for one another (issue slots 35 to 47 % busy).  A new token's row is
-// quantised into the cache by the CTA that attends it: the last page of a run is
-// never split, and its copies wait for the row (as a kernel before, k9_append,
-// it took 3 to 4 us more; calls of several passes still have that).
+// products and conversions wait for one another (issue slots 35 to 47 % busy).  A
+// new token's row is quantised into the cache by the CTA that attends it: the last
+// page of a run is never split, and its copies wait for the row (as a kernel
+// before, k9_append, it took 3 to 4 us more; calls of several passes still have
+// that).
 //
 // CTA: units (32 rows of one head, so one scale each of K and V) go round robin
 // to the streams of 8 warps, each with its own online softmax over 8 query heads
@@ -31,9 +32,9 @@
 // are.  Two running maxima, in whole powers of two: that of the scores, for the
 // weights and their sum, and that of score and scale, for P; a unit's weights
 // become P by one factor.  (Of the products alone, the sum would lose the weights
-// of pages with small scales and the range of large ones; 1 to 2 % faster.)  The largest P is held
-// between 2^14 and 2^15, and P is two f16: an element keeps 22 bits of itself and
-// an absolute 2^-39 of the largest (half of f16's smallest step).
+// of pages with small scales and the range of large ones; 1 to 2 % faster.)  The
+// largest P is held between 2^14 and 2^15, and P is two f16: an element keeps 22
+// bits of itself and an absolute 2^-39 of the largest (half of f16's smallest step).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>

@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(kThreads, 1) k8a_select_rows(const EvictArgs a
         load(n);
     }
     const int m = min(n, a.n_keep);
-    // rows that must not be written: a count of less than 0, and the weights stay (asked for by the kernel that moves the
-    // rows: 0.5 us of 20)
+    // rows that must not be written: a count of less than 0, and the weights stay (0.2 us of 20; asked for by the warps
+    // that move the rows 0.5)
     const int32_t held = !a.in_place && a.dst.block_rows > 0 ? a.err[kErrRefused] : 0;
     if (h == 0 && rank == 0 && t == 0) p.kept[s] = held == 0 ? m : -1;
     // rows [r0, r1) are this CTA's; [lo, hi) the candidates, of which `want` stay

@@ -555,12 +555,13 @@ int32_t ep_sp_evict_layer(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* s
  * The calls write scales 2^e with e the least integer for which the page's
  * largest magnitude is at most M * 2^e (M = 448 for e4m3, 127 for integers) and
  * at least -100, and bytes rounded to nearest, ties to even.  Rows written
- * behind others of a page grow its scale where they need to; the bytes that
+ * behind others of a page grow its scale where they need to (rows behind those
+ * count as none); the bytes that
  * were there are then rounded again to the new one.  Scales of rows that these
  * calls read must be positive and finite; the calls that only read (unpack,
  * decode) take any such scale, those that write behind rows want a power of
  * two, as they leave it themselves.  An infinity goes into the cache as the
- * largest magnitude, a NaN as 0; either is reported by ep_sp_sync_status (rc 9).
+ * largest magnitude of its page's scale, a NaN as 0; either is reported by ep_sp_sync_status (rc 9).
  * All four pointers are 16-byte aligned (the scales 4-byte). */
 #define EP_SP_E4M3 3
 #define EP_SP_I8 4
@@ -575,8 +576,9 @@ typedef struct ep_sp_kv8 {
 /* Rows [first[s], src->kv_lens[s]) of every sequence into the same rows of the
  * 8-bit cache (first: DEVICE [n_seq], or NULL for 0; one outside
  * [0, kv_lens[s]] is reported, rc 6, and its sequence left out).  Rows of dst
- * outside that range keep their values (those before first[s] in its page are
- * rounded to a grown scale).  src is a cache of the context's dtype as a
+ * before first[s] keep their values (those in its page are rounded to a grown
+ * scale), other pages theirs; kv_lens[s] is where the sequence then ends: what
+ * lies behind it in the last page keeps its bytes, not its scale.  src is a cache of the context's dtype as a
  * prefill leaves it; dst has the same n_seq, room for src->max_kv_len rows and
  * its own layout, its kv_lens is not read.  No page of dst may be written
  * through two sequences.  rc 2 on bad arguments. */
