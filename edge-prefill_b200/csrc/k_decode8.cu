@@ -261,8 +261,13 @@ __device__ __forceinline__ void append_row(const DecodeArgs& a, const Cache8& c,
 
 // LO: q has remainders (f32).  (P always has: where V's terms cancel, the 11 bits of
 // one f16 show in a bf16 output too; 8 sequences of 16 to 32 K rows 47.1 us, with one
-// f16 45.2.)  JOIN: the calls that join_cluster finishes.
-template <int D, bool I8, bool LO, bool JOIN>
+// f16 45.2.)  ADD: a unit's sums are added to the accumulators by f32 additions, which
+// round, where the products themselves cut: for f32 outputs, which 20 units a warp
+// would leave 8e-7 of themselves too small (3 sequences of 29,000 rows; 1.3e-7 with
+// it), 256 units and V of one sign 9e-5.  16-bit outputs round off more than that, and
+// would pay: batch 61.1 us without, 67.5 with it, 64 K rows 32.0 and 33.8.  JOIN: the
+// calls that join_cluster finishes.
+template <int D, bool I8, bool LO, bool ADD, bool JOIN>
 __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
     k10_decode8(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a,
                 const Cache8 c8, const DecodeSplit sp, const Layout8<D> ly) {
@@ -741,11 +746,13 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                     ph[b][t] = turned(split2<false>(x, y));
                     pl[b][t] = turned(split2<false>(x, y));
                 }
+            // (four tiles of columns at a time: a tile's products wait for one another)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                // (four tiles of columns at a time: a tile's second product waits for its first)
+            for (int x = 0; x < D / 32; x += 2) {
+                float t[4][4];
+                float(*to)[4] = ADD ? t : &o[2 * x];
 #pragma unroll
-                for (int x = 0; x < D / 32; x += 2) {
+                for (int b = 0; b < 2; ++b) {
                     uint32_t a0[8], a1[8];  // [tile * 2 + column]
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
@@ -755,11 +762,19 @@ __global__ void __launch_bounds__(kThreads8 + 32 * kFetchers, 1)
                         pairs8<I8>(prmt(v[b][1][0][x + y], v[b][1][1][x + y], 0x7362), a1[4 * y + 2], a1[4 * y + 3]);
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], ph[b][0], ph[b][1]);
+                    for (int j = 0; j < 4; ++j) {
+                        if (ADD && b == 0) mma8_first(to[j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], pl[b][0], pl[b][1]);
+                        else mma8(to[j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], pl[b][0], pl[b][1]);
+                    }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        mma8(o[2 * x + j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], pl[b][0], pl[b][1]);
+                        mma8(to[j], a0[2 * j], a0[2 * j + 1], a1[2 * j], a1[2 * j + 1], ph[b][0], ph[b][1]);
+                }
+                if constexpr (ADD) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[2 * x + j][e] += t[j][e];
                 }
             }
             __syncwarp();
@@ -888,7 +903,7 @@ size_t split8_of(int32_t n_seq, int32_t max_kv_len, int32_t n_head, int32_t n_he
     return at;
 }
 
-template <int D, bool I8, bool LO, bool JOIN>
+template <int D, bool I8, bool LO, bool ADD, bool JOIN>
 cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, cudaStream_t s) {
     CUtensorMap mk, mv;
     if (!cache8_map(&mk, c.k, D, a.n_head_kv, a.kv.rows) || !cache8_map(&mv, c.v, D, a.n_head_kv, a.kv.rows))
@@ -901,7 +916,7 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
     static std::atomic<unsigned> set_mask{0};
     if (dev >= 32 || !(set_mask.load(std::memory_order_acquire) & (1u << dev))) {
         const cudaError_t e =
-            cudaFuncSetAttribute(k10_decode8<D, I8, LO, JOIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            cudaFuncSetAttribute(k10_decode8<D, I8, LO, ADD, JOIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         if (dev < 32) set_mask.fetch_or(1u << dev, std::memory_order_release);
     }
@@ -928,7 +943,7 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
     cfg.blockDim = dim3(kThreads8 + 32 * kFetchers);
     cfg.dynamicSmemBytes = ly.bytes() + 1024;
     cfg.numAttrs = sp.cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k10_decode8<D, I8, LO, JOIN>, mk, mv, a, c, sp, ly);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k10_decode8<D, I8, LO, ADD, JOIN>, mk, mv, a, c, sp, ly);
     if (e != cudaSuccess || sp.direct) return e;
     const int heads = std::min(a.n_head / a.n_head_kv, sp.pass_heads);
     const int64_t grid = (int64_t)sp.joins * heads;
@@ -942,8 +957,13 @@ cudaError_t launch8_join(DecodeArgs a, const Cache8& c, const DecodeSplit& sp, c
 template <int D, bool I8>
 cudaError_t launch8_t(const DecodeArgs& a, const Cache8& c, const DecodeSplit& sp, cudaStream_t s) {
     const bool join = sp.cluster > 1;
-    if (a.dtype == 0) return join ? launch8_join<D, I8, true, true>(a, c, sp, s) : launch8_join<D, I8, true, false>(a, c, sp, s);
-    return join ? launch8_join<D, I8, false, true>(a, c, sp, s) : launch8_join<D, I8, false, false>(a, c, sp, s);
+    if (a.dtype == 0)
+        return join ? launch8_join<D, I8, true, true, true>(a, c, sp, s) : launch8_join<D, I8, true, true, false>(a, c, sp, s);
+    if (a.out_dtype == 0)
+        return join ? launch8_join<D, I8, false, true, true>(a, c, sp, s)
+                    : launch8_join<D, I8, false, true, false>(a, c, sp, s);
+    return join ? launch8_join<D, I8, false, false, true>(a, c, sp, s)
+                : launch8_join<D, I8, false, false, false>(a, c, sp, s);
 }
 
 }  // namespace

@@ -603,7 +603,8 @@ int32_t ep_sp_unpack_kv(ep_sp_ctx* ctx, int32_t layer, const ep_sp_kv_batch* src
  * then share the page of that row).  The products are exact but for what is taken
  * off q (an f32 q is held to 22 bits of its head's largest element, a bf16 q's
  * elements below 2^-31 of it to 2^-39), their sums, the scores and the softmax
- * statistics f32.  A weight times its page's V scale is held to 22 bits and to
+ * statistics f32 (sums for 16-bit outputs are cut, not rounded, at every 32 rows:
+ * up to 1e-4 of themselves for 65,536 rows of one sign in one SM).  A weight times its page's V scale is held to 22 bits and to
  * 2^-39 of the head's largest, whatever the scales (below 2^-112 to fewer), the
  * sum of the weights is taken before the scales.  A query head with an infinity
  * or a NaN has a row of NaN, a NaN code of e4m3 makes NaN of what it reaches.  A sequence's result
